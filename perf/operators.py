@@ -375,8 +375,7 @@ def run(s):
         case = s["case"]
         if kind == "verify":
             return ops.verify_drafts(s["logits"], s["ids"], s["cu"], s["uniforms"],
-                                     max_seqlen=s["max_new"], temperature=s["temperature"],
-                                     draft_probs=s["probs"])
+                                     temperature=s["temperature"], draft_probs=s["probs"])
         if kind == "cache":
             q = ops.kv_append_fp8(s["k"], s["v"], s["codes"], s["scales"], s["table"], s["lens"],
                                   s["cu"], q=s["q"], cos=s["cos"], sin=s["sin"])
