@@ -34,6 +34,15 @@
  *   ndl_greedy_argmax   the greedy sampler's argmax for a batch of logit rows
  *                       (needle/model/sampler.py:27-28)
  *
+ * and, beside them, a pool in 8 bits and the verification of drafted tokens, which the
+ * reference does not have:
+ *
+ *   ndl_kv_append_fp8   rotary embedding, quantisation and append into a pool of e4m3 codes
+ *   ndl_kv_read_fp8     ranges of cached tokens read back in the model's format
+ *   ndl_fp8_attention   attention of one token or a chunk per sequence over that pool
+ *   ndl_verify_drafts   accepted drafts and the next token of every sequence, from the
+ *                       target's logits and given random numbers
+ *
  * Conventions (every entry point):
  *   - Plain pointers to device memory, element counts and strides in ELEMENTS.
  *   - KV pool layout (needle/model/runner.py:65-78, attention.py:9-10):
@@ -64,7 +73,7 @@ extern "C" {
 typedef struct ihipStream_t* ndl_stream_t;
 
 /* 9: the float32 decode, prefill split and few-row linear entry points. */
-#define NDL_ABI_VERSION 9
+#define NDL_ABI_VERSION 10
 
 enum ndl_status {
   NDL_OK = 0,
@@ -494,6 +503,98 @@ size_t ndl_greedy_argmax_workspace_bytes(int64_t rows, int vocab);
 int ndl_greedy_argmax(void* out, int out_is_int64, const void* logits, int64_t row_stride,
                       int64_t rows, int vocab, int dtype, void* workspace,
                       size_t workspace_bytes, ndl_stream_t stream);
+
+/*
+ * The 8-bit pool: codes [2][num_blocks][num_kv_heads][block_size][head_dim], one e4m3 (OCP,
+ * no infinities) byte each, and scales [2][num_blocks][num_kv_heads][block_size], one byte per
+ * row (a token's head_dim values of one head).  A row's values are code * 2^(byte - 127), byte
+ * from 1 to 254 (0 only with codes of 0, as a zero-filled pool has).  Built for head_dim 64 and
+ * 128, block_size a power of two from 16 to 1024 and bf16 / fp16 activations
+ * (NDL_ERR_UNSUPPORTED otherwise).
+ *
+ * ndl_kv_append_fp8: k and v [num_tokens][num_kv_heads][head_dim] (token strides multiples of 8)
+ * into the slots of ndl_kv_append (cu_seqlens NULL: one token per sequence).  With a the largest
+ * finite magnitude of a row, 2^(byte - 127) is the smallest power of two (at least 2^-126) that
+ * has a <= 448 times it, and the codes are the values divided by it, rounded to nearest even; NaN
+ * where a value is not finite.  With cos and sin (rows of cs_tok_stride) k is rotated first, as
+ * ndl_rope_kv_append does, and with q and q_out (both or neither, q needs cos) q is rotated into
+ * q_out [num_tokens][num_heads][head_dim].  16-byte aligned pointers but for the scales.
+ */
+int ndl_kv_append_fp8(void* codes, void* scales, int64_t num_blocks, int num_kv_heads,
+                      int block_size, int head_dim, int dtype, const void* k,
+                      int64_t k_tok_stride, const void* v, int64_t v_tok_stride, void* q_out,
+                      const void* q, int64_t q_tok_stride, int num_heads, const void* cos,
+                      const void* sin, int64_t cs_tok_stride, const int32_t* block_table,
+                      int64_t bt_row_stride, int max_blocks_per_seq, const int32_t* cu_seqlens,
+                      const int32_t* context_lens, int num_seqs, int64_t num_tokens,
+                      ndl_stream_t stream);
+
+/*
+ * Tokens first[i] .. of sequence i, cu_seqlens[i + 1] - cu_seqlens[i] of them, read back into
+ * k_out and v_out [num_tokens][num_kv_heads][head_dim] (contiguous, 16-byte aligned) in `dtype`:
+ * exactly the pool's values in bf16, rounded once in fp16 where that has no such number.  A
+ * position follows the append's slot rule (past the table: its last column); a negative one and
+ * an invalid block id read as zeros; rows outside cu_seqlens are left as they were.
+ */
+int ndl_kv_read_fp8(void* k_out, void* v_out, const void* codes, const void* scales,
+                    int64_t num_blocks, int num_kv_heads, int block_size, int head_dim, int dtype,
+                    const int32_t* block_table, int64_t bt_row_stride, int max_blocks_per_seq,
+                    const int32_t* first, const int32_t* cu_seqlens, int num_seqs,
+                    int64_t num_tokens, ndl_stream_t stream);
+
+/*
+ * Attention over the 8-bit pool.  Token j of sequence i (packed by cu_seqlens; NULL: one token
+ * per sequence, then num_tokens == num_seqs and max_seqlen == 1) attends the first
+ * min(context_lens[i] + j + 1, max_blocks_per_seq * block_size) tokens of its sequence, the
+ * chunk's own among them: append first.  out [num_tokens][num_heads][head_dim]; q rows of
+ * q_tok_stride (a multiple of 8); groups of 1 to 16 query heads per kv head.  fp32 scores, softmax
+ * and sums; probabilities rounded to the 16-bit format for the matrix cores.  Nothing to attend
+ * (a negative context, invalid block ids only): zeros.
+ *
+ * max_seqlen bounds the tokens of a sequence (those past it are not computed); max_keys bounds
+ * the keys of a sequence and only chooses how the work is split.  The workspace
+ * (ndl_fp8_attention_workspace_bytes of the same sizes, on the same device; 0: none) is 256-byte
+ * aligned and belongs to one call at a time.
+ */
+size_t ndl_fp8_attention_workspace_bytes(int num_seqs, int max_seqlen, int64_t max_keys,
+                                         int num_heads, int num_kv_heads, int head_dim,
+                                         int block_size);
+int ndl_fp8_attention(void* out, const void* q, int64_t q_tok_stride, const void* codes,
+                      const void* scales, int64_t num_blocks, const int32_t* block_table,
+                      int64_t bt_row_stride, int max_blocks_per_seq, const int32_t* cu_seqlens,
+                      const int32_t* context_lens, int num_seqs, int64_t num_tokens,
+                      int max_seqlen, int64_t max_keys, int num_heads, int num_kv_heads,
+                      int head_dim, int block_size, int dtype, float scale, void* workspace,
+                      size_t workspace_bytes, ndl_stream_t stream);
+
+/*
+ * Verification of drafted tokens.  Sequence i has rows cu_seqlens[i] .. cu_seqlens[i + 1] (at
+ * least one) of logits and of ids, the chunk the target was given: row r judges the draft
+ * ids[r + 1], a sequence's last row none.  With p = softmax(logits[r] / temperature[i]) and q the
+ * draft's distribution, row r - i of draft_probs (NULL: the point at the draft), a draft x is
+ * accepted while uniforms[r] * q(x) < p(x) holds for it and all before it.  The next token is
+ * drawn with u = uniforms[cu_seqlens[i + 1] - 1]: from max(p - q, 0) of the first rejected row (p
+ * where that is 0 everywhere), or from p of the last row; it is the first v whose weights up to v
+ * sum to more than u times their total.
+ *
+ * Where temperature[i] is 0 or less, or a row's maximum is not finite, p is the point at the row's
+ * argmax in torch's order (ndl_greedy_argmax).  Draft probabilities that are NaN or negative
+ * count as 0 in max(p - q, 0), drafts outside the vocabulary are rejected, and u is taken within
+ * [0, 1].
+ *
+ * tokens [num_rows], in ids' type: a sequence's accepted drafts, the next token, then -1;
+ * accepted [num_seqs].  logits in `dtype`, any row stride of at least vocab; draft_probs float32
+ * [num_rows - num_seqs] rows; uniforms and temperature float32 [num_rows], [num_seqs]
+ * (temperature NULL: 1).  num_rows and num_seqs at most 65535.  The workspace is 256-byte aligned
+ * and belongs to one call at a time.
+ */
+size_t ndl_verify_drafts_workspace_bytes(int64_t num_rows, int num_seqs, int vocab);
+int ndl_verify_drafts(void* tokens, int32_t* accepted, const void* logits, int64_t row_stride,
+                      int dtype, const void* ids, int ids_are_int64, const int32_t* cu_seqlens,
+                      const float* uniforms, const float* temperature, const float* draft_probs,
+                      int64_t draft_stride, int64_t num_draft_rows, int64_t num_rows,
+                      int num_seqs, int vocab, void* workspace, size_t workspace_bytes,
+                      ndl_stream_t stream);
 
 #ifdef __cplusplus
 }

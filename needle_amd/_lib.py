@@ -16,7 +16,7 @@ import torch  # noqa: F401  (loads torch's HIP runtime before ours)
 _PKG_DIR = Path(__file__).resolve().parent
 LIB_PATH = _PKG_DIR / "libneedle_amd.so"
 
-NDL_ABI_VERSION = 9
+NDL_ABI_VERSION = 10
 NDL_DECODE_STATIC_SCRATCH_BYTES = 16 << 20
 NDL_PREFILL_SPLIT_MIN_KEYS = 768
 NDL_DTYPE_BF16 = 0
@@ -47,6 +47,12 @@ EXPORTED_SYMBOLS = (
     "ndl_skinny_linear_silu",
     "ndl_greedy_argmax_workspace_bytes",
     "ndl_greedy_argmax",
+    "ndl_kv_append_fp8",
+    "ndl_kv_read_fp8",
+    "ndl_fp8_attention_workspace_bytes",
+    "ndl_fp8_attention",
+    "ndl_verify_drafts_workspace_bytes",
+    "ndl_verify_drafts",
 )
 
 _c_i32 = ctypes.c_int
@@ -176,6 +182,37 @@ _SIGNATURES = {
     "ndl_greedy_argmax": (_c_i32, [
         _c_p, _c_i32, _c_p, _c_i64,                     # out, out int64, logits, stride
         _c_i64, _c_i32, _c_i32,                         # rows, vocab, dtype
+        _c_p, _c_sz, _c_p,                              # workspace, bytes, stream
+    ]),
+    "ndl_kv_append_fp8": (_c_i32, [
+        _c_p, _c_p, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32,  # codes, scales, NB, Hkv, bs, D, dtype
+        _c_p, _c_i64, _c_p, _c_i64,                     # k, k stride, v, v stride
+        _c_p, _c_p, _c_i64, _c_i32,                     # q_out, q, q stride, H
+        _c_p, _c_p, _c_i64,                             # cos, sin, cos/sin stride
+        _c_p, _c_i64, _c_i32,                           # block_table, row stride, W
+        _c_p, _c_p, _c_i32, _c_i64, _c_p,               # cu, ctx, B, T, stream
+    ]),
+    "ndl_kv_read_fp8": (_c_i32, [
+        _c_p, _c_p, _c_p, _c_p,                         # k_out, v_out, codes, scales
+        _c_i64, _c_i32, _c_i32, _c_i32, _c_i32,         # NB, Hkv, bs, D, dtype
+        _c_p, _c_i64, _c_i32,                           # block_table, row stride, W
+        _c_p, _c_p, _c_i32, _c_i64, _c_p,               # first, cu, B, T, stream
+    ]),
+    "ndl_fp8_attention_workspace_bytes": (_c_sz, [_c_i32, _c_i32, _c_i64] + [_c_i32] * 4),
+    "ndl_fp8_attention": (_c_i32, [
+        _c_p, _c_p, _c_i64,                             # out, q, q stride
+        _c_p, _c_p, _c_i64,                             # codes, scales, NB
+        _c_p, _c_i64, _c_i32,                           # block_table, row stride, W
+        _c_p, _c_p, _c_i32, _c_i64, _c_i32, _c_i64,     # cu, ctx, B, T, max_seqlen, max_keys
+        _c_i32, _c_i32, _c_i32, _c_i32, _c_i32,         # H, Hkv, D, bs, dtype
+        _c_f32, _c_p, _c_sz, _c_p,                      # scale, workspace, bytes, stream
+    ]),
+    "ndl_verify_drafts_workspace_bytes": (_c_sz, [_c_i64, _c_i32, _c_i32]),  # T, B, V
+    "ndl_verify_drafts": (_c_i32, [
+        _c_p, _c_p, _c_p, _c_i64, _c_i32,               # tokens, accepted, logits, stride, dtype
+        _c_p, _c_i32, _c_p, _c_p, _c_p,                 # ids, ids int64, cu, uniforms, temperature
+        _c_p, _c_i64, _c_i64,                           # draft probs, stride, rows
+        _c_i64, _c_i32, _c_i32,                         # T, B, V
         _c_p, _c_sz, _c_p,                              # workspace, bytes, stream
     ]),
 }

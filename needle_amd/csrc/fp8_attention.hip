@@ -1,0 +1,837 @@
+// Attention of a chunk of new tokens per sequence over the 8-bit paged pool (kv_fp8.hip): one
+// token (a decode step), a few (drafts to verify) or many (a prompt continued after a cached
+// prefix), gfx950.
+//
+//   out[j][h] = sum_t softmax_t(scale * q[j][h] . k[t][h / g]) v[t][h / g],
+//   t < min(ctx + j + 1, W * block_size),  k[t] = code * 2^(byte - 127), v likewise.
+//
+// The reference has no 8-bit pool; the meaning of the arguments is its _decode / _prefill's
+// (needle/layers/attention.py:120-134, :291-310), with a cached prefix attended.
+//
+// Bound: the codes, each read once (2 (D + 1) bytes per token and kv head).
+//   * Rows.  The g query heads of a kv head times the chunk's tokens are the N columns of
+//     16x16x32 MFMA tiles whose M rows are tokens (S^T = K Q^T) or head_dim (O^T = V^T P^T):
+//     up to 64 columns (NT tiles of 16) are a row block, longer chunks have several.
+//   * Codes to registers.  A wave takes 32 tokens at a time.  Their codes go straight to its own
+//     LDS ring (1 KiB of contiguous bytes per load), two stages deep: a stage is refilled as soon
+//     as its operands are in registers, so two tiles are in flight while a third computes, and
+//     no barrier is needed before the waves' results are combined.
+//   * Exact values.  e4m3 codes convert exactly to bf16 and fp16 (v_cvt_scalef32_pk_*_fp8), so
+//     the products are the 16-bit kernels' (fp32 sums).  K's scale multiplies the scores, where
+//     one factor is due anyway; V's is applied by the conversion, which is exact too.
+//   * P^T needs no data movement: with token slot 8 j + i of the PV product standing for token
+//     4 j + i (i < 4) or 12 + 4 j + i, the accumulator layout of S^T is the operand's.
+//   * Softmax in fp32 with exp2, scale * log2(e) folded.  The running maximum is raised (and the
+//     sums rescaled) only when a tile exceeds it by 8, so probabilities stay below 256.
+//     P is rounded to the 16-bit format for the matrix cores; its sum is taken before that.
+//   * Split.  Either a workgroup per (kv head, row block), or, where those would leave the GPU
+//     idle or unevenly loaded, all row blocks' tiles of a kv head laid end to end and cut into
+//     equal shares, one per resident workgroup; what a share holds of a row block goes to a
+//     workspace and is merged by a second launch.
+#include "ndl_common.hpp"
+
+namespace ndl {
+namespace {
+
+constexpr int kTile = 32;       // tokens per wave step
+constexpr int kWaves = 4;       // waves per workgroup; they take a row block's tiles in turn
+constexpr int kPad = 1;         // empty slots before each row block (its start's cost)
+constexpr float kRaise = 8.f;   // log2 of the largest probability before the maximum is raised
+
+struct ChunkArgs {
+  u16* out;
+  const u16* q;
+  int64_t q_stride;
+  const uint8_t* codes;
+  const uint8_t* scales;
+  int64_t plane_rows;           // rows (token, head) of a plane
+  int64_t num_blocks;
+  int num_heads, num_kv_heads, group;
+  const int32_t* block_table;
+  int64_t bt_row_stride;
+  int max_blocks;
+  int tile_shift;               // log2(block_size / 16)
+  const int32_t* cu_seqlens;    // null: one token per sequence
+  const int32_t* context_lens;
+  int num_seqs;
+  int64_t num_tokens;
+  int toks;                     // query tokens of a row block
+  int blocks_per_seq;           // row blocks a sequence can have
+  int64_t items;                // num_seqs * blocks_per_seq
+  float scale_log2;
+  // the split into equal shares (shares 0: a workgroup per row block)
+  int shares;                   // per kv head
+  int min_chunk;                // slots a share has at least
+  int64_t nseg;                 // segment slots per kv head: shares + items
+  float* ws_ml;                 // [kv head][segment][column][2]
+  float* ws_acc;                // [kv head][segment][column][D]
+};
+
+// A row block: tokens tok0 .. tok0 + n of the packed rows, the first at position pos.
+struct Item {
+  int64_t tok0;
+  int n;
+  int seq;
+  int64_t pos;
+  int64_t cap;                  // keys a table row holds
+  __device__ __forceinline__ int64_t keys() const {     // of its last token
+    const int64_t k = pos + n;
+    return n <= 0 || k <= 0 ? 0 : k < cap ? k : cap;
+  }
+  __device__ __forceinline__ int tiles() const { return (int)((keys() + kTile - 1) / kTile); }
+};
+
+__device__ __forceinline__ Item item_of(const ChunkArgs& a, int64_t e) {
+  Item it;
+  it.seq = (int)(e / a.blocks_per_seq);
+  const int j0 = (int)(e - (int64_t)it.seq * a.blocks_per_seq) * a.toks;
+  int64_t first = it.seq, count = 1;
+  if (a.cu_seqlens != nullptr) {
+    first = a.cu_seqlens[it.seq];
+    count = a.cu_seqlens[it.seq + 1] - first;
+    if (first < 0 || first + count > a.num_tokens) count = 0;
+  }
+  it.tok0 = first + j0;
+  it.n = (int)(count - j0 < a.toks ? count - j0 : a.toks);
+  it.pos = (int64_t)a.context_lens[it.seq] + j0;
+  it.cap = (int64_t)a.max_blocks << (4 + a.tile_shift);
+  return it;
+}
+
+__device__ __forceinline__ int slots_of(const ChunkArgs& a, int64_t e) {
+  if (e >= a.items) return 0;
+  const int n = item_of(a, e).tiles();
+  return n > 0 ? n + kPad : 0;
+}
+
+__device__ __forceinline__ int wave_scan(int v, int lane) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int o = __shfl_up(v, d, 64);
+    if (lane >= d) v += o;
+  }
+  return v;
+}
+
+// The slots of all row blocks before e (of a kv head's stream) and of all of them.
+struct StreamPos {
+  int64_t first, total;
+};
+__device__ __forceinline__ StreamPos stream_pos(const ChunkArgs& a, int lane, int64_t e) {
+  StreamPos r{0, 0};
+  for (int64_t base = 0; base < a.items; base += 64) {
+    const int v = slots_of(a, base + lane);
+    const int incl = wave_scan(v, lane);
+    if (e >= base && e < base + 64)
+      r.first = r.total + __builtin_amdgcn_readlane(incl - v, (int)(e - base));
+    r.total += __builtin_amdgcn_readlane(incl, 63);
+  }
+  return r;
+}
+__device__ __forceinline__ int64_t chunk_of(const ChunkArgs& a, int64_t total) {
+  const int64_t c = (total + a.shares - 1) / a.shares;
+  return c < a.min_chunk ? a.min_chunk : c;
+}
+// The row block that holds slot `at`, its first slot in *first; a.items if there is none.
+__device__ __forceinline__ int64_t stream_find(const ChunkArgs& a, int lane, int64_t at,
+                                               int64_t* first) {
+  int64_t carry = 0;
+  for (int64_t base = 0; base < a.items; base += 64) {
+    const int v = slots_of(a, base + lane);
+    const int incl = wave_scan(v, lane);
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(v > 0 && carry + incl > at);
+    if (hit) {
+      const int l = __builtin_ctzll(hit);
+      *first = carry + __builtin_amdgcn_readlane(incl - v, l);
+      return base + l;
+    }
+    carry += __builtin_amdgcn_readlane(incl, 63);
+  }
+  *first = carry;
+  return a.items;
+}
+
+// Waits until at most n (0 .. MAX) groups of I loads are in flight.
+template <int I, int MAX>
+__device__ __forceinline__ void vm_wait_groups(int n) {
+  if constexpr (MAX == 0) {
+    vm_wait<0>();
+  } else {
+    if (n >= MAX)
+      vm_wait<MAX * I>();
+    else
+      vm_wait_groups<I, MAX - 1>(n);
+  }
+}
+
+// Two codes of w's low or high half times scale, in the 16-bit format.
+template <bool F16, bool HI>
+__device__ __forceinline__ uint32_t value2(uint32_t w, float scale) {
+  if constexpr (F16)
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, HI));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, HI));
+}
+
+// 0xff in every byte of w that is a NaN code (0x7f or 0xff).
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
+  const uint32_t top = ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+  return (top >> 7) * 0xffu;
+}
+
+template <int D, bool F16, int NT>
+struct Shape {
+  static constexpr int kRowTile = kTile * D;                 // bytes of a tile's K (or V)
+  static constexpr int kStage = 2 * kRowTile + 256;          // K, V, scales
+  static constexpr int kDepth = NT == 4 ? 3 : 2;
+  static constexpr int kRing = kDepth * kStage;
+  static constexpr int kLoads = 2 * (kRowTile / 1024) + 1;   // per stage
+  static constexpr int kNg = NT == 1 ? 1 : 2;                // column tiles combined at a time
+  static constexpr int kSums = kWaves * kNg * 16 * D * 4;    // bytes of the waves' partial outputs
+  static constexpr int kMl = 2 * kWaves * NT * 16 * 4;
+  static constexpr int kLds = (kWaves * kRing > kSums ? kWaves * kRing : kSums) + kMl;
+};
+
+// A workgroup's share of the row blocks of one kv head.
+template <int D, bool F16, int NT>
+__global__ __launch_bounds__(64 * kWaves, NT == 4 ? 1 : 2) void chunk_attention_kernel(
+    ChunkArgs a) {
+  using T = Elt<F16>;
+  using X8 = typename T::x8;
+  using S = Shape<D, F16, NT>;
+  constexpr int KS = D / 32;      // k steps of the QK product
+  constexpr int DB = D / 16;      // 16-row tiles of O^T; head_dim index DB * m + b in tile b
+  constexpr int VW = DB / 4;      // words of codes a lane holds of one V row
+  __shared__ __attribute__((aligned(16))) unsigned char smem[S::kLds];
+  float* const ml = reinterpret_cast<float*>(smem + S::kLds - S::kMl);   // [2][wave][column]
+
+  const int lane = threadIdx.x & 63, j = lane >> 4, c = lane & 15;
+  const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  unsigned char* const ring = smem + wv * S::kRing;
+  const uint32_t ring_lds = lds_addr(ring);
+
+  // The kv heads of one share (or row block) run on one XCD at about the same time: workgroups
+  // are dealt to the XCDs in turn, and heads share the lines of scales, tables and lengths.
+  const int Hkv = a.num_kv_heads;
+  const unsigned per8 = 8u * Hkv, grp = blockIdx.x / per8, in8 = blockIdx.x - grp * per8;
+  const int head = (int)(in8 >> 3);
+  const int64_t unit = (int64_t)grp * 8 + (in8 & 7);
+
+  int64_t e, first = 0, from = 0, to = 0;   // the row block, its first slot; the share's slots
+  const bool whole = a.shares == 0;
+  if (whole) {
+    e = unit;
+    if (e >= a.items) return;
+  } else {
+    if (unit >= a.shares) return;
+    const StreamPos p = stream_pos(a, lane, -1);
+    const int64_t chunk = chunk_of(a, p.total);
+    from = unit * chunk;
+    to = from + chunk < p.total ? from + chunk : p.total;
+    if (from >= to) return;
+    e = stream_find(a, lane, from, &first);
+  }
+
+  const uint32_t swz = (uint32_t)((lane >> 3) * 128 + (((lane & 7) ^ (lane >> 3)) << 4));
+  const int bshift = 4 + a.tile_shift;
+  const uint32_t tmask = (1u << a.tile_shift) - 1;
+
+  for (; e < a.items; ++e) {
+    const Item it = item_of(a, e);
+    const int ntiles = it.tiles();
+    int t0 = 0, t1 = ntiles;
+    if (!whole) {
+      if (ntiles == 0) continue;
+      if (first >= to) break;
+      const int64_t base = first + kPad;
+      t0 = from > base ? (int)(from - base) : 0;
+      t1 = to < base + ntiles ? (int)(to - base) : ntiles;
+      first = base + ntiles;
+      if (t0 >= t1) continue;     // only the empty slot is this share's
+    } else if (it.n <= 0) {
+      return;
+    }
+    const int cols = it.n * a.group;
+
+    // Columns: 16 nt + c is query token col / g, head head * g + col % g.
+    X8 q[NT][KS];
+    int lim[NT];                  // keys the column attends
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      int col = 16 * nt + c;
+      if (col >= cols) col = cols - 1;      // computed like the last column, not stored
+      const int tok = col / a.group;
+      const u16* src = a.q + (it.tok0 + tok) * a.q_stride +
+                       (int64_t)(head * a.group + col - tok * a.group) * D;
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+        q[nt][s] = __builtin_bit_cast(X8, ld16(src + 64 * (s >> 1) + 16 * j + 8 * (s & 1)));
+      const int64_t k = it.pos + tok + 1;
+      lim[nt] = (int)(k < it.cap ? k : it.cap);
+    }
+    const int64_t k_first = it.pos + 1 < it.cap ? it.pos + 1 : it.cap;
+    const int all_keys = (int)it.keys();      // of the last token
+    const int min_keys = k_first < 0 ? 0 : (int)k_first;   // of the first
+
+    f32x4 acc[NT][DB];
+    float m[NT], l[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      m[nt] = kNegInf;
+      l[nt] = 0.f;
+#pragma unroll
+      for (int b = 0; b < DB; ++b) acc[nt][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    // This wave's tiles: t0 + wv, t0 + wv + kWaves, ..  Lane 2 u + s of a window holds 16-token
+    // half s of the window's tile u: its first row in a plane of kv head 0's slices, or -1.
+    const int cnt = t1 - t0 > wv ? (t1 - t0 - wv + kWaves - 1) / kWaves : 0;
+    const int32_t* const table = a.block_table + (int64_t)it.seq * a.bt_row_stride;
+    int window[1];                // block ids
+    auto load_window = [&](int u0) {
+      const int tt = 2 * (t0 + wv + kWaves * (u0 + (lane >> 1))) + (lane & 1);
+      int col = tt >> a.tile_shift;
+      if (col > a.max_blocks - 1) col = a.max_blocks - 1;
+      window[0] = table[col];
+    };
+    uint32_t bad_bits = 0;        // two bits per stage: its halves with an invalid block id
+    auto issue = [&](int u, int slot) {
+      if ((u & 31) == 0) load_window(u);
+      const uint32_t st = ring_lds + slot * S::kStage;
+      const int tile = t0 + wv + kWaves * u;
+      uint32_t srow[2];
+      uint32_t bad = 0;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        int b = __builtin_amdgcn_readlane(window[0], 2 * (u & 31) + s);
+        if (b < 0 || b >= a.num_blocks) {
+          b = 0;
+          bad |= 1u << s;
+        }
+        const int64_t row = (((int64_t)b * Hkv + head) << bshift) +
+                            (((uint32_t)(2 * tile + s) & tmask) << 4);
+        srow[s] = (uint32_t)row;
+        const uint8_t* kb = a.codes + row * D;
+        const uint8_t* vb = kb + a.plane_rows * D;
+#pragma unroll
+        for (int x = 0; x < D / 64; ++x) {
+          lds_dma16_nt(kb + 1024 * x, swz, st + s * 16 * D + 1024 * x);
+          lds_dma16_nt(vb + 1024 * x, (uint32_t)lane * 16, st + S::kRowTile + s * 16 * D + 1024 * x);
+        }
+      }
+      // scales: 4-byte word w of half s of plane p lands at word 8 p + 4 s + w
+      const uint32_t off = (lane & 8 ? (uint32_t)a.plane_rows : 0u) +
+                           (lane & 4 ? srow[1] : srow[0]) + 4u * (lane & 3);
+      lds_dma4(a.scales, off, st + 2 * S::kRowTile);
+      bad_bits = (bad_bits & ~(3u << (2 * slot))) | (bad << (2 * slot));
+    };
+#pragma unroll
+    for (int d = 0; d < S::kDepth; ++d)
+      if (d < cnt) issue(d, d);
+
+    int slot = 0;
+    for (int u = 0; u < cnt; ++u) {
+      vm_wait_groups<S::kLoads, S::kDepth - 1>(cnt - 1 - u);
+      asm volatile("" ::: "memory");
+      const unsigned char* st = ring + slot * S::kStage;
+      // operands: K half s, 16 codes at head_dim 64 h + 16 j of row c; V rows of slots 8 j + i
+      u32x4 kc[2][D / 64];
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int h = 0; h < D / 64; ++h) {
+          const int o = D == 128 ? c * 128 + (((4 * h + j) ^ (c & 7)) << 4)
+                                 : (c >> 1) * 128 + ((((c & 1) * 4 + j) ^ (c >> 1)) << 4);
+          kc[s][h] = *reinterpret_cast<const u32x4*>(st + s * 16 * D + o);
+        }
+      uint32_t vc[8][VW];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int row = (i >> 2) * 16 + 4 * j + (i & 3);
+        const unsigned char* p = st + S::kRowTile + row * D + DB * c;
+        if constexpr (VW == 2) {
+          const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+          vc[i][0] = x[0];
+          vc[i][1] = x[1];
+        } else {
+          vc[i][0] = *reinterpret_cast<const uint32_t*>(p);
+        }
+      }
+      uint32_t sk[2], sv[2];
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        sk[s] = *reinterpret_cast<const uint32_t*>(st + 2 * S::kRowTile + 16 * s + 4 * j);
+        sv[s] = *reinterpret_cast<const uint32_t*>(st + 2 * S::kRowTile + 32 + 16 * s + 4 * j);
+      }
+      const uint32_t bad = (bad_bits >> (2 * slot)) & 3u;
+      // in registers before the stage's next loads go out
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (u + S::kDepth < cnt) issue(u + S::kDepth, slot);
+      slot = slot + 1 == S::kDepth ? 0 : slot + 1;
+
+      // S^T: lane (j, c) holds tokens 16 s + 4 j + r of column c
+      f32x4 sc[2][NT];
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) sc[s][nt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int h = 0; h < D / 64; ++h)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const u32x4 kw{value2<F16, false>(kc[s][h][2 * x], 1.f),
+                           value2<F16, true>(kc[s][h][2 * x], 1.f),
+                           value2<F16, false>(kc[s][h][2 * x + 1], 1.f),
+                           value2<F16, true>(kc[s][h][2 * x + 1], 1.f)};
+            const X8 k8 = __builtin_bit_cast(X8, kw);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              sc[s][nt] = T::mfma16x16x32(k8, q[nt][2 * h + x], sc[s][nt]);
+          }
+      }
+      float vs[8];
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float ks = __uint_as_float(((sk[s] >> (8 * r)) & 0xffu) << 23) * a.scale_log2;
+          vs[4 * s + r] = __uint_as_float(((sv[s] >> (8 * r)) & 0xffu) << 23);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) sc[s][nt][r] *= ks;
+        }
+
+      const int tile = t0 + wv + kWaves * u;
+      const bool masked = bad != 0 || kTile * (tile + 1) > min_keys;
+      uint32_t nan_any = 0;
+      if (masked) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const int at = kTile * tile + 16 * s + 4 * j;     // the lane's first token
+          const bool off = (bad >> s) & 1;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const int left = off ? 0 : lim[nt] - at;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sc[s][nt][r] = r < left ? sc[s][nt][r] : kNegInf;
+          }
+          // what no column attends may hold anything, a NaN included: 0 * NaN must not happen
+          const int left = off ? 0 : all_keys - at;
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int w = 0; w < VW; ++w) {
+              vc[4 * s + r][w] = r < left ? vc[4 * s + r][w] : 0u;
+              nan_any |= nan_bytes(vc[4 * s + r][w]);
+            }
+        }
+      }
+
+      X8 p[NT];
+      bool raise = false;
+      float mt[NT];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float x = fmaxf(fmaxf(sc[0][nt][0], sc[0][nt][1]), fmaxf(sc[0][nt][2], sc[0][nt][3]));
+        x = fmaxf(x, fmaxf(fmaxf(sc[1][nt][0], sc[1][nt][1]), fmaxf(sc[1][nt][2], sc[1][nt][3])));
+        mt[nt] = max_xor32(max_xor16(x));
+        raise |= mt[nt] > m[nt] + kRaise;
+      }
+      if (__builtin_amdgcn_ballot_w64(raise)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const float nm = fmaxf(m[nt], mt[nt]);
+          const float f = m[nt] == nm ? 1.f : fast_exp2(m[nt] - nm);
+          m[nt] = nm;
+          l[nt] *= f;
+#pragma unroll
+          for (int b = 0; b < DB; ++b) acc[nt][b] *= f;
+        }
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float base = m[nt] == kNegInf ? 0.f : m[nt];    // nothing attended yet
+        float e8[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e8[i] = fast_exp2(sc[i >> 2][nt][i & 3] - base);
+        l[nt] += ((e8[0] + e8[1]) + (e8[2] + e8[3])) + ((e8[4] + e8[5]) + (e8[6] + e8[7]));
+        const u32x4 w{T::pack(e8[0], e8[1]), T::pack(e8[2], e8[3]), T::pack(e8[4], e8[5]),
+                      T::pack(e8[6], e8[7])};
+        p[nt] = __builtin_bit_cast(X8, w);
+      }
+
+      // A NaN in a value that some of the chunk's tokens attend and others do not: it is taken
+      // out of the product and put into the columns that attend it.
+      if (masked && a.toks > 1 && __builtin_amdgcn_ballot_w64(nan_any != 0)) {
+        constexpr uint32_t one = F16 ? 0x3c00u : 0x3f80u;
+        X8 seen[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          u32x4 w;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int s = i >> 1, at = kTile * tile + 16 * s + 4 * j + 2 * (i & 1);
+            const int left = (bad >> s) & 1 ? 0 : lim[nt] - at;
+            w[i] = (left > 0 ? one : 0u) | (left > 1 ? one << 16 : 0u);
+          }
+          seen[nt] = __builtin_bit_cast(X8, w);
+        }
+#pragma unroll
+        for (int b = 0; b < DB; ++b) {
+          u32x4 w;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t x = (nan_bytes(vc[2 * i][b >> 2]) >> (8 * (b & 3))) & 0xffu;
+            const uint32_t y = (nan_bytes(vc[2 * i + 1][b >> 2]) >> (8 * (b & 3))) & 0xffu;
+            w[i] = (x ? one : 0u) | (y ? one << 16 : 0u);
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const f32x4 hits = T::mfma16x16x32(__builtin_bit_cast(X8, w), seen[nt],
+                                               f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (hits[r] > 0.f) acc[nt][b][r] = __uint_as_float(0x7fc00000u);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int w = 0; w < VW; ++w) vc[i][w] &= ~nan_bytes(vc[i][w]);
+      }
+
+      // O^T += V^T P^T: a pair of head_dim tiles at a time, the rows' pairs of codes turned into
+      // pairs of tokens
+#pragma unroll
+      for (int b2 = 0; b2 < DB / 2; ++b2) {
+        uint32_t v2[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          v2[i] = b2 & 1 ? value2<F16, true>(vc[i][b2 >> 1], vs[i])
+                         : value2<F16, false>(vc[i][b2 >> 1], vs[i]);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          u32x4 w;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[i] = pack_halves(v2[2 * i], v2[2 * i + 1], x == 1);
+          const X8 v8 = __builtin_bit_cast(X8, w);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            acc[nt][2 * b2 + x] = T::mfma16x16x32(v8, p[nt], acc[nt][2 * b2 + x]);
+        }
+      }
+    }
+
+    // The waves' results: (m, l) first, then the outputs scaled to the common maximum, laid out
+    // so that wave r of the reduction holds head_dim DB (4 j + r) .. of column c.
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      l[nt] = add_xor32(add_xor16(l[nt]));
+      if (j == 0) {
+        ml[wv * 16 * NT + 16 * nt + c] = m[nt];
+        ml[(kWaves + wv) * 16 * NT + 16 * nt + c] = l[nt];
+      }
+    }
+    __syncthreads();
+    const bool part = !whole && (t0 > 0 || t1 < ntiles);
+    const int64_t seg = ((int64_t)head * a.nseg + unit + e) * (a.toks * a.group);
+#pragma unroll
+    for (int g0 = 0; g0 < NT; g0 += S::kNg) {
+      float* const sums = reinterpret_cast<float*>(smem);   // [wave][nt][r][lane][DB]
+      float mm[S::kNg], ll[S::kNg];
+#pragma unroll
+      for (int y = 0; y < S::kNg; ++y) {
+        const int nt = g0 + y, col = 16 * nt + c;
+        mm[y] = ml[col];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) mm[y] = fmaxf(mm[y], ml[w * 16 * NT + col]);
+        ll[y] = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+          const float mw = ml[w * 16 * NT + col];
+          ll[y] += ml[(kWaves + w) * 16 * NT + col] * (mw == mm[y] ? 1.f : fast_exp2(mw - mm[y]));
+        }
+        const float f = m[nt] == mm[y] ? 1.f : fast_exp2(m[nt] - mm[y]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int b4 = 0; b4 < DB; b4 += 4)
+            *reinterpret_cast<f32x4*>(sums + (((wv * S::kNg + y) * 4 + r) * 64 + lane) * DB + b4) =
+                f32x4{acc[nt][b4][r] * f, acc[nt][b4 + 1][r] * f, acc[nt][b4 + 2][r] * f,
+                      acc[nt][b4 + 3][r] * f};
+      }
+      __syncthreads();
+#pragma unroll
+      for (int y = 0; y < S::kNg; ++y) {
+        const int col = 16 * (g0 + y) + c;
+        float o[DB];
+#pragma unroll
+        for (int b = 0; b < DB; ++b) o[b] = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w)
+#pragma unroll
+          for (int b = 0; b < DB; ++b)
+            o[b] += sums[(((w * S::kNg + y) * 4 + wv) * 64 + lane) * DB + b];
+        if (col < cols) {
+          const int d0 = DB * (4 * j + wv);
+          if (part) {
+            float* const dst = a.ws_acc + (seg + col) * D + d0;
+#pragma unroll
+            for (int b = 0; b < DB; b += 4)
+              *reinterpret_cast<f32x4*>(dst + b) = f32x4{o[b], o[b + 1], o[b + 2], o[b + 3]};
+            if (j == 0 && wv == 0)
+              *reinterpret_cast<f32x2*>(a.ws_ml + (seg + col) * 2) = f32x2{mm[y], ll[y]};
+          } else {
+            const float inv = ll[y] == 0.f ? 0.f : 1.f / ll[y];   // nothing attended: zeros
+            const int tok = col / a.group;
+            u16* const dst = a.out + ((it.tok0 + tok) * a.num_heads + head * a.group + col -
+                                      tok * a.group) * (int64_t)D + d0;
+            uint32_t w[DB / 2];
+#pragma unroll
+            for (int b = 0; b < DB / 2; ++b) w[b] = T::pack(o[2 * b] * inv, o[2 * b + 1] * inv);
+            if constexpr (DB == 8)
+              st16(dst, u32x4{w[0], w[1], w[2], w[3]});
+            else
+              *reinterpret_cast<u32x2*>(dst) = u32x2{w[0], w[1]};
+          }
+        }
+      }
+      __syncthreads();     // before the sums or the ring are written again
+    }
+    if (whole) return;
+  }
+}
+
+// One wave per (token, query head): the parts of its row block that the shares hold, combined in
+// their order; zeros for a token with nothing to attend.  A row block inside one share was
+// written by the attention.
+template <int D, bool F16>
+__global__ __launch_bounds__(256) void chunk_merge_kernel(ChunkArgs a) {
+  using T = Elt<F16>;
+  constexpr int PER = D / 64;
+  const int lane = threadIdx.x & 63;
+  const int64_t w =
+      (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int64_t tok = w / a.num_heads;
+  const int h = (int)(w - tok * a.num_heads);
+  if (tok >= a.num_tokens) return;
+  int64_t e = tok, off = 0;
+  if (a.cu_seqlens != nullptr) {
+    if (tok < a.cu_seqlens[0] || tok >= a.cu_seqlens[a.num_seqs]) return;
+    int lo = 0, hi = a.num_seqs - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (a.cu_seqlens[mid] <= tok) lo = mid; else hi = mid - 1;
+    }
+    const int64_t jt = tok - a.cu_seqlens[lo], rb = jt / a.toks;
+    if (rb >= a.blocks_per_seq) return;    // past max_seqlen
+    e = (int64_t)lo * a.blocks_per_seq + rb;
+    off = jt - rb * a.toks;
+  }
+  const int kvh = h / a.group;
+  const int64_t col = off * a.group + (h - kvh * a.group);
+  const Item it = item_of(a, e);
+  if (it.n <= 0) return;
+  u16* const dst = a.out + (tok * a.num_heads + h) * D + lane * PER;
+  auto store = [&](const float (&o)[PER]) {
+    if constexpr (PER == 2)
+      *reinterpret_cast<uint32_t*>(dst) = T::pack(o[0], o[1]);
+    else
+      *dst = T::one(o[0]);
+  };
+  float o[PER];
+#pragma unroll
+  for (int x = 0; x < PER; ++x) o[x] = 0.f;
+  const int nt = it.tiles();
+  if (nt == 0) {
+    store(o);
+    return;
+  }
+  const StreamPos p = stream_pos(a, lane, e);
+  const int64_t chunk = chunk_of(a, p.total), base = p.first + kPad;
+  const int64_t s0 = base / chunk, s1 = (base + nt - 1) / chunk;
+  if (s0 == s1) return;
+  const int per = a.toks * a.group;
+  const int64_t seg = ((int64_t)kvh * a.nseg + s0 + e) * per + col;
+  const int n = (int)(s1 - s0 + 1);
+  const float* const ml = a.ws_ml + seg * 2;
+  const float* const src = a.ws_acc + seg * D + lane * PER;
+  float mx = kNegInf;
+  for (int i = lane; i < n; i += 64) mx = fmaxf(mx, ml[(int64_t)i * per * 2]);
+#pragma unroll
+  for (int x = 32; x >= 1; x >>= 1) mx = fmaxf(mx, xor_shfl(mx, x));
+  float l = 0.f;
+  for (int i = 0; i < n; ++i) {
+    const f32x2 v = *reinterpret_cast<const f32x2*>(ml + (int64_t)i * per * 2);
+    const float f = v[0] == mx ? 1.f : fast_exp2(v[0] - mx);
+    l += v[1] * f;
+#pragma unroll
+    for (int x = 0; x < PER; ++x) o[x] += src[(int64_t)i * per * D + x] * f;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int x = 0; x < PER; ++x) o[x] *= inv;
+  store(o);
+}
+
+// Column tiles of a row block: the fewest that hold max_seqlen tokens of a group's heads.
+int col_tiles(int64_t max_seqlen, int group) {
+  const int64_t cols = max_seqlen * group;
+  return cols <= 16 ? 1 : cols <= 32 ? 2 : 4;
+}
+
+struct Plan {
+  int nt, toks;
+  int64_t blocks_per_seq, items;
+  int shares;                 // 0: whole row blocks
+  int64_t nseg;
+  size_t ml_bytes, acc_bytes;
+};
+
+template <int D, bool F16>
+const void* kernel_of(int nt) {
+  return nt == 1 ? (const void*)chunk_attention_kernel<D, F16, 1>
+         : nt == 2 ? (const void*)chunk_attention_kernel<D, F16, 2>
+                   : (const void*)chunk_attention_kernel<D, F16, 4>;
+}
+
+constexpr int kMinChunk = 2 * kWaves;
+
+// resident: workgroups the GPU holds at once.
+Plan make_plan(int64_t num_seqs, int64_t max_seqlen, int64_t max_keys, int group,
+               int num_kv_heads, int head_dim, int64_t resident) {
+  Plan p{};
+  p.nt = col_tiles(max_seqlen, group);
+  p.toks = 16 * p.nt / group;
+  p.blocks_per_seq = (max_seqlen + p.toks - 1) / p.toks;
+  p.items = num_seqs * p.blocks_per_seq;
+  const int64_t tiles = (max_keys + kTile - 1) / kTile;
+  const int64_t units = p.items * num_kv_heads;
+  const bool whole = tiles <= 2 * kMinChunk || units >= 4 * resident;
+  if (!whole) {
+    int64_t s = resident / num_kv_heads / 8 * 8;
+    if (s < 8) s = 8;
+    p.shares = (int)s;
+    p.nseg = s + p.items;
+    const size_t cols = (size_t)num_kv_heads * p.nseg * p.toks * group;
+    p.ml_bytes = (cols * 8 + 255) / 256 * 256;
+    p.acc_bytes = cols * head_dim * 4;
+  }
+  return p;
+}
+
+bool shape_ok(int head_dim, int block_size, int num_heads, int num_kv_heads) {
+  return (head_dim == 64 || head_dim == 128) && block_tile_shift(block_size) >= 0 &&
+         num_heads > 0 && num_kv_heads > 0 && num_heads % num_kv_heads == 0 &&
+         num_heads / num_kv_heads <= 16;
+}
+
+Plan plan_for(int64_t num_seqs, int64_t max_seqlen, int64_t max_keys, int num_heads,
+              int num_kv_heads, int head_dim) {
+  const int group = num_heads / num_kv_heads, nt = col_tiles(max_seqlen, group);
+  // the formats' kernels use the same resources
+  int64_t res = resident_workgroups(
+      head_dim == 128 ? kernel_of<128, false>(nt) : kernel_of<64, false>(nt), 64 * kWaves);
+  if (res <= 0) res = 256;
+  return make_plan(num_seqs, max_seqlen, max_keys, group, num_kv_heads, head_dim, res);
+}
+
+template <int D, bool F16>
+int launch(const ChunkArgs& a, int nt, hipStream_t s) {
+  const int64_t units = a.shares ? a.shares : (a.items + 7) / 8 * 8;
+  const int64_t wgs = units * a.num_kv_heads;
+  if (wgs > 0x7fffffff) return NDL_ERR_INVALID_ARG;
+  const dim3 grid((unsigned)wgs), wg(64 * kWaves);
+  if (nt == 1)
+    hipLaunchKernelGGL((chunk_attention_kernel<D, F16, 1>), grid, wg, 0, s, a);
+  else if (nt == 2)
+    hipLaunchKernelGGL((chunk_attention_kernel<D, F16, 2>), grid, wg, 0, s, a);
+  else
+    hipLaunchKernelGGL((chunk_attention_kernel<D, F16, 4>), grid, wg, 0, s, a);
+  const int rc = check_launch();
+  if (rc != NDL_OK || a.shares == 0) return rc;
+  const int64_t rows = a.num_tokens * a.num_heads, blocks = (rows + 3) / 4;
+  if (blocks > 0x7fffffff) return NDL_ERR_INVALID_ARG;
+  hipLaunchKernelGGL((chunk_merge_kernel<D, F16>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+  return check_launch();
+}
+
+}  // namespace
+}  // namespace ndl
+
+extern "C" size_t ndl_fp8_attention_workspace_bytes(int num_seqs, int max_seqlen, int64_t max_keys,
+                                                    int num_heads, int num_kv_heads, int head_dim,
+                                                    int block_size) {
+  using namespace ndl;
+  if (num_seqs <= 0 || max_seqlen <= 0 || max_keys <= 0 ||
+      !shape_ok(head_dim, block_size, num_heads, num_kv_heads))
+    return 0;
+  const Plan p = plan_for(num_seqs, max_seqlen, max_keys, num_heads, num_kv_heads, head_dim);
+  return p.ml_bytes + p.acc_bytes;
+}
+
+extern "C" int ndl_fp8_attention(void* out, const void* q, int64_t q_tok_stride,
+                                 const void* codes, const void* scales, int64_t num_blocks,
+                                 const int32_t* block_table, int64_t bt_row_stride,
+                                 int max_blocks_per_seq, const int32_t* cu_seqlens,
+                                 const int32_t* context_lens, int num_seqs, int64_t num_tokens,
+                                 int max_seqlen, int64_t max_keys, int num_heads,
+                                 int num_kv_heads, int head_dim, int block_size, int dtype,
+                                 float scale, void* workspace, size_t workspace_bytes,
+                                 ndl_stream_t stream) {
+  using namespace ndl;
+  if (!dtype_supported(dtype) || !shape_ok(head_dim, block_size, num_heads, num_kv_heads))
+    return NDL_ERR_UNSUPPORTED;
+  if (num_seqs < 0 || num_tokens < 0 || num_blocks <= 0 || max_blocks_per_seq <= 0 ||
+      bt_row_stride < max_blocks_per_seq || max_seqlen <= 0 || max_keys <= 0)
+    return NDL_ERR_INVALID_ARG;
+  if (num_seqs == 0 || num_tokens == 0) return NDL_OK;
+  if (!out || !q || !codes || !scales || !block_table || !context_lens)
+    return NDL_ERR_INVALID_ARG;
+  if (cu_seqlens == nullptr && (num_tokens != num_seqs || max_seqlen != 1))
+    return NDL_ERR_INVALID_ARG;
+  if (q_tok_stride < (int64_t)num_heads * head_dim || (q_tok_stride & 7)) return NDL_ERR_INVALID_ARG;
+  if (((uintptr_t)out | (uintptr_t)q | (uintptr_t)codes) & 15u || (uintptr_t)scales & 3u)
+    return NDL_ERR_INVALID_ARG;
+  ChunkArgs a{};
+  a.plane_rows = num_blocks * num_kv_heads * (int64_t)block_size;
+  // a scale's address is the pool's and a 32-bit offset; positions are 32-bit
+  if (a.plane_rows > 0x7fffffff || (int64_t)max_blocks_per_seq * block_size > 0x7fffff00)
+    return NDL_ERR_UNSUPPORTED;
+  const Plan p = plan_for(num_seqs, max_seqlen, max_keys, num_heads, num_kv_heads, head_dim);
+  if (p.blocks_per_seq > 0x7fffffff) return NDL_ERR_INVALID_ARG;
+  if (p.shares) {
+    if (!workspace || workspace_bytes < p.ml_bytes + p.acc_bytes || (uintptr_t)workspace & 255u)
+      return NDL_ERR_WORKSPACE;
+    a.ws_ml = (float*)workspace;
+    a.ws_acc = (float*)((char*)workspace + p.ml_bytes);
+  }
+  a.out = (u16*)out;
+  a.q = (const u16*)q;
+  a.q_stride = q_tok_stride;
+  a.codes = (const uint8_t*)codes;
+  a.scales = (const uint8_t*)scales;
+  a.num_blocks = num_blocks;
+  a.num_heads = num_heads;
+  a.num_kv_heads = num_kv_heads;
+  a.group = num_heads / num_kv_heads;
+  a.block_table = block_table;
+  a.bt_row_stride = bt_row_stride;
+  a.max_blocks = max_blocks_per_seq;
+  a.tile_shift = block_tile_shift(block_size);
+  a.cu_seqlens = cu_seqlens;
+  a.context_lens = context_lens;
+  a.num_seqs = num_seqs;
+  a.num_tokens = num_tokens;
+  a.toks = p.toks;
+  a.blocks_per_seq = (int)p.blocks_per_seq;
+  a.items = p.items;
+  a.scale_log2 = scale * kLog2e;
+  a.shares = p.shares;
+  a.min_chunk = kMinChunk;
+  a.nseg = p.nseg;
+  const hipStream_t s = (hipStream_t)stream;
+  const bool f16 = dtype_is_f16(dtype);
+  if (head_dim == 128)
+    return f16 ? launch<128, true>(a, p.nt, s) : launch<128, false>(a, p.nt, s);
+  return f16 ? launch<64, true>(a, p.nt, s) : launch<64, false>(a, p.nt, s);
+}

@@ -1,0 +1,359 @@
+// The 8-bit KV cache: rows of K and V quantised as they are written into the paged pool, and
+// read back into the model's format.
+//
+// A row is one token's head_dim values of one head.  With a = max |x_d| over its finite values,
+//   e = the smallest integer >= -126 with a <= 448 * 2^e,
+//   code_d = e4m3(x_d * 2^-e)  (round to nearest even; NaN where x_d is not finite),
+//   byte = e + 127,
+// and the row's values are code_d * 2^e.  The scale is a power of two because e4m3 is a floating
+// format: its step is relative (2^-4 of a value at most), so a finer scale gains nothing, the
+// largest value lands in (224, 448] and everything down to 2^-14 of it keeps full precision; one
+// byte per row then does, the multiplication is exact, and so is code * 2^e in bf16 (and in fp16
+// above its subnormals).
+//
+// The reference has no such pool; the slot rule is its append's (needle/layers/attention.py:
+// 141-154, :224-237) and the rotation its _apply_rope (:277-288), as in rope_append.hip.
+//
+// Pools: codes [2][NB][Hkv][bs][D] bytes, scales [2][NB][Hkv][bs] bytes.
+#include "ndl_common.hpp"
+
+namespace ndl {
+namespace {
+
+struct QuantArgs {
+  uint8_t* codes;
+  uint8_t* scales;
+  int64_t plane_rows;          // rows (token, head) of a plane
+  int64_t num_blocks;
+  int num_heads, num_kv_heads;
+  int block_shift;             // log2(block_size)
+  const u16* k;
+  const u16* v;
+  int64_t k_stride, v_stride;
+  const u16* q;                // rotated into q_out (null: no q)
+  u16* q_out;
+  int64_t q_stride;
+  const u16* cos;              // null: k (and q) as they are
+  const u16* sin;
+  int64_t cs_stride;
+  const int32_t* block_table;
+  int64_t bt_row_stride;
+  int max_blocks;
+  const int32_t* cu_seqlens;
+  const int32_t* context_lens; // of a read: the first position of each sequence
+  int num_seqs;
+  int64_t num_tokens;
+  u16* k_out;                  // of a read
+  u16* v_out;
+};
+
+// Row index in a plane of (token t, kv head 0), or -1: t past the last sequence, a negative
+// position, an invalid block id.  t is wave-uniform.
+__device__ __forceinline__ int64_t slot_row(const QuantArgs& a, int64_t t) {
+  int i;
+  int64_t p;
+  if (a.cu_seqlens == nullptr) {
+    i = (int)t;
+    p = a.context_lens[i];
+  } else {
+    if (t < (int64_t)a.cu_seqlens[0] || t >= (int64_t)a.cu_seqlens[a.num_seqs]) return -1;
+    int lo = 0, hi = a.num_seqs - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if ((int64_t)a.cu_seqlens[mid] <= t) lo = mid; else hi = mid - 1;
+    }
+    i = lo;
+    p = (int64_t)a.context_lens[i] + (t - a.cu_seqlens[i]);
+  }
+  if (p < 0) return -1;
+  int64_t col = p >> a.block_shift;
+  if (col > a.max_blocks - 1) col = a.max_blocks - 1;
+  const int64_t b = a.block_table[(int64_t)i * a.bt_row_stride + col];
+  if (b < 0 || b >= a.num_blocks) return -1;
+  return ((b * a.num_kv_heads) << a.block_shift) + (p & ((1 << a.block_shift) - 1));
+}
+
+// Largest finite magnitude of the two 16-bit elements of w, as 16 bits; `inf`: the format's
+// infinity.
+__device__ __forceinline__ uint32_t finite_max(uint32_t w, uint32_t inf) {
+  const uint32_t a = w & 0x7fffu, b = (w >> 16) & 0x7fffu;
+  const uint32_t x = a < inf ? a : 0u, y = b < inf ? b : 0u;
+  return x > y ? x : y;
+}
+
+// Two 16-bit elements -> two codes in the low half (HI: the high half) of `old`.
+template <bool F16, bool HI>
+__device__ __forceinline__ int quant2(uint32_t w, float mul, int old) {
+  using T = Elt<F16>;
+  // what is not finite becomes NaN (a saturating conversion would hide an infinity)
+  const float nan = __uint_as_float(0x7fc00000u);
+  constexpr uint32_t inf = F16 ? 0x7c00u : 0x7f80u;
+  const float x = (w & 0x7fffu) < inf ? T::lo(w) * mul : nan;
+  const float y = ((w >> 16) & 0x7fffu) < inf ? T::hi(w) * mul : nan;
+  return __builtin_amdgcn_cvt_pk_fp8_f32(x, y, old, HI);
+}
+template <bool F16>
+__device__ __forceinline__ u32x2 quant8(const u32x4& w, float mul) {
+  const int a = quant2<F16, true>(w[1], mul, quant2<F16, false>(w[0], mul, 0));
+  const int b = quant2<F16, true>(w[3], mul, quant2<F16, false>(w[2], mul, 0));
+  return u32x2{(uint32_t)a, (uint32_t)b};
+}
+
+// One wave per (token, round of 64 items); an item is 8 elements of a row's first half and the 8
+// they rotate with, so D / 16 lanes hold a row and its maximum is a butterfly over them.  A
+// token's items are the 2 Hkv rows of K and V, then the H rows of q.  As in rope_append.hip the
+// loads go out first, then the slot is looked up; lanes past the last item load a valid one
+// again and store nothing.
+template <int D, bool F16>
+__global__ __launch_bounds__(256) void kv_append_fp8_kernel(QuantArgs a) {
+  constexpr int CPH = D / 16, HALF = D / 2;
+  const int lane = threadIdx.x & 63;
+  const int64_t w =
+      (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int H = a.num_heads, Hkv = a.num_kv_heads;
+  const int kv_items = 2 * Hkv * CPH, q_items = a.q ? H * CPH : 0;
+  const int kv_rounds = (kv_items + 63) >> 6, rounds = kv_rounds + ((q_items + 63) >> 6);
+  const int64_t t = w / rounds;
+  const int r = (int)(w - t * rounds);
+  if (t >= a.num_tokens) return;
+  const bool kv = r < kv_rounds;
+  const int items = kv ? kv_items : q_items;
+  const int item0 = 64 * (kv ? r : r - kv_rounds) + lane;
+  const bool live = item0 < items;
+  const int item = live ? item0 : items - 1;
+  const int row = item / CPH, d0 = 8 * (item - row * CPH);
+  const bool is_v = kv && row >= Hkv;
+  const int h = is_v ? row - Hkv : row;
+  const u16* src = kv ? (is_v ? a.v + t * a.v_stride : a.k + t * a.k_stride)
+                      : a.q + t * a.q_stride;
+  src += h * D + d0;
+  u32x4 lo = ld16(src), hi = ld16(src + HALF);
+  if (a.cos != nullptr) {
+    const u16 *cs = a.cos + t * a.cs_stride + d0, *sn = a.sin + t * a.cs_stride + d0;
+    const u32x4 clo = ld16(cs), chi = ld16(cs + HALF), slo = ld16(sn), shi = ld16(sn + HALF);
+    u32x4 rlo, rhi;
+    rope8<F16>(lo, hi, clo, chi, slo, shi, rlo, rhi);
+    if (!is_v) {
+      lo = rlo;
+      hi = rhi;
+    }
+  }
+  if (!kv) {
+    if (live) {
+      u16* const dst = a.q_out + (t * H + row) * D + d0;
+      st16(dst, lo);
+      st16(dst + HALF, hi);
+    }
+    return;
+  }
+  const int64_t slot = slot_row(a, t);
+  constexpr uint32_t inf = F16 ? 0x7c00u : 0x7f80u;
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t x = finite_max(lo[i], inf), y = finite_max(hi[i], inf);
+    m = m > x ? m : x;
+    m = m > y ? m : y;
+  }
+#pragma unroll
+  for (int o = 1; o < CPH; o <<= 1) {
+    const uint32_t x = (uint32_t)__shfl_xor((int)m, o, 64);
+    m = m > x ? m : x;
+  }
+  // 448 = 1.75 * 2^8: the row's exponent less 8, one more where its mantissa is past 1.75
+  const uint32_t bits = __float_as_uint(Elt<F16>::lo(m));
+  const int e8 = (int)(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+  const int byte = e8 < 1 ? 1 : e8;
+  const float mul = __uint_as_float((uint32_t)(254 - byte) << 23);
+  if (live && slot >= 0) {
+    const int64_t at = (is_v ? a.plane_rows : 0) + slot + ((int64_t)h << a.block_shift);
+    uint8_t* const dst = a.codes + at * D + d0;
+    *reinterpret_cast<u32x2*>(dst) = quant8<F16>(lo, mul);
+    *reinterpret_cast<u32x2*>(dst + HALF) = quant8<F16>(hi, mul);
+    if (d0 == 0) a.scales[at] = (uint8_t)byte;
+  }
+}
+
+// Two codes of w's low or high half times scale, in the 16-bit format.
+template <bool F16, bool HI>
+__device__ __forceinline__ uint32_t value2(uint32_t w, float scale) {
+  if constexpr (F16)
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, HI));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, HI));
+}
+
+// One wave per (token, round of 64 items); an item is 16 codes of one of the token's 2 Hkv rows.
+// Positions that have no slot read as zeros, tokens past the last sequence are not written.
+template <int D, bool F16>
+__global__ __launch_bounds__(256) void kv_read_fp8_kernel(QuantArgs a) {
+  constexpr int CPR = D / 16;
+  const int lane = threadIdx.x & 63;
+  const int64_t w =
+      (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int Hkv = a.num_kv_heads, items = 2 * Hkv * CPR, rounds = (items + 63) >> 6;
+  const int64_t t = w / rounds;
+  const int item = 64 * (int)(w - t * rounds) + lane;
+  if (t >= a.num_tokens) return;
+  if (t < (int64_t)a.cu_seqlens[0] || t >= (int64_t)a.cu_seqlens[a.num_seqs]) return;
+  const int64_t slot = slot_row(a, t);
+  if (item >= items) return;
+  const int row = item / CPR, d0 = 16 * (item - row * CPR);
+  const bool is_v = row >= Hkv;
+  const int h = is_v ? row - Hkv : row;
+  u32x4 c{0u, 0u, 0u, 0u};
+  float scale = 1.f;
+  if (slot >= 0) {
+    const int64_t at = (is_v ? a.plane_rows : 0) + slot + ((int64_t)h << a.block_shift);
+    c = ld16(a.codes + at * D + d0);
+    scale = __uint_as_float((uint32_t)a.scales[at] << 23);
+  }
+  u16* const dst = (is_v ? a.v_out : a.k_out) + (t * Hkv + h) * D + d0;
+  u32x4 o[2];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    o[i >> 1][2 * (i & 1)] = value2<F16, false>(c[i], scale);
+    o[i >> 1][2 * (i & 1) + 1] = value2<F16, true>(c[i], scale);
+  }
+  st16(dst, o[0]);
+  st16(dst + 8, o[1]);
+}
+
+int log2_of(int block_size) {
+  const int s = block_tile_shift(block_size);
+  return s < 0 ? -1 : s + 4;
+}
+
+}  // namespace
+}  // namespace ndl
+
+extern "C" int ndl_kv_append_fp8(void* codes, void* scales, int64_t num_blocks, int num_kv_heads,
+                                 int block_size, int head_dim, int dtype, const void* k,
+                                 int64_t k_tok_stride, const void* v, int64_t v_tok_stride,
+                                 void* q_out, const void* q, int64_t q_tok_stride, int num_heads,
+                                 const void* cos, const void* sin, int64_t cs_tok_stride,
+                                 const int32_t* block_table, int64_t bt_row_stride,
+                                 int max_blocks_per_seq, const int32_t* cu_seqlens,
+                                 const int32_t* context_lens, int num_seqs, int64_t num_tokens,
+                                 ndl_stream_t stream) {
+  using namespace ndl;
+  if (!dtype_supported(dtype) || (head_dim != 64 && head_dim != 128) || log2_of(block_size) < 0)
+    return NDL_ERR_UNSUPPORTED;
+  if (num_tokens < 0 || num_seqs < 0 || num_kv_heads <= 0 || num_blocks <= 0 ||
+      max_blocks_per_seq <= 0 || bt_row_stride < max_blocks_per_seq)
+    return NDL_ERR_INVALID_ARG;
+  if (num_tokens == 0) return NDL_OK;
+  if (!codes || !scales || !k || !v || !block_table || !context_lens || num_seqs == 0)
+    return NDL_ERR_INVALID_ARG;
+  if ((cos == nullptr) != (sin == nullptr) || (q == nullptr) != (q_out == nullptr) ||
+      (q != nullptr && cos == nullptr))
+    return NDL_ERR_INVALID_ARG;   // q is here to be rotated
+  if (cu_seqlens == nullptr && num_tokens != num_seqs) return NDL_ERR_INVALID_ARG;
+  const int64_t kv_row = (int64_t)num_kv_heads * head_dim;
+  if (k_tok_stride < kv_row || v_tok_stride < kv_row ||
+      (q != nullptr && (num_heads <= 0 || q_tok_stride < (int64_t)num_heads * head_dim)) ||
+      (cos != nullptr && cs_tok_stride < head_dim))
+    return NDL_ERR_INVALID_ARG;
+  if (((uintptr_t)codes | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q | (uintptr_t)q_out |
+       (uintptr_t)cos | (uintptr_t)sin) & 15u)
+    return NDL_ERR_INVALID_ARG;
+  if ((k_tok_stride | v_tok_stride | (q ? q_tok_stride : 0) | (cos ? cs_tok_stride : 0)) & 7)
+    return NDL_ERR_INVALID_ARG;
+  QuantArgs a{};
+  a.codes = (uint8_t*)codes;
+  a.scales = (uint8_t*)scales;
+  a.plane_rows = num_blocks * num_kv_heads * (int64_t)block_size;
+  a.num_blocks = num_blocks;
+  a.num_heads = num_heads;
+  a.num_kv_heads = num_kv_heads;
+  a.block_shift = log2_of(block_size);
+  a.k = (const u16*)k;
+  a.v = (const u16*)v;
+  a.k_stride = k_tok_stride;
+  a.v_stride = v_tok_stride;
+  a.q = (const u16*)q;
+  a.q_out = (u16*)q_out;
+  a.q_stride = q_tok_stride;
+  a.cos = (const u16*)cos;
+  a.sin = (const u16*)sin;
+  a.cs_stride = cs_tok_stride;
+  a.block_table = block_table;
+  a.bt_row_stride = bt_row_stride;
+  a.max_blocks = max_blocks_per_seq;
+  a.cu_seqlens = cu_seqlens;
+  a.context_lens = context_lens;
+  a.num_seqs = num_seqs;
+  a.num_tokens = num_tokens;
+  const int64_t cph = head_dim / 16;
+  const int64_t rounds =
+      (2 * num_kv_heads * cph + 63) / 64 + (q ? (num_heads * cph + 63) / 64 : 0);
+  const int64_t blocks = (num_tokens * rounds + 3) / 4;
+  if (blocks > 0x7fffffff) return NDL_ERR_INVALID_ARG;
+  const dim3 grid((unsigned)blocks), wg(256);
+  const hipStream_t s = (hipStream_t)stream;
+  const bool f16 = dtype_is_f16(dtype);
+  if (head_dim == 128) {
+    if (f16)
+      hipLaunchKernelGGL((kv_append_fp8_kernel<128, true>), grid, wg, 0, s, a);
+    else
+      hipLaunchKernelGGL((kv_append_fp8_kernel<128, false>), grid, wg, 0, s, a);
+  } else {
+    if (f16)
+      hipLaunchKernelGGL((kv_append_fp8_kernel<64, true>), grid, wg, 0, s, a);
+    else
+      hipLaunchKernelGGL((kv_append_fp8_kernel<64, false>), grid, wg, 0, s, a);
+  }
+  return check_launch();
+}
+
+extern "C" int ndl_kv_read_fp8(void* k_out, void* v_out, const void* codes, const void* scales,
+                               int64_t num_blocks, int num_kv_heads, int block_size,
+                               int head_dim, int dtype, const int32_t* block_table,
+                               int64_t bt_row_stride, int max_blocks_per_seq,
+                               const int32_t* first, const int32_t* cu_seqlens, int num_seqs,
+                               int64_t num_tokens, ndl_stream_t stream) {
+  using namespace ndl;
+  if (!dtype_supported(dtype) || (head_dim != 64 && head_dim != 128) || log2_of(block_size) < 0)
+    return NDL_ERR_UNSUPPORTED;
+  if (num_tokens < 0 || num_seqs < 0 || num_kv_heads <= 0 || num_blocks <= 0 ||
+      max_blocks_per_seq <= 0 || bt_row_stride < max_blocks_per_seq)
+    return NDL_ERR_INVALID_ARG;
+  if (num_tokens == 0 || num_seqs == 0) return NDL_OK;
+  if (!k_out || !v_out || !codes || !scales || !block_table || !first || !cu_seqlens)
+    return NDL_ERR_INVALID_ARG;
+  if (((uintptr_t)codes | (uintptr_t)k_out | (uintptr_t)v_out) & 15u) return NDL_ERR_INVALID_ARG;
+  QuantArgs a{};
+  a.codes = (uint8_t*)const_cast<void*>(codes);
+  a.scales = (uint8_t*)const_cast<void*>(scales);
+  a.plane_rows = num_blocks * num_kv_heads * (int64_t)block_size;
+  a.num_blocks = num_blocks;
+  a.num_kv_heads = num_kv_heads;
+  a.block_shift = log2_of(block_size);
+  a.block_table = block_table;
+  a.bt_row_stride = bt_row_stride;
+  a.max_blocks = max_blocks_per_seq;
+  a.cu_seqlens = cu_seqlens;
+  a.context_lens = first;
+  a.num_seqs = num_seqs;
+  a.num_tokens = num_tokens;
+  a.k_out = (u16*)k_out;
+  a.v_out = (u16*)v_out;
+  const int64_t rounds = (2 * num_kv_heads * (head_dim / 16) + 63) / 64;
+  const int64_t blocks = (num_tokens * rounds + 3) / 4;
+  if (blocks > 0x7fffffff) return NDL_ERR_INVALID_ARG;
+  const dim3 grid((unsigned)blocks), wg(256);
+  const hipStream_t s = (hipStream_t)stream;
+  const bool f16 = dtype_is_f16(dtype);
+  if (head_dim == 128) {
+    if (f16)
+      hipLaunchKernelGGL((kv_read_fp8_kernel<128, true>), grid, wg, 0, s, a);
+    else
+      hipLaunchKernelGGL((kv_read_fp8_kernel<128, false>), grid, wg, 0, s, a);
+  } else {
+    if (f16)
+      hipLaunchKernelGGL((kv_read_fp8_kernel<64, true>), grid, wg, 0, s, a);
+    else
+      hipLaunchKernelGGL((kv_read_fp8_kernel<64, false>), grid, wg, 0, s, a);
+  }
+  return check_launch();
+}

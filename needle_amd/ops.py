@@ -14,7 +14,7 @@ Argument meaning follows the reference:
 from __future__ import annotations
 
 import os
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 import torch.nn.functional as F
@@ -736,3 +736,321 @@ def greedy_argmax(logits: torch.Tensor, out: Optional[torch.Tensor] = None) -> t
                                _ptr(ws), nbytes, _stream(logits.device))
     _lib.check(rc, "ndl_greedy_argmax")
     return out
+
+
+# ---------------------------------------------------------------- the 8-bit pool
+
+class Fp8KVCache(NamedTuple):
+    """A layer's 8-bit pool, where kv_cache stands for a 16-bit one (Attention.forward): e4m3
+    codes [2, num_blocks, num_kv_heads, block_size, head_dim] and a byte per row (token, head),
+    [2, num_blocks, num_kv_heads, block_size].  A row's values are code * 2^(byte - 127)."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+    @property
+    def shape(self):
+        return self.codes.shape
+
+
+def fp8_kv_pool(num_blocks: int, num_kv_heads: int, block_size: int, head_dim: int, device=None,
+                pin_memory: bool = False) -> Fp8KVCache:
+    """A zero-filled pool (every value 0)."""
+    shape = (2, num_blocks, num_kv_heads, block_size)
+    codes = torch.zeros((*shape, head_dim), dtype=torch.uint8, device=device,
+                        pin_memory=pin_memory)
+    scales = torch.zeros(shape, dtype=torch.uint8, device=device, pin_memory=pin_memory)
+    return Fp8KVCache(codes.view(torch.float8_e4m3fn), scales)
+
+
+_FP8_CODES = (torch.float8_e4m3fn, torch.uint8)
+
+
+def _check_fp8_cache(kv_codes: torch.Tensor, kv_scales: torch.Tensor):
+    """(num_blocks, num_kv_heads, block_size, head_dim) of an 8-bit pool."""
+    if kv_codes.dim() != 5 or kv_codes.shape[0] != 2:
+        raise ValueError("kv_codes must be [2, num_blocks, num_kv_heads, block_size, head_dim], "
+                         f"got {tuple(kv_codes.shape)}")
+    if kv_codes.dtype not in _FP8_CODES or kv_scales.dtype != torch.uint8:
+        raise TypeError("kv_codes must be float8_e4m3fn (or its bytes, uint8) and kv_scales "
+                        f"uint8, got {kv_codes.dtype} and {kv_scales.dtype}")
+    if kv_scales.shape != kv_codes.shape[:4]:
+        raise ValueError(f"kv_scales must be {tuple(kv_codes.shape[:4])}, got "
+                         f"{tuple(kv_scales.shape)}")
+    _require(kv_codes.is_cuda and kv_scales.device == kv_codes.device,
+             "kv_codes and kv_scales must be on one GPU")
+    _require(kv_codes.is_contiguous() and kv_scales.is_contiguous(),
+             "kv_codes and kv_scales must be contiguous")
+    _, nb, hkv, bs, d = kv_codes.shape
+    if d not in (64, 128):
+        raise ValueError(f"the 8-bit pool is built for head_dim 64 and 128, got {d}")
+    if bs < 16 or bs > 1024 or bs & (bs - 1):
+        raise ValueError("the 8-bit pool is built for blocks of a power of two from 16 to 1024 "
+                         f"tokens, got {bs}")
+    return nb, hkv, bs, d
+
+
+def _check_16bit(name: str, dtype: torch.dtype) -> None:
+    if dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"{name} must be bfloat16 or float16 with an 8-bit pool, got {dtype}")
+
+
+def _check_table(block_table: torch.Tensor, num_blocks: int, device) -> int:
+    _check_int32("block_table", block_table, 2, device)
+    if _validate_enabled():
+        _validate_slots(block_table, num_blocks)
+    return block_table.shape[0]
+
+
+def kv_append_fp8(k: torch.Tensor, v: torch.Tensor, kv_codes: torch.Tensor,
+                  kv_scales: torch.Tensor, block_table: torch.Tensor,
+                  context_lens: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None, *,
+                  q: Optional[torch.Tensor] = None, cos: Optional[torch.Tensor] = None,
+                  sin: Optional[torch.Tensor] = None,
+                  out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """kv_append into an 8-bit pool (Fp8KVCache): k/v [T, Hkv, D] in bfloat16 or float16, each
+    row quantised as it is written: e4m3 codes of its values divided by the smallest power of
+    two (at least 2^-126) that leaves none above 448, rounded to nearest even; NaN where a value
+    is not finite.
+
+    cos / sin [T, D] rotate k first, with rope_kv_append's roundings, and q [T, H, D] too if it
+    is given: then the rotated q is returned (written to out, contiguous, if that is given).
+    cu_seqlens None: one token per sequence.
+    """
+    nb, hkv, bs, d = _check_fp8_cache(kv_codes, kv_scales)
+    dev, dtype = kv_codes.device, k.dtype
+    _check_16bit("k", dtype)
+    for name, x in (("v", v), ("q", q), ("cos", cos), ("sin", sin)):
+        if x is not None and x.dtype != dtype:
+            raise TypeError(f"{name} dtype must match k")
+    ks, vs, n_tok = _rows("k", k, hkv, d, dev), _rows("v", v, hkv, d, dev), k.shape[0]
+    _require(v.shape[0] == n_tok, "k and v token counts differ")
+    _require((cos is None) == (sin is None), "pass both cos and sin, or neither")
+    h, qs, cs = 0, 0, 0
+    if cos is not None:
+        for name, x in (("cos", cos), ("sin", sin)):
+            if x.dim() != 2 or x.shape[0] != n_tok or x.shape[1] != d:
+                raise ValueError(f"{name} must be [{n_tok}, {d}], got {tuple(x.shape)}")
+            if x.device != dev or x.stride(1) != 1:
+                raise ValueError(f"{name} rows must be contiguous on {dev}")
+        _require(cos.stride(0) == sin.stride(0) or n_tok <= 1, "cos and sin token strides differ")
+        cs = cos.stride(0) if n_tok > 1 else d
+    if q is not None:
+        _require(cos is not None, "q is passed to be rotated: pass cos and sin")
+        if q.dim() != 3:
+            raise ValueError(f"q must be [T, H, {d}], got {tuple(q.shape)}")
+        h = q.shape[1]
+        qs = _rows("q", q, h, d, dev)
+        _require(q.shape[0] == n_tok, "q/k/v token counts differ")
+        _require(h > 0, "q has no heads")
+        if out is None:
+            out = torch.empty((n_tok, h, d), dtype=dtype, device=dev)
+        else:
+            _require(out.shape == (n_tok, h, d) and out.is_contiguous() and out.dtype == dtype
+                     and out.device == dev, "out must be a contiguous [T, H, D] tensor like q")
+    else:
+        _require(out is None, "out is the rotated q: pass q with it")
+    n_seqs = _check_table(block_table, nb, dev)
+    _check_int32("context_lens", context_lens, 1, dev)
+    _require(context_lens.shape[0] == n_seqs, "context_lens/block_table batch mismatch")
+    if cu_seqlens is None:
+        _require(n_tok == n_seqs, f"decode append needs one token per sequence "
+                 f"({n_tok} tokens, {n_seqs} sequences)")
+    else:
+        _check_int32("cu_seqlens", cu_seqlens, 1, dev)
+        _require(cu_seqlens.shape[0] == n_seqs + 1, "cu_seqlens must be [num_seqs + 1]")
+    if n_tok == 0:
+        return out
+    _require(block_table.shape[1] > 0, "block_table has no columns")
+    rc = _lib.load().ndl_kv_append_fp8(
+        kv_codes.data_ptr(), kv_scales.data_ptr(), nb, hkv, bs, d, _DTYPES[dtype],
+        k.data_ptr(), ks, v.data_ptr(), vs, _ptr(out), _ptr(q), qs, h, _ptr(cos), _ptr(sin), cs,
+        block_table.data_ptr(), block_table.stride(0), block_table.shape[1], _ptr(cu_seqlens),
+        context_lens.data_ptr(), n_seqs, n_tok, _stream(dev))
+    _lib.check(rc, "ndl_kv_append_fp8")
+    return out
+
+
+def kv_read_fp8(kv_codes: torch.Tensor, kv_scales: torch.Tensor, block_table: torch.Tensor,
+                first: torch.Tensor, cu_seqlens: torch.Tensor, num_tokens: int, *,
+                dtype: torch.dtype = torch.bfloat16):
+    """Ranges of cached tokens in 16 bits: (k, v) [num_tokens, Hkv, D], packed by cu_seqlens, of
+    the tokens first[i], first[i] + 1, .. of each sequence.  bfloat16 has every value of the pool
+    exactly; float16 every one that came from a float16 row, but for its smallest subnormals.
+    first: int32 [num_seqs].  Rows outside cu_seqlens hold nothing in particular."""
+    nb, hkv, bs, d = _check_fp8_cache(kv_codes, kv_scales)
+    dev = kv_codes.device
+    _check_16bit("dtype", dtype)
+    n_seqs = _check_table(block_table, nb, dev)
+    _check_int32("first", first, 1, dev)
+    _check_int32("cu_seqlens", cu_seqlens, 1, dev)
+    _require(first.shape[0] == n_seqs, "first/block_table batch mismatch")
+    _require(cu_seqlens.shape[0] == n_seqs + 1, "cu_seqlens must be [num_seqs + 1]")
+    _require(num_tokens >= 0, "num_tokens is negative")
+    k = torch.empty((num_tokens, hkv, d), dtype=dtype, device=dev)
+    v = torch.empty_like(k)
+    if num_tokens == 0 or n_seqs == 0:
+        return k, v
+    _require(block_table.shape[1] > 0, "block_table has no columns")
+    rc = _lib.load().ndl_kv_read_fp8(
+        k.data_ptr(), v.data_ptr(), kv_codes.data_ptr(), kv_scales.data_ptr(), nb, hkv, bs, d,
+        _DTYPES[dtype], block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
+        first.data_ptr(), cu_seqlens.data_ptr(), n_seqs, num_tokens, _stream(dev))
+    _lib.check(rc, "ndl_kv_read_fp8")
+    return k, v
+
+
+def _fp8_attention(q, kv_codes, kv_scales, block_table, cu_seqlens, context_lens, max_seqlen,
+                   max_keys, scale, num_heads, num_kv_heads, head_dim, out, workspace):
+    nb, hkv, bs, d = _check_fp8_cache(kv_codes, kv_scales)
+    dev = kv_codes.device
+    _require(hkv == num_kv_heads and d == head_dim, "kv_codes shape disagrees with head counts")
+    _check_16bit("q", q.dtype)
+    qs = _rows("q", q, num_heads, head_dim, dev)
+    if num_heads % num_kv_heads or num_heads // num_kv_heads > 16:
+        raise ValueError(f"num_heads {num_heads} must be 1 to 16 times num_kv_heads "
+                         f"{num_kv_heads}")
+    n_seqs, n_tok = _check_table(block_table, nb, dev), q.shape[0]
+    _check_int32("context_lens", context_lens, 1, dev)
+    _require(context_lens.shape[0] == n_seqs, "context_lens/block_table batch mismatch")
+    if cu_seqlens is None:
+        _require(n_tok == n_seqs, "q / block_table batch mismatch")
+    else:
+        _check_int32("cu_seqlens", cu_seqlens, 1, dev)
+        _require(cu_seqlens.shape[0] == n_seqs + 1, "cu_seqlens must be [num_seqs + 1]")
+    if out is None:
+        out = torch.empty((n_tok, num_heads, head_dim), dtype=q.dtype, device=dev)
+    else:
+        _require(out.shape == (n_tok, num_heads, head_dim) and out.is_contiguous()
+                 and out.dtype == q.dtype and out.device == dev,
+                 f"out must be a contiguous {q.dtype} [{n_tok}, {num_heads}, {head_dim}] "
+                 f"tensor on {dev}")
+    if n_tok == 0 or n_seqs == 0:
+        return out
+    w = block_table.shape[1]
+    _require(w > 0, "block_table has no columns")
+    _require(max_seqlen > 0, "max_seqlen must be positive")
+    max_keys = min(w * bs, max_keys) if max_keys else w * bs
+    lib = _lib.load()
+    need = lib.ndl_fp8_attention_workspace_bytes(n_seqs, max_seqlen, max_keys, num_heads,
+                                                 num_kv_heads, head_dim, bs)
+    if need and (workspace is None or workspace.numel() * workspace.element_size() < need
+                 or workspace.device != dev):
+        workspace = decode_workspace(need, dev)
+    rc = lib.ndl_fp8_attention(
+        out.data_ptr(), q.data_ptr(), qs, kv_codes.data_ptr(), kv_scales.data_ptr(), nb,
+        block_table.data_ptr(), block_table.stride(0), w, _ptr(cu_seqlens),
+        context_lens.data_ptr(), n_seqs, n_tok, max_seqlen, max_keys, num_heads, num_kv_heads,
+        head_dim, bs, _DTYPES[q.dtype], float(scale), _ptr(workspace) if need else None, need,
+        _stream(dev))
+    _lib.check(rc, "ndl_fp8_attention")
+    return out
+
+
+def fp8_attention_workspace_bytes(num_seqs: int, max_seqlen: int, max_keys: int, num_heads: int,
+                                  num_kv_heads: int, head_dim: int, block_size: int = 16) -> int:
+    """Bytes of the workspace paged_decode_fp8 (max_seqlen 1, max_keys the table's) or
+    varlen_prefill_fp8 uses on the current GPU; 0 where the work is not split."""
+    return int(_lib.load().ndl_fp8_attention_workspace_bytes(
+        num_seqs, max_seqlen, max_keys, num_heads, num_kv_heads, head_dim, block_size))
+
+
+def paged_decode_fp8(q: torch.Tensor, kv_codes: torch.Tensor, kv_scales: torch.Tensor,
+                     block_table: torch.Tensor, context_lens: torch.Tensor, scale: float,
+                     num_heads: int, num_kv_heads: int, head_dim: int, *,
+                     out: Optional[torch.Tensor] = None,
+                     workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """paged_decode over an 8-bit pool (Fp8KVCache): q [num_seqs, H, D] in bfloat16 or float16,
+    sequence i attends min(context_lens[i] + 1, W * block_size) tokens.  Append (and rotate q)
+    with kv_append_fp8 first.  workspace: as decode_workspace gives, of
+    fp8_attention_workspace_bytes, for one call at a time."""
+    return _fp8_attention(q, kv_codes, kv_scales, block_table, None, context_lens, 1, 0, scale,
+                          num_heads, num_kv_heads, head_dim, out, workspace)
+
+
+def varlen_prefill_fp8(q: torch.Tensor, kv_codes: torch.Tensor, kv_scales: torch.Tensor,
+                       block_table: torch.Tensor, cu_seqlens: torch.Tensor,
+                       context_lens: torch.Tensor, max_seqlen: int, scale: float,
+                       num_heads: int, num_kv_heads: int, head_dim: int, *,
+                       max_context_len: int = 0, out: Optional[torch.Tensor] = None,
+                       workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """varlen_prefill over an 8-bit pool (Fp8KVCache): causal attention of packed chunks of new
+    tokens, from one per sequence to whole prompts, over what is cached and the chunk itself
+    (after kv_append_fp8).  Token j of sequence i attends min(context_lens[i] + j + 1,
+    W * block_size) tokens.  max_seqlen bounds a sequence's tokens, max_context_len its cached
+    ones (0: nothing cached, or not known; it only chooses how the work is split)."""
+    return _fp8_attention(q, kv_codes, kv_scales, block_table, cu_seqlens, context_lens,
+                          int(max_seqlen),
+                          int(max_context_len) + int(max_seqlen) if max_context_len else 0,
+                          scale, num_heads, num_kv_heads, head_dim, out, workspace)
+
+
+def verify_drafts(logits: torch.Tensor, ids: torch.Tensor, cu_seqlens: torch.Tensor,
+                  uniforms: torch.Tensor, *, temperature: Optional[torch.Tensor] = None,
+                  draft_probs: Optional[torch.Tensor] = None):
+    """Speculative decoding's verification: (tokens [T], accepted int32 [num_seqs]).
+
+    logits [T, vocab] (bfloat16, float16 or float32, rows contiguous, any row stride) are the
+    target's rows for the packed chunks ids [T] (int32 or int64): a sequence's newest token and
+    its drafts, at least one row each.  Row r judges the draft ids[r + 1]; a sequence's last row
+    judges none.  With p = softmax(logits[r] / temperature[i]) and q row r - i of draft_probs
+    (float32 [T - num_seqs, vocab]; None: the drafts have probability 1) a draft x is accepted
+    while uniforms[r] * q(x) < p(x), for it and all before it.  The next token follows
+    max(p - q, 0) of the first rejected row, or p of the last row, by the inverse of its
+    cumulative distribution at the sequence's last uniform: together distributed as the target.
+
+    temperature float32 [num_seqs] (None: 1); 0 takes the argmax, as does a row whose maximum is
+    not finite.  uniforms float32 [T] in [0, 1).  tokens, in ids' type: the accepted drafts, the
+    next token, then -1.  Graph-capturable; no host synchronisation."""
+    _require(logits.is_cuda, "logits must be a GPU tensor")
+    if logits.dtype not in _DTYPES:
+        raise TypeError(f"unsupported dtype {logits.dtype}")
+    if logits.dim() != 2:
+        raise ValueError(f"logits must be [rows, vocab], got {tuple(logits.shape)}")
+    rows, vocab = logits.shape
+    dev = logits.device
+    _require(vocab > 0, "logits have no columns")
+    _require(logits.stride(1) == 1 or vocab == 1, "logits rows must be contiguous")
+    _require(rows <= 1 or logits.stride(0) >= vocab, "logits rows overlap")
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"ids must be int32 or int64, got {ids.dtype}")
+    if ids.shape != (rows,) or not ids.is_contiguous() or ids.device != dev:
+        raise ValueError(f"ids must be a contiguous [{rows}] tensor on {dev}")
+    _check_int32("cu_seqlens", cu_seqlens, 1, dev)
+    n_seqs = cu_seqlens.shape[0] - 1
+    _require(n_seqs >= 0, "cu_seqlens must be [num_seqs + 1]")
+    _require(rows >= n_seqs, f"every sequence has a row: {rows} rows, {n_seqs} sequences")
+
+    def check(name, t, shape):
+        if t.dtype != torch.float32:
+            raise TypeError(f"{name} must be float32, got {t.dtype}")
+        if t.shape != shape or t.device != dev or (t.numel() and t.stride(-1) != 1
+                                                   and shape[-1] != 1):
+            raise ValueError(f"{name} must be {list(shape)} with contiguous rows on {dev}, got "
+                             f"{tuple(t.shape)}")
+
+    check("uniforms", uniforms, (rows,))
+    if temperature is not None:
+        check("temperature", temperature, (n_seqs,))
+    ds = vocab
+    if draft_probs is not None:
+        check("draft_probs", draft_probs, (rows - n_seqs, vocab))
+        if rows - n_seqs > 1:
+            ds = draft_probs.stride(0)
+            _require(ds >= vocab, "draft_probs rows overlap")
+    tokens = torch.empty_like(ids)
+    accepted = torch.empty(n_seqs, dtype=torch.int32, device=dev)
+    if n_seqs == 0:
+        return tokens, accepted
+    lib = _lib.load()
+    need = lib.ndl_verify_drafts_workspace_bytes(rows, n_seqs, vocab)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    # without drafts there are no draft rows, and no address either
+    probs = draft_probs if draft_probs is not None and rows > n_seqs else None
+    rc = lib.ndl_verify_drafts(
+        tokens.data_ptr(), accepted.data_ptr(), logits.data_ptr(),
+        logits.stride(0) if rows > 1 else vocab, _DTYPES[logits.dtype], ids.data_ptr(),
+        int(ids.dtype == torch.int64), cu_seqlens.data_ptr(), uniforms.data_ptr(),
+        _ptr(temperature), _ptr(probs), ds, rows - n_seqs, rows, n_seqs, vocab, ws.data_ptr(),
+        need, _stream(dev))
+    _lib.check(rc, "ndl_verify_drafts")
+    return tokens, accepted

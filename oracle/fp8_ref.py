@@ -1,0 +1,137 @@
+"""The 8-bit pool and draft verification from their definitions, in float64 on the CPU (tests
+only)."""
+from __future__ import annotations
+
+import math
+
+import torch
+
+E4M3_MAX = 448.0
+
+
+def code_values() -> torch.Tensor:
+    """The value of each e4m3 byte (NaN at 0x7f and 0xff)."""
+    out = []
+    for b in range(256):
+        m, e = b & 7, (b >> 3) & 15
+        v = (1 + m / 8) * 2.0 ** (e - 7) if e else m / 8 * 2.0 ** -6
+        v = math.nan if b & 127 == 127 else v
+        out.append(-v if b & 128 else v)
+    return torch.tensor(out, dtype=torch.float64)
+
+
+def quantise_row(x):
+    """(codes, byte) of one row of floats: the nearest code of x * 2^-e, ties to the even code."""
+    table = code_values()[:127]
+    finite = [abs(v) for v in x if math.isfinite(v)]
+    a, e = max(finite, default=0.0), -126
+    while a > E4M3_MAX * 2.0 ** e:
+        e += 1
+    codes = []
+    for v in x:
+        if not math.isfinite(v):
+            codes.append(0x7F)
+            continue
+        y = abs(v) * 2.0 ** -e
+        d = (table - y).abs()
+        near = (d == d.min()).nonzero()[:, 0].tolist()
+        c = near[0] if len(near) == 1 else next(i for i in near if i % 2 == 0)
+        codes.append(c | (0x80 if math.copysign(1.0, v) < 0 else 0))
+    return codes, e + 127
+
+
+def values(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+    """float64 values of codes [.., D] (bytes) under scales [..]."""
+    two = torch.tensor([2.0 ** (b - 127) for b in range(256)], dtype=torch.float64)
+    return code_values()[codes.view(torch.uint8).long()] * two[scales.long()].unsqueeze(-1)
+
+
+def slot(table_row, p, block_size, num_blocks):
+    """(block, row) of position p, or None."""
+    if p < 0:
+        return None
+    b = int(table_row[min(p // block_size, len(table_row) - 1)])
+    return (b, p % block_size) if 0 <= b < num_blocks else None
+
+
+def attention(q, codes, scales, block_table, cu, context_lens, scale):
+    """(out, weight) [T, H, D] in float64: the attention, and sum_t p_t |v_t|, what a rounding of
+    the probabilities is relative to; rows outside cu are NaN.  Also the largest
+    scale * sum_d |q_d k_d| of every row [T, H] and the attended lengths [T]."""
+    _, nb, hkv, bs, d = codes.shape
+    t, h, _ = q.shape
+    g = h // hkv
+    out = torch.full((t, h, d), math.nan, dtype=torch.float64)
+    weight, big = out.clone(), torch.zeros(t, h, dtype=torch.float64)
+    lens = torch.zeros(t, dtype=torch.long)
+    w = block_table.shape[1]
+    for i in range(block_table.shape[0]):
+        for j in range(int(cu[i + 1]) - int(cu[i])):
+            r = int(cu[i]) + j
+            n = min(int(context_lens[i]) + j + 1, w * bs)
+            pages = [slot(block_table[i], p, bs, nb) for p in range(max(n, 0))]
+            pages = [p for p in pages if p is not None]
+            lens[r] = len(pages)
+            if not pages:
+                out[r], weight[r] = 0.0, 0.0
+                continue
+            blk, row = (torch.tensor(x) for x in zip(*pages))
+            kv = values(codes[:, blk, :, row], scales[:, blk, :, row])     # [n, 2, Hkv, D]
+            for head in range(h):
+                k, v = kv[:, 0, head // g], kv[:, 1, head // g]
+                qr = q[r, head].double()
+                big[r, head] = (k.abs() @ qr.abs()).max() * abs(scale)
+                p = torch.softmax(k @ qr * scale, dim=0)
+                out[r, head], weight[r, head] = p @ v, p @ v.abs()
+    return out, weight, big, lens
+
+
+def point(row: torch.Tensor) -> int:
+    """torch's argmax: the first NaN, or the first of the largest."""
+    return int(row.argmax())
+
+
+def verify(logits, ids, cu, uniforms, temperature=None, draft_probs=None):
+    """(tokens, accepted) by the definition, one sequence at a time."""
+    t, v = logits.shape
+    n = len(cu) - 1
+    tokens, accepted = [-1] * t, [0] * n
+
+    def target(i, r):
+        row = logits[r].double()
+        temp = 1.0 if temperature is None else float(temperature[i])
+        if not temp > 0 or not math.isfinite(float(row.max())):
+            p = torch.zeros(v, dtype=torch.float64)
+            p[point(logits[r])] = 1.0
+            return p
+        return torch.softmax((row - row.max()) / temp, dim=0)
+
+    for i in range(n):
+        a, b = int(cu[i]), int(cu[i + 1])
+        k = 0
+        for r in range(a, b - 1):
+            x = int(ids[r + 1])
+            p = target(i, r)
+            q = torch.zeros(v, dtype=torch.float64)
+            if draft_probs is not None:
+                q = draft_probs[r - i].double()
+            elif 0 <= x < v:
+                q[x] = 1.0
+            if not (0 <= x < v and float(uniforms[r]) * float(q[x]) < float(p[x])):
+                break
+            tokens[a + k] = x
+            k += 1
+        accepted[i] = k
+        p = target(i, a + k)
+        weights = p
+        if a + k < b - 1:
+            weights = (p - torch.where(q > 0, q, 0.0)).clamp(min=0.0)
+            if not float(weights.sum()) > 0:
+                weights = p
+        u = float(uniforms[b - 1])
+        u = min(max(u, 0.0), 1.0) if u == u else 0.0
+        c = weights.cumsum(0)
+        hit = ((c > u * c[-1]) & (weights > 0)).nonzero()[:, 0]
+        some = (weights > 0).nonzero()[:, 0]
+        tokens[a + k] = int(hit[0]) if len(hit) else int(some[-1])
+    return tokens, accepted
