@@ -585,8 +585,9 @@ int ndl_fp8_attention(void* out, const void* q, int64_t q_tok_stride, const void
  * tokens [num_rows], in ids' type: a sequence's accepted drafts, the next token, then -1;
  * accepted [num_seqs].  logits in `dtype`, any row stride of at least vocab; draft_probs float32
  * [num_rows - num_seqs] rows; uniforms and temperature float32 [num_rows], [num_seqs]
- * (temperature NULL: 1).  num_rows and num_seqs at most 65535.  The workspace is 256-byte aligned
- * and belongs to one call at a time.
+ * (temperature NULL: 1).  num_rows and num_seqs at most 65535, vocab at most 2^18
+ * (NDL_ERR_UNSUPPORTED otherwise).  The workspace is 256-byte aligned and belongs to one call at a
+ * time.
  */
 size_t ndl_verify_drafts_workspace_bytes(int64_t num_rows, int num_seqs, int vocab);
 int ndl_verify_drafts(void* tokens, int32_t* accepted, const void* logits, int64_t row_stride,

@@ -28,10 +28,14 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kStatSlice = 4096;     // elements of a slice at least
-constexpr int kStatWgs = 2048;       // workgroups wanted over all rows
-constexpr int kSumSlice = 2048;
-constexpr int kSumWgs = 1024;
+constexpr int kStatWgs = 1536;       // workgroups wanted over all rows: what the GPU holds at once
+constexpr int kSumSlice = 2048;      // a step of a workgroup; slices are whole steps
+constexpr int kSumWgs = 2048;
 constexpr int kMaxSlices = 64;       // a lane of a wave each
+constexpr int kPickLen = 6144;       // elements of a chosen row's slice at most: they fit the LDS
+constexpr int kMaxVocab = 1 << 18;
+static_assert(kMaxVocab <= kMaxSlices * kPickLen, "a slice's weights fit the LDS");
+constexpr int kAccept = 64;          // rows judged at a time
 
 struct Info {            // of a sequence, written by `sums`
   int accepted;
@@ -86,26 +90,59 @@ __device__ __forceinline__ bool better(float va, int ia, float vb, int ib) {
   if (na || nb) return na && (!nb || ia < ib);
   return va > vb || (va == vb && ia < ib);
 }
-__device__ __forceinline__ void wave_best(float& v, int& i) {
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    const float ov = __shfl_xor(v, m, 64);
-    const int oi = __shfl_xor(i, m, 64);
-    if (better(ov, oi, v, i)) {
-      v = ov;
-      i = oi;
-    }
+// The value of the lane that a DPP pattern names (all of a row's lanes are active).
+template <int PATTERN>
+__device__ __forceinline__ float dpp(float v) {
+  return __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(v), PATTERN, 0xf, 0xf, true));
+}
+template <int PATTERN>
+__device__ __forceinline__ double dpp(double v) {
+  const uint64_t w = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_mov_dpp((int)(uint32_t)w, PATTERN, 0xf, 0xf, true);
+  const uint32_t hi = __builtin_amdgcn_mov_dpp((int)(uint32_t)(w >> 32), PATTERN, 0xf, 0xf, true);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// Lane l ^ 16 (ROWS 16) or l ^ 32: v_permlane*_swap returns the lower row's value in one result
+// and the upper one's in the other, so both lanes combine the same two in the same order.
+template <int ROWS>
+__device__ __forceinline__ u32x2 pair_of(uint32_t v) {
+  if constexpr (ROWS == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return u32x2{r[0], r[1]};
+  } else {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return u32x2{r[0], r[1]};
   }
 }
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
-  return v;
+template <int ROWS, class OP>
+__device__ __forceinline__ float across(float v, OP op) {
+  const u32x2 r = pair_of<ROWS>(__float_as_uint(v));
+  return op(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
-  return v;
+template <int ROWS, class OP>
+__device__ __forceinline__ double across(double v, OP op) {
+  const uint64_t w = __builtin_bit_cast(uint64_t, v);
+  const u32x2 lo = pair_of<ROWS>((uint32_t)w), hi = pair_of<ROWS>((uint32_t)(w >> 32));
+  return op(__builtin_bit_cast(double, (uint64_t)hi[0] << 32 | lo[0]),
+            __builtin_bit_cast(double, (uint64_t)hi[1] << 32 | lo[1]));
+}
+// v combined over the wave's 64 lanes, on the VALU (a butterfly through the LDS crossbar takes
+// about 100 cycles a step): pairs, quads, mirrored halves of 8 and of 16, then rows.
+template <class T, class OP>
+__device__ __forceinline__ T wave_all(T v, OP op) {
+  v = op(v, dpp<0xb1>(v));      // quad_perm [1, 0, 3, 2]
+  v = op(v, dpp<0x4e>(v));      // quad_perm [2, 3, 0, 1]
+  v = op(v, dpp<0x141>(v));     // row_half_mirror
+  v = op(v, dpp<0x140>(v));     // row_mirror
+  v = across<16>(v, op);
+  return across<32>(v, op);
+}
+template <class T>
+__device__ __forceinline__ T wave_sum(T v) {
+  return wave_all(v, [](T x, T y) { return x + y; });
+}
+__device__ __forceinline__ float wave_max(float v) {
+  return wave_all(v, [](float x, float y) { return fmaxf(x, y); });
 }
 
 __device__ __forceinline__ int64_t draft_at(const VerifyArgs& a, int64_t i) {
@@ -134,19 +171,33 @@ __device__ __forceinline__ float temperature_of(const VerifyArgs& a, int i) {
 __device__ __forceinline__ float rate_of(float temp) {
   return fmaxf(fminf(kLog2e / temp, 3e38f), 1e-30f);
 }
-// exp((l - top) / T) as 2^((l - top) k); 0 for a masked entry (-inf * 0 is not asked).
-__device__ __forceinline__ float term(float l, float top, float k) {
-  const float x = (l - top) * k;
-  return l == kNegInf ? 0.f : fast_exp2(x);
-}
 
-// Workgroup (slice s, row r): maximum, argmax and the sum of exp((l - maximum) / T).
+// Workgroup (slice s, row r): maximum and sum of exp((l - maximum) / T) in one pass.  Where the
+// row is a point (T = 0, or a slice that holds a NaN or an infinity: the sum is NaN then), the
+// maximum and its first index instead.
 template <int FMT>
 __global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerifyArgs a) {
   constexpr int EB = FMT == kFmtF32 ? 4 : 2, PER = 16 / EB;
-  constexpr int kBatch = FMT == kFmtF32 ? 8 : 4;      // loads in flight (32 elements)
-  const int s = blockIdx.x;
+  constexpr int kBatch = 4;            // 16-byte words of a thread's step, the next in flight
+  const int s = blockIdx.x, t = threadIdx.x;
   const int64_t r = blockIdx.y;
+  const char* const row = static_cast<const char*>(row_at<FMT>(a, r));
+  const int b0 = s * a.slice_len;
+  const int b1 = b0 + a.slice_len < a.vocab ? b0 + a.slice_len : a.vocab;
+  // up to the first 16-byte boundary of the slice entry by entry, whole 16-byte words from there
+  const int lead = (int)((16 - ((uintptr_t)(row + (int64_t)b0 * EB) & 15)) & 15) / EB;
+  const int h0 = b0 + lead < b1 ? b0 + lead : b1;
+  const int words = b1 > h0 ? (b1 - h0) / PER : 0, tail = h0 + words * PER;
+  const char* const body = row + (int64_t)h0 * EB;
+  u32x4 next[kBatch];
+  auto load = [&](int w0) {
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int w = w0 + u * kThreads;
+      next[u] = ldg16(body + (int64_t)(w < words ? w : t) * 16);   // t < words
+    }
+  };
+  if (t < words) load(t);
   // the row's sequence: its temperature
   int lo = 0, hi = a.num_seqs - 1;
   while (lo < hi) {
@@ -155,134 +206,244 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerifyArgs a) {
   }
   const float temp = temperature_of(a, lo);
   const float k = rate_of(temp);
-  const char* const row = static_cast<const char*>(row_at<FMT>(a, r));
-  const int b0 = s * a.slice_len;
-  const int b1 = b0 + a.slice_len < a.vocab ? b0 + a.slice_len : a.vocab;
-  // the first 16-byte boundary of the slice, whole 16-byte words from there
-  const int lead = (int)((16 - ((uintptr_t)(row + (int64_t)b0 * EB) & 15)) & 15) / EB;
-  const int h0 = b0 + lead < b1 ? b0 + lead : b1;
-  const int words = (b1 - h0) / PER, tail = h0 + words * PER;
-  const char* const body = row + (int64_t)h0 * EB;
   float top = kNegInf, sum = 0.f;
-  int arg = 0x7fffffff;
-  auto one = [&](float v, int i) {
-    if (better(v, i, top, arg)) {
-      sum *= top == v ? 1.f : fast_exp2((top - v) * k);
-      top = v;
-      arg = i;
-    }
-    sum += term(v, top, k);
-  };
-  const int t = threadIdx.x;
-  if (t < h0 - b0) one(elem<FMT>(row, b0 + t), b0 + t);
-  for (int w0 = t; w0 < words; w0 += kBatch * kThreads) {
-    u32x4 p[kBatch];
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      const int w = w0 + u * kThreads;
-      p[u] = ldg16(body + (int64_t)(w < words ? w : w0) * 16);
-    }
-    float v[kBatch * PER];
-    float best = kNegInf;
-    int at = 0x7fffffff;
-    bool nan = false;
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      const int w = w0 + u * kThreads;
-      const bool in = w < words;
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        if constexpr (FMT == kFmtF32) {
-          v[4 * u + x] = in ? __uint_as_float(p[u][x]) : kNegInf;
-        } else {
-          using T = Elt<FMT == kFmtF16>;
-          v[8 * u + 2 * x] = in ? T::lo(p[u][x]) : kNegInf;
-          v[8 * u + 2 * x + 1] = in ? T::hi(p[u][x]) : kNegInf;
-        }
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < kBatch * PER; ++e) {
-      nan |= v[e] != v[e];
-      best = fmaxf(best, v[e]);
-    }
-    if (nan || best > top || arg == 0x7fffffff) {     // a new maximum: where it is
-      for (int u = kBatch - 1; u >= 0; --u)
-#pragma unroll
-        for (int x = PER - 1; x >= 0; --x) {
-          float y = 0.f;
-#pragma unroll
-          for (int z = 0; z < kBatch; ++z) y = z == u ? v[z * PER + x] : y;
-          const int i = h0 + (w0 + u * kThreads) * PER + x;
-          if (w0 + u * kThreads < words && (nan ? y != y : y == best)) at = i;
-        }
-      const float nv = nan ? __uint_as_float(0x7fc00000u) : best;
-      if (better(nv, at, top, arg)) {
-        sum *= top == nv ? 1.f : fast_exp2((top - nv) * k);
-        top = nv;
-        arg = at;
-      }
-    }
-    if (temp > 0.f) {
-      float part = 0.f;
-#pragma unroll
-      for (int e = 0; e < kBatch * PER; ++e) part += term(v[e], top, k);
-      sum += part;
-    }
-  }
-  for (int i = tail + t; i < b1; i += kThreads) one(elem<FMT>(row, i), i);
-  // the wave, then the workgroup
-  float wtop = top;
-  int warg = arg;
-  wave_best(wtop, warg);
-  // lanes with nothing hold top = -inf and sum = 0: their factor must not be NaN
-  sum = wave_sum(top == wtop ? sum : sum == 0.f ? 0.f : sum * fast_exp2((top - wtop) * k));
   __shared__ float sv[kThreads / 64], ss[kThreads / 64];
   __shared__ int si[kThreads / 64];
-  if ((t & 63) == 0) {
-    sv[t >> 6] = wtop;
-    si[t >> 6] = warg;
-    ss[t >> 6] = sum;
-  }
-  __syncthreads();
-  if (t == 0) {
-    for (int w = 1; w < kThreads / 64; ++w)
-      if (better(sv[w], si[w], wtop, warg)) {
-        wtop = sv[w];
-        warg = si[w];
+  bool point = !(temp > 0.f);
+  if (!point) {
+    // entries past the slice and lanes without any: -inf, whose term is 0
+    auto raise = [&](float best) {
+      if (best > top) {
+        sum *= fast_exp2((top - best) * k);      // exp2(-inf) = 0 the first time
+        top = best;
       }
-    float z = 0.f;
+    };
+    auto term = [&](float l) {
+      return fast_exp2((l - (top == kNegInf ? 0.f : top)) * k);
+    };
+    auto one = [&](float l) {
+      raise(l);
+      sum += term(l);
+    };
+    for (int w0 = t; w0 < words; w0 += kBatch * kThreads) {
+      u32x4 p[kBatch];
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) p[u] = next[u];
+      if (w0 + kBatch * kThreads < words) load(w0 + kBatch * kThreads);
+      float v[kBatch * PER], best = kNegInf;
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const bool in = w0 + u * kThreads < words;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          if constexpr (FMT == kFmtF32) {
+            v[4 * u + x] = in ? __uint_as_float(p[u][x]) : kNegInf;
+          } else {
+            using T = Elt<FMT == kFmtF16>;
+            v[8 * u + 2 * x] = in ? T::lo(p[u][x]) : kNegInf;
+            v[8 * u + 2 * x + 1] = in ? T::hi(p[u][x]) : kNegInf;
+          }
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < kBatch * PER; ++e) best = fmaxf(best, v[e]);
+      raise(best);
+      float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int e = 0; e < kBatch * PER; ++e) part[e & 3] += term(v[e]);
+      sum += (part[0] + part[1]) + (part[2] + part[3]);
+    }
+    if (t < h0 - b0) one(elem<FMT>(row, b0 + t));
+    for (int i = tail + t; i < b1; i += kThreads) one(elem<FMT>(row, i));
+    float wtop = top;
+    wtop = wave_max(wtop);
+    // (a lane with nothing: -inf and 0, whose factor must not be NaN)
+    sum = wave_sum(top == wtop || sum == 0.f ? sum : sum * fast_exp2((top - wtop) * k));
+    if ((t & 63) == 0) {
+      sv[t >> 6] = wtop;
+      ss[t >> 6] = sum;
+    }
+    __syncthreads();
+    top = fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3]));
+    sum = 0.f;
     for (int w = 0; w < kThreads / 64; ++w)
-      if (ss[w] != 0.f) z += sv[w] == wtop ? ss[w] : ss[w] * fast_exp2((sv[w] - wtop) * k);
+      sum += sv[w] == top || ss[w] == 0.f ? ss[w] : ss[w] * fast_exp2((sv[w] - top) * k);
+    point = sum != sum;
+    __syncthreads();
+  }
+  int arg = b0 < b1 ? b0 : 0x7fffffff;   // what a slice of nothing but -inf has
+  if (point) {
+    // The maximum, and of each thread the step it is in; then the first such entry there.
+    auto entry = [&](int u, int x) {
+      if constexpr (FMT == kFmtF32)
+        return __uint_as_float(next[u][x]);
+      else
+        return x & 1 ? Elt<FMT == kFmtF16>::hi(next[u][x >> 1])
+                     : Elt<FMT == kFmtF16>::lo(next[u][x >> 1]);
+    };
+    float edge = kNegInf;      // of the entries that are not in whole words
+    int edge_at = 0x7fffffff, in = -1;
+    bool nan = false;
+    top = kNegInf;
+    auto one = [&](int i) {
+      const float v = elem<FMT>(row, i);
+      nan |= v != v;
+      if (v > edge) {
+        edge = v;
+        edge_at = i;
+      }
+    };
+    if (t < h0 - b0) one(b0 + t);
+    for (int i = tail + t; i < b1; i += kThreads) one(i);
+    if (t < words) load(t);
+    for (int w0 = t; w0 < words; w0 += kBatch * kThreads) {
+      float best = kNegInf;       // words past the slice repeat the thread's first
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u)
+#pragma unroll
+        for (int x = 0; x < PER; ++x) {
+          nan |= entry(u, x) != entry(u, x);
+          best = fmaxf(best, entry(u, x));
+        }
+      if (w0 + kBatch * kThreads < words) load(w0 + kBatch * kThreads);
+      if (best > top) {
+        top = best;
+        in = w0;
+      }
+    }
+    const bool wnan = __builtin_amdgcn_ballot_w64(nan) != 0;
+    float wtop = fmaxf(top, edge);
+    wtop = wave_max(wtop);
+    if ((t & 63) == 0) sv[t >> 6] = wnan ? __uint_as_float(0x7fc00000u) : wtop;
+    __syncthreads();
+    wtop = fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3]));
+    if (sv[0] != sv[0] || sv[1] != sv[1] || sv[2] != sv[2] || sv[3] != sv[3])
+      wtop = __uint_as_float(0x7fc00000u);
+    int at = 0x7fffffff;
+    if (wtop != wtop) {           // the first NaN
+      for (int i = b0 + t; i < b1 && at == 0x7fffffff; i += kThreads) {
+        const float v = elem<FMT>(row, i);
+        at = v != v ? i : at;
+      }
+    } else if (wtop > kNegInf) {
+      if (edge == wtop) at = edge_at;
+      if (in >= 0 && top == wtop) {
+        load(in);
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u)
+#pragma unroll
+          for (int x = 0; x < PER; ++x) {
+            const int w = in + u * kThreads, i = h0 + w * PER + x;
+            if (w < words && entry(u, x) == wtop && i < at) at = i;
+          }
+      }
+    }
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) {
+      const int o = __shfl_xor(at, m, 64);
+      at = o < at ? o : at;
+    }
+    if ((t & 63) == 0) si[t >> 6] = at;
+    __syncthreads();
+    for (int w = 0; w < kThreads / 64; ++w) at = si[w] < at ? si[w] : at;
+    top = wtop;
+    if (wtop != wtop || wtop > kNegInf) arg = at;
+  }
+  if (t == 0) {
     const int64_t o = r * a.slices + s;
-    a.part_max[o] = wtop;
-    a.part_arg[o] = warg;
-    a.part_sum[o] = z;
+    a.part_max[o] = top;
+    a.part_arg[o] = arg;
+    a.part_sum[o] = sum;
   }
 }
 
-// A row's statistics from its slices, in every lane of the wave.
-__device__ __forceinline__ void row_stats(const VerifyArgs& a, int64_t r, int lane, float k,
-                                          float* top, int* arg, double* sum) {
+// Row r's statistics from its slices, in every lane of a group of `width` (a power of two, at
+// least the slices).
+__device__ __forceinline__ void row_stats(const VerifyArgs& a, int64_t r, int lane, int width,
+                                          float k, float* top, int* arg, double* sum) {
   float v = kNegInf, z = 0.f;
   int i = 0x7fffffff;
-  if (lane < a.slices) {
-    v = a.part_max[r * a.slices + lane];
-    i = a.part_arg[r * a.slices + lane];
-    z = a.part_sum[r * a.slices + lane];
+  const int s = lane & (width - 1);
+  if (s < a.slices) {
+    v = a.part_max[r * a.slices + s];
+    i = a.part_arg[r * a.slices + s];
+    z = a.part_sum[r * a.slices + s];
   }
   *top = v;
   *arg = i;
-  wave_best(*top, *arg);
-  *sum = wave_sum(z == 0.f ? 0.0 : v == *top ? (double)z : (double)z * exp2((double)(v - *top) * k));
+  for (int m = 1; m < width; m <<= 1) {
+    const float ov = __shfl_xor(*top, m, 64);
+    const int oi = __shfl_xor(*arg, m, 64);
+    if (better(ov, oi, *top, *arg)) {
+      *top = ov;
+      *arg = oi;
+    }
+  }
+  double x = z == 0.f ? 0.0 : v == *top ? (double)z : (double)z * fast_exp2((v - *top) * k);
+  for (int m = 1; m < width; m <<= 1) x += __shfl_xor(x, m, 64);
+  *sum = x;
 }
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) <= 3.402823466e38f; }
 
-// weight of an entry: exp((l - top) / T) in fp64
-__device__ __forceinline__ double weight(float l, float top, double inv_t) {
-  return l == kNegInf ? 0.0 : exp(((double)l - (double)top) * inv_t);
+// 2^(j / 64)
+__device__ const double kPowers[64] = {
+    0x1.0000000000000p+0, 0x1.02c9a3e778061p+0, 0x1.059b0d3158574p+0, 0x1.0874518759bc8p+0,
+    0x1.0b5586cf9890fp+0, 0x1.0e3ec32d3d1a2p+0, 0x1.11301d0125b51p+0, 0x1.1429aaea92de0p+0,
+    0x1.172b83c7d517bp+0, 0x1.1a35beb6fcb75p+0, 0x1.1d4873168b9aap+0, 0x1.2063b88628cd6p+0,
+    0x1.2387a6e756238p+0, 0x1.26b4565e27cddp+0, 0x1.29e9df51fdee1p+0, 0x1.2d285a6e4030bp+0,
+    0x1.306fe0a31b715p+0, 0x1.33c08b26416ffp+0, 0x1.371a7373aa9cbp+0, 0x1.3a7db34e59ff7p+0,
+    0x1.3dea64c123422p+0, 0x1.4160a21f72e2ap+0, 0x1.44e086061892dp+0, 0x1.486a2b5c13cd0p+0,
+    0x1.4bfdad5362a27p+0, 0x1.4f9b2769d2ca7p+0, 0x1.5342b569d4f82p+0, 0x1.56f4736b527dap+0,
+    0x1.5ab07dd485429p+0, 0x1.5e76f15ad2148p+0, 0x1.6247eb03a5585p+0, 0x1.6623882552225p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.6dfb23c651a2fp+0, 0x1.71f75e8ec5f74p+0, 0x1.75feb564267c9p+0,
+    0x1.7a11473eb0187p+0, 0x1.7e2f336cf4e62p+0, 0x1.82589994cce13p+0, 0x1.868d99b4492edp+0,
+    0x1.8ace5422aa0dbp+0, 0x1.8f1ae99157736p+0, 0x1.93737b0cdc5e5p+0, 0x1.97d829fde4e50p+0,
+    0x1.9c49182a3f090p+0, 0x1.a0c667b5de565p+0, 0x1.a5503b23e255dp+0, 0x1.a9e6b5579fdbfp+0,
+    0x1.ae89f995ad3adp+0, 0x1.b33a2b84f15fbp+0, 0x1.b7f76f2fb5e47p+0, 0x1.bcc1e904bc1d2p+0,
+    0x1.c199bdd85529cp+0, 0x1.c67f12e57d14bp+0, 0x1.cb720dcef9069p+0, 0x1.d072d4a07897cp+0,
+    0x1.d5818dcfba487p+0, 0x1.da9e603db3285p+0, 0x1.dfc97337b9b5fp+0, 0x1.e502ee78b3ff6p+0,
+    0x1.ea4afa2a490dap+0, 0x1.efa1bee615a27p+0, 0x1.f50765b6e4540p+0, 0x1.fa7c1819e90d8p+0,
+};
+
+// exp((l - top) / T) in fp64, to about 1e-13 of it, 0 below 2^-900: 2^(n / 64) from the table, and
+// e^r, |r| <= ln 2 / 128, by its series to r^4.  n is read from the low bits of a sum with
+// 1.5 * 2^52, and added to the product's exponent: fp64 conversions run at a quarter of the rate.
+struct Exp {
+  const double* table;     // kPowers in LDS
+  double rate;             // 64 / (T ln 2)
+  __device__ __forceinline__ double operator()(float l, float top) const {
+    const double z = ((double)l - (double)top) * rate;      // at most 0; -inf for a masked entry
+    const double shifted = z + 6755399441055744.0;
+    const int n = (int)(uint32_t)__builtin_bit_cast(uint64_t, shifted);
+    const double r = (z - (shifted - 6755399441055744.0)) * 0.01083042469624914545;  // ln 2 / 64
+    const double e =
+        fma(r, fma(r, fma(r, fma(r, 1.0 / 24, 1.0 / 6), 0.5), 1.0), 1.0) * table[n & 63];
+    const uint64_t w = __builtin_bit_cast(uint64_t, e) + ((uint64_t)(uint32_t)((n >> 6) << 20) << 32);
+    return z > -57600.0 ? __builtin_bit_cast(double, w) : 0.0;
+  }
+};
+// Every thread calls it; a barrier is due before the first use.
+__device__ __forceinline__ Exp make_exp(double* table, float temp) {
+  if (threadIdx.x < 64) table[threadIdx.x] = kPowers[threadIdx.x];
+  return Exp{table, 92.33248261893164817 / (double)temp};
 }
 __device__ __forceinline__ double positive(double x) { return x > 0.0 ? x : 0.0; }   // NaN: 0
+
+constexpr int kRun = kSumSlice / kThreads;     // entries of a thread in flight
+
+// Entry v0 + u * kThreads of a row for u < kRun, -inf past b1.
+template <int FMT>
+__device__ __forceinline__ void load_run(const void* row, int v0, int b1, float (&l)[kRun]) {
+  // loaded without a branch: the loads would wait for one another
+#pragma unroll
+  for (int u = 0; u < kRun; ++u) {
+    const int v = v0 + u * kThreads;
+    l[u] = elem<FMT>(row, v < b1 ? v : b1 - 1);
+  }
+#pragma unroll
+  for (int u = 0; u < kRun; ++u)
+    if (v0 + u * kThreads >= b1) l[u] = kNegInf;
+}
 
 // Workgroup (slice, sequence): the sequence's accepted drafts and chosen row, then the sum of its
 // slice of that row's weights.  Slice 0 writes what the later launches read.
@@ -294,31 +455,16 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs a) {
   const int n = seq_rows(a, i, &first);
   const float temp = temperature_of(a, i);
   const float k = rate_of(temp);
-  const double inv_t = temp > 0.f ? 1.0 / (double)temp : 0.0;
+  __shared__ double table[64];
   __shared__ int reject;
   __shared__ double part[kThreads / 64];
-  if (t == 0) reject = n - 1;
-  __syncthreads();
-  for (int j = wv; j < n - 1; j += kThreads / 64) {
-    const int64_t r = first + j;
-    float top;
-    int arg;
-    double sum;
-    row_stats(a, r, lane, k, &top, &arg, &sum);
-    if (lane == 0) {
-      const int64_t x = draft_at(a, r + 1);
-      double p = 0.0, q = 1.0;
-      if (x >= 0 && x < a.vocab) {
-        if (temp > 0.f && finite(top))
-          p = weight(elem<FMT>(row_at<FMT>(a, r), x), top, inv_t) / sum;
-        else
-          p = x == arg ? 1.0 : 0.0;
-        const int64_t d = r - i;
-        if (a.probs) q = d >= 0 && d < a.probs_rows ? a.probs[d * a.probs_stride + x] : 0.f;
-      }
-      if (!((double)a.uniforms[r] * q < p)) atomicMin(&reject, j);
-    }
-  }
+  __shared__ float tops[kAccept];
+  __shared__ int args[kAccept];
+  __shared__ double totals[kAccept];
+  const Exp ex = make_exp(table, temp);
+  int width = 1;                       // lanes that a row's slices take
+  while (width < a.slices) width <<= 1;
+  if (t == 0) reject = n;
   __syncthreads();
   if (n <= 0) {
     if (s == 0 && t == 0) {
@@ -327,43 +473,79 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs a) {
     }
     return;
   }
-  const int acc = reject;
+  // kAccept rows at a time: their statistics by waves, the drafts' own entries by threads.  The
+  // last row (or the first rejected) ends it, its statistics still there.
+  int acc = 0, j0 = 0;
+  for (;; j0 += kAccept) {
+    const int m = n - j0 < kAccept ? n - j0 : kAccept;
+    const int64_t r = first + j0 + t;
+    const bool judge = t < m && j0 + t < n - 1;
+    int64_t x = -1;
+    float u = 0.f, lx = kNegInf, q = 1.f;
+    if (judge) {
+      x = draft_at(a, r + 1);
+      u = a.uniforms[r];
+      if (x >= 0 && x < a.vocab) {
+        lx = elem<FMT>(row_at<FMT>(a, r), x);
+        const int64_t d = r - i;
+        if (a.probs) q = d >= 0 && d < a.probs_rows ? a.probs[d * a.probs_stride + x] : 0.f;
+      }
+    }
+    for (int j = t / width; j < m; j += kThreads / width) {
+      float top;
+      int arg;
+      double sum;
+      row_stats(a, first + j0 + j, lane, width, k, &top, &arg, &sum);
+      if ((lane & (width - 1)) == 0) {
+        tops[j] = top;
+        args[j] = arg;
+        totals[j] = sum;
+      }
+    }
+    __syncthreads();
+    if (t < m) {
+      bool ok = false;
+      if (judge && x >= 0 && x < a.vocab) {
+        const double uq = (double)u * (double)q;
+        ok = temp > 0.f && finite(tops[t]) ? uq * totals[t] < ex(lx, tops[t])
+                                           : uq < (x == args[t] ? 1.0 : 0.0);
+      }
+      if (!ok) atomicMin(&reject, j0 + t);     // the last row has nothing to accept
+    }
+    __syncthreads();
+    acc = reject;
+    if (acc < n) break;
+    __syncthreads();
+  }
   const int64_t r = first + acc;
-  float top;
-  int arg;
-  double fsum;
-  row_stats(a, r, lane, k, &top, &arg, &fsum);
   Info f;
   f.accepted = acc;
   f.row = r;
   f.draft_row = r - i;
-  f.top = top;
-  if (!(temp > 0.f) || !finite(top)) {
+  f.top = tops[acc - j0];
+  f.token = args[acc - j0];
+  if (!(temp > 0.f) || !finite(f.top)) {
     f.kind = kPoint;
-    f.token = arg;
   } else if (acc == n - 1) {
     f.kind = kAll;
-    f.token = arg;
+  } else if (a.probs) {
+    f.kind = f.draft_row >= 0 && f.draft_row < a.probs_rows ? kLeft : kAll;
   } else {
     const int64_t x = draft_at(a, r + 1);
-    f.kind = a.probs ? (f.draft_row >= 0 && f.draft_row < a.probs_rows ? kLeft : kAll) : kBut;
-    f.token = a.probs ? arg : x >= 0 && x < a.vocab ? (int)x : -1;
+    f.kind = kBut;
+    f.token = x >= 0 && x < a.vocab ? (int)x : -1;
   }
   if (s == 0 && t == 0) a.info[i] = f;
   if (f.kind == kPoint) return;
   const void* const row = row_at<FMT>(a, r);
   const int b0 = s * a.sum_len, b1 = b0 + a.sum_len < a.vocab ? b0 + a.sum_len : a.vocab;
   double z = 0.0;
-  for (int v0 = b0 + t; v0 < b1; v0 += 8 * kThreads) {
-    float l[8];
+  for (int v0 = b0 + t; v0 < b1; v0 += kRun * kThreads) {
+    float l[kRun];
+    load_run<FMT>(row, v0, b1, l);
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const int v = v0 + u * kThreads;
-      l[u] = v < b1 ? elem<FMT>(row, v) : kNegInf;
-    }
-#pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const double w = weight(l[u], top, inv_t);
+    for (int u = 0; u < kRun; ++u) {
+      const double w = ex(l[u], f.top);
       z += f.kind == kBut && v0 + u * kThreads == f.token ? 0.0 : w;
     }
   }
@@ -384,42 +566,49 @@ __global__ __launch_bounds__(kThreads) void verify_left_kernel(VerifyArgs a) {
   const int i = blockIdx.y, s = blockIdx.x, t = threadIdx.x, lane = t & 63;
   const Info f = a.info[i];
   if (f.kind != kLeft) return;
-  const double inv_t = 1.0 / (double)temperature_of(a, i);
-  const double total = slice_total(a.sums + (int64_t)i * a.sum_slices, a.sum_slices, lane);
+  __shared__ double table[64];
+  __shared__ double part[kThreads / 64];
+  const Exp ex = make_exp(table, temperature_of(a, i));
+  const double scale =
+      1.0 / slice_total(a.sums + (int64_t)i * a.sum_slices, a.sum_slices, lane);
+  __syncthreads();
   const void* const row = row_at<FMT>(a, f.row);
   const float* const q = a.probs + f.draft_row * a.probs_stride;
   const int b0 = s * a.sum_len, b1 = b0 + a.sum_len < a.vocab ? b0 + a.sum_len : a.vocab;
   double z = 0.0;
-  for (int v0 = b0 + t; v0 < b1; v0 += 8 * kThreads) {
-    float l[8], d[8];
+  for (int v0 = b0 + t; v0 < b1; v0 += kRun * kThreads) {
+    float l[kRun], d[kRun];
+    load_run<FMT>(row, v0, b1, l);
+    load_run<kFmtF32>(q, v0, b1, d);
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const int v = v0 + u * kThreads;
-      l[u] = v < b1 ? elem<FMT>(row, v) : kNegInf;
-      d[u] = v < b1 ? q[v] : 0.f;
-    }
-#pragma unroll
-    for (int u = 0; u < 8; ++u)
-      z += positive(weight(l[u], f.top, inv_t) / total - positive((double)d[u]));
+    for (int u = 0; u < kRun; ++u)
+      z += positive(ex(l[u], f.top) * scale - positive((double)d[u]));
   }
   z = wave_sum(z);
-  __shared__ double part[kThreads / 64];
   if (lane == 0) part[t >> 6] = z;
   __syncthreads();
   if (t == 0) a.left[(int64_t)i * a.sum_slices + s] = (part[0] + part[1]) + (part[2] + part[3]);
 }
 
-__device__ __forceinline__ double wave_prefix(double v, int lane) {   // inclusive
+// Inclusive prefix sum: over the 16 lanes of a row by shifts, then the rows before it.
+__device__ __forceinline__ double wave_prefix(double v, int lane) {
+  v += dpp<0x111>(v);           // row_shr:1, 0 from outside the row
+  v += dpp<0x112>(v);
+  v += dpp<0x114>(v);
+  v += dpp<0x118>(v);
+  double before = 0.0;
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const double o = __shfl_up(v, d, 64);
-    if (lane >= d) v += o;
+  for (int r = 0; r < 3; ++r) {
+    const uint64_t w = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)w, 16 * r + 15);
+    const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)(w >> 32), 16 * r + 15);
+    before += lane > 16 * r + 15 ? __builtin_bit_cast(double, (uint64_t)hi << 32 | lo) : 0.0;
   }
-  return v;
+  return v + before;
 }
 
-// Workgroup per sequence: its tokens.  The slice whose prefix passes the goal, then the thread
-// (each takes a run of the slice), then the entry.
+// Workgroup per sequence: its tokens.  The slice whose prefix passes the goal; its weights into
+// LDS; then the thread (each takes a run of the slice), then the entry.
 template <int FMT>
 __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a) {
   const int i = blockIdx.x, t = threadIdx.x, lane = t & 63, wv = t >> 6;
@@ -434,6 +623,15 @@ __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a) {
   if (f.kind == kPoint) {
     if (t == 0) put_token(a, to, f.token);
     return;
+  }
+  extern __shared__ double run[];      // the slice's weights
+  __shared__ double table[64];
+  __shared__ double wsum[kThreads / 64];
+  __shared__ int found, fallback;
+  const Exp ex = make_exp(table, temperature_of(a, i));
+  if (t == 0) {
+    found = 0x7fffffff;
+    fallback = -1;
   }
   const int ns = a.sum_slices;
   const double* const plain = a.sums + (int64_t)i * ns;
@@ -465,38 +663,42 @@ __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a) {
   const uint64_t some = __builtin_amdgcn_ballot_w64(x > 0.0);
   const int pick = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
   const double before = __shfl(upto - x, pick, 64);
-  const double inv_t = 1.0 / (double)temperature_of(a, i);
+  const double scale = 1.0 / whole;
   const void* const row = row_at<FMT>(a, f.row);
   const float* const q = left ? a.probs + f.draft_row * a.probs_stride : nullptr;
-  auto value = [&](int v) -> double {
-    const double w = weight(elem<FMT>(row, v), f.top, inv_t);
-    if (left) return positive(w / whole - positive((double)q[v]));
-    return f.kind == kBut && v == f.token ? 0.0 : w;
-  };
   const int b0 = pick * a.sum_len, b1 = b0 + a.sum_len < a.vocab ? b0 + a.sum_len : a.vocab;
+  __syncthreads();
+  for (int v0 = b0 + t; v0 < b1; v0 += kRun * kThreads) {
+    float l[kRun], d[kRun];
+    load_run<FMT>(row, v0, b1, l);
+    if (left) load_run<kFmtF32>(q, v0, b1, d);
+#pragma unroll
+    for (int e = 0; e < kRun; ++e) {
+      const int v = v0 + e * kThreads;
+      double w = ex(l[e], f.top);
+      if (left) w = positive(w * scale - positive((double)d[e]));
+      if (f.kind == kBut && v == f.token) w = 0.0;
+      if (v < b1) run[v - b0] = w;
+    }
+  }
+  __syncthreads();
   const int per = (b1 - b0 + kThreads - 1) / kThreads;
-  const int v0 = b0 + t * per < b1 ? b0 + t * per : b1, v1 = v0 + per < b1 ? v0 + per : b1;
+  const int v0 = t * per < b1 - b0 ? t * per : b1 - b0;
+  const int v1 = v0 + per < b1 - b0 ? v0 + per : b1 - b0;
   double mine = 0.0;
-  for (int v = v0; v < v1; ++v) mine += value(v);
+  for (int v = v0; v < v1; ++v) mine += run[v];
   // prefix over the threads
   const double incl = wave_prefix(mine, lane);
-  __shared__ double wsum[kThreads / 64];
-  __shared__ int found, fallback;
   if (lane == 63) wsum[wv] = incl;
-  if (t == 0) {
-    found = 0x7fffffff;
-    fallback = -1;
-  }
   __syncthreads();
   double c = before + (incl - mine);
   for (int w = 0; w < wv; ++w) c += wsum[w];
   int hit = 0x7fffffff, seen = -1;
   if (mine > 0.0)
     for (int v = v0; v < v1; ++v) {
-      const double x = value(v);
-      c += x;
-      if (x > 0.0) seen = v;
-      if (x > 0.0 && c > goal) {
+      c += run[v];
+      if (run[v] > 0.0) seen = v;
+      if (run[v] > 0.0 && c > goal) {
         hit = v;
         break;
       }
@@ -504,7 +706,8 @@ __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a) {
   if (hit != 0x7fffffff) atomicMin(&found, hit);
   if (seen >= 0) atomicMax(&fallback, seen);
   __syncthreads();
-  if (t == 0) put_token(a, to, found != 0x7fffffff ? found : fallback >= 0 ? fallback : 0);
+  if (t == 0)
+    put_token(a, to, b0 + (found != 0x7fffffff ? found : fallback >= 0 ? fallback : 0));
 }
 
 int slices_for(int64_t rows, int vocab, int least, int wgs) {
@@ -516,13 +719,18 @@ int slices_for(int64_t rows, int vocab, int least, int wgs) {
 size_t up(size_t n) { return (n + 255) / 256 * 256; }
 
 struct Sizes {
-  int slices, sum_slices;
+  int slices, sum_slices, sum_len;
   size_t stat, info, sums, total;    // bytes of a part; three stats, two sums
 };
 Sizes sizes_of(int64_t rows, int num_seqs, int vocab) {
   Sizes z;
   z.slices = slices_for(rows, vocab, kStatSlice, kStatWgs);
-  z.sum_slices = slices_for(num_seqs, vocab, kSumSlice, kSumWgs);
+  const int steps = (vocab + kSumSlice - 1) / kSumSlice;
+  int per = steps / slices_for(num_seqs, vocab, kSumSlice, kSumWgs);   // steps of a slice
+  if (per > kPickLen / kSumSlice) per = kPickLen / kSumSlice;
+  if (per < (steps + kMaxSlices - 1) / kMaxSlices) per = (steps + kMaxSlices - 1) / kMaxSlices;
+  z.sum_len = per * kSumSlice;
+  z.sum_slices = (steps + per - 1) / per;
   z.stat = up((size_t)rows * z.slices * 4);
   z.info = up((size_t)num_seqs * sizeof(Info));
   z.sums = up((size_t)num_seqs * z.sum_slices * 8);
@@ -545,7 +753,8 @@ int launch_verify(const VerifyArgs& a, hipStream_t s) {
     rc = check_launch();
     if (rc != NDL_OK) return rc;
   }
-  hipLaunchKernelGGL((verify_pick_kernel<FMT>), dim3((unsigned)a.num_seqs), wg, 0, s, a);
+  hipLaunchKernelGGL((verify_pick_kernel<FMT>), dim3((unsigned)a.num_seqs), wg,
+                     (size_t)a.sum_len * sizeof(double), s, a);
   return check_launch();
 }
 
@@ -576,7 +785,8 @@ extern "C" int ndl_verify_drafts(void* tokens, int32_t* accepted, const void* lo
   const int eb = dtype_bytes(dtype);
   if ((uintptr_t)logits % eb || (uintptr_t)draft_probs & 3u || (uintptr_t)uniforms & 3u)
     return NDL_ERR_INVALID_ARG;
-  if (num_rows > 65535 || num_seqs > 65535 || vocab > (1 << 28)) return NDL_ERR_UNSUPPORTED;
+  if (num_rows > 65535 || num_seqs > 65535 || vocab > kMaxVocab)
+    return NDL_ERR_UNSUPPORTED;
   const Sizes z = sizes_of(num_rows, num_seqs, vocab);
   if (!workspace || workspace_bytes < z.total || (uintptr_t)workspace & 255u)
     return NDL_ERR_WORKSPACE;
@@ -600,7 +810,7 @@ extern "C" int ndl_verify_drafts(void* tokens, int32_t* accepted, const void* lo
   a.slice_len = (vocab + z.slices - 1) / z.slices;
   a.slice_len = (a.slice_len + 7) / 8 * 8;
   a.sum_slices = z.sum_slices;
-  a.sum_len = (vocab + z.sum_slices - 1) / z.sum_slices;
+  a.sum_len = z.sum_len;
   char* w = (char*)workspace;
   a.part_max = (float*)w;
   a.part_arg = (int*)(w + z.stat);
