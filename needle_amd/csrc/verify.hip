@@ -35,6 +35,8 @@ constexpr int kMaxSlices = 64;       // a lane of a wave each
 constexpr int kPickLen = 6144;       // elements of a chosen row's slice at most: they fit the LDS
 constexpr int kMaxVocab = 1 << 18;
 static_assert(kMaxVocab <= kMaxSlices * kPickLen, "a slice's weights fit the LDS");
+constexpr int kPickThreads = 1024;   // of the last launch: one workgroup per sequence
+constexpr int kPickRun = kPickLen / kPickThreads;
 constexpr int kAccept = 64;          // rows judged at a time
 
 struct Info {            // of a sequence, written by `sums`
@@ -357,31 +359,41 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerifyArgs a) {
   }
 }
 
-// Row r's statistics from its slices, in every lane of a group of `width` (a power of two, at
-// least the slices).
-__device__ __forceinline__ void row_stats(const VerifyArgs& a, int64_t r, int lane, int width,
-                                          float k, float* top, int* arg, double* sum) {
-  float v = kNegInf, z = 0.f;
-  int i = 0x7fffffff;
-  const int s = lane & (width - 1);
-  if (s < a.slices) {
-    v = a.part_max[r * a.slices + s];
-    i = a.part_arg[r * a.slices + s];
-    z = a.part_sum[r * a.slices + s];
-  }
-  *top = v;
-  *arg = i;
+// A row's statistics from its slices: a lane's slice, then combined over a group of `width` lanes
+// (a power of two, at least the slices).
+struct RowStats {
+  float top = kNegInf;
+  int arg = 0x7fffffff;
+  double sum = 0.0;
+};
+struct RowPart {
+  float top = kNegInf, sum = 0.f;
+  int arg = 0x7fffffff;
+};
+__device__ __forceinline__ RowPart load_part(const VerifyArgs& a, int64_t r, int s) {
+  RowPart p;
+  const int64_t o = r * a.slices + (s < a.slices ? s : 0);
+  p.top = a.part_max[o];
+  p.arg = a.part_arg[o];
+  p.sum = a.part_sum[o];
+  if (s >= a.slices) p = RowPart{};
+  return p;
+}
+__device__ __forceinline__ RowStats row_stats(const RowPart& p, int width, float k) {
+  RowStats f{p.top, p.arg, 0.0};
   for (int m = 1; m < width; m <<= 1) {
-    const float ov = __shfl_xor(*top, m, 64);
-    const int oi = __shfl_xor(*arg, m, 64);
-    if (better(ov, oi, *top, *arg)) {
-      *top = ov;
-      *arg = oi;
+    const float ov = __shfl_xor(f.top, m, 64);
+    const int oi = __shfl_xor(f.arg, m, 64);
+    if (better(ov, oi, f.top, f.arg)) {
+      f.top = ov;
+      f.arg = oi;
     }
   }
-  double x = z == 0.f ? 0.0 : v == *top ? (double)z : (double)z * fast_exp2((v - *top) * k);
-  for (int m = 1; m < width; m <<= 1) x += __shfl_xor(x, m, 64);
-  *sum = x;
+  f.sum = p.sum == 0.f ? 0.0
+          : p.top == f.top ? (double)p.sum
+                           : (double)p.sum * fast_exp2((p.top - f.top) * k);
+  for (int m = 1; m < width; m <<= 1) f.sum += __shfl_xor(f.sum, m, 64);
+  return f;
 }
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) <= 3.402823466e38f; }
 
@@ -431,18 +443,18 @@ __device__ __forceinline__ double positive(double x) { return x > 0.0 ? x : 0.0;
 
 constexpr int kRun = kSumSlice / kThreads;     // entries of a thread in flight
 
-// Entry v0 + u * kThreads of a row for u < kRun, -inf past b1.
-template <int FMT>
-__device__ __forceinline__ void load_run(const void* row, int v0, int b1, float (&l)[kRun]) {
+// Entry v0 + u * T of a row for u < RUN, -inf past b1.
+template <int FMT, int T = kThreads, int RUN = kRun>
+__device__ __forceinline__ void load_run(const void* row, int v0, int b1, float (&l)[RUN]) {
   // loaded without a branch: the loads would wait for one another
 #pragma unroll
-  for (int u = 0; u < kRun; ++u) {
-    const int v = v0 + u * kThreads;
+  for (int u = 0; u < RUN; ++u) {
+    const int v = v0 + u * T;
     l[u] = elem<FMT>(row, v < b1 ? v : b1 - 1);
   }
 #pragma unroll
-  for (int u = 0; u < kRun; ++u)
-    if (v0 + u * kThreads >= b1) l[u] = kNegInf;
+  for (int u = 0; u < RUN; ++u)
+    if (v0 + u * T >= b1) l[u] = kNegInf;
 }
 
 // Workgroup (slice, sequence): the sequence's accepted drafts and chosen row, then the sum of its
@@ -457,14 +469,13 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs a) {
   const float k = rate_of(temp);
   __shared__ double table[64];
   __shared__ int reject;
-  __shared__ double part[kThreads / 64];
+  __shared__ double sums[kThreads / 64];
   __shared__ float tops[kAccept];
   __shared__ int args[kAccept];
   __shared__ double totals[kAccept];
   const Exp ex = make_exp(table, temp);
   int width = 1;                       // lanes that a row's slices take
   while (width < a.slices) width <<= 1;
-  if (t == 0) reject = n;
   __syncthreads();
   if (n <= 0) {
     if (s == 0 && t == 0) {
@@ -480,6 +491,9 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs a) {
     const int m = n - j0 < kAccept ? n - j0 : kAccept;
     const int64_t r = first + j0 + t;
     const bool judge = t < m && j0 + t < n - 1;
+    // the first rows' parts go out before the drafts' own entries, which take two round trips
+    const int g = t / width, gs = kThreads / width;
+    RowPart part = load_part(a, first + j0 + (g < m ? g : 0), t & (width - 1));
     int64_t x = -1;
     float u = 0.f, lx = kNegInf, q = 1.f;
     if (judge) {
@@ -491,15 +505,13 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs a) {
         if (a.probs) q = d >= 0 && d < a.probs_rows ? a.probs[d * a.probs_stride + x] : 0.f;
       }
     }
-    for (int j = t / width; j < m; j += kThreads / width) {
-      float top;
-      int arg;
-      double sum;
-      row_stats(a, first + j0 + j, lane, width, k, &top, &arg, &sum);
-      if ((lane & (width - 1)) == 0) {
-        tops[j] = top;
-        args[j] = arg;
-        totals[j] = sum;
+    for (int j = g; j < m; j += gs) {
+      if (j != g) part = load_part(a, first + j0 + j, t & (width - 1));
+      const RowStats f = row_stats(part, width, k);
+      if ((t & (width - 1)) == 0) {
+        tops[j] = f.top;
+        args[j] = f.arg;
+        totals[j] = f.sum;
       }
     }
     __syncthreads();
@@ -510,7 +522,9 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs a) {
         ok = temp > 0.f && finite(tops[t]) ? uq * totals[t] < ex(lx, tops[t])
                                            : uq < (x == args[t] ? 1.0 : 0.0);
       }
-      if (!ok) atomicMin(&reject, j0 + t);     // the last row has nothing to accept
+      // the first row that is not accepted (the last has nothing to accept): t < m <= 64
+      const uint64_t no = __builtin_amdgcn_ballot_w64(!ok);
+      if (t == 0) reject = no ? j0 + __builtin_ctzll(no) : n;
     }
     __syncthreads();
     acc = reject;
@@ -550,9 +564,9 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs a) {
     }
   }
   z = wave_sum(z);
-  if (lane == 0) part[wv] = z;
+  if (lane == 0) sums[wv] = z;
   __syncthreads();
-  if (t == 0) a.sums[(int64_t)i * a.sum_slices + s] = (part[0] + part[1]) + (part[2] + part[3]);
+  if (t == 0) a.sums[(int64_t)i * a.sum_slices + s] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
 }
 
 // The slices' sums added in every lane (at most 64).
@@ -610,13 +624,16 @@ __device__ __forceinline__ double wave_prefix(double v, int lane) {
 // Workgroup per sequence: its tokens.  The slice whose prefix passes the goal; its weights into
 // LDS; then the thread (each takes a run of the slice), then the entry.
 template <int FMT>
-__global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a) {
+__global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(VerifyArgs a) {
   const int i = blockIdx.x, t = threadIdx.x, lane = t & 63, wv = t >> 6;
   int64_t first;
   const int n = seq_rows(a, i, &first);
+  const int ns = a.sum_slices;
+  const double plain = lane < ns ? a.sums[(int64_t)i * ns + lane] : 0.0;
+  const double less = a.probs && lane < ns ? a.left[(int64_t)i * ns + lane] : 0.0;
   if (n <= 0) return;
   const Info f = a.info[i];
-  for (int j = t; j < n; j += kThreads)
+  for (int j = t; j < n; j += kPickThreads)
     if (j != f.accepted) put_token(a, first + j, j < f.accepted ? draft_at(a, first + j + 1) : -1);
   if (t == 0) a.accepted[i] = f.accepted;
   const int64_t to = first + f.accepted;
@@ -626,28 +643,13 @@ __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a) {
   }
   extern __shared__ double run[];      // the slice's weights
   __shared__ double table[64];
-  __shared__ double wsum[kThreads / 64];
-  __shared__ int found, fallback;
+  __shared__ double wsum[kPickThreads / 64];
+  __shared__ int cross[kPickThreads / 64], last[kPickThreads / 64];
   const Exp ex = make_exp(table, temperature_of(a, i));
-  if (t == 0) {
-    found = 0x7fffffff;
-    fallback = -1;
-  }
-  const int ns = a.sum_slices;
-  const double* const plain = a.sums + (int64_t)i * ns;
-  const double whole = slice_total(plain, ns, lane);
-  bool left = f.kind == kLeft;
-  const double* sums = plain;
-  double total = whole;
-  if (left) {
-    const double rest = slice_total(a.left + (int64_t)i * ns, ns, lane);
-    if (rest > 0.0) {
-      sums = a.left + (int64_t)i * ns;
-      total = rest;
-    } else {
-      left = false;     // q covers p everywhere: p itself
-    }
-  }
+  const double whole = wave_sum(plain);
+  const double rest = f.kind == kLeft ? wave_sum(less) : 0.0;
+  const bool left = rest > 0.0;        // else q covers p everywhere: p itself
+  const double total = left ? rest : whole;
   if (!(total > 0.0)) {   // nothing but the rejected draft has weight
     if (t == 0) put_token(a, to, f.token < 0 ? 0 : f.token);
     return;
@@ -657,7 +659,7 @@ __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a) {
   const double goal = u * total;
   // every wave finds the slice: the first whose prefix of the sums passes the goal, or, by the
   // roundings of the total, the last with weight
-  const double x = lane < ns ? sums[lane] : 0.0;
+  const double x = left ? less : plain;
   const double upto = wave_prefix(x, lane);
   const uint64_t past = __builtin_amdgcn_ballot_w64(x > 0.0 && upto > goal);
   const uint64_t some = __builtin_amdgcn_ballot_w64(x > 0.0);
@@ -668,13 +670,13 @@ __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a) {
   const float* const q = left ? a.probs + f.draft_row * a.probs_stride : nullptr;
   const int b0 = pick * a.sum_len, b1 = b0 + a.sum_len < a.vocab ? b0 + a.sum_len : a.vocab;
   __syncthreads();
-  for (int v0 = b0 + t; v0 < b1; v0 += kRun * kThreads) {
-    float l[kRun], d[kRun];
-    load_run<FMT>(row, v0, b1, l);
-    if (left) load_run<kFmtF32>(q, v0, b1, d);
+  for (int v0 = b0 + t; v0 < b1; v0 += kPickRun * kPickThreads) {
+    float l[kPickRun], d[kPickRun];
+    load_run<FMT, kPickThreads, kPickRun>(row, v0, b1, l);
+    if (left) load_run<kFmtF32, kPickThreads, kPickRun>(q, v0, b1, d);
 #pragma unroll
-    for (int e = 0; e < kRun; ++e) {
-      const int v = v0 + e * kThreads;
+    for (int e = 0; e < kPickRun; ++e) {
+      const int v = v0 + e * kPickThreads;
       double w = ex(l[e], f.top);
       if (left) w = positive(w * scale - positive((double)d[e]));
       if (f.kind == kBut && v == f.token) w = 0.0;
@@ -682,7 +684,7 @@ __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a) {
     }
   }
   __syncthreads();
-  const int per = (b1 - b0 + kThreads - 1) / kThreads;
+  const int per = (b1 - b0 + kPickThreads - 1) / kPickThreads;
   const int v0 = t * per < b1 - b0 ? t * per : b1 - b0;
   const int v1 = v0 + per < b1 - b0 ? v0 + per : b1 - b0;
   double mine = 0.0;
@@ -692,22 +694,33 @@ __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a) {
   if (lane == 63) wsum[wv] = incl;
   __syncthreads();
   double c = before + (incl - mine);
-  for (int w = 0; w < wv; ++w) c += wsum[w];
-  int hit = 0x7fffffff, seen = -1;
-  if (mine > 0.0)
-    for (int v = v0; v < v1; ++v) {
-      c += run[v];
-      if (run[v] > 0.0) seen = v;
-      if (run[v] > 0.0 && c > goal) {
-        hit = v;
-        break;
-      }
-    }
-  if (hit != 0x7fffffff) atomicMin(&found, hit);
-  if (seen >= 0) atomicMax(&fallback, seen);
+#pragma unroll
+  for (int w = 0; w < kPickThreads / 64; ++w) c += w < wv ? wsum[w] : 0.0;
+  // the first thread whose run passes the goal, and the last with weight: one of each wave's
+  // lanes, then one of the waves (same-address LDS atomics take a cycle or more per lane)
+  const uint64_t over = __builtin_amdgcn_ballot_w64(mine > 0.0 && c + mine > goal);
+  const uint64_t any = __builtin_amdgcn_ballot_w64(mine > 0.0);
+  if (lane == 0) {
+    cross[wv] = over ? 64 * wv + __builtin_ctzll(over) : -1;
+    last[wv] = any ? 64 * wv + 63 - __builtin_clzll(any) : -1;
+  }
   __syncthreads();
-  if (t == 0)
-    put_token(a, to, b0 + (found != 0x7fffffff ? found : fallback >= 0 ? fallback : 0));
+  int who = -1, end = -1;
+#pragma unroll
+  for (int w = 0; w < kPickThreads / 64; ++w) {
+    who = who < 0 ? cross[w] : who;
+    end = last[w] >= 0 ? last[w] : end;
+  }
+  if (t != (who >= 0 ? who : end)) return;
+  int token = v0;
+  for (int v = v0; v < v1; ++v) {
+    c += run[v];
+    if (run[v] > 0.0) {
+      token = v;
+      if (c > goal) break;
+    }
+  }
+  put_token(a, to, b0 + token);
 }
 
 int slices_for(int64_t rows, int vocab, int least, int wgs) {
@@ -753,7 +766,7 @@ int launch_verify(const VerifyArgs& a, hipStream_t s) {
     rc = check_launch();
     if (rc != NDL_OK) return rc;
   }
-  hipLaunchKernelGGL((verify_pick_kernel<FMT>), dim3((unsigned)a.num_seqs), wg,
+  hipLaunchKernelGGL((verify_pick_kernel<FMT>), dim3((unsigned)a.num_seqs), dim3(kPickThreads),
                      (size_t)a.sum_len * sizeof(double), s, a);
   return check_launch();
 }
