@@ -549,16 +549,19 @@ int ndl_kv_read_fp8(void* k_out, void* v_out, const void* codes, const void* sca
  * chunk's own among them: append first.  out [num_tokens][num_heads][head_dim]; q rows of
  * q_tok_stride (a multiple of 8); groups of 1 to 16 query heads per kv head.  fp32 scores, softmax
  * and sums; probabilities rounded to the 16-bit format for the matrix cores.  Nothing to attend
- * (a negative context, invalid block ids only): zeros.
+ * (a negative context_lens[i], invalid block ids only): zeros.  A NaN in the pool reaches the
+ * tokens that attend it and no others.
  *
- * max_seqlen bounds the tokens of a sequence (those past it are not computed); max_keys bounds
- * the keys of a sequence and only chooses how the work is split.  The workspace
- * (ndl_fp8_attention_workspace_bytes of the same sizes, on the same device; 0: none) is 256-byte
- * aligned and belongs to one call at a time.
+ * max_seqlen bounds the tokens of a sequence (those past it are not computed) and max_keys its
+ * keys (context_lens[i] + tokens, at most max_blocks_per_seq * block_size; long chunks attend none
+ * past it): they choose how the work is split.  Chunks of 256 rows (max_seqlen times the group)
+ * and more unpack their keys into a 16-bit pool in the workspace first.  The workspace
+ * (ndl_fp8_attention_workspace_bytes of the same sizes, max_keys cut to the table's, on the same
+ * device; 0: none) is 256-byte aligned and belongs to one call at a time.
  */
-size_t ndl_fp8_attention_workspace_bytes(int num_seqs, int max_seqlen, int64_t max_keys,
-                                         int num_heads, int num_kv_heads, int head_dim,
-                                         int block_size);
+size_t ndl_fp8_attention_workspace_bytes(int num_seqs, int64_t num_tokens, int max_seqlen,
+                                         int64_t max_keys, int num_heads, int num_kv_heads,
+                                         int head_dim, int block_size);
 int ndl_fp8_attention(void* out, const void* q, int64_t q_tok_stride, const void* codes,
                       const void* scales, int64_t num_blocks, const int32_t* block_table,
                       int64_t bt_row_stride, int max_blocks_per_seq, const int32_t* cu_seqlens,

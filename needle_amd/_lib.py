@@ -198,7 +198,7 @@ _SIGNATURES = {
         _c_p, _c_i64, _c_i32,                           # block_table, row stride, W
         _c_p, _c_p, _c_i32, _c_i64, _c_p,               # first, cu, B, T, stream
     ]),
-    "ndl_fp8_attention_workspace_bytes": (_c_sz, [_c_i32, _c_i32, _c_i64] + [_c_i32] * 4),
+    "ndl_fp8_attention_workspace_bytes": (_c_sz, [_c_i32, _c_i64, _c_i32, _c_i64] + [_c_i32] * 4),
     "ndl_fp8_attention": (_c_i32, [
         _c_p, _c_p, _c_i64,                             # out, q, q stride
         _c_p, _c_p, _c_i64,                             # codes, scales, NB

@@ -24,6 +24,9 @@
 //   * Softmax in fp32 with exp2, scale * log2(e) folded.  The running maximum is raised (and the
 //     sums rescaled) only when a tile exceeds it by 8, so probabilities stay below 256.
 //     P is rounded to the 16-bit format for the matrix cores; its sum is taken before that.
+//   * Long chunks (kUnpackRows columns and more) are bound by the products, not by the codes: their
+//     keys are unpacked once into a 16-bit pool in the workspace, exactly, and attended by
+//     varlen_prefill.hip's kernels (see launch_unpacked).
 //   * Split.  Either a workgroup per (kv head, row block), or, where those would leave the GPU
 //     idle or unevenly loaded, all row blocks' tiles of a kv head laid end to end and cut into
 //     equal shares, one per resident workgroup; what a share holds of a row block goes to a
@@ -76,7 +79,7 @@ struct Item {
   int64_t cap;                  // keys a table row holds
   __device__ __forceinline__ int64_t keys() const {     // of its last token
     const int64_t k = pos + n;
-    return n <= 0 || k <= 0 ? 0 : k < cap ? k : cap;
+    return n <= 0 || pos < 0 ? 0 : k < cap ? k : cap;
   }
   __device__ __forceinline__ int tiles() const { return (int)((keys() + kTile - 1) / kTile); }
 };
@@ -93,7 +96,8 @@ __device__ __forceinline__ Item item_of(const ChunkArgs& a, int64_t e) {
   }
   it.tok0 = first + j0;
   it.n = (int)(count - j0 < a.toks ? count - j0 : a.toks);
-  it.pos = (int64_t)a.context_lens[it.seq] + j0;
+  const int64_t ctx = a.context_lens[it.seq];
+  it.pos = ctx < 0 ? -1 : ctx + j0;      // a negative context: nothing is attended
   it.cap = (int64_t)a.max_blocks << (4 + a.tile_shift);
   return it;
 }
@@ -673,6 +677,225 @@ __global__ __launch_bounds__(256) void chunk_merge_kernel(ChunkArgs a) {
   store(o);
 }
 
+// ---------------------------------------------------------------- long chunks
+
+struct UnpackArgs {
+  u16* pool;                    // [2][num_seqs * cols][Hkv][bs][D]
+  int32_t* table;               // [num_seqs][cols + 1], the last one invalid: keys past the
+                                // bound, which the prefill's column clamp leads there
+  int32_t* lens;                // [num_seqs]: context_lens, 0 for a negative one
+  int cols;
+  const uint8_t* codes;
+  const uint8_t* scales;
+  int64_t plane_rows, pool_rows;   // rows of a plane of the codes and of the 16-bit pool
+  int64_t num_blocks;
+  int num_kv_heads, num_heads, group;
+  const int32_t* block_table;
+  int64_t bt_row_stride;
+  int tile_shift;
+  const int32_t* cu_seqlens;
+  const int32_t* context_lens;
+  int64_t num_tokens;
+  u16* out;
+};
+struct Chunk {
+  int64_t tok0, pos, keys;
+  int n;
+};
+__device__ __forceinline__ Chunk chunk_of_seq(const UnpackArgs& a, int seq) {
+  Chunk c;
+  c.tok0 = a.cu_seqlens[seq];
+  const int64_t n = a.cu_seqlens[seq + 1] - c.tok0;
+  c.n = c.tok0 < 0 || n <= 0 || c.tok0 + n > a.num_tokens ? 0 : (int)n;
+  c.pos = a.context_lens[seq];
+  const int64_t cap = (int64_t)a.cols << (4 + a.tile_shift), k = c.pos + c.n;
+  c.keys = c.n == 0 || c.pos < 0 ? 0 : k < cap ? k : cap;
+  return c;
+}
+
+// The attended 16-token tiles of sequence blockIdx.y into its blocks of the 16-bit pool, a wave
+// per (tile, plane, kv head), heads next to each other as they lie in a block.  A NaN among the
+// chunk's own values becomes 0 here and reaches the tokens that attend it in chunk_nan_kernel:
+// the causal mask's 0 * NaN would bring it to those before it too.
+template <int D, bool F16>
+__global__ __launch_bounds__(256) void chunk_unpack_kernel(UnpackArgs a) {
+  constexpr int CPR = D / 16, RPL = 64 / CPR;    // lanes per row, rows per load
+  const int lane = threadIdx.x & 63, seq = blockIdx.y, Hkv = a.num_kv_heads;
+  const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const Chunk ch = chunk_of_seq(a, seq);
+  const int bshift = 4 + a.tile_shift;
+  const uint32_t tmask = (1u << a.tile_shift) - 1;
+  // a negative context attends nothing: its blocks are all invalid
+  const int64_t keys = ch.pos < 0 ? ch.n : ch.keys;
+  const int64_t tiles = (keys + 15) >> 4, items = tiles * 2 * Hkv;
+  int32_t* const row = a.table + (int64_t)seq * (a.cols + 1);
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    a.lens[seq] = ch.pos < 0 ? 0 : (int32_t)ch.pos;
+    row[a.cols] = -1;
+  }
+  const int r = lane / CPR;
+  for (int64_t item = (int64_t)blockIdx.x * 4 + wv; item < items; item += (int64_t)gridDim.x * 4) {
+    const int64_t tile = item / (2 * Hkv);
+    const int ph = (int)(item - tile * 2 * Hkv), plane = ph >= Hkv, head = ph - plane * Hkv;
+    const int col = (int)(tile >> a.tile_shift);
+    if (col >= a.cols) break;
+    const int b = a.block_table[(int64_t)seq * a.bt_row_stride + col];
+    const bool ok = b >= 0 && b < a.num_blocks && ch.pos >= 0;
+    const int64_t in_block = (int64_t)((uint32_t)tile & tmask) << 4;
+    const int64_t block = (int64_t)seq * a.cols + col;
+    if (ph == 0 && in_block == 0 && lane == 0) row[col] = ok ? (int)block : -1;
+    if (!ok) continue;
+    const int64_t from = (plane ? a.plane_rows : 0) + (((int64_t)b * Hkv + head) << bshift) + in_block;
+    u16* const dst = a.pool + ((plane ? a.pool_rows : 0) + ((block * Hkv + head) << bshift) +
+                               in_block) * D + lane * 16;
+    u32x4 c[16 / RPL];
+    float scale[16 / RPL];
+#pragma unroll
+    for (int x = 0; x < 16 / RPL; ++x) {
+      c[x] = ldg16(a.codes + from * D + x * 1024 + lane * 16);
+      scale[x] = __uint_as_float((uint32_t)a.scales[from + x * RPL + r] << 23);
+    }
+#pragma unroll
+    for (int x = 0; x < 16 / RPL; ++x) {
+      if (plane && 16 * tile + x * RPL + r >= ch.pos)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c[x][i] &= ~nan_bytes(c[x][i]);
+      u32x4 o[2];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        o[i >> 1][2 * (i & 1)] = value2<F16, false>(c[x][i], scale[x]);
+        o[i >> 1][2 * (i & 1) + 1] = value2<F16, true>(c[x][i], scale[x]);
+      }
+      st16(dst + x * RPL * D, o[0]);
+      st16(dst + x * RPL * D + 8, o[1]);
+    }
+  }
+}
+
+// A wave per (16 tokens of a chunk, kv head) of sequence blockIdx.y: where one of their values is
+// a NaN code, the output of that head_dim index becomes NaN from its token on.
+template <int D>
+__global__ __launch_bounds__(256) void chunk_nan_kernel(UnpackArgs a) {
+  constexpr int PER = D / 64;
+  const int lane = threadIdx.x & 63, seq = blockIdx.y, Hkv = a.num_kv_heads;
+  const int64_t w =
+      (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int head = (int)(w % Hkv);
+  const int64_t j0 = w / Hkv * 16;
+  const Chunk ch = chunk_of_seq(a, seq);
+  if (j0 >= ch.n) return;
+  const int bshift = 4 + a.tile_shift;
+  int code[16][PER];
+#pragma unroll
+  for (int x = 0; x < 16; ++x) {
+    const int64_t p = ch.pos + j0 + x;
+    bool in = j0 + x < ch.n && p >= 0 && p < ch.keys;
+    const int b = in ? a.block_table[(int64_t)seq * a.bt_row_stride + (p >> bshift)] : -1;
+    in = in && b >= 0 && b < a.num_blocks;
+    const int64_t row = in ? a.plane_rows + (((int64_t)b * Hkv + head) << bshift) +
+                                 (p & ((1 << bshift) - 1))
+                           : 0;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) code[x][e] = in ? a.codes[row * D + lane * PER + e] : 0;
+  }
+  int first[PER];
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    first[e] = 16;
+#pragma unroll
+    for (int x = 15; x >= 0; --x)
+      if ((code[x][e] & 0x7f) == 0x7f) first[e] = x;
+  }
+  bool any = false;
+#pragma unroll
+  for (int e = 0; e < PER; ++e) any |= first[e] < 16;
+  if (!__builtin_amdgcn_ballot_w64(any)) return;
+  for (int64_t j = j0; j < ch.n; ++j)
+    for (int g = 0; g < a.group; ++g)
+#pragma unroll
+      for (int e = 0; e < PER; ++e)
+        if (first[e] < 16 && j0 + first[e] <= j)   // bf16 and fp16: all bits but the sign
+          a.out[((ch.tok0 + j) * a.num_heads + head * a.group + g) * (int64_t)D + lane * PER + e] =
+              0x7fffu;
+}
+
+// Columns from which a row's codes are used often enough that unpacking them first is faster: us,
+// here / unpacked
+constexpr int64_t kUnpackRows = 256;
+constexpr int64_t kUnpackBytes = (int64_t)16 << 30;   // of the 16-bit pool
+
+struct Unpacked {
+  int cols;
+  int64_t blocks;
+  size_t table_bytes, lens_bytes, pool_bytes, prefill_bytes;
+  size_t total() const { return table_bytes + lens_bytes + pool_bytes + prefill_bytes; }
+};
+// Whether a call takes this path, and its workspace.
+bool unpacked_plan(int64_t num_seqs, int64_t num_tokens, int max_seqlen, int64_t max_keys,
+                   int num_heads, int num_kv_heads, int head_dim, int block_size, Unpacked* u) {
+  if ((int64_t)max_seqlen * (num_heads / num_kv_heads) < kUnpackRows || num_seqs > 65535)
+    return false;
+  const int64_t cols = (max_keys + block_size - 1) / block_size;
+  u->blocks = num_seqs * cols;
+  const int64_t bytes = u->blocks * block_size * num_kv_heads * head_dim * 4;
+  if (cols >= 0x7fffffff / block_size || u->blocks > 0x7fffffff || bytes > kUnpackBytes)
+    return false;
+  u->cols = (int)cols;
+  u->table_bytes = ((size_t)(u->blocks + num_seqs) * 4 + 255) / 256 * 256;
+  u->lens_bytes = ((size_t)num_seqs * 4 + 255) / 256 * 256;
+  u->pool_bytes = ((size_t)bytes + 255) / 256 * 256;
+  u->prefill_bytes =
+      ndl_varlen_prefill_workspace_bytes((int)num_seqs, num_tokens, max_seqlen, u->cols + 1,
+                                         num_heads, num_kv_heads, head_dim, block_size, NDL_DTYPE_BF16);
+  return true;
+}
+
+template <int D, bool F16>
+int launch_unpacked(const ChunkArgs& c, const Unpacked& u, int max_seqlen, int64_t max_keys,
+                    int block_size, float scale, void* workspace, hipStream_t s) {
+  UnpackArgs a{};
+  a.table = (int32_t*)workspace;
+  a.lens = (int32_t*)((char*)workspace + u.table_bytes);
+  a.pool = (u16*)((char*)workspace + u.table_bytes + u.lens_bytes);
+  a.cols = u.cols;
+  a.codes = c.codes;
+  a.scales = c.scales;
+  a.plane_rows = c.plane_rows;
+  a.pool_rows = u.blocks * c.num_kv_heads * (int64_t)block_size;
+  a.num_blocks = c.num_blocks;
+  a.num_kv_heads = c.num_kv_heads;
+  a.num_heads = c.num_heads;
+  a.group = c.group;
+  a.block_table = c.block_table;
+  a.bt_row_stride = c.bt_row_stride;
+  a.tile_shift = c.tile_shift;
+  a.cu_seqlens = c.cu_seqlens;
+  a.context_lens = c.context_lens;
+  a.num_tokens = c.num_tokens;
+  a.out = c.out;
+  // workgroups of a sequence: 2,048 over all sequences, no more than its items can use
+  const int64_t items = (max_keys + 15) / 16 * 2 * c.num_kv_heads;
+  int64_t wgs = (2048 + c.num_seqs - 1) / c.num_seqs;
+  if (wgs > (items + 3) / 4) wgs = (items + 3) / 4;
+  hipLaunchKernelGGL((chunk_unpack_kernel<D, F16>), dim3((unsigned)wgs, (unsigned)c.num_seqs),
+                     dim3(256), 0, s, a);
+  int rc = check_launch();
+  if (rc != NDL_OK) return rc;
+  // (the prefill sizes its split by the table, in the call as in the workspace query)
+  const int64_t cached = (int64_t)(u.cols + 1) * block_size;
+  void* const ws = u.prefill_bytes ? (char*)workspace + u.total() - u.prefill_bytes : nullptr;
+  rc = ndl_varlen_prefill_split(c.out, c.q, c.q_stride, nullptr, nullptr, 0, a.pool, u.blocks,
+                                a.table, u.cols + 1, u.cols + 1, c.cu_seqlens, a.lens, c.num_seqs,
+                                c.num_tokens, max_seqlen, (int)cached, c.num_heads,
+                                c.num_kv_heads, D, block_size, F16 ? NDL_DTYPE_F16 : NDL_DTYPE_BF16,
+                                scale, ws, u.prefill_bytes, s);
+  if (rc != NDL_OK) return rc;
+  const int64_t scan = ((int64_t)(max_seqlen + 15) / 16 * c.num_kv_heads + 3) / 4;
+  hipLaunchKernelGGL((chunk_nan_kernel<D>), dim3((unsigned)scan, (unsigned)c.num_seqs), dim3(256),
+                     0, s, a);
+  return check_launch();
+}
+
 // Column tiles of a row block: the fewest that hold max_seqlen tokens of a group's heads.
 int col_tiles(int64_t max_seqlen, int group) {
   const int64_t cols = max_seqlen * group;
@@ -758,13 +981,18 @@ int launch(const ChunkArgs& a, int nt, hipStream_t s) {
 }  // namespace
 }  // namespace ndl
 
-extern "C" size_t ndl_fp8_attention_workspace_bytes(int num_seqs, int max_seqlen, int64_t max_keys,
+extern "C" size_t ndl_fp8_attention_workspace_bytes(int num_seqs, int64_t num_tokens,
+                                                    int max_seqlen, int64_t max_keys,
                                                     int num_heads, int num_kv_heads, int head_dim,
                                                     int block_size) {
   using namespace ndl;
-  if (num_seqs <= 0 || max_seqlen <= 0 || max_keys <= 0 ||
-      !shape_ok(head_dim, block_size, num_heads, num_kv_heads))
+  if (num_seqs <= 0 || num_tokens <= 0 || max_seqlen <= 0 || max_keys <= 0 ||
+      max_keys > 0x7fffff00 || !shape_ok(head_dim, block_size, num_heads, num_kv_heads))
     return 0;
+  Unpacked u;
+  if (unpacked_plan(num_seqs, num_tokens, max_seqlen, max_keys, num_heads, num_kv_heads, head_dim,
+                    block_size, &u))
+    return u.total();
   const Plan p = plan_for(num_seqs, max_seqlen, max_keys, num_heads, num_kv_heads, head_dim);
   return p.ml_bytes + p.acc_bytes;
 }
@@ -797,14 +1025,8 @@ extern "C" int ndl_fp8_attention(void* out, const void* q, int64_t q_tok_stride,
   // a scale's address is the pool's and a 32-bit offset; positions are 32-bit
   if (a.plane_rows > 0x7fffffff || (int64_t)max_blocks_per_seq * block_size > 0x7fffff00)
     return NDL_ERR_UNSUPPORTED;
-  const Plan p = plan_for(num_seqs, max_seqlen, max_keys, num_heads, num_kv_heads, head_dim);
-  if (p.blocks_per_seq > 0x7fffffff) return NDL_ERR_INVALID_ARG;
-  if (p.shares) {
-    if (!workspace || workspace_bytes < p.ml_bytes + p.acc_bytes || (uintptr_t)workspace & 255u)
-      return NDL_ERR_WORKSPACE;
-    a.ws_ml = (float*)workspace;
-    a.ws_acc = (float*)((char*)workspace + p.ml_bytes);
-  }
+  if (max_keys > (int64_t)max_blocks_per_seq * block_size)
+    max_keys = (int64_t)max_blocks_per_seq * block_size;
   a.out = (u16*)out;
   a.q = (const u16*)q;
   a.q_stride = q_tok_stride;
@@ -822,6 +1044,31 @@ extern "C" int ndl_fp8_attention(void* out, const void* q, int64_t q_tok_stride,
   a.context_lens = context_lens;
   a.num_seqs = num_seqs;
   a.num_tokens = num_tokens;
+  const hipStream_t s = (hipStream_t)stream;
+  const bool f16 = dtype_is_f16(dtype);
+  Unpacked u;
+  if (cu_seqlens != nullptr && unpacked_plan(num_seqs, num_tokens, max_seqlen, max_keys, num_heads,
+                                             num_kv_heads, head_dim, block_size, &u)) {
+    if (!workspace || workspace_bytes < u.total() || (uintptr_t)workspace & 255u)
+      return NDL_ERR_WORKSPACE;
+    if (head_dim == 128)
+      return f16 ? launch_unpacked<128, true>(a, u, max_seqlen, max_keys, block_size, scale,
+                                              workspace, s)
+                 : launch_unpacked<128, false>(a, u, max_seqlen, max_keys, block_size, scale,
+                                               workspace, s);
+    return f16 ? launch_unpacked<64, true>(a, u, max_seqlen, max_keys, block_size, scale,
+                                           workspace, s)
+               : launch_unpacked<64, false>(a, u, max_seqlen, max_keys, block_size, scale,
+                                            workspace, s);
+  }
+  const Plan p = plan_for(num_seqs, max_seqlen, max_keys, num_heads, num_kv_heads, head_dim);
+  if (p.blocks_per_seq > 0x7fffffff) return NDL_ERR_INVALID_ARG;
+  if (p.shares) {
+    if (!workspace || workspace_bytes < p.ml_bytes + p.acc_bytes || (uintptr_t)workspace & 255u)
+      return NDL_ERR_WORKSPACE;
+    a.ws_ml = (float*)workspace;
+    a.ws_acc = (float*)((char*)workspace + p.ml_bytes);
+  }
   a.toks = p.toks;
   a.blocks_per_seq = (int)p.blocks_per_seq;
   a.items = p.items;
@@ -829,8 +1076,6 @@ extern "C" int ndl_fp8_attention(void* out, const void* q, int64_t q_tok_stride,
   a.shares = p.shares;
   a.min_chunk = kMinChunk;
   a.nseg = p.nseg;
-  const hipStream_t s = (hipStream_t)stream;
-  const bool f16 = dtype_is_f16(dtype);
   if (head_dim == 128)
     return f16 ? launch<128, true>(a, p.nt, s) : launch<128, false>(a, p.nt, s);
   return f16 ? launch<64, true>(a, p.nt, s) : launch<64, false>(a, p.nt, s);

@@ -931,7 +931,7 @@ def _fp8_attention(q, kv_codes, kv_scales, block_table, cu_seqlens, context_lens
     _require(max_seqlen > 0, "max_seqlen must be positive")
     max_keys = min(w * bs, max_keys) if max_keys else w * bs
     lib = _lib.load()
-    need = lib.ndl_fp8_attention_workspace_bytes(n_seqs, max_seqlen, max_keys, num_heads,
+    need = lib.ndl_fp8_attention_workspace_bytes(n_seqs, n_tok, max_seqlen, max_keys, num_heads,
                                                  num_kv_heads, head_dim, bs)
     if need and (workspace is None or workspace.numel() * workspace.element_size() < need
                  or workspace.device != dev):
@@ -946,12 +946,14 @@ def _fp8_attention(q, kv_codes, kv_scales, block_table, cu_seqlens, context_lens
     return out
 
 
-def fp8_attention_workspace_bytes(num_seqs: int, max_seqlen: int, max_keys: int, num_heads: int,
-                                  num_kv_heads: int, head_dim: int, block_size: int = 16) -> int:
-    """Bytes of the workspace paged_decode_fp8 (max_seqlen 1, max_keys the table's) or
-    varlen_prefill_fp8 uses on the current GPU; 0 where the work is not split."""
+def fp8_attention_workspace_bytes(num_seqs: int, num_tokens: int, max_seqlen: int, max_keys: int,
+                                  num_heads: int, num_kv_heads: int, head_dim: int,
+                                  block_size: int = 16) -> int:
+    """Bytes of the workspace paged_decode_fp8 (num_tokens num_seqs, max_seqlen 1, max_keys the
+    table's) or varlen_prefill_fp8 uses on the current GPU; 0 where none is used."""
     return int(_lib.load().ndl_fp8_attention_workspace_bytes(
-        num_seqs, max_seqlen, max_keys, num_heads, num_kv_heads, head_dim, block_size))
+        num_seqs, num_tokens, max_seqlen, max_keys, num_heads, num_kv_heads, head_dim,
+        block_size))
 
 
 def paged_decode_fp8(q: torch.Tensor, kv_codes: torch.Tensor, kv_scales: torch.Tensor,
@@ -977,7 +979,9 @@ def varlen_prefill_fp8(q: torch.Tensor, kv_codes: torch.Tensor, kv_scales: torch
     tokens, from one per sequence to whole prompts, over what is cached and the chunk itself
     (after kv_append_fp8).  Token j of sequence i attends min(context_lens[i] + j + 1,
     W * block_size) tokens.  max_seqlen bounds a sequence's tokens, max_context_len its cached
-    ones (0: nothing cached, or not known; it only chooses how the work is split)."""
+    ones (0: not known, the table's width then): sequences past these bounds are not attended
+    whole.  Chunks of 256 rows (max_seqlen times H / Hkv) and more unpack the keys into a 16-bit
+    workspace first, sized by the bounds, and are attended by varlen_prefill's kernels."""
     return _fp8_attention(q, kv_codes, kv_scales, block_table, cu_seqlens, context_lens,
                           int(max_seqlen),
                           int(max_context_len) + int(max_seqlen) if max_context_len else 0,

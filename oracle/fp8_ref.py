@@ -68,7 +68,7 @@ def attention(q, codes, scales, block_table, cu, context_lens, scale):
     for i in range(block_table.shape[0]):
         for j in range(int(cu[i + 1]) - int(cu[i])):
             r = int(cu[i]) + j
-            n = min(int(context_lens[i]) + j + 1, w * bs)
+            n = min(int(context_lens[i]) + j + 1, w * bs) if int(context_lens[i]) >= 0 else 0
             pages = [slot(block_table[i], p, bs, nb) for p in range(max(n, 0))]
             pages = [p for p in pages if p is not None]
             lens[r] = len(pages)

@@ -59,15 +59,16 @@ def test_attention_refusals(lib):
                 dict(q=P + 8), dict(most=0), dict(keys=0), dict(cu=None), dict(cu=None, t=3),
                 dict(stride=3), dict(nb=0)):
         assert attend(**bad) == -1, bad
-    need = lib.ndl_fp8_attention_workspace_bytes(3, 3, 8000, 8, 2, 64, 16)
+    need = lib.ndl_fp8_attention_workspace_bytes(3, 9, 3, 8000, 8, 2, 64, 16)
     assert need > 0
     assert attend(size=need - 1) == -3 and attend(ws=None, size=need) == -3
     assert attend(ws=P + 16, size=need) == -3
     assert attend(n=0) == 0 and attend(t=0) == 0
     # short tables need no workspace; nothing is sized for what is refused
-    assert lib.ndl_fp8_attention_workspace_bytes(3, 3, 64, 8, 2, 64, 16) == 0
-    for bad in ((3, 3, 8000, 9, 2, 64, 16), (0, 3, 8000, 8, 2, 64, 16), (3, 0, 8000, 8, 2, 64, 16),
-                (3, 3, 8000, 8, 2, 80, 16), (3, 3, 8000, 8, 2, 64, 17)):
+    assert lib.ndl_fp8_attention_workspace_bytes(3, 9, 3, 64, 8, 2, 64, 16) == 0
+    for bad in ((3, 9, 3, 8000, 9, 2, 64, 16), (0, 9, 3, 8000, 8, 2, 64, 16),
+                (3, 9, 0, 8000, 8, 2, 64, 16), (3, 9, 3, 8000, 8, 2, 80, 16),
+                (3, 9, 3, 8000, 8, 2, 64, 17)):
         assert lib.ndl_fp8_attention_workspace_bytes(*bad) == 0
 
 

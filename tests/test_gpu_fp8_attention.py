@@ -108,6 +108,10 @@ def test_chunks(shape, dtype, counts):
     lens = [37, 0, 250, 15][:len(counts)]
     c = Case(shape, counts, lens, dtype, seed=2)
     c.check(c.run())
+    c.ctx[0] = -2                     # attends nothing
+    got = c.run()
+    c.check(got)
+    assert not got[:counts[0]].any()
 
 
 @pytest.mark.parametrize("shape", [(14, 2, 64, 16), (32, 8, 128, 16), (7, 1, 128, 64)])
@@ -115,9 +119,34 @@ def test_chunks(shape, dtype, counts):
 def test_shares_and_merge(shape, counts):
     """Contexts long enough for the split into shares, of very different lengths."""
     c = Case(shape, counts, [2900, 3, 1111], seed=3)
-    assert ops.fp8_attention_workspace_bytes(3, max(counts), c.table.shape[1] * c.bs, c.h, c.hkv,
+    assert ops.fp8_attention_workspace_bytes(3, sum(counts), max(counts), c.table.shape[1] * c.bs, c.h, c.hkv,
                                              c.d, c.bs) > 0
     c.check(c.run(decode=max(counts) == 1))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(8, 2, 64, 16), (16, 4, 128, 32)])
+def test_row_blocks_of_one_chunk(shape, dtype):
+    """Chunks of several row blocks, just short of those that are unpacked first."""
+    c = Case(shape, [60, 33, 1, 17], [1500, 70, 800, 0], dtype, seed=15)
+    c.check(c.run())
+    c.check(c.run(max_context_len=1500))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("counts,lens", [([260], [0]), ([300, 1, 90], [77, 400, 0]),
+                                         ([257, 5], [1000, -3])])
+def test_long_chunks(shape, dtype, counts, lens):
+    """Chunks whose keys are unpacked into the workspace first."""
+    if shape[0] // shape[1] > 7:      # the oracle is slow on many heads
+        counts = [max(1, n // 4) for n in counts]
+    c = Case(shape, counts, lens, dtype, seed=16)
+    c.check(c.run())
+    ws = ops.decode_workspace(ops.fp8_attention_workspace_bytes(
+        len(lens), sum(counts), max(counts), max(lens) + max(counts), c.h, c.hkv, c.d, c.bs), DEV)
+    ws.fill_(0xFF)
+    c.check(c.run(max_context_len=max(lens), workspace=ws))
 
 
 def test_many_row_blocks_in_shares():
@@ -130,7 +159,7 @@ def test_many_row_blocks_in_shares():
 
 def test_tables_that_end_and_bad_blocks():
     """Keys past the table's columns are not attended; neither are those of an invalid block."""
-    for counts in ([1, 1, 1], [4, 4, 4]):
+    for counts in ([1, 1, 1], [4, 4, 4], [70, 20, 10]):
         c = Case((8, 2, 64, 16), counts, [70, 45, 0], seed=6, extra_cols=0)
         c.table = c.table[:, :3].contiguous()     # 48 keys
         c.table[1, 1] = -1
@@ -141,9 +170,10 @@ def test_tables_that_end_and_bad_blocks():
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-def test_a_nan_stays_where_it_is_attended(dtype):
+@pytest.mark.parametrize("count,d", [(9, 64), (80, 64), (9, 128), (80, 128)])
+def test_a_nan_stays_where_it_is_attended(dtype, count, d):
     """A NaN among the chunk's own values reaches the tokens from its position on, no others."""
-    c = Case((8, 2, 64, 16), [9, 4], [20, 61], dtype, seed=7)
+    c = Case((8, 2, d, 16), [count, 4], [20, 61], dtype, seed=7)
     for plane, seq, pos, d in ((1, 0, 24, 11), (1, 1, 64, 63), (0, 1, 63, 5), (1, 0, 28, 0)):
         b = int(c.table[seq, pos // 16])
         c.codes[plane, b, 1, pos % 16, d] = 0x7F if d % 2 else 0xFF
@@ -155,8 +185,8 @@ def test_a_nan_stays_where_it_is_attended(dtype):
 def test_scores_of_any_size():
     """Large scores (one key takes all), a raised maximum late in the row, and scale 0 and
     below."""
-    for scale in (40.0, 0.0, -0.3, 1e-6):
-        c = Case((8, 2, 128, 16), [3, 1], [700, 90], seed=8)
+    for scale, n in ((40.0, 3), (0.0, 3), (-0.3, 3), (1e-6, 3), (40.0, 66), (0.0, 66), (-0.3, 66)):
+        c = Case((8, 2, 128, 16), [n, 1], [700, 90], seed=8)
         c.scale = scale
         if scale == 40.0:
             c.q = (c.q.float() * 0.02).to(c.dtype)
@@ -171,8 +201,9 @@ def test_scores_of_any_size():
     c.check(c.run(decode=True))
 
 
-def test_strided_queries_and_padding_rows():
-    c = Case((14, 2, 64, 16), [3, 5, 1], [40, 0, 17], seed=10)
+@pytest.mark.parametrize("counts", [[3, 5, 1], [60, 5, 1]])
+def test_strided_queries_and_padding_rows(counts):
+    c = Case((14, 2, 64, 16), counts, [40, 0, 17], seed=10)
     n = int(c.cu[-1])
     wide = torch.full((n + 4, 18 * 64), float("nan"), dtype=c.dtype, device=DEV)
     q = wide[:, 64:64 + 14 * 64].view(n + 4, 14, 64)
@@ -186,7 +217,7 @@ def test_strided_queries_and_padding_rows():
 
 def test_same_inputs_same_bits_and_a_workspace_of_ones_own():
     c = Case((32, 8, 128, 16), [1] * 5, [3000, 17, 900, 1, 450], seed=11)
-    need = ops.fp8_attention_workspace_bytes(5, 1, c.table.shape[1] * 16, 32, 8, 128)
+    need = ops.fp8_attention_workspace_bytes(5, 5, 1, c.table.shape[1] * 16, 32, 8, 128)
     ws = ops.decode_workspace(need, DEV)
     first = c.run(decode=True)
     for _ in range(3):
@@ -195,7 +226,7 @@ def test_same_inputs_same_bits_and_a_workspace_of_ones_own():
                            first.view(torch.int16))
 
 
-@pytest.mark.parametrize("count", [1, 6])
+@pytest.mark.parametrize("count", [1, 6, 50])
 def test_captured_and_replayed(count):
     c = Case((14, 2, 64, 16), [count] * 3, [1900, 40, 333], seed=12)
     q, pool = c.q.to(DEV), (c.codes.to(DEV), c.scales.to(DEV))
