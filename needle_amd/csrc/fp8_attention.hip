@@ -11,7 +11,8 @@
 // Bound: the codes, each read once (2 (D + 1) bytes per token and kv head).
 //   * Rows.  The g query heads of a kv head times the chunk's tokens are the N columns of
 //     16x16x32 MFMA tiles whose M rows are tokens (S^T = K Q^T) or head_dim (O^T = V^T P^T):
-//     up to 64 columns (NT tiles of 16) are a row block, longer chunks have several.
+//     up to 32 columns (NT tiles of 16) are a row block, longer chunks have several (64 columns
+//     took more registers than there are).
 //   * Codes to registers.  A wave takes 32 tokens at a time.  Their codes go straight to its own
 //     LDS ring (1 KiB of contiguous bytes per load), two stages deep: a stage is refilled as soon
 //     as its operands are in registers, so two tiles are in flight while a third computes, and
@@ -37,7 +38,6 @@ namespace ndl {
 namespace {
 
 constexpr int kTile = 32;       // tokens per wave step
-constexpr int kWaves = 4;       // waves per workgroup; they take a row block's tiles in turn
 constexpr int kPad = 1;         // empty slots before each row block (its start's cost)
 constexpr float kRaise = 8.f;   // log2 of the largest probability before the maximum is raised
 
@@ -183,26 +183,25 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
   return (top >> 7) * 0xffu;
 }
 
-template <int D, bool F16, int NT>
+// NT: 16-column tiles of a row block; NW: waves of a workgroup, which take its tiles in turn.
+template <int D, int NT, int NW>
 struct Shape {
   static constexpr int kRowTile = kTile * D;                 // bytes of a tile's K (or V)
   static constexpr int kStage = 2 * kRowTile + 256;          // K, V, scales
-  static constexpr int kDepth = NT == 4 ? 3 : 2;
+  static constexpr int kDepth = 2;
   static constexpr int kRing = kDepth * kStage;
   static constexpr int kLoads = 2 * (kRowTile / 1024) + 1;   // per stage
-  static constexpr int kNg = NT == 1 ? 1 : 2;                // column tiles combined at a time
-  static constexpr int kSums = kWaves * kNg * 16 * D * 4;    // bytes of the waves' partial outputs
-  static constexpr int kMl = 2 * kWaves * NT * 16 * 4;
-  static constexpr int kLds = (kWaves * kRing > kSums ? kWaves * kRing : kSums) + kMl;
+  static constexpr int kSums = NW * NT * 16 * D * 4;         // bytes of the waves' partial outputs
+  static constexpr int kMl = 2 * NW * NT * 16 * 4;
+  static constexpr int kLds = (NW * kRing > kSums ? NW * kRing : kSums) + kMl;
 };
 
 // A workgroup's share of the row blocks of one kv head.
-template <int D, bool F16, int NT>
-__global__ __launch_bounds__(64 * kWaves, NT == 4 ? 1 : 2) void chunk_attention_kernel(
-    ChunkArgs a) {
+template <int D, bool F16, int NT, int NW>
+__global__ __launch_bounds__(64 * NW, 8 / NW) void chunk_attention_kernel(ChunkArgs a) {
   using T = Elt<F16>;
   using X8 = typename T::x8;
-  using S = Shape<D, F16, NT>;
+  using S = Shape<D, NT, NW>;
   constexpr int KS = D / 32;      // k steps of the QK product
   constexpr int DB = D / 16;      // 16-row tiles of O^T; head_dim index DB * m + b in tile b
   constexpr int VW = DB / 4;      // words of codes a lane holds of one V row
@@ -241,9 +240,20 @@ __global__ __launch_bounds__(64 * kWaves, NT == 4 ? 1 : 2) void chunk_attention_
   const uint32_t tmask = (1u << a.tile_shift) - 1;
 
   for (; e < a.items; ++e) {
+    // This wave's tiles: t0 + wv, t0 + wv + NW, ..  Lane 2 u + s of a window holds the block id of
+    // 16-token half s of the window's tile u (32 of the wave's tiles).
+    const int32_t* const table = a.block_table + (e / a.blocks_per_seq) * a.bt_row_stride;
+    int t0 = 0, window;
+    auto load_window = [&](int u0) {
+      const int tt = 2 * (t0 + wv + NW * (u0 + (lane >> 1))) + (lane & 1);
+      int col = tt >> a.tile_shift;
+      if (col > a.max_blocks - 1) col = a.max_blocks - 1;
+      window = table[col];
+    };
+    if (whole) load_window(0);        // before the lengths arrive
     const Item it = item_of(a, e);
     const int ntiles = it.tiles();
-    int t0 = 0, t1 = ntiles;
+    int t1 = ntiles;
     if (!whole) {
       if (ntiles == 0) continue;
       if (first >= to) break;
@@ -252,6 +262,7 @@ __global__ __launch_bounds__(64 * kWaves, NT == 4 ? 1 : 2) void chunk_attention_
       t1 = to < base + ntiles ? (int)(to - base) : ntiles;
       first = base + ntiles;
       if (t0 >= t1) continue;     // only the empty slot is this share's
+      load_window(0);
     } else if (it.n <= 0) {
       return;
     }
@@ -287,27 +298,17 @@ __global__ __launch_bounds__(64 * kWaves, NT == 4 ? 1 : 2) void chunk_attention_
       for (int b = 0; b < DB; ++b) acc[nt][b] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
-    // This wave's tiles: t0 + wv, t0 + wv + kWaves, ..  Lane 2 u + s of a window holds 16-token
-    // half s of the window's tile u: its first row in a plane of kv head 0's slices, or -1.
-    const int cnt = t1 - t0 > wv ? (t1 - t0 - wv + kWaves - 1) / kWaves : 0;
-    const int32_t* const table = a.block_table + (int64_t)it.seq * a.bt_row_stride;
-    int window[1];                // block ids
-    auto load_window = [&](int u0) {
-      const int tt = 2 * (t0 + wv + kWaves * (u0 + (lane >> 1))) + (lane & 1);
-      int col = tt >> a.tile_shift;
-      if (col > a.max_blocks - 1) col = a.max_blocks - 1;
-      window[0] = table[col];
-    };
+    const int cnt = t1 - t0 > wv ? (t1 - t0 - wv + NW - 1) / NW : 0;
     uint32_t bad_bits = 0;        // two bits per stage: its halves with an invalid block id
     auto issue = [&](int u, int slot) {
-      if ((u & 31) == 0) load_window(u);
+      if (u > 0 && (u & 31) == 0) load_window(u);
       const uint32_t st = ring_lds + slot * S::kStage;
-      const int tile = t0 + wv + kWaves * u;
+      const int tile = t0 + wv + NW * u;
       uint32_t srow[2];
       uint32_t bad = 0;
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        int b = __builtin_amdgcn_readlane(window[0], 2 * (u & 31) + s);
+        int b = __builtin_amdgcn_readlane(window, 2 * (u & 31) + s);
         if (b < 0 || b >= a.num_blocks) {
           b = 0;
           bad |= 1u << s;
@@ -404,7 +405,7 @@ __global__ __launch_bounds__(64 * kWaves, NT == 4 ? 1 : 2) void chunk_attention_
           for (int nt = 0; nt < NT; ++nt) sc[s][nt][r] *= ks;
         }
 
-      const int tile = t0 + wv + kWaves * u;
+      const int tile = t0 + wv + NW * u;
       const bool masked = bad != 0 || kTile * (tile + 1) > min_keys;
       uint32_t nan_any = 0;
       if (masked) {
@@ -526,82 +527,80 @@ __global__ __launch_bounds__(64 * kWaves, NT == 4 ? 1 : 2) void chunk_attention_
     }
 
     // The waves' results: (m, l) first, then the outputs scaled to the common maximum, laid out
-    // so that wave r of the reduction holds head_dim DB (4 j + r) .. of column c.
+    // so that one wave's lanes hold head_dim DB (4 j + r) .. of column tile nt's columns.
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       l[nt] = add_xor32(add_xor16(l[nt]));
       if (j == 0) {
         ml[wv * 16 * NT + 16 * nt + c] = m[nt];
-        ml[(kWaves + wv) * 16 * NT + 16 * nt + c] = l[nt];
+        ml[(NW + wv) * 16 * NT + 16 * nt + c] = l[nt];
       }
+    }
+    __syncthreads();
+    float* const sums = reinterpret_cast<float*>(smem);   // [wave][nt][r][lane][DB]
+    float mm[NT], ll[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int col = 16 * nt + c;
+      mm[nt] = ml[col];
+#pragma unroll
+      for (int w = 1; w < NW; ++w) mm[nt] = fmaxf(mm[nt], ml[w * 16 * NT + col]);
+      ll[nt] = 0.f;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        const float mw = ml[w * 16 * NT + col];
+        ll[nt] += ml[(NW + w) * 16 * NT + col] * (mw == mm[nt] ? 1.f : fast_exp2(mw - mm[nt]));
+      }
+      const float f = m[nt] == mm[nt] ? 1.f : fast_exp2(m[nt] - mm[nt]);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int b = 0; b < DB; b += 4)
+          *reinterpret_cast<f32x4*>(sums + (((wv * NT + nt) * 4 + r) * 64 + lane) * DB + b) =
+              f32x4{acc[nt][b][r] * f, acc[nt][b + 1][r] * f, acc[nt][b + 2][r] * f,
+                    acc[nt][b + 3][r] * f};
     }
     __syncthreads();
     const bool part = !whole && (t0 > 0 || t1 < ntiles);
     const int64_t seg = ((int64_t)head * a.nseg + unit + e) * (a.toks * a.group);
 #pragma unroll
-    for (int g0 = 0; g0 < NT; g0 += S::kNg) {
-      float* const sums = reinterpret_cast<float*>(smem);   // [wave][nt][r][lane][DB]
-      float mm[S::kNg], ll[S::kNg];
+    for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-      for (int y = 0; y < S::kNg; ++y) {
-        const int nt = g0 + y, col = 16 * nt + c;
-        mm[y] = ml[col];
-#pragma unroll
-        for (int w = 1; w < kWaves; ++w) mm[y] = fmaxf(mm[y], ml[w * 16 * NT + col]);
-        ll[y] = 0.f;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-          const float mw = ml[w * 16 * NT + col];
-          ll[y] += ml[(kWaves + w) * 16 * NT + col] * (mw == mm[y] ? 1.f : fast_exp2(mw - mm[y]));
-        }
-        const float f = m[nt] == mm[y] ? 1.f : fast_exp2(m[nt] - mm[y]);
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-          for (int b4 = 0; b4 < DB; b4 += 4)
-            *reinterpret_cast<f32x4*>(sums + (((wv * S::kNg + y) * 4 + r) * 64 + lane) * DB + b4) =
-                f32x4{acc[nt][b4][r] * f, acc[nt][b4 + 1][r] * f, acc[nt][b4 + 2][r] * f,
-                      acc[nt][b4 + 3][r] * f};
-      }
-      __syncthreads();
-#pragma unroll
-      for (int y = 0; y < S::kNg; ++y) {
-        const int col = 16 * (g0 + y) + c;
+      for (int r = 0; r < 4; ++r) {
+        if ((nt * 4 + r) % NW != wv) continue;
+        const int col = 16 * nt + c;
         float o[DB];
 #pragma unroll
         for (int b = 0; b < DB; ++b) o[b] = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w)
+        for (int w = 0; w < NW; ++w)
 #pragma unroll
-          for (int b = 0; b < DB; ++b)
-            o[b] += sums[(((w * S::kNg + y) * 4 + wv) * 64 + lane) * DB + b];
-        if (col < cols) {
-          const int d0 = DB * (4 * j + wv);
-          if (part) {
-            float* const dst = a.ws_acc + (seg + col) * D + d0;
+          for (int b = 0; b < DB; ++b) o[b] += sums[(((w * NT + nt) * 4 + r) * 64 + lane) * DB + b];
+        if (col >= cols) continue;
+        const int d0 = DB * (4 * j + r);
+        if (part) {
+          float* const dst = a.ws_acc + (seg + col) * D + d0;
 #pragma unroll
-            for (int b = 0; b < DB; b += 4)
-              *reinterpret_cast<f32x4*>(dst + b) = f32x4{o[b], o[b + 1], o[b + 2], o[b + 3]};
-            if (j == 0 && wv == 0)
-              *reinterpret_cast<f32x2*>(a.ws_ml + (seg + col) * 2) = f32x2{mm[y], ll[y]};
-          } else {
-            const float inv = ll[y] == 0.f ? 0.f : 1.f / ll[y];   // nothing attended: zeros
-            const int tok = col / a.group;
-            u16* const dst = a.out + ((it.tok0 + tok) * a.num_heads + head * a.group + col -
-                                      tok * a.group) * (int64_t)D + d0;
-            uint32_t w[DB / 2];
+          for (int b = 0; b < DB; b += 4)
+            *reinterpret_cast<f32x4*>(dst + b) = f32x4{o[b], o[b + 1], o[b + 2], o[b + 3]};
+          if (d0 == 0) *reinterpret_cast<f32x2*>(a.ws_ml + (seg + col) * 2) = f32x2{mm[nt], ll[nt]};
+        } else {
+          const float inv = ll[nt] == 0.f ? 0.f : 1.f / ll[nt];   // nothing attended: zeros
+          const int tok = col / a.group;
+          u16* const dst = a.out + ((it.tok0 + tok) * a.num_heads + head * a.group + col -
+                                    tok * a.group) * (int64_t)D + d0;
+          uint32_t w[DB / 2];
 #pragma unroll
-            for (int b = 0; b < DB / 2; ++b) w[b] = T::pack(o[2 * b] * inv, o[2 * b + 1] * inv);
-            if constexpr (DB == 8)
-              st16(dst, u32x4{w[0], w[1], w[2], w[3]});
-            else
-              *reinterpret_cast<u32x2*>(dst) = u32x2{w[0], w[1]};
-          }
+          for (int b = 0; b < DB / 2; ++b) w[b] = T::pack(o[2 * b] * inv, o[2 * b + 1] * inv);
+          if constexpr (DB == 8)
+            st16(dst, u32x4{w[0], w[1], w[2], w[3]});
+          else
+            *reinterpret_cast<u32x2*>(dst) = u32x2{w[0], w[1]};
         }
       }
-      __syncthreads();     // before the sums or the ring are written again
     }
     if (whole) return;
+    __syncthreads();     // before the ring is written again
   }
 }
 
@@ -659,17 +658,44 @@ __global__ __launch_bounds__(256) void chunk_merge_kernel(ChunkArgs a) {
   const int n = (int)(s1 - s0 + 1);
   const float* const ml = a.ws_ml + seg * 2;
   const float* const src = a.ws_acc + seg * D + lane * PER;
-  float mx = kNegInf;
-  for (int i = lane; i < n; i += 64) mx = fmaxf(mx, ml[(int64_t)i * per * 2]);
+  // a lane per part for (m, l), 64 at a time; the first parts' outputs are loaded along with them
+  constexpr int kPre = 8;
+  const int64_t step = (int64_t)per * D;
+  float pre[kPre][PER];
+#pragma unroll
+  for (int i = 0; i < kPre; ++i)
+#pragma unroll
+    for (int x = 0; x < PER; ++x) pre[i][x] = src[(i < n ? i : 0) * step + x];
+  const int mine = lane < n ? lane : n - 1;
+  f32x2 v = *reinterpret_cast<const f32x2*>(ml + (int64_t)mine * per * 2);
+  float mx = v[0];
+  for (int i = lane + 64; i < n; i += 64) mx = fmaxf(mx, ml[(int64_t)i * per * 2]);
 #pragma unroll
   for (int x = 32; x >= 1; x >>= 1) mx = fmaxf(mx, xor_shfl(mx, x));
   float l = 0.f;
-  for (int i = 0; i < n; ++i) {
-    const f32x2 v = *reinterpret_cast<const f32x2*>(ml + (int64_t)i * per * 2);
-    const float f = v[0] == mx ? 1.f : fast_exp2(v[0] - mx);
-    l += v[1] * f;
+  for (int i0 = 0; i0 < n; i0 += 64) {
+    if (i0 > 0) v = *reinterpret_cast<const f32x2*>(
+                    ml + (int64_t)(i0 + lane < n ? i0 + lane : n - 1) * per * 2);
+    const float f = i0 + lane >= n ? 0.f : v[0] == mx ? 1.f : fast_exp2(v[0] - mx);
+    float part = v[1] * f;
 #pragma unroll
-    for (int x = 0; x < PER; ++x) o[x] += src[(int64_t)i * per * D + x] * f;
+    for (int x = 32; x >= 1; x >>= 1) part += xor_shfl(part, x);
+    l += part;
+    const int m = n - i0 < 64 ? n - i0 : 64;
+    for (int i = 0; i < m; i += kPre) {
+      if (i0 + i > 0)
+#pragma unroll
+        for (int y = 0; y < kPre; ++y)
+#pragma unroll
+          for (int x = 0; x < PER; ++x) pre[y][x] = src[(i0 + i + y < n ? i0 + i + y : 0) * step + x];
+#pragma unroll
+      for (int y = 0; y < kPre; ++y) {
+        if (i + y >= m) break;
+        const float w = __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(f), i + y));
+#pragma unroll
+        for (int x = 0; x < PER; ++x) o[x] += pre[y][x] * w;
+      }
+    }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
@@ -896,14 +922,11 @@ int launch_unpacked(const ChunkArgs& c, const Unpacked& u, int max_seqlen, int64
   return check_launch();
 }
 
-// Column tiles of a row block: the fewest that hold max_seqlen tokens of a group's heads.
-int col_tiles(int64_t max_seqlen, int group) {
-  const int64_t cols = max_seqlen * group;
-  return cols <= 16 ? 1 : cols <= 32 ? 2 : 4;
-}
+// Column tiles of a row block: one where it holds max_seqlen tokens of a group's heads, else two.
+int col_tiles(int64_t max_seqlen, int group) { return max_seqlen * group <= 16 ? 1 : 2; }
 
 struct Plan {
-  int nt, toks;
+  int nt, toks, waves;
   int64_t blocks_per_seq, items;
   int shares;                 // 0: whole row blocks
   int64_t nseg;
@@ -911,13 +934,21 @@ struct Plan {
 };
 
 template <int D, bool F16>
-const void* kernel_of(int nt) {
-  return nt == 1 ? (const void*)chunk_attention_kernel<D, F16, 1>
-         : nt == 2 ? (const void*)chunk_attention_kernel<D, F16, 2>
-                   : (const void*)chunk_attention_kernel<D, F16, 4>;
+const void* kernel_of(int nt, int waves) {
+  if (waves == 4)
+    return nt == 1 ? (const void*)chunk_attention_kernel<D, F16, 1, 4>
+                   : (const void*)chunk_attention_kernel<D, F16, 2, 4>;
+  return nt == 1 ? (const void*)chunk_attention_kernel<D, F16, 1, 8>
+                 : (const void*)chunk_attention_kernel<D, F16, 2, 8>;
 }
 
-constexpr int kMinChunk = 2 * kWaves;
+#ifndef SHARE_WAVES
+#define SHARE_WAVES 4
+#define WHOLE_WAVES 8
+#define WHOLE_TILES 32
+#define MIN_CHUNK 8
+#endif
+constexpr int kMinChunk = MIN_CHUNK;
 
 // resident: workgroups the GPU holds at once.
 Plan make_plan(int64_t num_seqs, int64_t max_seqlen, int64_t max_keys, int group,
@@ -929,7 +960,8 @@ Plan make_plan(int64_t num_seqs, int64_t max_seqlen, int64_t max_keys, int group
   p.items = num_seqs * p.blocks_per_seq;
   const int64_t tiles = (max_keys + kTile - 1) / kTile;
   const int64_t units = p.items * num_kv_heads;
-  const bool whole = tiles <= 2 * kMinChunk || units >= 4 * resident;
+  const bool whole = tiles <= WHOLE_TILES || units >= 4 * resident;
+  p.waves = whole && units * 2 <= resident ? WHOLE_WAVES : SHARE_WAVES;
   if (!whole) {
     int64_t s = resident / num_kv_heads / 8 * 8;
     if (s < 8) s = 8;
@@ -953,23 +985,20 @@ Plan plan_for(int64_t num_seqs, int64_t max_seqlen, int64_t max_keys, int num_he
   const int group = num_heads / num_kv_heads, nt = col_tiles(max_seqlen, group);
   // the formats' kernels use the same resources
   int64_t res = resident_workgroups(
-      head_dim == 128 ? kernel_of<128, false>(nt) : kernel_of<64, false>(nt), 64 * kWaves);
+      head_dim == 128 ? kernel_of<128, false>(nt, SHARE_WAVES) : kernel_of<64, false>(nt, SHARE_WAVES), 64 * SHARE_WAVES);
   if (res <= 0) res = 256;
   return make_plan(num_seqs, max_seqlen, max_keys, group, num_kv_heads, head_dim, res);
 }
 
 template <int D, bool F16>
-int launch(const ChunkArgs& a, int nt, hipStream_t s) {
+int launch(ChunkArgs a, int nt, int waves, hipStream_t s) {
   const int64_t units = a.shares ? a.shares : (a.items + 7) / 8 * 8;
   const int64_t wgs = units * a.num_kv_heads;
   if (wgs > 0x7fffffff) return NDL_ERR_INVALID_ARG;
-  const dim3 grid((unsigned)wgs), wg(64 * kWaves);
-  if (nt == 1)
-    hipLaunchKernelGGL((chunk_attention_kernel<D, F16, 1>), grid, wg, 0, s, a);
-  else if (nt == 2)
-    hipLaunchKernelGGL((chunk_attention_kernel<D, F16, 2>), grid, wg, 0, s, a);
-  else
-    hipLaunchKernelGGL((chunk_attention_kernel<D, F16, 4>), grid, wg, 0, s, a);
+  void* args[] = {&a};
+  if (hipLaunchKernel(kernel_of<D, F16>(nt, waves), dim3((unsigned)wgs), dim3(64 * waves), args, 0,
+                      s) != hipSuccess)
+    return NDL_ERR_LAUNCH;
   const int rc = check_launch();
   if (rc != NDL_OK || a.shares == 0) return rc;
   const int64_t rows = a.num_tokens * a.num_heads, blocks = (rows + 3) / 4;
@@ -1077,6 +1106,6 @@ extern "C" int ndl_fp8_attention(void* out, const void* q, int64_t q_tok_stride,
   a.min_chunk = kMinChunk;
   a.nseg = p.nseg;
   if (head_dim == 128)
-    return f16 ? launch<128, true>(a, p.nt, s) : launch<128, false>(a, p.nt, s);
-  return f16 ? launch<64, true>(a, p.nt, s) : launch<64, false>(a, p.nt, s);
+    return f16 ? launch<128, true>(a, p.nt, p.waves, s) : launch<128, false>(a, p.nt, p.waves, s);
+  return f16 ? launch<64, true>(a, p.nt, p.waves, s) : launch<64, false>(a, p.nt, p.waves, s);
 }
