@@ -31,6 +31,12 @@ decltype(&ndl_varlen_prefill_workspace_bytes) p_prefill_workspace = nullptr;
 decltype(&ndl_varlen_prefill_split) p_prefill_split = nullptr;
 decltype(&ndl_rms_norm) p_rms_norm = nullptr;
 decltype(&ndl_silu_mul) p_silu_mul = nullptr;
+decltype(&ndl_kv_append_fp8) p_kv_append_fp8 = nullptr;
+decltype(&ndl_kv_read_fp8) p_kv_read_fp8 = nullptr;
+decltype(&ndl_fp8_attention_workspace_bytes) p_fp8_workspace = nullptr;
+decltype(&ndl_fp8_attention) p_fp8_attention = nullptr;
+decltype(&ndl_verify_drafts_workspace_bytes) p_verify_workspace = nullptr;
+decltype(&ndl_verify_drafts) p_verify_drafts = nullptr;
 
 // A plain GPU tensor (no subclass, no wrapper of a function transform), or null.
 const at::Tensor* gpu_tensor(PyObject* o) {
@@ -222,6 +228,15 @@ bool read_matrix(const at::Tensor& x, const at::Tensor& like, int64_t width, int
   return *stride % 8 == 0 && ((uintptr_t)x.data_ptr() & 15u) == 0;
 }
 
+PyObject* tensor_pair(at::Tensor&& x, at::Tensor&& y) {
+  PyObject* const a = THPVariable_Wrap(std::move(x));
+  PyObject* const b = a ? THPVariable_Wrap(std::move(y)) : nullptr;
+  PyObject* const pair = b ? PyTuple_Pack(2, a, b) : nullptr;
+  Py_XDECREF(a);
+  Py_XDECREF(b);
+  return pair;
+}
+
 // rms_norm(x, weight, eps, residual or None): the norm, or (norm, x + residual).
 PyObject* rms_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -253,12 +268,7 @@ PyObject* rms_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   Py_END_ALLOW_THREADS
   if (rc != NDL_OK) Py_RETURN_NONE;
   if (res == nullptr) return THPVariable_Wrap(std::move(out));
-  PyObject* const a = THPVariable_Wrap(std::move(out));
-  PyObject* const b = a ? THPVariable_Wrap(std::move(sum)) : nullptr;
-  PyObject* const pair = b ? PyTuple_Pack(2, a, b) : nullptr;
-  Py_XDECREF(a);
-  Py_XDECREF(b);
-  return pair;
+  return tensor_pair(std::move(out), std::move(sum));
   END_HANDLE_TH_ERRORS
 }
 
@@ -287,6 +297,230 @@ PyObject* silu_mul(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// An 8-bit pool: codes [2, NB, Hkv, bs, D] and scales [2, NB, Hkv, bs].
+struct Fp8Pool {
+  int64_t num_blocks, hkv, bs, d;
+};
+bool read_fp8_pool(const at::Tensor& codes, const at::Tensor& scales, Fp8Pool* p) {
+  if (codes.dim() != 5 || codes.size(0) != 2 || scales.dim() != 4 || !codes.is_contiguous() ||
+      !scales.is_contiguous() || scales.scalar_type() != at::kByte ||
+      (codes.scalar_type() != at::kFloat8_e4m3fn && codes.scalar_type() != at::kByte) ||
+      scales.device() != codes.device())
+    return false;
+  for (int i = 0; i < 4; ++i)
+    if (scales.size(i) != codes.size(i)) return false;
+  p->num_blocks = codes.size(1);
+  p->hkv = codes.size(2);
+  p->bs = codes.size(3);
+  p->d = codes.size(4);
+  return fits_int(p->hkv) && (p->d == 64 || p->d == 128) && p->bs >= 16 && p->bs <= 1024 &&
+         (p->bs & (p->bs - 1)) == 0;
+}
+bool is_16bit(at::ScalarType t) { return t == at::kBFloat16 || t == at::kHalf; }
+
+// Token stride of [T, heads, d] rows on the pool's device; false if not so.
+bool read_rows_of(const at::Tensor& x, const at::Tensor& pool, int64_t heads, int64_t d,
+                  int64_t* stride) {
+  if (x.dim() != 3 || x.size(1) != heads || x.size(2) != d || x.stride(2) != 1 ||
+      x.stride(1) != d || x.device() != pool.device())
+    return false;
+  *stride = x.size(0) > 1 ? x.stride(0) : heads * d;
+  return true;
+}
+// The tensor at o, or none at all: false where it is neither.
+bool maybe_tensor(PyObject* o, const at::Tensor** t) {
+  *t = nullptr;
+  return o == Py_None || (*t = gpu_tensor(o)) != nullptr;
+}
+
+// kv_append_fp8(k, v, codes, scales, block_table, context_lens, cu_seqlens or None, q or None,
+// cos or None, sin or None): the rotated q, or True without one.
+PyObject* kv_append_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 10 || p_kv_append_fp8 == nullptr || validating()) Py_RETURN_NONE;
+  const at::Tensor *t[6], *cu, *q, *cos, *sin;
+  for (int i = 0; i < 6; ++i)
+    if ((t[i] = gpu_tensor(args[i])) == nullptr) Py_RETURN_NONE;
+  if (!maybe_tensor(args[6], &cu) || !maybe_tensor(args[7], &q) || !maybe_tensor(args[8], &cos) ||
+      !maybe_tensor(args[9], &sin) || (cos == nullptr) != (sin == nullptr) ||
+      (q != nullptr && cos == nullptr))
+    Py_RETURN_NONE;
+  const at::Tensor &k = *t[0], &v = *t[1], &codes = *t[2], &scales = *t[3], &table = *t[4],
+                   &lens = *t[5];
+  Fp8Pool p;
+  int64_t ks, vs, qs = 0, cs = 0, heads = 0;
+  if (!read_fp8_pool(codes, scales, &p) || !is_16bit(k.scalar_type()) ||
+      v.scalar_type() != k.scalar_type() || !read_rows_of(k, codes, p.hkv, p.d, &ks) ||
+      !read_rows_of(v, codes, p.hkv, p.d, &vs) || !read_int32(table, codes, 2) ||
+      !read_int32(lens, codes, 1) || (cu != nullptr && !read_int32(*cu, codes, 1)))
+    Py_RETURN_NONE;
+  const int64_t tokens = k.size(0), seqs = table.size(0), width = table.size(1);
+  if (tokens == 0 || v.size(0) != tokens || lens.size(0) != seqs || width == 0 ||
+      !fits_int(seqs) || !fits_int(width) ||
+      (cu != nullptr ? cu->size(0) != seqs + 1 : tokens != seqs) ||
+      (cos != nullptr && !read_rope(*cos, *sin, k, tokens, p.d, &cs)))
+    Py_RETURN_NONE;
+  at::Tensor out;
+  if (q != nullptr) {
+    if (q->dim() != 3 || q->size(0) != tokens || q->scalar_type() != k.scalar_type()) Py_RETURN_NONE;
+    heads = q->size(1);
+    if (heads == 0 || !fits_int(heads) || !read_rows_of(*q, codes, heads, p.d, &qs)) Py_RETURN_NONE;
+    out = at::empty({tokens, heads, p.d}, q->options());
+  }
+  const ndl_stream_t s = stream_of(codes);
+  void* const outp = q ? out.data_ptr() : nullptr;
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = p_kv_append_fp8(codes.data_ptr(), scales.data_ptr(), p.num_blocks, (int)p.hkv, (int)p.bs,
+                       (int)p.d, dtype_code(k.scalar_type()), k.data_ptr(), ks, v.data_ptr(), vs,
+                       outp, q ? q->data_ptr() : nullptr, qs, (int)heads,
+                       cos ? cos->data_ptr() : nullptr, cos ? sin->data_ptr() : nullptr, cs,
+                       (const int32_t*)table.data_ptr(), table.stride(0), (int)width,
+                       cu ? (const int32_t*)cu->data_ptr() : nullptr,
+                       (const int32_t*)lens.data_ptr(), (int)seqs, tokens, s);
+  Py_END_ALLOW_THREADS
+  if (rc != NDL_OK) Py_RETURN_NONE;
+  if (q == nullptr) Py_RETURN_TRUE;
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// kv_read_fp8(codes, scales, block_table, first, cu_seqlens, num_tokens, dtype code): (k, v).
+PyObject* kv_read_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 7 || p_kv_read_fp8 == nullptr || validating()) Py_RETURN_NONE;
+  const at::Tensor* t[5];
+  for (int i = 0; i < 5; ++i)
+    if ((t[i] = gpu_tensor(args[i])) == nullptr) Py_RETURN_NONE;
+  const at::Tensor &codes = *t[0], &scales = *t[1], &table = *t[2], &first = *t[3], &cu = *t[4];
+  Fp8Pool p;
+  int64_t tokens, code;
+  if (!read_fp8_pool(codes, scales, &p) || !read_int32(table, codes, 2) ||
+      !read_int32(first, codes, 1) || !read_int32(cu, codes, 1) || !read_int(args[5], &tokens) ||
+      !read_int(args[6], &code) || (code != NDL_DTYPE_BF16 && code != NDL_DTYPE_F16))
+    Py_RETURN_NONE;
+  const int64_t seqs = table.size(0), width = table.size(1);
+  if (tokens == 0 || seqs == 0 || width == 0 || first.size(0) != seqs || cu.size(0) != seqs + 1 ||
+      !fits_int(seqs) || !fits_int(width))
+    Py_RETURN_NONE;
+  const auto opts = codes.options().dtype(code == NDL_DTYPE_F16 ? at::kHalf : at::kBFloat16);
+  at::Tensor k = at::empty({tokens, p.hkv, p.d}, opts), v = at::empty({tokens, p.hkv, p.d}, opts);
+  const ndl_stream_t s = stream_of(codes);
+  void *const kp = k.data_ptr(), *const vp = v.data_ptr();
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = p_kv_read_fp8(kp, vp, codes.data_ptr(), scales.data_ptr(), p.num_blocks, (int)p.hkv,
+                     (int)p.bs, (int)p.d, (int)code, (const int32_t*)table.data_ptr(),
+                     table.stride(0), (int)width, (const int32_t*)first.data_ptr(),
+                     (const int32_t*)cu.data_ptr(), (int)seqs, tokens, s);
+  Py_END_ALLOW_THREADS
+  if (rc != NDL_OK) Py_RETURN_NONE;
+  return tensor_pair(std::move(k), std::move(v));
+  END_HANDLE_TH_ERRORS
+}
+
+// fp8_attention(q, codes, scales, block_table, cu_seqlens or None, context_lens, max_seqlen,
+// max_keys (0: the table's), scale, num_heads, num_kv_heads, head_dim): the output.
+PyObject* fp8_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 12 || p_fp8_attention == nullptr || validating()) Py_RETURN_NONE;
+  const at::Tensor* t[4];
+  for (int i = 0; i < 4; ++i)
+    if ((t[i] = gpu_tensor(args[i])) == nullptr) Py_RETURN_NONE;
+  const at::Tensor &q = *t[0], &codes = *t[1], &scales = *t[2], &table = *t[3], *cu;
+  const at::Tensor* const lensp = gpu_tensor(args[5]);
+  int64_t most, keys, heads, hkv, d, qs;
+  Fp8Pool p;
+  if (lensp == nullptr || !maybe_tensor(args[4], &cu) || !read_int(args[6], &most) ||
+      !read_int(args[7], &keys) || !PyFloat_CheckExact(args[8]) || !read_int(args[9], &heads) ||
+      !read_int(args[10], &hkv) || !read_int(args[11], &d) || !read_fp8_pool(codes, scales, &p) ||
+      p.hkv != hkv || p.d != d || !is_16bit(q.scalar_type()) || hkv == 0 || heads == 0 ||
+      heads % hkv || heads / hkv > 16 || !read_rows_of(q, codes, heads, d, &qs))
+    Py_RETURN_NONE;
+  const at::Tensor& lens = *lensp;
+  const float scale = (float)PyFloat_AS_DOUBLE(args[8]);
+  const int64_t tokens = q.size(0), seqs = table.size(0);
+  if (!read_int32(table, codes, 2) || !read_int32(lens, codes, 1) || lens.size(0) != seqs ||
+      (cu != nullptr && !read_int32(*cu, codes, 1)))
+    Py_RETURN_NONE;
+  const int64_t width = table.size(1);
+  if (tokens == 0 || seqs == 0 || width == 0 || most == 0 || !fits_int(seqs) || !fits_int(width) ||
+      (cu != nullptr ? cu->size(0) != seqs + 1 : tokens != seqs || most != 1))
+    Py_RETURN_NONE;
+  if (keys == 0 || keys > width * p.bs) keys = width * p.bs;
+  at::Tensor out = at::empty({tokens, heads, d}, q.options()), ws;
+  const size_t need = p_fp8_workspace((int)seqs, tokens, (int)most, keys, (int)heads, (int)hkv,
+                                      (int)d, (int)p.bs);
+  if (need) ws = at::empty({(int64_t)need}, q.options().dtype(at::kByte));
+  void *const outp = out.data_ptr(), *const wsp = need ? ws.data_ptr() : nullptr;
+  const ndl_stream_t s = stream_of(codes);
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = p_fp8_attention(outp, q.data_ptr(), qs, codes.data_ptr(), scales.data_ptr(), p.num_blocks,
+                       (const int32_t*)table.data_ptr(), table.stride(0), (int)width,
+                       cu ? (const int32_t*)cu->data_ptr() : nullptr,
+                       (const int32_t*)lens.data_ptr(), (int)seqs, tokens, (int)most, keys,
+                       (int)heads, (int)hkv, (int)d, (int)p.bs, dtype_code(q.scalar_type()), scale,
+                       wsp, need, s);
+  Py_END_ALLOW_THREADS
+  if (rc != NDL_OK) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// verify_drafts(logits, ids, cu_seqlens, uniforms, temperature or None, draft_probs or None):
+// (tokens, accepted).
+PyObject* verify_drafts(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 6 || p_verify_drafts == nullptr) Py_RETURN_NONE;
+  const at::Tensor *t[4], *temp, *probs;
+  for (int i = 0; i < 4; ++i)
+    if ((t[i] = gpu_tensor(args[i])) == nullptr) Py_RETURN_NONE;
+  if (!maybe_tensor(args[4], &temp) || !maybe_tensor(args[5], &probs)) Py_RETURN_NONE;
+  const at::Tensor &logits = *t[0], &ids = *t[1], &cu = *t[2], &u = *t[3];
+  const int code = dtype_code(logits.scalar_type());
+  if (code < 0 || logits.dim() != 2 || ids.dim() != 1 || !ids.is_contiguous() ||
+      (ids.scalar_type() != at::kInt && ids.scalar_type() != at::kLong) ||
+      ids.device() != logits.device() || !read_int32(cu, logits, 1) || u.dim() != 1 ||
+      u.scalar_type() != at::kFloat || !u.is_contiguous() || u.device() != logits.device())
+    Py_RETURN_NONE;
+  const int64_t rows = logits.size(0), vocab = logits.size(1), seqs = cu.size(0) - 1;
+  if (rows == 0 || vocab == 0 || vocab > 0x7fffffff || seqs <= 0 || rows < seqs ||
+      ids.size(0) != rows || u.size(0) != rows || logits.stride(1) != 1 ||
+      (rows > 1 && logits.stride(0) < vocab))
+    Py_RETURN_NONE;
+  if (temp != nullptr && (temp->dim() != 1 || temp->size(0) != seqs || !temp->is_contiguous() ||
+                          temp->scalar_type() != at::kFloat || temp->device() != logits.device()))
+    Py_RETURN_NONE;
+  int64_t ds = vocab;
+  if (probs != nullptr) {
+    if (probs->dim() != 2 || probs->size(0) != rows - seqs || probs->size(1) != vocab ||
+        probs->scalar_type() != at::kFloat || probs->device() != logits.device() ||
+        (rows > seqs && probs->stride(1) != 1))
+      Py_RETURN_NONE;
+    if (rows - seqs > 1 && (ds = probs->stride(0)) < vocab) Py_RETURN_NONE;
+    if (rows == seqs) probs = nullptr;   // no drafts, and no address either
+  }
+  at::Tensor tokens = at::empty_like(ids), accepted = at::empty({seqs}, cu.options());
+  const size_t need = p_verify_workspace(rows, (int)seqs, (int)vocab);
+  at::Tensor ws = at::empty({(int64_t)need}, cu.options().dtype(at::kByte));
+  void *const tp = tokens.data_ptr(), *const wsp = ws.data_ptr();
+  int32_t* const ap = (int32_t*)accepted.data_ptr();
+  const ndl_stream_t s = stream_of(logits);
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = p_verify_drafts(tp, ap, logits.data_ptr(), rows > 1 ? logits.stride(0) : vocab, code,
+                       ids.data_ptr(), ids.scalar_type() == at::kLong,
+                       (const int32_t*)cu.data_ptr(), (const float*)u.data_ptr(),
+                       temp ? (const float*)temp->data_ptr() : nullptr,
+                       probs ? (const float*)probs->data_ptr() : nullptr, ds, rows - seqs, rows,
+                       (int)seqs, (int)vocab, wsp, need, s);
+  Py_END_ALLOW_THREADS
+  if (rc != NDL_OK) Py_RETURN_NONE;
+  return tensor_pair(std::move(tokens), std::move(accepted));
+  END_HANDLE_TH_ERRORS
+}
+
 // init({name: address}): the entry points to call.
 PyObject* init(PyObject*, PyObject* d) {
   auto get = [&](const char* name) -> void* {
@@ -305,6 +539,12 @@ PyObject* init(PyObject*, PyObject* d) {
   NDL_TAKE(p_prefill_split, "ndl_varlen_prefill_split");
   NDL_TAKE(p_rms_norm, "ndl_rms_norm");
   NDL_TAKE(p_silu_mul, "ndl_silu_mul");
+  NDL_TAKE(p_kv_append_fp8, "ndl_kv_append_fp8");
+  NDL_TAKE(p_kv_read_fp8, "ndl_kv_read_fp8");
+  NDL_TAKE(p_fp8_workspace, "ndl_fp8_attention_workspace_bytes");
+  NDL_TAKE(p_fp8_attention, "ndl_fp8_attention");
+  NDL_TAKE(p_verify_workspace, "ndl_verify_drafts_workspace_bytes");
+  NDL_TAKE(p_verify_drafts, "ndl_verify_drafts");
 #undef NDL_TAKE
   Py_RETURN_NONE;
 }
@@ -315,6 +555,10 @@ PyMethodDef methods[] = {
     {"varlen_prefill", (PyCFunction)(void (*)(void))varlen_prefill, METH_FASTCALL, nullptr},
     {"rms_norm", (PyCFunction)(void (*)(void))rms_norm, METH_FASTCALL, nullptr},
     {"silu_mul", (PyCFunction)(void (*)(void))silu_mul, METH_FASTCALL, nullptr},
+    {"kv_append_fp8", (PyCFunction)(void (*)(void))kv_append_fp8, METH_FASTCALL, nullptr},
+    {"kv_read_fp8", (PyCFunction)(void (*)(void))kv_read_fp8, METH_FASTCALL, nullptr},
+    {"fp8_attention", (PyCFunction)(void (*)(void))fp8_attention, METH_FASTCALL, nullptr},
+    {"verify_drafts", (PyCFunction)(void (*)(void))verify_drafts, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods,

@@ -816,6 +816,11 @@ def kv_append_fp8(k: torch.Tensor, v: torch.Tensor, kv_codes: torch.Tensor,
     is given: then the rotated q is returned (written to out, contiguous, if that is given).
     cu_seqlens None: one token per sequence.
     """
+    if out is None and _lib.NATIVE is not None:
+        done = _lib.NATIVE.kv_append_fp8(k, v, kv_codes, kv_scales, block_table, context_lens,
+                                         cu_seqlens, q, cos, sin)
+        if done is not None:
+            return None if q is None else done
     nb, hkv, bs, d = _check_fp8_cache(kv_codes, kv_scales)
     dev, dtype = kv_codes.device, k.dtype
     _check_16bit("k", dtype)
@@ -877,6 +882,11 @@ def kv_read_fp8(kv_codes: torch.Tensor, kv_scales: torch.Tensor, block_table: to
     the tokens first[i], first[i] + 1, .. of each sequence.  bfloat16 has every value of the pool
     exactly; float16 every one that came from a float16 row, but for its smallest subnormals.
     first: int32 [num_seqs].  Rows outside cu_seqlens hold nothing in particular."""
+    if _lib.NATIVE is not None:
+        done = _lib.NATIVE.kv_read_fp8(kv_codes, kv_scales, block_table, first, cu_seqlens,
+                                       num_tokens, _DTYPES.get(dtype))
+        if done is not None:
+            return done
     nb, hkv, bs, d = _check_fp8_cache(kv_codes, kv_scales)
     dev = kv_codes.device
     _check_16bit("dtype", dtype)
@@ -901,6 +911,12 @@ def kv_read_fp8(kv_codes: torch.Tensor, kv_scales: torch.Tensor, block_table: to
 
 def _fp8_attention(q, kv_codes, kv_scales, block_table, cu_seqlens, context_lens, max_seqlen,
                    max_keys, scale, num_heads, num_kv_heads, head_dim, out, workspace):
+    if out is None and workspace is None and _lib.NATIVE is not None:
+        out = _lib.NATIVE.fp8_attention(q, kv_codes, kv_scales, block_table, cu_seqlens,
+                                        context_lens, max_seqlen, max_keys, scale, num_heads,
+                                        num_kv_heads, head_dim)
+        if out is not None:
+            return out
     nb, hkv, bs, d = _check_fp8_cache(kv_codes, kv_scales)
     dev = kv_codes.device
     _require(hkv == num_kv_heads and d == head_dim, "kv_codes shape disagrees with head counts")
@@ -1005,6 +1021,11 @@ def verify_drafts(logits: torch.Tensor, ids: torch.Tensor, cu_seqlens: torch.Ten
     temperature float32 [num_seqs] (None: 1); 0 takes the argmax, as does a row whose maximum is
     not finite.  uniforms float32 [T] in [0, 1).  tokens, in ids' type: the accepted drafts, the
     next token, then -1.  Graph-capturable; no host synchronisation."""
+    if _lib.NATIVE is not None:
+        done = _lib.NATIVE.verify_drafts(logits, ids, cu_seqlens, uniforms, temperature,
+                                         draft_probs)
+        if done is not None:
+            return done
     _require(logits.is_cuda, "logits must be a GPU tensor")
     if logits.dtype not in _DTYPES:
         raise TypeError(f"unsupported dtype {logits.dtype}")
