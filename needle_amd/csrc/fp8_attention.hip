@@ -745,7 +745,7 @@ __device__ __forceinline__ Chunk chunk_of_seq(const UnpackArgs& a, int seq) {
 // the causal mask's 0 * NaN would bring it to those before it too.
 template <int D, bool F16>
 __global__ __launch_bounds__(256) void chunk_unpack_kernel(UnpackArgs a) {
-  constexpr int CPR = D / 16, RPL = 64 / CPR;    // lanes per row, rows per load
+  constexpr int LPR = D / 8, RPL = 64 / LPR;     // lanes per row (8 codes each), rows per load
   const int lane = threadIdx.x & 63, seq = blockIdx.y, Hkv = a.num_kv_heads;
   const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const Chunk ch = chunk_of_seq(a, seq);
@@ -759,7 +759,7 @@ __global__ __launch_bounds__(256) void chunk_unpack_kernel(UnpackArgs a) {
     a.lens[seq] = ch.pos < 0 ? 0 : (int32_t)ch.pos;
     row[a.cols] = -1;
   }
-  const int r = lane / CPR;
+  const int r = lane / LPR;
   for (int64_t item = (int64_t)blockIdx.x * 4 + wv; item < items; item += (int64_t)gridDim.x * 4) {
     const int64_t tile = item / (2 * Hkv);
     const int ph = (int)(item - tile * 2 * Hkv), plane = ph >= Hkv, head = ph - plane * Hkv;
@@ -773,27 +773,24 @@ __global__ __launch_bounds__(256) void chunk_unpack_kernel(UnpackArgs a) {
     if (!ok) continue;
     const int64_t from = (plane ? a.plane_rows : 0) + (((int64_t)b * Hkv + head) << bshift) + in_block;
     u16* const dst = a.pool + ((plane ? a.pool_rows : 0) + ((block * Hkv + head) << bshift) +
-                               in_block) * D + lane * 16;
-    u32x4 c[16 / RPL];
+                               in_block) * D + lane * 8;
+    u32x2 c[16 / RPL];
     float scale[16 / RPL];
 #pragma unroll
     for (int x = 0; x < 16 / RPL; ++x) {
-      c[x] = ldg16(a.codes + from * D + x * 1024 + lane * 16);
+      c[x] = ld8(a.codes + from * D + x * 512 + lane * 8);
       scale[x] = __uint_as_float((uint32_t)a.scales[from + x * RPL + r] << 23);
     }
 #pragma unroll
     for (int x = 0; x < 16 / RPL; ++x) {
-      if (plane && 16 * tile + x * RPL + r >= ch.pos)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) c[x][i] &= ~nan_bytes(c[x][i]);
-      u32x4 o[2];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        o[i >> 1][2 * (i & 1)] = value2<F16, false>(c[x][i], scale[x]);
-        o[i >> 1][2 * (i & 1) + 1] = value2<F16, true>(c[x][i], scale[x]);
+      if (plane && 16 * tile + x * RPL + r >= ch.pos) {
+        c[x][0] &= ~nan_bytes(c[x][0]);
+        c[x][1] &= ~nan_bytes(c[x][1]);
       }
-      st16(dst + x * RPL * D, o[0]);
-      st16(dst + x * RPL * D + 8, o[1]);
+      st16(dst + x * 512, u32x4{value2<F16, false>(c[x][0], scale[x]),
+                                value2<F16, true>(c[x][0], scale[x]),
+                                value2<F16, false>(c[x][1], scale[x]),
+                                value2<F16, true>(c[x][1], scale[x])});
     }
   }
 }
@@ -811,18 +808,27 @@ __global__ __launch_bounds__(256) void chunk_nan_kernel(UnpackArgs a) {
   const Chunk ch = chunk_of_seq(a, seq);
   if (j0 >= ch.n) return;
   const int bshift = 4 + a.tile_shift;
-  int code[16][PER];
+  // a lane per token for its slot, then a row of codes at a time, none behind a branch
+  int64_t mine = -1;
+  if (lane < 16) {
+    const int64_t p = ch.pos + j0 + lane;
+    if (j0 + lane < ch.n && ch.pos >= 0 && p < ch.keys) {
+      const int b = a.block_table[(int64_t)seq * a.bt_row_stride + (p >> bshift)];
+      if (b >= 0 && b < a.num_blocks)
+        mine = (((int64_t)b * Hkv + head) << bshift) + (p & ((1 << bshift) - 1));
+    }
+  }
+  uint32_t code[16];
+  bool in[16];
 #pragma unroll
   for (int x = 0; x < 16; ++x) {
-    const int64_t p = ch.pos + j0 + x;
-    bool in = j0 + x < ch.n && p >= 0 && p < ch.keys;
-    const int b = in ? a.block_table[(int64_t)seq * a.bt_row_stride + (p >> bshift)] : -1;
-    in = in && b >= 0 && b < a.num_blocks;
-    const int64_t row = in ? a.plane_rows + (((int64_t)b * Hkv + head) << bshift) +
-                                 (p & ((1 << bshift) - 1))
-                           : 0;
-#pragma unroll
-    for (int e = 0; e < PER; ++e) code[x][e] = in ? a.codes[row * D + lane * PER + e] : 0;
+    const int row = __builtin_amdgcn_readlane((int)mine, x);    // plane_rows fits 31 bits
+    in[x] = row >= 0;
+    const uint8_t* const p = a.codes + (a.plane_rows + (in[x] ? row : 0)) * D + lane * PER;
+    if constexpr (PER == 2)
+      code[x] = *reinterpret_cast<const uint16_t*>(p);
+    else
+      code[x] = *p;
   }
   int first[PER];
 #pragma unroll
@@ -830,7 +836,7 @@ __global__ __launch_bounds__(256) void chunk_nan_kernel(UnpackArgs a) {
     first[e] = 16;
 #pragma unroll
     for (int x = 15; x >= 0; --x)
-      if ((code[x][e] & 0x7f) == 0x7f) first[e] = x;
+      if (in[x] && ((code[x] >> (8 * e)) & 0x7f) == 0x7f) first[e] = x;
   }
   bool any = false;
 #pragma unroll
@@ -871,8 +877,8 @@ bool unpacked_plan(int64_t num_seqs, int64_t num_tokens, int max_seqlen, int64_t
   u->lens_bytes = ((size_t)num_seqs * 4 + 255) / 256 * 256;
   u->pool_bytes = ((size_t)bytes + 255) / 256 * 256;
   u->prefill_bytes =
-      ndl_varlen_prefill_workspace_bytes((int)num_seqs, num_tokens, max_seqlen, u->cols + 1,
-                                         num_heads, num_kv_heads, head_dim, block_size, NDL_DTYPE_BF16);
+      prefill_rounds_workspace_bytes((int)num_seqs, num_tokens, max_seqlen, u->cols + 1, num_heads,
+                                     num_kv_heads, head_dim, block_size);
   return true;
 }
 
@@ -899,9 +905,9 @@ int launch_unpacked(const ChunkArgs& c, const Unpacked& u, int max_seqlen, int64
   a.context_lens = c.context_lens;
   a.num_tokens = c.num_tokens;
   a.out = c.out;
-  // workgroups of a sequence: 2,048 over all sequences, no more than its items can use
+  // workgroups of a sequence: what the longest can use, 16,384 over all sequences
   const int64_t items = (max_keys + 15) / 16 * 2 * c.num_kv_heads;
-  int64_t wgs = (2048 + c.num_seqs - 1) / c.num_seqs;
+  int64_t wgs = (16384 + c.num_seqs - 1) / c.num_seqs;
   if (wgs > (items + 3) / 4) wgs = (items + 3) / 4;
   hipLaunchKernelGGL((chunk_unpack_kernel<D, F16>), dim3((unsigned)wgs, (unsigned)c.num_seqs),
                      dim3(256), 0, s, a);
@@ -910,11 +916,10 @@ int launch_unpacked(const ChunkArgs& c, const Unpacked& u, int max_seqlen, int64
   // (the prefill sizes its split by the table, in the call as in the workspace query)
   const int64_t cached = (int64_t)(u.cols + 1) * block_size;
   void* const ws = u.prefill_bytes ? (char*)workspace + u.total() - u.prefill_bytes : nullptr;
-  rc = ndl_varlen_prefill_split(c.out, c.q, c.q_stride, nullptr, nullptr, 0, a.pool, u.blocks,
-                                a.table, u.cols + 1, u.cols + 1, c.cu_seqlens, a.lens, c.num_seqs,
-                                c.num_tokens, max_seqlen, (int)cached, c.num_heads,
-                                c.num_kv_heads, D, block_size, F16 ? NDL_DTYPE_F16 : NDL_DTYPE_BF16,
-                                scale, ws, u.prefill_bytes, s);
+  rc = launch_prefill_rounds(c.out, c.q, c.q_stride, a.pool, u.blocks, a.table, u.cols + 1,
+                             u.cols + 1, c.cu_seqlens, a.lens, c.num_seqs, c.num_tokens, max_seqlen,
+                             (int)cached, c.num_heads, c.num_kv_heads, D, block_size,
+                             F16 ? NDL_DTYPE_F16 : NDL_DTYPE_BF16, scale, ws, u.prefill_bytes, s);
   if (rc != NDL_OK) return rc;
   const int64_t scan = ((int64_t)(max_seqlen + 15) / 16 * c.num_kv_heads + 3) / 4;
   hipLaunchKernelGGL((chunk_nan_kernel<D>), dim3((unsigned)scan, (unsigned)c.num_seqs), dim3(256),

@@ -183,11 +183,12 @@ __device__ __forceinline__ uint32_t value2(uint32_t w, float scale) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, HI));
 }
 
-// One wave per (token, round of 64 items); an item is 16 codes of one of the token's 2 Hkv rows.
+// One wave per (token, round of 64 items); an item is 8 codes of one of the token's 2 Hkv rows
+// (16 bytes written: a wave stores 1 KiB at once).
 // Positions that have no slot read as zeros, tokens past the last sequence are not written.
 template <int D, bool F16>
 __global__ __launch_bounds__(256) void kv_read_fp8_kernel(QuantArgs a) {
-  constexpr int CPR = D / 16;
+  constexpr int CPR = D / 8;
   const int lane = threadIdx.x & 63;
   const int64_t w =
       (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -198,25 +199,19 @@ __global__ __launch_bounds__(256) void kv_read_fp8_kernel(QuantArgs a) {
   if (t < (int64_t)a.cu_seqlens[0] || t >= (int64_t)a.cu_seqlens[a.num_seqs]) return;
   const int64_t slot = slot_row(a, t);
   if (item >= items) return;
-  const int row = item / CPR, d0 = 16 * (item - row * CPR);
+  const int row = item / CPR, d0 = 8 * (item - row * CPR);
   const bool is_v = row >= Hkv;
   const int h = is_v ? row - Hkv : row;
-  u32x4 c{0u, 0u, 0u, 0u};
+  u32x2 c{0u, 0u};
   float scale = 1.f;
   if (slot >= 0) {
     const int64_t at = (is_v ? a.plane_rows : 0) + slot + ((int64_t)h << a.block_shift);
-    c = ld16(a.codes + at * D + d0);
+    c = ld8(a.codes + at * D + d0);
     scale = __uint_as_float((uint32_t)a.scales[at] << 23);
   }
   u16* const dst = (is_v ? a.v_out : a.k_out) + (t * Hkv + h) * D + d0;
-  u32x4 o[2];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    o[i >> 1][2 * (i & 1)] = value2<F16, false>(c[i], scale);
-    o[i >> 1][2 * (i & 1) + 1] = value2<F16, true>(c[i], scale);
-  }
-  st16(dst, o[0]);
-  st16(dst + 8, o[1]);
+  st16(dst, u32x4{value2<F16, false>(c[0], scale), value2<F16, true>(c[0], scale),
+                  value2<F16, false>(c[1], scale), value2<F16, true>(c[1], scale)});
 }
 
 int log2_of(int block_size) {
@@ -338,7 +333,7 @@ extern "C" int ndl_kv_read_fp8(void* k_out, void* v_out, const void* codes, cons
   a.num_tokens = num_tokens;
   a.k_out = (u16*)k_out;
   a.v_out = (u16*)v_out;
-  const int64_t rounds = (2 * num_kv_heads * (head_dim / 16) + 63) / 64;
+  const int64_t rounds = (2 * num_kv_heads * (head_dim / 8) + 63) / 64;
   const int64_t blocks = (num_tokens * rounds + 3) / 4;
   if (blocks > 0x7fffffff) return NDL_ERR_INVALID_ARG;
   const dim3 grid((unsigned)blocks), wg(256);

@@ -1230,8 +1230,13 @@ struct PrefillSplit {
   int64_t takers;
   size_t plan_bytes, ml_bytes, bytes;
 };
+// rounds: also where whole tiles fill the GPU but for their last round (a caller whose prefixes
+// are long and uneven, whose tiles differ as much): the split is taken from a fifth of idle places
+// on.  us split / whole, 28/4 heads of 128, after uneven prefixes of 2,048 to 8,192: 336 places'
+// tiles (two rounds of 256) 243 / 322.
 inline bool prefill_split(int num_seqs, int64_t num_tokens, int64_t qtiles, int num_heads,
-                          int num_kv_heads, int head_dim, int64_t max_tiles, PrefillSplit* sp) {
+                          int num_kv_heads, int head_dim, int64_t max_tiles, bool rounds,
+                          PrefillSplit* sp) {
   const int64_t tiles = num_seqs * qtiles;   // of the plan: an upper bound per kv head
   if (tiles > kPrefSplitTiles || max_tiles * 16 < NDL_PREFILL_SPLIT_MIN_KEYS ||
       max_tiles > (1 << 20))
@@ -1242,7 +1247,12 @@ inline bool prefill_split(int num_seqs, int64_t num_tokens, int64_t qtiles, int 
   if (sp->takers < 2) return false;
   // workgroups whole tiles would keep busy: eight 32-row jobs each
   const int64_t busy = (num_tokens / kPrefRows + num_seqs) * num_heads / kPrefWaves;
-  if (busy >= slots || max_tiles / 2 * (slots - busy) < kPrefSplitGain * slots) return false;
+  if (busy >= slots) {
+    const int64_t places = (busy + slots - 1) / slots * slots;
+    if (!rounds || places * 5 < busy * 6) return false;
+  } else if (max_tiles / 2 * (slots - busy) < kPrefSplitGain * slots) {
+    return false;
+  }
   const size_t n = (size_t)2 * sp->takers * num_kv_heads * kPrefWaves * 64;   // lanes
   sp->plan_bytes = ((2 + (size_t)tiles) * sizeof(int32_t) + 255) & ~(size_t)255;
   sp->ml_bytes = n * 2 * sizeof(float);
@@ -1260,7 +1270,7 @@ static int launch_prefill(void* out, const void* q, int64_t q_tok_stride, const 
                           int max_seqlen, int max_context_len, int num_heads, int num_kv_heads,
                           int head_dim, int block_size, int dtype, float scale,
                           ndl_stream_t stream, void* workspace = nullptr,
-                          size_t workspace_bytes = 0) {
+                          size_t workspace_bytes = 0, bool rounds = false) {
   if (!dtype_known(dtype)) return NDL_ERR_UNSUPPORTED;
   const int tshift = block_tile_shift(block_size);
   if (tshift < 0 || (head_dim != 64 && head_dim != 128)) return NDL_ERR_UNSUPPORTED;
@@ -1334,7 +1344,7 @@ static int launch_prefill(void* out, const void* q, int64_t q_tok_stride, const 
   if (workspace != nullptr && ((uintptr_t)workspace & 15u) == 0 && !any_scale &&
       prefill_split(num_seqs, num_tokens, qtiles, num_heads, num_kv_heads, head_dim,
                     longest_tiles(max_blocks_per_seq, block_size, max_context_len, max_seqlen),
-                    &sp) &&
+                    rounds, &sp) &&
       workspace_bytes >= sp.bytes) {
     a.takers = (int)sp.takers;
     a.ws_plan = (int32_t*)workspace;
@@ -1418,11 +1428,11 @@ extern "C" int ndl_rope_varlen_prefill(void* out, const void* q, int64_t q_tok_s
                              dtype, scale, stream);
 }
 
-extern "C" size_t ndl_varlen_prefill_workspace_bytes(int num_seqs, int64_t num_tokens,
-                                                     int max_seqlen, int max_blocks_per_seq,
-                                                     int num_heads, int num_kv_heads,
-                                                     int head_dim, int block_size, int dtype) {
-  using namespace ndl;
+namespace ndl {
+
+static size_t prefill_workspace(int num_seqs, int64_t num_tokens, int max_seqlen,
+                                int max_blocks_per_seq, int num_heads, int num_kv_heads,
+                                int head_dim, int block_size, int dtype, bool rounds) {
   const int tshift = block_tile_shift(block_size);
   if (!dtype_supported(dtype) || tshift < 0 || (head_dim != 64 && head_dim != 128) ||
       num_seqs <= 0 || num_tokens <= 0 || max_seqlen <= 0 || max_blocks_per_seq <= 0 ||
@@ -1432,9 +1442,40 @@ extern "C" size_t ndl_varlen_prefill_workspace_bytes(int num_seqs, int64_t num_t
                               (num_heads / num_kv_heads) + kPrefWaves - 1) / kPrefWaves;
   PrefillSplit sp;
   return prefill_split(num_seqs, num_tokens, qtiles, num_heads, num_kv_heads, head_dim,
-                       (int64_t)max_blocks_per_seq << tshift, &sp)
+                       (int64_t)max_blocks_per_seq << tshift, rounds, &sp)
              ? sp.bytes
              : 0;
+}
+
+size_t prefill_rounds_workspace_bytes(int num_seqs, int64_t num_tokens, int max_seqlen,
+                                      int max_blocks_per_seq, int num_heads, int num_kv_heads,
+                                      int head_dim, int block_size) {
+  return prefill_workspace(num_seqs, num_tokens, max_seqlen, max_blocks_per_seq, num_heads,
+                           num_kv_heads, head_dim, block_size, NDL_DTYPE_BF16, true);
+}
+
+int launch_prefill_rounds(void* out, const void* q, int64_t q_tok_stride, const void* kv_cache,
+                          int64_t num_blocks, const int32_t* block_table, int64_t bt_row_stride,
+                          int max_blocks_per_seq, const int32_t* cu_seqlens,
+                          const int32_t* context_lens, int num_seqs, int64_t num_tokens,
+                          int max_seqlen, int max_context_len, int num_heads, int num_kv_heads,
+                          int head_dim, int block_size, int dtype, float scale, void* workspace,
+                          size_t workspace_bytes, ndl_stream_t stream) {
+  return launch_prefill(out, q, q_tok_stride, nullptr, nullptr, 0, kv_cache, num_blocks,
+                        block_table, bt_row_stride, max_blocks_per_seq, cu_seqlens, context_lens,
+                        num_seqs, num_tokens, max_seqlen, max_context_len, num_heads, num_kv_heads,
+                        head_dim, block_size, dtype, scale, stream, workspace, workspace_bytes,
+                        true);
+}
+
+}  // namespace ndl
+
+extern "C" size_t ndl_varlen_prefill_workspace_bytes(int num_seqs, int64_t num_tokens,
+                                                     int max_seqlen, int max_blocks_per_seq,
+                                                     int num_heads, int num_kv_heads,
+                                                     int head_dim, int block_size, int dtype) {
+  return ndl::prefill_workspace(num_seqs, num_tokens, max_seqlen, max_blocks_per_seq, num_heads,
+                                num_kv_heads, head_dim, block_size, dtype, false);
 }
 
 extern "C" int ndl_varlen_prefill_split(void* out, const void* q, int64_t q_tok_stride,
