@@ -99,78 +99,99 @@ __device__ __forceinline__ u32x2 quant8(const u32x4& w, float mul) {
   return u32x2{(uint32_t)a, (uint32_t)b};
 }
 
-// One wave per (token, round of 64 items); an item is 8 elements of a row's first half and the 8
-// they rotate with, so D / 16 lanes hold a row and its maximum is a butterfly over them.  A
-// token's items are the 2 Hkv rows of K and V, then the H rows of q.  As in rope_append.hip the
-// loads go out first, then the slot is looked up; lanes past the last item load a valid one
-// again and store nothing.
+// One wave per (token, kRounds rounds of 64 items); an item is 8 elements of a row's first half and
+// the 8 they rotate with, so D / 16 lanes hold a row and its maximum is a butterfly over them, and
+// a lane's elements of cos and sin are the same in every round.  A token's items are the 2 Hkv
+// rows of K and V, then the H rows of q.  All loads go out first, then the slot is looked up; what
+// lies past the last item loads a valid one again and stores nothing.
+constexpr int kRounds = 2;
+
 template <int D, bool F16>
 __global__ __launch_bounds__(256) void kv_append_fp8_kernel(QuantArgs a) {
-  constexpr int CPH = D / 16, HALF = D / 2;
+  constexpr int CPH = D / 16, HALF = D / 2, RPR = 64 / CPH;    // rows per round
   const int lane = threadIdx.x & 63;
   const int64_t w =
       (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const int H = a.num_heads, Hkv = a.num_kv_heads;
-  const int kv_items = 2 * Hkv * CPH, q_items = a.q ? H * CPH : 0;
-  const int kv_rounds = (kv_items + 63) >> 6, rounds = kv_rounds + ((q_items + 63) >> 6);
-  const int64_t t = w / rounds;
-  const int r = (int)(w - t * rounds);
+  const int H = a.q ? a.num_heads : 0, Hkv = a.num_kv_heads;
+  const int kv_rounds = (2 * Hkv + RPR - 1) / RPR, rounds = kv_rounds + (H + RPR - 1) / RPR;
+  const int groups = (rounds + kRounds - 1) / kRounds;
+  const int64_t t = w / groups;
+  const int r0 = (int)(w - t * groups) * kRounds;
   if (t >= a.num_tokens) return;
-  const bool kv = r < kv_rounds;
-  const int items = kv ? kv_items : q_items;
-  const int item0 = 64 * (kv ? r : r - kv_rounds) + lane;
-  const bool live = item0 < items;
-  const int item = live ? item0 : items - 1;
-  const int row = item / CPH, d0 = 8 * (item - row * CPH);
-  const bool is_v = kv && row >= Hkv;
-  const int h = is_v ? row - Hkv : row;
-  const u16* src = kv ? (is_v ? a.v + t * a.v_stride : a.k + t * a.k_stride)
-                      : a.q + t * a.q_stride;
-  src += h * D + d0;
-  u32x4 lo = ld16(src), hi = ld16(src + HALF);
-  if (a.cos != nullptr) {
+  const int d0 = 8 * (lane % CPH);
+  u32x4 lo[kRounds], hi[kRounds], clo, chi, slo, shi;
+  const bool rope = a.cos != nullptr;
+#pragma unroll
+  for (int i = 0; i < kRounds; ++i) {
+    const int r = r0 + i < rounds ? r0 + i : rounds - 1;
+    const bool kv = r < kv_rounds;
+    const int rows = kv ? 2 * Hkv : H;
+    int row = (kv ? r : r - kv_rounds) * RPR + lane / CPH;
+    if (row >= rows) row = rows - 1;
+    const u16* src = kv ? (row >= Hkv ? a.v + t * a.v_stride - (int64_t)Hkv * D
+                                      : a.k + t * a.k_stride)
+                        : a.q + t * a.q_stride;
+    src += (int64_t)row * D + d0;
+    lo[i] = ld16(src);
+    hi[i] = ld16(src + HALF);
+  }
+  if (rope) {
     const u16 *cs = a.cos + t * a.cs_stride + d0, *sn = a.sin + t * a.cs_stride + d0;
-    const u32x4 clo = ld16(cs), chi = ld16(cs + HALF), slo = ld16(sn), shi = ld16(sn + HALF);
-    u32x4 rlo, rhi;
-    rope8<F16>(lo, hi, clo, chi, slo, shi, rlo, rhi);
-    if (!is_v) {
-      lo = rlo;
-      hi = rhi;
-    }
+    clo = ld16(cs);
+    chi = ld16(cs + HALF);
+    slo = ld16(sn);
+    shi = ld16(sn + HALF);
   }
-  if (!kv) {
-    if (live) {
-      u16* const dst = a.q_out + (t * H + row) * D + d0;
-      st16(dst, lo);
-      st16(dst + HALF, hi);
-    }
-    return;
-  }
-  const int64_t slot = slot_row(a, t);
-  constexpr uint32_t inf = F16 ? 0x7c00u : 0x7f80u;
-  uint32_t m = 0;
+  const int64_t slot = r0 < kv_rounds ? slot_row(a, t) : -1;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t x = finite_max(lo[i], inf), y = finite_max(hi[i], inf);
-    m = m > x ? m : x;
-    m = m > y ? m : y;
-  }
+  for (int i = 0; i < kRounds; ++i) {
+    const int r = r0 + i;
+    if (r >= rounds) return;
+    const bool kv = r < kv_rounds;
+    const int row = (kv ? r : r - kv_rounds) * RPR + lane / CPH;
+    const bool live = row < (kv ? 2 * Hkv : H), is_v = kv && row >= Hkv;
+    if (rope) {
+      u32x4 rlo, rhi;
+      rope8<F16>(lo[i], hi[i], clo, chi, slo, shi, rlo, rhi);
+      if (!is_v) {
+        lo[i] = rlo;
+        hi[i] = rhi;
+      }
+    }
+    if (!kv) {
+      if (live) {
+        u16* const dst = a.q_out + (t * H + row) * D + d0;
+        st16(dst, lo[i]);
+        st16(dst + HALF, hi[i]);
+      }
+      continue;
+    }
+    constexpr uint32_t inf = F16 ? 0x7c00u : 0x7f80u;
+    uint32_t m = 0;
 #pragma unroll
-  for (int o = 1; o < CPH; o <<= 1) {
-    const uint32_t x = (uint32_t)__shfl_xor((int)m, o, 64);
-    m = m > x ? m : x;
-  }
-  // 448 = 1.75 * 2^8: the row's exponent less 8, one more where its mantissa is past 1.75
-  const uint32_t bits = __float_as_uint(Elt<F16>::lo(m));
-  const int e8 = (int)(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
-  const int byte = e8 < 1 ? 1 : e8;
-  const float mul = __uint_as_float((uint32_t)(254 - byte) << 23);
-  if (live && slot >= 0) {
-    const int64_t at = (is_v ? a.plane_rows : 0) + slot + ((int64_t)h << a.block_shift);
-    uint8_t* const dst = a.codes + at * D + d0;
-    *reinterpret_cast<u32x2*>(dst) = quant8<F16>(lo, mul);
-    *reinterpret_cast<u32x2*>(dst + HALF) = quant8<F16>(hi, mul);
-    if (d0 == 0) a.scales[at] = (uint8_t)byte;
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t x = finite_max(lo[i][e], inf), y = finite_max(hi[i][e], inf);
+      m = m > x ? m : x;
+      m = m > y ? m : y;
+    }
+#pragma unroll
+    for (int o = 1; o < CPH; o <<= 1) {
+      const uint32_t x = (uint32_t)__shfl_xor((int)m, o, 64);
+      m = m > x ? m : x;
+    }
+    // 448 = 1.75 * 2^8: the row's exponent less 8, one more where its mantissa is past 1.75
+    const uint32_t bits = __float_as_uint(Elt<F16>::lo(m));
+    const int e8 = (int)(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+    const int byte = e8 < 1 ? 1 : e8;
+    const float mul = __uint_as_float((uint32_t)(254 - byte) << 23);
+    if (live && slot >= 0) {
+      const int h = is_v ? row - Hkv : row;
+      const int64_t at = (is_v ? a.plane_rows : 0) + slot + ((int64_t)h << a.block_shift);
+      uint8_t* const dst = a.codes + at * D + d0;
+      *reinterpret_cast<u32x2*>(dst) = quant8<F16>(lo[i], mul);
+      *reinterpret_cast<u32x2*>(dst + HALF) = quant8<F16>(hi[i], mul);
+      if (d0 == 0) a.scales[at] = (uint8_t)byte;
+    }
   }
 }
 
@@ -183,35 +204,85 @@ __device__ __forceinline__ uint32_t value2(uint32_t w, float scale) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, HI));
 }
 
-// One wave per (token, round of 64 items); an item is 8 codes of one of the token's 2 Hkv rows
-// (16 bytes written: a wave stores 1 KiB at once).
+constexpr int kReadItems = 512;   // 8-code items a wave has in flight: 4 KiB of codes, 8 KiB out
+
+// The slot row of token t of a lane's own, as slot_row.  cu of up to 64 sequences is in the lanes
+// of `starts` (lane i: cu[i + 1]): the sequence is found by exchanges, without loads that wait for
+// one another.
+__device__ __forceinline__ int64_t slot_row_of_lane(const QuantArgs& a, int64_t t, int starts) {
+  const int n = a.num_seqs;
+  int i = 0;                       // sequences that end at or before t
+  if (n <= 64) {
+#pragma unroll
+    for (int step = 32; step >= 1; step >>= 1) {
+      const int probe = i + step - 1;
+      const int end = __shfl(starts, probe < 64 ? probe : 63, 64);
+      if (probe < n && end <= t) i += step;
+    }
+    // (64 sequences that all end before t: step 32 .. 1 sum to 63)
+    const int end = __shfl(starts, i < 64 ? i : 63, 64);
+    if (i < n && end <= t) ++i;
+  } else {
+    int lo = 0, hi = n;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (a.cu_seqlens[mid + 1] <= t) lo = mid + 1; else hi = mid;
+    }
+    i = lo;
+  }
+  if (i >= n) return -2;           // past the last sequence
+  const int first = a.cu_seqlens[i];
+  if (t < first) return -2;
+  const int64_t p = (int64_t)a.context_lens[i] + (t - first);
+  if (p < 0) return -1;
+  int64_t col = p >> a.block_shift;
+  if (col > a.max_blocks - 1) col = a.max_blocks - 1;
+  const int64_t b = a.block_table[(int64_t)i * a.bt_row_stride + col];
+  if (b < 0 || b >= a.num_blocks) return -1;
+  return ((b * a.num_kv_heads) << a.block_shift) + (p & ((1 << a.block_shift) - 1));
+}
+
+// One wave per kReadItems items of the packed tokens; an item is 8 codes of one of a token's
+// 2 Hkv rows, in the order of the tokens, so that a wave stores 1 KiB at once.  Lane k first finds the slot of the wave's k-th token.
 // Positions that have no slot read as zeros, tokens past the last sequence are not written.
 template <int D, bool F16>
 __global__ __launch_bounds__(256) void kv_read_fp8_kernel(QuantArgs a) {
-  constexpr int CPR = D / 8;
+  constexpr int CPR = D / 8, U = kReadItems / 64;
   const int lane = threadIdx.x & 63;
   const int64_t w =
       (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const int Hkv = a.num_kv_heads, items = 2 * Hkv * CPR, rounds = (items + 63) >> 6;
-  const int64_t t = w / rounds;
-  const int item = 64 * (int)(w - t * rounds) + lane;
-  if (t >= a.num_tokens) return;
-  if (t < (int64_t)a.cu_seqlens[0] || t >= (int64_t)a.cu_seqlens[a.num_seqs]) return;
-  const int64_t slot = slot_row(a, t);
-  if (item >= items) return;
-  const int row = item / CPR, d0 = 8 * (item - row * CPR);
-  const bool is_v = row >= Hkv;
-  const int h = is_v ? row - Hkv : row;
-  u32x2 c{0u, 0u};
-  float scale = 1.f;
-  if (slot >= 0) {
-    const int64_t at = (is_v ? a.plane_rows : 0) + slot + ((int64_t)h << a.block_shift);
-    c = ld8(a.codes + at * D + d0);
-    scale = __uint_as_float((uint32_t)a.scales[at] << 23);
+  const int Hkv = a.num_kv_heads, ipt = 2 * Hkv * CPR;     // items per token, at least 16
+  const int64_t item0 = w * kReadItems, tok0 = item0 / ipt;
+  if (tok0 >= a.num_tokens) return;
+  const int starts = a.cu_seqlens[lane < a.num_seqs ? lane + 1 : a.num_seqs];
+  const int64_t mine = slot_row_of_lane(a, tok0 + lane, starts);
+  const int off = (int)(item0 - tok0 * ipt);
+  const float inv = 1.f / (float)ipt;
+  u32x2 c[U];
+  float scale[U];
+  u16* dst[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int at = off + 64 * u + lane;                    // under 2^20: the quotient is exact
+    const int k = (int)(((float)at + 0.5f) * inv), item = at - k * ipt;
+    const int row = item / CPR, d0 = 8 * (item - row * CPR);
+    const bool is_v = row >= Hkv;
+    const int h = is_v ? row - Hkv : row;
+    const int64_t slot = __shfl(mine, k, 64);
+    const bool in = slot >= 0;
+    const int64_t src = in ? (is_v ? a.plane_rows : 0) + slot + ((int64_t)h << a.block_shift) : 0;
+    c[u] = ld8(a.codes + src * D + (in ? d0 : 0));
+    scale[u] = __uint_as_float((uint32_t)a.scales[src] << 23);
+    if (!in) c[u] = u32x2{0u, 0u};
+    dst[u] = slot == -2 || tok0 + k >= a.num_tokens
+                 ? nullptr
+                 : (is_v ? a.v_out : a.k_out) + ((tok0 + k) * Hkv + h) * D + d0;
   }
-  u16* const dst = (is_v ? a.v_out : a.k_out) + (t * Hkv + h) * D + d0;
-  st16(dst, u32x4{value2<F16, false>(c[0], scale), value2<F16, true>(c[0], scale),
-                  value2<F16, false>(c[1], scale), value2<F16, true>(c[1], scale)});
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (dst[u] != nullptr)
+      st16(dst[u], u32x4{value2<F16, false>(c[u][0], scale[u]), value2<F16, true>(c[u][0], scale[u]),
+                         value2<F16, false>(c[u][1], scale[u]), value2<F16, true>(c[u][1], scale[u])});
 }
 
 int log2_of(int block_size) {
@@ -279,10 +350,10 @@ extern "C" int ndl_kv_append_fp8(void* codes, void* scales, int64_t num_blocks, 
   a.context_lens = context_lens;
   a.num_seqs = num_seqs;
   a.num_tokens = num_tokens;
-  const int64_t cph = head_dim / 16;
-  const int64_t rounds =
-      (2 * num_kv_heads * cph + 63) / 64 + (q ? (num_heads * cph + 63) / 64 : 0);
-  const int64_t blocks = (num_tokens * rounds + 3) / 4;
+  const int64_t rpr = 64 / (head_dim / 16);
+  const int64_t rounds = (2 * num_kv_heads + rpr - 1) / rpr + (q ? (num_heads + rpr - 1) / rpr : 0);
+  const int64_t groups = (rounds + kRounds - 1) / kRounds;
+  const int64_t blocks = (num_tokens * groups + 3) / 4;
   if (blocks > 0x7fffffff) return NDL_ERR_INVALID_ARG;
   const dim3 grid((unsigned)blocks), wg(256);
   const hipStream_t s = (hipStream_t)stream;
@@ -333,8 +404,9 @@ extern "C" int ndl_kv_read_fp8(void* k_out, void* v_out, const void* codes, cons
   a.num_tokens = num_tokens;
   a.k_out = (u16*)k_out;
   a.v_out = (u16*)v_out;
-  const int64_t rounds = (2 * num_kv_heads * (head_dim / 8) + 63) / 64;
-  const int64_t blocks = (num_tokens * rounds + 3) / 4;
+  const int64_t items = num_tokens * 2 * num_kv_heads * (head_dim / 8);
+  const int64_t blocks = (items + 4 * kReadItems - 1) / (4 * kReadItems);
+  if (num_kv_heads > 4096) return NDL_ERR_UNSUPPORTED;
   if (blocks > 0x7fffffff) return NDL_ERR_INVALID_ARG;
   const dim3 grid((unsigned)blocks), wg(256);
   const hipStream_t s = (hipStream_t)stream;
