@@ -60,12 +60,12 @@ struct ChunkArgs {
   int64_t num_tokens;
   int toks;                     // query tokens of a row block
   int blocks_per_seq;           // row blocks a sequence can have
-  int64_t items;                // num_seqs * blocks_per_seq
+  int items;                    // num_seqs * blocks_per_seq
   float scale_log2;
   // the split into equal shares (shares 0: a workgroup per row block)
   int shares;                   // per kv head
   int min_chunk;                // slots a share has at least
-  int64_t nseg;                 // segment slots per kv head: shares + items
+  int nseg;                     // segment slots per kv head: shares + items
   float* ws_ml;                 // [kv head][segment][column][2]
   float* ws_acc;                // [kv head][segment][column][D]
 };
@@ -84,10 +84,14 @@ struct Item {
   __device__ __forceinline__ int tiles() const { return (int)((keys() + kTile - 1) / kTile); }
 };
 
-__device__ __forceinline__ Item item_of(const ChunkArgs& a, int64_t e) {
+// The sequence of row block e (32-bit: a 64-bit division takes a hundred instructions).
+__device__ __forceinline__ int seq_of_item(const ChunkArgs& a, int e) {
+  return a.blocks_per_seq == 1 ? e : (int)((uint32_t)e / (uint32_t)a.blocks_per_seq);
+}
+__device__ __forceinline__ Item item_of(const ChunkArgs& a, int e) {
   Item it;
-  it.seq = (int)(e / a.blocks_per_seq);
-  const int j0 = (int)(e - (int64_t)it.seq * a.blocks_per_seq) * a.toks;
+  it.seq = seq_of_item(a, e);
+  const int j0 = (e - it.seq * a.blocks_per_seq) * a.toks;
   int64_t first = it.seq, count = 1;
   if (a.cu_seqlens != nullptr) {
     first = a.cu_seqlens[it.seq];
@@ -102,47 +106,55 @@ __device__ __forceinline__ Item item_of(const ChunkArgs& a, int64_t e) {
   return it;
 }
 
-__device__ __forceinline__ int slots_of(const ChunkArgs& a, int64_t e) {
+__device__ __forceinline__ int slots_of(const ChunkArgs& a, int e) {
   if (e >= a.items) return 0;
   const int n = item_of(a, e).tiles();
   return n > 0 ? n + kPad : 0;
 }
 
+// Inclusive prefix sum over the wave: by shifts within rows of 16 lanes, then the rows before.
+template <int PATTERN>
+__device__ __forceinline__ int dpp_add(int v) {
+  return v + __builtin_amdgcn_update_dpp(0, v, PATTERN, 0xf, 0xf, true);
+}
 __device__ __forceinline__ int wave_scan(int v, int lane) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int o = __shfl_up(v, d, 64);
-    if (lane >= d) v += o;
-  }
-  return v;
+  v = dpp_add<0x111>(v);         // row_shr:1, 0 from outside the row
+  v = dpp_add<0x112>(v);
+  v = dpp_add<0x114>(v);
+  v = dpp_add<0x118>(v);
+  const int r0 = __builtin_amdgcn_readlane(v, 15), r1 = __builtin_amdgcn_readlane(v, 31),
+            r2 = __builtin_amdgcn_readlane(v, 47);
+  return v + (lane >= 16 ? r0 : 0) + (lane >= 32 ? r1 : 0) + (lane >= 48 ? r2 : 0);
 }
 
-// The slots of all row blocks before e (of a kv head's stream) and of all of them.
+// All row blocks' slots of a kv head's stream, those before row block e, and the lanes' own
+// (slots, prefix) of the last 64 looked at: all of them where there are no more.
 struct StreamPos {
-  int64_t first, total;
+  int first, total;
+  int v, incl;
 };
-__device__ __forceinline__ StreamPos stream_pos(const ChunkArgs& a, int lane, int64_t e) {
-  StreamPos r{0, 0};
-  for (int64_t base = 0; base < a.items; base += 64) {
-    const int v = slots_of(a, base + lane);
-    const int incl = wave_scan(v, lane);
+__device__ __forceinline__ StreamPos stream_pos(const ChunkArgs& a, int lane, int e) {
+  StreamPos r{0, 0, 0, 0};
+  for (int base = 0; base < a.items; base += 64) {
+    r.v = slots_of(a, base + lane);
+    r.incl = wave_scan(r.v, lane);
     if (e >= base && e < base + 64)
-      r.first = r.total + __builtin_amdgcn_readlane(incl - v, (int)(e - base));
-    r.total += __builtin_amdgcn_readlane(incl, 63);
+      r.first = r.total + __builtin_amdgcn_readlane(r.incl - r.v, e - base);
+    r.total += __builtin_amdgcn_readlane(r.incl, 63);
   }
   return r;
 }
-__device__ __forceinline__ int64_t chunk_of(const ChunkArgs& a, int64_t total) {
-  const int64_t c = (total + a.shares - 1) / a.shares;
+__device__ __forceinline__ int chunk_of(const ChunkArgs& a, int total) {
+  const int c = (int)((uint32_t)(total + a.shares - 1) / (uint32_t)a.shares);
   return c < a.min_chunk ? a.min_chunk : c;
 }
 // The row block that holds slot `at`, its first slot in *first; a.items if there is none.
-__device__ __forceinline__ int64_t stream_find(const ChunkArgs& a, int lane, int64_t at,
-                                               int64_t* first) {
-  int64_t carry = 0;
-  for (int64_t base = 0; base < a.items; base += 64) {
-    const int v = slots_of(a, base + lane);
-    const int incl = wave_scan(v, lane);
+__device__ __forceinline__ int stream_find(const ChunkArgs& a, int lane, const StreamPos& p,
+                                           int at, int* first) {
+  int carry = 0;
+  for (int base = 0; base < a.items; base += 64) {
+    const int v = a.items <= 64 ? p.v : slots_of(a, base + lane);
+    const int incl = a.items <= 64 ? p.incl : wave_scan(v, lane);
     const uint64_t hit = __builtin_amdgcn_ballot_w64(v > 0 && carry + incl > at);
     if (hit) {
       const int l = __builtin_ctzll(hit);
@@ -218,9 +230,9 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void chunk_attention_kernel(ChunkA
   const int Hkv = a.num_kv_heads;
   const unsigned per8 = 8u * Hkv, grp = blockIdx.x / per8, in8 = blockIdx.x - grp * per8;
   const int head = (int)(in8 >> 3);
-  const int64_t unit = (int64_t)grp * 8 + (in8 & 7);
+  const int unit = (int)(grp * 8 + (in8 & 7));
 
-  int64_t e, first = 0, from = 0, to = 0;   // the row block, its first slot; the share's slots
+  int e, first = 0, from = 0, to = 0;   // the row block, its first slot; the share's slots
   const bool whole = a.shares == 0;
   if (whole) {
     e = unit;
@@ -228,11 +240,12 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void chunk_attention_kernel(ChunkA
   } else {
     if (unit >= a.shares) return;
     const StreamPos p = stream_pos(a, lane, -1);
-    const int64_t chunk = chunk_of(a, p.total);
+    const int chunk = chunk_of(a, p.total);
+    // (slots, and shares times a chunk past them, fit 31 bits: make_plan)
     from = unit * chunk;
     to = from + chunk < p.total ? from + chunk : p.total;
     if (from >= to) return;
-    e = stream_find(a, lane, from, &first);
+    e = stream_find(a, lane, p, from, &first);
   }
 
   const uint32_t swz = (uint32_t)((lane >> 3) * 128 + (((lane & 7) ^ (lane >> 3)) << 4));
@@ -242,7 +255,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void chunk_attention_kernel(ChunkA
   for (; e < a.items; ++e) {
     // This wave's tiles: t0 + wv, t0 + wv + NW, ..  Lane 2 u + s of a window holds the block id of
     // 16-token half s of the window's tile u (32 of the wave's tiles).
-    const int32_t* const table = a.block_table + (e / a.blocks_per_seq) * a.bt_row_stride;
+    const int32_t* const table = a.block_table + (int64_t)seq_of_item(a, e) * a.bt_row_stride;
     int t0 = 0, window;
     auto load_window = [&](int u0) {
       const int tt = 2 * (t0 + wv + NW * (u0 + (lane >> 1))) + (lane & 1);
@@ -257,9 +270,9 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void chunk_attention_kernel(ChunkA
     if (!whole) {
       if (ntiles == 0) continue;
       if (first >= to) break;
-      const int64_t base = first + kPad;
-      t0 = from > base ? (int)(from - base) : 0;
-      t1 = to < base + ntiles ? (int)(to - base) : ntiles;
+      const int base = first + kPad;
+      t0 = from > base ? from - base : 0;
+      t1 = to < base + ntiles ? to - base : ntiles;
       first = base + ntiles;
       if (t0 >= t1) continue;     // only the empty slot is this share's
       load_window(0);
@@ -604,103 +617,95 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void chunk_attention_kernel(ChunkA
   }
 }
 
-// One wave per (token, query head): the parts of its row block that the shares hold, combined in
-// their order; zeros for a token with nothing to attend.  A row block inside one share was
-// written by the attention.
+// One workgroup per (row block, kv head, kMergeCols columns): the parts that the shares hold,
+// combined in their order; zeros for tokens with nothing to attend.  A row block inside one share
+// was written by the attention.
+constexpr int kMergeCols = 8;
+constexpr int kMergeParts = 64;   // at a time
+
 template <int D, bool F16>
 __global__ __launch_bounds__(256) void chunk_merge_kernel(ChunkArgs a) {
   using T = Elt<F16>;
-  constexpr int PER = D / 64;
-  const int lane = threadIdx.x & 63;
-  const int64_t w =
-      (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const int64_t tok = w / a.num_heads;
-  const int h = (int)(w - tok * a.num_heads);
-  if (tok >= a.num_tokens) return;
-  int64_t e = tok, off = 0;
-  if (a.cu_seqlens != nullptr) {
-    if (tok < a.cu_seqlens[0] || tok >= a.cu_seqlens[a.num_seqs]) return;
-    int lo = 0, hi = a.num_seqs - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (a.cu_seqlens[mid] <= tok) lo = mid; else hi = mid - 1;
-    }
-    const int64_t jt = tok - a.cu_seqlens[lo], rb = jt / a.toks;
-    if (rb >= a.blocks_per_seq) return;    // past max_seqlen
-    e = (int64_t)lo * a.blocks_per_seq + rb;
-    off = jt - rb * a.toks;
-  }
-  const int kvh = h / a.group;
-  const int64_t col = off * a.group + (h - kvh * a.group);
+  constexpr int PER = kMergeCols * D / 256;       // consecutive outputs of a thread: 4 or 2
+  __shared__ float2 part[kMergeParts][kMergeCols];
+  const int t = threadIdx.x, lane = t & 63;
+  const int e = blockIdx.x, head = blockIdx.y, c0 = blockIdx.z * kMergeCols;
   const Item it = item_of(a, e);
-  if (it.n <= 0) return;
-  u16* const dst = a.out + (tok * a.num_heads + h) * D + lane * PER;
-  auto store = [&](const float (&o)[PER]) {
-    if constexpr (PER == 2)
-      *reinterpret_cast<uint32_t*>(dst) = T::pack(o[0], o[1]);
-    else
-      *dst = T::one(o[0]);
-  };
+  const StreamPos p = stream_pos(a, lane, e);
+  if (it.n <= 0 || c0 >= it.n * a.group) return;
+  const int cols = it.n * a.group - c0 < kMergeCols ? it.n * a.group - c0 : kMergeCols;
+  const int c = t * PER / D, d0 = t * PER - c * D;
   float o[PER];
 #pragma unroll
   for (int x = 0; x < PER; ++x) o[x] = 0.f;
   const int nt = it.tiles();
-  if (nt == 0) {
-    store(o);
-    return;
-  }
-  const StreamPos p = stream_pos(a, lane, e);
-  const int64_t chunk = chunk_of(a, p.total), base = p.first + kPad;
-  const int64_t s0 = base / chunk, s1 = (base + nt - 1) / chunk;
-  if (s0 == s1) return;
-  const int per = a.toks * a.group;
-  const int64_t seg = ((int64_t)kvh * a.nseg + s0 + e) * per + col;
-  const int n = (int)(s1 - s0 + 1);
-  const float* const ml = a.ws_ml + seg * 2;
-  const float* const src = a.ws_acc + seg * D + lane * PER;
-  // a lane per part for (m, l), 64 at a time; the first parts' outputs are loaded along with them
-  constexpr int kPre = 8;
-  const int64_t step = (int64_t)per * D;
-  float pre[kPre][PER];
+  if (nt > 0) {
+    const int chunk = chunk_of(a, p.total), base = p.first + kPad;
+    const int s0 = (int)((uint32_t)base / (uint32_t)chunk);
+    const int s1 = (int)((uint32_t)(base + nt - 1) / (uint32_t)chunk);
+    if (s0 == s1) return;
+    const int n = s1 - s0 + 1, per = a.toks * a.group;
+    const int64_t seg = ((int64_t)head * a.nseg + s0 + e) * per + c0;
+    const float2* const ml = reinterpret_cast<const float2*>(a.ws_ml) + seg;
+    const float* const src = a.ws_acc + seg * D + (int64_t)(c < cols ? c : 0) * D + d0;
+    // this thread's column's maximum over all parts, then 64 parts at a time
+    const int64_t step = (int64_t)per * D;
+    float mx = kNegInf, l = 0.f;
+    for (int pass = 0; pass < 2; ++pass) {
+      for (int i0 = 0; i0 < n; i0 += kMergeParts) {
+        const int m = n - i0 < kMergeParts ? n - i0 : kMergeParts;
+        if (pass == 0 || n > kMergeParts) {
+          __syncthreads();
+          for (int i = t; i < m * kMergeCols; i += 256)
+            if (i % kMergeCols < cols)
+              part[i / kMergeCols][i % kMergeCols] =
+                  ml[(int64_t)(i0 + i / kMergeCols) * per + i % kMergeCols];
+          __syncthreads();
+        }
+        if (c >= cols) continue;
+        if (pass == 0) {
+          for (int i = 0; i < m; ++i) mx = fmaxf(mx, part[i][c].x);
+          continue;
+        }
+        for (int i = 0; i < m; i += 8) {
+          float v[8][PER];
 #pragma unroll
-  for (int i = 0; i < kPre; ++i)
+          for (int y = 0; y < 8; ++y) {
+            const float* const q = src + (int64_t)(i0 + (i + y < m ? i + y : i)) * step;
+            if constexpr (PER == 4) {
+              const f32x4 w = *reinterpret_cast<const f32x4*>(q);
 #pragma unroll
-    for (int x = 0; x < PER; ++x) pre[i][x] = src[(i < n ? i : 0) * step + x];
-  const int mine = lane < n ? lane : n - 1;
-  f32x2 v = *reinterpret_cast<const f32x2*>(ml + (int64_t)mine * per * 2);
-  float mx = v[0];
-  for (int i = lane + 64; i < n; i += 64) mx = fmaxf(mx, ml[(int64_t)i * per * 2]);
+              for (int x = 0; x < PER; ++x) v[y][x] = w[x];
+            } else {
+              const f32x2 w = *reinterpret_cast<const f32x2*>(q);
+              v[y][0] = w[0];
+              v[y][1] = w[1];
+            }
+          }
 #pragma unroll
-  for (int x = 32; x >= 1; x >>= 1) mx = fmaxf(mx, xor_shfl(mx, x));
-  float l = 0.f;
-  for (int i0 = 0; i0 < n; i0 += 64) {
-    if (i0 > 0) v = *reinterpret_cast<const f32x2*>(
-                    ml + (int64_t)(i0 + lane < n ? i0 + lane : n - 1) * per * 2);
-    const float f = i0 + lane >= n ? 0.f : v[0] == mx ? 1.f : fast_exp2(v[0] - mx);
-    float part = v[1] * f;
+          for (int y = 0; y < 8; ++y) {
+            if (i + y >= m) break;
+            const float2 ms = part[i + y][c];
+            const float f = ms.x == mx ? 1.f : fast_exp2(ms.x - mx);
+            l += ms.y * f;
 #pragma unroll
-    for (int x = 32; x >= 1; x >>= 1) part += xor_shfl(part, x);
-    l += part;
-    const int m = n - i0 < 64 ? n - i0 : 64;
-    for (int i = 0; i < m; i += kPre) {
-      if (i0 + i > 0)
-#pragma unroll
-        for (int y = 0; y < kPre; ++y)
-#pragma unroll
-          for (int x = 0; x < PER; ++x) pre[y][x] = src[(i0 + i + y < n ? i0 + i + y : 0) * step + x];
-#pragma unroll
-      for (int y = 0; y < kPre; ++y) {
-        if (i + y >= m) break;
-        const float w = __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(f), i + y));
-#pragma unroll
-        for (int x = 0; x < PER; ++x) o[x] += pre[y][x] * w;
+            for (int x = 0; x < PER; ++x) o[x] += v[y][x] * f;
+          }
+        }
       }
     }
-  }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-  for (int x = 0; x < PER; ++x) o[x] *= inv;
-  store(o);
+    for (int x = 0; x < PER; ++x) o[x] *= inv;
+  }
+  if (c >= cols) return;
+  const int col = c0 + c, tok = col / a.group;
+  u16* const dst = a.out + ((it.tok0 + tok) * a.num_heads + head * a.group + col - tok * a.group) *
+                               (int64_t)D + d0;
+  if constexpr (PER == 4)
+    *reinterpret_cast<u32x2*>(dst) = u32x2{T::pack(o[0], o[1]), T::pack(o[2], o[3])};
+  else
+    *reinterpret_cast<uint32_t*>(dst) = T::pack(o[0], o[1]);
 }
 
 // ---------------------------------------------------------------- long chunks
@@ -965,7 +970,9 @@ Plan make_plan(int64_t num_seqs, int64_t max_seqlen, int64_t max_keys, int group
   p.items = num_seqs * p.blocks_per_seq;
   const int64_t tiles = (max_keys + kTile - 1) / kTile;
   const int64_t units = p.items * num_kv_heads;
-  const bool whole = tiles <= WHOLE_TILES || units >= 4 * resident;
+  // (slots and segments are counted in 31 bits)
+  const bool whole = tiles <= WHOLE_TILES || units >= 4 * resident ||
+                     p.items * (tiles + kPad) + 2 * resident * kMinChunk > 0x40000000;
   p.waves = whole && units * 2 <= resident ? WHOLE_WAVES : SHARE_WAVES;
   if (!whole) {
     int64_t s = resident / num_kv_heads / 8 * 8;
@@ -997,7 +1004,7 @@ Plan plan_for(int64_t num_seqs, int64_t max_seqlen, int64_t max_keys, int num_he
 
 template <int D, bool F16>
 int launch(ChunkArgs a, int nt, int waves, hipStream_t s) {
-  const int64_t units = a.shares ? a.shares : (a.items + 7) / 8 * 8;
+  const int64_t units = a.shares ? a.shares : ((int64_t)a.items + 7) / 8 * 8;
   const int64_t wgs = units * a.num_kv_heads;
   if (wgs > 0x7fffffff) return NDL_ERR_INVALID_ARG;
   void* args[] = {&a};
@@ -1006,9 +1013,11 @@ int launch(ChunkArgs a, int nt, int waves, hipStream_t s) {
     return NDL_ERR_LAUNCH;
   const int rc = check_launch();
   if (rc != NDL_OK || a.shares == 0) return rc;
-  const int64_t rows = a.num_tokens * a.num_heads, blocks = (rows + 3) / 4;
-  if (blocks > 0x7fffffff) return NDL_ERR_INVALID_ARG;
-  hipLaunchKernelGGL((chunk_merge_kernel<D, F16>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+  const int groups = (a.toks * a.group + kMergeCols - 1) / kMergeCols;
+  if (a.num_kv_heads > 65535) return NDL_ERR_UNSUPPORTED;
+  hipLaunchKernelGGL((chunk_merge_kernel<D, F16>),
+                     dim3((unsigned)a.items, (unsigned)a.num_kv_heads, (unsigned)groups), dim3(256),
+                     0, s, a);
   return check_launch();
 }
 
@@ -1096,7 +1105,7 @@ extern "C" int ndl_fp8_attention(void* out, const void* q, int64_t q_tok_stride,
                                             workspace, s);
   }
   const Plan p = plan_for(num_seqs, max_seqlen, max_keys, num_heads, num_kv_heads, head_dim);
-  if (p.blocks_per_seq > 0x7fffffff) return NDL_ERR_INVALID_ARG;
+  if (p.items > 0x7fffff00) return NDL_ERR_INVALID_ARG;
   if (p.shares) {
     if (!workspace || workspace_bytes < p.ml_bytes + p.acc_bytes || (uintptr_t)workspace & 255u)
       return NDL_ERR_WORKSPACE;
@@ -1105,11 +1114,11 @@ extern "C" int ndl_fp8_attention(void* out, const void* q, int64_t q_tok_stride,
   }
   a.toks = p.toks;
   a.blocks_per_seq = (int)p.blocks_per_seq;
-  a.items = p.items;
+  a.items = (int)p.items;
   a.scale_log2 = scale * kLog2e;
   a.shares = p.shares;
   a.min_chunk = kMinChunk;
-  a.nseg = p.nseg;
+  a.nseg = (int)p.nseg;
   if (head_dim == 128)
     return f16 ? launch<128, true>(a, p.nt, p.waves, s) : launch<128, false>(a, p.nt, p.waves, s);
   return f16 ? launch<64, true>(a, p.nt, p.waves, s) : launch<64, false>(a, p.nt, p.waves, s);
