@@ -130,16 +130,18 @@ __device__ __forceinline__ int wave_scan(int v, int lane) {
 // All row blocks' slots of a kv head's stream, those before row block e, and the lanes' own
 // (slots, prefix) of the last 64 looked at: all of them where there are no more.
 struct StreamPos {
-  int first, total;
+  int first, slots, total;      // of row block e: its first slot, its slots
   int v, incl;
 };
 __device__ __forceinline__ StreamPos stream_pos(const ChunkArgs& a, int lane, int e) {
-  StreamPos r{0, 0, 0, 0};
+  StreamPos r{0, 0, 0, 0, 0};
   for (int base = 0; base < a.items; base += 64) {
     r.v = slots_of(a, base + lane);
     r.incl = wave_scan(r.v, lane);
-    if (e >= base && e < base + 64)
+    if (e >= base && e < base + 64) {
       r.first = r.total + __builtin_amdgcn_readlane(r.incl - r.v, e - base);
+      r.slots = __builtin_amdgcn_readlane(r.v, e - base);
+    }
     r.total += __builtin_amdgcn_readlane(r.incl, 63);
   }
   return r;
@@ -638,7 +640,9 @@ __global__ __launch_bounds__(256) void chunk_merge_kernel(ChunkArgs a) {
   float o[PER];
 #pragma unroll
   for (int x = 0; x < PER; ++x) o[x] = 0.f;
-  const int nt = it.tiles();
+  // its tiles by the scan that gave its place: whatever the lengths are, or become while this
+  // runs, the shares are within the workspace
+  const int nt = p.slots > 0 ? p.slots - kPad : 0;
   if (nt > 0) {
     const int chunk = chunk_of(a, p.total), base = p.first + kPad;
     const int s0 = (int)((uint32_t)base / (uint32_t)chunk);
@@ -957,6 +961,8 @@ const void* kernel_of(int nt, int waves) {
 #define WHOLE_WAVES 8
 #define WHOLE_TILES 32
 #define MIN_CHUNK 8
+#define LONG_TILES 0
+#define ALWAYS8 0
 #endif
 constexpr int kMinChunk = MIN_CHUNK;
 
@@ -972,8 +978,9 @@ Plan make_plan(int64_t num_seqs, int64_t max_seqlen, int64_t max_keys, int group
   const int64_t units = p.items * num_kv_heads;
   // (slots and segments are counted in 31 bits)
   const bool whole = tiles <= WHOLE_TILES || units >= 4 * resident ||
+                     (units * 2 >= resident && tiles <= LONG_TILES) ||
                      p.items * (tiles + kPad) + 2 * resident * kMinChunk > 0x40000000;
-  p.waves = whole && units * 2 <= resident ? WHOLE_WAVES : SHARE_WAVES;
+  p.waves = whole && (units * 2 <= resident || (ALWAYS8)) ? WHOLE_WAVES : SHARE_WAVES;
   if (!whole) {
     int64_t s = resident / num_kv_heads / 8 * 8;
     if (s < 8) s = 8;

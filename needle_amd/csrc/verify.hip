@@ -633,6 +633,7 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(VerifyArgs a)
   const double less = a.probs && lane < ns ? a.left[(int64_t)i * ns + lane] : 0.0;
   if (n <= 0) return;
   const Info f = a.info[i];
+  if (f.accepted >= n) return;     // cu has changed since the launches before
   for (int j = t; j < n; j += kPickThreads)
     if (j != f.accepted) put_token(a, first + j, j < f.accepted ? draft_at(a, first + j + 1) : -1);
   if (t == 0) a.accepted[i] = f.accepted;
