@@ -38,7 +38,6 @@ namespace ndl {
 namespace {
 
 constexpr int kTile = 32;       // tokens per wave step
-constexpr int kPad = 1;         // empty slots before each row block (its start's cost)
 constexpr float kRaise = 8.f;   // log2 of the largest probability before the maximum is raised
 
 struct ChunkArgs {
@@ -65,6 +64,7 @@ struct ChunkArgs {
   // the split into equal shares (shares 0: a workgroup per row block)
   int shares;                   // per kv head
   int min_chunk;                // slots a share has at least
+  int pad;                      // empty slots before each row block: what its start costs
   int nseg;                     // segment slots per kv head: shares + items
   float* ws_ml;                 // [kv head][segment][column][2]
   float* ws_acc;                // [kv head][segment][column][D]
@@ -109,7 +109,7 @@ __device__ __forceinline__ Item item_of(const ChunkArgs& a, int e) {
 __device__ __forceinline__ int slots_of(const ChunkArgs& a, int e) {
   if (e >= a.items) return 0;
   const int n = item_of(a, e).tiles();
-  return n > 0 ? n + kPad : 0;
+  return n > 0 ? n + a.pad : 0;
 }
 
 // Inclusive prefix sum over the wave: by shifts within rows of 16 lanes, then the rows before.
@@ -127,47 +127,75 @@ __device__ __forceinline__ int wave_scan(int v, int lane) {
   return v + (lane >= 16 ? r0 : 0) + (lane >= 32 ? r1 : 0) + (lane >= 48 ? r2 : 0);
 }
 
-// All row blocks' slots of a kv head's stream, those before row block e, and the lanes' own
-// (slots, prefix) of the last 64 looked at: all of them where there are no more.
-struct StreamPos {
-  int first, slots, total;      // of row block e: its first slot, its slots
-  int v, incl;
+// The row blocks of a kv head laid end to end, in slots: their prefix sums, 64 to a step.  Up to
+// kHeld row blocks stay in registers, loaded at once; more are read again where they are needed.
+constexpr int kSteps = 4, kHeld = 64 * kSteps;
+// A share's begin moves to a row block's end within an eighth of a share of it: us without / a
+// sixteenth / an eighth, the decode step of 64 sequences of 512 to 4,096 tokens 55.3 / 54.6 / 53.3.
+constexpr int kSnap = 8;
+struct Place {
+  int e, first, slots;          // a row block, its first slot, how many it has
 };
-__device__ __forceinline__ StreamPos stream_pos(const ChunkArgs& a, int lane, int e) {
-  StreamPos r{0, 0, 0, 0, 0};
-  for (int base = 0; base < a.items; base += 64) {
-    r.v = slots_of(a, base + lane);
-    r.incl = wave_scan(r.v, lane);
-    if (e >= base && e < base + 64) {
-      r.first = r.total + __builtin_amdgcn_readlane(r.incl - r.v, e - base);
-      r.slots = __builtin_amdgcn_readlane(r.v, e - base);
+struct Stream {
+  int total, chunk, snap;
+  int v[kSteps], incl[kSteps];
+
+  __device__ __forceinline__ void read(const ChunkArgs& a, int lane) {
+    total = 0;
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) v[k] = 64 * k < a.items ? slots_of(a, 64 * k + lane) : 0;
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+      incl[k] = total;
+      if (64 * k < a.items) {
+        incl[k] = wave_scan(v[k], lane) + total;
+        total = __builtin_amdgcn_readlane(incl[k], 63);
+      }
     }
-    r.total += __builtin_amdgcn_readlane(r.incl, 63);
+    for (int base = kHeld; base < a.items; base += 64)
+      total += __builtin_amdgcn_readlane(wave_scan(slots_of(a, base + lane), lane), 63);
+    const int c = (int)((uint32_t)(total + a.shares - 1) / (uint32_t)a.shares);
+    chunk = c < a.min_chunk ? a.min_chunk : c;
+    // (at least the empty slots: every part of a row block has a tile)
+    snap = chunk / kSnap > a.pad ? chunk / kSnap : a.pad;
   }
-  return r;
-}
-__device__ __forceinline__ int chunk_of(const ChunkArgs& a, int total) {
-  const int c = (int)((uint32_t)(total + a.shares - 1) / (uint32_t)a.shares);
-  return c < a.min_chunk ? a.min_chunk : c;
-}
-// The row block that holds slot `at`, its first slot in *first; a.items if there is none.
-__device__ __forceinline__ int stream_find(const ChunkArgs& a, int lane, const StreamPos& p,
-                                           int at, int* first) {
-  int carry = 0;
-  for (int base = 0; base < a.items; base += 64) {
-    const int v = a.items <= 64 ? p.v : slots_of(a, base + lane);
-    const int incl = a.items <= 64 ? p.incl : wave_scan(v, lane);
-    const uint64_t hit = __builtin_amdgcn_ballot_w64(v > 0 && carry + incl > at);
-    if (hit) {
-      const int l = __builtin_ctzll(hit);
-      *first = carry + __builtin_amdgcn_readlane(incl - v, l);
-      return base + l;
+  // The row block that holds slot `at` (at < total), or row block `e` if that is not negative.
+  __device__ __forceinline__ Place find(const ChunkArgs& a, int lane, int at, int e) const {
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+      const uint64_t hit = e >= 0 ? __builtin_amdgcn_ballot_w64(64 * k + lane == e)
+                                  : __builtin_amdgcn_ballot_w64(v[k] > 0 && incl[k] > at);
+      if (hit) {
+        const int l = __builtin_ctzll(hit);
+        const int n = __builtin_amdgcn_readlane(v[k], l);
+        return Place{64 * k + l, __builtin_amdgcn_readlane(incl[k], l) - n, n};
+      }
     }
-    carry += __builtin_amdgcn_readlane(incl, 63);
+    int carry = __builtin_amdgcn_readlane(incl[kSteps - 1], 63);
+    for (int base = kHeld; base < a.items; base += 64) {
+      const int w = slots_of(a, base + lane), in = wave_scan(w, lane) + carry;
+      const uint64_t hit = e >= 0 ? __builtin_amdgcn_ballot_w64(base + lane == e)
+                                  : __builtin_amdgcn_ballot_w64(w > 0 && in > at);
+      if (hit) {
+        const int l = __builtin_ctzll(hit);
+        const int n = __builtin_amdgcn_readlane(w, l);
+        return Place{base + l, __builtin_amdgcn_readlane(in, l) - n, n};
+      }
+      carry = __builtin_amdgcn_readlane(in, 63);
+    }
+    return Place{a.items, carry, 0};
   }
-  *first = carry;
-  return a.items;
-}
+  // Where share s begins: at s * chunk, or, if a row block begins or ends within `snap` slots of
+  // that, there: a sliver of a row block is not worth its part in the workspace.
+  __device__ __forceinline__ int begin(const ChunkArgs& a, int lane, int s) const {
+    const int x = s * chunk;       // fits 31 bits: make_plan
+    if (x >= total) return total;
+    const Place p = find(a, lane, x, -1);
+    if (x - p.first <= snap) return p.first;
+    if (p.first + p.slots - x <= snap) return p.first + p.slots;
+    return x;
+  }
+};
 
 // Waits until at most n (0 .. MAX) groups of I loads are in flight.
 template <int I, int MAX>
@@ -241,13 +269,14 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void chunk_attention_kernel(ChunkA
     if (e >= a.items) return;
   } else {
     if (unit >= a.shares) return;
-    const StreamPos p = stream_pos(a, lane, -1);
-    const int chunk = chunk_of(a, p.total);
-    // (slots, and shares times a chunk past them, fit 31 bits: make_plan)
-    from = unit * chunk;
-    to = from + chunk < p.total ? from + chunk : p.total;
+    Stream st;
+    st.read(a, lane);
+    from = st.begin(a, lane, unit);
+    to = st.begin(a, lane, unit + 1);
     if (from >= to) return;
-    e = stream_find(a, lane, p, from, &first);
+    const Place p = st.find(a, lane, from, -1);
+    e = p.e;
+    first = p.first;
   }
 
   const uint32_t swz = (uint32_t)((lane >> 3) * 128 + (((lane & 7) ^ (lane >> 3)) << 4));
@@ -272,7 +301,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void chunk_attention_kernel(ChunkA
     if (!whole) {
       if (ntiles == 0) continue;
       if (first >= to) break;
-      const int base = first + kPad;
+      const int base = first + a.pad;
       t0 = from > base ? from - base : 0;
       t1 = to < base + ntiles ? to - base : ntiles;
       first = base + ntiles;
@@ -633,7 +662,9 @@ __global__ __launch_bounds__(256) void chunk_merge_kernel(ChunkArgs a) {
   const int t = threadIdx.x, lane = t & 63;
   const int e = blockIdx.x, head = blockIdx.y, c0 = blockIdx.z * kMergeCols;
   const Item it = item_of(a, e);
-  const StreamPos p = stream_pos(a, lane, e);
+  Stream st;
+  st.read(a, lane);
+  const Place p = st.find(a, lane, 0, e);
   if (it.n <= 0 || c0 >= it.n * a.group) return;
   const int cols = it.n * a.group - c0 < kMergeCols ? it.n * a.group - c0 : kMergeCols;
   const int c = t * PER / D, d0 = t * PER - c * D;
@@ -642,12 +673,11 @@ __global__ __launch_bounds__(256) void chunk_merge_kernel(ChunkArgs a) {
   for (int x = 0; x < PER; ++x) o[x] = 0.f;
   // its tiles by the scan that gave its place: whatever the lengths are, or become while this
   // runs, the shares are within the workspace
-  const int nt = p.slots > 0 ? p.slots - kPad : 0;
-  if (nt > 0) {
-    const int chunk = chunk_of(a, p.total), base = p.first + kPad;
-    const int s0 = (int)((uint32_t)base / (uint32_t)chunk);
-    const int s1 = (int)((uint32_t)(base + nt - 1) / (uint32_t)chunk);
-    if (s0 == s1) return;
+  if (p.slots > 0) {
+    // the shares that begin inside it, past what Stream::begin moves to its ends
+    const int s0 = (int)((uint32_t)(p.first + st.snap) / (uint32_t)st.chunk);
+    const int s1 = (int)((uint32_t)(p.first + p.slots - st.snap - 1) / (uint32_t)st.chunk);
+    if (s0 >= s1) return;
     const int n = s1 - s0 + 1, per = a.toks * a.group;
     const int64_t seg = ((int64_t)head * a.nseg + s0 + e) * per + c0;
     const float2* const ml = reinterpret_cast<const float2*>(a.ws_ml) + seg;
@@ -940,7 +970,7 @@ int launch_unpacked(const ChunkArgs& c, const Unpacked& u, int max_seqlen, int64
 int col_tiles(int64_t max_seqlen, int group) { return max_seqlen * group <= 16 ? 1 : 2; }
 
 struct Plan {
-  int nt, toks, waves;
+  int nt, toks, waves, pad;
   int64_t blocks_per_seq, items;
   int shares;                 // 0: whole row blocks
   int64_t nseg;
@@ -956,15 +986,16 @@ const void* kernel_of(int nt, int waves) {
                  : (const void*)chunk_attention_kernel<D, F16, 2, 8>;
 }
 
-#ifndef SHARE_WAVES
-#define SHARE_WAVES 4
-#define WHOLE_WAVES 8
-#define WHOLE_TILES 32
-#define MIN_CHUNK 8
-#define LONG_TILES 0
-#define ALWAYS8 0
-#endif
-constexpr int kMinChunk = MIN_CHUNK;
+// Slots a share has at least: two tiles for each of four waves.
+constexpr int kMinChunk = 8;
+// Tiles up to which a row block is one workgroup's, whatever else there is: the shares' scan, their
+// parts and the merge launch cost more (us, shares / whole, 28/4 heads of 128, 8 sequences of 800
+// tokens: 15.3 / 9.8; of 1,500, 47 tiles, 13.0 / 13.6).
+constexpr int kWholeTiles = 32;
+// Empty slots before a row block, one column tile or two (its start, its waves' sums): us at 0, 1,
+// 2 and 4, decode as above 54.3, 53.2, 54.2, 54.0; chunks of 1 to 8 tokens after 512 to 4,096
+// 68.5, 67.8, 66.9, 64.9.
+constexpr int kPad1 = 1, kPad2 = 4;
 
 // resident: workgroups the GPU holds at once.
 Plan make_plan(int64_t num_seqs, int64_t max_seqlen, int64_t max_keys, int group,
@@ -977,12 +1008,15 @@ Plan make_plan(int64_t num_seqs, int64_t max_seqlen, int64_t max_keys, int group
   const int64_t tiles = (max_keys + kTile - 1) / kTile;
   const int64_t units = p.items * num_kv_heads;
   // (slots and segments are counted in 31 bits)
-  const bool whole = tiles <= WHOLE_TILES || units >= 4 * resident ||
-                     (units * 2 >= resident && tiles <= LONG_TILES) ||
-                     p.items * (tiles + kPad) + 2 * resident * kMinChunk > 0x40000000;
-  p.waves = whole && (units * 2 <= resident || (ALWAYS8)) ? WHOLE_WAVES : SHARE_WAVES;
+  const bool whole = tiles <= kWholeTiles || units >= 4 * resident ||
+                     p.items * (tiles + kPad2) + 2 * resident * kMinChunk > 0x40000000;
+  // Eight waves where four would leave half the GPU without any; shares of head_dim 64 keep four,
+  // of which a CU holds three and four workgroups (us, four / eight, 8 tokens each after 3,000: 32
+  // sequences of 28/4 heads of 128 55.1 / 44.6, of 14/2 heads of 64 29.3 / 36.2).
+  p.waves = (whole || head_dim == 128) && units * 2 <= resident ? 8 : 4;
+  p.pad = p.nt == 1 ? kPad1 : kPad2;
   if (!whole) {
-    int64_t s = resident / num_kv_heads / 8 * 8;
+    int64_t s = resident * 4 / p.waves / num_kv_heads / 8 * 8;
     if (s < 8) s = 8;
     p.shares = (int)s;
     p.nseg = s + p.items;
@@ -1004,7 +1038,7 @@ Plan plan_for(int64_t num_seqs, int64_t max_seqlen, int64_t max_keys, int num_he
   const int group = num_heads / num_kv_heads, nt = col_tiles(max_seqlen, group);
   // the formats' kernels use the same resources
   int64_t res = resident_workgroups(
-      head_dim == 128 ? kernel_of<128, false>(nt, SHARE_WAVES) : kernel_of<64, false>(nt, SHARE_WAVES), 64 * SHARE_WAVES);
+      head_dim == 128 ? kernel_of<128, false>(nt, 4) : kernel_of<64, false>(nt, 4), 256);
   if (res <= 0) res = 256;
   return make_plan(num_seqs, max_seqlen, max_keys, group, num_kv_heads, head_dim, res);
 }
@@ -1125,6 +1159,7 @@ extern "C" int ndl_fp8_attention(void* out, const void* q, int64_t q_tok_stride,
   a.scale_log2 = scale * kLog2e;
   a.shares = p.shares;
   a.min_chunk = kMinChunk;
+  a.pad = p.pad;
   a.nseg = (int)p.nseg;
   if (head_dim == 128)
     return f16 ? launch<128, true>(a, p.nt, p.waves, s) : launch<128, false>(a, p.nt, p.waves, s);
