@@ -554,8 +554,8 @@ int ndl_kv_read_fp8(void* k_out, void* v_out, const void* codes, const void* sca
  *
  * max_seqlen bounds the tokens of a sequence (those past it are not computed) and max_keys its
  * keys (context_lens[i] + tokens, at most max_blocks_per_seq * block_size; long chunks attend none
- * past it): they choose how the work is split.  Chunks of 256 rows (max_seqlen times the group)
- * and more unpack their keys into a 16-bit pool in the workspace first.  The workspace
+ * past it): they choose how the work is split.  Long chunks (224 rows of max_seqlen times the
+ * group, 2^24 scores by these bounds) unpack their keys into a 16-bit pool in the workspace first.  The workspace
  * (ndl_fp8_attention_workspace_bytes of the same sizes, max_keys cut to the table's, on the same
  * device; 0: none) is 256-byte aligned and belongs to one call at a time.
  */

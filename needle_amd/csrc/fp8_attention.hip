@@ -25,8 +25,8 @@
 //   * Softmax in fp32 with exp2, scale * log2(e) folded.  The running maximum is raised (and the
 //     sums rescaled) only when a tile exceeds it by 8, so probabilities stay below 256.
 //     P is rounded to the 16-bit format for the matrix cores; its sum is taken before that.
-//   * Long chunks (kUnpackRows columns and more) are bound by the products, not by the codes: their
-//     keys are unpacked once into a 16-bit pool in the workspace, exactly, and attended by
+//   * Long chunks (kUnpackRows columns, kUnpackScores scores) are bound by the products, not by the
+//     codes: their keys are unpacked once into a 16-bit pool in the workspace, exactly, and attended by
 //     varlen_prefill.hip's kernels (see launch_unpacked).
 //   * Split.  Either a workgroup per (kv head, row block), or, where those would leave the GPU
 //     idle or unevenly loaded, all row blocks' tiles of a kv head laid end to end and cut into
@@ -890,9 +890,14 @@ __global__ __launch_bounds__(256) void chunk_nan_kernel(UnpackArgs a) {
               0x7fffu;
 }
 
-// Columns from which a row's codes are used often enough that unpacking them first is faster: us,
-// here / unpacked
-constexpr int64_t kUnpackRows = 256;
+// Where unpacking first is the faster way: enough columns for a row's codes to be used often, and
+// enough scores in all to pay for its launches (unpacking, the prefill with its merge, the scan).
+// us, here / unpacked, chunks of c tokens after t: 28/4 heads of 128, 1 sequence, t 4,000, c 128
+// 36.6 / 46.6, 256 57.6 / 47.9; 4, t 1,000, 64 32.0 / 41.2, 128 48.9 / 43.9; 16, t 4,000, 16
+// 55.2 / 88.4, 32 103 / 91.4, 64 206 / 129; 32/8 heads, 16, t 4,000, 32 98.6 / 149, 64 199 / 181,
+// 128 367 / 216; 14/2 heads of 64, 4, t 12,000, 32 34.6 / 53.3, 128 93.2 / 68.7.
+constexpr int64_t kUnpackRows = 224;
+constexpr int64_t kUnpackScores = (int64_t)1 << 24;
 constexpr int64_t kUnpackBytes = (int64_t)16 << 30;   // of the 16-bit pool
 
 struct Unpacked {
@@ -904,7 +909,9 @@ struct Unpacked {
 // Whether a call takes this path, and its workspace.
 bool unpacked_plan(int64_t num_seqs, int64_t num_tokens, int max_seqlen, int64_t max_keys,
                    int num_heads, int num_kv_heads, int head_dim, int block_size, Unpacked* u) {
-  if ((int64_t)max_seqlen * (num_heads / num_kv_heads) < kUnpackRows || num_seqs > 65535)
+  const int64_t rows = (int64_t)max_seqlen * (num_heads / num_kv_heads);
+  if (rows < kUnpackRows || num_seqs > 65535 ||
+      (double)rows * (double)max_keys * (double)(num_seqs * num_kv_heads) < (double)kUnpackScores)
     return false;
   const int64_t cols = (max_keys + block_size - 1) / block_size;
   u->blocks = num_seqs * cols;

@@ -66,23 +66,36 @@ def attention(q, codes, scales, block_table, cu, context_lens, scale):
     lens = torch.zeros(t, dtype=torch.long)
     w = block_table.shape[1]
     for i in range(block_table.shape[0]):
-        for j in range(int(cu[i + 1]) - int(cu[i])):
-            r = int(cu[i]) + j
-            n = min(int(context_lens[i]) + j + 1, w * bs) if int(context_lens[i]) >= 0 else 0
-            pages = [slot(block_table[i], p, bs, nb) for p in range(max(n, 0))]
-            pages = [p for p in pages if p is not None]
-            lens[r] = len(pages)
-            if not pages:
-                out[r], weight[r] = 0.0, 0.0
-                continue
-            blk, row = (torch.tensor(x) for x in zip(*pages))
-            kv = values(codes[:, blk, :, row], scales[:, blk, :, row])     # [n, 2, Hkv, D]
-            for head in range(h):
-                k, v = kv[:, 0, head // g], kv[:, 1, head // g]
-                qr = q[r, head].double()
-                big[r, head] = (k.abs() @ qr.abs()).max() * abs(scale)
-                p = torch.softmax(k @ qr * scale, dim=0)
-                out[r, head], weight[r, head] = p @ v, p @ v.abs()
+        a, n = int(cu[i]), int(cu[i + 1]) - int(cu[i])
+        ctx = int(context_lens[i])
+        if n == 0:
+            continue
+        out[a:a + n], weight[a:a + n] = 0.0, 0.0
+        if ctx < 0:
+            continue
+        at = [(p, slot(block_table[i], p, bs, nb)) for p in range(min(ctx + n, w * bs))]
+        at = [(p, s) for p, s in at if s is not None]
+        if not at:
+            continue
+        pos = torch.tensor([p for p, _ in at])
+        blk, row = (torch.tensor(x) for x in zip(*(s for _, s in at)))
+        kv = values(codes[:, blk, :, row], scales[:, blk, :, row])         # [keys, 2, Hkv, D]
+        seen = pos[None, :] <= ctx + torch.arange(n)[:, None]              # [n, keys]
+        lens[a:a + n] = seen.sum(1)
+        some = seen.any(1)
+        for head in range(h):
+            k, v = kv[:, 0, head // g], kv[:, 1, head // g]
+            qr = q[a:a + n, head].double()
+            s = (qr @ k.T * scale).masked_fill(~seen, -math.inf)
+            p = torch.softmax(s, dim=1)
+            p = torch.where(some[:, None] & seen, p, 0.0)
+            # a NaN reaches the rows that attend it, and not as 0 * NaN
+            nan = (seen.double() @ v.isnan().double() > 0)
+            big[a:a + n, head] = torch.where(
+                seen, qr.abs() @ k.abs().T, 0.0).nan_to_num(0.0).amax(1) * abs(scale)
+            o = p @ v.nan_to_num(0.0)
+            out[a:a + n, head] = torch.where(nan, math.nan, o)
+            weight[a:a + n, head] = p @ v.nan_to_num(0.0).abs()
     return out, weight, big, lens
 
 

@@ -133,20 +133,47 @@ def test_row_blocks_of_one_chunk(shape, dtype):
     c.check(c.run(max_context_len=1500))
 
 
+def _wide(shape, counts):
+    """Table columns from which a call of these chunks unpacks its keys first."""
+    rows = max(counts) * (shape[0] // shape[1])
+    assert rows >= 224
+    return -(-(1 << 24) // (rows * shape[1] * len(counts) * shape[3]))
+
+
+def _unpacks(c, max_context_len=None):
+    keys = c.table.shape[1] * c.bs
+    if max_context_len is not None:
+        keys = min(keys, max_context_len + max(c.counts))
+    pool = len(c.counts) * -(-keys // c.bs) * c.bs * c.hkv * c.d * 4
+    return ops.fp8_attention_workspace_bytes(len(c.counts), sum(c.counts), max(c.counts), keys,
+                                             c.h, c.hkv, c.d, c.bs) >= pool
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("shape", SHAPES)
 @pytest.mark.parametrize("counts,lens", [([260], [0]), ([300, 1, 90], [77, 400, 0]),
                                          ([257, 5], [1000, -3])])
 def test_long_chunks(shape, dtype, counts, lens):
-    """Chunks whose keys are unpacked into the workspace first."""
-    if shape[0] // shape[1] > 7:      # the oracle is slow on many heads
-        counts = [max(1, n // 4) for n in counts]
-    c = Case(shape, counts, lens, dtype, seed=16)
+    """Chunks whose keys are unpacked into the workspace first, and, with a bound that says how
+    few there are, the same chunks as row blocks."""
+    c = Case(shape, counts, lens, dtype, seed=16, extra_cols=_wide(shape, counts))
+    assert _unpacks(c)
     c.check(c.run())
     ws = ops.decode_workspace(ops.fp8_attention_workspace_bytes(
-        len(lens), sum(counts), max(counts), max(lens) + max(counts), c.h, c.hkv, c.d, c.bs), DEV)
+        len(lens), sum(counts), max(counts), c.table.shape[1] * c.bs, c.h, c.hkv, c.d, c.bs), DEV)
     ws.fill_(0xFF)
-    c.check(c.run(max_context_len=max(lens), workspace=ws))
+    c.check(c.run(workspace=ws))
+    if not _unpacks(c, max(lens)):
+        c.check(c.run(max_context_len=max(lens)))
+
+
+def test_long_chunks_in_more_keys():
+    """Prefixes of thousands of tokens, split over the workgroups of the prefill."""
+    for shape, counts, lens in (((28, 4, 128, 16), [200, 64], [3100, 2500]),
+                                ((14, 2, 64, 64), [300], [5000])):
+        c = Case(shape, counts, lens, seed=17)
+        assert _unpacks(c, max(lens))
+        c.check(c.run(max_context_len=max(lens)))
 
 
 def test_many_row_blocks_in_shares():
@@ -159,9 +186,10 @@ def test_many_row_blocks_in_shares():
 
 def test_tables_that_end_and_bad_blocks():
     """Keys past the table's columns are not attended; neither are those of an invalid block."""
-    for counts in ([1, 1, 1], [4, 4, 4], [70, 20, 10]):
+    for counts in ([1, 1, 1], [4, 4, 4], [70, 20, 10], [30000, 20, 10]):
         c = Case((8, 2, 64, 16), counts, [70, 45, 0], seed=6, extra_cols=0)
         c.table = c.table[:, :3].contiguous()     # 48 keys
+        assert _unpacks(c) == (counts[0] == 30000)
         c.table[1, 1] = -1
         c.table[2, 0] = c.nb                      # all that the third attends
         got = c.run(decode=counts[0] == 1)
@@ -173,7 +201,10 @@ def test_tables_that_end_and_bad_blocks():
 @pytest.mark.parametrize("count,d", [(9, 64), (80, 64), (9, 128), (80, 128)])
 def test_a_nan_stays_where_it_is_attended(dtype, count, d):
     """A NaN among the chunk's own values reaches the tokens from its position on, no others."""
-    c = Case((8, 2, d, 16), [count, 4], [20, 61], dtype, seed=7)
+    shape = (8, 2, d, 16)
+    c = Case(shape, [count, 4], [20, 61], dtype, seed=7,
+             extra_cols=_wide(shape, [count, 4]) if count == 80 else 1)
+    assert _unpacks(c) == (count == 80)
     for plane, seq, pos, d in ((1, 0, 24, 11), (1, 1, 64, 63), (0, 1, 63, 5), (1, 0, 28, 0)):
         b = int(c.table[seq, pos // 16])
         c.codes[plane, b, 1, pos % 16, d] = 0x7F if d % 2 else 0xFF
@@ -186,7 +217,9 @@ def test_scores_of_any_size():
     """Large scores (one key takes all), a raised maximum late in the row, and scale 0 and
     below."""
     for scale, n in ((40.0, 3), (0.0, 3), (-0.3, 3), (1e-6, 3), (40.0, 66), (0.0, 66), (-0.3, 66)):
-        c = Case((8, 2, 128, 16), [n, 1], [700, 90], seed=8)
+        shape = (8, 2, 128, 16)
+        c = Case(shape, [n, 1], [700, 90], seed=8,
+                 extra_cols=_wide(shape, [n, 1]) if n == 66 else 1)
         c.scale = scale
         if scale == 40.0:
             c.q = (c.q.float() * 0.02).to(c.dtype)
@@ -203,7 +236,9 @@ def test_scores_of_any_size():
 
 @pytest.mark.parametrize("counts", [[3, 5, 1], [60, 5, 1]])
 def test_strided_queries_and_padding_rows(counts):
-    c = Case((14, 2, 64, 16), counts, [40, 0, 17], seed=10)
+    shape = (14, 2, 64, 16)
+    c = Case(shape, counts, [40, 0, 17], seed=10,
+             extra_cols=_wide(shape, counts) if max(counts) == 60 else 1)
     n = int(c.cu[-1])
     wide = torch.full((n + 4, 18 * 64), float("nan"), dtype=c.dtype, device=DEV)
     q = wide[:, 64:64 + 14 * 64].view(n + 4, 14, 64)
@@ -228,7 +263,9 @@ def test_same_inputs_same_bits_and_a_workspace_of_ones_own():
 
 @pytest.mark.parametrize("count", [1, 6, 50])
 def test_captured_and_replayed(count):
-    c = Case((14, 2, 64, 16), [count] * 3, [1900, 40, 333], seed=12)
+    shape = (14, 2, 64, 16)
+    c = Case(shape, [count] * 3, [1900, 40, 333], seed=12,
+             extra_cols=_wide(shape, [count] * 3) if count == 50 else 1)
     q, pool = c.q.to(DEV), (c.codes.to(DEV), c.scales.to(DEV))
     t, cu, ctx = c.table.to(DEV), c.cu.to(DEV), c.ctx.to(DEV)
 
