@@ -9,6 +9,7 @@ decode_graphs=True replays decode steps from HIP graphs captured per batch-size 
 their metadata stays on the device between steps (sequences longer than max_model_len, or
 batches beyond the largest bucket, run eagerly).  cpu_swap_bytes sizes a pinned CPU pool
 that preemption swaps blocks into (0: evicted sequences are recomputed).
+kv_cache_dtype="fp8" keeps K and V in 8 bits (ops.Fp8KVCache): about twice the blocks.
 """
 from __future__ import annotations
 
@@ -31,10 +32,11 @@ class LLMEngine:
                  max_gpu_blocks: int = 0, cpu_swap_bytes: int = 0, dtype: str = "bfloat16",
                  device: str = "cuda:0", seed: int = 0,
                  model: Optional[torch.nn.Module] = None, decode_graphs: bool = False,
-                 max_model_len: int = 0):
+                 max_model_len: int = 0, kv_cache_dtype: str = "auto"):
         self.block_size = block_size
         self.model_config = model_config
-        self.runner = ModelRunner(model_config, block_size, dtype, device, seed, model)
+        self.runner = ModelRunner(model_config, block_size, dtype, device, seed, model,
+                                  kv_cache_dtype=kv_cache_dtype)
         n_gpu, n_cpu = self.runner.profile_memory(gpu_memory_utilization, max_gpu_blocks,
                                                   cpu_swap_bytes)
         # With decode graphs the last pool block is the padding rows' scratch block, so the

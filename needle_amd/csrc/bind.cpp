@@ -12,6 +12,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -360,6 +361,7 @@ PyObject* kv_append_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
       (cu != nullptr ? cu->size(0) != seqs + 1 : tokens != seqs) ||
       (cos != nullptr && !read_rope(*cos, *sin, k, tokens, p.d, &cs)))
     Py_RETURN_NONE;
+  const c10::DeviceGuard guard(codes.device());
   at::Tensor out;
   if (q != nullptr) {
     if (q->dim() != 3 || q->size(0) != tokens || q->scalar_type() != k.scalar_type()) Py_RETURN_NONE;
@@ -403,6 +405,7 @@ PyObject* kv_read_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (tokens == 0 || seqs == 0 || width == 0 || first.size(0) != seqs || cu.size(0) != seqs + 1 ||
       !fits_int(seqs) || !fits_int(width))
     Py_RETURN_NONE;
+  const c10::DeviceGuard guard(codes.device());
   const auto opts = codes.options().dtype(code == NDL_DTYPE_F16 ? at::kHalf : at::kBFloat16);
   at::Tensor k = at::empty({tokens, p.hkv, p.d}, opts), v = at::empty({tokens, p.hkv, p.d}, opts);
   const ndl_stream_t s = stream_of(codes);
@@ -448,6 +451,7 @@ PyObject* fp8_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
       (cu != nullptr ? cu->size(0) != seqs + 1 : tokens != seqs || most != 1))
     Py_RETURN_NONE;
   if (keys == 0 || keys > width * p.bs) keys = width * p.bs;
+  const c10::DeviceGuard guard(codes.device());
   at::Tensor out = at::empty({tokens, heads, d}, q.options()), ws;
   const size_t need = p_fp8_workspace((int)seqs, tokens, (int)most, keys, (int)heads, (int)hkv,
                                       (int)d, (int)p.bs);
@@ -501,6 +505,7 @@ PyObject* verify_drafts(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (rows - seqs > 1 && (ds = probs->stride(0)) < vocab) Py_RETURN_NONE;
     if (rows == seqs) probs = nullptr;   // no drafts, and no address either
   }
+  const c10::DeviceGuard guard(logits.device());
   at::Tensor tokens = at::empty_like(ids), accepted = at::empty({seqs}, cu.options());
   const size_t need = p_verify_workspace(rows, (int)seqs, (int)vocab);
   at::Tensor ws = at::empty({(int64_t)need}, cu.options().dtype(at::kByte));

@@ -26,13 +26,13 @@
 //     sums rescaled) only when a tile exceeds it by 8, so probabilities stay below 256.
 //     P is rounded to the 16-bit format for the matrix cores; its sum is taken before that.
 //   * Long chunks (kUnpackRows columns, kUnpackScores scores) are bound by the products, not by the
-//     codes: their keys are unpacked once into a 16-bit pool in the workspace, exactly, and attended by
-//     varlen_prefill.hip's kernels (see launch_unpacked).
+//     codes: their keys are unpacked once into a 16-bit pool in the workspace, exactly, and
+//     attended by varlen_prefill.hip's kernels (see launch_unpacked).
 //   * Split.  Either a workgroup per (kv head, row block), or, where those would leave the GPU
 //     idle or unevenly loaded, all row blocks' tiles of a kv head laid end to end and cut into
 //     equal shares, one per resident workgroup; what a share holds of a row block goes to a
 //     workspace and is merged by a second launch.
-#include "ndl_common.hpp"
+#include "fp8.hpp"
 
 namespace ndl {
 namespace {
@@ -210,15 +210,6 @@ __device__ __forceinline__ void vm_wait_groups(int n) {
   }
 }
 
-// Two codes of w's low or high half times scale, in the 16-bit format.
-template <bool F16, bool HI>
-__device__ __forceinline__ uint32_t value2(uint32_t w, float scale) {
-  if constexpr (F16)
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, HI));
-  else
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, HI));
-}
-
 // 0xff in every byte of w that is a NaN code (0x7f or 0xff).
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
   const uint32_t top = ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
@@ -365,7 +356,8 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void chunk_attention_kernel(ChunkA
 #pragma unroll
         for (int x = 0; x < D / 64; ++x) {
           lds_dma16_nt(kb + 1024 * x, swz, st + s * 16 * D + 1024 * x);
-          lds_dma16_nt(vb + 1024 * x, (uint32_t)lane * 16, st + S::kRowTile + s * 16 * D + 1024 * x);
+          lds_dma16_nt(vb + 1024 * x, (uint32_t)lane * 16,
+                       st + S::kRowTile + s * 16 * D + 1024 * x);
         }
       }
       // scales: 4-byte word w of half s of plane p lands at word 8 p + 4 s + w
@@ -810,7 +802,8 @@ __global__ __launch_bounds__(256) void chunk_unpack_kernel(UnpackArgs a) {
     const int64_t block = (int64_t)seq * a.cols + col;
     if (ph == 0 && in_block == 0 && lane == 0) row[col] = ok ? (int)block : -1;
     if (!ok) continue;
-    const int64_t from = (plane ? a.plane_rows : 0) + (((int64_t)b * Hkv + head) << bshift) + in_block;
+    const int64_t from =
+        (plane ? a.plane_rows : 0) + (((int64_t)b * Hkv + head) << bshift) + in_block;
     u16* const dst = a.pool + ((plane ? a.pool_rows : 0) + ((block * Hkv + head) << bshift) +
                                in_block) * D + lane * 8;
     u32x2 c[16 / RPL];
@@ -1108,7 +1101,8 @@ extern "C" int ndl_fp8_attention(void* out, const void* q, int64_t q_tok_stride,
     return NDL_ERR_INVALID_ARG;
   if (cu_seqlens == nullptr && (num_tokens != num_seqs || max_seqlen != 1))
     return NDL_ERR_INVALID_ARG;
-  if (q_tok_stride < (int64_t)num_heads * head_dim || (q_tok_stride & 7)) return NDL_ERR_INVALID_ARG;
+  if (q_tok_stride < (int64_t)num_heads * head_dim || (q_tok_stride & 7))
+    return NDL_ERR_INVALID_ARG;
   if (((uintptr_t)out | (uintptr_t)q | (uintptr_t)codes) & 15u || (uintptr_t)scales & 3u)
     return NDL_ERR_INVALID_ARG;
   ChunkArgs a{};

@@ -15,7 +15,7 @@
 // 141-154, :224-237) and the rotation its _apply_rope (:277-288), as in rope_append.hip.
 //
 // Pools: codes [2][NB][Hkv][bs][D] bytes, scales [2][NB][Hkv][bs] bytes.
-#include "ndl_common.hpp"
+#include "fp8.hpp"
 
 namespace ndl {
 namespace {
@@ -195,15 +195,6 @@ __global__ __launch_bounds__(256) void kv_append_fp8_kernel(QuantArgs a) {
   }
 }
 
-// Two codes of w's low or high half times scale, in the 16-bit format.
-template <bool F16, bool HI>
-__device__ __forceinline__ uint32_t value2(uint32_t w, float scale) {
-  if constexpr (F16)
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, HI));
-  else
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, HI));
-}
-
 constexpr int kReadItems = 512;   // 8-code items a wave has in flight: 4 KiB of codes, 8 KiB out
 
 // The slot row of token t of a lane's own, as slot_row.  cu of up to 64 sequences is in the lanes
@@ -243,8 +234,9 @@ __device__ __forceinline__ int64_t slot_row_of_lane(const QuantArgs& a, int64_t 
 }
 
 // One wave per kReadItems items of the packed tokens; an item is 8 codes of one of a token's
-// 2 Hkv rows, in the order of the tokens, so that a wave stores 1 KiB at once.  Lane k first finds the slot of the wave's k-th token.
-// Positions that have no slot read as zeros, tokens past the last sequence are not written.
+// 2 Hkv rows, in the order of the tokens, so that a wave stores 1 KiB at once.  Lane k first finds
+// the slot of the wave's k-th token.  Positions that have no slot read as zeros, tokens past the
+// last sequence are not written.
 template <int D, bool F16>
 __global__ __launch_bounds__(256) void kv_read_fp8_kernel(QuantArgs a) {
   constexpr int CPR = D / 8, U = kReadItems / 64;
@@ -281,8 +273,9 @@ __global__ __launch_bounds__(256) void kv_read_fp8_kernel(QuantArgs a) {
 #pragma unroll
   for (int u = 0; u < U; ++u)
     if (dst[u] != nullptr)
-      st16(dst[u], u32x4{value2<F16, false>(c[u][0], scale[u]), value2<F16, true>(c[u][0], scale[u]),
-                         value2<F16, false>(c[u][1], scale[u]), value2<F16, true>(c[u][1], scale[u])});
+      st16(dst[u],
+           u32x4{value2<F16, false>(c[u][0], scale[u]), value2<F16, true>(c[u][0], scale[u]),
+                 value2<F16, false>(c[u][1], scale[u]), value2<F16, true>(c[u][1], scale[u])});
 }
 
 int log2_of(int block_size) {

@@ -41,7 +41,7 @@
 //     depend on nothing else in it, then the ring upkeep, masking and softmax.
 //   * Causal masking only on steps that reach past a wave's first query position;
 //     query tiles are dispatched longest-first.
-#include "ndl_common.hpp"
+#include "fp8.hpp"
 
 namespace ndl {
 

@@ -430,7 +430,8 @@ struct Exp {
     const double r = (z - (shifted - 6755399441055744.0)) * 0.01083042469624914545;  // ln 2 / 64
     const double e =
         fma(r, fma(r, fma(r, fma(r, 1.0 / 24, 1.0 / 6), 0.5), 1.0), 1.0) * table[n & 63];
-    const uint64_t w = __builtin_bit_cast(uint64_t, e) + ((uint64_t)(uint32_t)((n >> 6) << 20) << 32);
+    const uint64_t w =
+        __builtin_bit_cast(uint64_t, e) + ((uint64_t)(uint32_t)((n >> 6) << 20) << 32);
     return z > -57600.0 ? __builtin_bit_cast(double, w) : 0.0;
   }
 };

@@ -34,11 +34,13 @@ def requests(n: int = 256, seed: int = E2E_SEED, prompt=(64, 1024), output=(128,
 
 def build_engine(device: str = "cuda:0", max_gpu_blocks: int = 40000, seed: int = E2E_SEED,
                  model=None, max_num_seqs: int = 256, max_num_batched_tokens: int = 8192,
-                 decode_graphs: bool = True, max_model_len: int = 1536):
+                 decode_graphs: bool = True, max_model_len: int = 1536,
+                 kv_cache_dtype: str = "auto"):
     return LLMEngine(ModelConfig(**QWEN2_0_5B), max_num_seqs=max_num_seqs,
                      max_num_batched_tokens=max_num_batched_tokens,
                      max_gpu_blocks=max_gpu_blocks, device=device, seed=seed, model=model,
-                     decode_graphs=decode_graphs, max_model_len=max_model_len)
+                     decode_graphs=decode_graphs, max_model_len=max_model_len,
+                     kv_cache_dtype=kv_cache_dtype)
 
 
 def run(engine: LLMEngine, reqs, sync=None, time_limit_s: Optional[float] = None):
@@ -69,8 +71,9 @@ def main(argv=None) -> None:
     p = argparse.ArgumentParser(description=main.__doc__.splitlines()[0])
     p.add_argument("--requests", type=int, default=256)
     p.add_argument("--time-limit", type=float, default=None)
+    p.add_argument("--kv-cache-dtype", choices=("auto", "fp8"), default="auto")
     args = p.parse_args(argv)
-    engine = build_engine()
+    engine = build_engine(kv_cache_dtype=args.kv_cache_dtype)
     reqs = requests(args.requests)
     torch.cuda.synchronize()
     n_tok, secs, finished = run(engine, reqs, sync=torch.cuda.synchronize,

@@ -22,6 +22,10 @@ q and k already rotated, for callers that apply RoPE themselves
   _decode   (attention.py:140-159): ndl_paged_decode_append (the one-token-per-sequence
                                     append and the attention in one launch)
 
+With an 8-bit pool (kv_cache an ops.Fp8KVCache) the step is ndl_kv_append_fp8 (RoPE of q and k,
+quantisation and append of k and v in one launch), then ndl_fp8_attention over the pool, a prefill
+as a chunk and a decode step as one token per sequence.
+
 No host synchronisation happens on either path: the decode split-K grid is
 sized from block_table's width, prefill from max_seqlen (both host-known).
 
@@ -144,7 +148,10 @@ class Attention(nn.Module):
         q = q.view(total, self.num_heads, self.head_dim)
         k = k.view(total, self.num_kv_heads, self.head_dim)
         v = v.view(total, self.num_kv_heads, self.head_dim)
-        if self.fuse_rope:
+        if isinstance(kv_cache, ops.Fp8KVCache):
+            out = self._fp8(q, k, v, kv_cache, block_table, cu_seqlens, context_lens, max_seqlen,
+                            is_prefill, cos, sin)
+        elif self.fuse_rope:
             if is_prefill:
                 ops.rope_kv_append(None, k, v, cos, sin, kv_cache, block_table, context_lens,
                                    cu_seqlens)
@@ -161,6 +168,22 @@ class Attention(nn.Module):
             else:
                 out = self._decode(q, k, v, kv_cache, block_table, context_lens)
         return self.o_proj(out.view(total, self.num_heads * self.head_dim))
+
+    def _fp8(self, q, k, v, pool, block_table, cu_seqlens, context_lens, max_seqlen, is_prefill,
+             cos, sin):
+        """The step over an 8-bit pool."""
+        cu = cu_seqlens if is_prefill else None
+        if self.fuse_rope:
+            q = ops.kv_append_fp8(k, v, *pool, block_table, context_lens, cu, q=q, cos=cos,
+                                  sin=sin)
+        else:
+            q, k = apply_rope(q, k, cos, sin)
+            ops.kv_append_fp8(k, v, *pool, block_table, context_lens, cu)
+        heads = (self.scale, self.num_heads, self.num_kv_heads, self.head_dim)
+        if is_prefill:
+            return ops.varlen_prefill_fp8(q, *pool, block_table, cu_seqlens, context_lens,
+                                          int(max_seqlen), *heads)
+        return ops.paged_decode_fp8(q, *pool, block_table, context_lens, *heads)
 
     def _prefill(self, q, k, v, kv_cache, block_table, cu_seqlens, context_lens, max_seqlen):
         ops.write_kv(k, v, kv_cache, block_table, cu_seqlens, context_lens)

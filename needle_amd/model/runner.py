@@ -2,7 +2,8 @@
 
 Contract with the attention path (reference needle/model/runner.py:65-94, 194-249):
   * one KV pool per layer, [2, num_blocks, num_kv_heads, block_size, head_dim] in the
-    model dtype, zero-initialised, plus an optional pinned CPU pool for swapping;
+    model dtype, zero-initialised, plus an optional pinned CPU pool for swapping; with
+    kv_cache_dtype "fp8" an 8-bit one (ops.Fp8KVCache) of half the bytes instead;
   * prefill feeds every token of a sequence with context 0, decode its newest token with
     context length-1; positions ctx..ctx+n; cu_seqlens is the prefix sum of the token
     counts; block_table rows are padded with num_blocks-1 to the widest row; a step with
@@ -185,7 +186,16 @@ class ModelRunner:
 
     def __init__(self, model_config: ModelConfig, block_size: int = 16, dtype: str = "bfloat16",
                  device: str = "cuda:0", seed: int = 0, model: Optional[torch.nn.Module] = None,
-                 fuse: bool = True):
+                 fuse: bool = True, kv_cache_dtype: str = "auto"):
+        if kv_cache_dtype not in ("auto", "fp8"):
+            raise ValueError(f"kv_cache_dtype must be 'auto' (the model's) or 'fp8', got "
+                             f"{kv_cache_dtype!r}")
+        if kv_cache_dtype == "fp8" and dtype not in ("bfloat16", "float16"):
+            raise ValueError(f"an 8-bit KV cache needs a bfloat16 or float16 model, got {dtype}")
+        if kv_cache_dtype == "fp8" and model_config.head_dim not in (64, 128):
+            raise ValueError("an 8-bit KV cache is built for head_dim 64 and 128, got "
+                             f"{model_config.head_dim}")
+        self.fp8_cache = kv_cache_dtype == "fp8"
         self.model_config = model_config
         self.block_size = block_size
         self.device = torch.device(device)
@@ -204,8 +214,9 @@ class ModelRunner:
 
     def bytes_per_block(self) -> int:
         cfg = self.model_config
-        return (2 * cfg.num_kv_heads * self.block_size * cfg.head_dim
-                * torch.finfo(self.dtype).bits // 8 * cfg.num_hidden_layers)
+        row = cfg.head_dim + 1 if self.fp8_cache else \
+            cfg.head_dim * torch.finfo(self.dtype).bits // 8
+        return 2 * cfg.num_kv_heads * self.block_size * row * cfg.num_hidden_layers
 
     def profile_memory(self, gpu_memory_utilization: float = 0.90, max_gpu_blocks: int = 0,
                        cpu_swap_bytes: int = 0):
@@ -222,6 +233,13 @@ class ModelRunner:
 
     def init_kv_cache(self, num_gpu_blocks: int, num_cpu_blocks: int = 0) -> None:
         cfg = self.model_config
+        if self.fp8_cache:
+            shape = (cfg.num_kv_heads, self.block_size, cfg.head_dim)
+            self.kv_caches = [ops.fp8_kv_pool(num_gpu_blocks, *shape, device=self.device)
+                              for _ in range(cfg.num_hidden_layers)]
+            self.cpu_kv_caches = [ops.fp8_kv_pool(num_cpu_blocks, *shape, pin_memory=True)
+                                  for _ in range(cfg.num_hidden_layers if num_cpu_blocks else 0)]
+            return
         shape = (2, num_gpu_blocks, cfg.num_kv_heads, self.block_size, cfg.head_dim)
         self.kv_caches = [torch.zeros(shape, dtype=self.dtype, device=self.device)
                           for _ in range(cfg.num_hidden_layers)]

@@ -13,6 +13,7 @@ Argument meaning follows the reference:
 """
 from __future__ import annotations
 
+import contextlib
 import os
 from typing import NamedTuple, Optional
 
@@ -40,6 +41,13 @@ def _stream(dev: torch.device) -> int:
         return torch.cuda.current_stream(dev).cuda_stream
     idx = dev.index
     return _raw_stream(torch.cuda.current_device() if idx is None else idx)
+
+
+def _on(dev: torch.device):
+    """dev as the current device while a launch is sized and made (no guard where it is)."""
+    if dev.index is None or dev.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(dev)
 
 
 def _require(cond: bool, msg: str, exc=ValueError) -> None:
@@ -453,13 +461,21 @@ def kv_block_copy(dst_pools, src_pools, src_ids: torch.Tensor, dst_ids: torch.Te
     launch (the KV swap copies; the reference copies per layer and block,
     runner.py:175-192).
 
-    dst_pools / src_pools: equal-length lists of [2, NB, Hkv, bs, D] tensors, each on the GPU
-    or in pinned CPU memory (pin_memory=True).  src_ids / dst_ids: int32 [pairs] on the GPU or
-    pinned.  Enqueued on the current stream of the GPU the pools (or ids) live on.
+    dst_pools / src_pools: equal-length lists of [2, NB, Hkv, bs, D] tensors (or of Fp8KVCache:
+    two launches, codes and scales), each on the GPU or in pinned CPU memory (pin_memory=True).
+    src_ids / dst_ids: int32 [pairs] on the GPU or pinned.  Enqueued on the current stream of
+    the GPU the pools (or ids) live on.
     """
     import ctypes
     _require(len(dst_pools) == len(src_pools), "dst_pools and src_pools differ in length")
     if not dst_pools:
+        return
+    if any(isinstance(p, Fp8KVCache) for p in (*dst_pools, *src_pools)):
+        _require(all(isinstance(p, Fp8KVCache) for p in (*dst_pools, *src_pools)),
+                 "an 8-bit pool copies to an 8-bit pool", TypeError)
+        for part in (0, 1):
+            kv_block_copy([_as_16bit_pool(p)[part] for p in dst_pools],
+                          [_as_16bit_pool(p)[part] for p in src_pools], src_ids, dst_ids)
         return
     ref = dst_pools[0]
     _require(ref.dim() == 5 and ref.shape[0] == 2, "pools must be [2, NB, Hkv, bs, D]")
@@ -762,6 +778,14 @@ def fp8_kv_pool(num_blocks: int, num_kv_heads: int, block_size: int, head_dim: i
     return Fp8KVCache(codes.view(torch.float8_e4m3fn), scales)
 
 
+def _as_16bit_pool(pool: Fp8KVCache):
+    """The bytes of an 8-bit pool as two 16-bit pools, codes and scales, for kv_block_copy (which
+    moves raw bits): a block's codes, and its row of scale bytes, of whole 16-byte pieces."""
+    _, nb, hkv, bs, d = pool.codes.shape
+    return (pool.codes.view(torch.uint8).view(torch.bfloat16),
+            pool.scales.view(torch.bfloat16).view(2, nb, 1, hkv * bs // 16, 8))
+
+
 _FP8_CODES = (torch.float8_e4m3fn, torch.uint8)
 
 
@@ -866,11 +890,12 @@ def kv_append_fp8(k: torch.Tensor, v: torch.Tensor, kv_codes: torch.Tensor,
     if n_tok == 0:
         return out
     _require(block_table.shape[1] > 0, "block_table has no columns")
-    rc = _lib.load().ndl_kv_append_fp8(
-        kv_codes.data_ptr(), kv_scales.data_ptr(), nb, hkv, bs, d, _DTYPES[dtype],
-        k.data_ptr(), ks, v.data_ptr(), vs, _ptr(out), _ptr(q), qs, h, _ptr(cos), _ptr(sin), cs,
-        block_table.data_ptr(), block_table.stride(0), block_table.shape[1], _ptr(cu_seqlens),
-        context_lens.data_ptr(), n_seqs, n_tok, _stream(dev))
+    with _on(dev):
+        rc = _lib.load().ndl_kv_append_fp8(
+            kv_codes.data_ptr(), kv_scales.data_ptr(), nb, hkv, bs, d, _DTYPES[dtype],
+            k.data_ptr(), ks, v.data_ptr(), vs, _ptr(out), _ptr(q), qs, h, _ptr(cos), _ptr(sin), cs,
+            block_table.data_ptr(), block_table.stride(0), block_table.shape[1], _ptr(cu_seqlens),
+            context_lens.data_ptr(), n_seqs, n_tok, _stream(dev))
     _lib.check(rc, "ndl_kv_append_fp8")
     return out
 
@@ -901,10 +926,11 @@ def kv_read_fp8(kv_codes: torch.Tensor, kv_scales: torch.Tensor, block_table: to
     if num_tokens == 0 or n_seqs == 0:
         return k, v
     _require(block_table.shape[1] > 0, "block_table has no columns")
-    rc = _lib.load().ndl_kv_read_fp8(
-        k.data_ptr(), v.data_ptr(), kv_codes.data_ptr(), kv_scales.data_ptr(), nb, hkv, bs, d,
-        _DTYPES[dtype], block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
-        first.data_ptr(), cu_seqlens.data_ptr(), n_seqs, num_tokens, _stream(dev))
+    with _on(dev):
+        rc = _lib.load().ndl_kv_read_fp8(
+            k.data_ptr(), v.data_ptr(), kv_codes.data_ptr(), kv_scales.data_ptr(), nb, hkv, bs, d,
+            _DTYPES[dtype], block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
+            first.data_ptr(), cu_seqlens.data_ptr(), n_seqs, num_tokens, _stream(dev))
     _lib.check(rc, "ndl_kv_read_fp8")
     return k, v
 
@@ -947,17 +973,18 @@ def _fp8_attention(q, kv_codes, kv_scales, block_table, cu_seqlens, context_lens
     _require(max_seqlen > 0, "max_seqlen must be positive")
     max_keys = min(w * bs, max_keys) if max_keys else w * bs
     lib = _lib.load()
-    need = lib.ndl_fp8_attention_workspace_bytes(n_seqs, n_tok, max_seqlen, max_keys, num_heads,
-                                                 num_kv_heads, head_dim, bs)
-    if need and (workspace is None or workspace.numel() * workspace.element_size() < need
-                 or workspace.device != dev):
-        workspace = decode_workspace(need, dev)
-    rc = lib.ndl_fp8_attention(
-        out.data_ptr(), q.data_ptr(), qs, kv_codes.data_ptr(), kv_scales.data_ptr(), nb,
-        block_table.data_ptr(), block_table.stride(0), w, _ptr(cu_seqlens),
-        context_lens.data_ptr(), n_seqs, n_tok, max_seqlen, max_keys, num_heads, num_kv_heads,
-        head_dim, bs, _DTYPES[q.dtype], float(scale), _ptr(workspace) if need else None, need,
-        _stream(dev))
+    with _on(dev):
+        need = lib.ndl_fp8_attention_workspace_bytes(n_seqs, n_tok, max_seqlen, max_keys, num_heads,
+                                                     num_kv_heads, head_dim, bs)
+        if need and (workspace is None or workspace.numel() * workspace.element_size() < need
+                     or workspace.device != dev):
+            workspace = decode_workspace(need, dev)
+        rc = lib.ndl_fp8_attention(
+            out.data_ptr(), q.data_ptr(), qs, kv_codes.data_ptr(), kv_scales.data_ptr(), nb,
+            block_table.data_ptr(), block_table.stride(0), w, _ptr(cu_seqlens),
+            context_lens.data_ptr(), n_seqs, n_tok, max_seqlen, max_keys, num_heads, num_kv_heads,
+            head_dim, bs, _DTYPES[q.dtype], float(scale), _ptr(workspace) if need else None, need,
+            _stream(dev))
     _lib.check(rc, "ndl_fp8_attention")
     return out
 
@@ -1072,11 +1099,12 @@ def verify_drafts(logits: torch.Tensor, ids: torch.Tensor, cu_seqlens: torch.Ten
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     # without drafts there are no draft rows, and no address either
     probs = draft_probs if draft_probs is not None and rows > n_seqs else None
-    rc = lib.ndl_verify_drafts(
-        tokens.data_ptr(), accepted.data_ptr(), logits.data_ptr(),
-        logits.stride(0) if rows > 1 else vocab, _DTYPES[logits.dtype], ids.data_ptr(),
-        int(ids.dtype == torch.int64), cu_seqlens.data_ptr(), uniforms.data_ptr(),
-        _ptr(temperature), _ptr(probs), ds, rows - n_seqs, rows, n_seqs, vocab, ws.data_ptr(),
-        need, _stream(dev))
+    with _on(dev):
+        rc = lib.ndl_verify_drafts(
+            tokens.data_ptr(), accepted.data_ptr(), logits.data_ptr(),
+            logits.stride(0) if rows > 1 else vocab, _DTYPES[logits.dtype], ids.data_ptr(),
+            int(ids.dtype == torch.int64), cu_seqlens.data_ptr(), uniforms.data_ptr(),
+            _ptr(temperature), _ptr(probs), ds, rows - n_seqs, rows, n_seqs, vocab, ws.data_ptr(),
+            need, _stream(dev))
     _lib.check(rc, "ndl_verify_drafts")
     return tokens, accepted

@@ -54,6 +54,19 @@ def slot(table_row, p, block_size, num_blocks):
     return (b, p % block_size) if 0 <= b < num_blocks else None
 
 
+def append(k, v, codes, scales, block_table, cu, context_lens):
+    """Rows of k and v into the pool's bytes, in place."""
+    for i in range(block_table.shape[0]):
+        for t in range(int(cu[i]), int(cu[i + 1])):
+            at = slot(block_table[i], int(context_lens[i]) + t - int(cu[i]), codes.shape[3],
+                      codes.shape[1])
+            for plane, x in enumerate((k, v)):
+                for head in range(x.shape[1] if at is not None else 0):
+                    c, byte = quantise_row(x[t, head].double().tolist())
+                    codes[plane, at[0], head, at[1]] = torch.tensor(c, dtype=torch.uint8)
+                    scales[plane, at[0], head, at[1]] = byte
+
+
 def attention(q, codes, scales, block_table, cu, context_lens, scale):
     """(out, weight) [T, H, D] in float64: the attention, and sum_t p_t |v_t|, what a rounding of
     the probabilities is relative to; rows outside cu are NaN.  Also the largest

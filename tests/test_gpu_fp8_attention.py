@@ -119,8 +119,8 @@ def test_chunks(shape, dtype, counts):
 def test_shares_and_merge(shape, counts):
     """Contexts long enough for the split into shares, of very different lengths."""
     c = Case(shape, counts, [2900, 3, 1111], seed=3)
-    assert ops.fp8_attention_workspace_bytes(3, sum(counts), max(counts), c.table.shape[1] * c.bs, c.h, c.hkv,
-                                             c.d, c.bs) > 0
+    assert ops.fp8_attention_workspace_bytes(3, sum(counts), max(counts), c.table.shape[1] * c.bs,
+                                             c.h, c.hkv, c.d, c.bs) > 0
     c.check(c.run(decode=max(counts) == 1))
 
 

@@ -107,3 +107,18 @@ def test_skinny_linear_uses_m0_only_for_direct_lds_loads(device_asm):
         assert body[i].startswith("s_mov_b32 m0, s"), body[i]
         assert body[i + 1] == "s_nop 0" and \
             re.match(r"global_load_lds_dwordx4 ", body[i + 2]), body[i:i + 3]
+
+
+def test_fp8_attention_uses_m0_only_for_direct_lds_loads(device_asm):
+    body = [l.strip() for l in device_asm("fp8_attention")]
+    body = [l for l in body if l and not l.startswith((";", "."))]
+    uses = [i for i, l in enumerate(body) if re.search(r"\bm0\b", l)]
+    assert uses and len(uses) == sum("global_load_lds" in l for l in body)
+    for i in uses:
+        assert body[i].startswith("s_mov_b32 m0, s"), body[i]
+        assert body[i + 1] == "s_nop 0" and \
+            re.match(r"global_load_lds_dword(x4)? ", body[i + 2]), body[i:i + 3]
+
+
+def test_the_8_bit_appends_rope_has_no_fused_fp16_multiply_add(device_asm):
+    test_no_fused_fp16_multiply_add(device_asm, "kv_fp8")
