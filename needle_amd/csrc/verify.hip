@@ -50,6 +50,12 @@ struct Info {            // of a sequence, written by `sums`
 enum Kind { kNothing = 0, kPoint = 1, kAll = 2, kBut = 3, kLeft = 4 };
 // kPoint: all weight at `token`; kAll: exp; kBut: exp but for `token`; kLeft: max(p - q, 0)
 
+struct Judge {           // of a drafted token, written by `stats`
+  int x;                 // the token, -1 outside the vocabulary
+  float l, q;            // its logit and its draft probability
+  float u;
+};
+
 struct VerifyArgs {
   const void* logits;
   int64_t stride;
@@ -69,6 +75,7 @@ struct VerifyArgs {
   float* part_max;             // [rows][slices]
   int* part_arg;
   float* part_sum;
+  Judge* judge;                // [rows]
   Info* info;                  // [num_seqs]
   double* sums;                // [num_seqs][sum_slices]
   double* left;
@@ -174,15 +181,38 @@ __device__ __forceinline__ float rate_of(float temp) {
   return fmaxf(fminf(kLog2e / temp, 3e38f), 1e-30f);
 }
 
-// Workgroup (slice s, row r): maximum and sum of exp((l - maximum) / T) in one pass.  Where the
+// The drafted tokens of sequence i: what judges them beside the rows' statistics, in the shadow of
+// the rows' workgroups (three trips to memory).
+template <int FMT>
+__device__ __forceinline__ void judge_rows(const VerifyArgs& a, int i) {
+  int64_t first;
+  const int n = seq_rows(a, i, &first);
+  for (int j = threadIdx.x; j < n - 1; j += kThreads) {
+    const int64_t r = first + j, x = draft_at(a, r + 1), d = r - i;
+    Judge g{-1, kNegInf, 1.f, a.uniforms[r]};
+    if (x >= 0 && x < a.vocab) {
+      g.x = (int)x;
+      g.l = elem<FMT>(row_at<FMT>(a, r), x);
+      if (a.probs) g.q = d >= 0 && d < a.probs_rows ? a.probs[d * a.probs_stride + x] : 0.f;
+    }
+    a.judge[r] = g;
+  }
+}
+
+// A workgroup per sequence for judge_rows, then one per slice and row: maximum and sum of exp((l - maximum) / T) in one pass.  Where the
 // row is a point (T = 0, or a slice that holds a NaN or an infinity: the sum is NaN then), the
 // maximum and its first index instead.
 template <int FMT>
 __global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerifyArgs a) {
   constexpr int EB = FMT == kFmtF32 ? 4 : 2, PER = 16 / EB;
   constexpr int kBatch = 4;            // 16-byte words of a thread's step, the next in flight
-  const int s = blockIdx.x, t = threadIdx.x;
-  const int64_t r = blockIdx.y;
+  if (blockIdx.x < (unsigned)a.num_seqs) {
+    judge_rows<FMT>(a, (int)blockIdx.x);
+    return;
+  }
+  const unsigned unit = blockIdx.x - (unsigned)a.num_seqs;
+  const int64_t r = unit / (unsigned)a.slices;
+  const int s = (int)(unit - (unsigned)r * a.slices), t = threadIdx.x;
   const char* const row = static_cast<const char*>(row_at<FMT>(a, r));
   const int b0 = s * a.slice_len;
   const int b1 = b0 + a.slice_len < a.vocab ? b0 + a.slice_len : a.vocab;
@@ -379,20 +409,34 @@ __device__ __forceinline__ RowPart load_part(const VerifyArgs& a, int64_t r, int
   if (s >= a.slices) p = RowPart{};
   return p;
 }
+// f combined over groups of `width` lanes, as wave_all does over the wave.
+template <class OP>
+__device__ __forceinline__ double group_sum(double v, int width, OP op) {
+  if (width > 1) v = op(v, dpp<0xb1>(v));
+  if (width > 2) v = op(v, dpp<0x4e>(v));
+  if (width > 4) v = op(v, dpp<0x141>(v));
+  if (width > 8) v = op(v, dpp<0x140>(v));
+  if (width > 16) v = across<16>(v, op);
+  if (width > 32) v = across<32>(v, op);
+  return v;
+}
 __device__ __forceinline__ RowStats row_stats(const RowPart& p, int width, float k) {
-  RowStats f{p.top, p.arg, 0.0};
-  for (int m = 1; m < width; m <<= 1) {
-    const float ov = __shfl_xor(f.top, m, 64);
-    const int oi = __shfl_xor(f.arg, m, 64);
-    if (better(ov, oi, f.top, f.arg)) {
-      f.top = ov;
-      f.arg = oi;
-    }
-  }
-  f.sum = p.sum == 0.f ? 0.0
-          : p.top == f.top ? (double)p.sum
-                           : (double)p.sum * fast_exp2((p.top - f.top) * k);
-  for (int m = 1; m < width; m <<= 1) f.sum += __shfl_xor(f.sum, m, 64);
+  // (maximum, index) as one 64-bit word, moved like a double
+  auto word = [](float top, int arg) {
+    return __builtin_bit_cast(double, (uint64_t)__float_as_uint(top) << 32 | (uint32_t)arg);
+  };
+  auto top_of = [](double w) {
+    return __uint_as_float((uint32_t)(__builtin_bit_cast(uint64_t, w) >> 32));
+  };
+  auto arg_of = [](double w) { return (int)(uint32_t)__builtin_bit_cast(uint64_t, w); };
+  const double w = group_sum(word(p.top, p.arg), width, [&](double x, double y) {
+    return better(top_of(y), arg_of(y), top_of(x), arg_of(x)) ? y : x;
+  });
+  RowStats f{top_of(w), arg_of(w), 0.0};
+  f.sum = group_sum(p.sum == 0.f ? 0.0
+                    : p.top == f.top ? (double)p.sum
+                                     : (double)p.sum * fast_exp2((p.top - f.top) * k),
+                    width, [](double x, double y) { return x + y; });
   return f;
 }
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) <= 3.402823466e38f; }
@@ -472,7 +516,7 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs a) {
   __shared__ int reject;
   __shared__ double sums[kThreads / 64];
   __shared__ float tops[kAccept];
-  __shared__ int args[kAccept];
+  __shared__ int args[kAccept], drafts[kAccept];
   __shared__ double totals[kAccept];
   const Exp ex = make_exp(table, temp);
   int width = 1;                       // lanes that a row's slices take
@@ -490,24 +534,13 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs a) {
   int acc = 0, j0 = 0;
   for (;; j0 += kAccept) {
     const int m = n - j0 < kAccept ? n - j0 : kAccept;
-    const int64_t r = first + j0 + t;
     const bool judge = t < m && j0 + t < n - 1;
-    // the first rows' parts go out before the drafts' own entries, which take two round trips
     const int g = t / width, gs = kThreads / width;
-    RowPart part = load_part(a, first + j0 + (g < m ? g : 0), t & (width - 1));
-    int64_t x = -1;
-    float u = 0.f, lx = kNegInf, q = 1.f;
-    if (judge) {
-      x = draft_at(a, r + 1);
-      u = a.uniforms[r];
-      if (x >= 0 && x < a.vocab) {
-        lx = elem<FMT>(row_at<FMT>(a, r), x);
-        const int64_t d = r - i;
-        if (a.probs) q = d >= 0 && d < a.probs_rows ? a.probs[d * a.probs_stride + x] : 0.f;
-      }
-    }
+    const Judge d = a.judge[first + j0 + (t < m ? t : 0)];
+    RowPart next = load_part(a, first + j0 + (g < m ? g : 0), t & (width - 1));
     for (int j = g; j < m; j += gs) {
-      if (j != g) part = load_part(a, first + j0 + j, t & (width - 1));
+      const RowPart part = next;
+      next = load_part(a, first + j0 + (j + gs < m ? j + gs : j), t & (width - 1));
       const RowStats f = row_stats(part, width, k);
       if ((t & (width - 1)) == 0) {
         tops[j] = f.top;
@@ -517,11 +550,12 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs a) {
     }
     __syncthreads();
     if (t < m) {
+      drafts[t] = d.x;
       bool ok = false;
-      if (judge && x >= 0 && x < a.vocab) {
-        const double uq = (double)u * (double)q;
-        ok = temp > 0.f && finite(tops[t]) ? uq * totals[t] < ex(lx, tops[t])
-                                           : uq < (x == args[t] ? 1.0 : 0.0);
+      if (judge && d.x >= 0) {
+        const double uq = (double)d.u * (double)d.q;
+        ok = temp > 0.f && finite(tops[t]) ? uq * totals[t] < ex(d.l, tops[t])
+                                           : uq < (d.x == args[t] ? 1.0 : 0.0);
       }
       // the first row that is not accepted (the last has nothing to accept): t < m <= 64
       const uint64_t no = __builtin_amdgcn_ballot_w64(!ok);
@@ -546,9 +580,8 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs a) {
   } else if (a.probs) {
     f.kind = f.draft_row >= 0 && f.draft_row < a.probs_rows ? kLeft : kAll;
   } else {
-    const int64_t x = draft_at(a, r + 1);
     f.kind = kBut;
-    f.token = x >= 0 && x < a.vocab ? (int)x : -1;
+    f.token = drafts[acc - j0];
   }
   if (s == 0 && t == 0) a.info[i] = f;
   if (f.kind == kPoint) return;
@@ -735,7 +768,7 @@ size_t up(size_t n) { return (n + 255) / 256 * 256; }
 
 struct Sizes {
   int slices, sum_slices, sum_len;
-  size_t stat, info, sums, total;    // bytes of a part; three stats, two sums
+  size_t stat, judge, info, sums, total;   // bytes of a part; three stats, two sums
 };
 Sizes sizes_of(int64_t rows, int num_seqs, int vocab) {
   Sizes z;
@@ -747,17 +780,18 @@ Sizes sizes_of(int64_t rows, int num_seqs, int vocab) {
   z.sum_len = per * kSumSlice;
   z.sum_slices = (steps + per - 1) / per;
   z.stat = up((size_t)rows * z.slices * 4);
+  z.judge = up((size_t)rows * sizeof(Judge));
   z.info = up((size_t)num_seqs * sizeof(Info));
   z.sums = up((size_t)num_seqs * z.sum_slices * 8);
-  z.total = 3 * z.stat + z.info + 2 * z.sums;
+  z.total = 3 * z.stat + z.judge + z.info + 2 * z.sums;
   return z;
 }
 
 template <int FMT>
 int launch_verify(const VerifyArgs& a, hipStream_t s) {
   const dim3 wg(kThreads), per_seq((unsigned)a.sum_slices, (unsigned)a.num_seqs);
-  hipLaunchKernelGGL((verify_stats_kernel<FMT>), dim3((unsigned)a.slices, (unsigned)a.rows), wg,
-                     0, s, a);
+  hipLaunchKernelGGL((verify_stats_kernel<FMT>),
+                     dim3((unsigned)(a.num_seqs + a.rows * a.slices)), wg, 0, s, a);
   int rc = check_launch();
   if (rc != NDL_OK) return rc;
   hipLaunchKernelGGL((verify_sums_kernel<FMT>), per_seq, wg, 0, s, a);
@@ -830,9 +864,11 @@ extern "C" int ndl_verify_drafts(void* tokens, int32_t* accepted, const void* lo
   a.part_max = (float*)w;
   a.part_arg = (int*)(w + z.stat);
   a.part_sum = (float*)(w + 2 * z.stat);
-  a.info = (Info*)(w + 3 * z.stat);
-  a.sums = (double*)(w + 3 * z.stat + z.info);
-  a.left = (double*)(w + 3 * z.stat + z.info + z.sums);
+  w += 3 * z.stat;
+  a.judge = (Judge*)w;
+  a.info = (Info*)(w + z.judge);
+  a.sums = (double*)(w + z.judge + z.info);
+  a.left = (double*)(w + z.judge + z.info + z.sums);
   const hipStream_t s = (hipStream_t)stream;
   if (dtype_is_f32(dtype)) return launch_verify<kFmtF32>(a, s);
   return dtype_is_f16(dtype) ? launch_verify<kFmtF16>(a, s) : launch_verify<kFmtBF16>(a, s);
