@@ -23,6 +23,8 @@
 // Sums run in a fixed order without atomics: the same inputs give the same tokens.
 #include "ndl_common.hpp"
 
+#include <type_traits>
+
 namespace ndl {
 namespace {
 
@@ -257,26 +259,25 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerifyArgs a) {
       raise(l);
       sum += term(l);
     };
-    for (int w0 = t; w0 < words; w0 += kBatch * kThreads) {
-      u32x4 p[kBatch];
-#pragma unroll
-      for (int u = 0; u < kBatch; ++u) p[u] = next[u];
-      if (w0 + kBatch * kThreads < words) load(w0 + kBatch * kThreads);
+    // a step's entries; WHOLE: its words are all within the slice
+    auto step = [&](int w0, auto whole) {
+      constexpr bool WHOLE = decltype(whole)::value;
       float v[kBatch * PER], best = kNegInf;
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
-        const bool in = w0 + u * kThreads < words;
+        const bool in = WHOLE || w0 + u * kThreads < words;
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           if constexpr (FMT == kFmtF32) {
-            v[4 * u + x] = in ? __uint_as_float(p[u][x]) : kNegInf;
+            v[4 * u + x] = in ? __uint_as_float(next[u][x]) : kNegInf;
           } else {
             using T = Elt<FMT == kFmtF16>;
-            v[8 * u + 2 * x] = in ? T::lo(p[u][x]) : kNegInf;
-            v[8 * u + 2 * x + 1] = in ? T::hi(p[u][x]) : kNegInf;
+            v[8 * u + 2 * x] = in ? T::lo(next[u][x]) : kNegInf;
+            v[8 * u + 2 * x + 1] = in ? T::hi(next[u][x]) : kNegInf;
           }
         }
       }
+      if (w0 + kBatch * kThreads < words) load(w0 + kBatch * kThreads);
 #pragma unroll
       for (int e = 0; e < kBatch * PER; ++e) best = fmaxf(best, v[e]);
       raise(best);
@@ -284,7 +285,11 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerifyArgs a) {
 #pragma unroll
       for (int e = 0; e < kBatch * PER; ++e) part[e & 3] += term(v[e]);
       sum += (part[0] + part[1]) + (part[2] + part[3]);
-    }
+    };
+    int w0 = t;
+    for (; w0 + (kBatch - 1) * kThreads < words; w0 += kBatch * kThreads)
+      step(w0, std::true_type{});
+    if (w0 < words) step(w0, std::false_type{});
     if (t < h0 - b0) one(elem<FMT>(row, b0 + t));
     for (int i = tail + t; i < b1; i += kThreads) one(elem<FMT>(row, i));
     float wtop = top;
@@ -461,22 +466,22 @@ __device__ const double kPowers[64] = {
     0x1.ea4afa2a490dap+0, 0x1.efa1bee615a27p+0, 0x1.f50765b6e4540p+0, 0x1.fa7c1819e90d8p+0,
 };
 
-// exp((l - top) / T) in fp64, to about 1e-13 of it, 0 below 2^-900: 2^(n / 64) from the table, and
-// e^r, |r| <= ln 2 / 128, by its series to r^4.  n is read from the low bits of a sum with
-// 1.5 * 2^52, and added to the product's exponent: fp64 conversions run at a quarter of the rate.
+// exp((l - top) / T) in fp64, to about 1e-13 of it, 0 for a masked entry: 2^(n / 64) from the table,
+// and 2^(r / 64), |r| <= 1/2, by the exponential's series to the fourth power.  n is read from the
+// low bits of a sum with 1.5 * 2^52 (fp64 conversions run at a quarter of the rate).
 struct Exp {
   const double* table;     // kPowers in LDS
   double rate;             // 64 / (T ln 2)
   __device__ __forceinline__ double operator()(float l, float top) const {
-    const double z = ((double)l - (double)top) * rate;      // at most 0; -inf for a masked entry
+    constexpr double c = 0.01083042469624914545;            // ln 2 / 64
+    // at most 0; -inf and what underflows anyway to a power that does
+    const double z = __builtin_fmax(((double)l - (double)top) * rate, -140000.0);
     const double shifted = z + 6755399441055744.0;
     const int n = (int)(uint32_t)__builtin_bit_cast(uint64_t, shifted);
-    const double r = (z - (shifted - 6755399441055744.0)) * 0.01083042469624914545;  // ln 2 / 64
-    const double e =
-        fma(r, fma(r, fma(r, fma(r, 1.0 / 24, 1.0 / 6), 0.5), 1.0), 1.0) * table[n & 63];
-    const uint64_t w =
-        __builtin_bit_cast(uint64_t, e) + ((uint64_t)(uint32_t)((n >> 6) << 20) << 32);
-    return z > -57600.0 ? __builtin_bit_cast(double, w) : 0.0;
+    const double r = z - (shifted - 6755399441055744.0);
+    const double t = table[n & 63];
+    const double q = fma(fma(fma(r, c * c * c * c / 24, c * c * c / 6), r, c * c / 2), r, c) * r;
+    return __builtin_amdgcn_ldexp(fma(q, t, t), n >> 6);
   }
 };
 // Every thread calls it; a barrier is due before the first use.
@@ -486,10 +491,34 @@ __device__ __forceinline__ Exp make_exp(double* table, float temp) {
 }
 __device__ __forceinline__ double positive(double x) { return x > 0.0 ? x : 0.0; }   // NaN: 0
 
-constexpr int kRun = kSumSlice / kThreads;     // entries of a thread in flight
+constexpr int kRun = kSumSlice / kThreads;     // entries of a thread's step, next to each other
+static_assert(kRun == 8);
+
+// Entries v0 .. v0 + 7 of a row, -inf past b1.  A row begins at any multiple of its entries' size:
+// the loads are of unaligned words.
+template <int FMT>
+__device__ __forceinline__ void load_eight(const void* row, int v0, int b1, float (&l)[kRun]) {
+  if (v0 + kRun <= b1) {
+    if constexpr (FMT == kFmtF32) {
+      __builtin_memcpy(l, static_cast<const float*>(row) + v0, sizeof(l));
+    } else {
+      using T = Elt<FMT == kFmtF16>;
+      uint32_t w[4];
+      __builtin_memcpy(w, static_cast<const u16*>(row) + v0, sizeof(w));
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        l[2 * x] = T::lo(w[x]);
+        l[2 * x + 1] = T::hi(w[x]);
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int u = 0; u < kRun; ++u) l[u] = v0 + u < b1 ? elem<FMT>(row, v0 + u) : kNegInf;
+}
 
 // Entry v0 + u * T of a row for u < RUN, -inf past b1.
-template <int FMT, int T = kThreads, int RUN = kRun>
+template <int FMT, int T, int RUN>
 __device__ __forceinline__ void load_run(const void* row, int v0, int b1, float (&l)[RUN]) {
   // loaded without a branch: the loads would wait for one another
 #pragma unroll
@@ -587,15 +616,16 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs a) {
   if (f.kind == kPoint) return;
   const void* const row = row_at<FMT>(a, r);
   const int b0 = s * a.sum_len, b1 = b0 + a.sum_len < a.vocab ? b0 + a.sum_len : a.vocab;
+  const int but = f.kind == kBut ? f.token : -1;
   double z = 0.0;
-  for (int v0 = b0 + t; v0 < b1; v0 += kRun * kThreads) {
+  for (int v0 = b0 + t * kRun; v0 < b1; v0 += kSumSlice) {
     float l[kRun];
-    load_run<FMT>(row, v0, b1, l);
+    load_eight<FMT>(row, v0, b1, l);
 #pragma unroll
-    for (int u = 0; u < kRun; ++u) {
-      const double w = ex(l[u], f.top);
-      z += f.kind == kBut && v0 + u * kThreads == f.token ? 0.0 : w;
-    }
+    for (int u = 0; u < kRun; ++u)
+      if (v0 + u == but) l[u] = kNegInf;      // no weight
+#pragma unroll
+    for (int u = 0; u < kRun; ++u) z += ex(l[u], f.top);
   }
   z = wave_sum(z);
   if (lane == 0) sums[wv] = z;
@@ -624,10 +654,10 @@ __global__ __launch_bounds__(kThreads) void verify_left_kernel(VerifyArgs a) {
   const float* const q = a.probs + f.draft_row * a.probs_stride;
   const int b0 = s * a.sum_len, b1 = b0 + a.sum_len < a.vocab ? b0 + a.sum_len : a.vocab;
   double z = 0.0;
-  for (int v0 = b0 + t; v0 < b1; v0 += kRun * kThreads) {
+  for (int v0 = b0 + t * kRun; v0 < b1; v0 += kSumSlice) {
     float l[kRun], d[kRun];
-    load_run<FMT>(row, v0, b1, l);
-    load_run<kFmtF32>(q, v0, b1, d);
+    load_eight<FMT>(row, v0, b1, l);
+    load_eight<kFmtF32>(q, v0, b1, d);
 #pragma unroll
     for (int u = 0; u < kRun; ++u)
       z += positive(ex(l[u], f.top) * scale - positive((double)d[u]));
