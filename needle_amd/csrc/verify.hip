@@ -32,13 +32,15 @@ constexpr int kThreads = 256;
 constexpr int kStatSlice = 4096;     // elements of a slice at least
 constexpr int kStatWgs = 1536;       // workgroups wanted over all rows: what the GPU holds at once
 constexpr int kSumSlice = 2048;      // a step of a workgroup; slices are whole steps
-constexpr int kSumWgs = 2048;
+constexpr int kSumWgs = 2048;        // of sums and left: likewise
+constexpr int kStatSlices = 32;      // 8 rows' slices are combined at a time
 constexpr int kMaxSlices = 64;       // a lane of a wave each
-constexpr int kPickLen = 6144;       // elements of a chosen row's slice at most: they fit the LDS
+constexpr int kPickLen = 6144;       // elements of a chosen row's slice at most, for the last launch
 constexpr int kMaxVocab = 1 << 18;
-static_assert(kMaxVocab <= kMaxSlices * kPickLen, "a slice's weights fit the LDS");
-constexpr int kPickThreads = 1024;   // of the last launch: one workgroup per sequence
-constexpr int kPickRun = kPickLen / kPickThreads;
+static_assert(kMaxVocab <= kMaxSlices * kPickLen, "a row's slices cover it");
+constexpr int kRun = kSumSlice / kThreads;      // entries of a thread's step, next to each other
+constexpr int kPickThreads = kPickLen / kRun;   // of the last launch: one workgroup per sequence
+static_assert(kRun == 8 && kPickThreads % 64 == 0);
 constexpr int kAccept = 64;          // rows judged at a time
 
 struct Info {            // of a sequence, written by `sums`
@@ -80,7 +82,7 @@ struct VerifyArgs {
   Judge* judge;                // [rows]
   Info* info;                  // [num_seqs]
   double* sums;                // [num_seqs][sum_slices]
-  double* left;
+  double* left;                // likewise
 };
 
 template <int FMT>
@@ -201,9 +203,9 @@ __device__ __forceinline__ void judge_rows(const VerifyArgs& a, int i) {
   }
 }
 
-// A workgroup per sequence for judge_rows, then one per slice and row: maximum and sum of exp((l - maximum) / T) in one pass.  Where the
-// row is a point (T = 0, or a slice that holds a NaN or an infinity: the sum is NaN then), the
-// maximum and its first index instead.
+// A workgroup per sequence for judge_rows, then one per row and slice: maximum and sum of
+// exp((l - maximum) / T) in one pass.  Where the row is a point (T = 0, or a slice that holds a NaN
+// or an infinity: the sum is NaN then), the maximum and its first index instead.
 template <int FMT>
 __global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerifyArgs a) {
   constexpr int EB = FMT == kFmtF32 ? 4 : 2, PER = 16 / EB;
@@ -491,9 +493,6 @@ __device__ __forceinline__ Exp make_exp(double* table, float temp) {
 }
 __device__ __forceinline__ double positive(double x) { return x > 0.0 ? x : 0.0; }   // NaN: 0
 
-constexpr int kRun = kSumSlice / kThreads;     // entries of a thread's step, next to each other
-static_assert(kRun == 8);
-
 // Entries v0 .. v0 + 7 of a row, -inf past b1.  A row begins at any multiple of its entries' size:
 // the loads are of unaligned words.
 template <int FMT>
@@ -515,20 +514,6 @@ __device__ __forceinline__ void load_eight(const void* row, int v0, int b1, floa
   }
 #pragma unroll
   for (int u = 0; u < kRun; ++u) l[u] = v0 + u < b1 ? elem<FMT>(row, v0 + u) : kNegInf;
-}
-
-// Entry v0 + u * T of a row for u < RUN, -inf past b1.
-template <int FMT, int T, int RUN>
-__device__ __forceinline__ void load_run(const void* row, int v0, int b1, float (&l)[RUN]) {
-  // loaded without a branch: the loads would wait for one another
-#pragma unroll
-  for (int u = 0; u < RUN; ++u) {
-    const int v = v0 + u * T;
-    l[u] = elem<FMT>(row, v < b1 ? v : b1 - 1);
-  }
-#pragma unroll
-  for (int u = 0; u < RUN; ++u)
-    if (v0 + u * T >= b1) l[u] = kNegInf;
 }
 
 // Workgroup (slice, sequence): the sequence's accepted drafts and chosen row, then the sum of its
@@ -685,16 +670,16 @@ __device__ __forceinline__ double wave_prefix(double v, int lane) {
   return v + before;
 }
 
-// Workgroup per sequence: its tokens.  The slice whose prefix passes the goal; its weights into
-// LDS; then the thread (each takes a run of the slice), then the entry.
+// Workgroup per sequence: its tokens.  The slice whose prefix passes the goal; then the thread (each
+// takes a run of the slice), then the entry.
 template <int FMT>
 __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(VerifyArgs a) {
   const int i = blockIdx.x, t = threadIdx.x, lane = t & 63, wv = t >> 6;
   int64_t first;
   const int n = seq_rows(a, i, &first);
-  const int ns = a.sum_slices;
-  const double plain = lane < ns ? a.sums[(int64_t)i * ns + lane] : 0.0;
-  const double less = a.probs && lane < ns ? a.left[(int64_t)i * ns + lane] : 0.0;
+  const double plain = lane < a.sum_slices ? a.sums[(int64_t)i * a.sum_slices + lane] : 0.0;
+  const double less =
+      a.probs && lane < a.sum_slices ? a.left[(int64_t)i * a.sum_slices + lane] : 0.0;
   if (n <= 0) return;
   const Info f = a.info[i];
   if (f.accepted >= n) return;     // cu has changed since the launches before
@@ -706,7 +691,6 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(VerifyArgs a)
     if (t == 0) put_token(a, to, f.token);
     return;
   }
-  extern __shared__ double run[];      // the slice's weights
   __shared__ double table[64];
   __shared__ double wsum[kPickThreads / 64];
   __shared__ int cross[kPickThreads / 64], last[kPickThreads / 64];
@@ -734,26 +718,19 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(VerifyArgs a)
   const void* const row = row_at<FMT>(a, f.row);
   const float* const q = left ? a.probs + f.draft_row * a.probs_stride : nullptr;
   const int b0 = pick * a.sum_len, b1 = b0 + a.sum_len < a.vocab ? b0 + a.sum_len : a.vocab;
+  const int v0 = b0 + t * kRun;
+  float l[kRun], d[kRun];
+  load_eight<FMT>(row, v0, b1, l);
+  if (left) load_eight<kFmtF32>(q, v0, b1, d);
+  double run[kRun], mine = 0.0;
   __syncthreads();
-  for (int v0 = b0 + t; v0 < b1; v0 += kPickRun * kPickThreads) {
-    float l[kPickRun], d[kPickRun];
-    load_run<FMT, kPickThreads, kPickRun>(row, v0, b1, l);
-    if (left) load_run<kFmtF32, kPickThreads, kPickRun>(q, v0, b1, d);
 #pragma unroll
-    for (int e = 0; e < kPickRun; ++e) {
-      const int v = v0 + e * kPickThreads;
-      double w = ex(l[e], f.top);
-      if (left) w = positive(w * scale - positive((double)d[e]));
-      if (f.kind == kBut && v == f.token) w = 0.0;
-      if (v < b1) run[v - b0] = w;
-    }
+  for (int e = 0; e < kRun; ++e) {
+    run[e] = ex(l[e], f.top);
+    if (left) run[e] = positive(run[e] * scale - positive((double)d[e]));
+    if (f.kind == kBut && v0 + e == f.token) run[e] = 0.0;
+    mine += run[e];
   }
-  __syncthreads();
-  const int per = (b1 - b0 + kPickThreads - 1) / kPickThreads;
-  const int v0 = t * per < b1 - b0 ? t * per : b1 - b0;
-  const int v1 = v0 + per < b1 - b0 ? v0 + per : b1 - b0;
-  double mine = 0.0;
-  for (int v = v0; v < v1; ++v) mine += run[v];
   // prefix over the threads
   const double incl = wave_prefix(mine, lane);
   if (lane == 63) wsum[wv] = incl;
@@ -778,35 +755,36 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(VerifyArgs a)
   }
   if (t != (who >= 0 ? who : end)) return;
   int token = v0;
-  for (int v = v0; v < v1; ++v) {
-    c += run[v];
-    if (run[v] > 0.0) {
-      token = v;
-      if (c > goal) break;
+  bool found = false;
+#pragma unroll
+  for (int e = 0; e < kRun; ++e) {
+    c += run[e];
+    if (run[e] > 0.0 && !found) {
+      token = v0 + e;
+      found = c > goal;
     }
   }
-  put_token(a, to, b0 + token);
+  put_token(a, to, token);
 }
 
-int slices_for(int64_t rows, int vocab, int least, int wgs) {
-  const int64_t by_len = (vocab + least - 1) / least;
-  const int64_t by_wgs = (wgs + rows - 1) / rows;
-  int64_t s = by_len < by_wgs ? by_len : by_wgs;
-  return (int)(s < 1 ? 1 : s > kMaxSlices ? kMaxSlices : s);
-}
 size_t up(size_t n) { return (n + 255) / 256 * 256; }
 
 struct Sizes {
-  int slices, sum_slices, sum_len;
+  int slices, sum_len, sum_slices;
   size_t stat, judge, info, sums, total;   // bytes of a part; three stats, two sums
 };
 Sizes sizes_of(int64_t rows, int num_seqs, int vocab) {
   Sizes z;
-  z.slices = slices_for(rows, vocab, kStatSlice, kStatWgs);
+  const int64_t by_len = (vocab + kStatSlice - 1) / kStatSlice;
+  const int64_t by_wgs = (kStatWgs + rows - 1) / rows;
+  const int64_t few = by_len < by_wgs ? by_len : by_wgs;
+  z.slices = (int)(few < kStatSlices ? few : kStatSlices);
+  // one round of workgroups, as few slices as that takes: each judges its sequence first (96 rows
+  // of 50,257 float32: sums and left 8.8 + 7.0 us with 13 slices, 10.6 + 6.0 with 25)
   const int steps = (vocab + kSumSlice - 1) / kSumSlice;
-  int per = steps / slices_for(num_seqs, vocab, kSumSlice, kSumWgs);   // steps of a slice
-  if (per > kPickLen / kSumSlice) per = kPickLen / kSumSlice;
-  if (per < (steps + kMaxSlices - 1) / kMaxSlices) per = (steps + kMaxSlices - 1) / kMaxSlices;
+  const int64_t wanted = ((int64_t)steps * num_seqs + kSumWgs - 1) / kSumWgs;
+  const int most = kPickLen / kSumSlice, least = (steps + kMaxSlices - 1) / kMaxSlices;
+  const int per = wanted < least ? least : wanted > most ? most : (int)wanted;
   z.sum_len = per * kSumSlice;
   z.sum_slices = (steps + per - 1) / per;
   z.stat = up((size_t)rows * z.slices * 4);
@@ -819,21 +797,22 @@ Sizes sizes_of(int64_t rows, int num_seqs, int vocab) {
 
 template <int FMT>
 int launch_verify(const VerifyArgs& a, hipStream_t s) {
-  const dim3 wg(kThreads), per_seq((unsigned)a.sum_slices, (unsigned)a.num_seqs);
+  const dim3 wg(kThreads);
+  const unsigned seqs = (unsigned)a.num_seqs;
   hipLaunchKernelGGL((verify_stats_kernel<FMT>),
                      dim3((unsigned)(a.num_seqs + a.rows * a.slices)), wg, 0, s, a);
   int rc = check_launch();
   if (rc != NDL_OK) return rc;
-  hipLaunchKernelGGL((verify_sums_kernel<FMT>), per_seq, wg, 0, s, a);
+  hipLaunchKernelGGL((verify_sums_kernel<FMT>), dim3((unsigned)a.sum_slices, seqs), wg, 0, s, a);
   rc = check_launch();
   if (rc != NDL_OK) return rc;
   if (a.probs != nullptr) {
-    hipLaunchKernelGGL((verify_left_kernel<FMT>), per_seq, wg, 0, s, a);
+    hipLaunchKernelGGL((verify_left_kernel<FMT>), dim3((unsigned)a.sum_slices, seqs), wg, 0, s,
+                       a);
     rc = check_launch();
     if (rc != NDL_OK) return rc;
   }
-  hipLaunchKernelGGL((verify_pick_kernel<FMT>), dim3((unsigned)a.num_seqs), dim3(kPickThreads),
-                     (size_t)a.sum_len * sizeof(double), s, a);
+  hipLaunchKernelGGL((verify_pick_kernel<FMT>), dim3(seqs), dim3(kPickThreads), 0, s, a);
   return check_launch();
 }
 
