@@ -989,9 +989,12 @@ const void* kernel_of(int nt, int waves) {
 // Slots a share has at least: two tiles for each of four waves.
 constexpr int kMinChunk = 8;
 // Tiles up to which a row block is one workgroup's, whatever else there is: the shares' scan, their
-// parts and the merge launch cost more (us, shares / whole, 28/4 heads of 128, 8 sequences of 800
-// tokens: 15.3 / 9.8; of 1,500, 47 tiles, 13.0 / 13.6).
-constexpr int kWholeTiles = 32;
+// parts and the merge launch cost more (us, shares / whole, decode of 8 sequences: 14/2 heads of 64,
+// 1,000 tokens 12.6 / 8.1, 1,500 12.8 / 10.1, 3,000 14.7 / 16.2; 32/8 of 128 15.4 / 12.0, 16.1 /
+// 15.5, 18.5 / 25.4; 500 tokens in tables of 1,500, all that the host knows of them, 14.4 / 7.7).
+// Chunks of 5 tokens and 64 sequences part at about 2,000 to 3,000 tokens, and at less where one
+// sequence is much longer than the others.
+constexpr int kWholeTiles = 48;
 // Empty slots before a row block, one column tile or two (its start, its waves' sums): us at 0, 1,
 // 2 and 4, decode as above 54.3, 53.2, 54.2, 54.0; chunks of 1 to 8 tokens after 512 to 4,096
 // 68.5, 67.8, 66.9, 64.9.

@@ -87,6 +87,23 @@ def test_many_sequences(n):
     assert torch.equal(pool[0].cpu(), codes) and torch.equal(pool[1].cpu(), scales)
 
 
+@pytest.mark.parametrize("n", [64, 65, 300])
+@pytest.mark.parametrize("count", [1, 3, 40])
+def test_many_row_blocks_in_shares(n, count):
+    """Tables of 1,700 keys and more are cut into shares: row blocks of nothing, of one tile and of
+    many, more of them than a wave's lanes or four steps of the scan."""
+    counts = [1] * n if count == 1 else [(i * 7) % count for i in range(n)]
+    if count == 40:
+        counts = counts[:65]
+    lens = [(37 * i) % 400 - 1 for i in range(len(counts))]
+    lens[len(counts) // 2] = 1700
+    c = Case((4, 2, 64, 16), counts, lens, seed=n, extra_cols=10)
+    keys = c.table.shape[1] * 16
+    assert ops.fp8_attention_workspace_bytes(len(counts), int(c.cu[-1]), max(counts), keys, 4, 2,
+                                             64) > 0
+    c.check(c.run(decode=count == 1))
+
+
 def test_one_long_context():
     """One sequence over all workgroups, in blocks of 1,024 tokens."""
     c = Case((4, 1, 64, 1024), [1], [70001], seed=3)
