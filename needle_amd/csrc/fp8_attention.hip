@@ -32,6 +32,11 @@
 //     idle or unevenly loaded, all row blocks' tiles of a kv head laid end to end and cut into
 //     equal shares, one per resident workgroup; what a share holds of a row block goes to a
 //     workspace and is merged by a second launch.
+// Measured (us, bytes read at): 64 sequences of 512 to 4,096 tokens, 32/8 heads of 128, one token
+// each 49.0 + 4.8 of merge, 5.4 TB/s in the first launch; 24 sequences of 4,096 to 32,768, 28/4 heads,
+// float16, 73.6 + 4.7, 5.9 TB/s; 1 to 8 tokens each after 512 to 4,096 58.4 + 7.9, 4.6 TB/s.  A few
+// short sequences take 5 us, of which each step of a wave (a tile) is 1: about 250 instructions, two
+// waves to a SIMD; sixteen waves or deeper rings measured the same or slower.
 #include "fp8.hpp"
 
 namespace ndl {

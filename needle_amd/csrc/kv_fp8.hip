@@ -104,6 +104,11 @@ __device__ __forceinline__ u32x2 quant8(const u32x4& w, float mul) {
 // a lane's elements of cos and sin are the same in every round.  A token's items are the 2 Hkv
 // rows of K and V, then the H rows of q.  All loads go out first, then the slot is looked up; what
 // lies past the last item loads a valid one again and stores nothing.
+//
+// Bound by the bytes: 15,596 tokens of 28/4 heads of 128 with RoPE (279.6 MB, four fifths of them q
+// in and out) take 50.3 us, 5.6 TB/s.  Two rounds a wave: one takes 54 us (cos, sin and the slot read
+// twice as often), six 54.6 (fewer waves).  A step of a few tokens is its launch and two trips to
+// memory: 4.2 us.
 constexpr int kRounds = 2;
 
 template <int D, bool F16>
@@ -237,6 +242,9 @@ __device__ __forceinline__ int64_t slot_row_of_lane(const QuantArgs& a, int64_t 
 // 2 Hkv rows, in the order of the tokens, so that a wave stores 1 KiB at once.  Lane k first finds
 // the slot of the wave's k-th token.  Positions that have no slot read as zeros, tokens past the
 // last sequence are not written.
+//
+// Bound by the bytes: 34,224 tokens of 8 heads of 128 (210.8 MB) take 37.2 us, 5.7 TB/s, with eight
+// loads of a lane in flight; one load a wave, its slot looked up before it, takes 41.
 template <int D, bool F16>
 __global__ __launch_bounds__(256) void kv_read_fp8_kernel(QuantArgs a) {
   constexpr int CPR = D / 8, U = kReadItems / 64;

@@ -12,12 +12,16 @@
 // (a NaN, nothing left by a mask), stand for the point at the row's argmax in torch's order.
 // The reference samples one row at a time on the host (needle/model/sampler.py:16-46).
 //
-// Bound: every logit read once.  Three or four launches:
-//   stats   row slices: maximum, its index, sum of exponentials, in one pass (fp32 terms)
+// Bound: every logit read once, and what each launch waits for.  Three or four launches (us at 304
+// rows of 64 sequences, 151,936 bfloat16 logits, draft distributions / 5 rows of one, without):
+//   stats   row slices: maximum, its index, sum of exponentials, in one pass (fp32 terms); beside
+//           them what judges the drafts                            20.2 (4.6 TB/s) / 3.4
 //   sums    per sequence: accepts (every workgroup by itself, from the slices), then the chosen
-//           row's weights summed by slices
-//   left    with draft distributions: the sums of max(p - q, 0) by slices
-//   pick    finds the slice, then the token
+//           row's weights summed by slices                         12.6 / 5.2
+//   left    with draft distributions: the sums of max(p - q, 0) by slices   8.7
+//   pick    finds the slice, then the token                        5.6 / 4.6
+// stats issues about 10 instructions an entry (12 of the 20 us), sums and left 15 of fp64 for the
+// 64 chosen rows; the rest of the later three is trips to memory that wait for one another.
 // The chosen row's weights and sums are in fp64: a token's border is found among up to 2^17
 // others, where fp32 sums (2^-24 of the total each) would pick a neighbour now and then.
 // Sums run in a fixed order without atomics: the same inputs give the same tokens.
