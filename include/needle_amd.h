@@ -40,6 +40,7 @@
  *   ndl_kv_append_fp8   rotary embedding, quantisation and append into a pool of e4m3 codes
  *   ndl_kv_read_fp8     ranges of cached tokens read back in the model's format
  *   ndl_fp8_attention   attention of one token or a chunk per sequence over that pool
+ *   ndl_fp8_decode_append  a decode step's append (and rotary embedding) and its attention
  *   ndl_verify_drafts   accepted drafts and the next token of every sequence, from the
  *                       target's logits and given random numbers
  *
@@ -556,8 +557,8 @@ int ndl_kv_read_fp8(void* k_out, void* v_out, const void* codes, const void* sca
  * keys (context_lens[i] + tokens, at most max_blocks_per_seq * block_size; long chunks attend none
  * past it): they choose how the work is split.  Long chunks (224 rows of max_seqlen times the
  * group, 2^24 scores by these bounds) unpack their keys into a 16-bit pool in the workspace first.
- * The workspace (ndl_fp8_attention_workspace_bytes of the same sizes, max_keys cut to the table's, on the same
- * device; 0: none) is 256-byte aligned and belongs to one call at a time.
+ * The workspace (ndl_fp8_attention_workspace_bytes of the same sizes, max_keys cut to the table's,
+ * on the same device; 0: none) is 256-byte aligned and belongs to one call at a time.
  */
 size_t ndl_fp8_attention_workspace_bytes(int num_seqs, int64_t num_tokens, int max_seqlen,
                                          int64_t max_keys, int num_heads, int num_kv_heads,
@@ -569,6 +570,24 @@ int ndl_fp8_attention(void* out, const void* q, int64_t q_tok_stride, const void
                       int max_seqlen, int64_t max_keys, int num_heads, int num_kv_heads,
                       int head_dim, int block_size, int dtype, float scale, void* workspace,
                       size_t workspace_bytes, ndl_stream_t stream);
+
+/*
+ * A decode step in one launch (and the merge of a split): the rows k and v [num_seqs][num_kv_heads]
+ * [head_dim] (token strides multiples of 8, 16-byte aligned) appended at context_lens[i] as
+ * ndl_kv_append_fp8 does, and the attention of ndl_fp8_attention without cu_seqlens, with the same
+ * pool bytes and the same output.  cos and sin [num_seqs][head_dim] (both or neither): q and k are
+ * the projections' outputs and are rotated first.  No block that a sequence attends may be written
+ * for another one.  Workspace: ndl_fp8_attention_workspace_bytes(num_seqs, num_seqs, 1,
+ * max_blocks_per_seq * block_size, ...).
+ */
+int ndl_fp8_decode_append(void* out, const void* q, int64_t q_tok_stride, const void* k,
+                          int64_t k_tok_stride, const void* v, int64_t v_tok_stride,
+                          const void* cos, const void* sin, int64_t cs_stride, void* codes,
+                          void* scales, int64_t num_blocks, const int32_t* block_table,
+                          int64_t bt_row_stride, int max_blocks_per_seq,
+                          const int32_t* context_lens, int num_seqs, int num_heads,
+                          int num_kv_heads, int head_dim, int block_size, int dtype, float scale,
+                          void* workspace, size_t workspace_bytes, ndl_stream_t stream);
 
 /*
  * Verification of drafted tokens.  Sequence i has rows cu_seqlens[i] .. cu_seqlens[i + 1] (at

@@ -51,6 +51,7 @@ EXPORTED_SYMBOLS = (
     "ndl_kv_read_fp8",
     "ndl_fp8_attention_workspace_bytes",
     "ndl_fp8_attention",
+    "ndl_fp8_decode_append",
     "ndl_verify_drafts_workspace_bytes",
     "ndl_verify_drafts",
 )
@@ -204,6 +205,16 @@ _SIGNATURES = {
         _c_p, _c_p, _c_i64,                             # codes, scales, NB
         _c_p, _c_i64, _c_i32,                           # block_table, row stride, W
         _c_p, _c_p, _c_i32, _c_i64, _c_i32, _c_i64,     # cu, ctx, B, T, max_seqlen, max_keys
+        _c_i32, _c_i32, _c_i32, _c_i32, _c_i32,         # H, Hkv, D, bs, dtype
+        _c_f32, _c_p, _c_sz, _c_p,                      # scale, workspace, bytes, stream
+    ]),
+    "ndl_fp8_decode_append": (_c_i32, [
+        _c_p, _c_p, _c_i64,                             # out, q, q stride
+        _c_p, _c_i64, _c_p, _c_i64,                     # k, k stride, v, v stride
+        _c_p, _c_p, _c_i64,                             # cos, sin, stride
+        _c_p, _c_p, _c_i64,                             # codes, scales, NB
+        _c_p, _c_i64, _c_i32,                           # block_table, row stride, W
+        _c_p, _c_i32,                                   # ctx, B
         _c_i32, _c_i32, _c_i32, _c_i32, _c_i32,         # H, Hkv, D, bs, dtype
         _c_f32, _c_p, _c_sz, _c_p,                      # scale, workspace, bytes, stream
     ]),

@@ -36,6 +36,7 @@ decltype(&ndl_kv_append_fp8) p_kv_append_fp8 = nullptr;
 decltype(&ndl_kv_read_fp8) p_kv_read_fp8 = nullptr;
 decltype(&ndl_fp8_attention_workspace_bytes) p_fp8_workspace = nullptr;
 decltype(&ndl_fp8_attention) p_fp8_attention = nullptr;
+decltype(&ndl_fp8_decode_append) p_fp8_decode_append = nullptr;
 decltype(&ndl_verify_drafts_workspace_bytes) p_verify_workspace = nullptr;
 decltype(&ndl_verify_drafts) p_verify_drafts = nullptr;
 
@@ -364,7 +365,8 @@ PyObject* kv_append_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const c10::DeviceGuard guard(codes.device());
   at::Tensor out;
   if (q != nullptr) {
-    if (q->dim() != 3 || q->size(0) != tokens || q->scalar_type() != k.scalar_type()) Py_RETURN_NONE;
+    if (q->dim() != 3 || q->size(0) != tokens || q->scalar_type() != k.scalar_type())
+      Py_RETURN_NONE;
     heads = q->size(1);
     if (heads == 0 || !fits_int(heads) || !read_rows_of(*q, codes, heads, p.d, &qs)) Py_RETURN_NONE;
     out = at::empty({tokens, heads, p.d}, q->options());
@@ -423,10 +425,13 @@ PyObject* kv_read_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 // fp8_attention(q, codes, scales, block_table, cu_seqlens or None, context_lens, max_seqlen,
-// max_keys (0: the table's), scale, num_heads, num_kv_heads, head_dim): the output.
+// max_keys (0: the table's), scale, num_heads, num_kv_heads, head_dim[, k, v, cos or None, sin or
+// None: the decode step's rows to append]): the output.
 PyObject* fp8_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 12 || p_fp8_attention == nullptr || validating()) Py_RETURN_NONE;
+  if ((n != 12 && n != 16) || p_fp8_attention == nullptr || p_fp8_decode_append == nullptr ||
+      validating())
+    Py_RETURN_NONE;
   const at::Tensor* t[4];
   for (int i = 0; i < 4; ++i)
     if ((t[i] = gpu_tensor(args[i])) == nullptr) Py_RETURN_NONE;
@@ -451,6 +456,18 @@ PyObject* fp8_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
       (cu != nullptr ? cu->size(0) != seqs + 1 : tokens != seqs || most != 1))
     Py_RETURN_NONE;
   if (keys == 0 || keys > width * p.bs) keys = width * p.bs;
+  const at::Tensor *k = nullptr, *v = nullptr, *cos = nullptr, *sin = nullptr;
+  int64_t ks = 0, vs = 0, cs = 0;
+  if (n == 16) {
+    if (cu != nullptr || (k = gpu_tensor(args[12])) == nullptr ||
+        (v = gpu_tensor(args[13])) == nullptr || !maybe_tensor(args[14], &cos) ||
+        !maybe_tensor(args[15], &sin) || (cos == nullptr) != (sin == nullptr) ||
+        k->scalar_type() != q.scalar_type() || v->scalar_type() != q.scalar_type() ||
+        !read_rows_of(*k, codes, hkv, d, &ks) || !read_rows_of(*v, codes, hkv, d, &vs) ||
+        k->size(0) != tokens || v->size(0) != tokens ||
+        (cos != nullptr && !read_rope(*cos, *sin, q, tokens, d, &cs)))
+      Py_RETURN_NONE;
+  }
   const c10::DeviceGuard guard(codes.device());
   at::Tensor out = at::empty({tokens, heads, d}, q.options()), ws;
   const size_t need = p_fp8_workspace((int)seqs, tokens, (int)most, keys, (int)heads, (int)hkv,
@@ -460,12 +477,20 @@ PyObject* fp8_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const ndl_stream_t s = stream_of(codes);
   int rc;
   Py_BEGIN_ALLOW_THREADS
-  rc = p_fp8_attention(outp, q.data_ptr(), qs, codes.data_ptr(), scales.data_ptr(), p.num_blocks,
-                       (const int32_t*)table.data_ptr(), table.stride(0), (int)width,
-                       cu ? (const int32_t*)cu->data_ptr() : nullptr,
-                       (const int32_t*)lens.data_ptr(), (int)seqs, tokens, (int)most, keys,
-                       (int)heads, (int)hkv, (int)d, (int)p.bs, dtype_code(q.scalar_type()), scale,
-                       wsp, need, s);
+  if (k != nullptr)
+    rc = p_fp8_decode_append(outp, q.data_ptr(), qs, k->data_ptr(), ks, v->data_ptr(), vs,
+                             cos ? cos->data_ptr() : nullptr, cos ? sin->data_ptr() : nullptr, cs,
+                             codes.data_ptr(), scales.data_ptr(), p.num_blocks,
+                             (const int32_t*)table.data_ptr(), table.stride(0), (int)width,
+                             (const int32_t*)lens.data_ptr(), (int)seqs, (int)heads, (int)hkv,
+                             (int)d, (int)p.bs, dtype_code(q.scalar_type()), scale, wsp, need, s);
+  else
+    rc = p_fp8_attention(outp, q.data_ptr(), qs, codes.data_ptr(), scales.data_ptr(), p.num_blocks,
+                         (const int32_t*)table.data_ptr(), table.stride(0), (int)width,
+                         cu ? (const int32_t*)cu->data_ptr() : nullptr,
+                         (const int32_t*)lens.data_ptr(), (int)seqs, tokens, (int)most, keys,
+                         (int)heads, (int)hkv, (int)d, (int)p.bs, dtype_code(q.scalar_type()), scale,
+                         wsp, need, s);
   Py_END_ALLOW_THREADS
   if (rc != NDL_OK) Py_RETURN_NONE;
   return THPVariable_Wrap(std::move(out));
@@ -548,6 +573,7 @@ PyObject* init(PyObject*, PyObject* d) {
   NDL_TAKE(p_kv_read_fp8, "ndl_kv_read_fp8");
   NDL_TAKE(p_fp8_workspace, "ndl_fp8_attention_workspace_bytes");
   NDL_TAKE(p_fp8_attention, "ndl_fp8_attention");
+  NDL_TAKE(p_fp8_decode_append, "ndl_fp8_decode_append");
   NDL_TAKE(p_verify_workspace, "ndl_verify_drafts_workspace_bytes");
   NDL_TAKE(p_verify_drafts, "ndl_verify_drafts");
 #undef NDL_TAKE

@@ -33,10 +33,10 @@
 //     equal shares, one per resident workgroup; what a share holds of a row block goes to a
 //     workspace and is merged by a second launch.
 // Measured (us, bytes read at): 64 sequences of 512 to 4,096 tokens, 32/8 heads of 128, one token
-// each 49.0 + 4.8 of merge, 5.4 TB/s in the first launch; 24 sequences of 4,096 to 32,768, 28/4 heads,
-// float16, 73.6 + 4.7, 5.9 TB/s; 1 to 8 tokens each after 512 to 4,096 58.4 + 7.9, 4.6 TB/s.  A few
-// short sequences take 5 us, of which each step of a wave (a tile) is 1: about 250 instructions, two
-// waves to a SIMD; sixteen waves or deeper rings measured the same or slower.
+// each 49.0 + 4.8 of merge, 5.4 TB/s in the first launch; 24 sequences of 4,096 to 32,768, 28/4
+// heads, float16, 73.6 + 4.7, 5.9 TB/s; 1 to 8 tokens each after 512 to 4,096 58.4 + 7.9, 4.6 TB/s.
+// A few short sequences take 5 us, of which each step of a wave (a tile) is 1: about 250
+// instructions, two waves to a SIMD; sixteen waves or deeper rings measured the same or slower.
 #include "fp8.hpp"
 
 namespace ndl {
@@ -49,11 +49,17 @@ struct ChunkArgs {
   u16* out;
   const u16* q;
   int64_t q_stride;
-  const uint8_t* codes;
-  const uint8_t* scales;
+  uint8_t* codes;               // written only with new rows
+  uint8_t* scales;
   int64_t plane_rows;           // rows (token, head) of a plane
   int64_t num_blocks;
   int num_heads, num_kv_heads, group;
+  const u16* new_k;             // rows to append, of one token per sequence (null: none)
+  const u16* new_v;
+  int64_t k_stride, v_stride;
+  const u16* cos;               // with new rows: q and k are not rotated yet (null: they are)
+  const u16* sin;
+  int64_t cs_stride;
   const int32_t* block_table;
   int64_t bt_row_stride;
   int max_blocks;
@@ -234,9 +240,40 @@ struct Shape {
   static constexpr int kLds = (NW * kRing > kSums ? NW * kRing : kSums) + kMl;
 };
 
-// A workgroup's share of the row blocks of one kv head.
-template <int D, bool F16, int NT, int NW>
-__global__ __launch_bounds__(64 * NW, 8 / NW) void chunk_attention_kernel(ChunkArgs a) {
+// Rotates a column's q in the operand layout of chunk_attention_kernel: lane (j, c) holds head_dim
+// 64 (s >> 1) + 16 j + 8 (s & 1) .. + 7 in q[s].
+template <int D, bool F16, class X8>
+__device__ __forceinline__ void rope_q(X8* q, const u16* cos, const u16* sin, int j) {
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const int d = (D == 128 ? 16 * j : 16 * (j & 1)) + 8 * x;      // of the pair's first half
+    const u32x4 clo = ld16(cos + d), chi = ld16(cos + d + D / 2);
+    const u32x4 slo = ld16(sin + d), shi = ld16(sin + d + D / 2);
+    u32x4 lo = __builtin_bit_cast(u32x4, q[x]), hi, rlo, rhi;
+    if constexpr (D == 128) {
+      hi = __builtin_bit_cast(u32x4, q[2 + x]);
+      rope8<F16>(lo, hi, clo, chi, slo, shi, rlo, rhi);
+      q[x] = __builtin_bit_cast(X8, rlo);
+      q[2 + x] = __builtin_bit_cast(X8, rhi);
+    } else {
+      // the other half is 32 lanes away
+      u32x4 mine = lo, other;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) other[w] = (uint32_t)__shfl_xor((int)mine[w], 32, 64);
+      lo = j < 2 ? mine : other;
+      hi = j < 2 ? other : mine;
+      rope8<F16>(lo, hi, clo, chi, slo, shi, rlo, rhi);
+      q[x] = __builtin_bit_cast(X8, j < 2 ? rlo : rhi);
+    }
+  }
+}
+
+// A workgroup's share of the row blocks of one kv head.  NEW: the sequence's new row is quantised
+// by the wave whose tile holds its position, which puts it into the ring for itself and into the
+// pool.  (head_dim 64: 128 registers, as without, so that as many workgroups are resident.)
+template <int D, bool F16, int NT, int NW, bool NEW = false>
+__global__ __launch_bounds__(64 * NW, NEW && D == 64 ? 4 : 8 / NW)
+void chunk_attention_kernel(ChunkArgs a) {
   using T = Elt<F16>;
   using X8 = typename T::x8;
   using S = Shape<D, NT, NW>;
@@ -324,6 +361,18 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void chunk_attention_kernel(ChunkA
       const int64_t k = it.pos + tok + 1;
       lim[nt] = (int)(k < it.cap ? k : it.cap);
     }
+    // the new row's position in the table (past the end the last column is written again, as an
+    // append does) and the step of this wave that attends it
+    int at_new = -1, u_new = -1;
+    if constexpr (NEW) {
+      if (it.pos >= 0)
+        at_new = (int)(it.pos < it.cap ? it.pos
+                                       : it.cap - (1 << bshift) + (it.pos & ((1 << bshift) - 1)));
+      at_new = __builtin_amdgcn_readfirstlane(at_new);
+      const int tile = at_new >> 5;
+      if (at_new >= 0 && tile >= t0 && tile < t1 && (tile - t0) % NW == wv)
+        u_new = (tile - t0) / NW;
+    }
     const int64_t k_first = it.pos + 1 < it.cap ? it.pos + 1 : it.cap;
     const int all_keys = (int)it.keys();      // of the last token
     const int min_keys = k_first < 0 ? 0 : (int)k_first;   // of the first
@@ -375,11 +424,68 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void chunk_attention_kernel(ChunkA
     for (int d = 0; d < S::kDepth; ++d)
       if (d < cnt) issue(d, d);
 
+    // while these are on their way: q rotated, and the new row quantised.  A lane has 8 codes of
+    // each half of k (or, in the odd groups of D / 16 lanes, of v).
+    constexpr int CPH = D / 16;
+    const bool is_v = (lane / CPH) & 1;
+    u32x2 xlo, xhi;
+    int xbyte = 0;
+    if constexpr (NEW) {
+      const u16* const cs = a.cos + it.tok0 * a.cs_stride;
+      const u16* const sn = a.sin + it.tok0 * a.cs_stride;
+      if (a.cos != nullptr) rope_q<D, F16>(q[0], cs, sn, j);
+      if (u_new >= 0) {
+        const int d0 = 8 * (lane % CPH);
+        const u16* const src = (is_v ? a.new_v + it.tok0 * a.v_stride
+                                     : a.new_k + it.tok0 * a.k_stride) + head * D + d0;
+        u32x4 lo = ld16(src), hi = ld16(src + D / 2);
+        if (a.cos != nullptr) {
+          u32x4 rlo, rhi;
+          rope8<F16>(lo, hi, ld16(cs + d0), ld16(cs + d0 + D / 2), ld16(sn + d0),
+                     ld16(sn + d0 + D / 2), rlo, rhi);
+          lo = is_v ? lo : rlo;
+          hi = is_v ? hi : rhi;
+        }
+        xbyte = scale_byte<CPH, F16>(lo, hi);
+        const float mul = __uint_as_float((uint32_t)(254 - xbyte) << 23);
+        xlo = quant8<F16>(lo, mul);
+        xhi = quant8<F16>(hi, mul);
+      }
+    }
+
     int slot = 0;
     for (int u = 0; u < cnt; ++u) {
       vm_wait_groups<S::kLoads, S::kDepth - 1>(cnt - 1 - u);
       asm volatile("" ::: "memory");
-      const unsigned char* st = ring + slot * S::kStage;
+      unsigned char* const st = ring + slot * S::kStage;
+      if constexpr (NEW) {
+        if (u == u_new) {       // (LDS accesses of a wave are in order: the reads below see it)
+          int ln = lane;        // addresses worked out here: they would hold registers all along
+          asm volatile("" : "+v"(ln));
+          if (ln < 2 * CPH) {
+            const int d0 = 8 * (ln % CPH), r = at_new & 15, half = (at_new >> 4) & 1;
+            const bool v = ln >= CPH;
+            auto place = [&](int d) {
+              if (v) return S::kRowTile + (16 * half + r) * D + d;
+              const int row = D == 128 ? r : r >> 1;
+              const int chunk = D == 128 ? d >> 4 : (r & 1) * 4 + (d >> 4);
+              return half * 16 * D + row * 128 + ((chunk ^ (row & 7)) << 4) + (d & 15);
+            };
+            *reinterpret_cast<u32x2*>(st + place(d0)) = xlo;
+            *reinterpret_cast<u32x2*>(st + place(d0 + D / 2)) = xhi;
+            if (d0 == 0) st[2 * S::kRowTile + (v ? 32 : 0) + 16 * half + r] = (uint8_t)xbyte;
+            const int b = table[at_new >> bshift];
+            if (b >= 0 && b < a.num_blocks) {
+              const int64_t row = (v ? a.plane_rows : 0) + (((int64_t)b * Hkv + head) << bshift) +
+                                  (at_new & ((1 << bshift) - 1));
+              *reinterpret_cast<u32x2*>(a.codes + row * D + d0) = xlo;
+              *reinterpret_cast<u32x2*>(a.codes + row * D + d0 + D / 2) = xhi;
+              if (d0 == 0) a.scales[row] = (uint8_t)xbyte;
+            }
+          }
+          asm volatile("" ::: "memory");
+        }
+      }
       // operands: K half s, 16 codes at head_dim 64 h + 16 j of row c; V rows of slots 8 j + i
       u32x4 kc[2][D / 64];
 #pragma unroll
@@ -983,7 +1089,10 @@ struct Plan {
 };
 
 template <int D, bool F16>
-const void* kernel_of(int nt, int waves) {
+const void* kernel_of(int nt, int waves, bool append = false) {
+  if (append)       // one token per sequence: one column tile
+    return waves == 4 ? (const void*)chunk_attention_kernel<D, F16, 1, 4, true>
+                      : (const void*)chunk_attention_kernel<D, F16, 1, 8, true>;
   if (waves == 4)
     return nt == 1 ? (const void*)chunk_attention_kernel<D, F16, 1, 4>
                    : (const void*)chunk_attention_kernel<D, F16, 2, 4>;
@@ -994,9 +1103,9 @@ const void* kernel_of(int nt, int waves) {
 // Slots a share has at least: two tiles for each of four waves.
 constexpr int kMinChunk = 8;
 // Tiles up to which a row block is one workgroup's, whatever else there is: the shares' scan, their
-// parts and the merge launch cost more (us, shares / whole, decode of 8 sequences: 14/2 heads of 64,
-// 1,000 tokens 12.6 / 8.1, 1,500 12.8 / 10.1, 3,000 14.7 / 16.2; 32/8 of 128 15.4 / 12.0, 16.1 /
-// 15.5, 18.5 / 25.4; 500 tokens in tables of 1,500, all that the host knows of them, 14.4 / 7.7).
+// parts and the merge launch cost more (us, shares / whole, decode of 8 sequences: 14/2 heads of
+// 64, 1,000 tokens 12.6 / 8.1, 1,500 12.8 / 10.1, 3,000 14.7 / 16.2; 32/8 of 128 15.4 / 12.0,
+// 16.1 / 15.5, 18.5 / 25.4; 500 tokens in tables of 1,500, all that the host knows of them, 14.4 / 7.7).
 // Chunks of 5 tokens and 64 sequences part at about 2,000 to 3,000 tokens, and at less where one
 // sequence is much longer than the others.
 constexpr int kWholeTiles = 48;
@@ -1057,8 +1166,8 @@ int launch(ChunkArgs a, int nt, int waves, hipStream_t s) {
   const int64_t wgs = units * a.num_kv_heads;
   if (wgs > 0x7fffffff) return NDL_ERR_INVALID_ARG;
   void* args[] = {&a};
-  if (hipLaunchKernel(kernel_of<D, F16>(nt, waves), dim3((unsigned)wgs), dim3(64 * waves), args, 0,
-                      s) != hipSuccess)
+  if (hipLaunchKernel(kernel_of<D, F16>(nt, waves, a.new_k != nullptr), dim3((unsigned)wgs),
+                      dim3(64 * waves), args, 0, s) != hipSuccess)
     return NDL_ERR_LAUNCH;
   const int rc = check_launch();
   if (rc != NDL_OK || a.shares == 0) return rc;
@@ -1089,15 +1198,15 @@ extern "C" size_t ndl_fp8_attention_workspace_bytes(int num_seqs, int64_t num_to
   return p.ml_bytes + p.acc_bytes;
 }
 
-extern "C" int ndl_fp8_attention(void* out, const void* q, int64_t q_tok_stride,
-                                 const void* codes, const void* scales, int64_t num_blocks,
-                                 const int32_t* block_table, int64_t bt_row_stride,
-                                 int max_blocks_per_seq, const int32_t* cu_seqlens,
-                                 const int32_t* context_lens, int num_seqs, int64_t num_tokens,
-                                 int max_seqlen, int64_t max_keys, int num_heads,
-                                 int num_kv_heads, int head_dim, int block_size, int dtype,
-                                 float scale, void* workspace, size_t workspace_bytes,
-                                 ndl_stream_t stream) {
+// Both entry points; `a` holds the new rows and the rotation of the second one.
+static int fp8_attention(ndl::ChunkArgs a, void* out, const void* q, int64_t q_tok_stride,
+                         void* codes, void* scales, int64_t num_blocks,
+                         const int32_t* block_table, int64_t bt_row_stride,
+                         int max_blocks_per_seq, const int32_t* cu_seqlens,
+                         const int32_t* context_lens, int num_seqs, int64_t num_tokens,
+                         int max_seqlen, int64_t max_keys, int num_heads, int num_kv_heads,
+                         int head_dim, int block_size, int dtype, float scale, void* workspace,
+                         size_t workspace_bytes, ndl_stream_t stream) {
   using namespace ndl;
   if (!dtype_supported(dtype) || !shape_ok(head_dim, block_size, num_heads, num_kv_heads))
     return NDL_ERR_UNSUPPORTED;
@@ -1113,7 +1222,6 @@ extern "C" int ndl_fp8_attention(void* out, const void* q, int64_t q_tok_stride,
     return NDL_ERR_INVALID_ARG;
   if (((uintptr_t)out | (uintptr_t)q | (uintptr_t)codes) & 15u || (uintptr_t)scales & 3u)
     return NDL_ERR_INVALID_ARG;
-  ChunkArgs a{};
   a.plane_rows = num_blocks * num_kv_heads * (int64_t)block_size;
   // a scale's address is the pool's and a 32-bit offset; positions are 32-bit
   if (a.plane_rows > 0x7fffffff || (int64_t)max_blocks_per_seq * block_size > 0x7fffff00)
@@ -1123,8 +1231,8 @@ extern "C" int ndl_fp8_attention(void* out, const void* q, int64_t q_tok_stride,
   a.out = (u16*)out;
   a.q = (const u16*)q;
   a.q_stride = q_tok_stride;
-  a.codes = (const uint8_t*)codes;
-  a.scales = (const uint8_t*)scales;
+  a.codes = (uint8_t*)codes;
+  a.scales = (uint8_t*)scales;
   a.num_blocks = num_blocks;
   a.num_heads = num_heads;
   a.num_kv_heads = num_kv_heads;
@@ -1173,4 +1281,54 @@ extern "C" int ndl_fp8_attention(void* out, const void* q, int64_t q_tok_stride,
   if (head_dim == 128)
     return f16 ? launch<128, true>(a, p.nt, p.waves, s) : launch<128, false>(a, p.nt, p.waves, s);
   return f16 ? launch<64, true>(a, p.nt, p.waves, s) : launch<64, false>(a, p.nt, p.waves, s);
+}
+
+extern "C" int ndl_fp8_attention(void* out, const void* q, int64_t q_tok_stride,
+                                 const void* codes, const void* scales, int64_t num_blocks,
+                                 const int32_t* block_table, int64_t bt_row_stride,
+                                 int max_blocks_per_seq, const int32_t* cu_seqlens,
+                                 const int32_t* context_lens, int num_seqs, int64_t num_tokens,
+                                 int max_seqlen, int64_t max_keys, int num_heads,
+                                 int num_kv_heads, int head_dim, int block_size, int dtype,
+                                 float scale, void* workspace, size_t workspace_bytes,
+                                 ndl_stream_t stream) {
+  return fp8_attention({}, out, q, q_tok_stride, (void*)codes, (void*)scales, num_blocks,
+                       block_table, bt_row_stride, max_blocks_per_seq, cu_seqlens, context_lens,
+                       num_seqs, num_tokens, max_seqlen, max_keys, num_heads, num_kv_heads,
+                       head_dim, block_size, dtype, scale, workspace, workspace_bytes, stream);
+}
+
+extern "C" int ndl_fp8_decode_append(void* out, const void* q, int64_t q_tok_stride, const void* k,
+                                     int64_t k_tok_stride, const void* v, int64_t v_tok_stride,
+                                     const void* cos, const void* sin, int64_t cs_stride,
+                                     void* codes, void* scales, int64_t num_blocks,
+                                     const int32_t* block_table, int64_t bt_row_stride,
+                                     int max_blocks_per_seq, const int32_t* context_lens,
+                                     int num_seqs, int num_heads, int num_kv_heads, int head_dim,
+                                     int block_size, int dtype, float scale, void* workspace,
+                                     size_t workspace_bytes, ndl_stream_t stream) {
+  using namespace ndl;
+  if (num_seqs > 0 && head_dim > 0 && num_kv_heads > 0) {
+    const int64_t row = (int64_t)num_kv_heads * head_dim;
+    if (!k || !v || k_tok_stride < row || v_tok_stride < row ||
+        (k_tok_stride | v_tok_stride) & 7 || ((uintptr_t)k | (uintptr_t)v) & 15u)
+      return NDL_ERR_INVALID_ARG;
+    if ((cos == nullptr) != (sin == nullptr) ||
+        (cos != nullptr && (cs_stride < head_dim || (cs_stride & 7) ||
+                            ((uintptr_t)cos | (uintptr_t)sin) & 15u)))
+      return NDL_ERR_INVALID_ARG;
+  }
+  ChunkArgs a{};
+  a.new_k = (const u16*)k;
+  a.new_v = (const u16*)v;
+  a.k_stride = k_tok_stride;
+  a.v_stride = v_tok_stride;
+  a.cos = (const u16*)cos;
+  a.sin = (const u16*)sin;
+  a.cs_stride = cs_stride;
+  const int64_t keys = (int64_t)max_blocks_per_seq * block_size;
+  return fp8_attention(a, out, q, q_tok_stride, codes, scales, num_blocks, block_table,
+                       bt_row_stride, max_blocks_per_seq, nullptr, context_lens, num_seqs,
+                       num_seqs, 1, keys > 0 ? keys : 1, num_heads, num_kv_heads, head_dim,
+                       block_size, dtype, scale, workspace, workspace_bytes, stream);
 }

@@ -73,32 +73,6 @@ __device__ __forceinline__ int64_t slot_row(const QuantArgs& a, int64_t t) {
   return ((b * a.num_kv_heads) << a.block_shift) + (p & ((1 << a.block_shift) - 1));
 }
 
-// Largest finite magnitude of the two 16-bit elements of w, as 16 bits; `inf`: the format's
-// infinity.
-__device__ __forceinline__ uint32_t finite_max(uint32_t w, uint32_t inf) {
-  const uint32_t a = w & 0x7fffu, b = (w >> 16) & 0x7fffu;
-  const uint32_t x = a < inf ? a : 0u, y = b < inf ? b : 0u;
-  return x > y ? x : y;
-}
-
-// Two 16-bit elements -> two codes in the low half (HI: the high half) of `old`.
-template <bool F16, bool HI>
-__device__ __forceinline__ int quant2(uint32_t w, float mul, int old) {
-  using T = Elt<F16>;
-  // what is not finite becomes NaN (a saturating conversion would hide an infinity)
-  const float nan = __uint_as_float(0x7fc00000u);
-  constexpr uint32_t inf = F16 ? 0x7c00u : 0x7f80u;
-  const float x = (w & 0x7fffu) < inf ? T::lo(w) * mul : nan;
-  const float y = ((w >> 16) & 0x7fffu) < inf ? T::hi(w) * mul : nan;
-  return __builtin_amdgcn_cvt_pk_fp8_f32(x, y, old, HI);
-}
-template <bool F16>
-__device__ __forceinline__ u32x2 quant8(const u32x4& w, float mul) {
-  const int a = quant2<F16, true>(w[1], mul, quant2<F16, false>(w[0], mul, 0));
-  const int b = quant2<F16, true>(w[3], mul, quant2<F16, false>(w[2], mul, 0));
-  return u32x2{(uint32_t)a, (uint32_t)b};
-}
-
 // One wave per (token, kRounds rounds of 64 items); an item is 8 elements of a row's first half and
 // the 8 they rotate with, so D / 16 lanes hold a row and its maximum is a butterfly over them, and
 // a lane's elements of cos and sin are the same in every round.  A token's items are the 2 Hkv
@@ -171,23 +145,7 @@ __global__ __launch_bounds__(256) void kv_append_fp8_kernel(QuantArgs a) {
       }
       continue;
     }
-    constexpr uint32_t inf = F16 ? 0x7c00u : 0x7f80u;
-    uint32_t m = 0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint32_t x = finite_max(lo[i][e], inf), y = finite_max(hi[i][e], inf);
-      m = m > x ? m : x;
-      m = m > y ? m : y;
-    }
-#pragma unroll
-    for (int o = 1; o < CPH; o <<= 1) {
-      const uint32_t x = (uint32_t)__shfl_xor((int)m, o, 64);
-      m = m > x ? m : x;
-    }
-    // 448 = 1.75 * 2^8: the row's exponent less 8, one more where its mantissa is past 1.75
-    const uint32_t bits = __float_as_uint(Elt<F16>::lo(m));
-    const int e8 = (int)(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
-    const int byte = e8 < 1 ? 1 : e8;
+    const int byte = scale_byte<CPH, F16>(lo[i], hi[i]);
     const float mul = __uint_as_float((uint32_t)(254 - byte) << 23);
     if (live && slot >= 0) {
       const int h = is_v ? row - Hkv : row;

@@ -22,9 +22,9 @@ q and k already rotated, for callers that apply RoPE themselves
   _decode   (attention.py:140-159): ndl_paged_decode_append (the one-token-per-sequence
                                     append and the attention in one launch)
 
-With an 8-bit pool (kv_cache an ops.Fp8KVCache) the step is ndl_kv_append_fp8 (RoPE of q and k,
-quantisation and append of k and v in one launch), then ndl_fp8_attention over the pool, a prefill
-as a chunk and a decode step as one token per sequence.
+With an 8-bit pool (kv_cache an ops.Fp8KVCache) a prefill is ndl_kv_append_fp8 (RoPE of q and k,
+quantisation and append of k and v in one launch), then ndl_fp8_attention over the pool as a chunk;
+a decode step is ndl_fp8_decode_append, both in one launch.
 
 No host synchronisation happens on either path: the decode split-K grid is
 sized from block_table's width, prefill from max_seqlen (both host-known).
@@ -173,13 +173,16 @@ class Attention(nn.Module):
              cos, sin):
         """The step over an 8-bit pool."""
         cu = cu_seqlens if is_prefill else None
+        heads = (self.scale, self.num_heads, self.num_kv_heads, self.head_dim)
+        if self.fuse_rope and not is_prefill:
+            return ops.paged_decode_fp8(q, *pool, block_table, context_lens, *heads, new_k=k,
+                                        new_v=v, cos=cos, sin=sin)
         if self.fuse_rope:
             q = ops.kv_append_fp8(k, v, *pool, block_table, context_lens, cu, q=q, cos=cos,
                                   sin=sin)
         else:
             q, k = apply_rope(q, k, cos, sin)
             ops.kv_append_fp8(k, v, *pool, block_table, context_lens, cu)
-        heads = (self.scale, self.num_heads, self.num_kv_heads, self.head_dim)
         if is_prefill:
             return ops.varlen_prefill_fp8(q, *pool, block_table, cu_seqlens, context_lens,
                                           int(max_seqlen), *heads)

@@ -825,6 +825,19 @@ def _check_table(block_table: torch.Tensor, num_blocks: int, device) -> int:
     return block_table.shape[0]
 
 
+def _check_rope(cos, sin, dtype, n_tok, d, dev) -> int:
+    """Token stride of cos and sin [n_tok, d]."""
+    for name, x in (("cos", cos), ("sin", sin)):
+        if x.dtype != dtype:
+            raise TypeError(f"{name} dtype must match k")
+        if x.dim() != 2 or x.shape[0] != n_tok or x.shape[1] != d:
+            raise ValueError(f"{name} must be [{n_tok}, {d}], got {tuple(x.shape)}")
+        if x.device != dev or x.stride(1) != 1:
+            raise ValueError(f"{name} rows must be contiguous on {dev}")
+    _require(cos.stride(0) == sin.stride(0) or n_tok <= 1, "cos and sin token strides differ")
+    return cos.stride(0) if n_tok > 1 else d
+
+
 def kv_append_fp8(k: torch.Tensor, v: torch.Tensor, kv_codes: torch.Tensor,
                   kv_scales: torch.Tensor, block_table: torch.Tensor,
                   context_lens: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None, *,
@@ -856,13 +869,7 @@ def kv_append_fp8(k: torch.Tensor, v: torch.Tensor, kv_codes: torch.Tensor,
     _require((cos is None) == (sin is None), "pass both cos and sin, or neither")
     h, qs, cs = 0, 0, 0
     if cos is not None:
-        for name, x in (("cos", cos), ("sin", sin)):
-            if x.dim() != 2 or x.shape[0] != n_tok or x.shape[1] != d:
-                raise ValueError(f"{name} must be [{n_tok}, {d}], got {tuple(x.shape)}")
-            if x.device != dev or x.stride(1) != 1:
-                raise ValueError(f"{name} rows must be contiguous on {dev}")
-        _require(cos.stride(0) == sin.stride(0) or n_tok <= 1, "cos and sin token strides differ")
-        cs = cos.stride(0) if n_tok > 1 else d
+        cs = _check_rope(cos, sin, dtype, n_tok, d, dev)
     if q is not None:
         _require(cos is not None, "q is passed to be rotated: pass cos and sin")
         if q.dim() != 3:
@@ -936,11 +943,12 @@ def kv_read_fp8(kv_codes: torch.Tensor, kv_scales: torch.Tensor, block_table: to
 
 
 def _fp8_attention(q, kv_codes, kv_scales, block_table, cu_seqlens, context_lens, max_seqlen,
-                   max_keys, scale, num_heads, num_kv_heads, head_dim, out, workspace):
+                   max_keys, scale, num_heads, num_kv_heads, head_dim, out, workspace, *new):
+    """new: what a decode step appends and its rotation, (new_k, new_v, cos, sin), or nothing."""
     if out is None and workspace is None and _lib.NATIVE is not None:
         out = _lib.NATIVE.fp8_attention(q, kv_codes, kv_scales, block_table, cu_seqlens,
                                         context_lens, max_seqlen, max_keys, scale, num_heads,
-                                        num_kv_heads, head_dim)
+                                        num_kv_heads, head_dim, *new)
         if out is not None:
             return out
     nb, hkv, bs, d = _check_fp8_cache(kv_codes, kv_scales)
@@ -966,6 +974,18 @@ def _fp8_attention(q, kv_codes, kv_scales, block_table, cu_seqlens, context_lens
                  and out.dtype == q.dtype and out.device == dev,
                  f"out must be a contiguous {q.dtype} [{n_tok}, {num_heads}, {head_dim}] "
                  f"tensor on {dev}")
+    ks = vs = cs = 0
+    new_k, new_v, cos, sin = new or (None,) * 4
+    if new:
+        _require(new_k is not None and new_v is not None, "new_k and new_v go together")
+        for name, x in (("new_k", new_k), ("new_v", new_v)):
+            _require(x.dtype == q.dtype, f"{name} dtype must match q", TypeError)
+            _require(x.shape[0] == n_seqs, f"{name} must have one row per sequence")
+        ks = _rows("new_k", new_k, num_kv_heads, head_dim, dev)
+        vs = _rows("new_v", new_v, num_kv_heads, head_dim, dev)
+        _require((cos is None) == (sin is None), "cos and sin go together")
+        if cos is not None:
+            cs = _check_rope(cos, sin, q.dtype, n_seqs, head_dim, dev)
     if n_tok == 0 or n_seqs == 0:
         return out
     w = block_table.shape[1]
@@ -979,6 +999,15 @@ def _fp8_attention(q, kv_codes, kv_scales, block_table, cu_seqlens, context_lens
         if need and (workspace is None or workspace.numel() * workspace.element_size() < need
                      or workspace.device != dev):
             workspace = decode_workspace(need, dev)
+        if new:
+            rc = lib.ndl_fp8_decode_append(
+                out.data_ptr(), q.data_ptr(), qs, new_k.data_ptr(), ks, new_v.data_ptr(), vs,
+                _ptr(cos), _ptr(sin), cs, kv_codes.data_ptr(), kv_scales.data_ptr(), nb,
+                block_table.data_ptr(), block_table.stride(0), w, context_lens.data_ptr(),
+                n_seqs, num_heads, num_kv_heads, head_dim, bs, _DTYPES[q.dtype], float(scale),
+                _ptr(workspace) if need else None, need, _stream(dev))
+            _lib.check(rc, "ndl_fp8_decode_append")
+            return out
         rc = lib.ndl_fp8_attention(
             out.data_ptr(), q.data_ptr(), qs, kv_codes.data_ptr(), kv_scales.data_ptr(), nb,
             block_table.data_ptr(), block_table.stride(0), w, _ptr(cu_seqlens),
@@ -1003,13 +1032,27 @@ def paged_decode_fp8(q: torch.Tensor, kv_codes: torch.Tensor, kv_scales: torch.T
                      block_table: torch.Tensor, context_lens: torch.Tensor, scale: float,
                      num_heads: int, num_kv_heads: int, head_dim: int, *,
                      out: Optional[torch.Tensor] = None,
-                     workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+                     workspace: Optional[torch.Tensor] = None,
+                     new_k: Optional[torch.Tensor] = None, new_v: Optional[torch.Tensor] = None,
+                     cos: Optional[torch.Tensor] = None,
+                     sin: Optional[torch.Tensor] = None) -> torch.Tensor:
     """paged_decode over an 8-bit pool (Fp8KVCache): q [num_seqs, H, D] in bfloat16 or float16,
     sequence i attends min(context_lens[i] + 1, W * block_size) tokens.  Append (and rotate q)
-    with kv_append_fp8 first.  workspace: as decode_workspace gives, of
-    fp8_attention_workspace_bytes, for one call at a time."""
+    with kv_append_fp8 first, or hand the step's rows to this call.  workspace: as
+    decode_workspace gives, of fp8_attention_workspace_bytes, for one call at a time.
+
+    new_k / new_v ([num_seqs, Hkv, D]): the step's append, done in the same launch, with the same
+    pool bytes and output as kv_append_fp8 followed by this call.  Requires that no two sequences
+    attend the same block that one of them writes (as BlockAllocator's tables guarantee).
+    cos / sin ([num_seqs, D], with new_k / new_v): q and new_k are not yet rotated; the launch
+    rotates both first."""
+    new = ()
+    if new_k is not None or new_v is not None:
+        new = (new_k, new_v, cos, sin)
+    else:
+        _require(cos is None and sin is None, "cos / sin need new_k / new_v")
     return _fp8_attention(q, kv_codes, kv_scales, block_table, None, context_lens, 1, 0, scale,
-                          num_heads, num_kv_heads, head_dim, out, workspace)
+                          num_heads, num_kv_heads, head_dim, out, workspace, *new)
 
 
 def varlen_prefill_fp8(q: torch.Tensor, kv_codes: torch.Tensor, kv_scales: torch.Tensor,

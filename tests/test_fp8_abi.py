@@ -72,6 +72,28 @@ def test_attention_refusals(lib):
         assert lib.ndl_fp8_attention_workspace_bytes(*bad) == 0
 
 
+def test_decode_append_refusals(lib):
+    def step(out=P, q=P, qs=512, k=P, ks=128, v=P, vs=128, cos=P, sin=P, cs=64, codes=P, scales=P,
+             nb=4, table=P, stride=500, w=500, ctx=P, n=3, h=8, hkv=2, d=64, bs=16, dtype=0, ws=P,
+             size=0):
+        return lib.ndl_fp8_decode_append(out, q, qs, k, ks, v, vs, cos, sin, cs, codes, scales, nb,
+                                         table, stride, w, ctx, n, h, hkv, d, bs, dtype, 0.1, ws,
+                                         size, None)
+    for bad in (dict(dtype=2), dict(d=96, qs=768, ks=192, vs=192, cs=96), dict(bs=12), dict(h=9),
+                dict(h=34), dict(nb=1 << 27), dict(w=1 << 30, stride=1 << 30)):
+        assert step(**{**dict(qs=4096), **bad}) == -2, bad
+    for bad in (dict(k=None), dict(v=None), dict(ks=120), dict(vs=132), dict(k=P + 8),
+                dict(v=P + 2), dict(cos=None), dict(sin=None), dict(cs=60), dict(cs=68),
+                dict(cos=P + 4), dict(out=None), dict(q=None), dict(ctx=None), dict(table=None),
+                dict(codes=P + 8), dict(qs=500), dict(n=-1), dict(nb=0), dict(w=0),
+                dict(stride=499)):
+        assert step(**bad) == -1, bad
+    need = lib.ndl_fp8_attention_workspace_bytes(3, 3, 1, 8000, 8, 2, 64, 16)
+    assert need > 0
+    assert step(size=need - 1) == -3 and step(ws=None, size=need) == -3
+    assert step(n=0) == 0
+
+
 def test_verify_refusals(lib):
     def verify(tokens=P, acc=P, logits=P, stride=100, dtype=0, ids=P, cu=P, u=P, temp=None,
                probs=None, ds=0, rows=4, n=2, vocab=100, ws=P, size=0):
