@@ -63,6 +63,17 @@ __device__ __forceinline__ int scale_byte(const u32x4& lo, const u32x4& hi) {
   return e8 < 1 ? 1 : e8;
 }
 
+// lds_dma16 with an address of each lane's own.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void lds_dma16_each(const void* src, uint32_t lds_addr) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+               :
+               : "s"(__builtin_amdgcn_readfirstlane(lds_addr)), "v"(src)
+               : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
 // varlen_prefill.hip's attention for a caller with long, uneven prefixes: as
 // ndl_varlen_prefill_split, but split too where whole tiles would leave much of their last round
 // idle.  Its workspace: prefill_rounds_workspace_bytes.

@@ -240,33 +240,84 @@ struct Shape {
   static constexpr int kLds = (NW * kRing > kSums ? NW * kRing : kSums) + kMl;
 };
 
-// Rotates a column's q in the operand layout of chunk_attention_kernel: lane (j, c) holds head_dim
-// 64 (s >> 1) + 16 j + 8 (s & 1) .. + 7 in q[s].
-template <int D, bool F16, class X8>
-__device__ __forceinline__ void rope_q(X8* q, const u16* cos, const u16* sin, int j) {
+// 8 elements of x rotated with the other half's, by rope8's roundings: x cos + turned sin.
+template <bool F16>
+__device__ __forceinline__ u32x4 rope_half(const u32x4& x, const u32x4& turned, const u32x4& c,
+                                           const u32x4& s) {
+#pragma clang fp contract(off)
+  using T = Elt<F16>;
+  u32x4 out;
 #pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    const int d = (D == 128 ? 16 * j : 16 * (j & 1)) + 8 * x;      // of the pair's first half
-    const u32x4 clo = ld16(cos + d), chi = ld16(cos + d + D / 2);
-    const u32x4 slo = ld16(sin + d), shi = ld16(sin + d + D / 2);
-    u32x4 lo = __builtin_bit_cast(u32x4, q[x]), hi, rlo, rhi;
-    if constexpr (D == 128) {
-      hi = __builtin_bit_cast(u32x4, q[2 + x]);
-      rope8<F16>(lo, hi, clo, chi, slo, shi, rlo, rhi);
-      q[x] = __builtin_bit_cast(X8, rlo);
-      q[2 + x] = __builtin_bit_cast(X8, rhi);
-    } else {
-      // the other half is 32 lanes away
-      u32x4 mine = lo, other;
+  for (int w = 0; w < 4; ++w) {
+    const uint32_t xc = T::pack(T::lo(x[w]) * T::lo(c[w]), T::hi(x[w]) * T::hi(c[w]));
+    const uint32_t ts = T::pack(T::lo(turned[w]) * T::lo(s[w]), T::hi(turned[w]) * T::hi(s[w]));
+    out[w] = T::pack(T::lo(xc) + T::lo(ts), T::hi(xc) + T::hi(ts));
+  }
+  return out;
+}
+
+// A decode step's new row as the projections left it, and its cos and sin: the four rows go
+// straight to 1 KiB of LDS of the wave's own before the lengths arrive, and are used while the
+// ring's first loads are under way, so that they take no registers in between.
+template <int D, bool F16>
+struct NewRow {
+  static constexpr int kBytes = 1024, kRow = 2 * D;     // k, v, cos, sin
+  static constexpr int CPH = D / 16;
+  const unsigned char* at;
+  __device__ __forceinline__ void load(const ChunkArgs& a, int64_t tok, int head, int lane,
+                                       uint32_t lds) const {
+    const int row = (lane / (D / 8)) & 3;      // (head_dim 64: all of it twice)
+    const u16* src = (row == 1 ? a.new_v + tok * a.v_stride : a.new_k + tok * a.k_stride) +
+                     (int64_t)head * D;
+    if (row >= 2 && a.cos != nullptr) src = (row == 2 ? a.cos : a.sin) + tok * a.cs_stride;
+    lds_dma16_each(src + 8 * (lane % (D / 8)), lds);
+  }
+  __device__ __forceinline__ u32x4 part(int row, int d) const {
+    return *reinterpret_cast<const u32x4*>(at + row * kRow + 2 * d);
+  }
+  // q in the operand layout of chunk_attention_kernel: lane (j, c) holds head_dim 64 (i >> 1) +
+  // 16 j + 8 (i & 1) .. + 7 in q[i].
+  template <class X8>
+  __device__ __forceinline__ void rotate(X8* q, int j) const {
+    constexpr int KS = D / 32;
+    u32x4 x[KS];
 #pragma unroll
-      for (int w = 0; w < 4; ++w) other[w] = (uint32_t)__shfl_xor((int)mine[w], 32, 64);
-      lo = j < 2 ? mine : other;
-      hi = j < 2 ? other : mine;
-      rope8<F16>(lo, hi, clo, chi, slo, shi, rlo, rhi);
-      q[x] = __builtin_bit_cast(X8, j < 2 ? rlo : rhi);
+    for (int i = 0; i < KS; ++i) x[i] = __builtin_bit_cast(u32x4, q[i]);
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+      // the other half is in q[i ^ 2], or, at head_dim 64, 32 lanes away; the first half takes it
+      // negated
+      const bool second = D == 128 ? i >= 2 : j >= 2;
+      u32x4 turned;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const uint32_t o =
+            D == 128 ? x[i ^ (KS / 2)][w] : (uint32_t)__shfl_xor((int)x[i][w], 32, 64);
+        turned[w] = second ? o : o ^ 0x80008000u;
+      }
+      const int d = 64 * (i >> 1) + 16 * j + 8 * (i & 1);
+      q[i] = __builtin_bit_cast(X8, rope_half<F16>(x[i], turned, part(2, d), part(3, d)));
     }
   }
-}
+  // 8 codes of each half of k, or, in the odd groups of D / 16 lanes, of v; and the scale.
+  __device__ __forceinline__ int quantise(bool rope, int lane, u32x2* codes_lo,
+                                          u32x2* codes_hi) const {
+    const int d0 = 8 * (lane % CPH), v = (lane / CPH) & 1;
+    u32x4 lo = part(v, d0), hi = part(v, d0 + D / 2);
+    if (rope) {
+      u32x4 rlo, rhi;
+      rope8<F16>(lo, hi, part(2, d0), part(2, d0 + D / 2), part(3, d0), part(3, d0 + D / 2), rlo,
+                 rhi);
+      lo = v ? lo : rlo;
+      hi = v ? hi : rhi;
+    }
+    const int byte = scale_byte<CPH, F16>(lo, hi);
+    const float mul = __uint_as_float((uint32_t)(254 - byte) << 23);
+    *codes_lo = quant8<F16>(lo, mul);
+    *codes_hi = quant8<F16>(hi, mul);
+    return byte;
+  }
+};
 
 // A workgroup's share of the row blocks of one kv head.  NEW: the sequence's new row is quantised
 // by the wave whose tile holds its position, which puts it into the ring for itself and into the
@@ -280,13 +331,17 @@ void chunk_attention_kernel(ChunkArgs a) {
   constexpr int KS = D / 32;      // k steps of the QK product
   constexpr int DB = D / 16;      // 16-row tiles of O^T; head_dim index DB * m + b in tile b
   constexpr int VW = DB / 4;      // words of codes a lane holds of one V row
-  __shared__ __attribute__((aligned(16))) unsigned char smem[S::kLds];
+  using Row = NewRow<D, F16>;
+  constexpr int kRows = NEW ? NW * Row::kBytes : 0;
+  __shared__ __attribute__((aligned(16))) unsigned char smem[S::kLds + kRows];
   float* const ml = reinterpret_cast<float*>(smem + S::kLds - S::kMl);   // [2][wave][column]
 
   const int lane = threadIdx.x & 63, j = lane >> 4, c = lane & 15;
   const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   unsigned char* const ring = smem + wv * S::kRing;
   const uint32_t ring_lds = lds_addr(ring);
+  unsigned char* const fresh_lds = smem + S::kLds + wv * Row::kBytes;
+  const Row fresh{fresh_lds};
 
   // The kv heads of one share (or row block) run on one XCD at about the same time: workgroups
   // are dealt to the XCDs in turn, and heads share the lines of scales, tables and lengths.
@@ -327,6 +382,7 @@ void chunk_attention_kernel(ChunkArgs a) {
       if (col > a.max_blocks - 1) col = a.max_blocks - 1;
       window = table[col];
     };
+    if constexpr (NEW) fresh.load(a, seq_of_item(a, e), head, lane, lds_addr(fresh_lds));
     if (whole) load_window(0);        // before the lengths arrive
     const Item it = item_of(a, e);
     const int ntiles = it.tiles();
@@ -390,7 +446,10 @@ void chunk_attention_kernel(ChunkArgs a) {
     const int cnt = t1 - t0 > wv ? (t1 - t0 - wv + NW - 1) / NW : 0;
     uint32_t bad_bits = 0;        // two bits per stage: its halves with an invalid block id
     auto issue = [&](int u, int slot) {
-      if (u > 0 && (u & 31) == 0) load_window(u);
+      if (u > 0 && (u & 31) == 0) {
+        load_window(u);
+        asm volatile("" : "+v"(window));
+      }
       const uint32_t st = ring_lds + slot * S::kStage;
       const int tile = t0 + wv + NW * u;
       uint32_t srow[2];
@@ -420,37 +479,25 @@ void chunk_attention_kernel(ChunkArgs a) {
       lds_dma4(a.scales, off, st + 2 * S::kRowTile);
       bad_bits = (bad_bits & ~(3u << (2 * slot))) | (bad << (2 * slot));
     };
+    // What was loaded so far arrives here.  Left to the compiler its waits would be where the
+    // values are used, in the loop, and drain the ring, whose loads it does not see, at every step.
+    asm volatile("" : "+v"(window));
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int x = 0; x < KS; ++x) asm volatile("" : "+v"(q[nt][x]));
 #pragma unroll
     for (int d = 0; d < S::kDepth; ++d)
       if (d < cnt) issue(d, d);
 
-    // while these are on their way: q rotated, and the new row quantised.  A lane has 8 codes of
-    // each half of k (or, in the odd groups of D / 16 lanes, of v).
     constexpr int CPH = D / 16;
-    const bool is_v = (lane / CPH) & 1;
     u32x2 xlo, xhi;
     int xbyte = 0;
     if constexpr (NEW) {
-      const u16* const cs = a.cos + it.tok0 * a.cs_stride;
-      const u16* const sn = a.sin + it.tok0 * a.cs_stride;
-      if (a.cos != nullptr) rope_q<D, F16>(q[0], cs, sn, j);
-      if (u_new >= 0) {
-        const int d0 = 8 * (lane % CPH);
-        const u16* const src = (is_v ? a.new_v + it.tok0 * a.v_stride
-                                     : a.new_k + it.tok0 * a.k_stride) + head * D + d0;
-        u32x4 lo = ld16(src), hi = ld16(src + D / 2);
-        if (a.cos != nullptr) {
-          u32x4 rlo, rhi;
-          rope8<F16>(lo, hi, ld16(cs + d0), ld16(cs + d0 + D / 2), ld16(sn + d0),
-                     ld16(sn + d0 + D / 2), rlo, rhi);
-          lo = is_v ? lo : rlo;
-          hi = is_v ? hi : rhi;
-        }
-        xbyte = scale_byte<CPH, F16>(lo, hi);
-        const float mul = __uint_as_float((uint32_t)(254 - xbyte) << 23);
-        xlo = quant8<F16>(lo, mul);
-        xhi = quant8<F16>(hi, mul);
-      }
+      vm_wait_groups<S::kLoads, S::kDepth>(cnt);      // the rows are there, the ring need not be
+      asm volatile("" ::: "memory");
+      if (a.cos != nullptr) fresh.rotate(q[0], j);
+      if (u_new >= 0) xbyte = fresh.quantise(a.cos != nullptr, lane, &xlo, &xhi);
     }
 
     int slot = 0;
@@ -1105,7 +1152,8 @@ constexpr int kMinChunk = 8;
 // Tiles up to which a row block is one workgroup's, whatever else there is: the shares' scan, their
 // parts and the merge launch cost more (us, shares / whole, decode of 8 sequences: 14/2 heads of
 // 64, 1,000 tokens 12.6 / 8.1, 1,500 12.8 / 10.1, 3,000 14.7 / 16.2; 32/8 of 128 15.4 / 12.0,
-// 16.1 / 15.5, 18.5 / 25.4; 500 tokens in tables of 1,500, all that the host knows of them, 14.4 / 7.7).
+// 16.1 / 15.5, 18.5 / 25.4; 500 tokens in tables of 1,500, all that the host knows of them, 14.4 /
+// 7.7).
 // Chunks of 5 tokens and 64 sequences part at about 2,000 to 3,000 tokens, and at less where one
 // sequence is much longer than the others.
 constexpr int kWholeTiles = 48;
