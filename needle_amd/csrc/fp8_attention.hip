@@ -33,9 +33,9 @@
 //     equal shares, one per resident workgroup; what a share holds of a row block goes to a
 //     workspace and is merged by a second launch.
 // Measured (us, bytes read at): 64 sequences of 512 to 4,096 tokens, 32/8 heads of 128, one token
-// each 49.0 + 4.8 of merge, 5.4 TB/s in the first launch; 24 sequences of 4,096 to 32,768, 28/4
-// heads, float16, 73.6 + 4.7, 5.9 TB/s; 1 to 8 tokens each after 512 to 4,096 58.4 + 7.9, 4.6 TB/s.
-// A few short sequences take 5 us, of which each step of a wave (a tile) is 1: about 250
+// each 48 + 4.8 of merge, 5.5 TB/s in the first launch; 24 sequences of 4,096 to 32,768, 28/4
+// heads, float16, 72 + 6.3, 6.0 TB/s; 1 to 8 tokens each after 512 to 4,096 56 + 7.9, 4.8 TB/s.
+// A few short sequences take 5 us, of which each step of a wave (a tile) is 1: about 290
 // instructions, two waves to a SIMD; sixteen waves or deeper rings measured the same or slower.
 #include "fp8.hpp"
 
@@ -141,8 +141,10 @@ __device__ __forceinline__ int wave_scan(int v, int lane) {
 // The row blocks of a kv head laid end to end, in slots: their prefix sums, 64 to a step.  Up to
 // kHeld row blocks stay in registers, loaded at once; more are read again where they are needed.
 constexpr int kSteps = 4, kHeld = 64 * kSteps;
-// A share's begin moves to a row block's end within an eighth of a share of it: us without / a
-// sixteenth / an eighth, the decode step of 64 sequences of 512 to 4,096 tokens 55.3 / 54.6 / 53.3.
+// A share's begin moves to a row block's end within an eighth of a share of it: us without / an
+// eighth / a quarter / a third, 64 sequences of 512 to 4,096 tokens 50.9 / 48.8 / 48.9 / 51.9, with
+// 1 to 8 new tokens each 56.2 / 56.0 / 60.0 / 60.4; 100 of up to 3,000, 28/4 heads 37.1 / 35.6 /
+// 35.7 / 38.0.
 constexpr int kSnap = 8;
 struct Place {
   int e, first, slots;          // a row block, its first slot, how many it has
@@ -397,7 +399,7 @@ void chunk_attention_kernel(ChunkArgs a) {
       if (t0 >= t1) continue;     // only the empty slot is this share's
       load_window(0);
     } else if (it.n <= 0) {
-      return;
+      break;
     }
     const int cols = it.n * a.group;
 
@@ -796,6 +798,7 @@ void chunk_attention_kernel(ChunkArgs a) {
     if (whole) return;
     __syncthreads();     // before the ring is written again
   }
+  if constexpr (NEW) vm_wait<0>();     // rows of a row block that is not this share's
 }
 
 // One workgroup per (row block, kv head, kMergeCols columns): the parts that the shares hold,
@@ -1151,15 +1154,15 @@ const void* kernel_of(int nt, int waves, bool append = false) {
 constexpr int kMinChunk = 8;
 // Tiles up to which a row block is one workgroup's, whatever else there is: the shares' scan, their
 // parts and the merge launch cost more (us, shares / whole, decode of 8 sequences: 14/2 heads of
-// 64, 1,000 tokens 12.6 / 8.1, 1,500 12.8 / 10.1, 3,000 14.7 / 16.2; 32/8 of 128 15.4 / 12.0,
-// 16.1 / 15.5, 18.5 / 25.4; 500 tokens in tables of 1,500, all that the host knows of them, 14.4 /
-// 7.7).
-// Chunks of 5 tokens and 64 sequences part at about 2,000 to 3,000 tokens, and at less where one
-// sequence is much longer than the others.
+// 64, 1,000 tokens 12.2 / 8.2, 1,500 12.8 / 9.9, 3,000 14.6 / 15.8; 32/8 of 128 14.9 / 11.0,
+// 16.1 / 14.2, 17.7 / 22.6; 500 tokens in tables of 1,500, all that the host knows of them, 16.6 /
+// 7.7).  Chunks of 5 tokens and 64 sequences part at about 2,000 to 3,000 tokens, and at less where
+// one sequence is much longer than the others.
 constexpr int kWholeTiles = 48;
-// Empty slots before a row block, one column tile or two (its start, its waves' sums): us at 0, 1,
-// 2 and 4, decode as above 54.3, 53.2, 54.2, 54.0; chunks of 1 to 8 tokens after 512 to 4,096
-// 68.5, 67.8, 66.9, 64.9.
+// Empty slots before a row block, one column tile or two (its start, its waves' sums): us at 0 and
+// 0, 0 and 2, 1 and 4, 5 tokens each after up to 3,000: 32 sequences of 14/2 heads of 64 24.3 /
+// 23.5 / 21.5, of 28/4 of 128 35.7 / 33.9 / 33.3, 100 of 32/8 70.3 / 69.2 / 66.7, one token each
+// 52.5 / 52.8 / 51.2.
 constexpr int kPad1 = 1, kPad2 = 4;
 
 // resident: workgroups the GPU holds at once.
@@ -1175,10 +1178,11 @@ Plan make_plan(int64_t num_seqs, int64_t max_seqlen, int64_t max_keys, int group
   // (slots and segments are counted in 31 bits)
   const bool whole = tiles <= kWholeTiles || units >= 4 * resident ||
                      p.items * (tiles + kPad2) + 2 * resident * kMinChunk > 0x40000000;
-  // Eight waves where four would leave half the GPU without any; shares of head_dim 64 keep four,
-  // of which a CU holds three and four workgroups (us, four / eight, 8 tokens each after 3,000: 32
-  // sequences of 28/4 heads of 128 55.1 / 44.6, of 14/2 heads of 64 29.3 / 36.2).
-  p.waves = (whole || head_dim == 128) && units * 2 <= resident ? 8 : 4;
+  // Whole row blocks: eight waves where four would leave half the GPU without any (us, four /
+  // eight, 16 sequences of 1,000 tokens: 14/2 heads of 64 9.5 / 8.3, 32/8 of 128 11.8 / 11.5; 128
+  // of 32/8 28.4 / 34.8).  Shares: four (16 of 3,000, 32/8 heads, 1 and 8 tokens each 20.2 / 19.9
+  // and 26.2 / 28.1, 14/2 of 64 14.5 / 15.3 and 18.4 / 24.3).
+  p.waves = whole && units * 2 <= resident ? 8 : 4;
   p.pad = p.nt == 1 ? kPad1 : kPad2;
   if (!whole) {
     int64_t s = resident * 4 / p.waves / num_kv_heads / 8 * 8;
