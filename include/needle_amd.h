@@ -591,8 +591,8 @@ int ndl_fp8_decode_append(void* out, const void* q, int64_t q_tok_stride, const 
 
 /*
  * Verification of drafted tokens.  Sequence i has rows cu_seqlens[i] .. cu_seqlens[i + 1] (at
- * least one) of logits and of ids, the chunk the target was given: row r judges the draft
- * ids[r + 1], a sequence's last row none.  With p = softmax(logits[r] / temperature[i]) and q the
+ * least one) of logits and of ids, the chunk the target was given: row r decides on the draft
+ * ids[r + 1], a sequence's last row on none.  With p = softmax(logits[r] / temperature[i]) and q the
  * draft's distribution, row r - i of draft_probs (NULL: the point at the draft), a draft x is
  * accepted while uniforms[r] * q(x) < p(x) holds for it and all before it.  The next token is
  * drawn with u = uniforms[cu_seqlens[i + 1] - 1]: from max(p - q, 0) of the first rejected row (p

@@ -23,7 +23,8 @@
 //   * P^T needs no data movement: with token slot 8 j + i of the PV product standing for token
 //     4 j + i (i < 4) or 12 + 4 j + i, the accumulator layout of S^T is the operand's.
 //   * Softmax in fp32 with exp2, scale * log2(e) folded.  The running maximum is raised (and the
-//     sums rescaled) only when a tile exceeds it by 8, so probabilities stay below 256.
+//     sums rescaled) only when a tile exceeds it by 8, so probabilities stay below 256; a tile's
+//     maximum is taken across lanes only then.
 //     P is rounded to the 16-bit format for the matrix cores; its sum is taken before that.
 //   * Long chunks (kUnpackRows columns, kUnpackScores scores) are bound by the products, not by the
 //     codes: their keys are unpacked once into a 16-bit pool in the workspace, exactly, and
@@ -33,9 +34,9 @@
 //     equal shares, one per resident workgroup; what a share holds of a row block goes to a
 //     workspace and is merged by a second launch.
 // Measured (us, bytes read at): 64 sequences of 512 to 4,096 tokens, 32/8 heads of 128, one token
-// each 48 + 4.8 of merge, 5.5 TB/s in the first launch; 24 sequences of 4,096 to 32,768, 28/4
-// heads, float16, 72 + 6.3, 6.0 TB/s; 1 to 8 tokens each after 512 to 4,096 56 + 7.9, 4.8 TB/s.
-// A few short sequences take 5 us, of which each step of a wave (a tile) is 1: about 290
+// each 47 + 4.8 of merge, 5.6 TB/s in the first launch; 24 sequences of 4,096 to 32,768, 28/4
+// heads, float16, 72 + 6.3, 6.0 TB/s; 1 to 8 tokens each after 512 to 4,096 55 + 7.9, 4.9 TB/s.
+// A few short sequences take 5 us, of which each step of a wave (a tile) is 1: about 270
 // instructions, two waves to a SIMD; sixteen waves or deeper rings measured the same or slower.
 #include "fp8.hpp"
 
@@ -221,6 +222,31 @@ __device__ __forceinline__ void vm_wait_groups(int n) {
     else
       vm_wait_groups<I, MAX - 1>(n);
   }
+}
+
+// The power of two that byte r of w stands for: one instruction, where shifting and masking are
+// two.
+__device__ __forceinline__ float scale_of(uint32_t w, int r) {
+  uint32_t x;
+  if (r == 0)
+    asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD "
+        "src1_sel:BYTE_0" : "=v"(x) : "v"(23), "v"(w));
+  else if (r == 1)
+    asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD "
+        "src1_sel:BYTE_1" : "=v"(x) : "v"(23), "v"(w));
+  else if (r == 2)
+    asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD "
+        "src1_sel:BYTE_2" : "=v"(x) : "v"(23), "v"(w));
+  else
+    asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD "
+        "src1_sel:BYTE_3" : "=v"(x) : "v"(23), "v"(w));
+  return __uint_as_float(x);
+}
+// fmaxf of three without the compiler's quieting of each (no score is a signalling NaN).
+__device__ __forceinline__ float max3(float x, float y, float z) {
+  float m;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(m) : "v"(x), "v"(y), "v"(z));
+  return m;
 }
 
 // 0xff in every byte of w that is a NaN code (0x7f or 0xff).
@@ -481,16 +507,21 @@ void chunk_attention_kernel(ChunkArgs a) {
       lds_dma4(a.scales, off, st + 2 * S::kRowTile);
       bad_bits = (bad_bits & ~(3u << (2 * slot))) | (bad << (2 * slot));
     };
-    // What was loaded so far arrives here.  Left to the compiler its waits would be where the
-    // values are used, in the loop, and drain the ring, whose loads it does not see, at every step.
+    // What was loaded so far arrives here, q with the ring's first stages.  Left to the compiler its
+    // waits would be where the values are used, in the loop, and drain the ring, whose loads it does
+    // not see, at every step.
+    auto arrive = [&]() {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int x = 0; x < KS; ++x) asm volatile("" : "+v"(q[nt][x]));
+    };
     asm volatile("" : "+v"(window));
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int x = 0; x < KS; ++x) asm volatile("" : "+v"(q[nt][x]));
+    if constexpr (NEW) arrive();     // rotated while those are under way
 #pragma unroll
     for (int d = 0; d < S::kDepth; ++d)
       if (d < cnt) issue(d, d);
+    if constexpr (!NEW) arrive();
 
     constexpr int CPH = D / 16;
     u32x2 xlo, xhi;
@@ -590,13 +621,11 @@ void chunk_attention_kernel(ChunkArgs a) {
               sc[s][nt] = T::mfma16x16x32(k8, q[nt][2 * h + x], sc[s][nt]);
           }
       }
-      float vs[8];
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float ks = __uint_as_float(((sk[s] >> (8 * r)) & 0xffu) << 23) * a.scale_log2;
-          vs[4 * s + r] = __uint_as_float(((sv[s] >> (8 * r)) & 0xffu) << 23);
+          const float ks = scale_of(sk[s], r) * a.scale_log2;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) sc[s][nt][r] *= ks;
         }
@@ -632,15 +661,15 @@ void chunk_attention_kernel(ChunkArgs a) {
       float mt[NT];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float x = fmaxf(fmaxf(sc[0][nt][0], sc[0][nt][1]), fmaxf(sc[0][nt][2], sc[0][nt][3]));
-        x = fmaxf(x, fmaxf(fmaxf(sc[1][nt][0], sc[1][nt][1]), fmaxf(sc[1][nt][2], sc[1][nt][3])));
-        mt[nt] = max_xor32(max_xor16(x));
+        mt[nt] = max3(max3(sc[0][nt][0], sc[0][nt][1], sc[0][nt][2]),
+                      max3(sc[0][nt][3], sc[1][nt][0], sc[1][nt][1]),
+                      max3(sc[1][nt][2], sc[1][nt][3], sc[1][nt][3]));
         raise |= mt[nt] > m[nt] + kRaise;
       }
       if (__builtin_amdgcn_ballot_w64(raise)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          const float nm = fmaxf(m[nt], mt[nt]);
+          const float nm = fmaxf(m[nt], max_xor32(max_xor16(mt[nt])));
           const float f = m[nt] == nm ? 1.f : fast_exp2(m[nt] - nm);
           m[nt] = nm;
           l[nt] *= f;
@@ -702,6 +731,10 @@ void chunk_attention_kernel(ChunkArgs a) {
 
       // O^T += V^T P^T: a pair of head_dim tiles at a time, the rows' pairs of codes turned into
       // pairs of tokens
+      asm volatile("" : "+v"(sv[0]), "+v"(sv[1]));     // the scales no sooner than they are used
+      float vs[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) vs[i] = scale_of(sv[i >> 2], i & 3);
 #pragma unroll
       for (int b2 = 0; b2 < DB / 2; ++b2) {
         uint32_t v2[8];
@@ -1224,7 +1257,6 @@ int launch(ChunkArgs a, int nt, int waves, hipStream_t s) {
   const int rc = check_launch();
   if (rc != NDL_OK || a.shares == 0) return rc;
   const int groups = (a.toks * a.group + kMergeCols - 1) / kMergeCols;
-  if (a.num_kv_heads > 65535) return NDL_ERR_UNSUPPORTED;
   hipLaunchKernelGGL((chunk_merge_kernel<D, F16>),
                      dim3((unsigned)a.items, (unsigned)a.num_kv_heads, (unsigned)groups), dim3(256),
                      0, s, a);
@@ -1317,6 +1349,7 @@ static int fp8_attention(ndl::ChunkArgs a, void* out, const void* q, int64_t q_t
   const Plan p = plan_for(num_seqs, max_seqlen, max_keys, num_heads, num_kv_heads, head_dim);
   if (p.items > 0x7fffff00) return NDL_ERR_INVALID_ARG;
   if (p.shares) {
+    if (num_kv_heads > 65535) return NDL_ERR_UNSUPPORTED;     // a grid dimension of the merge
     if (!workspace || workspace_bytes < p.ml_bytes + p.acc_bytes || (uintptr_t)workspace & 255u)
       return NDL_ERR_WORKSPACE;
     a.ws_ml = (float*)workspace;

@@ -2,7 +2,7 @@
 // gfx950.  The random numbers are inputs, so the answer is a function of them.
 //
 // Sequence i has rows cu[i] .. cu[i + 1] of logits, one per token of the chunk it was given; row r
-// judges the draft ids[r + 1], its last row has none to judge.  With p_r = softmax(l_r / T_i) and
+// decides on the draft ids[r + 1], its last row on none.  With p_r = softmax(l_r / T_i) and
 // q_r the distribution that the draft was taken from (the point at the draft, without one):
 //   draft r is accepted while  u_r q_r(x) < p_r(x)  holds for it and all before it;
 //   after the first rejected row r the next token has the distribution max(p_r - q_r, 0) / sum
@@ -15,7 +15,7 @@
 // Bound: every logit read once, and what each launch waits for.  Three or four launches (us at 304
 // rows of 64 sequences, 151,936 bfloat16 logits, draft distributions / 5 rows of one, without):
 //   stats   row slices: maximum, its index, sum of exponentials, in one pass (fp32 terms); beside
-//           them what judges the drafts                            20.2 (4.6 TB/s) / 3.4
+//           them what decides on the drafts                        20.2 (4.6 TB/s) / 3.4
 //   sums    per sequence: accepts (every workgroup by itself, from the slices), then the chosen
 //           row's weights summed by slices                         12.6 / 5.2
 //   left    with draft distributions: the sums of max(p - q, 0) by slices   8.7
@@ -37,15 +37,15 @@ constexpr int kStatSlice = 4096;     // elements of a slice at least
 constexpr int kStatWgs = 1536;       // workgroups wanted over all rows: what the GPU holds at once
 constexpr int kSumSlice = 2048;      // a step of a workgroup; slices are whole steps
 constexpr int kSumWgs = 2048;        // of sums and left: likewise
-constexpr int kStatSlices = 32;      // 8 rows' slices are combined at a time
+constexpr int kStatSlices = 32;      // 8 rows' slices are combined at a time, at half a wave each
 constexpr int kMaxSlices = 64;       // a lane of a wave each
-constexpr int kPickLen = 6144;       // elements of a chosen row's slice at most, for the last launch
+constexpr int kPickLen = 6144;       // elements of a chosen row's slice at most (see pick)
 constexpr int kMaxVocab = 1 << 18;
 static_assert(kMaxVocab <= kMaxSlices * kPickLen, "a row's slices cover it");
 constexpr int kRun = kSumSlice / kThreads;      // entries of a thread's step, next to each other
 constexpr int kPickThreads = kPickLen / kRun;   // of the last launch: one workgroup per sequence
 static_assert(kRun == 8 && kPickThreads % 64 == 0);
-constexpr int kAccept = 64;          // rows judged at a time
+constexpr int kAccept = 64;          // rows decided on at a time
 
 struct Info {            // of a sequence, written by `sums`
   int accepted;
@@ -58,7 +58,7 @@ struct Info {            // of a sequence, written by `sums`
 enum Kind { kNothing = 0, kPoint = 1, kAll = 2, kBut = 3, kLeft = 4 };
 // kPoint: all weight at `token`; kAll: exp; kBut: exp but for `token`; kLeft: max(p - q, 0)
 
-struct Judge {           // of a drafted token, written by `stats`
+struct Drafted {         // of a drafted token, written by `stats`
   int x;                 // the token, -1 outside the vocabulary
   float l, q;            // its logit and its draft probability
   float u;
@@ -83,7 +83,7 @@ struct VerifyArgs {
   float* part_max;             // [rows][slices]
   int* part_arg;
   float* part_sum;
-  Judge* judge;                // [rows]
+  Drafted* drafted;            // [rows]
   Info* info;                  // [num_seqs]
   double* sums;                // [num_seqs][sum_slices]
   double* left;                // likewise
@@ -189,25 +189,25 @@ __device__ __forceinline__ float rate_of(float temp) {
   return fmaxf(fminf(kLog2e / temp, 3e38f), 1e-30f);
 }
 
-// The drafted tokens of sequence i: what judges them beside the rows' statistics, in the shadow of
-// the rows' workgroups (three trips to memory).
+// The drafted tokens of sequence i: what decides on them beside the rows' statistics, in the shadow
+// of the rows' workgroups (three trips to memory).
 template <int FMT>
-__device__ __forceinline__ void judge_rows(const VerifyArgs& a, int i) {
+__device__ __forceinline__ void gather_drafts(const VerifyArgs& a, int i) {
   int64_t first;
   const int n = seq_rows(a, i, &first);
   for (int j = threadIdx.x; j < n - 1; j += kThreads) {
     const int64_t r = first + j, x = draft_at(a, r + 1), d = r - i;
-    Judge g{-1, kNegInf, 1.f, a.uniforms[r]};
+    Drafted g{-1, kNegInf, 1.f, a.uniforms[r]};
     if (x >= 0 && x < a.vocab) {
       g.x = (int)x;
       g.l = elem<FMT>(row_at<FMT>(a, r), x);
       if (a.probs) g.q = d >= 0 && d < a.probs_rows ? a.probs[d * a.probs_stride + x] : 0.f;
     }
-    a.judge[r] = g;
+    a.drafted[r] = g;
   }
 }
 
-// A workgroup per sequence for judge_rows, then one per row and slice: maximum and sum of
+// A workgroup per sequence for gather_drafts, then one per row and slice: maximum and sum of
 // exp((l - maximum) / T) in one pass.  Where the row is a point (T = 0, or a slice that holds a NaN
 // or an infinity: the sum is NaN then), the maximum and its first index instead.
 template <int FMT>
@@ -215,7 +215,7 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerifyArgs a) {
   constexpr int EB = FMT == kFmtF32 ? 4 : 2, PER = 16 / EB;
   constexpr int kBatch = 4;            // 16-byte words of a thread's step, the next in flight
   if (blockIdx.x < (unsigned)a.num_seqs) {
-    judge_rows<FMT>(a, (int)blockIdx.x);
+    gather_drafts<FMT>(a, (int)blockIdx.x);
     return;
   }
   const unsigned unit = blockIdx.x - (unsigned)a.num_seqs;
@@ -420,7 +420,7 @@ __device__ __forceinline__ RowPart load_part(const VerifyArgs& a, int64_t r, int
   if (s >= a.slices) p = RowPart{};
   return p;
 }
-// f combined over groups of `width` lanes, as wave_all does over the wave.
+// v combined over groups of `width` lanes (1 to 32), as wave_all does over the wave.
 template <class OP>
 __device__ __forceinline__ double group_sum(double v, int width, OP op) {
   if (width > 1) v = op(v, dpp<0xb1>(v));
@@ -428,7 +428,6 @@ __device__ __forceinline__ double group_sum(double v, int width, OP op) {
   if (width > 4) v = op(v, dpp<0x141>(v));
   if (width > 8) v = op(v, dpp<0x140>(v));
   if (width > 16) v = across<16>(v, op);
-  if (width > 32) v = across<32>(v, op);
   return v;
 }
 __device__ __forceinline__ RowStats row_stats(const RowPart& p, int width, float k) {
@@ -472,9 +471,9 @@ __device__ const double kPowers[64] = {
     0x1.ea4afa2a490dap+0, 0x1.efa1bee615a27p+0, 0x1.f50765b6e4540p+0, 0x1.fa7c1819e90d8p+0,
 };
 
-// exp((l - top) / T) in fp64, to about 1e-13 of it, 0 for a masked entry: 2^(n / 64) from the table,
-// and 2^(r / 64), |r| <= 1/2, by the exponential's series to the fourth power.  n is read from the
-// low bits of a sum with 1.5 * 2^52 (fp64 conversions run at a quarter of the rate).
+// exp((l - top) / T) in fp64, to about 1e-13 of it, 0 for a masked entry: 2^(n / 64) from the
+// table, and 2^(r / 64), |r| <= 1/2, by the exponential's series to the fourth power.  n is read
+// from the low bits of a sum with 1.5 * 2^52 (fp64 conversions run at a quarter of the rate).
 struct Exp {
   const double* table;     // kPowers in LDS
   double rate;             // 64 / (T ln 2)
@@ -552,9 +551,9 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs a) {
   int acc = 0, j0 = 0;
   for (;; j0 += kAccept) {
     const int m = n - j0 < kAccept ? n - j0 : kAccept;
-    const bool judge = t < m && j0 + t < n - 1;
+    const bool draft = t < m && j0 + t < n - 1;
     const int g = t / width, gs = kThreads / width;
-    const Judge d = a.judge[first + j0 + (t < m ? t : 0)];
+    const Drafted d = a.drafted[first + j0 + (t < m ? t : 0)];
     RowPart next = load_part(a, first + j0 + (g < m ? g : 0), t & (width - 1));
     for (int j = g; j < m; j += gs) {
       const RowPart part = next;
@@ -570,7 +569,7 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs a) {
     if (t < m) {
       drafts[t] = d.x;
       bool ok = false;
-      if (judge && d.x >= 0) {
+      if (draft && d.x >= 0) {
         const double uq = (double)d.u * (double)d.q;
         ok = temp > 0.f && finite(tops[t]) ? uq * totals[t] < ex(d.l, tops[t])
                                            : uq < (d.x == args[t] ? 1.0 : 0.0);
@@ -674,8 +673,8 @@ __device__ __forceinline__ double wave_prefix(double v, int lane) {
   return v + before;
 }
 
-// Workgroup per sequence: its tokens.  The slice whose prefix passes the goal; then the thread (each
-// takes a run of the slice), then the entry.
+// Workgroup per sequence: its tokens.  The slice whose prefix passes the goal; then the thread
+// (each takes a run of the slice), then the entry.
 template <int FMT>
 __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(VerifyArgs a) {
   const int i = blockIdx.x, t = threadIdx.x, lane = t & 63, wv = t >> 6;
@@ -775,7 +774,7 @@ size_t up(size_t n) { return (n + 255) / 256 * 256; }
 
 struct Sizes {
   int slices, sum_len, sum_slices;
-  size_t stat, judge, info, sums, total;   // bytes of a part; three stats, two sums
+  size_t stat, drafted, info, sums, total;   // bytes of a part; three stats, two sums
 };
 Sizes sizes_of(int64_t rows, int num_seqs, int vocab) {
   Sizes z;
@@ -783,7 +782,7 @@ Sizes sizes_of(int64_t rows, int num_seqs, int vocab) {
   const int64_t by_wgs = (kStatWgs + rows - 1) / rows;
   const int64_t few = by_len < by_wgs ? by_len : by_wgs;
   z.slices = (int)(few < kStatSlices ? few : kStatSlices);
-  // one round of workgroups, as few slices as that takes: each judges its sequence first (96 rows
+  // one round of workgroups, as few slices as that takes: each decides on its drafts first (96 rows
   // of 50,257 float32: sums and left 8.8 + 7.0 us with 13 slices, 10.6 + 6.0 with 25)
   const int steps = (vocab + kSumSlice - 1) / kSumSlice;
   const int64_t wanted = ((int64_t)steps * num_seqs + kSumWgs - 1) / kSumWgs;
@@ -792,10 +791,10 @@ Sizes sizes_of(int64_t rows, int num_seqs, int vocab) {
   z.sum_len = per * kSumSlice;
   z.sum_slices = (steps + per - 1) / per;
   z.stat = up((size_t)rows * z.slices * 4);
-  z.judge = up((size_t)rows * sizeof(Judge));
+  z.drafted = up((size_t)rows * sizeof(Drafted));
   z.info = up((size_t)num_seqs * sizeof(Info));
   z.sums = up((size_t)num_seqs * z.sum_slices * 8);
-  z.total = 3 * z.stat + z.judge + z.info + 2 * z.sums;
+  z.total = 3 * z.stat + z.drafted + z.info + 2 * z.sums;
   return z;
 }
 
@@ -878,10 +877,10 @@ extern "C" int ndl_verify_drafts(void* tokens, int32_t* accepted, const void* lo
   a.part_arg = (int*)(w + z.stat);
   a.part_sum = (float*)(w + 2 * z.stat);
   w += 3 * z.stat;
-  a.judge = (Judge*)w;
-  a.info = (Info*)(w + z.judge);
-  a.sums = (double*)(w + z.judge + z.info);
-  a.left = (double*)(w + z.judge + z.info + z.sums);
+  a.drafted = (Drafted*)w;
+  a.info = (Info*)(w + z.drafted);
+  a.sums = (double*)(w + z.drafted + z.info);
+  a.left = (double*)(w + z.drafted + z.info + z.sums);
   const hipStream_t s = (hipStream_t)stream;
   if (dtype_is_f32(dtype)) return launch_verify<kFmtF32>(a, s);
   return dtype_is_f16(dtype) ? launch_verify<kFmtF16>(a, s) : launch_verify<kFmtBF16>(a, s);

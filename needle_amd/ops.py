@@ -850,7 +850,8 @@ def kv_append_fp8(k: torch.Tensor, v: torch.Tensor, kv_codes: torch.Tensor,
     is not finite.
 
     cos / sin [T, D] rotate k first, with rope_kv_append's roundings, and q [T, H, D] too if it
-    is given: then the rotated q is returned (written to out, contiguous, if that is given).
+    is given: then the rotated q is returned (written to out, contiguous, if that is given; it
+    may be q).
     cu_seqlens None: one token per sequence.
     """
     if out is None and _lib.NATIVE is not None:
@@ -1082,8 +1083,8 @@ def verify_drafts(logits: torch.Tensor, ids: torch.Tensor, cu_seqlens: torch.Ten
 
     logits [T, vocab] (bfloat16, float16 or float32, rows contiguous, any row stride) are the
     target's rows for the packed chunks ids [T] (int32 or int64): a sequence's newest token and
-    its drafts, at least one row each.  Row r judges the draft ids[r + 1]; a sequence's last row
-    judges none.  With p = softmax(logits[r] / temperature[i]) and q row r - i of draft_probs
+    its drafts, at least one row each.  Row r decides on the draft ids[r + 1]; a sequence's last row
+    on none.  With p = softmax(logits[r] / temperature[i]) and q row r - i of draft_probs
     (float32 [T - num_seqs, vocab]; None: the drafts have probability 1) a draft x is accepted
     while uniforms[r] * q(x) < p(x), for it and all before it.  The next token follows
     max(p - q, 0) of the first rejected row, or p of the last row, by the inverse of its

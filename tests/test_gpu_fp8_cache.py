@@ -239,3 +239,18 @@ def test_captured_steps_replay(monkeypatch):
         torch.cuda.synchronize()
         assert torch.equal(g.codes, e.codes) and torch.equal(g.scales, e.scales), r
         assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1]), r
+
+
+@pytest.mark.parametrize("shape", SHAPES[:3])
+def test_q_is_rotated_in_place(shape):
+    """out may be q itself."""
+    h, hkv, d, bs = shape
+    gen, pool, table, ctx, cu = _case(shape, [3, 20], [5, 0], 8)
+    q, k, v = (torch.randn(23, n, d, generator=gen).bfloat16().to(DEV) for n in (h, hkv, hkv))
+    cos, sin = (torch.randn(23, d, generator=gen).bfloat16().to(DEV) for _ in range(2))
+    meta = [x.to(DEV) for x in (table, ctx, cu)]
+    a, b = ([x.to(DEV) for x in pool] for _ in range(2))
+    want = ops.kv_append_fp8(k, v, *a, *meta, q=q, cos=cos, sin=sin)
+    got = ops.kv_append_fp8(k, v, *b, *meta, q=q, cos=cos, sin=sin, out=q)
+    assert got is q and torch.equal(got, want)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])

@@ -114,7 +114,7 @@ def test_one_long_context():
 
 @pytest.mark.parametrize("probs", [True, False])
 def test_many_drafts(probs):
-    """Sequences of more rows than are judged at a time, all accepted or rejected late."""
+    """Sequences of more rows than are decided on at a time, all accepted or rejected late."""
     case = verify_case([64, 65, 66, 130, 1, 200], 77, torch.float32, 5, probs)
     logits, ids, cu, u, t, draft = case
     verify_check(case)
