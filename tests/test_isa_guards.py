@@ -120,5 +120,6 @@ def test_fp8_attention_uses_m0_only_for_direct_lds_loads(device_asm):
             re.match(r"global_load_lds_dword(x4)? ", body[i + 2]), body[i:i + 3]
 
 
-def test_the_8_bit_appends_rope_has_no_fused_fp16_multiply_add(device_asm):
-    test_no_fused_fp16_multiply_add(device_asm, "kv_fp8")
+@pytest.mark.parametrize("name", ["kv_fp8", "fp8_attention"])
+def test_the_8_bit_pools_rope_has_no_fused_fp16_multiply_add(device_asm, name):
+    test_no_fused_fp16_multiply_add(device_asm, name)
