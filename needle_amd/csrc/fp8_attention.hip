@@ -40,6 +40,8 @@
 // instructions, two waves to a SIMD; sixteen waves or deeper rings measured the same or slower.
 #include "fp8.hpp"
 
+#include "chunk_shares.hpp"
+
 namespace ndl {
 namespace {
 
@@ -142,16 +144,12 @@ __device__ __forceinline__ int wave_scan(int v, int lane) {
 // The row blocks of a kv head laid end to end, in slots: their prefix sums, 64 to a step.  Up to
 // kHeld row blocks stay in registers, loaded at once; more are read again where they are needed.
 constexpr int kSteps = 4, kHeld = 64 * kSteps;
-// A share's begin moves to a row block's end within an eighth of a share of it: us without / an
-// eighth / a quarter / a third, 64 sequences of 512 to 4,096 tokens 50.9 / 48.8 / 48.9 / 51.9, with
-// 1 to 8 new tokens each 56.2 / 56.0 / 60.0 / 60.4; 100 of up to 3,000, 28/4 heads 37.1 / 35.6 /
-// 35.7 / 38.0.
-constexpr int kSnap = 8;
 struct Place {
   int e, first, slots;          // a row block, its first slot, how many it has
 };
 struct Stream {
-  int total, chunk, snap;
+  int total;
+  Cut cut;
   int v[kSteps], incl[kSteps];
 
   __device__ __forceinline__ void read(const ChunkArgs& a, int lane) {
@@ -168,10 +166,7 @@ struct Stream {
     }
     for (int base = kHeld; base < a.items; base += 64)
       total += __builtin_amdgcn_readlane(wave_scan(slots_of(a, base + lane), lane), 63);
-    const int c = (int)((uint32_t)(total + a.shares - 1) / (uint32_t)a.shares);
-    chunk = c < a.min_chunk ? a.min_chunk : c;
-    // (at least the empty slots: every part of a row block has a tile)
-    snap = chunk / kSnap > a.pad ? chunk / kSnap : a.pad;
+    cut = cut_of(total, a.shares, a.min_chunk, a.pad);
   }
   // The row block that holds slot `at` (at < total), or row block `e` if that is not negative.
   __device__ __forceinline__ Place find(const ChunkArgs& a, int lane, int at, int e) const {
@@ -199,15 +194,12 @@ struct Stream {
     }
     return Place{a.items, carry, 0};
   }
-  // Where share s begins: at s * chunk, or, if a row block begins or ends within `snap` slots of
-  // that, there: a sliver of a row block is not worth its part in the workspace.
+  // Where share s begins.
   __device__ __forceinline__ int begin(const ChunkArgs& a, int lane, int s) const {
-    const int x = s * chunk;       // fits 31 bits: make_plan
+    const int x = s * cut.chunk;   // fits 31 bits: make_plan
     if (x >= total) return total;
     const Place p = find(a, lane, x, -1);
-    if (x - p.first <= snap) return p.first;
-    if (p.first + p.slots - x <= snap) return p.first + p.slots;
-    return x;
+    return share_begin(x, p.first, p.slots, cut.snap);
   }
 };
 
@@ -418,10 +410,8 @@ void chunk_attention_kernel(ChunkArgs a) {
     if (!whole) {
       if (ntiles == 0) continue;
       if (first >= to) break;
-      const int base = first + a.pad;
-      t0 = from > base ? from - base : 0;
-      t1 = to < base + ntiles ? to - base : ntiles;
-      first = base + ntiles;
+      share_tiles(first, a.pad, ntiles, from, to, &t0, &t1);
+      first += a.pad + ntiles;
       if (t0 >= t1) continue;     // only the empty slot is this share's
       load_window(0);
     } else if (it.n <= 0) {
@@ -857,13 +847,11 @@ __global__ __launch_bounds__(256) void chunk_merge_kernel(ChunkArgs a) {
   float o[PER];
 #pragma unroll
   for (int x = 0; x < PER; ++x) o[x] = 0.f;
-  // its tiles by the scan that gave its place: whatever the lengths are, or become while this
-  // runs, the shares are within the workspace
+  // its slots by the scan that gave its place and the cut: whatever the lengths are, or become while
+  // this runs, share_parts names shares that there are, whose parts the workspace holds
   if (p.slots > 0) {
-    // the shares that begin inside it, past what Stream::begin moves to its ends
-    const int s0 = (int)((uint32_t)(p.first + st.snap) / (uint32_t)st.chunk);
-    const int s1 = (int)((uint32_t)(p.first + p.slots - st.snap - 1) / (uint32_t)st.chunk);
-    if (s0 >= s1) return;
+    int s0, s1;
+    if (!share_parts(p.first, p.slots, st.cut, &s0, &s1)) return;   // written by the attention
     const int n = s1 - s0 + 1, per = a.toks * a.group;
     const int64_t seg = ((int64_t)head * a.nseg + s0 + e) * per + c0;
     const float2* const ml = reinterpret_cast<const float2*>(a.ws_ml) + seg;
