@@ -551,7 +551,7 @@ int ndl_kv_read_fp8(void* k_out, void* v_out, const void* codes, const void* sca
  * q_tok_stride (a multiple of 8); groups of 1 to 16 query heads per kv head.  fp32 scores, softmax
  * and sums; probabilities rounded to the 16-bit format for the matrix cores.  Nothing to attend
  * (a negative context_lens[i], invalid block ids only): zeros.  A NaN in the pool reaches the
- * tokens that attend it and no others.
+ * tokens that attend it and no others; rows that none attends may hold anything, in scales and codes.
  *
  * max_seqlen bounds the tokens of a sequence (those past it are not computed) and max_keys its
  * keys (context_lens[i] + tokens, at most max_blocks_per_seq * block_size; long chunks attend none

@@ -634,8 +634,10 @@ void chunk_attention_kernel(ChunkArgs a) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) sc[s][nt][r] = r < left ? sc[s][nt][r] : kNegInf;
           }
-          // what no column attends may hold anything, a NaN included: 0 * NaN must not happen
+          // what no column attends may hold anything, a NaN included: 0 * NaN must not happen,
+          // nor 0 times the scale of 255, which is one too
           const int left = off ? 0 : all_keys - at;
+          sv[s] &= left >= 4 ? ~0u : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
 #pragma unroll
           for (int r = 0; r < 4; ++r)
 #pragma unroll
