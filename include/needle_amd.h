@@ -533,7 +533,8 @@ int ndl_kv_append_fp8(void* codes, void* scales, int64_t num_blocks, int num_kv_
 /*
  * Tokens first[i] .. of sequence i, cu_seqlens[i + 1] - cu_seqlens[i] of them, read back into
  * k_out and v_out [num_tokens][num_kv_heads][head_dim] (contiguous, 16-byte aligned) in `dtype`:
- * exactly the pool's values in bf16, rounded once in fp16 where that has no such number.  A
+ * exactly the pool's values in bf16, rounded once in fp16 where that has no such number (an fp16
+ * row's values of 63,488 and more, whose code is 65,536, become infinity).  A
  * position follows the append's slot rule (past the table: its last column); a negative one and
  * an invalid block id read as zeros; rows outside cu_seqlens are left as they were.
  */
@@ -552,6 +553,8 @@ int ndl_kv_read_fp8(void* k_out, void* v_out, const void* codes, const void* sca
  * and sums; probabilities rounded to the 16-bit format for the matrix cores.  Nothing to attend
  * (a negative context_lens[i], invalid block ids only): zeros.  A NaN in the pool reaches the
  * tokens that attend it and no others; rows that none attends may hold anything, in scales and codes.
+ * In fp16 the pool is of fp16 rows (scale bytes up to 135): a value of 65,536 counts as that or as
+ * 65,504.
  *
  * max_seqlen bounds the tokens of a sequence (those past it are not computed) and max_keys its
  * keys (context_lens[i] + tokens, at most max_blocks_per_seq * block_size; long chunks attend none

@@ -19,7 +19,8 @@
 //     no barrier is needed before the waves' results are combined.
 //   * Exact values.  e4m3 codes convert exactly to bf16 and fp16 (v_cvt_scalef32_pk_*_fp8), so
 //     the products are the 16-bit kernels' (fp32 sums).  K's scale multiplies the scores, where
-//     one factor is due anyway; V's is applied by the conversion, which is exact too.
+//     one factor is due anyway; V's is applied by the conversion, which is exact too but for fp16's
+//     subnormals (its other end, 65,536, is worked round).
 //   * P^T needs no data movement: with token slot 8 j + i of the PV product standing for token
 //     4 j + i (i < 4) or 12 + 4 j + i, the accumulator layout of S^T is the operand's.
 //   * Softmax in fp32 with exp2, scale * log2(e) folded.  The running maximum is raised (and the
@@ -27,8 +28,8 @@
 //     maximum is taken across lanes only then.
 //     P is rounded to the 16-bit format for the matrix cores; its sum is taken before that.
 //   * Long chunks (kUnpackRows columns, kUnpackScores scores) are bound by the products, not by the
-//     codes: their keys are unpacked once into a 16-bit pool in the workspace, exactly, and
-//     attended by varlen_prefill.hip's kernels (see launch_unpacked).
+//     codes: their keys are unpacked once into a 16-bit pool in the workspace and attended by
+//     varlen_prefill.hip's kernels (see launch_unpacked).
 //   * Split.  Either a workgroup per (kv head, row block), or, where those would leave the GPU
 //     idle or unevenly loaded, all row blocks' tiles of a kv head laid end to end and cut into
 //     equal shares, one per resident workgroup; what a share holds of a row block goes to a
@@ -239,6 +240,17 @@ __device__ __forceinline__ float max3(float x, float y, float z) {
   float m;
   asm("v_max3_f32 %0, %1, %2, %3" : "=v"(m) : "v"(x), "v"(y), "v"(z));
   return m;
+}
+
+// Two outputs in the 16-bit format.  In float16 those past it are its largest: they are sums of
+// values of 65,536 that were 65,504 or less before they were codes.
+template <bool F16>
+__device__ __forceinline__ uint32_t pack_out(float x, float y) {
+  if constexpr (F16) {
+    x = x > 65504.f ? 65504.f : x < -65504.f ? -65504.f : x;     // (a NaN stays)
+    y = y > 65504.f ? 65504.f : y < -65504.f ? -65504.f : y;
+  }
+  return Elt<F16>::pack(x, y);
 }
 
 // 0xff in every byte of w that is a NaN code (0x7f or 0xff).
@@ -721,6 +733,29 @@ void chunk_attention_kernel(ChunkArgs a) {
           for (int w = 0; w < VW; ++w) vc[i][w] &= ~nan_bytes(vc[i][w]);
       }
 
+      // A float16 row's values from 63,488 on are 256 * 2^8 as codes, 65,536, which float16 has not:
+      // such a row is converted under 2^7 and its probabilities (256 at most) doubled, both exact.
+      // Few rows reach 448 (a byte of 128): one test a step for all of them.
+      if constexpr (F16) {
+        if (__builtin_amdgcn_ballot_w64(((sv[0] | sv[1]) & 0x80808080u) != 0)) {
+          float f[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t big = ((sv[i >> 2] >> (8 * (i & 3))) & 0xffu) == 135u;
+            sv[i >> 2] -= big << (8 * (i & 3));
+            f[i] = big ? 2.f : 1.f;
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            u32x4 w = __builtin_bit_cast(u32x4, p[nt]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              w[i] = T::pack(T::lo(w[i]) * f[2 * i], T::hi(w[i]) * f[2 * i + 1]);
+            p[nt] = __builtin_bit_cast(X8, w);
+          }
+        }
+      }
+
       // O^T += V^T P^T: a pair of head_dim tiles at a time, the rows' pairs of codes turned into
       // pairs of tokens
       asm volatile("" : "+v"(sv[0]), "+v"(sv[1]));     // the scales no sooner than they are used
@@ -812,7 +847,7 @@ void chunk_attention_kernel(ChunkArgs a) {
                                     tok * a.group) * (int64_t)D + d0;
           uint32_t w[DB / 2];
 #pragma unroll
-          for (int b = 0; b < DB / 2; ++b) w[b] = T::pack(o[2 * b] * inv, o[2 * b + 1] * inv);
+          for (int b = 0; b < DB / 2; ++b) w[b] = pack_out<F16>(o[2 * b] * inv, o[2 * b + 1] * inv);
           if constexpr (DB == 8)
             st16(dst, u32x4{w[0], w[1], w[2], w[3]});
           else
@@ -834,7 +869,6 @@ constexpr int kMergeParts = 64;   // at a time
 
 template <int D, bool F16>
 __global__ __launch_bounds__(256) void chunk_merge_kernel(ChunkArgs a) {
-  using T = Elt<F16>;
   constexpr int PER = kMergeCols * D / 256;       // consecutive outputs of a thread: 4 or 2
   __shared__ float2 part[kMergeParts][kMergeCols];
   const int t = threadIdx.x, lane = t & 63;
@@ -913,9 +947,9 @@ __global__ __launch_bounds__(256) void chunk_merge_kernel(ChunkArgs a) {
   u16* const dst = a.out + ((it.tok0 + tok) * a.num_heads + head * a.group + col - tok * a.group) *
                                (int64_t)D + d0;
   if constexpr (PER == 4)
-    *reinterpret_cast<u32x2*>(dst) = u32x2{T::pack(o[0], o[1]), T::pack(o[2], o[3])};
+    *reinterpret_cast<u32x2*>(dst) = u32x2{pack_out<F16>(o[0], o[1]), pack_out<F16>(o[2], o[3])};
   else
-    *reinterpret_cast<uint32_t*>(dst) = T::pack(o[0], o[1]);
+    *reinterpret_cast<uint32_t*>(dst) = pack_out<F16>(o[0], o[1]);
 }
 
 // ---------------------------------------------------------------- long chunks
@@ -958,6 +992,8 @@ __device__ __forceinline__ Chunk chunk_of_seq(const UnpackArgs& a, int seq) {
 // per (tile, plane, kv head), heads next to each other as they lie in a block.  A NaN among the
 // chunk's own values becomes 0 here and reaches the tokens that attend it in chunk_nan_kernel:
 // the causal mask's 0 * NaN would bring it to those before it too.
+// In float16, which has no 65,536 (a row's values from 63,488 on), keys are halved, for which the
+// scores' scale makes up, and a value is 65,504, the nearest there is.
 template <int D, bool F16>
 __global__ __launch_bounds__(256) void chunk_unpack_kernel(UnpackArgs a) {
   constexpr int LPR = D / 8, RPL = 64 / LPR;     // lanes per row (8 codes each), rows per load
@@ -1003,10 +1039,17 @@ __global__ __launch_bounds__(256) void chunk_unpack_kernel(UnpackArgs a) {
         c[x][0] &= ~nan_bytes(c[x][0]);
         c[x][1] &= ~nan_bytes(c[x][1]);
       }
-      st16(dst + x * 512, u32x4{value2<F16, false>(c[x][0], scale[x]),
-                                value2<F16, true>(c[x][0], scale[x]),
-                                value2<F16, false>(c[x][1], scale[x]),
-                                value2<F16, true>(c[x][1], scale[x])});
+      if (F16 && !plane) scale[x] *= 0.5f;
+      u32x4 out{value2<F16, false>(c[x][0], scale[x]), value2<F16, true>(c[x][0], scale[x]),
+                value2<F16, false>(c[x][1], scale[x]), value2<F16, true>(c[x][1], scale[x])};
+      if (F16 && plane && scale[x] >= 256.f) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if ((out[i] & 0x7fffu) == 0x7c00u) out[i] -= 1u;
+          if ((out[i] & 0x7fff0000u) == 0x7c000000u) out[i] -= 0x10000u;
+        }
+      }
+      st16(dst + x * 512, out);
     }
   }
 }
@@ -1136,6 +1179,7 @@ int launch_unpacked(const ChunkArgs& c, const Unpacked& u, int max_seqlen, int64
                      dim3(256), 0, s, a);
   int rc = check_launch();
   if (rc != NDL_OK) return rc;
+  if (F16) scale *= 2.f;     // of halved keys
   // (the prefill sizes its split by the table, in the call as in the workspace query)
   const int64_t cached = (int64_t)(u.cols + 1) * block_size;
   void* const ws = u.prefill_bytes ? (char*)workspace + u.total() - u.prefill_bytes : nullptr;

@@ -8,8 +8,9 @@
 // and the row's values are code_d * 2^e.  The scale is a power of two because e4m3 is a floating
 // format: its step is relative (2^-4 of a value at most), so a finer scale gains nothing, the
 // largest value lands in (224, 448] and everything down to 2^-14 of it keeps full precision; one
-// byte per row then does, the multiplication is exact, and so is code * 2^e in bf16 (and in fp16
-// above its subnormals).
+// byte per row then does, the multiplication is exact, and so is code * 2^e in bf16.  In fp16 it is
+// between that format's ends: below 2^-14 it is rounded to a subnormal, and an fp16 row's values from
+// 63,488 on have the code of 65,536, which reads back as infinity.
 //
 // The reference has no such pool; the slot rule is its append's (needle/layers/attention.py:
 // 141-154, :224-237) and the rotation its _apply_rope (:277-288), as in rope_append.hip.

@@ -913,7 +913,8 @@ def kv_read_fp8(kv_codes: torch.Tensor, kv_scales: torch.Tensor, block_table: to
                 dtype: torch.dtype = torch.bfloat16):
     """Ranges of cached tokens in 16 bits: (k, v) [num_tokens, Hkv, D], packed by cu_seqlens, of
     the tokens first[i], first[i] + 1, .. of each sequence.  bfloat16 has every value of the pool
-    exactly; float16 every one that came from a float16 row, but for its smallest subnormals.
+    exactly; float16 every one that came from a float16 row, but for its smallest subnormals and
+    the codes of entries of 63,488 and more, which are 65,536 and read as infinity.
     first: int32 [num_seqs].  Rows outside cu_seqlens hold nothing in particular."""
     if _lib.NATIVE is not None:
         done = _lib.NATIVE.kv_read_fp8(kv_codes, kv_scales, block_table, first, cu_seqlens,
