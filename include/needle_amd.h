@@ -604,8 +604,8 @@ int ndl_fp8_decode_append(void* out, const void* q, int64_t q_tok_stride, const 
  *
  * Where temperature[i] is 0 or less, or a row's maximum is not finite, p is the point at the row's
  * argmax in torch's order (ndl_greedy_argmax).  Draft probabilities that are NaN or negative
- * count as 0 in max(p - q, 0), drafts outside the vocabulary are rejected, and u is taken within
- * [0, 1].
+ * count as 0 in max(p - q, 0), drafts outside the vocabulary are rejected, as are those whose row
+ * draft_probs has not (after a sequence without rows), and u is taken within [0, 1].
  *
  * tokens [num_rows], in ids' type: a sequence's accepted drafts, the next token, then -1;
  * accepted [num_seqs].  logits in `dtype`, any row stride of at least vocab; draft_probs float32

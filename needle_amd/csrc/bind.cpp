@@ -528,7 +528,7 @@ PyObject* verify_drafts(PyObject*, PyObject* const* args, Py_ssize_t n) {
         (rows > seqs && probs->stride(1) != 1))
       Py_RETURN_NONE;
     if (rows - seqs > 1 && (ds = probs->stride(0)) < vocab) Py_RETURN_NONE;
-    if (rows == seqs) probs = nullptr;   // no drafts, and no address either
+    if (rows == seqs) probs = &u;    // no rows and no address: one of which nothing is read
   }
   const c10::DeviceGuard guard(logits.device());
   at::Tensor tokens = at::empty_like(ids), accepted = at::empty({seqs}, cu.options());

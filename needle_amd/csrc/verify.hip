@@ -59,7 +59,7 @@ enum Kind { kNothing = 0, kPoint = 1, kAll = 2, kBut = 3, kLeft = 4 };
 // kPoint: all weight at `token`; kAll: exp; kBut: exp but for `token`; kLeft: max(p - q, 0)
 
 struct Drafted {         // of a drafted token, written by `stats`
-  int x;                 // the token, -1 outside the vocabulary
+  int x;                 // the token, -1 outside the vocabulary and without a draft row
   float l, q;            // its logit and its draft probability
   float u;
 };
@@ -198,10 +198,11 @@ __device__ __forceinline__ void gather_drafts(const VerifyArgs& a, int i) {
   for (int j = threadIdx.x; j < n - 1; j += kThreads) {
     const int64_t r = first + j, x = draft_at(a, r + 1), d = r - i;
     Drafted g{-1, kNegInf, 1.f, a.uniforms[r]};
-    if (x >= 0 && x < a.vocab) {
+    // (a row that draft_probs has not, as after a sequence without rows: nothing to judge it by)
+    if (x >= 0 && x < a.vocab && (!a.probs || (d >= 0 && d < a.probs_rows))) {
       g.x = (int)x;
       g.l = elem<FMT>(row_at<FMT>(a, r), x);
-      if (a.probs) g.q = d >= 0 && d < a.probs_rows ? a.probs[d * a.probs_stride + x] : 0.f;
+      if (a.probs) g.q = a.probs[d * a.probs_stride + x];
     }
     a.drafted[r] = g;
   }
@@ -809,7 +810,7 @@ int launch_verify(const VerifyArgs& a, hipStream_t s) {
   hipLaunchKernelGGL((verify_sums_kernel<FMT>), dim3((unsigned)a.sum_slices, seqs), wg, 0, s, a);
   rc = check_launch();
   if (rc != NDL_OK) return rc;
-  if (a.probs != nullptr) {
+  if (a.probs != nullptr && a.probs_rows > 0) {
     hipLaunchKernelGGL((verify_left_kernel<FMT>), dim3((unsigned)a.sum_slices, seqs), wg, 0, s,
                        a);
     rc = check_launch();

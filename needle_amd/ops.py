@@ -1092,8 +1092,10 @@ def verify_drafts(logits: torch.Tensor, ids: torch.Tensor, cu_seqlens: torch.Ten
     cumulative distribution at the sequence's last uniform: together distributed as the target.
 
     temperature float32 [num_seqs] (None: 1); 0 takes the argmax, as does a row whose maximum is
-    not finite.  uniforms float32 [T] in [0, 1).  tokens, in ids' type: the accepted drafts, the
-    next token, then -1.  Graph-capturable; no host synchronisation."""
+    not finite.  uniforms float32 [T] in [0, 1).  A draft whose row draft_probs has not (after a
+    sequence without rows) is rejected.  tokens, in ids' type: the accepted drafts, the next token,
+    then -1; rows outside cu_seqlens hold nothing in particular.  Graph-capturable; no host
+    synchronisation."""
     if _lib.NATIVE is not None:
         done = _lib.NATIVE.verify_drafts(logits, ids, cu_seqlens, uniforms, temperature,
                                          draft_probs)
@@ -1142,8 +1144,8 @@ def verify_drafts(logits: torch.Tensor, ids: torch.Tensor, cu_seqlens: torch.Ten
     lib = _lib.load()
     need = lib.ndl_verify_drafts_workspace_bytes(rows, n_seqs, vocab)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    # without drafts there are no draft rows, and no address either
-    probs = draft_probs if draft_probs is not None and rows > n_seqs else None
+    # no draft rows may have no address either: one of which nothing is read says that they are given
+    probs = draft_probs if draft_probs is None or rows > n_seqs else uniforms
     with _on(dev):
         rc = lib.ndl_verify_drafts(
             tokens.data_ptr(), accepted.data_ptr(), logits.data_ptr(),
