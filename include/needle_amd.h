@@ -559,10 +559,12 @@ int ndl_kv_read_fp8(void* k_out, void* v_out, const void* codes, const void* sca
  * max_seqlen bounds the tokens of a sequence (those past it are not computed) and max_keys its
  * keys (context_lens[i] + tokens, at most max_blocks_per_seq * block_size; long chunks attend none
  * past it): they choose how the work is split.  Long chunks (224 rows of max_seqlen times the
- * group, 2^24 scores by these bounds) unpack their keys into a 16-bit pool in the workspace first.
+ * group, 2^24 scores by these bounds) unpack their keys into a 16-bit pool in the workspace first: of
+ * as many sequences of max_keys as NDL_FP8_UNPACK_BYTES hold, one at least, the others after them.
  * The workspace (ndl_fp8_attention_workspace_bytes of the same sizes, max_keys cut to the table's,
  * on the same device; 0: none) is 256-byte aligned and belongs to one call at a time.
  */
+#define NDL_FP8_UNPACK_BYTES (4ll << 30)
 size_t ndl_fp8_attention_workspace_bytes(int num_seqs, int64_t num_tokens, int max_seqlen,
                                          int64_t max_keys, int num_heads, int num_kv_heads,
                                          int head_dim, int block_size);

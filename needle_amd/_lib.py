@@ -19,6 +19,7 @@ LIB_PATH = _PKG_DIR / "libneedle_amd.so"
 NDL_ABI_VERSION = 10
 NDL_DECODE_STATIC_SCRATCH_BYTES = 16 << 20
 NDL_PREFILL_SPLIT_MIN_KEYS = 768
+NDL_FP8_UNPACK_BYTES = 4 << 30
 NDL_DTYPE_BF16 = 0
 NDL_DTYPE_F16 = 1
 NDL_DTYPE_F32 = 2

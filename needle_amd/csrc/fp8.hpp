@@ -76,7 +76,9 @@ __device__ __forceinline__ void lds_dma16_each(const void* src, uint32_t lds_add
 
 // varlen_prefill.hip's attention for a caller with long, uneven prefixes: as
 // ndl_varlen_prefill_split, but split too where whole tiles would leave much of their last round
-// idle.  Its workspace: prefill_rounds_workspace_bytes.
+// idle.  The sequences may be some of a batch's, from any on: num_tokens are the batch's rows,
+// seqs_tokens bounds these sequences'.  Its workspace: prefill_rounds_workspace_bytes (of
+// seqs_tokens).
 size_t prefill_rounds_workspace_bytes(int num_seqs, int64_t num_tokens, int max_seqlen,
                                       int max_blocks_per_seq, int num_heads, int num_kv_heads,
                                       int head_dim, int block_size);
@@ -84,8 +86,8 @@ int launch_prefill_rounds(void* out, const void* q, int64_t q_tok_stride, const 
                           int64_t num_blocks, const int32_t* block_table, int64_t bt_row_stride,
                           int max_blocks_per_seq, const int32_t* cu_seqlens,
                           const int32_t* context_lens, int num_seqs, int64_t num_tokens,
-                          int max_seqlen, int max_context_len, int num_heads, int num_kv_heads,
-                          int head_dim, int block_size, int dtype, float scale, void* workspace,
-                          size_t workspace_bytes, ndl_stream_t stream);
+                          int64_t seqs_tokens, int max_seqlen, int max_context_len, int num_heads,
+                          int num_kv_heads, int head_dim, int block_size, int dtype, float scale,
+                          void* workspace, size_t workspace_bytes, ndl_stream_t stream);
 
 }  // namespace ndl

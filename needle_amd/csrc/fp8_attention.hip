@@ -1118,33 +1118,56 @@ __global__ __launch_bounds__(256) void chunk_nan_kernel(UnpackArgs a) {
 // 128 367 / 216; 14/2 heads of 64, 4, t 12,000, 32 34.6 / 53.3, 128 93.2 / 68.7.
 constexpr int64_t kUnpackRows = 224;
 constexpr int64_t kUnpackScores = (int64_t)1 << 24;
-constexpr int64_t kUnpackBytes = (int64_t)16 << 30;   // of the 16-bit pool
+// The 16-bit pool of a group of sequences, which are unpacked and attended together; one sequence is
+// a group of its own up to kUnpackMost, past which its chunk stays row blocks.  (Tables are as wide
+// as the longest sequence's, so the pool is the rectangle of all: one long prompt among many short
+// ones would take all there is.)  A group's launches end before the next one's begin: us, 32
+// sequences after 16,384, 32/8 heads of 128, in a pool of 2.1 GB / three of 0.7, 64 tokens each
+// 1,094 / 1,150, 256 tokens 2,695 / 2,795; 64 of 128 after 8,192, 28/4 heads, one of 1.1 GB / two
+// 1,347 / 1,356.
+constexpr int64_t kUnpackBytes = NDL_FP8_UNPACK_BYTES;
+constexpr int64_t kUnpackMost = (int64_t)16 << 30;
 
 struct Unpacked {
-  int cols;
+  int cols, seqs;               // of the table; sequences of a group
   int64_t blocks;
   size_t table_bytes, lens_bytes, pool_bytes, prefill_bytes;
   size_t total() const { return table_bytes + lens_bytes + pool_bytes + prefill_bytes; }
 };
+// Tokens that a group of seqs sequences can have.
+int64_t group_tokens(int64_t seqs, int64_t num_tokens, int max_seqlen) {
+  const int64_t most = seqs * max_seqlen;
+  return most < num_tokens ? most : num_tokens;
+}
 // Whether a call takes this path, and its workspace.
 bool unpacked_plan(int64_t num_seqs, int64_t num_tokens, int max_seqlen, int64_t max_keys,
                    int num_heads, int num_kv_heads, int head_dim, int block_size, Unpacked* u) {
   const int64_t rows = (int64_t)max_seqlen * (num_heads / num_kv_heads);
-  if (rows < kUnpackRows || num_seqs > 65535 ||
+  if (rows < kUnpackRows ||
       (double)rows * (double)max_keys * (double)(num_seqs * num_kv_heads) < (double)kUnpackScores)
     return false;
   const int64_t cols = (max_keys + block_size - 1) / block_size;
-  u->blocks = num_seqs * cols;
-  const int64_t bytes = u->blocks * block_size * num_kv_heads * head_dim * 4;
-  if (cols >= 0x7fffffff / block_size || u->blocks > 0x7fffffff || bytes > kUnpackBytes)
-    return false;
+  if (cols >= 0x7fffffff / block_size) return false;
+  const int64_t each = cols * block_size * num_kv_heads * head_dim * 4;
+  if (each > kUnpackMost) return false;
+  int64_t most = kUnpackBytes / each;
+  if (most > 65535) most = 65535;       // a grid dimension
+  if (most < 1) most = 1;
+  const int64_t groups = (num_seqs + most - 1) / most, seqs = (num_seqs + groups - 1) / groups;
   u->cols = (int)cols;
-  u->table_bytes = ((size_t)(u->blocks + num_seqs) * 4 + 255) / 256 * 256;
-  u->lens_bytes = ((size_t)num_seqs * 4 + 255) / 256 * 256;
-  u->pool_bytes = ((size_t)bytes + 255) / 256 * 256;
-  u->prefill_bytes =
-      prefill_rounds_workspace_bytes((int)num_seqs, num_tokens, max_seqlen, u->cols + 1, num_heads,
-                                     num_kv_heads, head_dim, block_size);
+  u->seqs = (int)seqs;
+  u->blocks = seqs * cols;
+  u->table_bytes = ((size_t)(u->blocks + seqs) * 4 + 255) / 256 * 256;
+  u->lens_bytes = ((size_t)seqs * 4 + 255) / 256 * 256;
+  u->pool_bytes = ((size_t)(seqs * each) + 255) / 256 * 256;
+  u->prefill_bytes = 0;
+  for (const int64_t n : {seqs, num_seqs % seqs}) {     // even groups, the last one
+    const size_t b = n == 0 ? 0
+                            : prefill_rounds_workspace_bytes(
+                                  (int)n, group_tokens(n, num_tokens, max_seqlen), max_seqlen,
+                                  u->cols + 1, num_heads, num_kv_heads, head_dim, block_size);
+    if (b > u->prefill_bytes) u->prefill_bytes = b;
+  }
   return true;
 }
 
@@ -1164,34 +1187,39 @@ int launch_unpacked(const ChunkArgs& c, const Unpacked& u, int max_seqlen, int64
   a.num_kv_heads = c.num_kv_heads;
   a.num_heads = c.num_heads;
   a.group = c.group;
-  a.block_table = c.block_table;
   a.bt_row_stride = c.bt_row_stride;
   a.tile_shift = c.tile_shift;
-  a.cu_seqlens = c.cu_seqlens;
-  a.context_lens = c.context_lens;
   a.num_tokens = c.num_tokens;
   a.out = c.out;
-  // workgroups of a sequence: what the longest can use, 16,384 over all sequences
-  const int64_t items = (max_keys + 15) / 16 * 2 * c.num_kv_heads;
-  int64_t wgs = (16384 + c.num_seqs - 1) / c.num_seqs;
-  if (wgs > (items + 3) / 4) wgs = (items + 3) / 4;
-  hipLaunchKernelGGL((chunk_unpack_kernel<D, F16>), dim3((unsigned)wgs, (unsigned)c.num_seqs),
-                     dim3(256), 0, s, a);
-  int rc = check_launch();
-  if (rc != NDL_OK) return rc;
-  if (F16) scale *= 2.f;     // of halved keys
   // (the prefill sizes its split by the table, in the call as in the workspace query)
   const int64_t cached = (int64_t)(u.cols + 1) * block_size;
-  void* const ws = u.prefill_bytes ? (char*)workspace + u.total() - u.prefill_bytes : nullptr;
-  rc = launch_prefill_rounds(c.out, c.q, c.q_stride, a.pool, u.blocks, a.table, u.cols + 1,
-                             u.cols + 1, c.cu_seqlens, a.lens, c.num_seqs, c.num_tokens, max_seqlen,
-                             (int)cached, c.num_heads, c.num_kv_heads, D, block_size,
-                             F16 ? NDL_DTYPE_F16 : NDL_DTYPE_BF16, scale, ws, u.prefill_bytes, s);
-  if (rc != NDL_OK) return rc;
+  const int64_t items = (max_keys + 15) / 16 * 2 * c.num_kv_heads;
   const int64_t scan = ((int64_t)(max_seqlen + 15) / 16 * c.num_kv_heads + 3) / 4;
-  hipLaunchKernelGGL((chunk_nan_kernel<D>), dim3((unsigned)scan, (unsigned)c.num_seqs), dim3(256),
-                     0, s, a);
-  return check_launch();
+  void* const ws = u.prefill_bytes ? (char*)workspace + u.total() - u.prefill_bytes : nullptr;
+  if (F16) scale *= 2.f;     // of halved keys
+  for (int64_t i0 = 0; i0 < c.num_seqs; i0 += u.seqs) {
+    const int n = (int)(c.num_seqs - i0 < u.seqs ? c.num_seqs - i0 : u.seqs);
+    a.block_table = c.block_table + i0 * c.bt_row_stride;
+    a.cu_seqlens = c.cu_seqlens + i0;
+    a.context_lens = c.context_lens + i0;
+    // workgroups of a sequence: what the longest can use, 16,384 over all of the group
+    int64_t wgs = (16384 + n - 1) / n;
+    if (wgs > (items + 3) / 4) wgs = (items + 3) / 4;
+    hipLaunchKernelGGL((chunk_unpack_kernel<D, F16>), dim3((unsigned)wgs, (unsigned)n), dim3(256),
+                       0, s, a);
+    int rc = check_launch();
+    if (rc != NDL_OK) return rc;
+    rc = launch_prefill_rounds(c.out, c.q, c.q_stride, a.pool, u.blocks, a.table, u.cols + 1,
+                               u.cols + 1, a.cu_seqlens, a.lens, n, c.num_tokens,
+                               group_tokens(n, c.num_tokens, max_seqlen), max_seqlen, (int)cached,
+                               c.num_heads, c.num_kv_heads, D, block_size,
+                               F16 ? NDL_DTYPE_F16 : NDL_DTYPE_BF16, scale, ws, u.prefill_bytes, s);
+    if (rc != NDL_OK) return rc;
+    hipLaunchKernelGGL((chunk_nan_kernel<D>), dim3((unsigned)scan, (unsigned)n), dim3(256), 0, s, a);
+    rc = check_launch();
+    if (rc != NDL_OK) return rc;
+  }
+  return NDL_OK;
 }
 
 // Column tiles of a row block: one where it holds max_seqlen tokens of a group's heads, else two.

@@ -1270,7 +1270,8 @@ static int launch_prefill(void* out, const void* q, int64_t q_tok_stride, const 
                           int max_seqlen, int max_context_len, int num_heads, int num_kv_heads,
                           int head_dim, int block_size, int dtype, float scale,
                           ndl_stream_t stream, void* workspace = nullptr,
-                          size_t workspace_bytes = 0, bool rounds = false) {
+                          size_t workspace_bytes = 0, bool rounds = false,
+                          int64_t rounds_tokens = 0) {
   if (!dtype_known(dtype)) return NDL_ERR_UNSUPPORTED;
   const int tshift = block_tile_shift(block_size);
   if (tshift < 0 || (head_dim != 64 && head_dim != 128)) return NDL_ERR_UNSUPPORTED;
@@ -1342,7 +1343,8 @@ static int launch_prefill(void* out, const void* q, int64_t q_tok_stride, const 
   const bool f16 = dtype_is_f16(dtype);
   PrefillSplit sp;
   if (workspace != nullptr && ((uintptr_t)workspace & 15u) == 0 && !any_scale &&
-      prefill_split(num_seqs, num_tokens, qtiles, num_heads, num_kv_heads, head_dim,
+      prefill_split(num_seqs, rounds ? rounds_tokens : num_tokens, qtiles, num_heads, num_kv_heads,
+                    head_dim,
                     longest_tiles(max_blocks_per_seq, block_size, max_context_len, max_seqlen),
                     rounds, &sp) &&
       workspace_bytes >= sp.bytes) {
@@ -1458,14 +1460,14 @@ int launch_prefill_rounds(void* out, const void* q, int64_t q_tok_stride, const 
                           int64_t num_blocks, const int32_t* block_table, int64_t bt_row_stride,
                           int max_blocks_per_seq, const int32_t* cu_seqlens,
                           const int32_t* context_lens, int num_seqs, int64_t num_tokens,
-                          int max_seqlen, int max_context_len, int num_heads, int num_kv_heads,
-                          int head_dim, int block_size, int dtype, float scale, void* workspace,
-                          size_t workspace_bytes, ndl_stream_t stream) {
+                          int64_t seqs_tokens, int max_seqlen, int max_context_len, int num_heads,
+                          int num_kv_heads, int head_dim, int block_size, int dtype, float scale,
+                          void* workspace, size_t workspace_bytes, ndl_stream_t stream) {
   return launch_prefill(out, q, q_tok_stride, nullptr, nullptr, 0, kv_cache, num_blocks,
                         block_table, bt_row_stride, max_blocks_per_seq, cu_seqlens, context_lens,
                         num_seqs, num_tokens, max_seqlen, max_context_len, num_heads, num_kv_heads,
                         head_dim, block_size, dtype, scale, stream, workspace, workspace_bytes,
-                        true);
+                        true, seqs_tokens);
 }
 
 }  // namespace ndl

@@ -220,13 +220,19 @@ class ModelRunner:
 
     def profile_memory(self, gpu_memory_utilization: float = 0.90, max_gpu_blocks: int = 0,
                        cpu_swap_bytes: int = 0):
-        """Blocks that fit in this share of the free device memory (optionally capped), and
-        the CPU swap pool's blocks for cpu_swap_bytes (runner.py:44-63 sizes that pool at
+        """Blocks that fit in this share of the free device memory (optionally capped; with an
+        8-bit pool less its attention's largest workspace), and the CPU swap pool's blocks for cpu_swap_bytes (runner.py:44-63 sizes that pool at
         half the GPU pool, ~128 GB of pinned memory on this GPU, so here the caller says)."""
         if self.device.type != "cuda":
             return (max_gpu_blocks or 512), cpu_swap_bytes // self.bytes_per_block()
         free, _total = torch.cuda.mem_get_info(self.device)
-        n = max(1, int(free * gpu_memory_utilization) // self.bytes_per_block())
+        budget = int(free * gpu_memory_utilization)
+        if self.fp8_cache:       # a prefill's unpacked keys come out of the same memory
+            cfg, most = self.model_config, self.model_config.max_position_embeddings
+            budget -= ops.fp8_attention_workspace_bytes(
+                1024, 1024 * most, most, most, cfg.num_attention_heads, cfg.num_kv_heads,
+                cfg.head_dim, self.block_size)
+        n = max(1, budget // self.bytes_per_block())
         if max_gpu_blocks:
             n = min(n, max_gpu_blocks)
         return n, cpu_swap_bytes // self.bytes_per_block()

@@ -1069,8 +1069,8 @@ def varlen_prefill_fp8(q: torch.Tensor, kv_codes: torch.Tensor, kv_scales: torch
     W * block_size) tokens.  max_seqlen bounds a sequence's tokens, max_context_len its cached
     ones (0: not known, the table's width then): sequences past these bounds are not attended
     whole.  Long chunks (224 rows of max_seqlen times H / Hkv and 2^24 scores by these bounds)
-    unpack the keys into a 16-bit workspace first, sized by the bounds, and are attended by
-    varlen_prefill's kernels."""
+    unpack the keys into a 16-bit workspace first, of as many sequences of the bounds' keys as 4 GiB
+    hold (one at least) at a time, and are attended by varlen_prefill's kernels."""
     return _fp8_attention(q, kv_codes, kv_scales, block_table, cu_seqlens, context_lens,
                           int(max_seqlen),
                           int(max_context_len) + int(max_seqlen) if max_context_len else 0,
