@@ -1314,8 +1314,10 @@ int launch(ChunkArgs a, int nt, int waves, hipStream_t s) {
   if (wgs > 0x7fffffff) return NDL_ERR_INVALID_ARG;
   void* args[] = {&a};
   if (hipLaunchKernel(kernel_of<D, F16>(nt, waves, a.new_k != nullptr), dim3((unsigned)wgs),
-                      dim3(64 * waves), args, 0, s) != hipSuccess)
+                      dim3(64 * waves), args, 0, s) != hipSuccess) {
+    (void)hipGetLastError();  // clear the error so that the next call's check sees its own
     return NDL_ERR_LAUNCH;
+  }
   const int rc = check_launch();
   if (rc != NDL_OK || a.shares == 0) return rc;
   const int groups = (a.toks * a.group + kMergeCols - 1) / kMergeCols;
