@@ -511,7 +511,9 @@ int ndl_greedy_argmax(void* out, int out_is_int64, const void* logits, int64_t r
  * row (a token's head_dim values of one head).  A row's values are code * 2^(byte - 127), byte
  * from 1 to 254 (0 only with codes of 0, as a zero-filled pool has).  Built for head_dim 64 and
  * 128, block_size a power of two from 16 to 1024 and bf16 / fp16 activations
- * (NDL_ERR_UNSUPPORTED otherwise).
+ * (NDL_ERR_UNSUPPORTED otherwise).  A call of so many tokens or sequences that a launch of it would
+ * have 2^32 threads (2^24 sequences times kv heads, 2^26 tokens at one kv head) is refused
+ * (NDL_ERR_INVALID_ARG).
  *
  * ndl_kv_append_fp8: k and v [num_tokens][num_kv_heads][head_dim] (token strides multiples of 8)
  * into the slots of ndl_kv_append (cu_seqlens NULL: one token per sequence).  With a the largest

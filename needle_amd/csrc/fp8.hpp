@@ -6,6 +6,12 @@
 
 namespace ndl {
 
+// Whether a launch's first grid dimension can be that many workgroups: HIP counts its threads in 32
+// bits, and launches the rest of a larger one without an error.
+inline bool grid_fits(int64_t workgroups, int threads) {
+  return workgroups <= (int64_t)0xffffffffu / threads;
+}
+
 // Two e4m3 codes of w's low or high half times scale (a power of two), in the 16-bit format.
 template <bool F16, bool HI>
 __device__ __forceinline__ uint32_t value2(uint32_t w, float scale) {

@@ -1139,6 +1139,10 @@ int64_t group_tokens(int64_t seqs, int64_t num_tokens, int max_seqlen) {
   const int64_t most = seqs * max_seqlen;
   return most < num_tokens ? most : num_tokens;
 }
+// Workgroups of chunk_nan_kernel per sequence.
+int64_t nan_scan_workgroups(int max_seqlen, int num_kv_heads) {
+  return (((int64_t)max_seqlen + 15) / 16 * num_kv_heads + 3) / 4;
+}
 // Whether a call takes this path, and its workspace.
 bool unpacked_plan(int64_t num_seqs, int64_t num_tokens, int max_seqlen, int64_t max_keys,
                    int num_heads, int num_kv_heads, int head_dim, int block_size, Unpacked* u) {
@@ -1147,7 +1151,8 @@ bool unpacked_plan(int64_t num_seqs, int64_t num_tokens, int max_seqlen, int64_t
       (double)rows * (double)max_keys * (double)(num_seqs * num_kv_heads) < (double)kUnpackScores)
     return false;
   const int64_t cols = (max_keys + block_size - 1) / block_size;
-  if (cols >= 0x7fffffff / block_size) return false;
+  if (cols >= 0x7fffffff / block_size || !grid_fits(nan_scan_workgroups(max_seqlen, num_kv_heads), 256))
+    return false;
   const int64_t each = cols * block_size * num_kv_heads * head_dim * 4;
   if (each > kUnpackMost) return false;
   int64_t most = kUnpackBytes / each;
@@ -1194,7 +1199,7 @@ int launch_unpacked(const ChunkArgs& c, const Unpacked& u, int max_seqlen, int64
   // (the prefill sizes its split by the table, in the call as in the workspace query)
   const int64_t cached = (int64_t)(u.cols + 1) * block_size;
   const int64_t items = (max_keys + 15) / 16 * 2 * c.num_kv_heads;
-  const int64_t scan = ((int64_t)(max_seqlen + 15) / 16 * c.num_kv_heads + 3) / 4;
+  const int64_t scan = nan_scan_workgroups(max_seqlen, c.num_kv_heads);
   void* const ws = u.prefill_bytes ? (char*)workspace + u.total() - u.prefill_bytes : nullptr;
   if (F16) scale *= 2.f;     // of halved keys
   for (int64_t i0 = 0; i0 < c.num_seqs; i0 += u.seqs) {
@@ -1311,7 +1316,7 @@ template <int D, bool F16>
 int launch(ChunkArgs a, int nt, int waves, hipStream_t s) {
   const int64_t units = a.shares ? a.shares : ((int64_t)a.items + 7) / 8 * 8;
   const int64_t wgs = units * a.num_kv_heads;
-  if (wgs > 0x7fffffff) return NDL_ERR_INVALID_ARG;
+  if (!grid_fits(wgs, 64 * waves)) return NDL_ERR_INVALID_ARG;
   void* args[] = {&a};
   if (hipLaunchKernel(kernel_of<D, F16>(nt, waves, a.new_k != nullptr), dim3((unsigned)wgs),
                       dim3(64 * waves), args, 0, s) != hipSuccess) {

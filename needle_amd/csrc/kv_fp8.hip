@@ -314,7 +314,7 @@ extern "C" int ndl_kv_append_fp8(void* codes, void* scales, int64_t num_blocks, 
   const int64_t rounds = (2 * num_kv_heads + rpr - 1) / rpr + (q ? (num_heads + rpr - 1) / rpr : 0);
   const int64_t groups = (rounds + kRounds - 1) / kRounds;
   const int64_t blocks = (num_tokens * groups + 3) / 4;
-  if (blocks > 0x7fffffff) return NDL_ERR_INVALID_ARG;
+  if (!grid_fits(blocks, 256)) return NDL_ERR_INVALID_ARG;
   const dim3 grid((unsigned)blocks), wg(256);
   const hipStream_t s = (hipStream_t)stream;
   const bool f16 = dtype_is_f16(dtype);
@@ -367,7 +367,7 @@ extern "C" int ndl_kv_read_fp8(void* k_out, void* v_out, const void* codes, cons
   const int64_t items = num_tokens * 2 * num_kv_heads * (head_dim / 8);
   const int64_t blocks = (items + 4 * kReadItems - 1) / (4 * kReadItems);
   if (num_kv_heads > 4096) return NDL_ERR_UNSUPPORTED;
-  if (blocks > 0x7fffffff) return NDL_ERR_INVALID_ARG;
+  if (!grid_fits(blocks, 256)) return NDL_ERR_INVALID_ARG;
   const dim3 grid((unsigned)blocks), wg(256);
   const hipStream_t s = (hipStream_t)stream;
   const bool f16 = dtype_is_f16(dtype);
