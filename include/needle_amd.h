@@ -73,7 +73,9 @@ extern "C" {
 /* Same object as hipStream_t; declared here so callers need no HIP headers. */
 typedef struct ihipStream_t* ndl_stream_t;
 
-/* 9: the float32 decode, prefill split and few-row linear entry points. */
+/* 9: the float32 decode, prefill split and few-row linear entry points.  10: ndl_kv_append_fp8,
+ * ndl_kv_read_fp8, ndl_fp8_attention, ndl_fp8_decode_append, ndl_verify_drafts and the workspace
+ * queries of the last three. */
 #define NDL_ABI_VERSION 10
 
 enum ndl_status {
@@ -521,7 +523,9 @@ int ndl_greedy_argmax(void* out, int out_is_int64, const void* logits, int64_t r
  * has a <= 448 times it, and the codes are the values divided by it, rounded to nearest even; NaN
  * where a value is not finite.  With cos and sin (rows of cs_tok_stride) k is rotated first, as
  * ndl_rope_kv_append does, and with q and q_out (both or neither, q needs cos) q is rotated into
- * q_out [num_tokens][num_heads][head_dim].  16-byte aligned pointers but for the scales.
+ * q_out [num_tokens][num_heads][head_dim].  16-byte aligned pointers but for the scales.  Two tokens
+ * of a call in one slot (past the table's end) leave a row that may be neither's: the codes of one,
+ * the scale of the other.
  */
 int ndl_kv_append_fp8(void* codes, void* scales, int64_t num_blocks, int num_kv_heads,
                       int block_size, int head_dim, int dtype, const void* k,
@@ -611,8 +615,8 @@ int ndl_fp8_decode_append(void* out, const void* q, int64_t q_tok_stride, const 
  * count as 0 in max(p - q, 0), drafts outside the vocabulary are rejected, as are those whose row
  * draft_probs has not (after a sequence without rows), and u is taken within [0, 1].
  *
- * tokens [num_rows], in ids' type: a sequence's accepted drafts, the next token, then -1;
- * accepted [num_seqs].  logits in `dtype`, any row stride of at least vocab; draft_probs float32
+ * tokens [num_rows], in ids' type: a sequence's accepted drafts, the next token, then -1, rows
+ * outside cu_seqlens left as they were; accepted [num_seqs].  logits in `dtype`, any row stride of at least vocab; draft_probs float32
  * [num_rows - num_seqs] rows; uniforms and temperature float32 [num_rows], [num_seqs]
  * (temperature NULL: 1).  num_rows and num_seqs at most 65535, vocab at most 2^18
  * (NDL_ERR_UNSUPPORTED otherwise).  The workspace is 256-byte aligned and belongs to one call at a
