@@ -36,7 +36,7 @@
 //     workspace and is merged by a second launch.
 // Measured (us, bytes read at): 64 sequences of 512 to 4,096 tokens, 32/8 heads of 128, one token
 // each 47 + 4.8 of merge, 5.6 TB/s in the first launch; 24 sequences of 4,096 to 32,768, 28/4
-// heads, float16, 72 + 6.3, 6.0 TB/s; 1 to 8 tokens each after 512 to 4,096 55 + 7.9, 4.9 TB/s.
+// heads, float16, 72 + 6.9, 6.0 TB/s; 1 to 8 tokens each after 512 to 4,096 55 + 7.9, 4.9 TB/s.
 // A few short sequences take 5 us, of which each step of a wave (a tile) is 1: about 270
 // instructions, two waves to a SIMD; sixteen waves or deeper rings measured the same or slower.
 #include "fp8.hpp"
@@ -735,7 +735,9 @@ void chunk_attention_kernel(ChunkArgs a) {
 
       // A float16 row's values from 63,488 on are 256 * 2^8 as codes, 65,536, which float16 has not:
       // such a row is converted under 2^7 and its probabilities (256 at most) doubled, both exact.
-      // Few rows reach 448 (a byte of 128): one test a step for all of them.
+      // Few rows reach 448 (a byte of 128): one test a step for all of them (us without / with, 24
+      // sequences of 4,096 to 32,768, 28/4 heads 82.4 / 83.2; 64 of 2,048 to 4,096 with 5 drafts 85.1 /
+      // 85.7).
       if constexpr (F16) {
         if (__builtin_amdgcn_ballot_w64(((sv[0] | sv[1]) & 0x80808080u) != 0)) {
           float f[8];
