@@ -75,8 +75,9 @@ typedef struct ihipStream_t* ndl_stream_t;
 
 /* 9: the float32 decode, prefill split and few-row linear entry points.  10: ndl_kv_append_fp8,
  * ndl_kv_read_fp8, ndl_fp8_attention, ndl_fp8_decode_append, ndl_verify_drafts and the workspace
- * queries of the last three. */
-#define NDL_ABI_VERSION 10
+ * queries of the last three.  11: ndl_tree_mask, ndl_tree_attention, ndl_fp8_tree_attention,
+ * ndl_verify_tree, ndl_kv_compact, ndl_attention_mass, ndl_kv_select and their workspace queries. */
+#define NDL_ABI_VERSION 11
 
 enum ndl_status {
   NDL_OK = 0,
@@ -629,6 +630,67 @@ int ndl_verify_drafts(void* tokens, int32_t* accepted, const void* logits, int64
                       int64_t draft_stride, int64_t num_draft_rows, int64_t num_rows,
                       int num_seqs, int vocab, void* workspace, size_t workspace_bytes,
                       ndl_stream_t stream);
+
+/*
+ * Drafted trees.  The nodes of sequence i's tree are its rows cu_seqlens[i] .. of the packed rows,
+ * node 0 its newest token; parents[t] is the node (within the sequence) that row t's token follows.
+ * A parent comes before its children: any other number (-1, the node's own or a later one) says
+ * that the node follows the cached tokens alone.
+ *
+ * ndl_tree_mask: bit b % 64 of word b / 64 of a token's mask row (mask_words uint64, rows of
+ * mask_stride, 8-byte aligned) is set where node b is the token itself or one of its ancestors,
+ * and depth is the number of those ancestors (the token's position less the context's length).
+ * Nodes past the words have no bit.  max_seqlen bounds the nodes of a sequence: those past its
+ * multiple of 256 are left as they were, as are rows outside cu_seqlens.
+ */
+int ndl_tree_mask(void* mask, int64_t mask_stride, int mask_words, int32_t* depth,
+                  const int32_t* parents, const int32_t* cu_seqlens, int num_seqs,
+                  int64_t num_tokens, int max_seqlen, ndl_stream_t stream);
+
+/*
+ * Attention of trees over a 16-bit pool (bf16, fp16).  The nodes' K and V are in the cache already,
+ * node b of sequence i at position context_lens[i] + b.  Each token attends the first
+ * context_lens[i] tokens and the nodes whose bits its mask row has (ndl_tree_mask's, or any other:
+ * bits of nodes that the sequence has not are not looked at), within the
+ * max_blocks_per_seq * block_size tokens of the table.  out [num_tokens][num_heads][head_dim];
+ * q rows of q_tok_stride (a multiple of 8); groups of 1 to 16 query heads per kv head.  fp32 scores,
+ * softmax and sums; probabilities rounded to the 16-bit format for the matrix cores.  Nothing to
+ * attend (a negative context_lens[i], an empty mask row without a context, invalid block ids only):
+ * zeros.  What is not finite reaches the tokens that attend it and no others; rows that none
+ * attends may hold anything.
+ *
+ * max_seqlen bounds the tokens of a sequence (those past it may not be computed) and max_keys its keys
+ * (context_lens[i] + tokens): they choose how the work is split.  The workspace
+ * (ndl_tree_attention_workspace_bytes of the same sizes, max_keys cut to the table's, on the same
+ * device; 0: none) is 256-byte aligned and belongs to one call at a time.
+ */
+size_t ndl_tree_attention_workspace_bytes(int num_seqs, int max_seqlen, int64_t max_keys,
+                                          int num_heads, int num_kv_heads, int head_dim,
+                                          int block_size);
+int ndl_tree_attention(void* out, const void* q, int64_t q_tok_stride, const void* kv_cache,
+                       int64_t num_blocks, const int32_t* block_table, int64_t bt_row_stride,
+                       int max_blocks_per_seq, const int32_t* cu_seqlens,
+                       const int32_t* context_lens, const void* mask, int64_t mask_stride,
+                       int mask_words, int num_seqs, int64_t num_tokens, int max_seqlen,
+                       int64_t max_keys, int num_heads, int num_kv_heads, int head_dim,
+                       int block_size, int dtype, float scale, void* workspace,
+                       size_t workspace_bytes, ndl_stream_t stream);
+
+/*
+ * The same over the 8-bit pool, with what ndl_fp8_attention says of its values.  The workspace is
+ * ndl_fp8_tree_attention_workspace_bytes.
+ */
+size_t ndl_fp8_tree_attention_workspace_bytes(int num_seqs, int max_seqlen, int64_t max_keys,
+                                              int num_heads, int num_kv_heads, int head_dim,
+                                              int block_size);
+int ndl_fp8_tree_attention(void* out, const void* q, int64_t q_tok_stride, const void* codes,
+                           const void* scales, int64_t num_blocks, const int32_t* block_table,
+                           int64_t bt_row_stride, int max_blocks_per_seq,
+                           const int32_t* cu_seqlens, const int32_t* context_lens,
+                           const void* mask, int64_t mask_stride, int mask_words, int num_seqs,
+                           int64_t num_tokens, int max_seqlen, int64_t max_keys, int num_heads,
+                           int num_kv_heads, int head_dim, int block_size, int dtype, float scale,
+                           void* workspace, size_t workspace_bytes, ndl_stream_t stream);
 
 #ifdef __cplusplus
 }

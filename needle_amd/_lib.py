@@ -16,7 +16,7 @@ import torch  # noqa: F401  (loads torch's HIP runtime before ours)
 _PKG_DIR = Path(__file__).resolve().parent
 LIB_PATH = _PKG_DIR / "libneedle_amd.so"
 
-NDL_ABI_VERSION = 10
+NDL_ABI_VERSION = 11
 NDL_DECODE_STATIC_SCRATCH_BYTES = 16 << 20
 NDL_PREFILL_SPLIT_MIN_KEYS = 768
 NDL_FP8_UNPACK_BYTES = 4 << 30
@@ -55,6 +55,11 @@ EXPORTED_SYMBOLS = (
     "ndl_fp8_decode_append",
     "ndl_verify_drafts_workspace_bytes",
     "ndl_verify_drafts",
+    "ndl_tree_mask",
+    "ndl_tree_attention_workspace_bytes",
+    "ndl_tree_attention",
+    "ndl_fp8_tree_attention_workspace_bytes",
+    "ndl_fp8_tree_attention",
 )
 
 _c_i32 = ctypes.c_int
@@ -226,6 +231,30 @@ _SIGNATURES = {
         _c_p, _c_i64, _c_i64,                           # draft probs, stride, rows
         _c_i64, _c_i32, _c_i32,                         # T, B, V
         _c_p, _c_sz, _c_p,                              # workspace, bytes, stream
+    ]),
+    "ndl_tree_mask": (_c_i32, [
+        _c_p, _c_i64, _c_i32, _c_p,                     # mask, stride, words, depth
+        _c_p, _c_p, _c_i32, _c_i64, _c_i32, _c_p,       # parents, cu, B, T, max_seqlen, stream
+    ]),
+    "ndl_tree_attention_workspace_bytes": (_c_sz, [_c_i32, _c_i32, _c_i64] + [_c_i32] * 4),
+    "ndl_tree_attention": (_c_i32, [
+        _c_p, _c_p, _c_i64,                             # out, q, q stride
+        _c_p, _c_i64,                                   # cache, NB
+        _c_p, _c_i64, _c_i32,                           # block_table, row stride, W
+        _c_p, _c_p, _c_p, _c_i64, _c_i32,               # cu, ctx, mask, stride, words
+        _c_i32, _c_i64, _c_i32, _c_i64,                 # B, T, max_seqlen, max_keys
+        _c_i32, _c_i32, _c_i32, _c_i32, _c_i32,         # H, Hkv, D, bs, dtype
+        _c_f32, _c_p, _c_sz, _c_p,                      # scale, workspace, bytes, stream
+    ]),
+    "ndl_fp8_tree_attention_workspace_bytes": (_c_sz, [_c_i32, _c_i32, _c_i64] + [_c_i32] * 4),
+    "ndl_fp8_tree_attention": (_c_i32, [
+        _c_p, _c_p, _c_i64,                             # out, q, q stride
+        _c_p, _c_p, _c_i64,                             # codes, scales, NB
+        _c_p, _c_i64, _c_i32,                           # block_table, row stride, W
+        _c_p, _c_p, _c_p, _c_i64, _c_i32,               # cu, ctx, mask, stride, words
+        _c_i32, _c_i64, _c_i32, _c_i64,                 # B, T, max_seqlen, max_keys
+        _c_i32, _c_i32, _c_i32, _c_i32, _c_i32,         # H, Hkv, D, bs, dtype
+        _c_f32, _c_p, _c_sz, _c_p,                      # scale, workspace, bytes, stream
     ]),
 }
 

@@ -41,15 +41,14 @@
 // instructions, two waves to a SIMD; sixteen waves or deeper rings measured the same or slower.
 #include "fp8.hpp"
 
-#include "chunk_shares.hpp"
+#include "chunk_stream.hpp"
 
 namespace ndl {
 namespace {
 
-constexpr int kTile = 32;       // tokens per wave step
 constexpr float kRaise = 8.f;   // log2 of the largest probability before the maximum is raised
 
-struct ChunkArgs {
+struct ChunkOperands {
   u16* out;
   const u16* q;
   int64_t q_stride;
@@ -64,144 +63,11 @@ struct ChunkArgs {
   const u16* cos;               // with new rows: q and k are not rotated yet (null: they are)
   const u16* sin;
   int64_t cs_stride;
-  const int32_t* block_table;
-  int64_t bt_row_stride;
-  int max_blocks;
-  int tile_shift;               // log2(block_size / 16)
-  const int32_t* cu_seqlens;    // null: one token per sequence
-  const int32_t* context_lens;
-  int num_seqs;
-  int64_t num_tokens;
-  int toks;                     // query tokens of a row block
-  int blocks_per_seq;           // row blocks a sequence can have
-  int items;                    // num_seqs * blocks_per_seq
-  float scale_log2;
-  // the split into equal shares (shares 0: a workgroup per row block)
-  int shares;                   // per kv head
-  int min_chunk;                // slots a share has at least
-  int pad;                      // empty slots before each row block: what its start costs
-  int nseg;                     // segment slots per kv head: shares + items
-  float* ws_ml;                 // [kv head][segment][column][2]
-  float* ws_acc;                // [kv head][segment][column][D]
 };
-
-// A row block: tokens tok0 .. tok0 + n of the packed rows, the first at position pos.
-struct Item {
-  int64_t tok0;
-  int n;
-  int seq;
-  int64_t pos;
-  int64_t cap;                  // keys a table row holds
-  __device__ __forceinline__ int64_t keys() const {     // of its last token
-    const int64_t k = pos + n;
-    return n <= 0 || pos < 0 ? 0 : k < cap ? k : cap;
-  }
-  __device__ __forceinline__ int tiles() const { return (int)((keys() + kTile - 1) / kTile); }
-};
-
-// The sequence of row block e (32-bit: a 64-bit division takes a hundred instructions).
-__device__ __forceinline__ int seq_of_item(const ChunkArgs& a, int e) {
-  return a.blocks_per_seq == 1 ? e : (int)((uint32_t)e / (uint32_t)a.blocks_per_seq);
-}
-__device__ __forceinline__ Item item_of(const ChunkArgs& a, int e) {
-  Item it;
-  it.seq = seq_of_item(a, e);
-  const int j0 = (e - it.seq * a.blocks_per_seq) * a.toks;
-  int64_t first = it.seq, count = 1;
-  if (a.cu_seqlens != nullptr) {
-    first = a.cu_seqlens[it.seq];
-    count = a.cu_seqlens[it.seq + 1] - first;
-    if (first < 0 || first + count > a.num_tokens) count = 0;
-  }
-  it.tok0 = first + j0;
-  it.n = (int)(count - j0 < a.toks ? count - j0 : a.toks);
-  const int64_t ctx = a.context_lens[it.seq];
-  it.pos = ctx < 0 ? -1 : ctx + j0;      // a negative context: nothing is attended
-  it.cap = (int64_t)a.max_blocks << (4 + a.tile_shift);
-  return it;
-}
-
-__device__ __forceinline__ int slots_of(const ChunkArgs& a, int e) {
-  if (e >= a.items) return 0;
-  const int n = item_of(a, e).tiles();
-  return n > 0 ? n + a.pad : 0;
-}
-
-// Inclusive prefix sum over the wave: by shifts within rows of 16 lanes, then the rows before.
-template <int PATTERN>
-__device__ __forceinline__ int dpp_add(int v) {
-  return v + __builtin_amdgcn_update_dpp(0, v, PATTERN, 0xf, 0xf, true);
-}
-__device__ __forceinline__ int wave_scan(int v, int lane) {
-  v = dpp_add<0x111>(v);         // row_shr:1, 0 from outside the row
-  v = dpp_add<0x112>(v);
-  v = dpp_add<0x114>(v);
-  v = dpp_add<0x118>(v);
-  const int r0 = __builtin_amdgcn_readlane(v, 15), r1 = __builtin_amdgcn_readlane(v, 31),
-            r2 = __builtin_amdgcn_readlane(v, 47);
-  return v + (lane >= 16 ? r0 : 0) + (lane >= 32 ? r1 : 0) + (lane >= 48 ? r2 : 0);
-}
-
-// The row blocks of a kv head laid end to end, in slots: their prefix sums, 64 to a step.  Up to
-// kHeld row blocks stay in registers, loaded at once; more are read again where they are needed.
-constexpr int kSteps = 4, kHeld = 64 * kSteps;
-struct Place {
-  int e, first, slots;          // a row block, its first slot, how many it has
-};
-struct Stream {
-  int total;
-  Cut cut;
-  int v[kSteps], incl[kSteps];
-
-  __device__ __forceinline__ void read(const ChunkArgs& a, int lane) {
-    total = 0;
-#pragma unroll
-    for (int k = 0; k < kSteps; ++k) v[k] = 64 * k < a.items ? slots_of(a, 64 * k + lane) : 0;
-#pragma unroll
-    for (int k = 0; k < kSteps; ++k) {
-      incl[k] = total;
-      if (64 * k < a.items) {
-        incl[k] = wave_scan(v[k], lane) + total;
-        total = __builtin_amdgcn_readlane(incl[k], 63);
-      }
-    }
-    for (int base = kHeld; base < a.items; base += 64)
-      total += __builtin_amdgcn_readlane(wave_scan(slots_of(a, base + lane), lane), 63);
-    cut = cut_of(total, a.shares, a.min_chunk, a.pad);
-  }
-  // The row block that holds slot `at` (at < total), or row block `e` if that is not negative.
-  __device__ __forceinline__ Place find(const ChunkArgs& a, int lane, int at, int e) const {
-#pragma unroll
-    for (int k = 0; k < kSteps; ++k) {
-      const uint64_t hit = e >= 0 ? __builtin_amdgcn_ballot_w64(64 * k + lane == e)
-                                  : __builtin_amdgcn_ballot_w64(v[k] > 0 && incl[k] > at);
-      if (hit) {
-        const int l = __builtin_ctzll(hit);
-        const int n = __builtin_amdgcn_readlane(v[k], l);
-        return Place{64 * k + l, __builtin_amdgcn_readlane(incl[k], l) - n, n};
-      }
-    }
-    int carry = __builtin_amdgcn_readlane(incl[kSteps - 1], 63);
-    for (int base = kHeld; base < a.items; base += 64) {
-      const int w = slots_of(a, base + lane), in = wave_scan(w, lane) + carry;
-      const uint64_t hit = e >= 0 ? __builtin_amdgcn_ballot_w64(base + lane == e)
-                                  : __builtin_amdgcn_ballot_w64(w > 0 && in > at);
-      if (hit) {
-        const int l = __builtin_ctzll(hit);
-        const int n = __builtin_amdgcn_readlane(w, l);
-        return Place{base + l, __builtin_amdgcn_readlane(in, l) - n, n};
-      }
-      carry = __builtin_amdgcn_readlane(in, 63);
-    }
-    return Place{a.items, carry, 0};
-  }
-  // Where share s begins.
-  __device__ __forceinline__ int begin(const ChunkArgs& a, int lane, int s) const {
-    const int x = s * cut.chunk;   // fits 31 bits: make_plan
-    if (x >= total) return total;
-    const Place p = find(a, lane, x, -1);
-    return share_begin(x, p.first, p.slots, cut.snap);
-  }
+struct ChunkArgs : ChunkOperands, RowBlocks {
+  const uint64_t* mask;         // of a tree's tokens: rows of bits of the chunk's tokens (else null)
+  int64_t mask_stride;
+  int words;
 };
 
 // Waits until at most n (0 .. MAX) groups of I loads are in flight.
@@ -353,8 +219,9 @@ struct NewRow {
 
 // A workgroup's share of the row blocks of one kv head.  NEW: the sequence's new row is quantised
 // by the wave whose tile holds its position, which puts it into the ring for itself and into the
-// pool.  (head_dim 64: 128 registers, as without, so that as many workgroups are resident.)
-template <int D, bool F16, int NT, int NW, bool NEW = false>
+// pool.  TREE: a token attends what its row of the mask says of the chunk.  (head_dim 64: 128
+// registers, as without, so that as many workgroups are resident.)
+template <int D, bool F16, int NT, int NW, bool NEW = false, bool TREE = false>
 __global__ __launch_bounds__(64 * NW, NEW && D == 64 ? 4 : 8 / NW)
 void chunk_attention_kernel(ChunkArgs a) {
   using T = Elt<F16>;
@@ -389,7 +256,7 @@ void chunk_attention_kernel(ChunkArgs a) {
     if (e >= a.items) return;
   } else {
     if (unit >= a.shares) return;
-    Stream st;
+    Stream<TREE> st;
     st.read(a, lane);
     from = st.begin(a, lane, unit);
     to = st.begin(a, lane, unit + 1);
@@ -416,7 +283,7 @@ void chunk_attention_kernel(ChunkArgs a) {
     };
     if constexpr (NEW) fresh.load(a, seq_of_item(a, e), head, lane, lds_addr(fresh_lds));
     if (whole) load_window(0);        // before the lengths arrive
-    const Item it = item_of(a, e);
+    const Item it = item_of<TREE>(a, e);
     const int ntiles = it.tiles();
     int t1 = ntiles;
     if (!whole) {
@@ -433,7 +300,7 @@ void chunk_attention_kernel(ChunkArgs a) {
 
     // Columns: 16 nt + c is query token col / g, head head * g + col % g.
     X8 q[NT][KS];
-    int lim[NT];                  // keys the column attends
+    int lim[NT];                  // keys the column attends (TREE: the token)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       int col = 16 * nt + c;
@@ -445,7 +312,7 @@ void chunk_attention_kernel(ChunkArgs a) {
       for (int s = 0; s < KS; ++s)
         q[nt][s] = __builtin_bit_cast(X8, ld16(src + 64 * (s >> 1) + 16 * j + 8 * (s & 1)));
       const int64_t k = it.pos + tok + 1;
-      lim[nt] = (int)(k < it.cap ? k : it.cap);
+      lim[nt] = TREE ? tok : (int)(k < it.cap ? k : it.cap);
     }
     // the new row's position in the table (past the end the last column is written again, as an
     // append does) and the step of this wave that attends it
@@ -459,7 +326,10 @@ void chunk_attention_kernel(ChunkArgs a) {
       if (at_new >= 0 && tile >= t0 && tile < t1 && (tile - t0) % NW == wv)
         u_new = (tile - t0) / NW;
     }
-    const int64_t k_first = it.pos + 1 < it.cap ? it.pos + 1 : it.cap;
+    // keys that every token attends: up to the first one, or (TREE) up to the chunk
+    const int64_t chunk_at = it.pos - (int64_t)(e - it.seq * a.blocks_per_seq) * a.toks;
+    const int64_t k_all = TREE ? chunk_at : it.pos + 1;
+    const int64_t k_first = k_all < it.cap ? k_all : it.cap;
     const int all_keys = (int)it.keys();      // of the last token
     const int min_keys = k_first < 0 ? 0 : (int)k_first;   // of the first
 
@@ -635,13 +505,32 @@ void chunk_attention_kernel(ChunkArgs a) {
       const int tile = t0 + wv + NW * u;
       const bool masked = bad != 0 || kTile * (tile + 1) > min_keys;
       uint32_t nan_any = 0;
+      uint32_t vis[NT];             // TREE: the columns' bits of this tile
       if (masked) {
+        if constexpr (TREE) {
+          const int kv0 = kTile * tile;
+          uint32_t some = low_bits(all_keys - kv0);
+          if (bad & 1) some &= 0xffff0000u;
+          if (bad & 2) some &= 0x0000ffffu;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            vis[nt] = kv0 + kTile > min_keys
+                          ? some & bits_at(a.mask + (it.tok0 + lim[nt]) * a.mask_stride, a.words,
+                                           kv0 - (int)chunk_at)
+                          : some;
+        }
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           const int at = kTile * tile + 16 * s + 4 * j;     // the lane's first token
           const bool off = (bad >> s) & 1;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
+            if constexpr (TREE) {
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                sc[s][nt][r] = (vis[nt] >> (16 * s + 4 * j + r)) & 1u ? sc[s][nt][r] : kNegInf;
+              continue;
+            }
             const int left = off ? 0 : lim[nt] - at;
 #pragma unroll
             for (int r = 0; r < 4; ++r) sc[s][nt][r] = r < left ? sc[s][nt][r] : kNegInf;
@@ -695,7 +584,7 @@ void chunk_attention_kernel(ChunkArgs a) {
 
       // A NaN in a value that some of the chunk's tokens attend and others do not: it is taken
       // out of the product and put into the columns that attend it.
-      if (masked && a.toks > 1 && __builtin_amdgcn_ballot_w64(nan_any != 0)) {
+      if (masked && (TREE || a.toks > 1) && __builtin_amdgcn_ballot_w64(nan_any != 0)) {
         constexpr uint32_t one = F16 ? 0x3c00u : 0x3f80u;
         X8 seen[NT];
 #pragma unroll
@@ -704,6 +593,11 @@ void chunk_attention_kernel(ChunkArgs a) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int s = i >> 1, at = kTile * tile + 16 * s + 4 * j + 2 * (i & 1);
+            if constexpr (TREE) {
+              const uint32_t two = vis[nt] >> (16 * s + 4 * j + 2 * (i & 1));
+              w[i] = (two & 1u ? one : 0u) | (two & 2u ? one << 16 : 0u);
+              continue;
+            }
             const int left = (bad >> s) & 1 ? 0 : lim[nt] - at;
             w[i] = (left > 0 ? one : 0u) | (left > 1 ? one << 16 : 0u);
           }
@@ -863,95 +757,19 @@ void chunk_attention_kernel(ChunkArgs a) {
   if constexpr (NEW) vm_wait<0>();     // rows of a row block that is not this share's
 }
 
-// One workgroup per (row block, kv head, kMergeCols columns): the parts that the shares hold,
-// combined in their order; zeros for tokens with nothing to attend.  A row block inside one share
-// was written by the attention.
-constexpr int kMergeCols = 8;
-constexpr int kMergeParts = 64;   // at a time
-
-template <int D, bool F16>
+template <int D, bool F16, bool TREE>
 __global__ __launch_bounds__(256) void chunk_merge_kernel(ChunkArgs a) {
-  constexpr int PER = kMergeCols * D / 256;       // consecutive outputs of a thread: 4 or 2
-  __shared__ float2 part[kMergeParts][kMergeCols];
-  const int t = threadIdx.x, lane = t & 63;
-  const int e = blockIdx.x, head = blockIdx.y, c0 = blockIdx.z * kMergeCols;
-  const Item it = item_of(a, e);
-  Stream st;
-  st.read(a, lane);
-  const Place p = st.find(a, lane, 0, e);
-  if (it.n <= 0 || c0 >= it.n * a.group) return;
-  const int cols = it.n * a.group - c0 < kMergeCols ? it.n * a.group - c0 : kMergeCols;
-  const int c = t * PER / D, d0 = t * PER - c * D;
-  float o[PER];
-#pragma unroll
-  for (int x = 0; x < PER; ++x) o[x] = 0.f;
-  // its slots by the scan that gave its place and the cut: whatever the lengths are, or become while
-  // this runs, share_parts names shares that there are, whose parts the workspace holds
-  if (p.slots > 0) {
-    int s0, s1;
-    if (!share_parts(p.first, p.slots, st.cut, &s0, &s1)) return;   // written by the attention
-    const int n = s1 - s0 + 1, per = a.toks * a.group;
-    const int64_t seg = ((int64_t)head * a.nseg + s0 + e) * per + c0;
-    const float2* const ml = reinterpret_cast<const float2*>(a.ws_ml) + seg;
-    const float* const src = a.ws_acc + seg * D + (int64_t)(c < cols ? c : 0) * D + d0;
-    // this thread's column's maximum over all parts, then 64 parts at a time
-    const int64_t step = (int64_t)per * D;
-    float mx = kNegInf, l = 0.f;
-    for (int pass = 0; pass < 2; ++pass) {
-      for (int i0 = 0; i0 < n; i0 += kMergeParts) {
-        const int m = n - i0 < kMergeParts ? n - i0 : kMergeParts;
-        if (pass == 0 || n > kMergeParts) {
-          __syncthreads();
-          for (int i = t; i < m * kMergeCols; i += 256)
-            if (i % kMergeCols < cols)
-              part[i / kMergeCols][i % kMergeCols] =
-                  ml[(int64_t)(i0 + i / kMergeCols) * per + i % kMergeCols];
-          __syncthreads();
-        }
-        if (c >= cols) continue;
-        if (pass == 0) {
-          for (int i = 0; i < m; ++i) mx = fmaxf(mx, part[i][c].x);
-          continue;
-        }
-        for (int i = 0; i < m; i += 8) {
-          float v[8][PER];
-#pragma unroll
-          for (int y = 0; y < 8; ++y) {
-            const float* const q = src + (int64_t)(i0 + (i + y < m ? i + y : i)) * step;
-            if constexpr (PER == 4) {
-              const f32x4 w = *reinterpret_cast<const f32x4*>(q);
-#pragma unroll
-              for (int x = 0; x < PER; ++x) v[y][x] = w[x];
-            } else {
-              const f32x2 w = *reinterpret_cast<const f32x2*>(q);
-              v[y][0] = w[0];
-              v[y][1] = w[1];
-            }
-          }
-#pragma unroll
-          for (int y = 0; y < 8; ++y) {
-            if (i + y >= m) break;
-            const float2 ms = part[i + y][c];
-            const float f = ms.x == mx ? 1.f : fast_exp2(ms.x - mx);
-            l += ms.y * f;
-#pragma unroll
-            for (int x = 0; x < PER; ++x) o[x] += v[y][x] * f;
-          }
-        }
-      }
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-    for (int x = 0; x < PER; ++x) o[x] *= inv;
-  }
-  if (c >= cols) return;
-  const int col = c0 + c, tok = col / a.group;
-  u16* const dst = a.out + ((it.tok0 + tok) * a.num_heads + head * a.group + col - tok * a.group) *
-                               (int64_t)D + d0;
-  if constexpr (PER == 4)
-    *reinterpret_cast<u32x2*>(dst) = u32x2{pack_out<F16>(o[0], o[1]), pack_out<F16>(o[2], o[3])};
-  else
-    *reinterpret_cast<uint32_t*>(dst) = pack_out<F16>(o[0], o[1]);
+  merge_row_block<D, TREE>(a, a.group, [&](const Item& it, int head, int col, int d0,
+                                            const float* o, float, float) {
+    constexpr int PER = kMergeCols * D / 256;
+    const int tok = col / a.group;
+    u16* const dst = a.out + ((it.tok0 + tok) * a.num_heads + head * a.group + col -
+                              tok * a.group) * (int64_t)D + d0;
+    if constexpr (PER == 4)
+      *reinterpret_cast<u32x2*>(dst) = u32x2{pack_out<F16>(o[0], o[1]), pack_out<F16>(o[2], o[3])};
+    else
+      *reinterpret_cast<uint32_t*>(dst) = pack_out<F16>(o[0], o[1]);
+  });
 }
 
 // ---------------------------------------------------------------- long chunks
@@ -1240,16 +1058,20 @@ struct Plan {
   size_t ml_bytes, acc_bytes;
 };
 
+template <int D, bool F16, bool TREE>
+const void* chunk_kernel(int nt, int waves) {
+  if (waves == 4)
+    return nt == 1 ? (const void*)chunk_attention_kernel<D, F16, 1, 4, false, TREE>
+                   : (const void*)chunk_attention_kernel<D, F16, 2, 4, false, TREE>;
+  return nt == 1 ? (const void*)chunk_attention_kernel<D, F16, 1, 8, false, TREE>
+                 : (const void*)chunk_attention_kernel<D, F16, 2, 8, false, TREE>;
+}
 template <int D, bool F16>
-const void* kernel_of(int nt, int waves, bool append = false) {
+const void* kernel_of(int nt, int waves, bool append = false, bool tree = false) {
   if (append)       // one token per sequence: one column tile
     return waves == 4 ? (const void*)chunk_attention_kernel<D, F16, 1, 4, true>
                       : (const void*)chunk_attention_kernel<D, F16, 1, 8, true>;
-  if (waves == 4)
-    return nt == 1 ? (const void*)chunk_attention_kernel<D, F16, 1, 4>
-                   : (const void*)chunk_attention_kernel<D, F16, 2, 4>;
-  return nt == 1 ? (const void*)chunk_attention_kernel<D, F16, 1, 8>
-                 : (const void*)chunk_attention_kernel<D, F16, 2, 8>;
+  return tree ? chunk_kernel<D, F16, true>(nt, waves) : chunk_kernel<D, F16, false>(nt, waves);
 }
 
 // Slots a share has at least: two tiles for each of four waves.
@@ -1320,7 +1142,7 @@ int launch(ChunkArgs a, int nt, int waves, hipStream_t s) {
   const int64_t wgs = units * a.num_kv_heads;
   if (!grid_fits(wgs, 64 * waves)) return NDL_ERR_INVALID_ARG;
   void* args[] = {&a};
-  if (hipLaunchKernel(kernel_of<D, F16>(nt, waves, a.new_k != nullptr), dim3((unsigned)wgs),
+  if (hipLaunchKernel(kernel_of<D, F16>(nt, waves, a.new_k != nullptr, a.mask != nullptr), dim3((unsigned)wgs),
                       dim3(64 * waves), args, 0, s) != hipSuccess) {
     (void)hipGetLastError();  // clear the error so that the next call's check sees its own
     return NDL_ERR_LAUNCH;
@@ -1328,9 +1150,11 @@ int launch(ChunkArgs a, int nt, int waves, hipStream_t s) {
   const int rc = check_launch();
   if (rc != NDL_OK || a.shares == 0) return rc;
   const int groups = (a.toks * a.group + kMergeCols - 1) / kMergeCols;
-  hipLaunchKernelGGL((chunk_merge_kernel<D, F16>),
-                     dim3((unsigned)a.items, (unsigned)a.num_kv_heads, (unsigned)groups), dim3(256),
-                     0, s, a);
+  const dim3 grid((unsigned)a.items, (unsigned)a.num_kv_heads, (unsigned)groups);
+  if (a.mask != nullptr)
+    hipLaunchKernelGGL((chunk_merge_kernel<D, F16, true>), grid, dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL((chunk_merge_kernel<D, F16, false>), grid, dim3(256), 0, s, a);
   return check_launch();
 }
 
@@ -1353,7 +1177,7 @@ extern "C" size_t ndl_fp8_attention_workspace_bytes(int num_seqs, int64_t num_to
   return p.ml_bytes + p.acc_bytes;
 }
 
-// Both entry points; `a` holds the new rows and the rotation of the second one.
+// All entry points; `a` holds the new rows and the rotation of a decode step, or a tree's mask.
 static int fp8_attention(ndl::ChunkArgs a, void* out, const void* q, int64_t q_tok_stride,
                          void* codes, void* scales, int64_t num_blocks,
                          const int32_t* block_table, int64_t bt_row_stride,
@@ -1403,7 +1227,7 @@ static int fp8_attention(ndl::ChunkArgs a, void* out, const void* q, int64_t q_t
   const hipStream_t s = (hipStream_t)stream;
   const bool f16 = dtype_is_f16(dtype);
   Unpacked u;
-  if (cu_seqlens != nullptr && unpacked_plan(num_seqs, num_tokens, max_seqlen, max_keys, num_heads,
+  if (cu_seqlens != nullptr && a.mask == nullptr && unpacked_plan(num_seqs, num_tokens, max_seqlen, max_keys, num_heads,
                                              num_kv_heads, head_dim, block_size, &u)) {
     if (!workspace || workspace_bytes < u.total() || (uintptr_t)workspace & 255u)
       return NDL_ERR_WORKSPACE;
@@ -1487,4 +1311,41 @@ extern "C" int ndl_fp8_decode_append(void* out, const void* q, int64_t q_tok_str
                        bt_row_stride, max_blocks_per_seq, nullptr, context_lens, num_seqs,
                        num_seqs, 1, keys > 0 ? keys : 1, num_heads, num_kv_heads, head_dim,
                        block_size, dtype, scale, workspace, workspace_bytes, stream);
+}
+
+extern "C" size_t ndl_fp8_tree_attention_workspace_bytes(int num_seqs, int max_seqlen,
+                                                         int64_t max_keys, int num_heads,
+                                                         int num_kv_heads, int head_dim,
+                                                         int block_size) {
+  using namespace ndl;
+  if (num_seqs <= 0 || max_seqlen <= 0 || max_keys <= 0 || max_keys > 0x7fffff00 ||
+      !shape_ok(head_dim, block_size, num_heads, num_kv_heads))
+    return 0;
+  const Plan p = plan_for(num_seqs, max_seqlen, max_keys, num_heads, num_kv_heads, head_dim);
+  return p.ml_bytes + p.acc_bytes;
+}
+
+extern "C" int ndl_fp8_tree_attention(void* out, const void* q, int64_t q_tok_stride,
+                                      const void* codes, const void* scales, int64_t num_blocks,
+                                      const int32_t* block_table, int64_t bt_row_stride,
+                                      int max_blocks_per_seq, const int32_t* cu_seqlens,
+                                      const int32_t* context_lens, const void* mask,
+                                      int64_t mask_stride, int mask_words, int num_seqs,
+                                      int64_t num_tokens, int max_seqlen, int64_t max_keys,
+                                      int num_heads, int num_kv_heads, int head_dim,
+                                      int block_size, int dtype, float scale, void* workspace,
+                                      size_t workspace_bytes, ndl_stream_t stream) {
+  using namespace ndl;
+  if (num_seqs > 0 && num_tokens > 0 &&
+      (!cu_seqlens || !mask || mask_words <= 0 || mask_stride < mask_words ||
+       (uintptr_t)mask & 7u))
+    return NDL_ERR_INVALID_ARG;
+  ChunkArgs a{};
+  a.mask = (const uint64_t*)mask;
+  a.mask_stride = mask_stride;
+  a.words = mask_words;
+  return fp8_attention(a, out, q, q_tok_stride, (void*)codes, (void*)scales, num_blocks,
+                       block_table, bt_row_stride, max_blocks_per_seq, cu_seqlens, context_lens,
+                       num_seqs, num_tokens, max_seqlen, max_keys, num_heads, num_kv_heads,
+                       head_dim, block_size, dtype, scale, workspace, workspace_bytes, stream);
 }

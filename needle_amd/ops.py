@@ -1155,3 +1155,133 @@ def verify_drafts(logits: torch.Tensor, ids: torch.Tensor, cu_seqlens: torch.Ten
             need, _stream(dev))
     _lib.check(rc, "ndl_verify_drafts")
     return tokens, accepted
+
+
+# ---------------------------------------------------------------- drafted trees
+
+def tree_mask(parents: torch.Tensor, cu_seqlens: torch.Tensor, max_seqlen: int):
+    """Which nodes a drafted tree's tokens attend: (mask int64 [T, ceil(max_seqlen / 64)],
+    depth int32 [T]), once a step for tree_attention of every layer.
+
+    parents int32 [T]: for each packed token the node of its own sequence (0 .. its rows) that it
+    follows.  Node 0 is the sequence's newest token, and parents come before their children: any other
+    number (-1, say) stands for a node that follows the cached tokens alone.  Bit b % 64 of word
+    b // 64 is set for the token itself and its ancestors; depth counts the ancestors, so that
+    context_lens[i] + depth is the token's position for the rotary embedding.  max_seqlen bounds a
+    sequence's tokens.  Rows outside cu_seqlens hold nothing in particular."""
+    _require(parents.is_cuda, "parents must be a GPU tensor")
+    dev = parents.device
+    _check_int32("parents", parents, 1, dev)
+    _check_int32("cu_seqlens", cu_seqlens, 1, dev)
+    n_seqs, n_tok = cu_seqlens.shape[0] - 1, parents.shape[0]
+    _require(n_seqs >= 0, "cu_seqlens must be [num_seqs + 1]")
+    _require(max_seqlen > 0, "max_seqlen must be positive")
+    words = (max_seqlen + 63) // 64
+    mask = torch.empty((n_tok, words), dtype=torch.int64, device=dev)
+    depth = torch.empty(n_tok, dtype=torch.int32, device=dev)
+    if n_tok == 0 or n_seqs == 0:
+        return mask, depth
+    with _on(dev):
+        rc = _lib.load().ndl_tree_mask(
+            mask.data_ptr(), words, words, depth.data_ptr(), parents.data_ptr(),
+            cu_seqlens.data_ptr(), n_seqs, n_tok, max_seqlen, _stream(dev))
+    _lib.check(rc, "ndl_tree_mask")
+    return mask, depth
+
+
+def tree_attention_workspace_bytes(num_seqs: int, max_seqlen: int, max_keys: int, num_heads: int,
+                                   num_kv_heads: int, head_dim: int, block_size: int = 16,
+                                   fp8: bool = False) -> int:
+    """Bytes of the workspace tree_attention uses over a 16-bit (fp8: an 8-bit) pool on the current
+    GPU, max_keys at most the table's; 0 where none is used."""
+    lib = _lib.load()
+    query = (lib.ndl_fp8_tree_attention_workspace_bytes if fp8
+             else lib.ndl_tree_attention_workspace_bytes)
+    return int(query(num_seqs, max_seqlen, max_keys, num_heads, num_kv_heads, head_dim,
+                     block_size))
+
+
+def _check_out(out, n_tok, num_heads, head_dim, like):
+    shape = (n_tok, num_heads, head_dim)
+    if out is None:
+        return torch.empty(shape, dtype=like.dtype, device=like.device)
+    _require(out.shape == shape and out.is_contiguous() and out.dtype == like.dtype
+             and out.device == like.device,
+             f"out must be a contiguous {like.dtype} {list(shape)} tensor on {like.device}")
+    return out
+
+
+def _check_group(num_heads, num_kv_heads):
+    if num_kv_heads <= 0 or num_heads % num_kv_heads or not 0 < num_heads // num_kv_heads <= 16:
+        raise ValueError(f"num_heads {num_heads} must be 1 to 16 times num_kv_heads "
+                         f"{num_kv_heads}")
+
+
+def tree_attention(q: torch.Tensor, kv_cache, block_table: torch.Tensor,
+                   cu_seqlens: torch.Tensor, context_lens: torch.Tensor, mask: torch.Tensor,
+                   max_seqlen: int, scale: float, num_heads: int, num_kv_heads: int,
+                   head_dim: int, *, max_context_len: int = 0,
+                   out: Optional[torch.Tensor] = None,
+                   workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """varlen_prefill for drafted trees: each token of a sequence's chunk attends what is cached and
+    those of the chunk's tokens whose bits its row of mask (tree_mask) has, itself among them.
+    The chunk's K and V are in the cache already (kv_append, kv_append_fp8), token j of sequence i at
+    position context_lens[i] + j, whatever position its rotary embedding stands for.
+
+    q [T, H, D] in bfloat16 or float16; kv_cache a 16-bit pool of the same type, or an Fp8KVCache.
+    mask int64 [T, words]: bit b % 64 of word b // 64 for token b of the sequence.  A token that
+    attends nothing gets zeros.  max_seqlen bounds a sequence's tokens, max_context_len its cached
+    ones (0: not known, the table's width then): sequences past these bounds are not attended
+    whole."""
+    pool = kv_cache.codes if isinstance(kv_cache, Fp8KVCache) else kv_cache
+    _check_cache(pool) if pool is kv_cache else _check_fp8_cache(*kv_cache)
+    dev = pool.device
+    _, nb, hkv, bs, d = pool.shape
+    _require(hkv == num_kv_heads and d == head_dim, "kv_cache shape disagrees with head counts")
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"q must be bfloat16 or float16, got {q.dtype}")
+    if pool is kv_cache:
+        _require(q.dtype == pool.dtype, "q dtype must match kv_cache", TypeError)
+    qs = _rows("q", q, num_heads, head_dim, dev)
+    _check_group(num_heads, num_kv_heads)
+    n_seqs, n_tok = _check_table(block_table, nb, dev), q.shape[0]
+    _check_int32("cu_seqlens", cu_seqlens, 1, dev)
+    _check_int32("context_lens", context_lens, 1, dev)
+    _require(cu_seqlens.shape[0] == n_seqs + 1 and context_lens.shape[0] == n_seqs,
+             "cu_seqlens / context_lens / block_table batch mismatch")
+    if mask.dtype != torch.int64:
+        raise TypeError(f"mask must be int64, got {mask.dtype}")
+    if mask.dim() != 2 or mask.shape[0] != n_tok or mask.shape[1] < 1:
+        raise ValueError(f"mask must be [{n_tok}, words], got {tuple(mask.shape)}")
+    words = mask.shape[1]
+    if mask.device != dev or (n_tok and words > 1 and mask.stride(1) != 1):
+        raise ValueError(f"mask rows must be contiguous on {dev}")
+    ms = mask.stride(0) if n_tok > 1 else words
+    _require(ms >= words, "mask rows overlap")
+    out = _check_out(out, n_tok, num_heads, head_dim, q)
+    if n_tok == 0 or n_seqs == 0:
+        return out
+    w = block_table.shape[1]
+    _require(w > 0, "block_table has no columns")
+    _require(max_seqlen > 0, "max_seqlen must be positive")
+    _require(max_context_len >= 0, "max_context_len is negative")
+    max_keys = min(w * bs, max_context_len + max_seqlen) if max_context_len else w * bs
+    lib = _lib.load()
+    fp8 = pool is not kv_cache
+    with _on(dev):
+        need = tree_attention_workspace_bytes(n_seqs, max_seqlen, max_keys, num_heads,
+                                              num_kv_heads, head_dim, bs, fp8)
+        if need and (workspace is None or workspace.numel() * workspace.element_size() < need
+                     or workspace.device != dev):
+            workspace = decode_workspace(need, dev)
+        tail = (nb, block_table.data_ptr(), block_table.stride(0), w, cu_seqlens.data_ptr(),
+                context_lens.data_ptr(), mask.data_ptr(), ms, words, n_seqs, n_tok, max_seqlen,
+                max_keys, num_heads, num_kv_heads, head_dim, bs, _DTYPES[q.dtype], float(scale),
+                _ptr(workspace) if need else None, need, _stream(dev))
+        if fp8:
+            rc = lib.ndl_fp8_tree_attention(out.data_ptr(), q.data_ptr(), qs, pool.data_ptr(),
+                                            kv_cache.scales.data_ptr(), *tail)
+        else:
+            rc = lib.ndl_tree_attention(out.data_ptr(), q.data_ptr(), qs, pool.data_ptr(), *tail)
+    _lib.check(rc, "ndl_fp8_tree_attention" if fp8 else "ndl_tree_attention")
+    return out
