@@ -692,6 +692,33 @@ int ndl_fp8_tree_attention(void* out, const void* q, int64_t q_tok_stride, const
                            int num_kv_heads, int head_dim, int block_size, int dtype, float scale,
                            void* workspace, size_t workspace_bytes, ndl_stream_t stream);
 
+/*
+ * Verification of drafted trees.  Row r of logits and of ids is a node of its sequence's tree
+ * (parents as above; ids[r] its token, logits[r] the target's row for what follows it), node 0 the
+ * newest token.  From node 0 on, with p = softmax(logits[r] / temperature[i]) of the node r and its
+ * children in the order of their rows, the path goes to the first child whose token's p, added to
+ * those of the children before it (a token that several have counts once), is more than
+ * uniforms[r].  Where there is none the next token is drawn with
+ * u = uniforms[cu_seqlens[i + 1] - 1], a leaf's: from p of the last node without its children's
+ * tokens, the first v whose weights up to v sum to more than u times their total (the row's argmax
+ * where they have all weight).  The tokens are distributed as the target's; a chain gives what
+ * ndl_verify_drafts gives without draft_probs.
+ *
+ * Where temperature[i] is 0 or less, or a row's maximum is not finite, p is the point at the row's
+ * argmax in torch's order.  Tokens outside the vocabulary are not taken; a sequence's rows past its
+ * 1,024th are no part of its tree.
+ *
+ * tokens [num_rows], in ids' type: the path's tokens after node 0, the next token, then -1; path
+ * [num_rows]: the path's nodes (0, ..), then -1; accepted [num_seqs]: the nodes after node 0.  Rows
+ * outside cu_seqlens are left as they were.  Sizes, formats and workspace as ndl_verify_drafts.
+ */
+size_t ndl_verify_tree_workspace_bytes(int64_t num_rows, int num_seqs, int vocab);
+int ndl_verify_tree(void* tokens, int32_t* accepted, int32_t* path, const void* logits,
+                    int64_t row_stride, int dtype, const void* ids, int ids_are_int64,
+                    const int32_t* parents, const int32_t* cu_seqlens, const float* uniforms,
+                    const float* temperature, int64_t num_rows, int num_seqs, int vocab,
+                    void* workspace, size_t workspace_bytes, ndl_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

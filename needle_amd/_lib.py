@@ -60,6 +60,8 @@ EXPORTED_SYMBOLS = (
     "ndl_tree_attention",
     "ndl_fp8_tree_attention_workspace_bytes",
     "ndl_fp8_tree_attention",
+    "ndl_verify_tree_workspace_bytes",
+    "ndl_verify_tree",
 )
 
 _c_i32 = ctypes.c_int
@@ -255,6 +257,12 @@ _SIGNATURES = {
         _c_i32, _c_i64, _c_i32, _c_i64,                 # B, T, max_seqlen, max_keys
         _c_i32, _c_i32, _c_i32, _c_i32, _c_i32,         # H, Hkv, D, bs, dtype
         _c_f32, _c_p, _c_sz, _c_p,                      # scale, workspace, bytes, stream
+    ]),
+    "ndl_verify_tree_workspace_bytes": (_c_sz, [_c_i64, _c_i32, _c_i32]),  # T, B, V
+    "ndl_verify_tree": (_c_i32, [
+        _c_p, _c_p, _c_p, _c_p, _c_i64, _c_i32,         # tokens, accepted, path, logits, stride, dtype
+        _c_p, _c_i32, _c_p, _c_p, _c_p, _c_p,           # ids, int64, parents, cu, uniforms, temp.
+        _c_i64, _c_i32, _c_i32, _c_p, _c_sz, _c_p,      # T, B, V, workspace, bytes, stream
     ]),
 }
 

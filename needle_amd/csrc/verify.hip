@@ -25,6 +25,14 @@
 // The chosen row's weights and sums are in fp64: a token's border is found among up to 2^17
 // others, where fp32 sums (2^-24 of the total each) would pick a neighbour now and then.
 // Sums run in a fixed order without atomics: the same inputs give the same tokens.
+//
+// Trees (TREE): the rows are nodes, row j of a sequence follows the node parents[j] before it (node 0,
+// the newest token, is where the path begins).  At a node with children c1 < c2 < .., tokens x1, x2,
+// .., the path goes on to the first ck with  u < p(x1) + .. + p(xk)  (a token that siblings share
+// counts once); where there is none the next token has the node's p without its children's tokens.
+// That is a draw of p for every node, so the tokens are distributed as the target's; a chain gives
+// what points give above.  Four launches: after stats a workgroup per sequence walks its tree (walk),
+// then sums and pick as above, the children's tokens as bits over a slice.
 #include "ndl_common.hpp"
 
 #include <type_traits>
@@ -51,7 +59,7 @@ struct Info {            // of a sequence, written by `sums`
   int accepted;
   int kind;              // see Kind
   int64_t row;           // chosen row
-  int64_t draft_row;     // its row of draft_probs
+  int64_t draft_row;     // its row of draft_probs (TREE: the node)
   int token;             // the point's token, or the draft that was rejected
   float top;             // the row's maximum
 };
@@ -60,9 +68,12 @@ enum Kind { kNothing = 0, kPoint = 1, kAll = 2, kBut = 3, kLeft = 4 };
 
 struct Drafted {         // of a drafted token, written by `stats`
   int x;                 // the token, -1 outside the vocabulary and without a draft row
-  float l, q;            // its logit and its draft probability
+  float l, q;            // its logit and its draft probability (TREE: its parent's bits)
   float u;
 };
+constexpr int kTreeNodes = 1024;     // of a sequence: further rows are no part of its tree
+constexpr int kWalkThreads = 1024;
+constexpr int kNodeBytes = 40;       // of LDS that the walk needs for one
 
 struct VerifyArgs {
   const void* logits;
@@ -87,6 +98,8 @@ struct VerifyArgs {
   Info* info;                  // [num_seqs]
   double* sums;                // [num_seqs][sum_slices]
   double* left;                // likewise
+  const int32_t* parents;      // a tree's
+  int32_t* path;
 };
 
 template <int FMT>
@@ -191,10 +204,26 @@ __device__ __forceinline__ float rate_of(float temp) {
 
 // The drafted tokens of sequence i: what decides on them beside the rows' statistics, in the shadow
 // of the rows' workgroups (three trips to memory).
-template <int FMT>
+template <int FMT, bool TREE>
 __device__ __forceinline__ void gather_drafts(const VerifyArgs& a, int i) {
   int64_t first;
   const int n = seq_rows(a, i, &first);
+  if constexpr (TREE) {
+    for (int j = threadIdx.x; j < n; j += kThreads) {
+      const int p = a.parents[first + j];
+      const int64_t x = draft_at(a, first + j);
+      Drafted g{-1, kNegInf, __int_as_float(-1), 0.f};
+      if (p >= 0 && p < j) {
+        g.q = __int_as_float(p);
+        if (x >= 0 && x < a.vocab) {
+          g.x = (int)x;
+          g.l = elem<FMT>(row_at<FMT>(a, first + p), x);
+        }
+      }
+      a.drafted[first + j] = g;
+    }
+    return;
+  }
   for (int j = threadIdx.x; j < n - 1; j += kThreads) {
     const int64_t r = first + j, x = draft_at(a, r + 1), d = r - i;
     Drafted g{-1, kNegInf, 1.f, a.uniforms[r]};
@@ -211,12 +240,12 @@ __device__ __forceinline__ void gather_drafts(const VerifyArgs& a, int i) {
 // A workgroup per sequence for gather_drafts, then one per row and slice: maximum and sum of
 // exp((l - maximum) / T) in one pass.  Where the row is a point (T = 0, or a slice that holds a NaN
 // or an infinity: the sum is NaN then), the maximum and its first index instead.
-template <int FMT>
+template <int FMT, bool TREE>
 __global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerifyArgs a) {
   constexpr int EB = FMT == kFmtF32 ? 4 : 2, PER = 16 / EB;
   constexpr int kBatch = 4;            // 16-byte words of a thread's step, the next in flight
   if (blockIdx.x < (unsigned)a.num_seqs) {
-    gather_drafts<FMT>(a, (int)blockIdx.x);
+    gather_drafts<FMT, TREE>(a, (int)blockIdx.x);
     return;
   }
   const unsigned unit = blockIdx.x - (unsigned)a.num_seqs;
@@ -520,9 +549,145 @@ __device__ __forceinline__ void load_eight(const void* row, int v0, int b1, floa
   for (int u = 0; u < kRun; ++u) l[u] = v0 + u < b1 ? elem<FMT>(row, v0 + u) : kNegInf;
 }
 
+// The tokens of a tree's children at node `at`, one bit each over entries b0 .. b1 - 1 of the
+// vocabulary (all threads; `bits` holds them).
+template <int THREADS>
+__device__ __forceinline__ void child_bits(const VerifyArgs& a, int64_t first, int n, int64_t at,
+                                           int b0, int b1, uint32_t* bits) {
+  for (int w = threadIdx.x; w < (b1 - b0 + 31) / 32; w += THREADS) bits[w] = 0;
+  __syncthreads();
+  if (n > kTreeNodes) n = kTreeNodes;
+  for (int j = threadIdx.x; j < n; j += THREADS) {
+    const Drafted d = a.drafted[first + j];
+    if (__float_as_int(d.q) == at && d.x >= b0 && d.x < b1)
+      atomicOr(&bits[(d.x - b0) >> 5], 1u << ((d.x - b0) & 31));
+  }
+  __syncthreads();
+}
+// The bits of entries v0 .. v0 + 7, v0 a multiple of 8 from b0 on.
+__device__ __forceinline__ uint32_t eight_bits(const uint32_t* bits, int v0, int b0) {
+  return (bits[(v0 - b0) >> 5] >> ((v0 - b0) & 31)) & 0xffu;
+}
+
+// A workgroup per sequence: its tree walked from node 0.  Rows' statistics by groups of lanes, the
+// nodes' probabilities by threads, then one wave goes from node to node.
+template <int FMT>
+__global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyArgs a) {
+  extern __shared__ double walk_lds[];
+  const int i = blockIdx.x, t = threadIdx.x, lane = t & 63;
+  int64_t first;
+  const int rows = seq_rows(a, i, &first);
+  if (rows <= 0) {
+    if (t == 0) {
+      a.accepted[i] = 0;
+      a.info[i] = Info{0, kNothing, 0, 0, 0, 0.f};
+    }
+    return;
+  }
+  const int n = rows < kTreeNodes ? rows : kTreeNodes;
+  double* const totals = walk_lds;                        // [n] each
+  double* const chance = totals + n;                      // of a node where it hangs
+  float* const tops = reinterpret_cast<float*>(chance + n);
+  int* const args = reinterpret_cast<int*>(tops + n);
+  int* const up = args + n;
+  int* const token = up + n;
+  float* const us = reinterpret_cast<float*>(token + n);
+  int* const trail = reinterpret_cast<int*>(us + n);      // the path
+  static_assert(2 * sizeof(double) + 6 * 4 == kNodeBytes, "per node");
+  __shared__ double table[64];
+  __shared__ int steps, last_kids;
+  const float temp = temperature_of(a, i);
+  const float k = rate_of(temp);
+  const Exp ex = make_exp(table, temp);
+  int width = 1;                       // lanes that a row's slices take
+  while (width < a.slices) width <<= 1;
+  const int gs = kWalkThreads / width, g = t / width;
+  RowPart next = load_part(a, first + (g < n ? g : 0), t & (width - 1));
+  for (int j = g; j < n; j += gs) {
+    const RowPart part = next;
+    next = load_part(a, first + (j + gs < n ? j + gs : j), t & (width - 1));
+    const RowStats f = row_stats(part, width, k);
+    if ((t & (width - 1)) == 0) {
+      tops[j] = f.top;
+      args[j] = f.arg;
+      totals[j] = f.sum;
+    }
+  }
+  for (int j = t; j < n; j += kWalkThreads) {
+    const Drafted d = a.drafted[first + j];
+    up[j] = __float_as_int(d.q);
+    token[j] = d.x;
+    us[j] = a.uniforms[first + j];
+    trail[j] = -1;
+    chance[j] = (double)d.l;           // its logit for now
+  }
+  __syncthreads();
+  for (int j = t; j < n; j += kWalkThreads) {
+    const int p = up[j], x = token[j];
+    double c = 0.0;
+    if (p >= 0 && x >= 0)
+      c = temp > 0.f && finite(tops[p]) ? ex((float)chance[j], tops[p]) / totals[p]
+                                        : (x == args[p] ? 1.0 : 0.0);
+    chance[j] = c;
+  }
+  __syncthreads();
+  if (t < 64) {
+    int at = 0, acc = 0, kids = 0;
+    for (;;) {
+      if (lane == 0) trail[acc] = at;
+      double upto = 0.0;
+      const double u = (double)us[at];
+      int to = -1;
+      kids = 0;
+      for (int base = at + 1; base < n && to < 0; base += 64) {
+        const int j = base + lane;
+        uint64_t mine = __builtin_amdgcn_ballot_w64(j < n && up[j < n ? j : 0] == at &&
+                                                    token[j < n ? j : 0] >= 0);
+        kids |= mine != 0;
+        for (; mine && to < 0; mine &= mine - 1) {
+          const int c = base + __builtin_ctzll(mine), x = token[c];
+          bool again = false;          // an earlier sibling has the token
+          for (int b = at + 1; b < c && !again; b += 64) {
+            const int o = b + lane < c ? b + lane : c;
+            again = __builtin_amdgcn_ballot_w64(o < c && up[o] == at && token[o] == x) != 0;
+          }
+          if (again) continue;
+          upto += chance[c];
+          if (u < upto) to = c;
+        }
+      }
+      if (to < 0) break;
+      at = to;
+      ++acc;
+    }
+    if (lane == 0) {
+      steps = acc;
+      last_kids = kids;
+    }
+  }
+  __syncthreads();
+  const int acc = steps;
+  for (int j = t; j < rows; j += kWalkThreads) {
+    const int node = j < n ? trail[j] : -1;
+    a.path[first + j] = node;
+    if (j != acc) put_token(a, first + j, j < acc ? draft_at(a, first + trail[j + 1]) : -1);
+  }
+  if (t != 0) return;
+  a.accepted[i] = acc;
+  const int at = trail[acc];
+  Info f;
+  f.accepted = acc;
+  f.row = first + at;
+  f.draft_row = at;
+  f.top = tops[at];
+  f.token = args[at];
+  f.kind = !(temp > 0.f) || !finite(f.top) ? kPoint : last_kids ? kBut : kAll;
+  a.info[i] = f;
+}
+
 // Workgroup (slice, sequence): the sequence's accepted drafts and chosen row, then the sum of its
 // slice of that row's weights.  Slice 0 writes what the later launches read.
-template <int FMT>
+template <int FMT, bool TREE>
 __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs a) {
   const int i = blockIdx.y, s = blockIdx.x, t = threadIdx.x, lane = t & 63;
   const int wv = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -531,6 +696,7 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs a) {
   const float temp = temperature_of(a, i);
   const float k = rate_of(temp);
   __shared__ double table[64];
+  __shared__ uint32_t bits[TREE ? kPickLen / 32 : 1];
   __shared__ int reject;
   __shared__ double sums[kThreads / 64];
   __shared__ float tops[kAccept];
@@ -539,73 +705,81 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs a) {
   const Exp ex = make_exp(table, temp);
   int width = 1;                       // lanes that a row's slices take
   while (width < a.slices) width <<= 1;
-  __syncthreads();
-  if (n <= 0) {
-    if (s == 0 && t == 0) {
-      a.accepted[i] = 0;
-      a.info[i] = Info{0, kNothing, 0, 0, 0, 0.f};
-    }
-    return;
-  }
-  // kAccept rows at a time: their statistics by waves, the drafts' own entries by threads.  The
-  // last row (or the first rejected) ends it, its statistics still there.
-  int acc = 0, j0 = 0;
-  for (;; j0 += kAccept) {
-    const int m = n - j0 < kAccept ? n - j0 : kAccept;
-    const bool draft = t < m && j0 + t < n - 1;
-    const int g = t / width, gs = kThreads / width;
-    const Drafted d = a.drafted[first + j0 + (t < m ? t : 0)];
-    RowPart next = load_part(a, first + j0 + (g < m ? g : 0), t & (width - 1));
-    for (int j = g; j < m; j += gs) {
-      const RowPart part = next;
-      next = load_part(a, first + j0 + (j + gs < m ? j + gs : j), t & (width - 1));
-      const RowStats f = row_stats(part, width, k);
-      if ((t & (width - 1)) == 0) {
-        tops[j] = f.top;
-        args[j] = f.arg;
-        totals[j] = f.sum;
-      }
-    }
-    __syncthreads();
-    if (t < m) {
-      drafts[t] = d.x;
-      bool ok = false;
-      if (draft && d.x >= 0) {
-        const double uq = (double)d.u * (double)d.q;
-        ok = temp > 0.f && finite(tops[t]) ? uq * totals[t] < ex(d.l, tops[t])
-                                           : uq < (d.x == args[t] ? 1.0 : 0.0);
-      }
-      // the first row that is not accepted (the last has nothing to accept): t < m <= 64
-      const uint64_t no = __builtin_amdgcn_ballot_w64(!ok);
-      if (t == 0) reject = no ? j0 + __builtin_ctzll(no) : n;
-    }
-    __syncthreads();
-    acc = reject;
-    if (acc < n) break;
-    __syncthreads();
-  }
-  const int64_t r = first + acc;
   Info f;
-  f.accepted = acc;
-  f.row = r;
-  f.draft_row = r - i;
-  f.top = tops[acc - j0];
-  f.token = args[acc - j0];
-  if (!(temp > 0.f) || !finite(f.top)) {
-    f.kind = kPoint;
-  } else if (acc == n - 1) {
-    f.kind = kAll;
-  } else if (a.probs) {
-    f.kind = f.draft_row >= 0 && f.draft_row < a.probs_rows ? kLeft : kAll;
+  if constexpr (TREE) {
+    __syncthreads();
+    f = a.info[i];
+    if (n <= 0 || f.kind == kNothing) return;
   } else {
-    f.kind = kBut;
-    f.token = drafts[acc - j0];
+    __syncthreads();
+    if (n <= 0) {
+      if (s == 0 && t == 0) {
+        a.accepted[i] = 0;
+        a.info[i] = Info{0, kNothing, 0, 0, 0, 0.f};
+      }
+      return;
+    }
+    // kAccept rows at a time: their statistics by waves, the drafts' own entries by threads.  The
+    // last row (or the first rejected) ends it, its statistics still there.
+    int acc = 0, j0 = 0;
+    for (;; j0 += kAccept) {
+      const int m = n - j0 < kAccept ? n - j0 : kAccept;
+      const bool draft = t < m && j0 + t < n - 1;
+      const int g = t / width, gs = kThreads / width;
+      const Drafted d = a.drafted[first + j0 + (t < m ? t : 0)];
+      RowPart next = load_part(a, first + j0 + (g < m ? g : 0), t & (width - 1));
+      for (int j = g; j < m; j += gs) {
+        const RowPart part = next;
+        next = load_part(a, first + j0 + (j + gs < m ? j + gs : j), t & (width - 1));
+        const RowStats f = row_stats(part, width, k);
+        if ((t & (width - 1)) == 0) {
+          tops[j] = f.top;
+          args[j] = f.arg;
+          totals[j] = f.sum;
+        }
+      }
+      __syncthreads();
+      if (t < m) {
+        drafts[t] = d.x;
+        bool ok = false;
+        if (draft && d.x >= 0) {
+          const double uq = (double)d.u * (double)d.q;
+          ok = temp > 0.f && finite(tops[t]) ? uq * totals[t] < ex(d.l, tops[t])
+                                             : uq < (d.x == args[t] ? 1.0 : 0.0);
+        }
+        // the first row that is not accepted (the last has nothing to accept): t < m <= 64
+        const uint64_t no = __builtin_amdgcn_ballot_w64(!ok);
+        if (t == 0) reject = no ? j0 + __builtin_ctzll(no) : n;
+      }
+      __syncthreads();
+      acc = reject;
+      if (acc < n) break;
+      __syncthreads();
+    }
+    const int64_t r = first + acc;
+    f.accepted = acc;
+    f.row = r;
+    f.draft_row = r - i;
+    f.top = tops[acc - j0];
+    f.token = args[acc - j0];
+    if (!(temp > 0.f) || !finite(f.top)) {
+      f.kind = kPoint;
+    } else if (acc == n - 1) {
+      f.kind = kAll;
+    } else if (a.probs) {
+      f.kind = f.draft_row >= 0 && f.draft_row < a.probs_rows ? kLeft : kAll;
+    } else {
+      f.kind = kBut;
+      f.token = drafts[acc - j0];
+    }
+    if (s == 0 && t == 0) a.info[i] = f;
   }
-  if (s == 0 && t == 0) a.info[i] = f;
   if (f.kind == kPoint) return;
-  const void* const row = row_at<FMT>(a, r);
+  const void* const row = row_at<FMT>(a, f.row);
   const int b0 = s * a.sum_len, b1 = b0 + a.sum_len < a.vocab ? b0 + a.sum_len : a.vocab;
-  const int but = f.kind == kBut ? f.token : -1;
+  const int but = !TREE && f.kind == kBut ? f.token : -1;
+  if (TREE && f.kind == kBut)
+    child_bits<kThreads>(a, first, n, f.draft_row, b0, b1, bits);
   double z = 0.0;
   for (int v0 = b0 + t * kRun; v0 < b1; v0 += kSumSlice) {
     float l[kRun];
@@ -613,6 +787,12 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs a) {
 #pragma unroll
     for (int u = 0; u < kRun; ++u)
       if (v0 + u == but) l[u] = kNegInf;      // no weight
+    if (TREE && f.kind == kBut) {
+      const uint32_t kids = eight_bits(bits, v0, b0);
+#pragma unroll
+      for (int u = 0; u < kRun; ++u)
+        if ((kids >> u) & 1u) l[u] = kNegInf;
+    }
 #pragma unroll
     for (int u = 0; u < kRun; ++u) z += ex(l[u], f.top);
   }
@@ -676,7 +856,7 @@ __device__ __forceinline__ double wave_prefix(double v, int lane) {
 
 // Workgroup per sequence: its tokens.  The slice whose prefix passes the goal; then the thread
 // (each takes a run of the slice), then the entry.
-template <int FMT>
+template <int FMT, bool TREE>
 __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(VerifyArgs a) {
   const int i = blockIdx.x, t = threadIdx.x, lane = t & 63, wv = t >> 6;
   int64_t first;
@@ -687,15 +867,21 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(VerifyArgs a)
   if (n <= 0) return;
   const Info f = a.info[i];
   if (f.accepted >= n) return;     // cu has changed since the launches before
-  for (int j = t; j < n; j += kPickThreads)
-    if (j != f.accepted) put_token(a, first + j, j < f.accepted ? draft_at(a, first + j + 1) : -1);
-  if (t == 0) a.accepted[i] = f.accepted;
+  if constexpr (TREE) {
+    if (f.kind == kNothing) return;
+  } else {
+    for (int j = t; j < n; j += kPickThreads)
+      if (j != f.accepted)
+        put_token(a, first + j, j < f.accepted ? draft_at(a, first + j + 1) : -1);
+    if (t == 0) a.accepted[i] = f.accepted;
+  }
   const int64_t to = first + f.accepted;
   if (f.kind == kPoint) {
     if (t == 0) put_token(a, to, f.token);
     return;
   }
   __shared__ double table[64];
+  __shared__ uint32_t bits[TREE ? kPickLen / 32 : 1];
   __shared__ double wsum[kPickThreads / 64];
   __shared__ int cross[kPickThreads / 64], last[kPickThreads / 64];
   const Exp ex = make_exp(table, temperature_of(a, i));
@@ -704,7 +890,29 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(VerifyArgs a)
   const bool left = rest > 0.0;        // else q covers p everywhere: p itself
   const double total = left ? rest : whole;
   if (!(total > 0.0)) {   // nothing but the rejected draft has weight
-    if (t == 0) put_token(a, to, f.token < 0 ? 0 : f.token);
+    if constexpr (TREE) {                // but its children: the likeliest, the row's argmax
+      float l = kNegInf;
+      int x = 0x7fffffff;
+      for (int j = t; t < 64 && j < n && j < kTreeNodes; j += 64) {
+        const Drafted d = a.drafted[first + j];
+        if (__float_as_int(d.q) == f.draft_row && d.x >= 0 && better(d.l, d.x, l, x)) {
+          l = d.l;
+          x = d.x;
+        }
+      }
+#pragma unroll
+      for (int m = 32; m >= 1; m >>= 1) {
+        const float ol = __shfl_xor(l, m, 64);
+        const int ox = __shfl_xor(x, m, 64);
+        if (better(ol, ox, l, x)) {
+          l = ol;
+          x = ox;
+        }
+      }
+      if (t == 0) put_token(a, to, x == 0x7fffffff ? 0 : x);
+    } else {
+      if (t == 0) put_token(a, to, f.token < 0 ? 0 : f.token);
+    }
     return;
   }
   const float u0 = a.uniforms[first + n - 1];
@@ -728,11 +936,16 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(VerifyArgs a)
   if (left) load_eight<kFmtF32>(q, v0, b1, d);
   double run[kRun], mine = 0.0;
   __syncthreads();
+  uint32_t kids = 0;
+  if (TREE && f.kind == kBut) {
+    child_bits<kPickThreads>(a, first, n, f.draft_row, b0, b1, bits);
+    kids = v0 < b1 ? eight_bits(bits, v0, b0) : 0u;
+  }
 #pragma unroll
   for (int e = 0; e < kRun; ++e) {
     run[e] = ex(l[e], f.top);
     if (left) run[e] = positive(run[e] * scale - positive((double)d[e]));
-    if (f.kind == kBut && v0 + e == f.token) run[e] = 0.0;
+    if (TREE ? (kids >> e) & 1u : f.kind == kBut && v0 + e == f.token) run[e] = 0.0;
     mine += run[e];
   }
   // prefix over the threads
@@ -799,15 +1012,29 @@ Sizes sizes_of(int64_t rows, int num_seqs, int vocab) {
   return z;
 }
 
-template <int FMT>
+template <int FMT, bool TREE = false>
 int launch_verify(const VerifyArgs& a, hipStream_t s) {
   const dim3 wg(kThreads);
   const unsigned seqs = (unsigned)a.num_seqs;
-  hipLaunchKernelGGL((verify_stats_kernel<FMT>),
+  hipLaunchKernelGGL((verify_stats_kernel<FMT, TREE>),
                      dim3((unsigned)(a.num_seqs + a.rows * a.slices)), wg, 0, s, a);
   int rc = check_launch();
   if (rc != NDL_OK) return rc;
-  hipLaunchKernelGGL((verify_sums_kernel<FMT>), dim3((unsigned)a.sum_slices, seqs), wg, 0, s, a);
+  if constexpr (TREE) {
+    const int lds = (int)(a.rows < kTreeNodes ? a.rows : kTreeNodes) * kNodeBytes;
+    VerifyArgs args = a;
+    void* params[] = {&args};
+    if (hipLaunchKernel((const void*)verify_walk_kernel<FMT>, dim3(seqs), dim3(kWalkThreads), params,
+                        lds, s) !=
+        hipSuccess) {
+      (void)hipGetLastError();
+      return NDL_ERR_LAUNCH;
+    }
+    rc = check_launch();
+    if (rc != NDL_OK) return rc;
+  }
+  hipLaunchKernelGGL((verify_sums_kernel<FMT, TREE>), dim3((unsigned)a.sum_slices, seqs), wg, 0, s,
+                     a);
   rc = check_launch();
   if (rc != NDL_OK) return rc;
   if (a.probs != nullptr && a.probs_rows > 0) {
@@ -816,8 +1043,26 @@ int launch_verify(const VerifyArgs& a, hipStream_t s) {
     rc = check_launch();
     if (rc != NDL_OK) return rc;
   }
-  hipLaunchKernelGGL((verify_pick_kernel<FMT>), dim3(seqs), dim3(kPickThreads), 0, s, a);
+  hipLaunchKernelGGL((verify_pick_kernel<FMT, TREE>), dim3(seqs), dim3(kPickThreads), 0, s, a);
   return check_launch();
+}
+
+// The parts of the workspace and the slices of a call's rows.
+void lay_out(VerifyArgs* a, const Sizes& z, void* workspace) {
+  a->slices = z.slices;
+  a->slice_len = (a->vocab + z.slices - 1) / z.slices;
+  a->slice_len = (a->slice_len + 7) / 8 * 8;
+  a->sum_slices = z.sum_slices;
+  a->sum_len = z.sum_len;
+  char* w = (char*)workspace;
+  a->part_max = (float*)w;
+  a->part_arg = (int*)(w + z.stat);
+  a->part_sum = (float*)(w + 2 * z.stat);
+  w += 3 * z.stat;
+  a->drafted = (Drafted*)w;
+  a->info = (Info*)(w + z.drafted);
+  a->sums = (double*)(w + z.drafted + z.info);
+  a->left = (double*)(w + z.drafted + z.info + z.sums);
 }
 
 }  // namespace
@@ -868,21 +1113,55 @@ extern "C" int ndl_verify_drafts(void* tokens, int32_t* accepted, const void* lo
   a.rows = num_rows;
   a.num_seqs = num_seqs;
   a.vocab = vocab;
-  a.slices = z.slices;
-  a.slice_len = (vocab + z.slices - 1) / z.slices;
-  a.slice_len = (a.slice_len + 7) / 8 * 8;
-  a.sum_slices = z.sum_slices;
-  a.sum_len = z.sum_len;
-  char* w = (char*)workspace;
-  a.part_max = (float*)w;
-  a.part_arg = (int*)(w + z.stat);
-  a.part_sum = (float*)(w + 2 * z.stat);
-  w += 3 * z.stat;
-  a.drafted = (Drafted*)w;
-  a.info = (Info*)(w + z.drafted);
-  a.sums = (double*)(w + z.drafted + z.info);
-  a.left = (double*)(w + z.drafted + z.info + z.sums);
+  lay_out(&a, z, workspace);
   const hipStream_t s = (hipStream_t)stream;
   if (dtype_is_f32(dtype)) return launch_verify<kFmtF32>(a, s);
   return dtype_is_f16(dtype) ? launch_verify<kFmtF16>(a, s) : launch_verify<kFmtBF16>(a, s);
+}
+
+extern "C" size_t ndl_verify_tree_workspace_bytes(int64_t num_rows, int num_seqs, int vocab) {
+  return ndl_verify_drafts_workspace_bytes(num_rows, num_seqs, vocab);
+}
+
+extern "C" int ndl_verify_tree(void* tokens, int32_t* accepted, int32_t* path, const void* logits,
+                               int64_t row_stride, int dtype, const void* ids, int ids_are_int64,
+                               const int32_t* parents, const int32_t* cu_seqlens,
+                               const float* uniforms, const float* temperature, int64_t num_rows,
+                               int num_seqs, int vocab, void* workspace, size_t workspace_bytes,
+                               ndl_stream_t stream) {
+  using namespace ndl;
+  if (!dtype_known(dtype)) return NDL_ERR_UNSUPPORTED;
+  if (num_rows < 0 || num_seqs < 0 || vocab <= 0) return NDL_ERR_INVALID_ARG;
+  if (num_seqs == 0) return NDL_OK;
+  if (num_rows == 0) return NDL_ERR_INVALID_ARG;   // every sequence has a row
+  if (!tokens || !accepted || !path || !logits || !ids || !parents || !cu_seqlens || !uniforms ||
+      row_stride < vocab)
+    return NDL_ERR_INVALID_ARG;
+  if ((uintptr_t)logits % dtype_bytes(dtype) || (uintptr_t)uniforms & 3u)
+    return NDL_ERR_INVALID_ARG;
+  if (num_rows > 65535 || num_seqs > 65535 || vocab > kMaxVocab)
+    return NDL_ERR_UNSUPPORTED;
+  const Sizes z = sizes_of(num_rows, num_seqs, vocab);
+  if (!workspace || workspace_bytes < z.total || (uintptr_t)workspace & 255u)
+    return NDL_ERR_WORKSPACE;
+  VerifyArgs a{};
+  a.logits = logits;
+  a.stride = row_stride;
+  a.ids = ids;
+  a.ids64 = ids_are_int64 ? 1 : 0;
+  a.cu = cu_seqlens;
+  a.uniforms = uniforms;
+  a.temperature = temperature;
+  a.tokens = tokens;
+  a.accepted = accepted;
+  a.rows = num_rows;
+  a.num_seqs = num_seqs;
+  a.vocab = vocab;
+  a.parents = parents;
+  a.path = path;
+  lay_out(&a, z, workspace);
+  const hipStream_t s = (hipStream_t)stream;
+  if (dtype_is_f32(dtype)) return launch_verify<kFmtF32, true>(a, s);
+  return dtype_is_f16(dtype) ? launch_verify<kFmtF16, true>(a, s)
+                             : launch_verify<kFmtBF16, true>(a, s);
 }

@@ -1077,6 +1077,41 @@ def varlen_prefill_fp8(q: torch.Tensor, kv_codes: torch.Tensor, kv_scales: torch
                           scale, num_heads, num_kv_heads, head_dim, out, workspace)
 
 
+def _check_f32(name, t, shape, dev):
+    if t.dtype != torch.float32:
+        raise TypeError(f"{name} must be float32, got {t.dtype}")
+    if t.shape != shape or t.device != dev or (t.numel() and t.stride(-1) != 1
+                                               and shape[-1] != 1):
+        raise ValueError(f"{name} must be {list(shape)} with contiguous rows on {dev}, got "
+                         f"{tuple(t.shape)}")
+
+
+def _check_verify(logits, ids, cu_seqlens, uniforms, temperature):
+    """(device, rows, vocab, sequences) of a verification's rows."""
+    _require(logits.is_cuda, "logits must be a GPU tensor")
+    if logits.dtype not in _DTYPES:
+        raise TypeError(f"unsupported dtype {logits.dtype}")
+    if logits.dim() != 2:
+        raise ValueError(f"logits must be [rows, vocab], got {tuple(logits.shape)}")
+    rows, vocab = logits.shape
+    dev = logits.device
+    _require(vocab > 0, "logits have no columns")
+    _require(logits.stride(1) == 1 or vocab == 1, "logits rows must be contiguous")
+    _require(rows <= 1 or logits.stride(0) >= vocab, "logits rows overlap")
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"ids must be int32 or int64, got {ids.dtype}")
+    if ids.shape != (rows,) or not ids.is_contiguous() or ids.device != dev:
+        raise ValueError(f"ids must be a contiguous [{rows}] tensor on {dev}")
+    _check_int32("cu_seqlens", cu_seqlens, 1, dev)
+    n_seqs = cu_seqlens.shape[0] - 1
+    _require(n_seqs >= 0, "cu_seqlens must be [num_seqs + 1]")
+    _require(rows >= n_seqs, f"every sequence has a row: {rows} rows, {n_seqs} sequences")
+    _check_f32("uniforms", uniforms, (rows,), dev)
+    if temperature is not None:
+        _check_f32("temperature", temperature, (n_seqs,), dev)
+    return dev, rows, vocab, n_seqs
+
+
 def verify_drafts(logits: torch.Tensor, ids: torch.Tensor, cu_seqlens: torch.Tensor,
                   uniforms: torch.Tensor, *, temperature: Optional[torch.Tensor] = None,
                   draft_probs: Optional[torch.Tensor] = None):
@@ -1101,39 +1136,10 @@ def verify_drafts(logits: torch.Tensor, ids: torch.Tensor, cu_seqlens: torch.Ten
                                          draft_probs)
         if done is not None:
             return done
-    _require(logits.is_cuda, "logits must be a GPU tensor")
-    if logits.dtype not in _DTYPES:
-        raise TypeError(f"unsupported dtype {logits.dtype}")
-    if logits.dim() != 2:
-        raise ValueError(f"logits must be [rows, vocab], got {tuple(logits.shape)}")
-    rows, vocab = logits.shape
-    dev = logits.device
-    _require(vocab > 0, "logits have no columns")
-    _require(logits.stride(1) == 1 or vocab == 1, "logits rows must be contiguous")
-    _require(rows <= 1 or logits.stride(0) >= vocab, "logits rows overlap")
-    if ids.dtype not in (torch.int32, torch.int64):
-        raise TypeError(f"ids must be int32 or int64, got {ids.dtype}")
-    if ids.shape != (rows,) or not ids.is_contiguous() or ids.device != dev:
-        raise ValueError(f"ids must be a contiguous [{rows}] tensor on {dev}")
-    _check_int32("cu_seqlens", cu_seqlens, 1, dev)
-    n_seqs = cu_seqlens.shape[0] - 1
-    _require(n_seqs >= 0, "cu_seqlens must be [num_seqs + 1]")
-    _require(rows >= n_seqs, f"every sequence has a row: {rows} rows, {n_seqs} sequences")
-
-    def check(name, t, shape):
-        if t.dtype != torch.float32:
-            raise TypeError(f"{name} must be float32, got {t.dtype}")
-        if t.shape != shape or t.device != dev or (t.numel() and t.stride(-1) != 1
-                                                   and shape[-1] != 1):
-            raise ValueError(f"{name} must be {list(shape)} with contiguous rows on {dev}, got "
-                             f"{tuple(t.shape)}")
-
-    check("uniforms", uniforms, (rows,))
-    if temperature is not None:
-        check("temperature", temperature, (n_seqs,))
+    dev, rows, vocab, n_seqs = _check_verify(logits, ids, cu_seqlens, uniforms, temperature)
     ds = vocab
     if draft_probs is not None:
-        check("draft_probs", draft_probs, (rows - n_seqs, vocab))
+        _check_f32("draft_probs", draft_probs, (rows - n_seqs, vocab), dev)
         if rows - n_seqs > 1:
             ds = draft_probs.stride(0)
             _require(ds >= vocab, "draft_probs rows overlap")
@@ -1285,3 +1291,45 @@ def tree_attention(q: torch.Tensor, kv_cache, block_table: torch.Tensor,
             rc = lib.ndl_tree_attention(out.data_ptr(), q.data_ptr(), qs, pool.data_ptr(), *tail)
     _lib.check(rc, "ndl_fp8_tree_attention" if fp8 else "ndl_tree_attention")
     return out
+
+
+def verify_tree(logits: torch.Tensor, ids: torch.Tensor, parents: torch.Tensor,
+                cu_seqlens: torch.Tensor, uniforms: torch.Tensor, *,
+                temperature: Optional[torch.Tensor] = None):
+    """verify_drafts for drafted trees: (tokens [T], accepted int32 [num_seqs], path int32 [T]).
+
+    logits [T, vocab] (bfloat16, float16 or float32, rows contiguous, any row stride) are the
+    target's rows for the nodes ids [T] (int32 or int64) of each sequence's tree, parents int32 [T]
+    as for tree_mask; node 0 is the sequence's newest token.  From there, with
+    p = softmax(logits[r] / temperature[i]) of the node r, the path goes on to the first of its
+    children (in the order of their rows) whose token's p, added to those of the children before it,
+    is more than uniforms[r]; a token that several children have counts once.  Where there is none,
+    the next token is drawn from the node's p without its children's tokens, by the inverse of the
+    cumulative distribution at the sequence's last uniform (its last node is a leaf): together
+    distributed as the target.  A chain gives what verify_drafts gives without draft_probs.
+
+    temperature float32 [num_seqs] (None: 1); 0 takes the argmax, as does a row whose maximum is
+    not finite.  uniforms float32 [T] in [0, 1).  A sequence's rows past its 1,024th are no part of
+    its tree.  tokens, in ids' type: the path's tokens after node 0, the next token, then -1;
+    accepted: how many the path has; path: its nodes, 0 among them, then -1 (kv_compact moves their
+    rows together).  Rows outside cu_seqlens hold nothing in particular.  Graph-capturable; no host
+    synchronisation."""
+    dev, rows, vocab, n_seqs = _check_verify(logits, ids, cu_seqlens, uniforms, temperature)
+    _check_int32("parents", parents, 1, dev)
+    _require(parents.shape[0] == rows, "logits and parents differ in rows")
+    tokens, path = torch.empty_like(ids), torch.empty(rows, dtype=torch.int32, device=dev)
+    accepted = torch.empty(n_seqs, dtype=torch.int32, device=dev)
+    if n_seqs == 0:
+        return tokens, accepted, path
+    lib = _lib.load()
+    need = lib.ndl_verify_tree_workspace_bytes(rows, n_seqs, vocab)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    with _on(dev):
+        rc = lib.ndl_verify_tree(
+            tokens.data_ptr(), accepted.data_ptr(), path.data_ptr(), logits.data_ptr(),
+            logits.stride(0) if rows > 1 else vocab, _DTYPES[logits.dtype], ids.data_ptr(),
+            int(ids.dtype == torch.int64), parents.data_ptr(), cu_seqlens.data_ptr(),
+            uniforms.data_ptr(), _ptr(temperature), rows, n_seqs, vocab, ws.data_ptr(), need,
+            _stream(dev))
+    _lib.check(rc, "ndl_verify_tree")
+    return tokens, accepted, path

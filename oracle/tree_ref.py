@@ -167,10 +167,17 @@ def verify(logits, ids, parents, cu, uniforms, temperature=None):
             continue
         u = float(uniforms[b - 1])
         u = min(max(u, 0.0), 1.0) if u == u else 0.0
-        c = weights.cumsum(0)
-        hit = ((c > u * c[-1]) & (weights > 0)).nonzero()[:, 0]
-        some = (weights > 0).nonzero()[:, 0]
-        tokens[a + k] = int(hit[0]) if len(hit) else int(some[-1])
+        # sums of whole numbers: a border that u falls on exactly is kept
+        w = [int(math.ldexp(x, 200)) for x in weights.tolist()]
+        num, den = u.as_integer_ratio()
+        goal, upto, last = num * sum(w), 0, 0
+        for x, y in enumerate(w):
+            upto += y
+            if y > 0:
+                last = x
+                if upto * den > goal:
+                    break
+        tokens[a + k] = last
     return tokens, accepted, path
 
 
