@@ -719,6 +719,41 @@ int ndl_verify_tree(void* tokens, int32_t* accepted, int32_t* path, const void* 
                     const float* temperature, int64_t num_rows, int num_seqs, int vocab,
                     void* workspace, size_t workspace_bytes, ndl_stream_t stream);
 
+/*
+ * Rows of cached tokens moved together: row first[i] + j of sequence i (first NULL: j) becomes what row
+ * first[i] + keep[j] was, for j < counts[i].  keep is [num_seqs][num_kv_heads][keep_width], a list
+ * for each kv head, or, with cu_seqlens, [num_keep] packed by it, a list for all kv heads alike
+ * (ndl_verify_tree's path).  In every one of num_layers (at most 128) pools, both planes; scales: those of
+ * 8-bit pools (NULL: 16-bit or float32 ones); row_bytes: of a row of a pool (a multiple of 16); and in
+ * mass float32 [num_blocks][num_kv_heads][block_size] (NULL: none).  `pools` and `scales` are host
+ * arrays of device addresses.
+ *
+ * Without dst_table rows move in place and a list has to ascend, keep[j] >= j; with it they go to the
+ * blocks that its rows name, none of which may be one that rows are read from.  An entry below 0, a
+ * position past its table, an invalid block id, a negative first[i] and a row that stays where it is
+ * move nothing; counts past the list end with it.
+ */
+int ndl_kv_compact(void* const* pools, void* const* scales, int num_layers, float* mass,
+                   int64_t num_blocks, int num_kv_heads, int block_size, int row_bytes,
+                   const int32_t* block_table, int64_t bt_row_stride, int max_blocks_per_seq,
+                   const int32_t* dst_table, int64_t dst_row_stride, int dst_max_blocks,
+                   const int32_t* keep, int keep_width, const int32_t* cu_seqlens,
+                   int64_t num_keep, const int32_t* first, const int32_t* counts, int num_seqs,
+                   ndl_stream_t stream);
+
+/*
+ * The tokens of each kv head that stay in a cache of `budget`: kept[i] = min(lens[i], budget), and
+ * keep [num_seqs][num_kv_heads][budget] their positions, ascending, then -1.  Of a longer sequence
+ * the first `sinks`, the last `recent` (at most budget together), and of the rest those with the
+ * largest weights in mass float32 [num_blocks][num_kv_heads][block_size], of equal ones the first.
+ * A NaN counts as the largest, a position with an invalid block id as the smallest weight; lens is
+ * cut to what the table holds, and a negative one is 0.
+ */
+int ndl_kv_select(int32_t* keep, int32_t* kept, const float* mass, int64_t num_blocks,
+                  int num_kv_heads, int block_size, const int32_t* block_table,
+                  int64_t bt_row_stride, int max_blocks_per_seq, const int32_t* lens, int num_seqs,
+                  int budget, int sinks, int recent, ndl_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -62,6 +62,8 @@ EXPORTED_SYMBOLS = (
     "ndl_fp8_tree_attention",
     "ndl_verify_tree_workspace_bytes",
     "ndl_verify_tree",
+    "ndl_kv_compact",
+    "ndl_kv_select",
 )
 
 _c_i32 = ctypes.c_int
@@ -263,6 +265,18 @@ _SIGNATURES = {
         _c_p, _c_p, _c_p, _c_p, _c_i64, _c_i32,         # tokens, accepted, path, logits, stride, dtype
         _c_p, _c_i32, _c_p, _c_p, _c_p, _c_p,           # ids, int64, parents, cu, uniforms, temp.
         _c_i64, _c_i32, _c_i32, _c_p, _c_sz, _c_p,      # T, B, V, workspace, bytes, stream
+    ]),
+    "ndl_kv_compact": (_c_i32, [
+        _c_p, _c_p, _c_i32, _c_p,                       # pools, scales, layers, mass
+        _c_i64, _c_i32, _c_i32, _c_i32,                 # NB, Hkv, bs, row bytes
+        _c_p, _c_i64, _c_i32, _c_p, _c_i64, _c_i32,     # tables: stride, W
+        _c_p, _c_i32, _c_p, _c_i64,                     # keep, width, cu, entries
+        _c_p, _c_p, _c_i32, _c_p,                       # first, counts, B, stream
+    ]),
+    "ndl_kv_select": (_c_i32, [
+        _c_p, _c_p, _c_p, _c_i64, _c_i32, _c_i32,       # keep, kept, mass, NB, Hkv, bs
+        _c_p, _c_i64, _c_i32, _c_p, _c_i32,             # block_table, stride, W, lens, B
+        _c_i32, _c_i32, _c_i32, _c_p,                   # budget, sinks, recent, stream
     ]),
 }
 

@@ -1333,3 +1333,127 @@ def verify_tree(logits: torch.Tensor, ids: torch.Tensor, parents: torch.Tensor,
             _stream(dev))
     _lib.check(rc, "ndl_verify_tree")
     return tokens, accepted, path
+
+
+# ---------------------------------------------------------------- caches that keep some rows
+
+def kv_mass_pool(num_blocks: int, num_kv_heads: int, block_size: int,
+                 device=None) -> torch.Tensor:
+    """Weights of a pool's rows, float32 [num_blocks, num_kv_heads, block_size], zero: a number for
+    each cached token and kv head, found through the block table as its K and V are."""
+    return torch.zeros((num_blocks, num_kv_heads, block_size), dtype=torch.float32, device=device)
+
+
+def _check_mass(mass, nb, hkv, bs, dev) -> None:
+    if mass.dtype != torch.float32:
+        raise TypeError(f"mass must be float32, got {mass.dtype}")
+    if mass.shape != (nb, hkv, bs) or not mass.is_contiguous() or mass.device != dev:
+        raise ValueError(f"mass must be a contiguous {[nb, hkv, bs]} tensor on {dev}, got "
+                         f"{tuple(mass.shape)}")
+
+
+def kv_compact(pools, block_table: torch.Tensor, keep: torch.Tensor, counts: torch.Tensor, *,
+               first: Optional[torch.Tensor] = None,
+               cu_seqlens: Optional[torch.Tensor] = None,
+               dst_table: Optional[torch.Tensor] = None,
+               mass: Optional[torch.Tensor] = None) -> None:
+    """Move the cached rows that stay together, in every layer's pool, both planes, in one launch:
+    row first[i] + j of sequence i (first None: j) becomes what row first[i] + keep[j] was, for
+    j < counts[i].
+
+    pools: a list of [2, NB, Hkv, bs, D] tensors, or of Fp8KVCache, up to 128 of one shape and type.
+    keep int32: [num_seqs, Hkv, K], a list for each kv head (kv_select's), or, with cu_seqlens
+    (int32 [num_seqs + 1]), [T], packed, a list for all kv heads alike: verify_tree's path, with
+    first the tokens cached before the tree and counts = accepted + 1.  counts, first int32
+    [num_seqs].  mass (kv_mass_pool): weights that move with the rows.
+
+    Without dst_table the rows move in place; a list has to ascend, with keep[j] >= j.  With
+    dst_table (int32 [num_seqs, columns]) they go to its blocks, none of which may hold rows that are
+    read.  Negative entries, positions past a table and invalid block ids move nothing."""
+    import ctypes
+    pools = list(pools)
+    _require(len(pools) > 0, "no pools given")
+    fp8 = isinstance(pools[0], Fp8KVCache)
+    _require(all(isinstance(p, Fp8KVCache) == fp8 for p in pools),
+             "16-bit and 8-bit pools cannot be mixed", TypeError)
+    main = [p.codes if fp8 else p for p in pools]
+    shape, dtype, dev = main[0].shape, main[0].dtype, main[0].device
+    for p, x in zip(pools, main):
+        _check_fp8_cache(*p) if fp8 else _check_cache(p)
+        _require(x.shape == shape and x.device == dev, "pools must share one shape and GPU")
+        _require(x.dtype == dtype or fp8, "pools must share one dtype", TypeError)
+    _, nb, hkv, bs, d = shape
+    row_bytes = d * main[0].element_size()
+    _require(row_bytes % 16 == 0, f"rows of {row_bytes} bytes are not whole 16-byte pieces")
+    _require(len(pools) <= 128, f"at most 128 pools a call, got {len(pools)}")
+    n_seqs = _check_table(block_table, nb, dev)
+    _check_int32("counts", counts, 1, dev)
+    _require(counts.shape[0] == n_seqs, "counts/block_table batch mismatch")
+    if first is not None:
+        _check_int32("first", first, 1, dev)
+        _require(first.shape[0] == n_seqs, "first/block_table batch mismatch")
+    if cu_seqlens is None:
+        _check_int32("keep", keep, 3, dev)
+        _require(tuple(keep.shape[:2]) == (n_seqs, hkv) and keep.is_contiguous(),
+                 f"keep must be a contiguous [{n_seqs}, {hkv}, K] tensor (or packed by cu_seqlens)")
+    else:
+        _check_int32("keep", keep, 1, dev)
+        _check_int32("cu_seqlens", cu_seqlens, 1, dev)
+        _require(cu_seqlens.shape[0] == n_seqs + 1, "cu_seqlens must be [num_seqs + 1]")
+    if dst_table is not None:
+        _require(_check_table(dst_table, nb, dev) == n_seqs, "dst_table/block_table batch mismatch")
+    if mass is not None:
+        _check_mass(mass, nb, hkv, bs, dev)
+    if n_seqs == 0 or keep.numel() == 0:
+        return
+    _require(block_table.shape[1] > 0 and (dst_table is None or dst_table.shape[1] > 0),
+             "a block table has no columns")
+    arr = ctypes.c_void_p * len(pools)
+    dst = (None, 0, 0) if dst_table is None else (dst_table.data_ptr(), dst_table.stride(0),
+                                                  dst_table.shape[1])
+    with _on(dev):
+        rc = _lib.load().ndl_kv_compact(
+            arr(*[x.data_ptr() for x in main]),
+            arr(*[p.scales.data_ptr() for p in pools]) if fp8 else None, len(pools), _ptr(mass),
+            nb, hkv, bs, row_bytes, block_table.data_ptr(), block_table.stride(0),
+            block_table.shape[1], *dst, keep.data_ptr(),
+            keep.shape[2] if cu_seqlens is None else 0, _ptr(cu_seqlens), keep.numel(),
+            _ptr(first), counts.data_ptr(), n_seqs, _stream(dev))
+    _lib.check(rc, "ndl_kv_compact")
+
+
+def kv_select(mass: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor, budget: int, *,
+              sinks: int = 0, recent: int = 0):
+    """The tokens of each kv head that stay when a cache is cut to `budget`: (keep int32
+    [num_seqs, Hkv, budget], their positions, ascending, then -1; kept int32 [num_seqs] =
+    min(lens, budget)), for kv_compact.
+
+    mass (kv_mass_pool): the weights, as attention_mass adds them up; lens int32 [num_seqs]: the cached
+    tokens.  Of a sequence of more than budget tokens the first `sinks` and the last `recent` stay
+    (at most budget together), and of those between the ones with the largest weights, of equal ones
+    the first.  A NaN counts as the largest weight."""
+    if mass.dim() != 3:
+        raise ValueError(f"mass must be [num_blocks, num_kv_heads, block_size], got "
+                         f"{tuple(mass.shape)}")
+    _require(mass.is_cuda, "mass must be a GPU tensor")
+    nb, hkv, bs = mass.shape
+    dev = mass.device
+    _check_mass(mass, nb, hkv, bs, dev)
+    n_seqs = _check_table(block_table, nb, dev)
+    _check_int32("lens", lens, 1, dev)
+    _require(lens.shape[0] == n_seqs, "lens/block_table batch mismatch")
+    _require(budget > 0, "budget must be positive")
+    _require(sinks >= 0 and recent >= 0 and sinks + recent <= budget,
+             f"sinks {sinks} and recent {recent} must be within the budget {budget}")
+    keep = torch.empty((n_seqs, hkv, budget), dtype=torch.int32, device=dev)
+    kept = torch.empty(n_seqs, dtype=torch.int32, device=dev)
+    if n_seqs == 0:
+        return keep, kept
+    _require(block_table.shape[1] > 0, "block_table has no columns")
+    with _on(dev):
+        rc = _lib.load().ndl_kv_select(
+            keep.data_ptr(), kept.data_ptr(), mass.data_ptr(), nb, hkv, bs, block_table.data_ptr(),
+            block_table.stride(0), block_table.shape[1], lens.data_ptr(), n_seqs, budget, sinks,
+            recent, _stream(dev))
+    _lib.check(rc, "ndl_kv_select")
+    return keep, kept
