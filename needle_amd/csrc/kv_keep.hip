@@ -11,15 +11,16 @@ namespace {
 // ---------------------------------------------------------------- rows moved together
 //
 // Row first + j of a sequence <- row first + keep[j], j < count: of one kv head, or of all alike.
-// Bound: the rows, read and written once, and the trips before them (index, block id, row: three, the
-// index and the block ids of the next rows under way while these move).
-//   * A row is whole 16-byte pieces, a lane each (a scale byte or a weight: a lane a row).
+// Bound: the rows, read and written once, and the trips before them (length, index, block ids).
+//   * A lane finds a row's source and place, for up to 64 rows of a wave's step and for several planes
+//     (layers, K and V); then the wave's lanes take 16-byte pieces of those rows, up to 16 loads under
+//     way, and the next step's rows are found meanwhile.  (A scale byte or a weight: a lane a row.)
 //   * In place the indices ascend, so a row's source is never written before it is read: a later row
-//     has a later source and a later place.  One wave (short lists) or one workgroup (long ones, a
-//     barrier between the reads of a step and its writes) takes a list from front to back.
+//     has a later source and a later place.  One wave (short lists) or the 16 of a workgroup (long
+//     ones, a barrier between the reads of a step and its writes) take a list from front to back.
 //   * Into other blocks nothing is ordered, and lists are cut into as many pieces as fill the GPU.
 constexpr int kMaxPools = 128;
-constexpr int kItems = 4;         // pieces of a lane under way
+constexpr int kLoads = 16;        // of a lane under way
 
 struct MoveArgs {
   char* pool[kMaxPools];
@@ -41,12 +42,14 @@ struct MoveArgs {
   const int32_t* first;           // or null: 0
   const int32_t* counts;
   int num_seqs;
+  int pieces, pieces_shift;       // of a row; their log2, or -1
+  int planes_each;                // planes of the pools that a workgroup takes
 };
 
-// Positions and blocks of row j of a list: byte offsets of its source and its place, -1 where there
-// is none (nothing to do for row j).
+// Source and place of row j of a list, as rows of a plane; kNone where there is nothing to do.
+constexpr uint32_t kNone = ~0u;
 struct Move {
-  int64_t from, to;
+  uint32_t from, to;
 };
 
 struct List {
@@ -73,97 +76,124 @@ __device__ __forceinline__ List list_of(const MoveArgs& a, int seq, int head) {
   l.to = a.to + seq * a.to_stride;
   return l;
 }
-__device__ __forceinline__ Move move_of(const MoveArgs& a, const List& l, int j, int head,
-                                        int row_bytes) {
-  Move m{-1, -1};
-  if (j >= l.n) return m;
+__device__ __forceinline__ Move move_of(const MoveArgs& a, const List& l, int j, int head) {
+  const Move none{kNone, kNone};
+  if (j >= l.n) return none;
   const int k = l.keep[j];
   const int64_t s = l.base + k, d = l.base + j;
   if (k < 0 || s >= (int64_t)a.table_cols * a.block_size ||
       d >= (int64_t)a.to_cols * a.block_size)
-    return m;
-  const uint32_t bs = (uint32_t)a.block_size;
+    return none;
+  const uint32_t bs = (uint32_t)a.block_size, hkv = (uint32_t)a.num_kv_heads;
   const uint32_t sc = (uint32_t)s / bs, dc = (uint32_t)d / bs;
   const int sb = l.table[sc], db = l.to[dc];
-  if (sb < 0 || sb >= a.num_blocks || db < 0 || db >= a.num_blocks) return m;
-  const int64_t from =
-      (((int64_t)sb * a.num_kv_heads + head) * bs + ((uint32_t)s - sc * bs)) * row_bytes;
-  const int64_t to =
-      (((int64_t)db * a.num_kv_heads + head) * bs + ((uint32_t)d - dc * bs)) * row_bytes;
-  if (from == to) return m;
-  return Move{from, to};
+  if (sb < 0 || sb >= a.num_blocks || db < 0 || db >= a.num_blocks) return none;
+  const Move m{((uint32_t)sb * hkv + (uint32_t)head) * bs + ((uint32_t)s - sc * bs),
+               ((uint32_t)db * hkv + (uint32_t)head) * bs + ((uint32_t)d - dc * bs)};
+  return m.from == m.to ? none : m;
 }
 
-// THREADS threads take the rows j0 .. j1 - 1 of a list, WORD bytes a piece.
-template <int THREADS, bool IN_PLACE, class WORD>
-__device__ __forceinline__ void move_rows(const MoveArgs& a, const List& l, char* plane, int head,
-                                          int row_bytes, int t, int j0, int j1) {
-  const int pieces = row_bytes / (int)sizeof(WORD);      // of a row
-  const int total = (j1 - j0) * pieces;                  // fits: the entry point checks
-  auto slots = [&](int i0, Move* m) {
+// A wave's rows j0, j0 + WAVES * per, .. of a list, `per` at a time.  A list in place is whole: every
+// read of a step before its writes, within a wave by their order (a place written here is before the
+// sources still on their way), across waves by a wait and a barrier.
+template <int WAVES, bool IN_PLACE>
+__device__ __forceinline__ void move_rows(const MoveArgs& a, const List& l, int head, int plane0,
+                                          int plane1, int lane, int wave, int j0, int j1) {
+  const int64_t plane_bytes = a.num_blocks * a.num_kv_heads * a.block_size * a.row_bytes;
+  const int per = a.pieces > kLoads ? kLoads * 64 / a.pieces : 64;
+  auto find = [&](int base) {
+    return lane < per && base + lane < j1 ? move_of(a, l, base + lane, head) : Move{kNone, kNone};
+  };
+  const int step = WAVES * per;
+  Move next = find(j0 + wave * per);
+  for (int base = j0; base < j1; base += step) {
+    const Move m = next;
+    const int mine = base + wave * per;
+    if (mine + step < j1) next = find(mine + step);
+    const int rows = j1 - mine < per ? j1 - mine : per, total = rows > 0 ? rows * a.pieces : 0;
+    for (int y = plane0; y < plane1; ++y) {
+      char* const plane = a.pool[y >> 1] + (y & 1) * plane_bytes;
+      u32x4 v[kLoads];
 #pragma unroll
-    for (int x = 0; x < kItems; ++x) {
-      const int i = i0 + x * THREADS + t, j = (int)((uint32_t)i / (uint32_t)pieces);
-      m[x] = i < total ? move_of(a, l, j0 + j, head, row_bytes) : Move{-1, -1};
-      const int64_t in = (int64_t)(i - j * pieces) * (int)sizeof(WORD);
-      if (m[x].from >= 0) {
-        m[x].from += in;
-        m[x].to += in;
+      for (int x = 0; x < kLoads; ++x) {
+        if (64 * x >= total) break;
+        const int i = 64 * x + lane;
+        const int r = a.pieces_shift >= 0 ? i >> a.pieces_shift : i / a.pieces;
+        const uint32_t from = (uint32_t)__shfl((int)m.from, r & 63, 64);
+        if (i < total && from != kNone)
+          v[x] = *reinterpret_cast<const u32x4*>(plane + (int64_t)from * a.row_bytes +
+                                                 16 * (i - r * a.pieces));
+      }
+      if constexpr (IN_PLACE && WAVES > 1) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+      }
+#pragma unroll
+      for (int x = 0; x < kLoads; ++x) {
+        if (64 * x >= total) break;
+        const int i = 64 * x + lane;
+        const int r = a.pieces_shift >= 0 ? i >> a.pieces_shift : i / a.pieces;
+        const uint32_t to = (uint32_t)__shfl((int)m.to, r & 63, 64);
+        if (i < total && to != kNone)
+          *reinterpret_cast<u32x4*>(plane + (int64_t)to * a.row_bytes + 16 * (i - r * a.pieces)) =
+              v[x];
       }
     }
-  };
-  Move next[kItems];
-  slots(0, next);
-  for (int i0 = 0; i0 < total; i0 += kItems * THREADS) {
-    Move m[kItems];
-    WORD v[kItems];
-#pragma unroll
-    for (int x = 0; x < kItems; ++x) {
-      m[x] = next[x];
-      if (m[x].from >= 0) v[x] = *reinterpret_cast<const WORD*>(plane + m[x].from);
-    }
-    if (i0 + kItems * THREADS < total) slots(i0 + kItems * THREADS, next);
-    // every read of this step before its writes: within a wave by their order (a place written here
-    // is before the sources still on their way), across waves by a wait and a barrier
-    if constexpr (IN_PLACE && THREADS > 64) {
+  }
+}
+// The same of numbers, one a row: scale bytes, weights.
+template <int WAVES, bool IN_PLACE, class WORD>
+__device__ __forceinline__ void move_words(const MoveArgs& a, const List& l, int head, WORD* plane,
+                                           int lane, int wave, int j0, int j1) {
+  const int step = WAVES * 64;
+  Move next = j0 + 64 * wave + lane < j1 ? move_of(a, l, j0 + 64 * wave + lane, head)
+                                         : Move{kNone, kNone};
+  for (int base = j0; base < j1; base += step) {
+    const Move m = next;
+    const int j = base + step + 64 * wave + lane;
+    WORD v{};
+    if (m.from != kNone) v = plane[m.from];
+    next = j < j1 ? move_of(a, l, j, head) : Move{kNone, kNone};
+    if constexpr (IN_PLACE && WAVES > 1) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
     }
-#pragma unroll
-    for (int x = 0; x < kItems; ++x)
-      if (m[x].from >= 0) *reinterpret_cast<WORD*>(plane + m[x].to) = v[x];
+    if (m.from != kNone) plane[m.to] = v;
   }
 }
 
-// blockIdx.x: lists (sequence, kv head), 256 / THREADS of them to a workgroup where a wave takes one;
-// blockIdx.y: the planes of the pools, of their scales, the weights; blockIdx.z: a piece of the list.
-template <int THREADS, bool IN_PLACE>
-__global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void kv_move_kernel(MoveArgs a) {
-  constexpr int kBlock = THREADS < 256 ? 256 : THREADS;
-  const int t = threadIdx.x % THREADS;
-  const int64_t unit = (int64_t)blockIdx.x * (kBlock / THREADS) + threadIdx.x / THREADS;
+// blockIdx.x: lists (sequence, kv head), four to a workgroup where a wave takes one; blockIdx.y: groups
+// of the pools' planes, then the planes of their scales, then the weights; blockIdx.z: a piece of the
+// list.
+template <int WAVES, bool IN_PLACE>
+__global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void kv_move_kernel(MoveArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int64_t unit = WAVES == 1 ? (int64_t)blockIdx.x * 4 + wv : blockIdx.x;
+  const int wave = WAVES == 1 ? 0 : wv;
   if (unit >= (int64_t)a.num_seqs * a.num_kv_heads) return;
   const int seq = (int)(unit / a.num_kv_heads), head = (int)(unit - (int64_t)seq * a.num_kv_heads);
   const List l = list_of(a, seq, head);
   int j0 = 0, j1 = l.n;
   if (!IN_PLACE) {
-    const int per = (l.n + (int)gridDim.z - 1) / (int)gridDim.z;
+    const int per = ((l.n + (int)gridDim.z - 1) / (int)gridDim.z + 63) / 64 * 64;
+    if ((int64_t)per * blockIdx.z >= l.n) return;
     j0 = per * (int)blockIdx.z;
-    j1 = j0 + per < l.n ? j0 + per : l.n;
+    j1 = l.n - j0 > per ? j0 + per : l.n;
   }
   if (j0 >= j1) return;
-  const int64_t rows = a.num_blocks * a.num_kv_heads * a.block_size;    // of a plane
-  const int y = blockIdx.y, main = 2 * a.pools;
-  if (y < main) {
-    move_rows<THREADS, IN_PLACE, u32x4>(a, l, a.pool[y >> 1] + (y & 1) * rows * a.row_bytes, head,
-                                        a.row_bytes, t, j0, j1);
-  } else if (y == main && a.mass) {
-    move_rows<THREADS, IN_PLACE, uint32_t>(a, l, reinterpret_cast<char*>(a.mass), head, 4, t, j0,
-                                           j1);
+  const int main = 2 * a.pools, groups = (main + a.planes_each - 1) / a.planes_each;
+  const int y = blockIdx.y;
+  if (y < groups) {
+    const int y0 = y * a.planes_each, y1 = y0 + a.planes_each < main ? y0 + a.planes_each : main;
+    move_rows<WAVES, IN_PLACE>(a, l, head, y0, y1, lane, wave, j0, j1);
+  } else if (y - groups < main && a.scales[0]) {
+    const int s = y - groups;
+    uint8_t* const plane = reinterpret_cast<uint8_t*>(a.scales[s >> 1]) +
+                           (s & 1) * (a.num_blocks * a.num_kv_heads * a.block_size);
+    move_words<WAVES, IN_PLACE>(a, l, head, plane, lane, wave, j0, j1);
   } else {
-    const int s = y - main - (a.mass ? 1 : 0);
-    move_rows<THREADS, IN_PLACE, uint8_t>(a, l, a.scales[s >> 1] + (s & 1) * rows, head, 1, t, j0,
-                                          j1);
+    move_words<WAVES, IN_PLACE>(a, l, head, a.mass, lane, wave, j0, j1);
   }
 }
 
@@ -173,11 +203,12 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void kv_move_kernel(
 // those between the largest weights, of equal ones the first, in the order of their positions.
 // A workgroup per (kv head, sequence): a radix select over the weights as ordered 32-bit keys, eight
 // bits a pass from the top, then one pass that writes positions.  Bound: the passes' trips through
-// LDS (keys are read from the pool once; those past kHeld again each pass) for few and short lists,
+// LDS (keys are read from the pool once; those past kHeldMany again each pass) for few and short lists,
 // which leave most of the GPU idle.
 constexpr int kSelThreads = 1024;
 constexpr int kSelWaves = kSelThreads / 64;
-constexpr int kHeld = 15360;          // keys in LDS (64 KiB in all: more a launch has to ask for)
+// Keys in LDS, by position: of a short table, or as many as a workgroup can have.
+constexpr int kHeldFew = 8192, kHeldMany = 38912;
 
 struct SelectArgs {
   int32_t* keep;                      // [seq][kv head][budget]
@@ -199,8 +230,9 @@ __device__ __forceinline__ uint32_t key_of(float v) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-__global__ __launch_bounds__(kSelThreads) void kv_select_kernel(SelectArgs a, int held) {
-  extern __shared__ uint32_t keys[];                     // [held]
+template <int HELD>
+__global__ __launch_bounds__(kSelThreads) void kv_select_kernel(SelectArgs a) {
+  __shared__ __attribute__((aligned(16))) uint32_t keys[HELD];
   __shared__ uint32_t hist[256];
   __shared__ int above[kSelWaves], equal[kSelWaves];
   __shared__ uint32_t s_prefix;
@@ -223,19 +255,48 @@ __global__ __launch_bounds__(kSelThreads) void kv_select_kernel(SelectArgs a, in
   for (int j = t; j < a.recent; j += kSelThreads)
     out[a.budget - a.recent + j] = len - a.recent + j;
   const int want = a.budget - a.sinks - a.recent;        // of these:
-  const int n = len - a.sinks - a.recent;                // candidates, more than want
+  const int lo = a.sinks, hi = len - a.recent;           // candidates: more than want
   if (want == 0) return;
   const int32_t* const table = a.table + seq * a.table_stride;
   const uint32_t bs = (uint32_t)a.block_size;
-  auto load = [&](int i) {
-    const uint32_t p = (uint32_t)(a.sinks + i), c = p / bs;
-    const int b = table[c];
-    if (b < 0 || b >= a.num_blocks) return 0u;
-    return key_of(a.mass[((int64_t)b * a.num_kv_heads + head) * bs + (p - c * bs)]);
+  auto row_of = [&](uint32_t p, int b) {
+    return ((int64_t)b * a.num_kv_heads + head) * bs + (p - p / bs * bs);
   };
-  auto key = [&](int i) { return i < held ? keys[i] : load(i); };
-#pragma unroll 4
-  for (int i = t; i < n && i < held; i += kSelThreads) keys[i] = load(i);
+  auto valid = [&](int b) { return b >= 0 && b < a.num_blocks; };
+  auto load = [&](int p) {
+    const int b = table[(uint32_t)p / bs];
+    return valid(b) ? key_of(a.mass[row_of((uint32_t)p, b)]) : 0u;
+  };
+  auto key = [&](int p) { return p < HELD ? keys[p] : load(p); };
+  if (bs % 4 == 0 && ((uintptr_t)a.mass & 15u) == 0) {
+    // four positions a lane: all block ids, then all weights under way
+    constexpr int kQuads = 4;
+    const int end = hi < HELD ? hi : HELD;
+    for (int p0 = 4 * t; p0 < end; p0 += 4 * kSelThreads * kQuads) {
+      int b[kQuads];
+#pragma unroll
+      for (int x = 0; x < kQuads; ++x) {
+        const int p = p0 + 4 * kSelThreads * x;
+        b[x] = p < end ? table[(uint32_t)p / bs] : -1;
+      }
+      f32x4 v[kQuads];
+#pragma unroll
+      for (int x = 0; x < kQuads; ++x)
+        if (valid(b[x]))
+          v[x] = *reinterpret_cast<const f32x4*>(
+              a.mass + row_of((uint32_t)(p0 + 4 * kSelThreads * x), b[x]));
+#pragma unroll
+      for (int x = 0; x < kQuads; ++x) {
+        const int p = p0 + 4 * kSelThreads * x;
+        if (p >= end) break;
+        u32x4 k = {0u, 0u, 0u, 0u};
+        if (valid(b[x])) k = u32x4{key_of(v[x][0]), key_of(v[x][1]), key_of(v[x][2]), key_of(v[x][3])};
+        *reinterpret_cast<u32x4*>(&keys[p]) = k;
+      }
+    }
+  } else {
+    for (int p = t; p < hi && p < HELD; p += kSelThreads) keys[p] = load(p);
+  }
   // The want-th largest key: its bits from the top, those above fixed as `prefix`.
   uint32_t prefix = 0;
   int left = want;                                       // of those that share the prefix
@@ -243,18 +304,23 @@ __global__ __launch_bounds__(kSelThreads) void kv_select_kernel(SelectArgs a, in
     if (t < 256) hist[t] = 0;
     __syncthreads();
     const uint32_t fixed = shift == 24 ? 0u : ~0u << (shift + 8);
-    for (int i = t; i < n; i += kSelThreads) {
+    for (int i = lo + t; i < hi; i += kSelThreads) {
       const uint32_t k = key(i);
-      const bool in = (k & fixed) == prefix;
-      // lanes with the digit of the first one count at once (weights of 0 are many)
+      bool in = (k & fixed) == prefix;
+      // lanes with one digit count at once, a few digits of a wave (weights of 0 are many, and the
+      // first digits few); the others each
       const uint32_t digit = (k >> shift) & 255u;
-      const uint64_t active = __builtin_amdgcn_ballot_w64(in);
-      if (!active) continue;
-      const int leader = __builtin_ctzll(active);
-      const uint32_t d0 = (uint32_t)__builtin_amdgcn_readlane((int)digit, leader);
-      const uint64_t same = __builtin_amdgcn_ballot_w64(in && digit == d0);
-      if (lane == leader) atomicAdd(&hist[d0], (uint32_t)__builtin_popcountll(same));
-      if (in && digit != d0) atomicAdd(&hist[digit], 1u);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const uint64_t active = __builtin_amdgcn_ballot_w64(in);
+        if (!active) break;
+        const int leader = __builtin_ctzll(active);
+        const uint32_t d0 = (uint32_t)__builtin_amdgcn_readlane((int)digit, leader);
+        const uint64_t same = __builtin_amdgcn_ballot_w64(in && digit == d0);
+        if (lane == leader) atomicAdd(&hist[d0], (uint32_t)__builtin_popcountll(same));
+        in = in && digit != d0;
+      }
+      if (in) atomicAdd(&hist[digit], 1u);
     }
     __syncthreads();
     if (wv == 0) {
@@ -285,8 +351,8 @@ __global__ __launch_bounds__(kSelThreads) void kv_select_kernel(SelectArgs a, in
     left = s_left;
   }
   // Each wave takes a run of positions: it counts, then writes behind those of the waves before.
-  const int run = (n + kSelWaves - 1) / kSelWaves;
-  const int i0 = wv * run, i1 = i0 + run < n ? i0 + run : n;
+  const int run = (hi - lo + kSelWaves - 1) / kSelWaves;
+  const int i0 = lo + wv * run, i1 = i0 + run < hi ? i0 + run : hi;
   int more = 0, same = 0;
   for (int b = i0; b < i1; b += 64) {
     const uint32_t k = b + lane < i1 ? key(b + lane) : 0u;
@@ -312,7 +378,7 @@ __global__ __launch_bounds__(kSelThreads) void kv_select_kernel(SelectArgs a, in
     const bool mine = in && (k > prefix || (k == prefix &&
                                             ties + __builtin_popcountll(eq & below) < left));
     const uint64_t take = __builtin_amdgcn_ballot_w64(mine);
-    if (mine) out[a.sinks + at + __builtin_popcountll(take & below)] = a.sinks + b + lane;
+    if (mine) out[a.sinks + at + __builtin_popcountll(take & below)] = b + lane;
     at += __builtin_popcountll(take);
     ties += __builtin_popcountll(eq);
   }
@@ -340,7 +406,8 @@ extern "C" int ndl_kv_compact(void* const* pools, void* const* scales, int num_l
   if (num_seqs == 0 || (num_layers == 0 && !mass) || most == 0) return NDL_OK;
   if ((num_layers && !pools) || !block_table || !keep || !counts) return NDL_ERR_INVALID_ARG;
   if (num_layers > kMaxPools || (int64_t)max_blocks_per_seq * block_size > 0x7fffff00 ||
-      (int64_t)dst_max_blocks * block_size > 0x7fffff00 || most * (row_bytes / 16) > 0x7fff0000)
+      (int64_t)dst_max_blocks * block_size > 0x7fffff00 || most > 0x7fff0000 ||
+      num_blocks > (int64_t)0xfffffff0 / num_kv_heads / block_size || row_bytes > 16 * kLoads * 64)
     return NDL_ERR_UNSUPPORTED;
   MoveArgs a{};
   for (int i = 0; i < num_layers; ++i) {
@@ -370,26 +437,39 @@ extern "C" int ndl_kv_compact(void* const* pools, void* const* scales, int num_l
   a.first = first;
   a.counts = counts;
   a.num_seqs = num_seqs;
+  a.pieces = row_bytes / 16;
+  a.pieces_shift = -1;
+  for (int x = 0; x < 16; ++x)
+    if (a.pieces == 1 << x) a.pieces_shift = x;
   const int64_t units = (int64_t)num_seqs * num_kv_heads;
-  const int planes = 2 * num_layers * (scales ? 2 : 1) + (mass ? 1 : 0);
+  const int main = 2 * num_layers, small = (scales ? main : 0) + (mass ? 1 : 0);
   const hipStream_t s = (hipStream_t)stream;
   if (!grid_fits(units, 1024)) return NDL_ERR_UNSUPPORTED;
-  if (dst_table) {
-    // pieces of a list: what its longest needs, up to four rounds of the GPU's workgroups
-    const int64_t step = (int64_t)256 * kItems * 16 / row_bytes;
-    int64_t z = (most + step - 1) / step;
-    const int64_t fill = (4 * 2048 + units * planes - 1) / (units * planes);
-    if (z > fill) z = fill;
-    if (z > 65535) z = 65535;
-    hipLaunchKernelGGL((kv_move_kernel<256, false>),
-                       dim3((unsigned)units, (unsigned)planes, (unsigned)z), dim3(256), 0, s, a);
-  } else if (most <= 64 || cu_seqlens) {
-    hipLaunchKernelGGL((kv_move_kernel<64, true>), dim3((unsigned)((units + 3) / 4), (unsigned)planes),
-                       dim3(256), 0, s, a);
-  } else {
-    hipLaunchKernelGGL((kv_move_kernel<1024, true>), dim3((unsigned)units, (unsigned)planes),
-                       dim3(1024), 0, s, a);
+  const bool waves = dst_table || most <= 64 || cu_seqlens;      // a wave a list, or a piece of one
+  // Pieces of a list: 64 rows and more, up to two rounds of the waves that the GPU holds; planes to
+  // a wave: more where there are lists enough.
+  int64_t z = 1;
+  a.planes_each = 1;
+  if (waves) {
+    const int64_t hold = 256 * 32;
+    if (dst_table) {
+      z = (most + 63) / 64;
+      const int64_t fill = 2 * hold / (units * (main + small)) + 1;
+      if (z > fill) z = fill;
+      if (z > 65535) z = 65535;
+    }
+    const int64_t each = units * z * main / hold;
+    a.planes_each = (int)(each < 1 ? 1 : each > 8 ? 8 : each);
   }
+  const int groups = (main + a.planes_each - 1) / a.planes_each;
+  const dim3 grid((unsigned)(waves ? (units + 3) / 4 : units), (unsigned)(groups + small),
+                  (unsigned)z);
+  if (dst_table)
+    hipLaunchKernelGGL((kv_move_kernel<1, false>), grid, dim3(256), 0, s, a);
+  else if (waves)
+    hipLaunchKernelGGL((kv_move_kernel<1, true>), grid, dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL((kv_move_kernel<16, true>), grid, dim3(1024), 0, s, a);
   return check_launch();
 }
 
@@ -409,9 +489,12 @@ extern "C" int ndl_kv_select(int32_t* keep, int32_t* kept, const float* mass, in
     return NDL_ERR_UNSUPPORTED;
   SelectArgs a{keep, kept, mass, num_blocks, num_kv_heads, block_size, block_table, bt_row_stride,
                max_blocks_per_seq, lens, budget, sinks, recent};
-  const int64_t cap = (int64_t)max_blocks_per_seq * block_size;
-  const int held = (int)(cap < kHeld ? cap : kHeld);
-  hipLaunchKernelGGL(kv_select_kernel, dim3((unsigned)num_kv_heads, (unsigned)num_seqs),
-                     dim3(kSelThreads), held * 4, (hipStream_t)stream, a, held);
+  const dim3 grid((unsigned)num_kv_heads, (unsigned)num_seqs);
+  if ((int64_t)max_blocks_per_seq * block_size <= kHeldFew)
+    hipLaunchKernelGGL((kv_select_kernel<kHeldFew>), grid, dim3(kSelThreads), 0,
+                       (hipStream_t)stream, a);
+  else
+    hipLaunchKernelGGL((kv_select_kernel<kHeldMany>), grid, dim3(kSelThreads), 0,
+                       (hipStream_t)stream, a);
   return check_launch();
 }

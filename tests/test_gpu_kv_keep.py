@@ -221,7 +221,7 @@ def test_tables_with_invalid_blocks_and_lengths_past_them():
 
 
 def test_select_more_tokens_than_are_held():
-    lens = [40000, 15361, 15360 + 70]
+    lens = [40000, 38912, 38912 + 70]
     c = Cache(lens, hkv=1, bs=64, seed=12)
     m = (c.mass() * 1000).round()
     check_select(m, c.table, i32(lens), 5000, 4, 60)
