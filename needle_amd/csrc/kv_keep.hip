@@ -13,14 +13,16 @@ namespace {
 // Row first + j of a sequence <- row first + keep[j], j < count: of one kv head, or of all alike.
 // Bound: the rows, read and written once, and the trips before them (length, index, block ids).
 //   * A lane finds a row's source and place, for up to 64 rows of a wave's step and for several planes
-//     (layers, K and V); then the wave's lanes take 16-byte pieces of those rows, up to 16 loads under
+//     (layers, K and V); then the wave's lanes take 16-byte pieces of those rows, 8 or 16 loads under
 //     way, and the next step's rows are found meanwhile.  (A scale byte or a weight: a lane a row.)
 //   * In place the indices ascend, so a row's source is never written before it is read: a later row
 //     has a later source and a later place.  One wave (short lists) or the 16 of a workgroup (long
 //     ones, a barrier between the reads of a step and its writes) take a list from front to back.
 //   * Into other blocks nothing is ordered, and lists are cut into as many pieces as fill the GPU.
 constexpr int kMaxPools = 128;
-constexpr int kLoads = 16;        // of a lane under way
+// Loads of a lane under way: us, 8 / 16, in place 32 layers of 32 trees' paths 12.2 / 14.9, into other
+// blocks 16 x 2,048 rows of 8 heads 67 / 62 (fewer waves fit, but lists are longer).
+constexpr int loads_of(bool in_place) { return in_place ? 8 : 16; }
 
 struct MoveArgs {
   char* pool[kMaxPools];
@@ -100,6 +102,7 @@ template <int WAVES, bool IN_PLACE>
 __device__ __forceinline__ void move_rows(const MoveArgs& a, const List& l, int head, int plane0,
                                           int plane1, int lane, int wave, int j0, int j1) {
   const int64_t plane_bytes = a.num_blocks * a.num_kv_heads * a.block_size * a.row_bytes;
+  constexpr int kLoads = loads_of(IN_PLACE);
   const int per = a.pieces > kLoads ? kLoads * 64 / a.pieces : 64;
   auto find = [&](int base) {
     return lane < per && base + lane < j1 ? move_of(a, l, base + lane, head) : Move{kNone, kNone};
@@ -306,21 +309,16 @@ __global__ __launch_bounds__(kSelThreads) void kv_select_kernel(SelectArgs a) {
     const uint32_t fixed = shift == 24 ? 0u : ~0u << (shift + 8);
     for (int i = lo + t; i < hi; i += kSelThreads) {
       const uint32_t k = key(i);
-      bool in = (k & fixed) == prefix;
-      // lanes with one digit count at once, a few digits of a wave (weights of 0 are many, and the
-      // first digits few); the others each
+      const bool in = (k & fixed) == prefix;
+      // lanes with the first one's digit count at once (weights of 0 are many), the others each
       const uint32_t digit = (k >> shift) & 255u;
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const uint64_t active = __builtin_amdgcn_ballot_w64(in);
-        if (!active) break;
-        const int leader = __builtin_ctzll(active);
-        const uint32_t d0 = (uint32_t)__builtin_amdgcn_readlane((int)digit, leader);
-        const uint64_t same = __builtin_amdgcn_ballot_w64(in && digit == d0);
-        if (lane == leader) atomicAdd(&hist[d0], (uint32_t)__builtin_popcountll(same));
-        in = in && digit != d0;
-      }
-      if (in) atomicAdd(&hist[digit], 1u);
+      const uint64_t active = __builtin_amdgcn_ballot_w64(in);
+      if (!active) continue;
+      const int leader = __builtin_ctzll(active);
+      const uint32_t d0 = (uint32_t)__builtin_amdgcn_readlane((int)digit, leader);
+      const uint64_t same = __builtin_amdgcn_ballot_w64(in && digit == d0);
+      if (lane == leader) atomicAdd(&hist[d0], (uint32_t)__builtin_popcountll(same));
+      if (in && digit != d0) atomicAdd(&hist[digit], 1u);
     }
     __syncthreads();
     if (wv == 0) {
@@ -407,7 +405,7 @@ extern "C" int ndl_kv_compact(void* const* pools, void* const* scales, int num_l
   if ((num_layers && !pools) || !block_table || !keep || !counts) return NDL_ERR_INVALID_ARG;
   if (num_layers > kMaxPools || (int64_t)max_blocks_per_seq * block_size > 0x7fffff00 ||
       (int64_t)dst_max_blocks * block_size > 0x7fffff00 || most > 0x7fff0000 ||
-      num_blocks > (int64_t)0xfffffff0 / num_kv_heads / block_size || row_bytes > 16 * kLoads * 64)
+      num_blocks > (int64_t)0xfffffff0 / num_kv_heads / block_size || row_bytes > 16 * loads_of(true) * 64)
     return NDL_ERR_UNSUPPORTED;
   MoveArgs a{};
   for (int i = 0; i < num_layers; ++i) {
