@@ -720,6 +720,33 @@ int ndl_verify_tree(void* tokens, int32_t* accepted, int32_t* path, const void* 
                     void* workspace, size_t workspace_bytes, ndl_stream_t stream);
 
 /*
+ * Attention over a 16-bit pool (bf16, fp16) that also adds up the weights of every cached token and kv
+ * head, in mass float32 [num_blocks][num_kv_heads][block_size].  Token j of sequence i (packed by
+ * cu_seqlens; NULL: one token per sequence, then num_tokens == num_seqs and max_seqlen == 1) attends
+ * the first min(context_lens[i] + j + 1, max_blocks_per_seq * block_size) tokens, as
+ * ndl_paged_decode and ndl_varlen_prefill have it (K and V of the new tokens are in the cache).
+ * With p the softmax's weights of the call's tokens and query heads, position x gets
+ * decay * mass + sum p where it was cached (x < context_lens[i]) and sum p where it is new; a decay
+ * of 0 forgets what was there.  Sums are fp32 and run in a fixed order.  Positions with invalid block
+ * ids and sequences that attend nothing keep what they have; no block may be attended by two
+ * sequences.
+ *
+ * max_seqlen and max_keys bound a sequence's tokens and keys: those past them may not be computed and
+ * get no weight.  The workspace (ndl_attention_mass_workspace_bytes of the same sizes, max_keys cut
+ * to the table's, on the same device) is 256-byte aligned and belongs to one call at a time.
+ */
+size_t ndl_attention_mass_workspace_bytes(int num_seqs, int64_t num_tokens, int max_seqlen,
+                                          int64_t max_keys, int num_heads, int num_kv_heads,
+                                          int head_dim, int block_size);
+int ndl_attention_mass(void* out, float* mass, const void* q, int64_t q_tok_stride,
+                       const void* kv_cache, int64_t num_blocks, const int32_t* block_table,
+                       int64_t bt_row_stride, int max_blocks_per_seq, const int32_t* cu_seqlens,
+                       const int32_t* context_lens, int num_seqs, int64_t num_tokens,
+                       int max_seqlen, int64_t max_keys, int num_heads, int num_kv_heads,
+                       int head_dim, int block_size, int dtype, float scale, float decay,
+                       void* workspace, size_t workspace_bytes, ndl_stream_t stream);
+
+/*
  * Rows of cached tokens moved together: row first[i] + j of sequence i (first NULL: j) becomes what row
  * first[i] + keep[j] was, for j < counts[i].  keep is [num_seqs][num_kv_heads][keep_width], a list
  * for each kv head, or, with cu_seqlens, [num_keep] packed by it, a list for all kv heads alike

@@ -62,6 +62,8 @@ EXPORTED_SYMBOLS = (
     "ndl_fp8_tree_attention",
     "ndl_verify_tree_workspace_bytes",
     "ndl_verify_tree",
+    "ndl_attention_mass_workspace_bytes",
+    "ndl_attention_mass",
     "ndl_kv_compact",
     "ndl_kv_select",
 )
@@ -265,6 +267,15 @@ _SIGNATURES = {
         _c_p, _c_p, _c_p, _c_p, _c_i64, _c_i32,         # tokens, accepted, path, logits, stride, dtype
         _c_p, _c_i32, _c_p, _c_p, _c_p, _c_p,           # ids, int64, parents, cu, uniforms, temp.
         _c_i64, _c_i32, _c_i32, _c_p, _c_sz, _c_p,      # T, B, V, workspace, bytes, stream
+    ]),
+    "ndl_attention_mass_workspace_bytes": (_c_sz, [_c_i32, _c_i64, _c_i32, _c_i64] + [_c_i32] * 4),
+    "ndl_attention_mass": (_c_i32, [
+        _c_p, _c_p, _c_p, _c_i64,                       # out, mass, q, q stride
+        _c_p, _c_i64,                                   # cache, NB
+        _c_p, _c_i64, _c_i32,                           # block_table, row stride, W
+        _c_p, _c_p, _c_i32, _c_i64, _c_i32, _c_i64,     # cu, ctx, B, T, max_seqlen, max_keys
+        _c_i32, _c_i32, _c_i32, _c_i32, _c_i32,         # H, Hkv, D, bs, dtype
+        _c_f32, _c_f32, _c_p, _c_sz, _c_p,              # scale, decay, workspace, bytes, stream
     ]),
     "ndl_kv_compact": (_c_i32, [
         _c_p, _c_p, _c_i32, _c_p,                       # pools, scales, layers, mass

@@ -36,6 +36,9 @@ namespace {
 
 constexpr float kRaise = 256.f;   // a lane's sum of a tile's probabilities past which the maximum is raised
 
+// kScored: causal, and the scores stay behind in a.scores (row blocks of up to 32 columns).
+enum Chunk { kCausal, kTree, kScored };
+
 struct TreeOperands {
   u16* out;
   const u16* q;
@@ -48,6 +51,9 @@ struct TreeOperands {
   int64_t mask_stride;
   int words;
   float* lse;
+  float* scores;                // [kv head][sequence][column][score_keys], scaled, log2
+  int64_t score_keys;
+  int score_cols;
   uint32_t q_flip, q_keep;      // of two elements of q: signs flipped (scale < 0), kept (scale not 0)
 };
 struct TreeArgs : TreeOperands, RowBlocks {};
@@ -96,8 +102,9 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
 
 // A workgroup's share of the row blocks of one kv head.  Its four waves are as many groups of columns
 // (CG) side by side as a row block has columns for, times as many groups of keys (KG) as are left.
-template <int D, bool F16, bool TREE>
+template <int D, bool F16, Chunk KIND>
 __global__ __launch_bounds__(64 * kWaves, 2) void tree_attention_kernel(TreeArgs a) {
+  constexpr bool TREE = KIND == kTree;
   using T = Elt<F16>;
   using X8 = typename T::x8;
   using S = TreeShape<D>;
@@ -363,6 +370,21 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_attention_kernel(TreeArgs
             sc[r] = (here >> (8 * (r >> 2) + (r & 3))) & 1u ? sc[r] : kNegInf;
         }
 
+        if constexpr (KIND == kScored) {
+          // four keys to a store; past the keys and where nothing is attended -inf
+          if (live && col < a.score_cols) {
+            float* const at =
+                a.scores +
+                (((int64_t)head * a.num_seqs + it.seq) * a.score_cols + col) * a.score_keys +
+                kTile * (t0 + kg + KG * u) + 4 * h;
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              *reinterpret_cast<f32x4*>(at + 8 * x) =
+                  f32x4{sc[4 * x] * a.scale_log2, sc[4 * x + 1] * a.scale_log2,
+                        sc[4 * x + 2] * a.scale_log2, sc[4 * x + 3] * a.scale_log2};
+          }
+        }
+
         // Probabilities against the running maximum as it stands.  Where one exceeds 2^kRaise its
         // lane's sum does, and then (or while a column has no maximum yet) the maximum is raised, the
         // sums rescaled and the probabilities taken again: no maximum is computed otherwise.
@@ -546,12 +568,16 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_attention_kernel(TreeArgs
         }
       }
     };
-    if (cols <= 32)
+    if constexpr (KIND == kScored) {
       row_block(std::integral_constant<int, 1>{});
-    else if (cols <= 64)
-      row_block(std::integral_constant<int, 2>{});
-    else
-      row_block(std::integral_constant<int, 4>{});
+    } else {
+      if (cols <= 32)
+        row_block(std::integral_constant<int, 1>{});
+      else if (cols <= 64)
+        row_block(std::integral_constant<int, 2>{});
+      else
+        row_block(std::integral_constant<int, 4>{});
+    }
     if (whole) return;
     __syncthreads();     // before the ring is written again
   }
@@ -576,19 +602,18 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
 
 // ---------------------------------------------------------------- launches
 
-const void* kernel_for(int head_dim, bool f16, bool tree) {
-  if (head_dim == 128) {
-    if (f16)
-      return tree ? (const void*)tree_attention_kernel<128, true, true>
-                  : (const void*)tree_attention_kernel<128, true, false>;
-    return tree ? (const void*)tree_attention_kernel<128, false, true>
-                : (const void*)tree_attention_kernel<128, false, false>;
-  }
-  if (f16)
-    return tree ? (const void*)tree_attention_kernel<64, true, true>
-                : (const void*)tree_attention_kernel<64, true, false>;
-  return tree ? (const void*)tree_attention_kernel<64, false, true>
-              : (const void*)tree_attention_kernel<64, false, false>;
+template <int D, bool F16>
+const void* kernel_of(Chunk kind) {
+  return kind == kTree     ? (const void*)tree_attention_kernel<D, F16, kTree>
+         : kind == kScored ? (const void*)tree_attention_kernel<D, F16, kScored>
+                           : (const void*)tree_attention_kernel<D, F16, kCausal>;
+}
+const void* kernel_for(int head_dim, bool f16, Chunk kind) {
+  if (head_dim == 128) return f16 ? kernel_of<128, true>(kind) : kernel_of<128, false>(kind);
+  return f16 ? kernel_of<64, true>(kind) : kernel_of<64, false>(kind);
+}
+Chunk kind_of(const ChunkAttention& c) {
+  return c.mask != nullptr ? kTree : c.scores != nullptr ? kScored : kCausal;
 }
 
 constexpr int kMinChunk = 8;      // slots a share has at least
@@ -607,17 +632,18 @@ Plan plan_for(const ChunkAttention& c) {
   Plan p{};
   const int group = c.num_heads / c.num_kv_heads;
   // the formats' kernels use the same resources
-  int64_t res = resident_workgroups(kernel_for(c.head_dim, false, true), 64 * kWaves);
+  int64_t res = resident_workgroups(kernel_for(c.head_dim, false, kTree), 64 * kWaves);
   if (res <= 0) res = 256;
   const int64_t tiles = (c.max_keys + kTile - 1) / kTile;
   // Columns of a row block: as few as leave no part of the GPU idle.
   int64_t units = 0;
   for (int cols = 32 * kWaves; cols >= 32; cols /= 2) {
+    if (cols > 32 && (int64_t)c.max_seqlen * group <= cols / 2) continue;
     p.toks = cols / group;
     p.blocks_per_seq = (c.max_seqlen + p.toks - 1) / p.toks;
     p.items = c.num_seqs * p.blocks_per_seq;
     units = p.items * c.num_kv_heads;
-    if (units * 2 > res || c.max_seqlen * group <= 32) break;
+    if (units * 2 > res) break;
   }
   // (slots and segments are counted in 31 bits)
   const bool whole = tiles <= kWholeTiles || units >= res ||
@@ -746,6 +772,9 @@ int launch_chunk_attention(const ChunkAttention& call, void* workspace, size_t w
   a.mask_stride = c.mask_stride;
   a.words = c.mask_words;
   a.lse = c.lse;
+  a.scores = c.scores;
+  a.score_keys = c.score_keys;
+  a.score_cols = c.max_seqlen * a.group;
   a.block_table = c.block_table;
   a.bt_row_stride = c.bt_row_stride;
   a.max_blocks = c.max_blocks_per_seq;
@@ -770,7 +799,7 @@ int launch_chunk_attention(const ChunkAttention& call, void* workspace, size_t w
   const int64_t wgs = units * a.num_kv_heads;
   if (!grid_fits(wgs, threads)) return NDL_ERR_INVALID_ARG;
   void* args[] = {&a};
-  if (hipLaunchKernel(kernel_for(c.head_dim, dtype_is_f16(c.dtype), c.mask != nullptr),
+  if (hipLaunchKernel(kernel_for(c.head_dim, dtype_is_f16(c.dtype), kind_of(c)),
                       dim3((unsigned)wgs), dim3(threads), args, 0, s) != hipSuccess) {
     (void)hipGetLastError();  // clear the error so that the next call's check sees its own
     return NDL_ERR_LAUNCH;

@@ -21,6 +21,10 @@ struct ChunkAttention {
   int64_t mask_stride;
   int mask_words;
   float* lse;                      // [token][head], log2 of the softmax's denominator; null: none
+  // [kv head][sequence][max_seqlen * group][score_keys], of at most kScoredColumns columns: scores
+  // times scale and log2 e, those that are not attended -inf, of whole 32-key tiles.  Null: none.
+  float* scores;
+  int64_t score_keys;
   int num_seqs;
   int64_t num_tokens;
   int max_seqlen;
@@ -28,6 +32,8 @@ struct ChunkAttention {
   int num_heads, num_kv_heads, head_dim, block_size, dtype;
   float scale;
 };
+
+constexpr int kScoredColumns = 32;     // tokens times heads of a group that scores are kept of
 
 // Whether a launch can be made of these, NDL_OK or the error.
 int check_chunk_attention(const ChunkAttention& c);

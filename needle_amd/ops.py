@@ -1352,6 +1352,77 @@ def _check_mass(mass, nb, hkv, bs, dev) -> None:
                          f"{tuple(mass.shape)}")
 
 
+def attention_mass_workspace_bytes(num_seqs: int, num_tokens: int, max_seqlen: int, max_keys: int,
+                                   num_heads: int, num_kv_heads: int, head_dim: int,
+                                   block_size: int = 16) -> int:
+    """Bytes of the workspace attention_mass uses on the current GPU, max_keys at most the
+    table's."""
+    return int(_lib.load().ndl_attention_mass_workspace_bytes(
+        num_seqs, num_tokens, max_seqlen, max_keys, num_heads, num_kv_heads, head_dim, block_size))
+
+
+def attention_mass(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor,
+                   context_lens: torch.Tensor, mass: torch.Tensor, scale: float, num_heads: int,
+                   num_kv_heads: int, head_dim: int, *, cu_seqlens: Optional[torch.Tensor] = None,
+                   max_seqlen: int = 1, max_context_len: int = 0, decay: float = 1.0,
+                   out: Optional[torch.Tensor] = None,
+                   workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """paged_decode (cu_seqlens None: one token per sequence) or varlen_prefill, which also adds up
+    the attention weights of every cached token and kv head, in mass (kv_mass_pool): a cached
+    token's number becomes decay times what it was plus its weights in this call, summed over the
+    call's tokens and the query heads of the kv head; a new token's (position context_lens[i] and
+    on) becomes its weights alone.  kv_select picks the tokens that stay by them.
+
+    q [T, H, D] in bfloat16 or float16, kv_cache a 16-bit pool of the same type in which the tokens'
+    K and V are already (kv_append).  For the weights that a prompt's last tokens give, hand over
+    their q alone, with context_lens the tokens before them.  max_seqlen bounds a sequence's tokens,
+    max_context_len its cached ones (0: not known, the table's width then).  decay 0 forgets what
+    was there.  No two sequences may attend one block.  workspace: as decode_workspace gives, of
+    attention_mass_workspace_bytes, for one call at a time."""
+    _check_cache(kv_cache)
+    dev = kv_cache.device
+    _, nb, hkv, bs, d = kv_cache.shape
+    _require(hkv == num_kv_heads and d == head_dim, "kv_cache shape disagrees with head counts")
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"q must be bfloat16 or float16, got {q.dtype}")
+    _require(q.dtype == kv_cache.dtype, "q dtype must match kv_cache", TypeError)
+    qs = _rows("q", q, num_heads, head_dim, dev)
+    _check_group(num_heads, num_kv_heads)
+    _check_mass(mass, nb, hkv, bs, dev)
+    n_seqs, n_tok = _check_table(block_table, nb, dev), q.shape[0]
+    _check_int32("context_lens", context_lens, 1, dev)
+    _require(context_lens.shape[0] == n_seqs, "context_lens/block_table batch mismatch")
+    if cu_seqlens is None:
+        _require(n_tok == n_seqs, "q / block_table batch mismatch")
+        _require(max_seqlen == 1, "without cu_seqlens every sequence has one token")
+    else:
+        _check_int32("cu_seqlens", cu_seqlens, 1, dev)
+        _require(cu_seqlens.shape[0] == n_seqs + 1, "cu_seqlens must be [num_seqs + 1]")
+    out = _check_out(out, n_tok, num_heads, head_dim, q)
+    if n_tok == 0 or n_seqs == 0:
+        return out
+    w = block_table.shape[1]
+    _require(w > 0, "block_table has no columns")
+    _require(max_seqlen > 0, "max_seqlen must be positive")
+    _require(max_context_len >= 0, "max_context_len is negative")
+    max_keys = min(w * bs, max_context_len + max_seqlen) if max_context_len else w * bs
+    lib = _lib.load()
+    with _on(dev):
+        need = attention_mass_workspace_bytes(n_seqs, n_tok, max_seqlen, max_keys, num_heads,
+                                              num_kv_heads, head_dim, bs)
+        if workspace is None or workspace.numel() * workspace.element_size() < need \
+                or workspace.device != dev:
+            workspace = decode_workspace(need, dev)
+        rc = lib.ndl_attention_mass(
+            out.data_ptr(), mass.data_ptr(), q.data_ptr(), qs, kv_cache.data_ptr(), nb,
+            block_table.data_ptr(), block_table.stride(0), w, _ptr(cu_seqlens),
+            context_lens.data_ptr(), n_seqs, n_tok, max_seqlen, max_keys, num_heads, num_kv_heads,
+            head_dim, bs, _DTYPES[q.dtype], float(scale), float(decay), workspace.data_ptr(), need,
+            _stream(dev))
+    _lib.check(rc, "ndl_attention_mass")
+    return out
+
+
 def kv_compact(pools, block_table: torch.Tensor, keep: torch.Tensor, counts: torch.Tensor, *,
                first: Optional[torch.Tensor] = None,
                cu_seqlens: Optional[torch.Tensor] = None,
