@@ -39,6 +39,17 @@ decltype(&ndl_fp8_attention) p_fp8_attention = nullptr;
 decltype(&ndl_fp8_decode_append) p_fp8_decode_append = nullptr;
 decltype(&ndl_verify_drafts_workspace_bytes) p_verify_workspace = nullptr;
 decltype(&ndl_verify_drafts) p_verify_drafts = nullptr;
+decltype(&ndl_tree_mask) p_tree_mask = nullptr;
+decltype(&ndl_tree_attention_workspace_bytes) p_tree_workspace = nullptr;
+decltype(&ndl_tree_attention) p_tree_attention = nullptr;
+decltype(&ndl_fp8_tree_attention_workspace_bytes) p_fp8_tree_workspace = nullptr;
+decltype(&ndl_fp8_tree_attention) p_fp8_tree_attention = nullptr;
+decltype(&ndl_verify_tree_workspace_bytes) p_verify_tree_workspace = nullptr;
+decltype(&ndl_verify_tree) p_verify_tree = nullptr;
+decltype(&ndl_attention_mass_workspace_bytes) p_mass_workspace = nullptr;
+decltype(&ndl_attention_mass) p_attention_mass = nullptr;
+decltype(&ndl_kv_compact) p_kv_compact = nullptr;
+decltype(&ndl_kv_select) p_kv_select = nullptr;
 
 // A plain GPU tensor (no subclass, no wrapper of a function transform), or null.
 const at::Tensor* gpu_tensor(PyObject* o) {
@@ -551,6 +562,320 @@ PyObject* verify_drafts(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// tree_mask(parents, cu_seqlens, max_seqlen): (mask, depth).
+PyObject* tree_mask(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 3 || p_tree_mask == nullptr) Py_RETURN_NONE;
+  const at::Tensor *const parents = gpu_tensor(args[0]), *const cu = gpu_tensor(args[1]);
+  int64_t most;
+  if (parents == nullptr || cu == nullptr || !read_int32(*parents, *parents, 1) ||
+      !read_int32(*cu, *parents, 1) || !read_int(args[2], &most) || most == 0)
+    Py_RETURN_NONE;
+  const int64_t tokens = parents->size(0), seqs = cu->size(0) - 1, words = (most + 63) / 64;
+  if (tokens == 0 || seqs <= 0 || !fits_int(seqs)) Py_RETURN_NONE;
+  const c10::DeviceGuard guard(parents->device());
+  at::Tensor mask = at::empty({tokens, words}, parents->options().dtype(at::kLong));
+  at::Tensor depth = at::empty({tokens}, parents->options());
+  void* const mp = mask.data_ptr();
+  int32_t* const dp = (int32_t*)depth.data_ptr();
+  const ndl_stream_t s = stream_of(*parents);
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = p_tree_mask(mp, words, (int)words, dp, (const int32_t*)parents->data_ptr(),
+                   (const int32_t*)cu->data_ptr(), (int)seqs, tokens, (int)most, s);
+  Py_END_ALLOW_THREADS
+  if (rc != NDL_OK) Py_RETURN_NONE;
+  return tensor_pair(std::move(mask), std::move(depth));
+  END_HANDLE_TH_ERRORS
+}
+
+// What tree_attention and attention_mass have in common: the pool (16-bit), q, table, lengths, and
+// from args[at] on max_seqlen, max_context_len, scale, num_heads, num_kv_heads, head_dim.
+struct ChunkCall {
+  int64_t most, context, heads, hkv, d, bs, num_blocks, qs, tokens, seqs, width, keys;
+  float scale;
+};
+bool read_chunk(const at::Tensor& q, const at::Tensor& pool, const at::Tensor& table,
+                const at::Tensor* cu, const at::Tensor& lens, PyObject* const* args,
+                ChunkCall* c) {
+  if (!read_int(args[0], &c->most) || !read_int(args[1], &c->context) ||
+      !PyFloat_CheckExact(args[2]) || !read_int(args[3], &c->heads) ||
+      !read_int(args[4], &c->hkv) || !read_int(args[5], &c->d) || c->hkv == 0 || c->heads == 0 ||
+      c->heads % c->hkv || c->heads / c->hkv > 16 || !is_16bit(q.scalar_type()) ||
+      pool.size(2) != c->hkv || pool.size(4) != c->d || !read_rows_of(q, pool, c->heads, c->d, &c->qs))
+    return false;
+  c->scale = (float)PyFloat_AS_DOUBLE(args[2]);
+  c->num_blocks = pool.size(1);
+  c->bs = pool.size(3);
+  c->tokens = q.size(0);
+  if (!read_int32(table, pool, 2) || !read_int32(lens, pool, 1) ||
+      (cu != nullptr && !read_int32(*cu, pool, 1)))
+    return false;
+  c->seqs = table.size(0);
+  c->width = table.size(1);
+  if (c->tokens == 0 || c->seqs == 0 || c->width == 0 || c->most == 0 || !fits_int(c->seqs) ||
+      !fits_int(c->width) || !fits_int(c->bs) || lens.size(0) != c->seqs ||
+      (cu != nullptr ? cu->size(0) != c->seqs + 1 : c->tokens != c->seqs || c->most != 1))
+    return false;
+  c->keys = c->width * c->bs;
+  if (c->context > 0 && c->context + c->most < c->keys) c->keys = c->context + c->most;
+  return true;
+}
+
+// tree_attention(q, pool or codes, scales or None, block_table, cu_seqlens, context_lens, mask,
+// max_seqlen, max_context_len, scale, num_heads, num_kv_heads, head_dim): the output.
+PyObject* tree_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 13 || p_tree_attention == nullptr || p_fp8_tree_attention == nullptr || validating())
+    Py_RETURN_NONE;
+  const at::Tensor *const q = gpu_tensor(args[0]), *const pool = gpu_tensor(args[1]), *scales;
+  const at::Tensor *const table = gpu_tensor(args[3]), *const cu = gpu_tensor(args[4]),
+                   *const lens = gpu_tensor(args[5]), *const mask = gpu_tensor(args[6]);
+  if (!q || !pool || !maybe_tensor(args[2], &scales) || !table || !cu || !lens || !mask)
+    Py_RETURN_NONE;
+  Cache c16;
+  Fp8Pool c8;
+  ChunkCall c;
+  if (scales != nullptr ? !read_fp8_pool(*pool, *scales, &c8)
+                        : !read_cache(*pool, &c16) || pool->scalar_type() != q->scalar_type())
+    Py_RETURN_NONE;
+  if (!read_chunk(*q, *pool, *table, cu, *lens, args + 7, &c)) Py_RETURN_NONE;
+  if (mask->scalar_type() != at::kLong || mask->dim() != 2 || mask->size(0) != c.tokens ||
+      mask->size(1) < 1 || !fits_int(mask->size(1)) || mask->device() != pool->device() ||
+      (mask->size(1) > 1 && mask->stride(1) != 1))
+    Py_RETURN_NONE;
+  const int64_t words = mask->size(1), ms = c.tokens > 1 ? mask->stride(0) : words;
+  if (ms < words) Py_RETURN_NONE;
+  const c10::DeviceGuard guard(pool->device());
+  at::Tensor out = at::empty({c.tokens, c.heads, c.d}, q->options()), ws;
+  const size_t need = (scales ? p_fp8_tree_workspace : p_tree_workspace)(
+      (int)c.seqs, (int)c.most, c.keys, (int)c.heads, (int)c.hkv, (int)c.d, (int)c.bs);
+  if (need) ws = at::empty({(int64_t)need}, q->options().dtype(at::kByte));
+  void *const outp = out.data_ptr(), *const wsp = need ? ws.data_ptr() : nullptr;
+  const ndl_stream_t s = stream_of(*pool);
+  const int code = dtype_code(q->scalar_type());
+  const int32_t *const tp = (const int32_t*)table->data_ptr(),
+                *const cp = (const int32_t*)cu->data_ptr(),
+                *const lp = (const int32_t*)lens->data_ptr();
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  if (scales != nullptr)
+    rc = p_fp8_tree_attention(outp, q->data_ptr(), c.qs, pool->data_ptr(), scales->data_ptr(),
+                              c.num_blocks, tp, table->stride(0), (int)c.width, cp, lp,
+                              mask->data_ptr(), ms, (int)words, (int)c.seqs, c.tokens, (int)c.most,
+                              c.keys, (int)c.heads, (int)c.hkv, (int)c.d, (int)c.bs, code, c.scale,
+                              wsp, need, s);
+  else
+    rc = p_tree_attention(outp, q->data_ptr(), c.qs, pool->data_ptr(), c.num_blocks, tp,
+                          table->stride(0), (int)c.width, cp, lp, mask->data_ptr(), ms, (int)words,
+                          (int)c.seqs, c.tokens, (int)c.most, c.keys, (int)c.heads, (int)c.hkv,
+                          (int)c.d, (int)c.bs, code, c.scale, wsp, need, s);
+  Py_END_ALLOW_THREADS
+  if (rc != NDL_OK) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// float32 [num_blocks, num_kv_heads, block_size] of a pool.
+bool read_mass(const at::Tensor& mass, const at::Tensor& pool) {
+  return mass.scalar_type() == at::kFloat && mass.dim() == 3 && mass.is_contiguous() &&
+         mass.device() == pool.device() && mass.size(0) == pool.size(1) &&
+         mass.size(1) == pool.size(2) && mass.size(2) == pool.size(3);
+}
+
+// attention_mass(q, pool, block_table, cu_seqlens or None, context_lens, mass, max_seqlen,
+// max_context_len, scale, num_heads, num_kv_heads, head_dim, decay): the output.
+PyObject* attention_mass(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 13 || p_attention_mass == nullptr || validating()) Py_RETURN_NONE;
+  const at::Tensor *const q = gpu_tensor(args[0]), *const pool = gpu_tensor(args[1]),
+                   *const table = gpu_tensor(args[2]), *cu, *const lens = gpu_tensor(args[4]),
+                   *const mass = gpu_tensor(args[5]);
+  Cache c16;
+  ChunkCall c;
+  if (!q || !pool || !table || !maybe_tensor(args[3], &cu) || !lens || !mass ||
+      !read_cache(*pool, &c16) || pool->scalar_type() != q->scalar_type() ||
+      !read_chunk(*q, *pool, *table, cu, *lens, args + 6, &c) || !read_mass(*mass, *pool) ||
+      !PyFloat_CheckExact(args[12]))
+    Py_RETURN_NONE;
+  const float decay = (float)PyFloat_AS_DOUBLE(args[12]);
+  const c10::DeviceGuard guard(pool->device());
+  at::Tensor out = at::empty({c.tokens, c.heads, c.d}, q->options());
+  const size_t need = p_mass_workspace((int)c.seqs, c.tokens, (int)c.most, c.keys, (int)c.heads,
+                                       (int)c.hkv, (int)c.d, (int)c.bs);
+  at::Tensor ws = at::empty({(int64_t)need}, q->options().dtype(at::kByte));
+  void *const outp = out.data_ptr(), *const wsp = ws.data_ptr();
+  const ndl_stream_t s = stream_of(*pool);
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = p_attention_mass(outp, (float*)mass->data_ptr(), q->data_ptr(), c.qs, pool->data_ptr(),
+                        c.num_blocks, (const int32_t*)table->data_ptr(), table->stride(0),
+                        (int)c.width, cu ? (const int32_t*)cu->data_ptr() : nullptr,
+                        (const int32_t*)lens->data_ptr(), (int)c.seqs, c.tokens, (int)c.most,
+                        c.keys, (int)c.heads, (int)c.hkv, (int)c.d, (int)c.bs,
+                        dtype_code(q->scalar_type()), c.scale, decay, wsp, need, s);
+  Py_END_ALLOW_THREADS
+  if (rc != NDL_OK) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// verify_tree(logits, ids, parents, cu_seqlens, uniforms, temperature or None): (tokens, accepted,
+// path).
+PyObject* verify_tree(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 6 || p_verify_tree == nullptr) Py_RETURN_NONE;
+  const at::Tensor *t[5], *temp;
+  for (int i = 0; i < 5; ++i)
+    if ((t[i] = gpu_tensor(args[i])) == nullptr) Py_RETURN_NONE;
+  if (!maybe_tensor(args[5], &temp)) Py_RETURN_NONE;
+  const at::Tensor &logits = *t[0], &ids = *t[1], &parents = *t[2], &cu = *t[3], &u = *t[4];
+  const int code = dtype_code(logits.scalar_type());
+  if (code < 0 || logits.dim() != 2 || ids.dim() != 1 || !ids.is_contiguous() ||
+      (ids.scalar_type() != at::kInt && ids.scalar_type() != at::kLong) ||
+      ids.device() != logits.device() || !read_int32(cu, logits, 1) ||
+      !read_int32(parents, logits, 1) || u.dim() != 1 || u.scalar_type() != at::kFloat ||
+      !u.is_contiguous() || u.device() != logits.device())
+    Py_RETURN_NONE;
+  const int64_t rows = logits.size(0), vocab = logits.size(1), seqs = cu.size(0) - 1;
+  if (rows == 0 || vocab == 0 || vocab > 0x7fffffff || seqs <= 0 || rows < seqs ||
+      ids.size(0) != rows || parents.size(0) != rows || u.size(0) != rows ||
+      logits.stride(1) != 1 || (rows > 1 && logits.stride(0) < vocab))
+    Py_RETURN_NONE;
+  if (temp != nullptr && (temp->dim() != 1 || temp->size(0) != seqs || !temp->is_contiguous() ||
+                          temp->scalar_type() != at::kFloat || temp->device() != logits.device()))
+    Py_RETURN_NONE;
+  const c10::DeviceGuard guard(logits.device());
+  at::Tensor tokens = at::empty_like(ids), accepted = at::empty({seqs}, cu.options()),
+             path = at::empty({rows}, cu.options());
+  const size_t need = p_verify_tree_workspace(rows, (int)seqs, (int)vocab);
+  at::Tensor ws = at::empty({(int64_t)need}, cu.options().dtype(at::kByte));
+  void *const tp = tokens.data_ptr(), *const wsp = ws.data_ptr();
+  int32_t *const ap = (int32_t*)accepted.data_ptr(), *const pp = (int32_t*)path.data_ptr();
+  const ndl_stream_t s = stream_of(logits);
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = p_verify_tree(tp, ap, pp, logits.data_ptr(), rows > 1 ? logits.stride(0) : vocab, code,
+                     ids.data_ptr(), ids.scalar_type() == at::kLong,
+                     (const int32_t*)parents.data_ptr(), (const int32_t*)cu.data_ptr(),
+                     (const float*)u.data_ptr(), temp ? (const float*)temp->data_ptr() : nullptr,
+                     rows, (int)seqs, (int)vocab, wsp, need, s);
+  Py_END_ALLOW_THREADS
+  if (rc != NDL_OK) Py_RETURN_NONE;
+  PyObject* const out = PyTuple_New(3);
+  if (out == nullptr) return nullptr;
+  at::Tensor* const parts[3] = {&tokens, &accepted, &path};
+  for (int i = 0; i < 3; ++i) {
+    PyObject* const o = THPVariable_Wrap(std::move(*parts[i]));
+    if (o == nullptr) {
+      Py_DECREF(out);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(out, i, o);
+  }
+  return out;
+  END_HANDLE_TH_ERRORS
+}
+
+// kv_select(mass, block_table, lens, budget, sinks, recent): (keep, kept).
+PyObject* kv_select(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 6 || p_kv_select == nullptr || validating()) Py_RETURN_NONE;
+  const at::Tensor *const mass = gpu_tensor(args[0]), *const table = gpu_tensor(args[1]),
+                   *const lens = gpu_tensor(args[2]);
+  int64_t budget, sinks, recent;
+  if (!mass || !table || !lens || !read_int(args[3], &budget) || !read_int(args[4], &sinks) ||
+      !read_int(args[5], &recent) || budget == 0 || sinks + recent > budget ||
+      mass->scalar_type() != at::kFloat || mass->dim() != 3 || !mass->is_contiguous() ||
+      !read_int32(*table, *mass, 2) || !read_int32(*lens, *mass, 1))
+    Py_RETURN_NONE;
+  const int64_t seqs = table->size(0), width = table->size(1), hkv = mass->size(1);
+  if (seqs == 0 || width == 0 || lens->size(0) != seqs || !fits_int(seqs) || !fits_int(width) ||
+      !fits_int(hkv) || !fits_int(mass->size(2)) || mass->numel() == 0)
+    Py_RETURN_NONE;
+  const c10::DeviceGuard guard(mass->device());
+  at::Tensor keep = at::empty({seqs, hkv, budget}, table->options());
+  at::Tensor kept = at::empty({seqs}, table->options());
+  int32_t *const kp = (int32_t*)keep.data_ptr(), *const np = (int32_t*)kept.data_ptr();
+  const ndl_stream_t s = stream_of(*mass);
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = p_kv_select(kp, np, (const float*)mass->data_ptr(), mass->size(0), (int)hkv,
+                   (int)mass->size(2), (const int32_t*)table->data_ptr(), table->stride(0),
+                   (int)width, (const int32_t*)lens->data_ptr(), (int)seqs, (int)budget,
+                   (int)sinks, (int)recent, s);
+  Py_END_ALLOW_THREADS
+  if (rc != NDL_OK) Py_RETURN_NONE;
+  return tensor_pair(std::move(keep), std::move(kept));
+  END_HANDLE_TH_ERRORS
+}
+
+// kv_compact(list of pools (or codes), list of scales or None, block_table, keep, counts, first or
+// None, cu_seqlens or None, dst_table or None, mass or None).  True when launched.
+PyObject* kv_compact(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 9 || p_kv_compact == nullptr || validating() || !PyList_CheckExact(args[0]))
+    Py_RETURN_NONE;
+  const bool fp8 = args[1] != Py_None;
+  const Py_ssize_t layers = PyList_GET_SIZE(args[0]);
+  if (layers == 0 || layers > 128 ||
+      (fp8 && (!PyList_CheckExact(args[1]) || PyList_GET_SIZE(args[1]) != layers)))
+    Py_RETURN_NONE;
+  void *pools[128], *scales[128];
+  const at::Tensor* pool = nullptr;
+  for (Py_ssize_t i = 0; i < layers; ++i) {
+    const at::Tensor* const x = gpu_tensor(PyList_GET_ITEM(args[0], i));
+    if (x == nullptr) Py_RETURN_NONE;
+    Cache c16;
+    Fp8Pool c8;
+    if (fp8) {
+      const at::Tensor* const y = gpu_tensor(PyList_GET_ITEM(args[1], i));
+      if (y == nullptr || !read_fp8_pool(*x, *y, &c8)) Py_RETURN_NONE;
+      scales[i] = y->data_ptr();
+    } else if (!read_cache(*x, &c16) || (pool && x->scalar_type() != pool->scalar_type())) {
+      Py_RETURN_NONE;
+    }
+    if (pool == nullptr) pool = x;
+    if (x->sizes() != pool->sizes() || x->device() != pool->device()) Py_RETURN_NONE;
+    pools[i] = x->data_ptr();
+  }
+  const at::Tensor *const table = gpu_tensor(args[2]), *const keep = gpu_tensor(args[3]),
+                   *const counts = gpu_tensor(args[4]), *first, *cu, *dst, *mass;
+  if (!table || !keep || !counts || !maybe_tensor(args[5], &first) ||
+      !maybe_tensor(args[6], &cu) || !maybe_tensor(args[7], &dst) || !maybe_tensor(args[8], &mass))
+    Py_RETURN_NONE;
+  const int64_t hkv = pool->size(2), bs = pool->size(3);
+  const int64_t row = pool->size(4) * (int64_t)pool->element_size();
+  if (!read_int32(*table, *pool, 2) || !read_int32(*counts, *pool, 1) ||
+      !read_int32(*keep, *pool, cu ? 1 : 3) || (cu && !read_int32(*cu, *pool, 1)) ||
+      (first && !read_int32(*first, *pool, 1)) || (dst && !read_int32(*dst, *pool, 2)) ||
+      (mass && !read_mass(*mass, *pool)))
+    Py_RETURN_NONE;
+  const int64_t seqs = table->size(0), width = table->size(1);
+  if (seqs == 0 || width == 0 || keep->numel() == 0 || !fits_int(seqs) || !fits_int(width) ||
+      !fits_int(hkv) || !fits_int(bs) || row % 16 || !fits_int(row) || counts->size(0) != seqs ||
+      (first && first->size(0) != seqs) || (dst && (dst->size(0) != seqs || dst->size(1) == 0)) ||
+      (cu ? cu->size(0) != seqs + 1
+          : keep->size(0) != seqs || keep->size(1) != hkv || !keep->is_contiguous() ||
+                !fits_int(keep->size(2))))
+    Py_RETURN_NONE;
+  const c10::DeviceGuard guard(pool->device());
+  const ndl_stream_t s = stream_of(*pool);
+  auto ints = [](const at::Tensor* x) { return x ? (const int32_t*)x->data_ptr() : nullptr; };
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = p_kv_compact(pools, fp8 ? scales : nullptr, (int)layers,
+                    mass ? (float*)mass->data_ptr() : nullptr, pool->size(1), (int)hkv, (int)bs,
+                    (int)row, ints(table), table->stride(0), (int)width, ints(dst),
+                    dst ? dst->stride(0) : 0, dst ? (int)dst->size(1) : 0, ints(keep),
+                    cu ? 0 : (int)keep->size(2), ints(cu), keep->numel(), ints(first),
+                    ints(counts), (int)seqs, s);
+  Py_END_ALLOW_THREADS
+  if (rc != NDL_OK) Py_RETURN_NONE;
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
 // init({name: address}): the entry points to call.
 PyObject* init(PyObject*, PyObject* d) {
   auto get = [&](const char* name) -> void* {
@@ -576,6 +901,17 @@ PyObject* init(PyObject*, PyObject* d) {
   NDL_TAKE(p_fp8_decode_append, "ndl_fp8_decode_append");
   NDL_TAKE(p_verify_workspace, "ndl_verify_drafts_workspace_bytes");
   NDL_TAKE(p_verify_drafts, "ndl_verify_drafts");
+  NDL_TAKE(p_tree_mask, "ndl_tree_mask");
+  NDL_TAKE(p_tree_workspace, "ndl_tree_attention_workspace_bytes");
+  NDL_TAKE(p_tree_attention, "ndl_tree_attention");
+  NDL_TAKE(p_fp8_tree_workspace, "ndl_fp8_tree_attention_workspace_bytes");
+  NDL_TAKE(p_fp8_tree_attention, "ndl_fp8_tree_attention");
+  NDL_TAKE(p_verify_tree_workspace, "ndl_verify_tree_workspace_bytes");
+  NDL_TAKE(p_verify_tree, "ndl_verify_tree");
+  NDL_TAKE(p_mass_workspace, "ndl_attention_mass_workspace_bytes");
+  NDL_TAKE(p_attention_mass, "ndl_attention_mass");
+  NDL_TAKE(p_kv_compact, "ndl_kv_compact");
+  NDL_TAKE(p_kv_select, "ndl_kv_select");
 #undef NDL_TAKE
   Py_RETURN_NONE;
 }
@@ -590,6 +926,12 @@ PyMethodDef methods[] = {
     {"kv_read_fp8", (PyCFunction)(void (*)(void))kv_read_fp8, METH_FASTCALL, nullptr},
     {"fp8_attention", (PyCFunction)(void (*)(void))fp8_attention, METH_FASTCALL, nullptr},
     {"verify_drafts", (PyCFunction)(void (*)(void))verify_drafts, METH_FASTCALL, nullptr},
+    {"tree_mask", (PyCFunction)(void (*)(void))tree_mask, METH_FASTCALL, nullptr},
+    {"tree_attention", (PyCFunction)(void (*)(void))tree_attention, METH_FASTCALL, nullptr},
+    {"attention_mass", (PyCFunction)(void (*)(void))attention_mass, METH_FASTCALL, nullptr},
+    {"verify_tree", (PyCFunction)(void (*)(void))verify_tree, METH_FASTCALL, nullptr},
+    {"kv_select", (PyCFunction)(void (*)(void))kv_select, METH_FASTCALL, nullptr},
+    {"kv_compact", (PyCFunction)(void (*)(void))kv_compact, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods,

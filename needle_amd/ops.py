@@ -1175,12 +1175,17 @@ def tree_mask(parents: torch.Tensor, cu_seqlens: torch.Tensor, max_seqlen: int):
     b // 64 is set for the token itself and its ancestors; depth counts the ancestors, so that
     context_lens[i] + depth is the token's position for the rotary embedding.  max_seqlen bounds a
     sequence's tokens.  Rows outside cu_seqlens hold nothing in particular."""
+    if _lib.NATIVE is not None:
+        done = _lib.NATIVE.tree_mask(parents, cu_seqlens, max_seqlen)
+        if done is not None:
+            return done
     _require(parents.is_cuda, "parents must be a GPU tensor")
     dev = parents.device
     _check_int32("parents", parents, 1, dev)
     _check_int32("cu_seqlens", cu_seqlens, 1, dev)
     n_seqs, n_tok = cu_seqlens.shape[0] - 1, parents.shape[0]
     _require(n_seqs >= 0, "cu_seqlens must be [num_seqs + 1]")
+    max_seqlen = int(max_seqlen)
     _require(max_seqlen > 0, "max_seqlen must be positive")
     words = (max_seqlen + 63) // 64
     mask = torch.empty((n_tok, words), dtype=torch.int64, device=dev)
@@ -1239,6 +1244,13 @@ def tree_attention(q: torch.Tensor, kv_cache, block_table: torch.Tensor,
     attends nothing gets zeros.  max_seqlen bounds a sequence's tokens, max_context_len its cached
     ones (0: not known, the table's width then): sequences past these bounds are not attended
     whole."""
+    if out is None and workspace is None and _lib.NATIVE is not None:
+        pool, scales = kv_cache if isinstance(kv_cache, Fp8KVCache) else (kv_cache, None)
+        out = _lib.NATIVE.tree_attention(q, pool, scales, block_table, cu_seqlens, context_lens,
+                                         mask, max_seqlen, max_context_len, scale, num_heads,
+                                         num_kv_heads, head_dim)
+        if out is not None:
+            return out
     pool = kv_cache.codes if isinstance(kv_cache, Fp8KVCache) else kv_cache
     _check_cache(pool) if pool is kv_cache else _check_fp8_cache(*kv_cache)
     dev = pool.device
@@ -1269,6 +1281,7 @@ def tree_attention(q: torch.Tensor, kv_cache, block_table: torch.Tensor,
         return out
     w = block_table.shape[1]
     _require(w > 0, "block_table has no columns")
+    max_seqlen, max_context_len = int(max_seqlen), int(max_context_len)
     _require(max_seqlen > 0, "max_seqlen must be positive")
     _require(max_context_len >= 0, "max_context_len is negative")
     max_keys = min(w * bs, max_context_len + max_seqlen) if max_context_len else w * bs
@@ -1314,6 +1327,10 @@ def verify_tree(logits: torch.Tensor, ids: torch.Tensor, parents: torch.Tensor,
     accepted: how many the path has; path: its nodes, 0 among them, then -1 (kv_compact moves their
     rows together).  Rows outside cu_seqlens hold nothing in particular.  Graph-capturable; no host
     synchronisation."""
+    if _lib.NATIVE is not None:
+        done = _lib.NATIVE.verify_tree(logits, ids, parents, cu_seqlens, uniforms, temperature)
+        if done is not None:
+            return done
     dev, rows, vocab, n_seqs = _check_verify(logits, ids, cu_seqlens, uniforms, temperature)
     _check_int32("parents", parents, 1, dev)
     _require(parents.shape[0] == rows, "logits and parents differ in rows")
@@ -1379,6 +1396,12 @@ def attention_mass(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.T
     max_context_len its cached ones (0: not known, the table's width then).  decay 0 forgets what
     was there.  No two sequences may attend one block.  workspace: as decode_workspace gives, of
     attention_mass_workspace_bytes, for one call at a time."""
+    if out is None and workspace is None and _lib.NATIVE is not None:
+        out = _lib.NATIVE.attention_mass(q, kv_cache, block_table, cu_seqlens, context_lens, mass,
+                                         max_seqlen, max_context_len, scale, num_heads,
+                                         num_kv_heads, head_dim, decay)
+        if out is not None:
+            return out
     _check_cache(kv_cache)
     dev = kv_cache.device
     _, nb, hkv, bs, d = kv_cache.shape
@@ -1403,6 +1426,7 @@ def attention_mass(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.T
         return out
     w = block_table.shape[1]
     _require(w > 0, "block_table has no columns")
+    max_seqlen, max_context_len = int(max_seqlen), int(max_context_len)
     _require(max_seqlen > 0, "max_seqlen must be positive")
     _require(max_context_len >= 0, "max_context_len is negative")
     max_keys = min(w * bs, max_context_len + max_seqlen) if max_context_len else w * bs
@@ -1445,9 +1469,16 @@ def kv_compact(pools, block_table: torch.Tensor, keep: torch.Tensor, counts: tor
     pools = list(pools)
     _require(len(pools) > 0, "no pools given")
     fp8 = isinstance(pools[0], Fp8KVCache)
+    if not fp8 and _lib.NATIVE is not None and _lib.NATIVE.kv_compact(
+            pools, None, block_table, keep, counts, first, cu_seqlens, dst_table, mass):
+        return
     _require(all(isinstance(p, Fp8KVCache) == fp8 for p in pools),
              "16-bit and 8-bit pools cannot be mixed", TypeError)
     main = [p.codes if fp8 else p for p in pools]
+    if fp8 and _lib.NATIVE is not None and _lib.NATIVE.kv_compact(
+            main, [p.scales for p in pools], block_table, keep, counts, first, cu_seqlens,
+            dst_table, mass):
+        return
     shape, dtype, dev = main[0].shape, main[0].dtype, main[0].device
     for p, x in zip(pools, main):
         _check_fp8_cache(*p) if fp8 else _check_cache(p)
@@ -1503,6 +1534,10 @@ def kv_select(mass: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor,
     tokens.  Of a sequence of more than budget tokens the first `sinks` and the last `recent` stay
     (at most budget together), and of those between the ones with the largest weights, of equal ones
     the first.  A NaN counts as the largest weight."""
+    if _lib.NATIVE is not None:
+        done = _lib.NATIVE.kv_select(mass, block_table, lens, budget, sinks, recent)
+        if done is not None:
+            return done
     if mass.dim() != 3:
         raise ValueError(f"mass must be [num_blocks, num_kv_heads, block_size], got "
                          f"{tuple(mass.shape)}")
@@ -1513,6 +1548,7 @@ def kv_select(mass: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor,
     n_seqs = _check_table(block_table, nb, dev)
     _check_int32("lens", lens, 1, dev)
     _require(lens.shape[0] == n_seqs, "lens/block_table batch mismatch")
+    budget, sinks, recent = int(budget), int(sinks), int(recent)
     _require(budget > 0, "budget must be positive")
     _require(sinks >= 0 and recent >= 0 and sinks + recent <= budget,
              f"sinks {sinks} and recent {recent} must be within the budget {budget}")
