@@ -176,24 +176,25 @@ struct Stream {
   }
 };
 
-// One workgroup per (row block, kv head, kMergeCols columns): the parts that the shares hold,
+// One workgroup per (row block, kv head, COLS columns): the parts that the shares hold,
 // combined in their order; zeros for tokens with nothing to attend.  A row block inside one share
 // was written by the attention.  put(row block, head, column, head_dim, outputs, maximum, sum).
 constexpr int kMergeCols = 8;
 constexpr int kMergeParts = 64;   // at a time
 
-template <int D, bool TREE, class PUT>
+template <int D, bool TREE, int COLS = kMergeCols, class PUT>
 __device__ __forceinline__ void merge_row_block(const RowBlocks& a, int group, PUT put) {
-  constexpr int PER = kMergeCols * D / 256;       // consecutive outputs of a thread: 4 or 2
-  __shared__ float2 part[kMergeParts][kMergeCols];
+  constexpr int PER = COLS * D / 256;             // consecutive outputs of a thread
+  constexpr int UNROLL = PER <= 4 ? 8 : 2;        // parts whose loads are under way
+  __shared__ float2 part[kMergeParts][COLS];
   const int t = threadIdx.x, lane = t & 63;
-  const int e = blockIdx.x, head = blockIdx.y, c0 = blockIdx.z * kMergeCols;
+  const int e = blockIdx.x, head = blockIdx.y, c0 = blockIdx.z * COLS;
   const Item it = item_of<TREE>(a, e);
   Stream<TREE> st;
   st.read(a, lane);
   const Place p = st.find(a, lane, 0, e);
   if (it.n <= 0 || c0 >= it.n * group) return;
-  const int cols = it.n * group - c0 < kMergeCols ? it.n * group - c0 : kMergeCols;
+  const int cols = it.n * group - c0 < COLS ? it.n * group - c0 : COLS;
   const int c = t * PER / D, d0 = t * PER - c * D;
   float o[PER];
 #pragma unroll
@@ -215,10 +216,10 @@ __device__ __forceinline__ void merge_row_block(const RowBlocks& a, int group, P
         const int m = n - i0 < kMergeParts ? n - i0 : kMergeParts;
         if (pass == 0 || n > kMergeParts) {
           __syncthreads();
-          for (int i = t; i < m * kMergeCols; i += 256)
-            if (i % kMergeCols < cols)
-              part[i / kMergeCols][i % kMergeCols] =
-                  ml[(int64_t)(i0 + i / kMergeCols) * per + i % kMergeCols];
+          for (int i = t; i < m * COLS; i += 256)
+            if (i % COLS < cols)
+              part[i / COLS][i % COLS] =
+                  ml[(int64_t)(i0 + i / COLS) * per + i % COLS];
           __syncthreads();
         }
         if (c >= cols) continue;
@@ -226,15 +227,18 @@ __device__ __forceinline__ void merge_row_block(const RowBlocks& a, int group, P
           for (int i = 0; i < m; ++i) mx = fmaxf(mx, part[i][c].x);
           continue;
         }
-        for (int i = 0; i < m; i += 8) {
-          float v[8][PER];
+        for (int i = 0; i < m; i += UNROLL) {
+          float v[UNROLL][PER];
 #pragma unroll
-          for (int y = 0; y < 8; ++y) {
+          for (int y = 0; y < UNROLL; ++y) {
             const float* const q = src + (int64_t)(i0 + (i + y < m ? i + y : i)) * step;
-            if constexpr (PER == 4) {
-              const f32x4 w = *reinterpret_cast<const f32x4*>(q);
+            if constexpr (PER >= 4) {
 #pragma unroll
-              for (int x = 0; x < PER; ++x) v[y][x] = w[x];
+              for (int z = 0; z < PER; z += 4) {
+                const f32x4 w = *reinterpret_cast<const f32x4*>(q + z);
+#pragma unroll
+                for (int x = 0; x < 4; ++x) v[y][z + x] = w[x];
+              }
             } else {
               const f32x2 w = *reinterpret_cast<const f32x2*>(q);
               v[y][0] = w[0];
@@ -242,7 +246,7 @@ __device__ __forceinline__ void merge_row_block(const RowBlocks& a, int group, P
             }
           }
 #pragma unroll
-          for (int y = 0; y < 8; ++y) {
+          for (int y = 0; y < UNROLL; ++y) {
             if (i + y >= m) break;
             const float2 ms = part[i + y][c];
             const float f = ms.x == mx ? 1.f : fast_exp2(ms.x - mx);

@@ -58,13 +58,13 @@ struct TreeOperands {
 };
 struct TreeArgs : TreeOperands, RowBlocks {};
 
-constexpr int kWaves = 4;
-constexpr int kStages = 4;      // of the ring, over all groups
+constexpr int kWaves = 8;
 
 template <int D>
 struct TreeShape {
   static constexpr int kPlane = kTile * D * 2;             // bytes of a tile's K (or V)
   static constexpr int kStage = 2 * kPlane;
+  static constexpr int kStages = (128 << 10) / kStage;     // of the ring, over all groups
   static constexpr int kPieces = kPlane / 1024;            // loads of a plane
   static constexpr int kRing = kStages * kStage;
   static constexpr int kSums = kWaves * 32 * D * 4;        // the waves' partial outputs
@@ -100,7 +100,7 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
   return ((w & inf) == inf ? 0xffffu : 0u) | ((w >> 16 & inf) == inf ? 0xffff0000u : 0u);
 }
 
-// A workgroup's share of the row blocks of one kv head.  Its four waves are as many groups of columns
+// A workgroup's share of the row blocks of one kv head.  Its eight waves are as many groups of columns
 // (CG) side by side as a row block has columns for, times as many groups of keys (KG) as are left.
 template <int D, bool F16, Chunk KIND>
 __global__ __launch_bounds__(64 * kWaves, 2) void tree_attention_kernel(TreeArgs a) {
@@ -158,7 +158,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_attention_kernel(TreeArgs
     const int cols = it.n * a.group;
 
     auto row_block = [&](auto groups) {
-      constexpr int CG = decltype(groups)::value, KG = NW / CG, NS = kStages / KG;
+      constexpr int CG = decltype(groups)::value, KG = NW / CG, NS = S::kStages / KG;
       constexpr int LOADS = 2 * S::kPieces / CG;       // of a wave, per stage
       constexpr int AHEAD = CG == 1 ? NS : NS - 1;     // stages in flight when a step begins
       static_assert(LOADS >= 1 && AHEAD * LOADS < 64, "loads of a wave");
@@ -226,7 +226,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_attention_kernel(TreeArgs
       const uint32_t src_row = (uint32_t)(lane / CPR) * (2 * D);
       const uint32_t src_k = src_row + 16u * ((lane % CPR) ^ k_swizzle<D>(lane / CPR));
       const uint32_t src_v = src_row + 16u * ((lane % CPR) ^ v_swizzle(lane / CPR));
-      // What a wave loads of a stage: all (CG 1), K or V (2), half of K or of V (4).
+      // What a wave loads of a stage: all (CG 1), K or V (2), half of K or of V (4), a quarter (8).
       const bool cg_v = 2 * cg / CG;
       const char* const my_plane = reinterpret_cast<const char*>(CG > 1 && cg_v ? a.vplane : a.kplane);
       const uint32_t my_src = cg_v ? src_v : src_k;
@@ -240,20 +240,21 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_attention_kernel(TreeArgs
         uint32_t off = my_src, off_v = src_v;
         asm volatile("" : "+v"(off), "+v"(off_v));   // (a load's own offset: no register over the loop)
 #pragma unroll
-        for (int s = 0; s < (CG == 4 ? 1 : 2); ++s) {
-          const int half = CG == 4 ? cg & 1 : s;
+        for (int s = 0; s < (CG >= 4 ? 1 : 2); ++s) {
+          const int half = CG == 4 ? cg & 1 : CG == 8 ? (cg >> 1) & 1 : s;
           const uint64_t at =
               (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)window, 2 * (u & 31) + half) *
               (32 * D);
 #pragma unroll
-          for (int x = 0; x < S::kPieces / 2; ++x) {
+          for (int y = 0; y < (CG == 8 ? S::kPieces / 4 : S::kPieces / 2); ++y) {
+            const int x = CG == 8 ? (cg & 1) * (S::kPieces / 4) + y : y;
             const uint32_t to = st + (uint32_t)(half * S::kPieces / 2 + x) * 1024;
             // (k_swizzle of a load's first row: the same in both halves)
             const uint32_t turn = 16u * k_swizzle<D>(x * RPL);
             if constexpr (CG == 1) {
-              lds_dma16(my_plane + at + 1024 * x, off ^ turn, to);
-              lds_dma16(reinterpret_cast<const char*>(a.vplane) + at + 1024 * x, off_v,
-                        to + S::kPlane);
+              lds_dma16_nt(my_plane + at + 1024 * x, off ^ turn, to);
+              lds_dma16_nt(reinterpret_cast<const char*>(a.vplane) + at + 1024 * x, off_v,
+                           to + S::kPlane);
             } else {
               lds_dma16(my_plane + at + 1024 * x, cg_v ? off : off ^ turn,
                         cg_v ? to + S::kPlane : to);
@@ -267,9 +268,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_attention_kernel(TreeArgs
       // What was loaded so far arrives here: the compiler's own waits in the loop would drain the
       // ring, whose loads it does not see, at every step.
       asm volatile("" : "+v"(window));
-#pragma unroll
-      for (int d = 0; d < AHEAD; ++d)
-        if (d < cnt) issue(d, d);
+#pragma unroll 1
+      for (int d = 0; d < AHEAD && d < cnt; ++d) issue(d, d);
 #pragma unroll
       for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(q[s]));
 
@@ -575,27 +575,30 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_attention_kernel(TreeArgs
         row_block(std::integral_constant<int, 1>{});
       else if (cols <= 64)
         row_block(std::integral_constant<int, 2>{});
-      else
+      else if (cols <= 128)
         row_block(std::integral_constant<int, 4>{});
+      else
+        row_block(std::integral_constant<int, 8>{});
     }
     if (whole) return;
     __syncthreads();     // before the ring is written again
   }
 }
 
+constexpr int kJoinCols = 32;     // of a workgroup of the merge
 template <int D, bool F16, bool TREE>
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
   using T = Elt<F16>;
-  merge_row_block<D, TREE>(a, a.group, [&](const Item& it, int head, int col, int d0,
-                                           const float* o, float m, float l) {
-    constexpr int PER = kMergeCols * D / 256;
+  merge_row_block<D, TREE, kJoinCols>(a, a.group, [&](const Item& it, int head, int col, int d0,
+                                                      const float* o, float m, float l) {
+    constexpr int PER = kJoinCols * D / 256;
     const int tok = col / a.group;
     const int64_t row = (it.tok0 + tok) * a.num_heads + head * a.group + col - tok * a.group;
     u16* const dst = a.out + row * D + d0;
-    if constexpr (PER == 4)
-      *reinterpret_cast<u32x2*>(dst) = u32x2{T::pack(o[0], o[1]), T::pack(o[2], o[3])};
-    else
-      *reinterpret_cast<uint32_t*>(dst) = T::pack(o[0], o[1]);
+#pragma unroll
+    for (int x = 0; x < PER; x += 8)
+      st16(dst + x, u32x4{T::pack(o[x], o[x + 1]), T::pack(o[x + 2], o[x + 3]),
+                          T::pack(o[x + 4], o[x + 5]), T::pack(o[x + 6], o[x + 7])});
     if (d0 == 0 && a.lse != nullptr) a.lse[row] = m + __log2f(l);
   });
 }
@@ -645,8 +648,12 @@ Plan plan_for(const ChunkAttention& c) {
     units = p.items * c.num_kv_heads;
     if (units * 2 > res) break;
   }
+  // Whole row blocks where there are enough to even out: of wide ones two for each place (their parts
+  // are large: 64 trees of 16 .. 64 nodes after up to 4,096 tokens, 32 heads on 8: 164 us whole, 178
+  // in shares), of narrow ones four (those sequences' last tokens and their weights: 125 us in shares,
+  // 139 whole).
   // (slots and segments are counted in 31 bits)
-  const bool whole = tiles <= kWholeTiles || units >= res ||
+  const bool whole = tiles <= kWholeTiles || units >= (p.toks * group > 32 ? 2 : 4) * res ||
                      p.items * (tiles + kPad) + 2 * res * kMinChunk > 0x40000000;
   if (!whole) {
     int64_t s = res / c.num_kv_heads / 8 * 8;
@@ -806,7 +813,7 @@ int launch_chunk_attention(const ChunkAttention& call, void* workspace, size_t w
   }
   const int rc = check_launch();
   if (rc != NDL_OK || a.shares == 0) return rc;
-  const int groups = (a.toks * a.group + kMergeCols - 1) / kMergeCols;
+  const int groups = (a.toks * a.group + kJoinCols - 1) / kJoinCols;
   const dim3 grid((unsigned)a.items, (unsigned)a.num_kv_heads, (unsigned)groups);
   const bool f16 = dtype_is_f16(c.dtype), tree = c.mask != nullptr;
   if (c.head_dim == 128) {
