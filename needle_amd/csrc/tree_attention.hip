@@ -638,7 +638,8 @@ Plan plan_for(const ChunkAttention& c) {
   int64_t res = resident_workgroups(kernel_for(c.head_dim, false, kTree), 64 * kWaves);
   if (res <= 0) res = 256;
   const int64_t tiles = (c.max_keys + kTile - 1) / kTile;
-  // Columns of a row block: as few as leave no part of the GPU idle.
+  // Columns of a row block: all that the kernel takes, or, where row blocks are whole, as few as leave
+  // no part of the GPU idle.
   int64_t units = 0;
   for (int cols = 32 * kWaves; cols >= 32; cols /= 2) {
     if (cols > 32 && (int64_t)c.max_seqlen * group <= cols / 2) continue;
@@ -646,7 +647,7 @@ Plan plan_for(const ChunkAttention& c) {
     p.blocks_per_seq = (c.max_seqlen + p.toks - 1) / p.toks;
     p.items = c.num_seqs * p.blocks_per_seq;
     units = p.items * c.num_kv_heads;
-    if (units * 2 > res) break;
+    if (units * 2 > res || tiles > kWholeTiles) break;
   }
   // Whole row blocks where there are enough to even out: of wide ones two for each place (their parts
   // are large: 64 trees of 16 .. 64 nodes after up to 4,096 tokens, 32 heads on 8: 164 us whole, 178
