@@ -14,7 +14,7 @@
 //     behind (4 bytes each, where K and V are 512 bytes a token at head_dim 128) and a pass over
 //     those takes the exponentials and sums.  us, scores kept / made again, see add_scores_kernel.
 //   * More: the scores are made again, from K alone: the columns' Q in LDS in operand layout, a wave's
-//     64 keys in registers for all columns, the sum over columns kept in the accumulator layout and
+//     32 keys in registers for all columns, the sum over columns kept in the accumulator layout and
 //     joined across lanes once, at the end.
 // Sums run in a fixed order, without atomics; a key's number is written by one lane.
 #include "fp8.hpp"
@@ -24,10 +24,10 @@ namespace ndl {
 namespace {
 
 constexpr int kKeys = 32;             // of a tile
-constexpr int kTiles = 2;             // of a wave
-constexpr int kMassWaves = 4;
+constexpr int kTiles = 1;             // of a wave
+constexpr int kMassWaves = 8;
 constexpr int kMassKeys = kMassWaves * kTiles * kKeys;      // of a workgroup
-constexpr int kGroups = 8;            // 32-column groups in LDS at a time
+constexpr int kGroups = 4;            // 32-column groups in LDS at a time
 
 struct MassArgs {
   float* mass;
@@ -110,6 +110,15 @@ __global__ __launch_bounds__(256) void add_scores_kernel(MassArgs a) {
   add_to(a, at, x, c.ctx, sum);
 }
 
+template <int M>
+__device__ __forceinline__ void halve(float* a, int lane) {
+  const bool up = lane & M;
+#pragma unroll
+  for (int r = 0; r < M; ++r) {
+    const float keep = up ? a[r + M] : a[r], give = up ? a[r] : a[r + M];
+    a[r] = keep + __shfl_xor(give, M, 64);
+  }
+}
 // v[r] summed over the lanes of its half (r: key 8 (r / 4) + 4 h + r % 4): the number of key
 // `lane & 31` in lanes 0 to 31.  Halves of the registers change hands at each step, so that 16 sums
 // take 16 exchanges.
@@ -118,14 +127,10 @@ __device__ __forceinline__ float sums_by_key(const f32x16& v, int lane) {
 #pragma unroll
   for (int r = 0; r < 16; ++r) a[r] = v[r];
   // after the steps lane bits 3, 2, 1, 0 hold the bits of r that they took
-#pragma unroll
-  for (int m = 8; m >= 1; m >>= 1)
-#pragma unroll
-    for (int r = 0; r < m; ++r) {
-      const bool up = lane & m;
-      const float keep = up ? a[r + m] : a[r], give = up ? a[r] : a[r + m];
-      a[r] = keep + __shfl_xor(give, m, 64);
-    }
+  halve<8>(a, lane);
+  halve<4>(a, lane);
+  halve<2>(a, lane);
+  halve<1>(a, lane);
   const float s = a[0] + __shfl_xor(a[0], 16, 64);       // of r = lane & 15, half lane >> 5
   // key k is r = 4 (k >> 3) + (k & 3) of half (k >> 2) & 1
   const int k = lane & 31;
@@ -195,11 +200,17 @@ __global__ __launch_bounds__(64 * kMassWaves) void add_weights_kernel(MassArgs a
         f32x16 sc = {};
 #pragma unroll
         for (int s = 0; s < KS; ++s) sc = T::mfma32x32x16(k[i][s], q[s], sc);
-        const int left = lim - (x0 + kKeys * i + 4 * h);
+        const int first = x0 + kKeys * i;
+        if (first + kKeys <= c.ctx && 32 * (g + 1) <= here) {     // every column attends every key
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float p = fast_exp2(fmaf(sc[r], a.scale_log2, -lse));
-          sum[i][r] += 8 * (r >> 2) + (r & 3) < left ? p : 0.f;
+          for (int r = 0; r < 16; ++r) sum[i][r] += fast_exp2(fmaf(sc[r], a.scale_log2, -lse));
+        } else {
+          const int left = lim - (first + 4 * h);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const float p = fast_exp2(fmaf(sc[r], a.scale_log2, -lse));
+            sum[i][r] += 8 * (r >> 2) + (r & 3) < left ? p : 0.f;
+          }
         }
       }
     }
@@ -346,14 +357,14 @@ extern "C" int ndl_attention_mass(void* out, float* mass, const void* q, int64_t
   const bool f16 = dtype_is_f16(dtype);
   if (head_dim == 128) {
     if (f16)
-      hipLaunchKernelGGL((add_weights_kernel<128, true>), grid, dim3(256), 0, s, a);
+      hipLaunchKernelGGL((add_weights_kernel<128, true>), grid, dim3(64 * kMassWaves), 0, s, a);
     else
-      hipLaunchKernelGGL((add_weights_kernel<128, false>), grid, dim3(256), 0, s, a);
+      hipLaunchKernelGGL((add_weights_kernel<128, false>), grid, dim3(64 * kMassWaves), 0, s, a);
   } else {
     if (f16)
-      hipLaunchKernelGGL((add_weights_kernel<64, true>), grid, dim3(256), 0, s, a);
+      hipLaunchKernelGGL((add_weights_kernel<64, true>), grid, dim3(64 * kMassWaves), 0, s, a);
     else
-      hipLaunchKernelGGL((add_weights_kernel<64, false>), grid, dim3(256), 0, s, a);
+      hipLaunchKernelGGL((add_weights_kernel<64, false>), grid, dim3(64 * kMassWaves), 0, s, a);
   }
   return check_launch();
 }
