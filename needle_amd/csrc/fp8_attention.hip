@@ -42,6 +42,7 @@
 #include "fp8.hpp"
 
 #include "chunk_stream.hpp"
+#include "tree_attention.hpp"
 
 namespace ndl {
 namespace {
@@ -1178,6 +1179,13 @@ extern "C" size_t ndl_fp8_attention_workspace_bytes(int num_seqs, int64_t num_to
 }
 
 // All entry points; `a` holds the new rows and the rotation of a decode step, or a tree's mask.
+// Trees of more columns than this have tree_attention.hip's row blocks of up to 256, where a key's codes
+// are unpacked once for all of them.
+constexpr int kWideColumns = 64;
+static bool wide_trees(const void* mask, int max_seqlen, int group) {
+  return mask != nullptr && (int64_t)max_seqlen * group > kWideColumns;
+}
+
 static int fp8_attention(ndl::ChunkArgs a, void* out, const void* q, int64_t q_tok_stride,
                          void* codes, void* scales, int64_t num_blocks,
                          const int32_t* block_table, int64_t bt_row_stride,
@@ -1240,6 +1248,34 @@ static int fp8_attention(ndl::ChunkArgs a, void* out, const void* q, int64_t q_t
                                            workspace, s)
                : launch_unpacked<64, false>(a, u, max_seqlen, max_keys, block_size, scale,
                                             workspace, s);
+  }
+  if (wide_trees(a.mask, max_seqlen, a.group)) {
+    ChunkAttention c{};
+    c.out = out;
+    c.q = q;
+    c.q_tok_stride = q_tok_stride;
+    c.kv_cache = codes;
+    c.scales = scales;
+    c.num_blocks = num_blocks;
+    c.block_table = block_table;
+    c.bt_row_stride = bt_row_stride;
+    c.max_blocks_per_seq = max_blocks_per_seq;
+    c.cu_seqlens = cu_seqlens;
+    c.context_lens = context_lens;
+    c.mask = a.mask;
+    c.mask_stride = a.mask_stride;
+    c.mask_words = a.words;
+    c.num_seqs = num_seqs;
+    c.num_tokens = num_tokens;
+    c.max_seqlen = max_seqlen;
+    c.max_keys = max_keys;
+    c.num_heads = num_heads;
+    c.num_kv_heads = num_kv_heads;
+    c.head_dim = head_dim;
+    c.block_size = block_size;
+    c.dtype = dtype;
+    c.scale = scale;
+    return launch_chunk_attention(c, workspace, workspace_bytes, s);
   }
   const Plan p = plan_for(num_seqs, max_seqlen, max_keys, num_heads, num_kv_heads, head_dim);
   if (p.items > 0x7fffff00) return NDL_ERR_INVALID_ARG;
@@ -1321,6 +1357,16 @@ extern "C" size_t ndl_fp8_tree_attention_workspace_bytes(int num_seqs, int max_s
   if (num_seqs <= 0 || max_seqlen <= 0 || max_keys <= 0 || max_keys > 0x7fffff00 ||
       !shape_ok(head_dim, block_size, num_heads, num_kv_heads))
     return 0;
+  if (wide_trees(&max_keys, max_seqlen, num_heads / num_kv_heads)) {
+    ChunkAttention c{};
+    c.num_seqs = num_seqs;
+    c.max_seqlen = max_seqlen;
+    c.max_keys = max_keys;
+    c.num_heads = num_heads;
+    c.num_kv_heads = num_kv_heads;
+    c.head_dim = head_dim;
+    return chunk_attention_workspace(c);
+  }
   const Plan p = plan_for(num_seqs, max_seqlen, max_keys, num_heads, num_kv_heads, head_dim);
   return p.ml_bytes + p.acc_bytes;
 }

@@ -54,12 +54,17 @@ struct TreeOperands {
   float* scores;                // [kv head][sequence][column][score_keys], scaled, log2
   int64_t score_keys;
   int score_cols;
+  const uint8_t* kscale;        // of an 8-bit pool, whose planes hold codes
+  const uint8_t* vscale;
   uint32_t q_flip, q_keep;      // of two elements of q: signs flipped (scale < 0), kept (scale not 0)
 };
 struct TreeArgs : TreeOperands, RowBlocks {};
 
 constexpr int kWaves = 8;
 
+// With an 8-bit pool (FP8) a wave unpacks the codes that it has loaded itself, up to kCodeDepth steps
+// ahead, into one of its group's two 16-bit stages.
+constexpr int kCodeDepth = 6;
 template <int D>
 struct TreeShape {
   static constexpr int kPlane = kTile * D * 2;             // bytes of a tile's K (or V)
@@ -93,6 +98,17 @@ __device__ __forceinline__ void wait_groups(int n) {
   }
 }
 
+// Two outputs in the 16-bit format.  Of an 8-bit pool, in float16, those past it are its largest: they
+// are sums of values of up to 65,504 and of what rounding the probabilities added.
+template <bool F16, bool FP8>
+__device__ __forceinline__ uint32_t pack_out(float x, float y) {
+  if constexpr (F16 && FP8) {
+    x = x > 65504.f ? 65504.f : x < -65504.f ? -65504.f : x;     // (a NaN stays)
+    y = y > 65504.f ? 65504.f : y < -65504.f ? -65504.f : y;
+  }
+  return Elt<F16>::pack(x, y);
+}
+
 // 0xffff in each half of w that is an infinity or a NaN.
 template <bool F16>
 __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
@@ -102,7 +118,7 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
 
 // A workgroup's share of the row blocks of one kv head.  Its eight waves are as many groups of columns
 // (CG) side by side as a row block has columns for, times as many groups of keys (KG) as are left.
-template <int D, bool F16, Chunk KIND>
+template <int D, bool F16, Chunk KIND, bool FP8 = false>
 __global__ __launch_bounds__(64 * kWaves, 2) void tree_attention_kernel(TreeArgs a) {
   constexpr bool TREE = KIND == kTree;
   using T = Elt<F16>;
@@ -158,9 +174,16 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_attention_kernel(TreeArgs
     const int cols = it.n * a.group;
 
     auto row_block = [&](auto groups) {
-      constexpr int CG = decltype(groups)::value, KG = NW / CG, NS = S::kStages / KG;
+      constexpr int CG = decltype(groups)::value, KG = NW / CG, NS = FP8 ? 2 : S::kStages / KG;
       constexpr int LOADS = 2 * S::kPieces / CG;       // of a wave, per stage
       constexpr int AHEAD = CG == 1 ? NS : NS - 1;     // stages in flight when a step begins
+      // (8-bit) loads of 1 KiB of a tile's codes, and how many of them are a wave's
+      constexpr int CODE_LOADS = D / 16, MINE = CODE_LOADS > CG ? CODE_LOADS / CG : 1;
+      constexpr int CODE_ROWS = 1024 / D;              // rows of a load
+      constexpr int CODE_SLOT = MINE * 1280;           // a wave's codes of a stage, and their scales
+      constexpr int ROOM = (S::kLds - S::kMl - 2 * KG * S::kStage) / (NW * CODE_SLOT);
+      constexpr int DEPTH = ROOM < kCodeDepth ? ROOM : kCodeDepth;      // stages of codes in flight
+      static_assert(!FP8 || DEPTH >= 3, "room for the codes");
       static_assert(LOADS >= 1 && AHEAD * LOADS < 64, "loads of a wave");
       // (the lane through an empty asm: what is worked out from it stays within the row block)
       int lane = lane0;
@@ -231,10 +254,30 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_attention_kernel(TreeArgs
       const char* const my_plane = reinterpret_cast<const char*>(CG > 1 && cg_v ? a.vplane : a.kplane);
       const uint32_t my_src = cg_v ? src_v : src_k;
       uint32_t bad_bits = 0;        // two bits per stage: its halves with an invalid block id
+      const uint32_t codes_lds =
+          lds_addr(smem) + 2 * KG * S::kStage + wv * DEPTH * CODE_SLOT;
       auto issue = [&](int u, int slot) {
         if (u > 0 && (u & 31) == 0) {
           load_window(u);
           asm volatile("" : "+v"(window));
+        }
+        if constexpr (FP8) {
+#pragma unroll
+          for (int i = 0; i < MINE; ++i) {
+            // load x: of K below half of them, of V past them
+            const int x = (cg + i * CG) % CODE_LOADS, row0 = x % (CODE_LOADS / 2) * CODE_ROWS;
+            const bool v = x >= CODE_LOADS / 2;
+            const uint32_t rows = (uint32_t)__builtin_amdgcn_readlane(
+                                      (int)window, 2 * (u & 31) + row0 / 16) * 16u + row0 % 16;
+            const uint32_t to = codes_lds + slot * CODE_SLOT + i * 1280;
+            lds_dma16(reinterpret_cast<const char*>(v ? a.vplane : a.kplane) + (uint64_t)rows * D,
+                      16u * lane, to);
+            // the dword with the scale of the lane's row
+            lds_dma4((v ? a.vscale : a.kscale) + rows, (uint32_t)(lane / (D / 16)) & ~3u, to + 1024);
+          }
+          bad_bits = (bad_bits & ~(3u << (2 * (u & 15)))) |
+                     ((uint32_t)(win_bad >> (2 * (u & 31))) & 3u) << (2 * (u & 15));
+          return;
         }
         const uint32_t st = ring_lds + slot * S::kStage;
         uint32_t off = my_src, off_v = src_v;
@@ -265,11 +308,47 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_attention_kernel(TreeArgs
           bad_bits = (bad_bits & ~(3u << (2 * slot))) |
                      ((uint32_t)(win_bad >> (2 * (u & 31))) & 3u) << (2 * slot);
       };
+      // The wave's codes of a stage, into 16-bit stage u & 1.  In float16, which has no 65,536 (a row's
+      // values from 63,488 on), keys are halved, for which the scores' scale makes up, and a value is
+      // 65,504, the nearest there is.
+      auto unpack = [&](int u, int slot) {
+#pragma unroll
+        for (int i = 0; i < MINE; ++i) {
+          typedef const __attribute__((address_space(3))) u32x4* lds16;
+          typedef __attribute__((address_space(3))) u32x4* lds16w;
+          typedef const __attribute__((address_space(3))) uint32_t* lds4;
+          const int x = (cg + i * CG) % CODE_LOADS, row0 = x % (CODE_LOADS / 2) * CODE_ROWS;
+          const bool v = x >= CODE_LOADS / 2;
+          const uint32_t from = codes_lds + slot * CODE_SLOT + i * 1280;
+          const u32x4 w = *(lds16)(uintptr_t)(from + 16 * lane);
+          const uint32_t four = *(lds4)(uintptr_t)(from + 1024 + 4 * lane);
+          const int r = lane / (D / 16), row = row0 + r, p = 2 * (lane % (D / 16));
+          float scale = __uint_as_float((four >> (8 * (r & 3)) & 0xffu) << 23);
+          if (F16 && !v) scale *= 0.5f;
+          uint32_t o[8];
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            o[2 * y] = value2<F16, false>(w[y], scale);
+            o[2 * y + 1] = value2<F16, true>(w[y], scale);
+          }
+          if (F16 && v && scale >= 256.f) {
+#pragma unroll
+            for (int y = 0; y < 8; ++y) {
+              if ((o[y] & 0x7fffu) == 0x7c00u) o[y] -= 1u;
+              if ((o[y] & 0x7fff0000u) == 0x7c000000u) o[y] -= 0x10000u;
+            }
+          }
+          const int swz = v ? v_swizzle(row) : k_swizzle<D>(row);
+          const uint32_t to = ring_lds + (u & 1) * S::kStage + (v ? S::kPlane : 0) + row * (2 * D);
+          *(lds16w)(uintptr_t)(to + 16 * (p ^ swz)) = u32x4{o[0], o[1], o[2], o[3]};
+          *(lds16w)(uintptr_t)(to + 16 * ((p + 1) ^ swz)) = u32x4{o[4], o[5], o[6], o[7]};
+        }
+      };
       // What was loaded so far arrives here: the compiler's own waits in the loop would drain the
       // ring, whose loads it does not see, at every step.
       asm volatile("" : "+v"(window));
 #pragma unroll 1
-      for (int d = 0; d < AHEAD && d < cnt; ++d) issue(d, d);
+      for (int d = 0; d < (FP8 ? DEPTH : AHEAD) && d < cnt; ++d) issue(d, d);
 #pragma unroll
       for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(q[s]));
 
@@ -294,7 +373,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_attention_kernel(TreeArgs
         const uint32_t st = slot * S::kStage;
         uint32_t mine = ~0u;                // the column's keys
         if constexpr (MASKED) {
-          const uint32_t bad = (bad_bits >> (2 * slot)) & 3u;
+          const uint32_t bad = (bad_bits >> (2 * (FP8 ? u & 15 : slot))) & 3u;
           const int kv0 = kTile * (t0 + kg + KG * u);
           // what any column attends, then this one
           uint32_t some = low_bits(all_keys - kv0);
@@ -458,8 +537,28 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_attention_kernel(TreeArgs
         }
       };
 
-      int u = 0, slot = 0;
+      int u = 0, slot = 0, code = 0;     // code: FP8: the slot of the next tile's codes
+      // The next tile's codes, which have arrived, become 16-bit ones; later codes take their place.
+      auto next_codes = [&](int n) {     // n: the tile
+        if constexpr (FP8) {
+          if (n >= cnt) return;
+          const int last = n + DEPTH - 1 < cnt - 1 ? n + DEPTH - 1 : cnt - 1;     // issued
+          wait_groups<2 * MINE, DEPTH - 1>(last - n);
+          asm volatile("" ::: "memory");
+          unpack(n, code);
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+          if (n + DEPTH < cnt) issue(n + DEPTH, code);
+          code = code + 1 == DEPTH ? 0 : code + 1;
+        }
+      };
+      if constexpr (FP8) next_codes(0);
       auto begin = [&] {
+        if constexpr (FP8) {
+          // every wave's part of this stage is there, every wave's reads of the one before done
+          asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+          next_codes(u + 1);
+          return;
+        }
         if (u < cnt) wait_groups<LOADS, AHEAD - 1>(cnt - 1 - u);
         if constexpr (CG > 1) {
           // every wave's loads of this stage are there, every wave's reads of the one before done
@@ -480,7 +579,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_attention_kernel(TreeArgs
       bool begun = false;
       while (u < steps) {
         begin();
-        begun = u >= plain || ((bad_bits >> (2 * slot)) & 3u) != 0;
+        begun = u >= plain || ((bad_bits >> (2 * (FP8 ? u & 15 : slot))) & 3u) != 0;
         if (begun) break;
         if (!idle) step(u, slot, std::false_type{});
         end();
@@ -521,7 +620,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_attention_kernel(TreeArgs
           *reinterpret_cast<f32x4*>(a.ws_acc + seg + 8 * x) = o;
         else
           *reinterpret_cast<u32x2*>(a.out + row + 8 * x) =
-              u32x2{T::pack(o[0] * inv, o[1] * inv), T::pack(o[2] * inv, o[3] * inv)};
+              u32x2{pack_out<F16, FP8>(o[0] * inv, o[1] * inv),
+                    pack_out<F16, FP8>(o[2] * inv, o[3] * inv)};
       };
       auto quad = [&](int x) {
         return f32x4{acc[x >> 2][4 * (x & 3)], acc[x >> 2][4 * (x & 3) + 1],
@@ -570,6 +670,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_attention_kernel(TreeArgs
     };
     if constexpr (KIND == kScored) {
       row_block(std::integral_constant<int, 1>{});
+    } else if constexpr (FP8) {
+      if (cols <= 128)
+        row_block(std::integral_constant<int, 4>{});
+      else
+        row_block(std::integral_constant<int, 8>{});
     } else {
       if (cols <= 32)
         row_block(std::integral_constant<int, 1>{});
@@ -586,9 +691,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_attention_kernel(TreeArgs
 }
 
 constexpr int kJoinCols = 32;     // of a workgroup of the merge
-template <int D, bool F16, bool TREE>
+template <int D, bool F16, bool TREE, bool FP8 = false>
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
-  using T = Elt<F16>;
   merge_row_block<D, TREE, kJoinCols>(a, a.group, [&](const Item& it, int head, int col, int d0,
                                                       const float* o, float m, float l) {
     constexpr int PER = kJoinCols * D / 256;
@@ -597,8 +701,9 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
     u16* const dst = a.out + row * D + d0;
 #pragma unroll
     for (int x = 0; x < PER; x += 8)
-      st16(dst + x, u32x4{T::pack(o[x], o[x + 1]), T::pack(o[x + 2], o[x + 3]),
-                          T::pack(o[x + 4], o[x + 5]), T::pack(o[x + 6], o[x + 7])});
+      st16(dst + x,
+           u32x4{pack_out<F16, FP8>(o[x], o[x + 1]), pack_out<F16, FP8>(o[x + 2], o[x + 3]),
+                 pack_out<F16, FP8>(o[x + 4], o[x + 5]), pack_out<F16, FP8>(o[x + 6], o[x + 7])});
     if (d0 == 0 && a.lse != nullptr) a.lse[row] = m + __log2f(l);
   });
 }
@@ -606,14 +711,15 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
 // ---------------------------------------------------------------- launches
 
 template <int D, bool F16>
-const void* kernel_of(Chunk kind) {
+const void* kernel_of(Chunk kind, bool fp8) {
+  if (fp8) return (const void*)tree_attention_kernel<D, F16, kTree, true>;
   return kind == kTree     ? (const void*)tree_attention_kernel<D, F16, kTree>
          : kind == kScored ? (const void*)tree_attention_kernel<D, F16, kScored>
                            : (const void*)tree_attention_kernel<D, F16, kCausal>;
 }
-const void* kernel_for(int head_dim, bool f16, Chunk kind) {
-  if (head_dim == 128) return f16 ? kernel_of<128, true>(kind) : kernel_of<128, false>(kind);
-  return f16 ? kernel_of<64, true>(kind) : kernel_of<64, false>(kind);
+const void* kernel_for(int head_dim, bool f16, Chunk kind, bool fp8 = false) {
+  if (head_dim == 128) return f16 ? kernel_of<128, true>(kind, fp8) : kernel_of<128, false>(kind, fp8);
+  return f16 ? kernel_of<64, true>(kind, fp8) : kernel_of<64, false>(kind, fp8);
 }
 Chunk kind_of(const ChunkAttention& c) {
   return c.mask != nullptr ? kTree : c.scores != nullptr ? kScored : kCausal;
@@ -668,9 +774,14 @@ Plan plan_for(const ChunkAttention& c) {
   return p;
 }
 
-template <int D, bool F16, bool TREE>
-void launch_merge(const TreeArgs& a, dim3 grid, hipStream_t s) {
-  hipLaunchKernelGGL((tree_merge_kernel<D, F16, TREE>), grid, dim3(256), 0, s, a);
+template <int D, bool F16>
+void launch_merge(const TreeArgs& a, bool tree, bool fp8, dim3 grid, hipStream_t s) {
+  if (F16 && fp8)
+    hipLaunchKernelGGL((tree_merge_kernel<D, F16, true, F16>), grid, dim3(256), 0, s, a);
+  else if (tree)
+    hipLaunchKernelGGL((tree_merge_kernel<D, F16, true>), grid, dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL((tree_merge_kernel<D, F16, false>), grid, dim3(256), 0, s, a);
 }
 
 // ---------------------------------------------------------------- masks from parents
@@ -771,7 +882,13 @@ int launch_chunk_attention(const ChunkAttention& call, void* workspace, size_t w
   a.q = (const u16*)c.q;
   a.q_stride = c.q_tok_stride;
   a.kplane = (const u16*)c.kv_cache;
-  a.vplane = a.kplane + c.num_blocks * c.num_kv_heads * (int64_t)c.block_size * c.head_dim;
+  const int64_t rows = c.num_blocks * c.num_kv_heads * (int64_t)c.block_size;     // of a plane
+  a.vplane = a.kplane + rows * c.head_dim;
+  if (c.scales != nullptr) {
+    a.vplane = (const u16*)((const char*)c.kv_cache + rows * c.head_dim);
+    a.kscale = (const uint8_t*)c.scales;
+    a.vscale = a.kscale + rows;
+  }
   a.num_blocks = c.num_blocks;
   a.num_heads = c.num_heads;
   a.num_kv_heads = c.num_kv_heads;
@@ -798,6 +915,7 @@ int launch_chunk_attention(const ChunkAttention& call, void* workspace, size_t w
   a.q_flip = c.scale < 0.f ? 0x80008000u : 0u;
   a.q_keep = c.scale == 0.f ? 0u : ~0u;
   a.scale_log2 = c.scale == 0.f ? 1.f : fabsf(c.scale) * kLog2e;
+  if (c.scales != nullptr && dtype_is_f16(c.dtype)) a.scale_log2 *= 2.f;     // (keys are halved)
   a.shares = p.shares;
   a.min_chunk = kMinChunk;
   a.pad = kPad;
@@ -807,7 +925,8 @@ int launch_chunk_attention(const ChunkAttention& call, void* workspace, size_t w
   const int64_t wgs = units * a.num_kv_heads;
   if (!grid_fits(wgs, threads)) return NDL_ERR_INVALID_ARG;
   void* args[] = {&a};
-  if (hipLaunchKernel(kernel_for(c.head_dim, dtype_is_f16(c.dtype), kind_of(c)),
+  if (hipLaunchKernel(kernel_for(c.head_dim, dtype_is_f16(c.dtype), kind_of(c),
+                                 c.scales != nullptr),
                       dim3((unsigned)wgs), dim3(threads), args, 0, s) != hipSuccess) {
     (void)hipGetLastError();  // clear the error so that the next call's check sees its own
     return NDL_ERR_LAUNCH;
@@ -817,13 +936,11 @@ int launch_chunk_attention(const ChunkAttention& call, void* workspace, size_t w
   const int groups = (a.toks * a.group + kJoinCols - 1) / kJoinCols;
   const dim3 grid((unsigned)a.items, (unsigned)a.num_kv_heads, (unsigned)groups);
   const bool f16 = dtype_is_f16(c.dtype), tree = c.mask != nullptr;
-  if (c.head_dim == 128) {
-    if (f16) tree ? launch_merge<128, true, true>(a, grid, s) : launch_merge<128, true, false>(a, grid, s);
-    else tree ? launch_merge<128, false, true>(a, grid, s) : launch_merge<128, false, false>(a, grid, s);
-  } else {
-    if (f16) tree ? launch_merge<64, true, true>(a, grid, s) : launch_merge<64, true, false>(a, grid, s);
-    else tree ? launch_merge<64, false, true>(a, grid, s) : launch_merge<64, false, false>(a, grid, s);
-  }
+  const bool fp8 = c.scales != nullptr;
+  if (c.head_dim == 128)
+    f16 ? launch_merge<128, true>(a, tree, fp8, grid, s) : launch_merge<128, false>(a, tree, fp8, grid, s);
+  else
+    f16 ? launch_merge<64, true>(a, tree, fp8, grid, s) : launch_merge<64, false>(a, tree, fp8, grid, s);
   return check_launch();
 }
 

@@ -1,16 +1,17 @@
-// What tree_attention.hip offers attention_mass.hip.
+// What tree_attention.hip offers attention_mass.hip and fp8_attention.hip.
 #pragma once
 
 #include "ndl_common.hpp"
 
 namespace ndl {
 
-// Attention of a chunk of new tokens per sequence over a 16-bit paged pool.
+// Attention of a chunk of new tokens per sequence over a 16-bit paged pool, or, of trees, an 8-bit one.
 struct ChunkAttention {
   void* out;
   const void* q;
   int64_t q_tok_stride;
-  const void* kv_cache;
+  const void* kv_cache;            // an 8-bit pool's codes
+  const void* scales;              // and its scales; null: a 16-bit pool
   int64_t num_blocks;
   const int32_t* block_table;
   int64_t bt_row_stride;

@@ -225,4 +225,4 @@ def test_tree_attention_uses_m0_only_for_direct_lds_loads(tmp_path):
     for i in uses:
         assert re.match(r"s_mov_b32 m0, (s\d+|vcc_lo|vcc_hi)$", body[i]), body[i]
         assert body[i + 1] == "s_nop 0" and \
-            re.match(r"global_load_lds_dwordx4 ", body[i + 2]), body[i:i + 3]
+            re.match(r"global_load_lds_dword(x4)? ", body[i + 2]), body[i:i + 3]
