@@ -186,6 +186,7 @@ template <int D, bool TREE, int COLS = kMergeCols, class PUT>
 __device__ __forceinline__ void merge_row_block(const RowBlocks& a, int group, PUT put) {
   constexpr int PER = COLS * D / 256;             // consecutive outputs of a thread
   constexpr int UNROLL = PER <= 4 ? 8 : 2;        // parts whose loads are under way
+  constexpr int TPC = 256 / COLS;                 // threads of a column
   __shared__ float2 part[kMergeParts][COLS];
   const int t = threadIdx.x, lane = t & 63;
   const int e = blockIdx.x, head = blockIdx.y, c0 = blockIdx.z * COLS;
@@ -222,38 +223,58 @@ __device__ __forceinline__ void merge_row_block(const RowBlocks& a, int group, P
                   ml[(int64_t)(i0 + i / COLS) * per + i % COLS];
           __syncthreads();
         }
-        if (c >= cols) continue;
         if (pass == 0) {
-          for (int i = 0; i < m; ++i) mx = fmaxf(mx, part[i][c].x);
+          if (c < cols) {
+#pragma unroll 8
+            for (int i = 0; i < m; ++i) mx = fmaxf(mx, part[i][c].x);
+          }
           continue;
         }
-        for (int i = 0; i < m; i += UNROLL) {
+        // the maxima become the parts' factors, each once
+        __syncthreads();
+        if (c < cols)
+          for (int i = t % TPC; i < m; i += TPC) {
+            const float x = part[i][c].x;
+            part[i][c].x = x == mx ? 1.f : fast_exp2(x - mx);
+          }
+        __syncthreads();
+        if (c >= cols) continue;
+        auto load = [&](int i, float* v) {
+          const float* const q = src + (int64_t)(i0 + i) * step;
+          if constexpr (PER >= 4) {
+#pragma unroll
+            for (int z = 0; z < PER; z += 4) {
+              const f32x4 w = *reinterpret_cast<const f32x4*>(q + z);
+#pragma unroll
+              for (int x = 0; x < 4; ++x) v[z + x] = w[x];
+            }
+          } else {
+            const f32x2 w = *reinterpret_cast<const f32x2*>(q);
+            v[0] = w[0];
+            v[1] = w[1];
+          }
+        };
+        auto add = [&](int i, const float* v) {
+          const float2 ms = part[i][c];
+          l += ms.y * ms.x;
+#pragma unroll
+          for (int x = 0; x < PER; ++x) o[x] += v[x] * ms.x;
+        };
+        int i = 0;
+        for (; i + UNROLL <= m; i += UNROLL) {
           float v[UNROLL][PER];
 #pragma unroll
-          for (int y = 0; y < UNROLL; ++y) {
-            const float* const q = src + (int64_t)(i0 + (i + y < m ? i + y : i)) * step;
-            if constexpr (PER >= 4) {
+          for (int y = 0; y < UNROLL; ++y) load(i + y, v[y]);
 #pragma unroll
-              for (int z = 0; z < PER; z += 4) {
-                const f32x4 w = *reinterpret_cast<const f32x4*>(q + z);
+          for (int y = 0; y < UNROLL; ++y) add(i + y, v[y]);
+        }
+        if (i < m) {
+          float v[UNROLL][PER];
 #pragma unroll
-                for (int x = 0; x < 4; ++x) v[y][z + x] = w[x];
-              }
-            } else {
-              const f32x2 w = *reinterpret_cast<const f32x2*>(q);
-              v[y][0] = w[0];
-              v[y][1] = w[1];
-            }
-          }
+          for (int y = 0; y < UNROLL; ++y) load(i + y < m ? i + y : i, v[y]);
 #pragma unroll
-          for (int y = 0; y < UNROLL; ++y) {
-            if (i + y >= m) break;
-            const float2 ms = part[i + y][c];
-            const float f = ms.x == mx ? 1.f : fast_exp2(ms.x - mx);
-            l += ms.y * f;
-#pragma unroll
-            for (int x = 0; x < PER; ++x) o[x] += v[y][x] * f;
-          }
+          for (int y = 0; y < UNROLL; ++y)
+            if (i + y < m) add(i + y, v[y]);
         }
       }
     }

@@ -1179,11 +1179,19 @@ extern "C" size_t ndl_fp8_attention_workspace_bytes(int num_seqs, int64_t num_to
 }
 
 // All entry points; `a` holds the new rows and the rotation of a decode step, or a tree's mask.
-// Trees of more columns than this have tree_attention.hip's row blocks of up to 256, where a key's codes
-// are unpacked once for all of them.
+// Trees of more columns than kWideColumns and of kWideScores scores in all have tree_attention.hip's
+// row blocks of up to 256, where a key's codes are unpacked once for all of them; fewer the row blocks
+// of 32 here, of which there are more.  us, here / there, 28/4 heads of 128: 8 sequences after 12,000,
+// 63 columns 62.0 / 53.0, 126 94.8 / 57.4, 252 159 / 83.0; 4 after 4,000, 126 32.0 / 32.9, 252 42.4 /
+// 39.1; 4 after 1,400, 252 19.9 / 37.9; 1 after 16,000, 252 41.0 / 58.8; 32/8 heads, 64 after 2,300,
+// 36 112 / 114, 72 175 / 118, 256 452 / 204; 16 after 300, 128 15.9 / 18.0, 256 32.2 / 21.9.
 constexpr int kWideColumns = 64;
-static bool wide_trees(const void* mask, int max_seqlen, int group) {
-  return mask != nullptr && (int64_t)max_seqlen * group > kWideColumns;
+constexpr int64_t kWideScores = 12 << 20;
+static bool wide_trees(int num_seqs, int max_seqlen, int64_t max_keys, int num_heads,
+                       int num_kv_heads) {
+  const int64_t cols = (int64_t)max_seqlen * (num_heads / num_kv_heads);
+  return cols > kWideColumns &&
+         (double)cols * (double)max_keys * num_seqs * num_kv_heads >= (double)kWideScores;
 }
 
 static int fp8_attention(ndl::ChunkArgs a, void* out, const void* q, int64_t q_tok_stride,
@@ -1249,7 +1257,8 @@ static int fp8_attention(ndl::ChunkArgs a, void* out, const void* q, int64_t q_t
                : launch_unpacked<64, false>(a, u, max_seqlen, max_keys, block_size, scale,
                                             workspace, s);
   }
-  if (wide_trees(a.mask, max_seqlen, a.group)) {
+  if (a.mask != nullptr &&
+      wide_trees(num_seqs, max_seqlen, max_keys, num_heads, num_kv_heads)) {
     ChunkAttention c{};
     c.out = out;
     c.q = q;
@@ -1357,7 +1366,7 @@ extern "C" size_t ndl_fp8_tree_attention_workspace_bytes(int num_seqs, int max_s
   if (num_seqs <= 0 || max_seqlen <= 0 || max_keys <= 0 || max_keys > 0x7fffff00 ||
       !shape_ok(head_dim, block_size, num_heads, num_kv_heads))
     return 0;
-  if (wide_trees(&max_keys, max_seqlen, num_heads / num_kv_heads)) {
+  if (wide_trees(num_seqs, max_seqlen, max_keys, num_heads, num_kv_heads)) {
     ChunkAttention c{};
     c.num_seqs = num_seqs;
     c.max_seqlen = max_seqlen;

@@ -690,20 +690,28 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_attention_kernel(TreeArgs
   }
 }
 
-constexpr int kJoinCols = 32;     // of a workgroup of the merge
-template <int D, bool F16, bool TREE, bool FP8 = false>
+// Columns of a workgroup of the merge: many where that makes workgroups enough (each finds its parts
+// first).
+constexpr int kJoinMany = 32, kJoinFew = 8, kJoinFrom = 512;
+template <int D, bool F16, bool TREE, bool FP8, int COLS>
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
-  merge_row_block<D, TREE, kJoinCols>(a, a.group, [&](const Item& it, int head, int col, int d0,
-                                                      const float* o, float m, float l) {
-    constexpr int PER = kJoinCols * D / 256;
+  merge_row_block<D, TREE, COLS>(a, a.group, [&](const Item& it, int head, int col, int d0,
+                                                 const float* o, float m, float l) {
+    constexpr int PER = COLS * D / 256;
     const int tok = col / a.group;
     const int64_t row = (it.tok0 + tok) * a.num_heads + head * a.group + col - tok * a.group;
-    u16* const dst = a.out + row * D + d0;
+    uint32_t* const dst = reinterpret_cast<uint32_t*>(a.out + row * D + d0);
+    uint32_t w[PER / 2];
 #pragma unroll
-    for (int x = 0; x < PER; x += 8)
-      st16(dst + x,
-           u32x4{pack_out<F16, FP8>(o[x], o[x + 1]), pack_out<F16, FP8>(o[x + 2], o[x + 3]),
-                 pack_out<F16, FP8>(o[x + 4], o[x + 5]), pack_out<F16, FP8>(o[x + 6], o[x + 7])});
+    for (int x = 0; x < PER / 2; ++x) w[x] = pack_out<F16, FP8>(o[2 * x], o[2 * x + 1]);
+    if constexpr (PER >= 8) {
+#pragma unroll
+      for (int x = 0; x < PER / 2; x += 4)
+        st16(reinterpret_cast<u16*>(dst + x), u32x4{w[x], w[x + 1], w[x + 2], w[x + 3]});
+    } else {
+#pragma unroll
+      for (int x = 0; x < PER / 2; ++x) dst[x] = w[x];
+    }
     if (d0 == 0 && a.lse != nullptr) a.lse[row] = m + __log2f(l);
   });
 }
@@ -774,14 +782,24 @@ Plan plan_for(const ChunkAttention& c) {
   return p;
 }
 
-template <int D, bool F16>
+template <int D, bool F16, int COLS>
 void launch_merge(const TreeArgs& a, bool tree, bool fp8, dim3 grid, hipStream_t s) {
   if (F16 && fp8)
-    hipLaunchKernelGGL((tree_merge_kernel<D, F16, true, F16>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((tree_merge_kernel<D, F16, true, F16, COLS>), grid, dim3(256), 0, s, a);
   else if (tree)
-    hipLaunchKernelGGL((tree_merge_kernel<D, F16, true>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((tree_merge_kernel<D, F16, true, false, COLS>), grid, dim3(256), 0, s, a);
   else
-    hipLaunchKernelGGL((tree_merge_kernel<D, F16, false>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((tree_merge_kernel<D, F16, false, false, COLS>), grid, dim3(256), 0, s, a);
+}
+template <int D, bool F16>
+void launch_merge(const TreeArgs& a, bool tree, bool fp8, hipStream_t s) {
+  const int cols = a.toks * a.group;
+  const bool many = (int64_t)a.items * a.num_kv_heads * ((cols + kJoinMany - 1) / kJoinMany) >=
+                    kJoinFrom;
+  const int each = many ? kJoinMany : kJoinFew;
+  const dim3 grid((unsigned)a.items, (unsigned)a.num_kv_heads, (unsigned)((cols + each - 1) / each));
+  many ? launch_merge<D, F16, kJoinMany>(a, tree, fp8, grid, s)
+       : launch_merge<D, F16, kJoinFew>(a, tree, fp8, grid, s);
 }
 
 // ---------------------------------------------------------------- masks from parents
@@ -933,14 +951,11 @@ int launch_chunk_attention(const ChunkAttention& call, void* workspace, size_t w
   }
   const int rc = check_launch();
   if (rc != NDL_OK || a.shares == 0) return rc;
-  const int groups = (a.toks * a.group + kJoinCols - 1) / kJoinCols;
-  const dim3 grid((unsigned)a.items, (unsigned)a.num_kv_heads, (unsigned)groups);
-  const bool f16 = dtype_is_f16(c.dtype), tree = c.mask != nullptr;
-  const bool fp8 = c.scales != nullptr;
+  const bool f16 = dtype_is_f16(c.dtype), tree = c.mask != nullptr, fp8 = c.scales != nullptr;
   if (c.head_dim == 128)
-    f16 ? launch_merge<128, true>(a, tree, fp8, grid, s) : launch_merge<128, false>(a, tree, fp8, grid, s);
+    f16 ? launch_merge<128, true>(a, tree, fp8, s) : launch_merge<128, false>(a, tree, fp8, s);
   else
-    f16 ? launch_merge<64, true>(a, tree, fp8, grid, s) : launch_merge<64, false>(a, tree, fp8, grid, s);
+    f16 ? launch_merge<64, true>(a, tree, fp8, s) : launch_merge<64, false>(a, tree, fp8, s);
   return check_launch();
 }
 
