@@ -176,7 +176,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_attention_kernel(TreeArgs
     auto row_block = [&](auto groups) {
       constexpr int CG = decltype(groups)::value, KG = NW / CG, NS = FP8 ? 2 : S::kStages / KG;
       constexpr int LOADS = 2 * S::kPieces / CG;       // of a wave, per stage
-      constexpr int AHEAD = CG == 1 ? NS : NS - 1;     // stages in flight when a step begins
+      // Steps between barriers: half of the ring is worked on while the other half is loaded.
+      constexpr int BATCH = CG == 1 ? 1 : NS / 2, AHEAD = CG == 1 ? NS : BATCH;
       // (8-bit) loads of 1 KiB of a tile's codes, and how many of them are a wave's
       constexpr int CODE_LOADS = D / 16, MINE = CODE_LOADS > CG ? CODE_LOADS / CG : 1;
       constexpr int CODE_ROWS = 1024 / D;              // rows of a load
@@ -184,7 +185,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_attention_kernel(TreeArgs
       constexpr int ROOM = (S::kLds - S::kMl - 2 * KG * S::kStage) / (NW * CODE_SLOT);
       constexpr int DEPTH = ROOM < kCodeDepth ? ROOM : kCodeDepth;      // stages of codes in flight
       static_assert(!FP8 || DEPTH >= 3, "room for the codes");
-      static_assert(LOADS >= 1 && AHEAD * LOADS < 64, "loads of a wave");
+      static_assert(LOADS >= 1 && NS % BATCH == 0 && AHEAD * LOADS < 64, "loads of a wave");
       // (the lane through an empty asm: what is worked out from it stays within the row block)
       int lane = lane0;
       asm volatile("" : "+v"(lane));
@@ -559,12 +560,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_attention_kernel(TreeArgs
           next_codes(u + 1);
           return;
         }
-        if (u < cnt) wait_groups<LOADS, AHEAD - 1>(cnt - 1 - u);
         if constexpr (CG > 1) {
-          // every wave's loads of this stage are there, every wave's reads of the one before done
-          asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-          if (u + NS - 1 < cnt) issue(u + NS - 1, slot == 0 ? NS - 1 : slot - 1);
+          if (u % BATCH != 0) return;
+          // every wave's loads of these stages are there, every wave's reads of those before done
+          asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+          for (int x = BATCH; x < 2 * BATCH; ++x)
+            if (u + x < cnt) issue(u + x, (u + x) % NS);
         } else {
+          wait_groups<LOADS, AHEAD - 1>(cnt - 1 - u);
           asm volatile("" ::: "memory");
         }
       };
