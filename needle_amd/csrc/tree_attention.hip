@@ -10,21 +10,34 @@
 // (needle/layers/attention.py:120-134, :291-310), with a cached prefix attended.
 //
 //   * Rows.  The g query heads of a kv head times the chunk's tokens are the columns, 32 to a wave
-//     (S^T = K Q^T and O^T = V^T P^T on 32x32x16 MFMA, keys and head_dim as rows): CG waves side by
-//     side hold a row block of up to 32 CG columns, so that a tree is read over once and its keys
-//     serve all its nodes; KG such groups take the row block's 32-key tiles in turn.
+//     (S^T = K Q^T and O^T = V^T P^T on 32x32x16 MFMA, keys and head_dim as rows): of a workgroup's
+//     eight waves CG (1, 2, 4, 8: what the row block's columns need) side by side hold up to 256
+//     columns, so that a tree's keys are read once for all its nodes, and 8 / CG such groups take the
+//     row block's 32-key tiles in turn.  (Four waves and 128 columns, trees of up to 256 columns: every
+//     second row block reads all keys again, 184 us where this takes 159.)
 //   * Keys.  A group's tile goes straight to its LDS ring in whole rows (1 KiB a load), K and V in
 //     16-byte pieces swizzled by row so that the operand reads (K: ds_read_b128, V: transposing
-//     ds_read_b64_tr_b16) spread over the banks.
+//     ds_read_b64_tr_b16) spread over the banks.  Groups of several waves meet at a barrier for half
+//     the ring's tiles (at each one: 165 us for 159); the loads of single waves, which no other row
+//     block repeats, pass the caches by (weights of 64 sequences' last tokens: 140 us for 125).
+//   * An 8-bit pool's codes (trees of more than 64 columns, see fp8_attention.hip) go to a ring of each
+//     wave's own; the wave unpacks what it has loaded, scale and all, into the group's 16-bit tiles.
 //   * P^T needs no data movement: the accumulator layout of S^T is the operand's, with k order
 //     8 h + e for key 16 t + 4 h + (e & 3) + 8 (e >> 2).
 //   * Softmax in fp32 with exp2.  The maximum is raised (and the sums rescaled) only when a tile's
-//     probabilities pass 256; P is rounded to the 16-bit format for the matrix cores, its sum is
-//     taken before that.
+//     probabilities pass 256; P is rounded to the 16-bit format for the matrix cores (half a step of it,
+//     what the output's own rounding costs too), its sum is taken before that.
 //   * The mask costs nothing below the context: only tiles that reach into the chunk look at it, as
 //     32 bits per column.
 //   * Split: as fp8_attention.hip's (chunk_stream.hpp), a workgroup per (kv head, row block) or
 //     equal shares of all of a kv head's tiles, merged by a second launch.
+// Measured (us, a call): 64 trees of 16 to 64 nodes after 512 to 4,096 tokens, 32/8 heads of 128, bf16
+// 159 (the keys at 3.2 TB/s, 480 TFLOP/s); 4 trees of 16 after 64 to 800, 14/2 heads of 64, 8.6; 8
+// trees of 40 to 60 after 4,096 to 32,768 in an 8-bit pool, 28/4 heads of 128, float16, 165 (590
+// TFLOP/s).  The wide ones are bound by neither: of a SIMD's cycles the matrix cores take 27 %, the
+// softmax 30 %, and LDS is busy for as many; two waves to a SIMD (222 of 256 registers) overlap them
+// only in part.  Scores made a tile ahead took longer (178 us for 165, the registers), a product put
+// off past the barrier in half the waves too (172).
 #include "chunk_stream.hpp"
 #include "fp8.hpp"
 #include "tree_attention.hpp"
@@ -63,7 +76,7 @@ struct TreeArgs : TreeOperands, RowBlocks {};
 constexpr int kWaves = 8;
 
 // With an 8-bit pool (FP8) a wave unpacks the codes that it has loaded itself, up to kCodeDepth steps
-// ahead, into one of its group's two 16-bit stages.
+// ahead, into its group's 16-bit stages.
 constexpr int kCodeDepth = 6;
 template <int D>
 struct TreeShape {
@@ -174,7 +187,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_attention_kernel(TreeArgs
     const int cols = it.n * a.group;
 
     auto row_block = [&](auto groups) {
-      constexpr int CG = decltype(groups)::value, KG = NW / CG, NS = FP8 ? 2 : S::kStages / KG;
+      constexpr int CG = decltype(groups)::value, KG = NW / CG;
+      constexpr int NS = !FP8 ? S::kStages / KG : S::kStages / KG >= 8 ? 4 : 2;     // of a group
       constexpr int LOADS = 2 * S::kPieces / CG;       // of a wave, per stage
       // Steps between barriers: half of the ring is worked on while the other half is loaded.
       constexpr int BATCH = CG == 1 ? 1 : NS / 2, AHEAD = CG == 1 ? NS : BATCH;
@@ -182,7 +196,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_attention_kernel(TreeArgs
       constexpr int CODE_LOADS = D / 16, MINE = CODE_LOADS > CG ? CODE_LOADS / CG : 1;
       constexpr int CODE_ROWS = 1024 / D;              // rows of a load
       constexpr int CODE_SLOT = MINE * 1280;           // a wave's codes of a stage, and their scales
-      constexpr int ROOM = (S::kLds - S::kMl - 2 * KG * S::kStage) / (NW * CODE_SLOT);
+      constexpr int ROOM = (S::kLds - S::kMl - NS * KG * S::kStage) / (NW * CODE_SLOT);
       constexpr int DEPTH = ROOM < kCodeDepth ? ROOM : kCodeDepth;      // stages of codes in flight
       static_assert(!FP8 || DEPTH >= 3, "room for the codes");
       static_assert(LOADS >= 1 && NS % BATCH == 0 && AHEAD * LOADS < 64, "loads of a wave");
@@ -256,7 +270,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_attention_kernel(TreeArgs
       const uint32_t my_src = cg_v ? src_v : src_k;
       uint32_t bad_bits = 0;        // two bits per stage: its halves with an invalid block id
       const uint32_t codes_lds =
-          lds_addr(smem) + 2 * KG * S::kStage + wv * DEPTH * CODE_SLOT;
+          lds_addr(smem) + NS * KG * S::kStage + wv * DEPTH * CODE_SLOT;
       auto issue = [&](int u, int slot) {
         if (u > 0 && (u & 31) == 0) {
           load_window(u);
@@ -309,7 +323,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_attention_kernel(TreeArgs
           bad_bits = (bad_bits & ~(3u << (2 * slot))) |
                      ((uint32_t)(win_bad >> (2 * (u & 31))) & 3u) << (2 * slot);
       };
-      // The wave's codes of a stage, into 16-bit stage u & 1.  In float16, which has no 65,536 (a row's
+      // The wave's codes of a stage, into 16-bit stage u % NS.  In float16, which has no 65,536 (a row's
       // values from 63,488 on), keys are halved, for which the scores' scale makes up, and a value is
       // 65,504, the nearest there is.
       auto unpack = [&](int u, int slot) {
@@ -340,7 +354,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_attention_kernel(TreeArgs
             }
           }
           const int swz = v ? v_swizzle(row) : k_swizzle<D>(row);
-          const uint32_t to = ring_lds + (u & 1) * S::kStage + (v ? S::kPlane : 0) + row * (2 * D);
+          const uint32_t to = ring_lds + (u % NS) * S::kStage + (v ? S::kPlane : 0) + row * (2 * D);
           *(lds16w)(uintptr_t)(to + 16 * (p ^ swz)) = u32x4{o[0], o[1], o[2], o[3]};
           *(lds16w)(uintptr_t)(to + 16 * ((p + 1) ^ swz)) = u32x4{o[4], o[5], o[6], o[7]};
         }
@@ -552,12 +566,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_attention_kernel(TreeArgs
           code = code + 1 == DEPTH ? 0 : code + 1;
         }
       };
-      if constexpr (FP8) next_codes(0);
+      if constexpr (FP8)
+        for (int n = 0; n < BATCH; ++n) next_codes(n);
       auto begin = [&] {
         if constexpr (FP8) {
-          // every wave's part of this stage is there, every wave's reads of the one before done
-          asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-          next_codes(u + 1);
+          // every wave's part of these stages is there, every wave's reads of those before done
+          if (u % BATCH == 0) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+          next_codes(u + BATCH);
           return;
         }
         if constexpr (CG > 1) {
