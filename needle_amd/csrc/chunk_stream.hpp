@@ -178,15 +178,16 @@ struct Stream {
 
 // One workgroup per (row block, kv head, COLS columns): the parts that the shares hold,
 // combined in their order; zeros for tokens with nothing to attend.  A row block inside one share
-// was written by the attention.  put(row block, head, column, head_dim, outputs, maximum, sum).
+// was written by the attention.  MANY: whole steps of parts without a test for each, whose loads stay
+// together (64 parts of one sequence: 12 us less), which takes registers (2 to 6 parts of 64 sequences:
+// 2 us more).  put(row block, head, column, head_dim, outputs, maximum, sum).
 constexpr int kMergeCols = 8;
 constexpr int kMergeParts = 64;   // at a time
 
-template <int D, bool TREE, int COLS = kMergeCols, class PUT>
+template <int D, bool TREE, int COLS = kMergeCols, bool MANY = false, class PUT>
 __device__ __forceinline__ void merge_row_block(const RowBlocks& a, int group, PUT put) {
   constexpr int PER = COLS * D / 256;             // consecutive outputs of a thread
   constexpr int UNROLL = PER <= 4 ? 8 : 2;        // parts whose loads are under way
-  constexpr int TPC = 256 / COLS;                 // threads of a column
   __shared__ float2 part[kMergeParts][COLS];
   const int t = threadIdx.x, lane = t & 63;
   const int e = blockIdx.x, head = blockIdx.y, c0 = blockIdx.z * COLS;
@@ -223,22 +224,11 @@ __device__ __forceinline__ void merge_row_block(const RowBlocks& a, int group, P
                   ml[(int64_t)(i0 + i / COLS) * per + i % COLS];
           __syncthreads();
         }
+        if (c >= cols) continue;
         if (pass == 0) {
-          if (c < cols) {
-#pragma unroll 8
-            for (int i = 0; i < m; ++i) mx = fmaxf(mx, part[i][c].x);
-          }
+          for (int i = 0; i < m; ++i) mx = fmaxf(mx, part[i][c].x);
           continue;
         }
-        // the maxima become the parts' factors, each once
-        __syncthreads();
-        if (c < cols)
-          for (int i = t % TPC; i < m; i += TPC) {
-            const float x = part[i][c].x;
-            part[i][c].x = x == mx ? 1.f : fast_exp2(x - mx);
-          }
-        __syncthreads();
-        if (c >= cols) continue;
         auto load = [&](int i, float* v) {
           const float* const q = src + (int64_t)(i0 + i) * step;
           if constexpr (PER >= 4) {
@@ -256,25 +246,28 @@ __device__ __forceinline__ void merge_row_block(const RowBlocks& a, int group, P
         };
         auto add = [&](int i, const float* v) {
           const float2 ms = part[i][c];
-          l += ms.y * ms.x;
+          const float f = ms.x == mx ? 1.f : fast_exp2(ms.x - mx);
+          l += ms.y * f;
 #pragma unroll
-          for (int x = 0; x < PER; ++x) o[x] += v[x] * ms.x;
+          for (int x = 0; x < PER; ++x) o[x] += v[x] * f;
         };
         int i = 0;
-        for (; i + UNROLL <= m; i += UNROLL) {
+        for (; MANY && i + UNROLL <= m; i += UNROLL) {
           float v[UNROLL][PER];
 #pragma unroll
           for (int y = 0; y < UNROLL; ++y) load(i + y, v[y]);
 #pragma unroll
           for (int y = 0; y < UNROLL; ++y) add(i + y, v[y]);
         }
-        if (i < m) {
+        for (; i < m; i += UNROLL) {
           float v[UNROLL][PER];
 #pragma unroll
           for (int y = 0; y < UNROLL; ++y) load(i + y < m ? i + y : i, v[y]);
 #pragma unroll
-          for (int y = 0; y < UNROLL; ++y)
-            if (i + y < m) add(i + y, v[y]);
+          for (int y = 0; y < UNROLL; ++y) {
+            if (i + y >= m) break;
+            add(i + y, v[y]);
+          }
         }
       }
     }

@@ -14,11 +14,11 @@
 //     eight waves CG (1, 2, 4, 8: what the row block's columns need) side by side hold up to 256
 //     columns, so that a tree's keys are read once for all its nodes, and 8 / CG such groups take the
 //     row block's 32-key tiles in turn.  (Four waves and 128 columns, trees of up to 256 columns: every
-//     second row block reads all keys again, 184 us where this takes 159.)
+//     second row block reads all keys again, 170 us where this takes 155.)
 //   * Keys.  A group's tile goes straight to its LDS ring in whole rows (1 KiB a load), K and V in
 //     16-byte pieces swizzled by row so that the operand reads (K: ds_read_b128, V: transposing
 //     ds_read_b64_tr_b16) spread over the banks.  Groups of several waves meet at a barrier for half
-//     the ring's tiles (at each one: 165 us for 159); the loads of single waves, which no other row
+//     the ring's tiles (at each one: 165 us); the loads of single waves, which no other row
 //     block repeats, pass the caches by (weights of 64 sequences' last tokens: 140 us for 125).
 //   * An 8-bit pool's codes (trees of more than 64 columns, see fp8_attention.hip) go to a ring of each
 //     wave's own; the wave unpacks what it has loaded, scale and all, into the group's 16-bit tiles.
@@ -32,12 +32,12 @@
 //   * Split: as fp8_attention.hip's (chunk_stream.hpp), a workgroup per (kv head, row block) or
 //     equal shares of all of a kv head's tiles, merged by a second launch.
 // Measured (us, a call): 64 trees of 16 to 64 nodes after 512 to 4,096 tokens, 32/8 heads of 128, bf16
-// 159 (the keys at 3.2 TB/s, 480 TFLOP/s); 4 trees of 16 after 64 to 800, 14/2 heads of 64, 8.6; 8
+// 155 (the keys at 3.2 TB/s, 490 TFLOP/s); 4 trees of 16 after 64 to 800, 14/2 heads of 64, 8.6; 8
 // trees of 40 to 60 after 4,096 to 32,768 in an 8-bit pool, 28/4 heads of 128, float16, 165 (590
 // TFLOP/s).  The wide ones are bound by neither: of a SIMD's cycles the matrix cores take 27 %, the
 // softmax 30 %, and LDS is busy for as many; two waves to a SIMD (222 of 256 registers) overlap them
-// only in part.  Scores made a tile ahead took longer (178 us for 165, the registers), a product put
-// off past the barrier in half the waves too (172).
+// only in part.  Scores made a tile ahead took longer (195 us for 178, in shares), a product put off past
+// the barrier in half the waves too (172 for 165).
 #include "chunk_stream.hpp"
 #include "fp8.hpp"
 #include "tree_attention.hpp"
@@ -713,7 +713,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_attention_kernel(TreeArgs
 constexpr int kJoinMany = 32, kJoinFew = 8, kJoinFrom = 512;
 template <int D, bool F16, bool TREE, bool FP8, int COLS>
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
-  merge_row_block<D, TREE, COLS>(a, a.group, [&](const Item& it, int head, int col, int d0,
+  merge_row_block<D, TREE, COLS, true>(a, a.group, [&](const Item& it, int head, int col, int d0,
                                                  const float* o, float m, float l) {
     constexpr int PER = COLS * D / 256;
     const int tok = col / a.group;
