@@ -44,6 +44,15 @@
  *   ndl_verify_drafts   accepted drafts and the next token of every sequence, from the
  *                       target's logits and given random numbers
  *
+ * and trees of drafted tokens and caches that keep some of their rows, over both pools:
+ *
+ *   ndl_tree_mask       which nodes a tree's tokens attend, from their parents
+ *   ndl_tree_attention, ndl_fp8_tree_attention  attention of a chunk under such masks
+ *   ndl_verify_tree     the accepted path of every tree and the token that follows
+ *   ndl_attention_mass  attention that adds up the weights of every cached token
+ *   ndl_kv_select       the cached tokens that stay, by those weights
+ *   ndl_kv_compact      rows of cached tokens moved together, in every layer's pool
+ *
  * Conventions (every entry point):
  *   - Plain pointers to device memory, element counts and strides in ELEMENTS.
  *   - KV pool layout (needle/model/runner.py:65-78, attention.py:9-10):

@@ -708,8 +708,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_attention_kernel(TreeArgs
   }
 }
 
-// Columns of a workgroup of the merge: many where that makes workgroups enough (each finds its parts
-// first).
+// Columns of a workgroup of the merge: many where that makes workgroups enough, each of which finds its
+// parts first (32 columns / 8, calls of us: 1 tree of 126 columns after 16,000, 28/4 heads, 51.7 / 44.1;
+// 24 of 511 after 2,000 124 / 135).
 constexpr int kJoinMany = 32, kJoinFew = 8, kJoinFrom = 512;
 template <int D, bool F16, bool TREE, bool FP8, int COLS>
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {

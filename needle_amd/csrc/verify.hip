@@ -32,7 +32,9 @@
 // counts once); where there is none the next token has the node's p without its children's tokens.
 // That is a draw of p for every node, so the tokens are distributed as the target's; a chain gives
 // what points give above.  Four launches: after stats a workgroup per sequence walks its tree (walk),
-// then sums and pick as above, the children's tokens as bits over a slice.
+// then sums and pick as above, the children's tokens as bits over a slice.  us, stats / walk / sums /
+// pick: 32 trees of 16 to 64 nodes of 128,256 logits 53.1 (6.1 TB/s) / 5.8 / 7.0 / 5.5, a tree of 60
+// of 151,936 6.4 / 5.3 / 3.0 / 4.9.
 #include "ndl_common.hpp"
 
 #include <type_traits>
