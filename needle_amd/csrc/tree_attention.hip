@@ -465,8 +465,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_attention_kernel(TreeArgs
         }
 
         if constexpr (KIND == kScored) {
-          // four keys to a store; past the keys and where nothing is attended -inf
-          if (live && col < a.score_cols) {
+          // four keys to a store; past the keys and where nothing is attended -inf (a context may be
+          // longer than the call's bound, which the rows are of)
+          if (live && col < a.score_cols && kTile * (int64_t)(t0 + kg + KG * u) < a.score_keys) {
             float* const at =
                 a.scores +
                 (((int64_t)head * a.num_seqs + it.seq) * a.score_cols + col) * a.score_keys +

@@ -224,3 +224,30 @@ def test_refusals():
         c.run(max_seqlen=0)
     assert c.run(cu_seqlens=torch.zeros(3, dtype=torch.int32, device=DEV),
                  q=torch.empty(0, 8, 64, dtype=c.dtype, device=DEV))[0].shape == (0, 8, 64)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("counts", [[1, 1, 1], [2, 1, 2], [30, 4, 9]])
+def test_contexts_past_the_bound_of_a_call(counts, dtype):
+    """Keys past max_context_len + max_seqlen get no weight, and nothing is written past the
+    workspace."""
+    c = Case((32, 8, 128, 16), counts, [700, 20, 1900], dtype, seed=21)
+    bound, most = 100, max(counts)
+    need = ops.attention_mass_workspace_bytes(3, sum(counts), most, bound + most, c.h, c.hkv, c.d,
+                                              c.bs)
+    ws = torch.full((need + (4 << 20),), 0xA5, dtype=torch.uint8, device=DEV)
+    out, mass = c.run(max_context_len=bound, workspace=ws)
+    assert (ws[need:] == 0xA5).all()
+    r = tree_ref.attention(c.q, c.pool, c.table, c.cu, c.ctx, c.scale)
+    check(out, r, c.dtype, c.d, int(c.cu[-1]))
+    want = tree_ref.mass(r, c.before, c.cu, c.ctx, c.h)
+    mass = mass.cpu()
+    for i, n in enumerate(c.lens):
+        p = torch.arange(n + counts[i])
+        blk = c.table[i].long()[p // 16]
+        inside = p < bound + most
+        got, old = mass[blk, :, p % 16], c.before[blk, :, p % 16]
+        same = (got == old) | (got.isnan() & old.isnan())
+        assert same[~inside].all()
+        torch.testing.assert_close(got[inside].double(), want[blk, :, p % 16][inside],
+                                   rtol=2.0 ** -10, atol=1e-6)
