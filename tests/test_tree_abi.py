@@ -114,6 +114,7 @@ def test_select_refusals(lib):
                 dict(sinks=16, recent=17)):
         assert select(**bad) == -1, bad
     assert select(n=65536) == -2 and select(w=1 << 28, stride=1 << 28) == -2
+    assert select(w=(1 << 27) - 8, stride=1 << 27) == -2     # positions are counted on in 32 bits
     assert select(n=0) == 0
 
 
