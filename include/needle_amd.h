@@ -762,7 +762,7 @@ int ndl_attention_mass(void* out, float* mass, const void* q, int64_t q_tok_stri
  * (ndl_verify_tree's path).  In every one of num_layers (at most 128) pools, both planes; scales: those of
  * 8-bit pools (NULL: 16-bit or float32 ones); row_bytes: of a row of a pool (a multiple of 16); and in
  * mass float32 [num_blocks][num_kv_heads][block_size] (NULL: none).  `pools` and `scales` are host
- * arrays of device addresses.
+ * arrays of device addresses, no pool twice.
  *
  * Without dst_table rows move in place and a list has to ascend, keep[j] >= j; with it they go to the
  * blocks that its rows name, none of which may be one that rows are read from.  An entry below 0, a

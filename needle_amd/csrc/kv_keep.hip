@@ -412,6 +412,8 @@ extern "C" int ndl_kv_compact(void* const* pools, void* const* scales, int num_l
   for (int i = 0; i < num_layers; ++i) {
     a.pool[i] = (char*)pools[i];
     if (!pools[i] || (uintptr_t)pools[i] & 15u) return NDL_ERR_INVALID_ARG;
+    for (int j = 0; j < i; ++j)      // (rows moved twice at once)
+      if (pools[j] == pools[i]) return NDL_ERR_INVALID_ARG;
     if (!scales) continue;
     a.scales[i] = (char*)scales[i];
     if (!scales[i]) return NDL_ERR_INVALID_ARG;

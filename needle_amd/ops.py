@@ -1456,7 +1456,8 @@ def kv_compact(pools, block_table: torch.Tensor, keep: torch.Tensor, counts: tor
     row first[i] + j of sequence i (first None: j) becomes what row first[i] + keep[j] was, for
     j < counts[i].
 
-    pools: a list of [2, NB, Hkv, bs, D] tensors, or of Fp8KVCache, up to 128 of one shape and type.
+    pools: a list of [2, NB, Hkv, bs, D] tensors, or of Fp8KVCache, up to 128 of one shape and type,
+    none twice.
     keep int32: [num_seqs, Hkv, K], a list for each kv head (kv_select's), or, with cu_seqlens
     (int32 [num_seqs + 1]), [T], packed, a list for all kv heads alike: verify_tree's path, with
     first the tokens cached before the tree and counts = accepted + 1.  counts, first int32
@@ -1488,6 +1489,7 @@ def kv_compact(pools, block_table: torch.Tensor, keep: torch.Tensor, counts: tor
     row_bytes = d * main[0].element_size()
     _require(row_bytes % 16 == 0, f"rows of {row_bytes} bytes are not whole 16-byte pieces")
     _require(len(pools) <= 128, f"at most 128 pools a call, got {len(pools)}")
+    _require(len({x.data_ptr() for x in main}) == len(main), "a pool is given twice")
     n_seqs = _check_table(block_table, nb, dev)
     _check_int32("counts", counts, 1, dev)
     _require(counts.shape[0] == n_seqs, "counts/block_table batch mismatch")

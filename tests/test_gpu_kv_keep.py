@@ -283,7 +283,8 @@ def test_refusals():
         a.update(bad)
         with pytest.raises(TypeError):
             ops.kv_compact(a["pools"], table, a["keep"], a["counts"], mass=a["mass"])
-    for bad in (dict(pools=[]), dict(pools=[pool, pool[:, :4].contiguous()]),
+    for bad in (dict(pools=[]), dict(pools=[pool, pool]),
+                dict(pools=[pool, pool[:, :4].contiguous()]),
                 dict(keep=keep[:, :1]), dict(keep=keep[..., ::2]), dict(counts=n[:1]),
                 dict(mass=mass[:3]), dict(pools=[pool.cpu()]), dict(keep=keep.cpu()),
                 dict(first=n[:1]), dict(cu=n), dict(dst=table[:1]), dict(pools=[pool] * 129)):

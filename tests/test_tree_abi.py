@@ -120,7 +120,8 @@ def test_select_refusals(lib):
 
 def test_compact_refusals(lib):
     import ctypes
-    here = (ctypes.c_void_p * 129)(*[P] * 129)
+    here = (ctypes.c_void_p * 129)(*[P + 4096 * i for i in range(129)])
+    twice = (ctypes.c_void_p * 2)(P, P)
     odd = (ctypes.c_void_p * 2)(P, P + 8)
     none = (ctypes.c_void_p * 2)(P, None)
 
@@ -129,7 +130,8 @@ def test_compact_refusals(lib):
              counts=P, n=3):
         return lib.ndl_kv_compact(pools, scales, layers, mass, nb, hkv, bs, row, table, stride, w,
                                   to, ts, tw, keep, width, cu, rows, first, counts, n, None)
-    for bad in (dict(pools=None), dict(pools=odd), dict(pools=none), dict(scales=none),
+    for bad in (dict(pools=None), dict(pools=odd), dict(pools=none), dict(pools=twice),
+                dict(scales=none),
                 dict(table=None), dict(keep=None), dict(counts=None), dict(mass=P + 2),
                 dict(layers=-1), dict(n=-1), dict(nb=0), dict(hkv=0), dict(bs=0), dict(row=0),
                 dict(row=24), dict(w=0), dict(stride=7), dict(to=P), dict(to=P, ts=3, tw=4),
