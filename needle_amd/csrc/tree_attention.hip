@@ -32,7 +32,7 @@
 //   * Split: as fp8_attention.hip's (chunk_stream.hpp), a workgroup per (kv head, row block) or
 //     equal shares of all of a kv head's tiles, merged by a second launch.
 // Measured (us, a call): 64 trees of 16 to 64 nodes after 512 to 4,096 tokens, 32/8 heads of 128, bf16
-// 155 (the keys at 3.2 TB/s, 490 TFLOP/s); 4 trees of 16 after 64 to 800, 14/2 heads of 64, 8.6; 8
+// 155 to 162 (the keys at 3.2 TB/s, 480 TFLOP/s); 4 trees of 16 after 64 to 800, 14/2 heads of 64, 8.6; 8
 // trees of 40 to 60 after 4,096 to 32,768 in an 8-bit pool, 28/4 heads of 128, float16, 165 (590
 // TFLOP/s).  The wide ones are bound by neither: of a SIMD's cycles the matrix cores take 27 %, the
 // softmax 30 %, and LDS is busy for as many; two waves to a SIMD (222 of 256 registers) overlap them
