@@ -19,8 +19,8 @@
 //     joined across lanes once, at the end.  (8 waves of 32 keys rather than 4 of 64: twice as many to a
 //     SIMD, 26 us for 34 of 8 prompts of 2,000 to 16,000 tokens, 32 tokens each, 28/4 heads.)
 // Bound (64 sequences' step): K and V read once, 4.3 TB/s over the call.  The 8 prompts' 83 us are the
-// attention 42 (shares of 20 tiles, of which the start and end take as long as 10), its merge 13 and
-// the weights 26, where products and exponentials of the 224 columns take about 12 each.
+// attention 42 (shares of 20 tiles), its merge 13 and the weights 26 (by instruction counts 5 of them
+// products and 8 exponentials; the rest is trips to memory of workgroups that live for 256 keys).
 // Sums run in a fixed order, without atomics; a key's number is written by one lane.
 #include "fp8.hpp"
 #include "tree_attention.hpp"
