@@ -328,7 +328,7 @@ void chunk_attention_kernel(ChunkArgs a) {
         u_new = (tile - t0) / NW;
     }
     // keys that every token attends: up to the first one, or (TREE) up to the chunk
-    const int64_t chunk_at = it.pos - (int64_t)(e - it.seq * a.blocks_per_seq) * a.toks;
+    const int chunk_at = (int)(it.pos - (int64_t)(e - it.seq * a.blocks_per_seq) * a.toks);
     const int64_t k_all = TREE ? chunk_at : it.pos + 1;
     const int64_t k_first = k_all < it.cap ? k_all : it.cap;
     const int all_keys = (int)it.keys();      // of the last token
@@ -515,9 +515,10 @@ void chunk_attention_kernel(ChunkArgs a) {
           if (bad & 2) some &= 0x0000ffffu;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
-            vis[nt] = kv0 + kTile > min_keys
+            // (by the context, not min_keys: a table may end before it)
+            vis[nt] = kv0 + kTile > chunk_at
                           ? some & bits_at(a.mask + (it.tok0 + lim[nt]) * a.mask_stride, a.words,
-                                           kv0 - (int)chunk_at)
+                                           kv0 - chunk_at)
                           : some;
         }
 #pragma unroll
