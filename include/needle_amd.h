@@ -783,7 +783,8 @@ int ndl_kv_compact(void* const* pools, void* const* scales, int num_layers, floa
  * the first `sinks`, the last `recent` (at most budget together), and of the rest those with the
  * largest weights in mass float32 [num_blocks][num_kv_heads][block_size], of equal ones the first.
  * A NaN counts as the largest, a position with an invalid block id as the smallest weight; lens is
- * cut to what the table holds, and a negative one is 0.
+ * cut to what the table holds, and a negative one is 0.  num_seqs at most 65535, the budget and the
+ * tokens that the table holds at most 2^31 - 2^16 (NDL_ERR_UNSUPPORTED otherwise).
  */
 int ndl_kv_select(int32_t* keep, int32_t* kept, const float* mass, int64_t num_blocks,
                   int num_kv_heads, int block_size, const int32_t* block_table,
