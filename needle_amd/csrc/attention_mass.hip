@@ -314,10 +314,11 @@ extern "C" int ndl_attention_mass(void* out, float* mass, const void* q, int64_t
   if (!mass || (uintptr_t)mass & 3u) return NDL_ERR_INVALID_ARG;
   const int64_t cap = (int64_t)max_blocks_per_seq * block_size;
   if (c.max_keys > cap) c.max_keys = cap;
+  const MassSizes z = sizes_of(c);
   const int64_t blocks = (c.max_keys + 255) / 256 * num_kv_heads;
   static_assert(kMassKeys == 256, "keys of a workgroup, either way");
-  if (num_seqs > 65535 || !grid_fits(blocks, 256)) return NDL_ERR_UNSUPPORTED;
-  const MassSizes z = sizes_of(c);
+  const int threads = z.score_keys ? 256 : 64 * kMassWaves;      // of the weights' launch
+  if (num_seqs > 65535 || !grid_fits(blocks, threads)) return NDL_ERR_UNSUPPORTED;
   if (!workspace || workspace_bytes < z.total() || (uintptr_t)workspace & 255u)
     return NDL_ERR_WORKSPACE;
   c.lse = (float*)workspace;
@@ -356,20 +357,20 @@ extern "C" int ndl_attention_mass(void* out, float* mass, const void* q, int64_t
   a.num_seqs = num_seqs;
   const dim3 grid((unsigned)blocks, (unsigned)num_seqs);
   if (z.score_keys) {
-    hipLaunchKernelGGL(add_scores_kernel, grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL(add_scores_kernel, grid, dim3(threads), 0, s, a);
     return check_launch();
   }
   const bool f16 = dtype_is_f16(dtype);
   if (head_dim == 128) {
     if (f16)
-      hipLaunchKernelGGL((add_weights_kernel<128, true>), grid, dim3(64 * kMassWaves), 0, s, a);
+      hipLaunchKernelGGL((add_weights_kernel<128, true>), grid, dim3(threads), 0, s, a);
     else
-      hipLaunchKernelGGL((add_weights_kernel<128, false>), grid, dim3(64 * kMassWaves), 0, s, a);
+      hipLaunchKernelGGL((add_weights_kernel<128, false>), grid, dim3(threads), 0, s, a);
   } else {
     if (f16)
-      hipLaunchKernelGGL((add_weights_kernel<64, true>), grid, dim3(64 * kMassWaves), 0, s, a);
+      hipLaunchKernelGGL((add_weights_kernel<64, true>), grid, dim3(threads), 0, s, a);
     else
-      hipLaunchKernelGGL((add_weights_kernel<64, false>), grid, dim3(64 * kMassWaves), 0, s, a);
+      hipLaunchKernelGGL((add_weights_kernel<64, false>), grid, dim3(threads), 0, s, a);
   }
   return check_launch();
 }
