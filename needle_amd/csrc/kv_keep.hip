@@ -487,7 +487,7 @@ extern "C" int ndl_kv_select(int32_t* keep, int32_t* kept, const float* mass, in
   if (!keep || !kept || !mass || !block_table || !lens || (uintptr_t)mass & 3u)
     return NDL_ERR_INVALID_ARG;
   // (positions and entries of a list are counted on by a workgroup's threads in 31 bits)
-  if (num_seqs > 65535 || budget > 0x7fff0000 ||
+  if (num_seqs > 65535 || budget > 0x7fff0000 || !grid_fits(num_kv_heads, kSelThreads) ||
       (int64_t)max_blocks_per_seq * block_size > 0x7fff0000)
     return NDL_ERR_UNSUPPORTED;
   SelectArgs a{keep, kept, mass, num_blocks, num_kv_heads, block_size, block_table, bt_row_stride,

@@ -32,3 +32,10 @@ def test_grids_of_the_weights(lib):
     # one workgroup fewer goes on to the workspace, which is missing
     for per, hkv in (((1 << 22) - 1, 2), ((1 << 23) - 1, 1), ((1 << 20) - 1, 8)):
         assert weigh(per, hkv) == -3, (per, hkv)
+
+
+def test_grids_of_the_selection(lib):
+    """A workgroup of 1,024 threads for a kv head of a sequence."""
+    def select(hkv):
+        return lib.ndl_kv_select(P, P, P, 1, hkv, 16, P, 8, 8, P, 3, 32, 4, 8, None)
+    assert select(1 << 22) == -2 and select(MOST) == -2
