@@ -778,7 +778,7 @@ Plan plan_for(const ChunkAttention& c) {
   for (int cols = 32 * kWaves; cols >= 32; cols /= 2) {
     if (cols > 32 && (int64_t)c.max_seqlen * group <= cols / 2) continue;
     p.toks = cols / group;
-    p.blocks_per_seq = (c.max_seqlen + p.toks - 1) / p.toks;
+    p.blocks_per_seq = ((int64_t)c.max_seqlen + p.toks - 1) / p.toks;
     p.items = c.num_seqs * p.blocks_per_seq;
     units = p.items * c.num_kv_heads;
     if (units * 2 > res || tiles > kWholeTiles) break;

@@ -39,3 +39,27 @@ def test_grids_of_the_selection(lib):
     def select(hkv):
         return lib.ndl_kv_select(P, P, P, 1, hkv, 16, P, 8, 8, P, 3, 32, 4, 8, None)
     assert select(1 << 22) == -2 and select(MOST) == -2
+
+
+@pytest.mark.parametrize("which", ["16-bit", "8-bit", "mass"])
+def test_bounds_of_tokens_next_to_31_bits(lib, which):
+    """The row blocks of max_seqlen tokens (8 sequences, group 1: 2^31 tokens by 256, more than a grid or
+    31 bits of row blocks hold): refused as a large bound is, no negative number of them."""
+    def call(most, keys):
+        chunk = (P, P, 128, P, *((P,) if which == "8-bit" else ()), 4, P, 500, 500, P, P)
+        rest = (8, 90, most, keys, 2, 2, 64, 16, 0, 0.1)
+        if which == "mass":
+            return lib.ndl_attention_mass(P, *chunk, *rest, 1.0, P, 1 << 50, None)
+        f = lib.ndl_fp8_tree_attention if which == "8-bit" else lib.ndl_tree_attention
+        return f(*chunk, P, 2, 2, *rest, P, 1 << 50, None)
+
+    def need(most, keys):
+        if which == "mass":
+            return lib.ndl_attention_mass_workspace_bytes(8, 90, most, keys, 2, 2, 64, 16)
+        f = (lib.ndl_fp8_tree_attention_workspace_bytes if which == "8-bit" else
+             lib.ndl_tree_attention_workspace_bytes)
+        return f(8, most, keys, 2, 2, 64, 16)
+    for keys in (64, 8000):
+        for most in (1 << 29, MOST - 256, MOST - 255, MOST):
+            assert call(most, keys) == -1, (most, keys)
+            assert need(most, keys) == need(1 << 29, keys) < 1 << 20
