@@ -736,9 +736,9 @@ int ndl_verify_tree(void* tokens, int32_t* accepted, int32_t* path, const void* 
  * ndl_paged_decode and ndl_varlen_prefill have it (K and V of the new tokens are in the cache).
  * With p the softmax's weights of the call's tokens and query heads, position x gets
  * decay * mass + sum p where it was cached (x < context_lens[i]) and sum p where it is new; a decay
- * of 0 forgets what was there.  Sums are fp32 and run in a fixed order.  Positions with invalid block
- * ids and sequences that attend nothing keep what they have; no block may be attended by two
- * sequences.
+ * of 0 forgets what was there.  A row whose scores are all -inf has zeros and gives no weight.  Sums
+ * are fp32 and run in a fixed order.  Positions with invalid block ids and sequences that attend
+ * nothing keep what they have; no block may be attended by two sequences.
  *
  * max_seqlen and max_keys bound a sequence's tokens and keys: those past them may not be computed and
  * get no weight.  The workspace (ndl_attention_mass_workspace_bytes of the same sizes, max_keys cut

@@ -189,7 +189,9 @@ __global__ __launch_bounds__(64 * kMassWaves) void add_weights_kernel(MassArgs a
 #pragma unroll
       for (int s = 0; s < KS; ++s) lq[g][s][lane] = ld16(src + 16 * s);
       if (h == 0) {
-        llse[32 * g + c32] = a.lse[at];
+        // (a sum of 0, where every score is -inf: no weight, as add_scores_kernel has it)
+        const float lse = a.lse[at];
+        llse[32 * g + c32] = lse == kNegInf ? -kNegInf : lse;
         llim[32 * g + c32] = live ? c.ctx + tok + 1 : 0;      // keys that the column attends
       }
     }

@@ -2,11 +2,13 @@
 because those of the bounds would take more than the workspace may.  Bounds:
 test_gpu_attention_mass.py's.
 """
+import math
+
 import pytest
 import torch
 
 from needle_amd import ops
-from test_gpu_attention_mass import DEV, Case
+from test_gpu_attention_mass import Case
 
 pytestmark = pytest.mark.gpu
 DTYPES = [torch.bfloat16, torch.float16]
@@ -53,3 +55,23 @@ def test_just_within_the_kept_scores():
     c.table = torch.cat([c.table, torch.full((2, cols - c.table.shape[1]), -1,
                                              dtype=torch.int32)], 1)
     c.check(c.run(decode=True))
+
+def test_rows_whose_scores_are_all_minus_infinity():
+    """The softmax's sum is 0: no weight and zeros, whether scores are kept or made again, for that row
+    alone."""
+    for counts in ([8, 2], [40, 2]):
+        c = Case((8, 2, 64, 16), counts, [0, 100], seed=34)
+        # the first token's own key, the only one it attends, is -inf in a dimension where the queries
+        # of kv head 1 are positive
+        c.pool[0, int(c.table[0, 0]), 1, 0, 3] = -math.inf
+        c.q[:, 4:, 3] = c.q[:, 4:, 3].abs() + 0.5
+        out, mass = c.run()
+        assert not out[0, 4:].any()
+        assert out[0, :4].isfinite().all() and out[1:].isfinite().all()
+        p = torch.arange(counts[0])
+        got = mass.cpu()[c.table[0].long()[p // 16], :, p % 16]
+        assert got.isfinite().all(), (counts, got)
+        # a head's tokens give 1 each, the first one's row nothing on kv head 1
+        total = got.sum(0)
+        want = torch.tensor([4.0 * counts[0], 4.0 * (counts[0] - 1)])
+        assert (total - want).abs().max() < 2.0 ** -12 * want.max(), total
