@@ -626,9 +626,9 @@ int ndl_fp8_decode_append(void* out, const void* q, int64_t q_tok_stride, const 
  * draft_probs has not (after a sequence without rows), and u is taken within [0, 1].
  *
  * tokens [num_rows], in ids' type: a sequence's accepted drafts, the next token, then -1, rows
- * outside cu_seqlens left as they were; accepted [num_seqs].  logits in `dtype`, any row stride of at least vocab; draft_probs float32
- * [num_rows - num_seqs] rows; uniforms and temperature float32 [num_rows], [num_seqs]
- * (temperature NULL: 1).  num_rows and num_seqs at most 65535, vocab at most 2^18
+ * outside cu_seqlens left as they were; accepted [num_seqs].  logits in `dtype`, any row stride of
+ * at least vocab; draft_probs float32 [num_rows - num_seqs] rows; uniforms and temperature float32
+ * [num_rows], [num_seqs] (temperature NULL: 1).  num_rows and num_seqs at most 65535, vocab at most 2^18
  * (NDL_ERR_UNSUPPORTED otherwise).  The workspace is 256-byte aligned and belongs to one call at a
  * time.
  */

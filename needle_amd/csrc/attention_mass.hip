@@ -29,9 +29,8 @@ namespace ndl {
 namespace {
 
 constexpr int kKeys = 32;             // of a tile
-constexpr int kTiles = 1;             // of a wave
 constexpr int kMassWaves = 8;
-constexpr int kMassKeys = kMassWaves * kTiles * kKeys;      // of a workgroup
+constexpr int kMassKeys = kMassWaves * kKeys;      // of a workgroup: a tile for each wave
 constexpr int kGroups = 4;            // 32-column groups in LDS at a time
 
 struct MassArgs {
@@ -154,26 +153,25 @@ __global__ __launch_bounds__(64 * kMassWaves) void add_weights_kernel(MassArgs a
   const int lane = threadIdx.x & 63, c32 = lane & 31, h = lane >> 5;
   const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int head = blockIdx.x % a.num_kv_heads, seq = blockIdx.y;
-  const int x0 = (int)(blockIdx.x / a.num_kv_heads) * kMassKeys + wv * kTiles * kKeys;
+  const int x0 = (int)(blockIdx.x / a.num_kv_heads) * kMassKeys + wv * kKeys;
   const Chunk c = chunk_of(a, seq);
   if ((int)(blockIdx.x / a.num_kv_heads) * kMassKeys >= c.keys) return;
   const int32_t* const table = a.block_table + seq * a.bt_row_stride;
 
   // This wave's keys, a row per lane: 16-byte pieces 2 s + h.  Keys past the last one and of invalid
   // blocks: the last block that there is (their sums are not written).
-  X8 k[kTiles][KS];
-#pragma unroll
-  for (int i = 0; i < kTiles; ++i) {
-    int x = x0 + kKeys * i + c32;
+  X8 k[KS];
+  {
+    int x = x0 + c32;
     if (x >= c.keys) x = c.keys - 1;
     int b = table[x >> a.block_shift];
     if (b < 0 || b >= a.num_blocks) b = 0;
     const u16* const row = a.kplane + ((((int64_t)b * a.num_kv_heads + head) << a.block_shift) +
                                        (x & ((1 << a.block_shift) - 1))) * D + 8 * h;
 #pragma unroll
-    for (int s = 0; s < KS; ++s) k[i][s] = __builtin_bit_cast(X8, ld16(row + 16 * s));
+    for (int s = 0; s < KS; ++s) k[s] = __builtin_bit_cast(X8, ld16(row + 16 * s));
   }
-  f32x16 sum[kTiles] = {};
+  f32x16 sum = {};
   const int cols = c.n * a.group;
   for (int col0 = 0; col0 < cols; col0 += 32 * kGroups) {
     const int here = cols - col0 < 32 * kGroups ? cols - col0 : 32 * kGroups;
@@ -202,34 +200,27 @@ __global__ __launch_bounds__(64 * kMassWaves) void add_weights_kernel(MassArgs a
       for (int s = 0; s < KS; ++s) q[s] = __builtin_bit_cast(X8, lq[g][s][lane]);
       const float lse = llse[32 * g + c32];
       const int lim = llim[32 * g + c32];
+      f32x16 sc = {};
 #pragma unroll
-      for (int i = 0; i < kTiles; ++i) {
-        f32x16 sc = {};
+      for (int s = 0; s < KS; ++s) sc = T::mfma32x32x16(k[s], q[s], sc);
+      if (x0 + kKeys <= c.ctx && 32 * (g + 1) <= here) {     // every column attends every key
 #pragma unroll
-        for (int s = 0; s < KS; ++s) sc = T::mfma32x32x16(k[i][s], q[s], sc);
-        const int first = x0 + kKeys * i;
-        if (first + kKeys <= c.ctx && 32 * (g + 1) <= here) {     // every column attends every key
+        for (int r = 0; r < 16; ++r) sum[r] += fast_exp2(fmaf(sc[r], a.scale_log2, -lse));
+      } else {
+        const int left = lim - (x0 + 4 * h);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) sum[i][r] += fast_exp2(fmaf(sc[r], a.scale_log2, -lse));
-        } else {
-          const int left = lim - (first + 4 * h);
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const float p = fast_exp2(fmaf(sc[r], a.scale_log2, -lse));
-            sum[i][r] += 8 * (r >> 2) + (r & 3) < left ? p : 0.f;
-          }
+        for (int r = 0; r < 16; ++r) {
+          const float p = fast_exp2(fmaf(sc[r], a.scale_log2, -lse));
+          sum[r] += 8 * (r >> 2) + (r & 3) < left ? p : 0.f;
         }
       }
     }
   }
-#pragma unroll
-  for (int i = 0; i < kTiles; ++i) {
-    const float s = sums_by_key(sum[i], lane);
-    const int x = x0 + kKeys * i + c32;
-    if (h != 0 || x >= c.keys) continue;
-    float* const at = number_of(a, table, x, head);
-    if (at != nullptr) add_to(a, at, x, c.ctx, s);
-  }
+  const float s = sums_by_key(sum, lane);
+  const int x = x0 + c32;
+  if (h != 0 || x >= c.keys) return;
+  float* const at = number_of(a, table, x, head);
+  if (at != nullptr) add_to(a, at, x, c.ctx, s);
 }
 
 // What a call keeps of its scores, 0 where it makes them again: past kScoredColumns columns, or where

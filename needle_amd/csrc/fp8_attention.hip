@@ -1144,8 +1144,8 @@ int launch(ChunkArgs a, int nt, int waves, hipStream_t s) {
   const int64_t wgs = units * a.num_kv_heads;
   if (!grid_fits(wgs, 64 * waves)) return NDL_ERR_INVALID_ARG;
   void* args[] = {&a};
-  if (hipLaunchKernel(kernel_of<D, F16>(nt, waves, a.new_k != nullptr, a.mask != nullptr), dim3((unsigned)wgs),
-                      dim3(64 * waves), args, 0, s) != hipSuccess) {
+  if (hipLaunchKernel(kernel_of<D, F16>(nt, waves, a.new_k != nullptr, a.mask != nullptr),
+                      dim3((unsigned)wgs), dim3(64 * waves), args, 0, s) != hipSuccess) {
     (void)hipGetLastError();  // clear the error so that the next call's check sees its own
     return NDL_ERR_LAUNCH;
   }
@@ -1244,8 +1244,9 @@ static int fp8_attention(ndl::ChunkArgs a, void* out, const void* q, int64_t q_t
   const hipStream_t s = (hipStream_t)stream;
   const bool f16 = dtype_is_f16(dtype);
   Unpacked u;
-  if (cu_seqlens != nullptr && a.mask == nullptr && unpacked_plan(num_seqs, num_tokens, max_seqlen, max_keys, num_heads,
-                                             num_kv_heads, head_dim, block_size, &u)) {
+  if (cu_seqlens != nullptr && a.mask == nullptr &&
+      unpacked_plan(num_seqs, num_tokens, max_seqlen, max_keys, num_heads, num_kv_heads, head_dim,
+                    block_size, &u)) {
     if (!workspace || workspace_bytes < u.total() || (uintptr_t)workspace & 255u)
       return NDL_ERR_WORKSPACE;
     if (head_dim == 128)

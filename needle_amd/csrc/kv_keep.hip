@@ -406,7 +406,8 @@ extern "C" int ndl_kv_compact(void* const* pools, void* const* scales, int num_l
   if ((num_layers && !pools) || !block_table || !keep || !counts) return NDL_ERR_INVALID_ARG;
   if (num_layers > kMaxPools || (int64_t)max_blocks_per_seq * block_size > 0x7fffff00 ||
       (int64_t)dst_max_blocks * block_size > 0x7fffff00 || most > 0x7fff0000 ||
-      num_blocks > (int64_t)0xfffffff0 / num_kv_heads / block_size || row_bytes > 16 * loads_of(true) * 64)
+      num_blocks > (int64_t)0xfffffff0 / num_kv_heads / block_size ||
+      row_bytes > 16 * loads_of(true) * 64)
     return NDL_ERR_UNSUPPORTED;
   MoveArgs a{};
   for (int i = 0; i < num_layers; ++i) {

@@ -47,7 +47,8 @@
 namespace ndl {
 namespace {
 
-constexpr float kRaise = 256.f;   // a lane's sum of a tile's probabilities past which the maximum is raised
+constexpr float kRaiseSum = 256.f;   // a lane's sum of a tile's probabilities past which the
+                                     // maximum is raised
 
 // kScored: causal, and the scores stay behind in a.scores (row blocks of up to 32 columns).
 enum Chunk { kCausal, kTree, kScored };
@@ -480,9 +481,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_attention_kernel(TreeArgs
           }
         }
 
-        // Probabilities against the running maximum as it stands.  Where one exceeds 2^kRaise its
-        // lane's sum does, and then (or while a column has no maximum yet) the maximum is raised, the
-        // sums rescaled and the probabilities taken again: no maximum is computed otherwise.
+        // Probabilities against the running maximum as it stands.  Where a lane's sum of them exceeds
+        // kRaiseSum, or while a column has no maximum yet, the maximum is raised, the sums are rescaled
+        // and the probabilities taken again: no maximum is computed otherwise.
         uint32_t pw[8];
         float sum;
         auto probs = [&] {
@@ -499,7 +500,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_attention_kernel(TreeArgs
           sum = p[0];
         };
         probs();
-        if (__builtin_amdgcn_ballot_w64(!(sum <= kRaise) || m == kNegInf)) {
+        if (__builtin_amdgcn_ballot_w64(!(sum <= kRaiseSum) || m == kNegInf)) {
           float mt = fmaxf(sc[0], sc[1]);
 #pragma unroll
           for (int r = 2; r < 16; r += 2) mt = fmaxf(fmaxf(mt, sc[r]), sc[r + 1]);
