@@ -686,7 +686,8 @@ int ndl_tree_attention(void* out, const void* q, int64_t q_tok_stride, const voi
                        size_t workspace_bytes, ndl_stream_t stream);
 
 /*
- * The same over the 8-bit pool, with what ndl_fp8_attention says of its values.  The workspace is
+ * The same over the 8-bit pool, with what ndl_fp8_attention says of its values.  In fp16, trees of many
+ * columns count keys of odd multiples of 2^-24 as one of their neighbours.  The workspace is
  * ndl_fp8_tree_attention_workspace_bytes.
  */
 size_t ndl_fp8_tree_attention_workspace_bytes(int num_seqs, int max_seqlen, int64_t max_keys,
@@ -742,7 +743,9 @@ int ndl_verify_tree(void* tokens, int32_t* accepted, int32_t* path, const void* 
  *
  * max_seqlen and max_keys bound a sequence's tokens and keys: those past them may not be computed and
  * get no weight.  The workspace (ndl_attention_mass_workspace_bytes of the same sizes, max_keys cut
- * to the table's, on the same device) is 256-byte aligned and belongs to one call at a time.
+ * to the table's, on the same device) is 256-byte aligned and belongs to one call at a time.  Up to 32
+ * rows of max_seqlen times the group it holds their scores, 4 bytes for each of max_keys keys, kv head
+ * and sequence, as long as that is at most 1 GiB.
  */
 size_t ndl_attention_mass_workspace_bytes(int num_seqs, int64_t num_tokens, int max_seqlen,
                                           int64_t max_keys, int num_heads, int num_kv_heads,
@@ -764,8 +767,9 @@ int ndl_attention_mass(void* out, float* mass, const void* q, int64_t q_tok_stri
  * mass float32 [num_blocks][num_kv_heads][block_size] (NULL: none).  `pools` and `scales` are host
  * arrays of device addresses, no pool twice.
  *
- * Without dst_table rows move in place and a list has to ascend, keep[j] >= j; with it they go to the
- * blocks that its rows name, none of which may be one that rows are read from.  An entry below 0, a
+ * Without dst_table rows move in place, a list has to ascend, keep[j] >= j, and no block in which rows
+ * move may be another sequence's too; with it they go to the blocks that its rows name, none of which
+ * may be one that rows are read from, or another sequence's.  An entry below 0, a
  * position past its table, an invalid block id, a negative first[i] and a row that stays where it is
  * move nothing; counts past the list end with it.
  */

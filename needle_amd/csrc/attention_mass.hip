@@ -18,7 +18,8 @@
 //     32 keys in registers for all columns, the sum over columns kept in the accumulator layout and
 //     joined across lanes once, at the end.  (8 waves of 32 keys rather than 4 of 64: twice as many to a
 //     SIMD, 26 us for 34 of 8 prompts of 2,000 to 16,000 tokens, 32 tokens each, 28/4 heads.)
-// Bound (64 sequences' step): K and V read once, 4.3 TB/s over the call.  The 8 prompts' 83 us are the
+// Scores kept are at most 1 GiB by the host's bounds (max_context_len, or all that the table holds).
+// Bound (64 sequences' step): K and V read once, 4.3 TB/s over the call.  The 8 prompts' 84 us are the
 // attention 42 (shares of 20 tiles), its merge 13 and the weights 26 (by instruction counts 5 of them
 // products and 8 exponentials; the rest is trips to memory of workgroups that live for 256 keys).
 // Sums run in a fixed order, without atomics; a key's number is written by one lane.

@@ -1,5 +1,5 @@
-// The arithmetic by which fp8_attention.hip cuts the row blocks of a kv head into equal shares and
-// finds the parts again: plain integers, nothing of the GPU.
+// The arithmetic by which fp8_attention.hip and tree_attention.hip cut the row blocks of a kv head into
+// equal shares and find the parts again: plain integers, nothing of the GPU.
 //
 // The row blocks lie end to end in slots, a slot per tile after `pad` empty ones.  Share s begins at
 // slot s * chunk, or at a row block's end within `snap` slots of that: a sliver of a row block is

@@ -1,5 +1,5 @@
-// What the kernels of the 8-bit pool (kv_fp8.hip, fp8_attention.hip) share, and what they ask of
-// the 16-bit prefill (varlen_prefill.hip).
+// What the kernels of the 8-bit pool (kv_fp8.hip, fp8_attention.hip, tree_attention.hip) share, and what
+// they ask of the 16-bit prefill (varlen_prefill.hip); the check of a grid's size.
 #pragma once
 
 #include "ndl_common.hpp"

@@ -1183,9 +1183,11 @@ extern "C" size_t ndl_fp8_attention_workspace_bytes(int num_seqs, int64_t num_to
 // Trees of more columns than kWideColumns and of kWideScores scores in all have tree_attention.hip's
 // row blocks of up to 256, where a key's codes are unpacked once for all of them; fewer the row blocks
 // of 32 here, of which there are more.  us, here / there, 28/4 heads of 128: 8 sequences after 12,000,
-// 63 columns 62.0 / 53.0, 126 94.8 / 57.4, 252 159 / 83.0; 4 after 4,000, 126 32.0 / 32.9, 252 42.4 /
-// 39.1; 4 after 1,400, 252 19.9 / 37.9; 1 after 16,000, 252 41.0 / 58.8; 32/8 heads, 64 after 2,300,
-// 36 112 / 114, 72 175 / 118, 256 452 / 204; 16 after 300, 128 15.9 / 18.0, 256 32.2 / 21.9.
+// 63 columns 63.7 / 53.1, 126 97.5 / 58.7, 252 161 / 83.5; 4 after 4,000, 126 32.8 / 30.3, 252 43.0 /
+// 37.6; 4 after 1,400, 252 20.2 / 38.4; 1 after 16,000, 252 41.5 / 41.0; 32/8 heads, 64 after 2,300,
+// 36 113 / 117, 72 175 / 122, 256 452 / 209; 16 after 300, 128 16.8 / 18.9, 256 33.6 / 22.1.  At three
+// of these the rule takes the slower side: 63 columns after 12,000 (by 20 %), 126 after 4,000 (8 %) and
+// 256 after 300 (52 %, just below kWideScores).
 constexpr int kWideColumns = 64;
 constexpr int64_t kWideScores = 12 << 20;
 static bool wide_trees(int num_seqs, int max_seqlen, int64_t max_keys, int num_heads,

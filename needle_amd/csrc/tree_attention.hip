@@ -32,12 +32,16 @@
 //   * Split: as fp8_attention.hip's (chunk_stream.hpp), a workgroup per (kv head, row block) or
 //     equal shares of all of a kv head's tiles, merged by a second launch.
 // Measured (us, a call): 64 trees of 16 to 64 nodes after 512 to 4,096 tokens, 32/8 heads of 128, bf16
-// 155 to 162 (the keys at 3.2 TB/s, 480 TFLOP/s); 4 trees of 16 after 64 to 800, 14/2 heads of 64, 8.6; 8
-// trees of 40 to 60 after 4,096 to 32,768 in an 8-bit pool, 28/4 heads of 128, float16, 165 (590
-// TFLOP/s).  The wide ones are bound by neither: of a SIMD's cycles the matrix cores take 27 %, the
-// softmax 30 %, and LDS is busy for as many; two waves to a SIMD (222 of 256 registers) overlap them
-// only in part.  Scores made a tile ahead took longer (195 us for 178, in shares), a product put off past
-// the barrier in half the waves too (172 for 165).
+// 155 to 162 (the keys at 2.8 to 2.95 TB/s, 470 to 490 TFLOP/s); 4 trees of 16 after 64 to 800, 14/2
+// heads of 64, 8.7; 8 trees of 40 to 60 after 4,096 to 32,768 in an 8-bit pool, 28/4 heads of 128,
+// float16, 165 (590 TFLOP/s).  What bounds the wide ones:
+//   * Whole row blocks go to the XCDs in the order of the sequences, so uneven ones wait for the fullest
+//     XCD: of those 64 trees its CUs have up to 137 steps of 32 keys where the mean is 94 (equal contexts
+//     with as many keys, 111 for 97: 144 us).
+//   * A step, 1.2 to 1.4 us on a full GPU, is neither bytes nor products: of a SIMD's cycles the matrix
+//     cores take 27 %, the softmax 30 %, and LDS is busy for as many; two waves to a SIMD (222 of 256
+//     registers) overlap them only in part.  Scores made a tile ahead took longer (195 us for 178, in
+//     shares), a product put off past the barrier in half the waves too (172 for 165).
 #include "chunk_stream.hpp"
 #include "fp8.hpp"
 #include "tree_attention.hpp"
@@ -326,7 +330,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_attention_kernel(TreeArgs
       };
       // The wave's codes of a stage, into 16-bit stage u % NS.  In float16, which has no 65,536 (a row's
       // values from 63,488 on), keys are halved, for which the scores' scale makes up, and a value is
-      // 65,504, the nearest there is.
+      // 65,504, the nearest there is.  A float16 row's values are multiples of 2^-24, so a halved key is
+      // off by 2^-25 at most (odd multiples: 2^-24 of the key), every other is exact.
       auto unpack = [&](int u, int slot) {
 #pragma unroll
         for (int i = 0; i < MINE; ++i) {

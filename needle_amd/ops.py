@@ -1395,7 +1395,9 @@ def attention_mass(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.T
     their q alone, with context_lens the tokens before them.  max_seqlen bounds a sequence's tokens,
     max_context_len its cached ones (0: not known, the table's width then).  decay 0 forgets what
     was there.  No two sequences may attend one block.  workspace: as decode_workspace gives, of
-    attention_mass_workspace_bytes, for one call at a time."""
+    attention_mass_workspace_bytes, for one call at a time.  Up to 32 rows (max_seqlen times the group;
+    a decode step) it holds their scores for every key of these bounds, 1 GiB at most (past that they
+    are made again): give max_context_len where the table is much wider than what is cached."""
     if out is None and workspace is None and _lib.NATIVE is not None:
         out = _lib.NATIVE.attention_mass(q, kv_cache, block_table, cu_seqlens, context_lens, mass,
                                          max_seqlen, max_context_len, scale, num_heads,
@@ -1463,9 +1465,10 @@ def kv_compact(pools, block_table: torch.Tensor, keep: torch.Tensor, counts: tor
     first the tokens cached before the tree and counts = accepted + 1.  counts, first int32
     [num_seqs].  mass (kv_mass_pool): weights that move with the rows.
 
-    Without dst_table the rows move in place; a list has to ascend, with keep[j] >= j.  With
-    dst_table (int32 [num_seqs, columns]) they go to its blocks, none of which may hold rows that are
-    read.  Negative entries, positions past a table and invalid block ids move nothing."""
+    Without dst_table the rows move in place; a list has to ascend, with keep[j] >= j, and no block in
+    which rows move may be another sequence's too (a shared prefix before `first` may).  With dst_table
+    (int32 [num_seqs, columns]) they go to its blocks, none of which may hold rows that are read or
+    belong to two sequences.  Negative entries, positions past a table and invalid block ids move nothing."""
     import ctypes
     pools = list(pools)
     _require(len(pools) > 0, "no pools given")
