@@ -1404,6 +1404,8 @@ def attention_mass(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.T
                                          num_kv_heads, head_dim, decay)
         if out is not None:
             return out
+    if isinstance(kv_cache, Fp8KVCache):
+        raise TypeError("attention_mass reads a 16-bit pool, got an Fp8KVCache")
     _check_cache(kv_cache)
     dev = kv_cache.device
     _, nb, hkv, bs, d = kv_cache.shape

@@ -1,8 +1,9 @@
 """Sizes next to the entry points' limits, which the counting behind them has to hold: refused, or planned
 for as smaller ones are, before any launch (CPU)."""
 import pytest
+import torch
 
-from needle_amd import _lib
+from needle_amd import _lib, ops
 
 P = 1 << 20      # an aligned stand-in address that is never dereferenced
 MOST = (1 << 31) - 1
@@ -63,3 +64,12 @@ def test_bounds_of_tokens_next_to_31_bits(lib, which):
         for most in (1 << 29, MOST - 256, MOST - 255, MOST):
             assert call(most, keys) == -1, (most, keys)
             assert need(most, keys) == need(1 << 29, keys) < 1 << 20
+
+
+def test_the_weights_over_an_8_bit_pool():
+    pool = ops.Fp8KVCache(torch.zeros(2, 3, 2, 16, 64, dtype=torch.float8_e4m3fn),
+                          torch.zeros(2, 3, 2, 16, dtype=torch.uint8))
+    table, lens = torch.zeros(1, 1, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(TypeError, match="16-bit"):
+        ops.attention_mass(torch.zeros(1, 4, 64), pool, table, lens, torch.zeros(3, 2, 16), 0.1, 4,
+                           2, 64)
