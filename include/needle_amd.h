@@ -44,7 +44,8 @@
  *   ndl_verify_drafts   accepted drafts and the next token of every sequence, from the
  *                       target's logits and given random numbers
  *
- * and trees of drafted tokens and caches that keep some of their rows, over both pools:
+ * and trees of drafted tokens and caches that keep some of their rows, over both pools
+ * (ndl_attention_mass: the 16-bit one):
  *
  *   ndl_tree_mask       which nodes a tree's tokens attend, from their parents
  *   ndl_tree_attention, ndl_fp8_tree_attention  attention of a chunk under such masks
@@ -712,7 +713,8 @@ int ndl_fp8_tree_attention(void* out, const void* q, int64_t q_tok_stride, const
  * u = uniforms[cu_seqlens[i + 1] - 1], a leaf's: from p of the last node without its children's
  * tokens, the first v whose weights up to v sum to more than u times their total (the row's argmax
  * where they have all weight).  The tokens are distributed as the target's; a chain gives what
- * ndl_verify_drafts gives without draft_probs.
+ * ndl_verify_drafts gives without draft_probs.  Sums of a row's weights are of fp32 terms: p on the
+ * path is off by a few 2^-24 of itself, the drawn token's weights are fp64.
  *
  * Where temperature[i] is 0 or less, or a row's maximum is not finite, p is the point at the row's
  * argmax in torch's order.  Tokens outside the vocabulary are not taken; a sequence's rows past its
@@ -786,7 +788,7 @@ int ndl_kv_compact(void* const* pools, void* const* scales, int num_layers, floa
  * keep [num_seqs][num_kv_heads][budget] their positions, ascending, then -1.  Of a longer sequence
  * the first `sinks`, the last `recent` (at most budget together), and of the rest those with the
  * largest weights in mass float32 [num_blocks][num_kv_heads][block_size], of equal ones the first.
- * A NaN counts as the largest, a position with an invalid block id as the smallest weight; lens is
+ * A NaN counts as the largest weight, a position with an invalid block id as less than any; lens is
  * cut to what the table holds, and a negative one is 0.  num_seqs at most 65535, the budget and the
  * tokens that the table holds at most 2^31 - 2^16 (NDL_ERR_UNSUPPORTED otherwise).
  */
